@@ -332,6 +332,41 @@ int tac_quarot_w8a16(const uint16_t* X, const int8_t* W, const uint16_t* w_scale
                      uint16_t* Y, void* workspace, uint64_t workspace_bytes, int M, int N, int K,
                      int block, void* stream);
 
+/* ---- INT8 linear layers with a scale for each token -------------------------
+ * Element types of the floating-point arguments below. */
+enum tac_type { TAC_F32 = 0, TAC_F16 = 1, TAC_BF16 = 2 };
+
+/* Rows of X[M,K] (x_type, row stride ldx elements) quantised to INT8, a scale
+ * each: t = max(max_k |x|, 1e-8), scale[m] = t / 127, Q = rint(x * (127 / t))
+ * in float32, round half to even, magnitudes at most 127.  Q [M, K_pad] with
+ * K_pad = K rounded up to 16, padding columns zero.  A row that holds an
+ * infinity or a NaN gets the scale NaN.  Q 16-byte aligned; X may have any
+ * alignment of its type.  The reference quantises per tensor
+ * (runtime/w8a16_simulator_reference.py:96-135); the per-row form has no
+ * counterpart there. */
+int tac_quantize_rows_i8(const void* X, int x_type, int64_t ldx, int8_t* Q, float* scale, int M, int K,
+                         void* stream);
+
+/* Y[M,N] (y_type) = (A[M,K] @ Bt[N,K]^T) * a_scale[m] * b_scale[n] (+ bias[n]):
+ * INT8 x INT8 with exact int32 sums, ((float(sum) * a_scale) * b_scale) + bias
+ * in float32 and one rounding.  A, Bt row-major and 16-byte aligned, K a
+ * multiple of 16 below 2^17; any M up to 2^20 and any N.  b_scale is TAC_F32
+ * or TAC_F16 (the type tac_quantize_weight_i8 writes); bias may be null.
+ * Asynchronous on `stream`; tac_gemm_status reports device faults. */
+int tac_gemm_i8_scaled(const int8_t* A, const int8_t* Bt, const float* a_scale, const void* b_scale,
+                       int b_scale_type, const void* bias, int bias_type, void* Y, int y_type, int M, int N,
+                       int K, void* stream);
+
+/* The same product of floating-point rows, quantised in the call as
+ * tac_quantize_rows_i8 does: Y = linear(X[M,K]) with Bt [N, K_pad] int8, K_pad
+ * = K rounded up to 16.  A multiplier in columns K .. K_pad of Bt meets a zero.
+ * Calls that share a workspace (256-byte aligned, at least
+ * tac_linear_w8a8_workspace_bytes) must not overlap. */
+uint64_t tac_linear_w8a8_workspace_bytes(int M, int K);
+int tac_linear_w8a8(const void* X, int x_type, int64_t ldx, const int8_t* Bt, const void* b_scale,
+                    int b_scale_type, const void* bias, int bias_type, void* Y, int y_type, void* workspace,
+                    uint64_t workspace_bytes, int M, int N, int K, void* stream);
+
 /* ---- Offline weight quantisation ------------------------------------------
  * Per-channel (per_channel = 1) or per-tensor symmetric INT8 quantisation of
  * a float32 weight W[out_ch, in_features] (row-major, PyTorch layout), as

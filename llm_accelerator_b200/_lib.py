@@ -49,6 +49,7 @@ class ExecInfo(C.Structure):
                 ("final_regs", Regs)]
 
 
+TYPE_F32, TYPE_F16, TYPE_BF16 = 0, 1, 2   # enum tac_type
 COMPILE_NO_PACK = 1   # TAC_COMPILE_NO_PACK
 
 
@@ -59,6 +60,7 @@ class CompileOpts(C.Structure):
 
 _P = C.c_void_p
 _U64 = C.c_uint64
+_I64 = C.c_int64
 _I = C.c_int
 
 # name -> (restype, argtypes); every symbol include/taccel_b200.h declares
@@ -108,6 +110,10 @@ SIGNATURES = {
     "tac_fwht_f16": (_I, [_P, _P, _I, _I, _I, _P]),
     "tac_quarot_workspace_bytes": (_U64, [_I, _I]),
     "tac_quarot_w8a16": (_I, [_P, _P, _P, _P, _P, _P, _U64, _I, _I, _I, _I, _P]),
+    "tac_quantize_rows_i8": (_I, [_P, _I, _I64, _P, _P, _I, _I, _P]),
+    "tac_gemm_i8_scaled": (_I, [_P, _P, _P, _P, _I, _P, _I, _P, _I, _I, _I, _I, _P]),
+    "tac_linear_w8a8_workspace_bytes": (_U64, [_I, _I]),
+    "tac_linear_w8a8": (_I, [_P, _I, _I64, _P, _P, _I, _P, _I, _P, _I, _P, _U64, _I, _I, _I, _P]),
     "tac_quantize_weight_i8": (_I, [_P, _I, _I, _I, _P, _P, _P, _P]),
     "tac_bundle_open": (_I, [C.c_char_p, C.POINTER(BundleView), C.POINTER(_P)]),
     "tac_bundle_close": (_I, [_P]),

@@ -1,0 +1,198 @@
+// INT8 linear layers with a scale for each token and output channel: the row
+// quantiser, the scaled product (tac_w8a8.cuh) and both in one call.
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cstdint>
+
+#include "../../include/taccel_b200.h"
+#include "tac_tmap.h"
+#include "tac_w8a8.cuh"
+
+namespace tac {
+int* gemm_fault_word();
+}
+
+namespace {
+
+using namespace tac;
+
+bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+bool type_ok(int t) { return t == TAC_F32 || t == TAC_F16 || t == TAC_BF16; }
+int status() { return cudaGetLastError() == cudaSuccess ? TAC_OK : TAC_E_CUDA; }
+
+int sm_count() {
+  static int sms[64] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
+  if (!sms[dev]) {
+    int n = 0;
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
+    sms[dev] = n;
+  }
+  return sms[dev];
+}
+
+// ---- row quantiser --------------------------------------------------------------------------------------------------
+// t = max(max |x|, 1e-8), scale = t / 127, q = rint(x * (127 / t)) in float32;
+// a row that holds an infinity or a NaN gets the scale NaN.  The maximum is
+// taken over the magnitudes' bits, in which infinities and NaN order above
+// every finite value.
+constexpr int kQrThreads = 128;
+
+template <typename T>
+__device__ __forceinline__ float to_f(T v);
+template <>
+__device__ __forceinline__ float to_f(float v) { return v; }
+template <>
+__device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
+template <>
+__device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
+
+template <typename T>
+__global__ void __launch_bounds__(kQrThreads) quant_rows_kernel(const T* __restrict__ X, int64_t ldx,
+                                                                int8_t* __restrict__ Q, int ldq,
+                                                                float* __restrict__ scale, int K) {
+  __shared__ uint32_t red[kQrThreads / 32];
+  const int64_t row = blockIdx.x;
+  const T* x = X + row * ldx;
+  int8_t* q = Q + row * ldq;
+  uint32_t mb = 0;
+  for (int k = threadIdx.x; k < K; k += kQrThreads) mb = max(mb, __float_as_uint(to_f(x[k])) & 0x7fffffffu);
+  mb = __reduce_max_sync(0xffffffffu, mb);
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = mb;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kQrThreads / 32; ++w) mb = max(mb, red[w]);
+  const bool finite = mb < 0x7f800000u;
+  const float t = fmaxf(__uint_as_float(mb), 1e-8f);
+  const float inv = finite ? __fdiv_rn(127.0f, t) : 0.f;
+  if (threadIdx.x == 0) scale[row] = finite ? __fdiv_rn(t, 127.0f) : __uint_as_float(0x7fc00000u);
+  for (int k = threadIdx.x; k < ldq; k += kQrThreads) {
+    int v = 0;
+    if (k < K && finite) v = __float2int_rn(__fmul_rn(to_f(x[k]), inv));
+    q[k] = int8_t(v);
+  }
+}
+
+int launch_quant_rows(const void* X, int type, int64_t ldx, int8_t* Q, float* scale, int M, int K, cudaStream_t st) {
+  const int ldq = (K + 15) / 16 * 16;
+  if (type == TAC_F32)
+    quant_rows_kernel<<<M, kQrThreads, 0, st>>>(static_cast<const float*>(X), ldx, Q, ldq, scale, K);
+  else if (type == TAC_F16)
+    quant_rows_kernel<<<M, kQrThreads, 0, st>>>(static_cast<const __half*>(X), ldx, Q, ldq, scale, K);
+  else
+    quant_rows_kernel<<<M, kQrThreads, 0, st>>>(static_cast<const __nv_bfloat16*>(X), ldx, Q, ldq, scale, K);
+  return status();
+}
+
+// ---- scaled product -------------------------------------------------------------------------------------------------
+bool map_rows(CUtensorMap* m, const int8_t* base, int K, int rows, int box_rows) {
+  const cuuint64_t dims[2] = {cuuint64_t(K), cuuint64_t(rows)}, strides[1] = {cuuint64_t(K)};
+  const cuuint32_t box[2] = {128, cuuint32_t(box_rows)};
+  return tmap_encode_u8(m, base, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+constexpr int kSkMaxSmem = 200 * 1024;
+
+int launch_splitk(const int8_t* A, const int8_t* Bt, W8Params p, cudaStream_t st) {
+  static bool smem_set[64] = {};
+  int dev = 0;
+  const int sms = sm_count();
+  if (!sms || cudaGetDevice(&dev) != cudaSuccess) return TAC_E_CUDA;
+  if (!smem_set[dev]) {
+    if (cudaFuncSetAttribute(w8_splitk_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSkMaxSmem) != cudaSuccess)
+      return TAC_E_CUDA;
+    smem_set[dev] = true;
+  }
+  p.k_blocks = (p.K + 127) / 128;
+  p.tn = p.M <= 16 ? 16 : p.M <= 32 ? 32 : p.M <= 64 ? 64 : 128;
+  const int64_t tiles = int64_t((p.N + 127) / 128) * ((p.M + p.tn - 1) / p.tn);
+  int split = 1;
+  while (split < 8 && 2 * split <= p.k_blocks && tiles * split * 2 <= 2 * sms) split *= 2;
+  const int per = (p.k_blocks + split - 1) / split, sb = sk_stage_bytes(p.tn);
+  p.stages = std::min(std::min(per, 8), std::max(2, 96 * 1024 / sb));
+  const int part = split > 1 ? p.tn * 512 : 0;
+  CUtensorMap tw, ta;
+  if (!map_rows(&tw, Bt, p.K, p.N, 128) || !map_rows(&ta, A, p.K, p.M, p.tn)) return TAC_E_CUDA;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((p.N + 127) / 128, (p.M + p.tn - 1) / p.tn, split);
+  cfg.blockDim = dim3(kSkThreads);
+  cfg.dynamicSmemBytes = std::max(p.stages * sb, part) + 1024;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 1;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = split;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, w8_splitk_kernel, tw, ta, p) == cudaSuccess ? TAC_OK : TAC_E_CUDA;
+}
+
+// Checks that both products share; also the limits of 32-bit sums and of the grid.
+int check_product(const void* Bt, const void* b_scale, int b_type, const void* bias, int bias_type, const void* Y,
+                  int y_type, int M, int N, int K) {
+  if (!Bt || !b_scale || !Y || M <= 0 || N <= 0 || K <= 0) return TAC_E_ARGUMENT;
+  if ((b_type != TAC_F32 && b_type != TAC_F16) || !type_ok(y_type) || (bias && !type_ok(bias_type))) return TAC_E_ARGUMENT;
+  if (K >= (1 << 17) || M > (1 << 20) || !aligned(Bt, 16)) return TAC_E_ARGUMENT;   // |sum| <= K * 128^2 < 2^31
+  return TAC_OK;
+}
+
+int run_product(const int8_t* A, const int8_t* Bt, const float* a_scale, const void* b_scale, int b_type,
+                const void* bias, int bias_type, void* Y, int y_type, int M, int N, int K, cudaStream_t st) {
+  W8Params p{};
+  p.a_scale = a_scale;
+  p.b_scale = b_scale;
+  p.bias = bias;
+  p.y = Y;
+  p.b_type = b_type;
+  p.bias_type = bias_type;
+  p.y_type = y_type;
+  p.M = M;
+  p.N = N;
+  p.K = K;
+  p.fault = gemm_fault_word();
+  if (!p.fault) return TAC_E_CUDA;
+  return launch_splitk(A, Bt, p, st);
+}
+
+uint64_t align256(uint64_t v) { return (v + 255) & ~uint64_t(255); }
+
+}  // namespace
+
+extern "C" int tac_quantize_rows_i8(const void* X, int x_type, int64_t ldx, int8_t* Q, float* scale, int M, int K,
+                                    void* stream) {
+  if (!X || !Q || !scale || !type_ok(x_type) || M <= 0 || K <= 0 || (M > 1 && ldx < K) || !aligned(Q, 16))
+    return TAC_E_ARGUMENT;
+  return launch_quant_rows(X, x_type, ldx, Q, scale, M, K, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int tac_gemm_i8_scaled(const int8_t* A, const int8_t* Bt, const float* a_scale, const void* b_scale,
+                                  int b_scale_type, const void* bias, int bias_type, void* Y, int y_type, int M, int N,
+                                  int K, void* stream) {
+  if (!A || !a_scale || K % 16 || !aligned(A, 16)) return TAC_E_ARGUMENT;
+  if (int s = check_product(Bt, b_scale, b_scale_type, bias, bias_type, Y, y_type, M, N, K)) return s;
+  return run_product(A, Bt, a_scale, b_scale, b_scale_type, bias, bias_type, Y, y_type, M, N, K,
+                     static_cast<cudaStream_t>(stream));
+}
+
+extern "C" uint64_t tac_linear_w8a8_workspace_bytes(int M, int K) {
+  if (M <= 0 || K <= 0) return 0;
+  return align256(uint64_t(M) * ((uint64_t(K) + 15) / 16 * 16)) + align256(uint64_t(M) * 4);
+}
+
+extern "C" int tac_linear_w8a8(const void* X, int x_type, int64_t ldx, const int8_t* Bt, const void* b_scale,
+                               int b_scale_type, const void* bias, int bias_type, void* Y, int y_type, void* workspace,
+                               uint64_t workspace_bytes, int M, int N, int K, void* stream) {
+  if (!X || !type_ok(x_type) || !workspace || !aligned(workspace, 256) || (M > 1 && ldx < K)) return TAC_E_ARGUMENT;
+  if (int s = check_product(Bt, b_scale, b_scale_type, bias, bias_type, Y, y_type, M, N, K)) return s;
+  if (workspace_bytes < tac_linear_w8a8_workspace_bytes(M, K)) return TAC_E_ARGUMENT;
+  const int Kp = (K + 15) / 16 * 16;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  int8_t* q = static_cast<int8_t*>(workspace);
+  float* s = reinterpret_cast<float*>(q + align256(uint64_t(M) * Kp));
+  if (int e = launch_quant_rows(X, x_type, ldx, q, s, M, K, st)) return e;
+  return run_product(q, Bt, s, b_scale, b_scale_type, bias, bias_type, Y, y_type, M, N, Kp, st);
+}

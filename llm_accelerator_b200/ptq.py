@@ -8,6 +8,9 @@ device-memory plumbing).
                                (software/taccel/runtime/tiny_fixture.py:149-159)
 ``quantize_tensor(W)``         the same quantiser in quantize_tensor's
                                [out, in] layout (software/taccel/quantizer/quantize.py:6-33)
+``quantize_rows(X)``           tac_quantize_rows_i8: activations to int8, a
+                               scale for each row (the A operand and a_scale
+                               of ``gemm.gemm_i8_scaled``)
 ``rotate_residual_stream_state_dict(sd, model_args, R)``
                                QuaRot's offline weight rotation
                                (software/taccel/quantizer/rotation.py:158-321):
@@ -52,6 +55,30 @@ def quantize_tensor(W, per_channel: bool = True):
     n, k = (1, W.numel()) if W.dim() == 1 else W.shape
     q, s = quantize_linear_weight(W, per_channel)
     return q[:k, :n].t().contiguous(), s[:n].contiguous()
+
+
+def quantize_rows(X):
+    """(q int8 [M, K_pad], scale float32 [M]) of X [M, K] (float32, float16 or bfloat16, contiguous rows at any row
+    stride): t = max(max |x|, 1e-8), scale = t / 127, q = rint(x * (127 / t)); K_pad = K rounded up to 16, padding
+    columns zero.  A row that holds an infinity or a NaN gets the scale NaN."""
+    import torch
+    from .gemm import _on_device, _type
+    xt = _type(X.dtype, "X")
+    if not X.is_cuda:
+        raise TypeError("X must be a CUDA tensor")
+    if X.dim() != 2 or X.shape[1] == 0 or (X.shape[1] > 1 and X.stride(1) != 1):
+        raise ValueError(f"X must be [M, K] with contiguous rows, got shape {tuple(X.shape)}, stride {X.stride()}")
+    M, K = X.shape
+    ldx = X.stride(0) if M > 1 else K
+    if ldx < K:
+        raise ValueError(f"rows of X overlap (stride {ldx}, {K} columns)")
+    q = torch.empty((M, -(-K // 16) * 16), dtype=torch.int8, device=X.device)
+    scale = torch.empty(M, dtype=torch.float32, device=X.device)
+    if M:
+        L.check(_on_device(X.device, lambda st: L.lib.tac_quantize_rows_i8(X.data_ptr(), xt, ldx, q.data_ptr(),
+                                                                           scale.data_ptr(), M, K, st)),
+                "tac_quantize_rows_i8")
+    return q, scale
 
 
 def rotate_residual_stream_state_dict(state_dict: dict, model_args: dict, R) -> list:
