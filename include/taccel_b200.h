@@ -367,6 +367,68 @@ int tac_linear_w8a8(const void* X, int x_type, int64_t ldx, const int8_t* Bt, co
                     int b_scale_type, const void* bias, int bias_type, void* Y, int y_type, void* workspace,
                     uint64_t workspace_bytes, int M, int N, int K, void* stream);
 
+/* ---- 4-bit paged key / value cache ------------------------------------------
+ * The cache of one layer: pages of page_size tokens (16, 32, 64 or 128), for
+ * each key-value head of head_dim (64 or 128) values a token.  A row x (one
+ * token, one head) is held as lo = min(0, min x), hi = max(0, max x),
+ * s = bf16((hi - lo) / 15), z = rint(-lo / s) and codes
+ * c = clip(rint(x / s) + z, 0, 15), and stands for s (c - z): codes
+ * [num_pages][heads][page_size][head_dim / 2], code 2j in the low and 2j + 1 in
+ * the high half of byte j; parameter words [num_pages][heads][page_size], the
+ * bits of s above those of z.  A row that holds an infinity or a NaN stands
+ * for NaN.  All arrays 16-byte aligned device memory.  The reference's cache is
+ * INT8 with one scale (the KV-append STOREs of its programs); this form has no
+ * counterpart there. */
+typedef struct tac_kv4_cache {
+  uint8_t* k_codes;
+  uint8_t* v_codes;
+  uint32_t* k_params;
+  uint32_t* v_params;
+  int32_t num_pages;
+  int32_t page_size;
+  int32_t heads;
+  int32_t head_dim;
+} tac_kv4_cache;
+
+/* Common to the three calls: sequence b (of `batch`) has lens[b] tokens, new
+ * ones included, on the pages page_table[b][0 .. width); its new tokens are
+ * rows indptr[b] .. indptr[b + 1) of the `total` rows (indptr null: row b,
+ * total = batch), the last of its positions.  All three arrays are int32
+ * device memory.  A page number outside [0, num_pages) is a page without
+ * tokens; a row before position 0, or past the table, has no place.  Nothing
+ * in these arrays can lead outside the cache or the rows.  width * page_size
+ * at most 2^30. */
+
+/* Quantises the new tokens' keys and values into the cache.  K, V [total]
+ * [heads][head_dim] of `type`, element strides k_tok, k_head, v_tok, v_head
+ * (values of a head contiguous).  Rows without a place are skipped.  Two
+ * sequences must not append to one page position. */
+int tac_kv4_append(const tac_kv4_cache* cache, const int32_t* page_table, const int32_t* lens, const int32_t* indptr,
+                   int batch, int width, int total, const void* K, int64_t k_tok, int64_t k_head, const void* V,
+                   int64_t v_tok, int64_t v_head, int type, void* stream);
+
+/* What the new tokens' rows stand for: K, V float32 [total][heads][head_dim],
+ * 16-byte aligned; zeros for rows without a place, rows of no sequence
+ * included. */
+int tac_kv4_read(const tac_kv4_cache* cache, const int32_t* page_table, const int32_t* lens, const int32_t* indptr,
+                 int batch, int width, int total, float* K, float* V, void* stream);
+
+/* Attention of the new tokens over their sequences' cached tokens:
+ * O[i] = sum_j p_j v_j, p = softmax_j(scale * Q[i] . k_j) over the tokens j of
+ * the sequence, with causal != 0 those up to the row's own position.  Q
+ * [total][q_heads][head_dim] FP16 or BF16 (`type`) with element strides q_tok,
+ * q_head; query head h reads key-value head h / (q_heads / heads).  O
+ * [total][q_heads][head_dim] contiguous, of the same type; lse (or null)
+ * float32 [total][q_heads] gets log sum_j exp(scale * Q . k_j).  A row that
+ * sees no token gets zeros and an lse of -inf; rows of no sequence are left as
+ * they are.  The workspace (256-byte aligned, at least the bytes of the query
+ * below on the same device) must not be shared by calls that overlap. */
+uint64_t tac_kv4_attention_workspace_bytes(int batch, int total, int q_heads, int kv_heads, int head_dim);
+int tac_kv4_attention(const tac_kv4_cache* cache, const int32_t* page_table, const int32_t* lens,
+                      const int32_t* indptr, int batch, int width, int total, const void* Q, int64_t q_tok,
+                      int64_t q_head, int q_heads, int type, float scale, int causal, void* O, float* lse,
+                      void* workspace, uint64_t workspace_bytes, void* stream);
+
 /* ---- Offline weight quantisation ------------------------------------------
  * Per-channel (per_channel = 1) or per-tensor symmetric INT8 quantisation of
  * a float32 weight W[out_ch, in_features] (row-major, PyTorch layout), as

@@ -50,6 +50,13 @@ class ExecInfo(C.Structure):
 
 
 TYPE_F32, TYPE_F16, TYPE_BF16 = 0, 1, 2   # enum tac_type
+
+
+class Kv4CacheRecord(C.Structure):   # tac_kv4_cache
+    _fields_ = [("k_codes", C.c_void_p), ("v_codes", C.c_void_p), ("k_params", C.c_void_p), ("v_params", C.c_void_p),
+                ("num_pages", C.c_int32), ("page_size", C.c_int32), ("heads", C.c_int32), ("head_dim", C.c_int32)]
+
+
 COMPILE_NO_PACK = 1   # TAC_COMPILE_NO_PACK
 
 
@@ -114,6 +121,11 @@ SIGNATURES = {
     "tac_gemm_i8_scaled": (_I, [_P, _P, _P, _P, _I, _P, _I, _P, _I, _I, _I, _I, _P]),
     "tac_linear_w8a8_workspace_bytes": (_U64, [_I, _I]),
     "tac_linear_w8a8": (_I, [_P, _I, _I64, _P, _P, _I, _P, _I, _P, _I, _P, _U64, _I, _I, _I, _P]),
+    "tac_kv4_append": (_I, [_P, _P, _P, _P, _I, _I, _I, _P, _I64, _I64, _P, _I64, _I64, _I, _P]),
+    "tac_kv4_read": (_I, [_P, _P, _P, _P, _I, _I, _I, _P, _P, _P]),
+    "tac_kv4_attention_workspace_bytes": (_U64, [_I, _I, _I, _I, _I]),
+    "tac_kv4_attention": (_I, [_P, _P, _P, _P, _I, _I, _I, _P, _I64, _I64, _I, _I, C.c_float, _I, _P, _P, _P, _U64,
+                               _P]),
     "tac_quantize_weight_i8": (_I, [_P, _I, _I, _I, _P, _P, _P, _P]),
     "tac_bundle_open": (_I, [C.c_char_p, C.POINTER(BundleView), C.POINTER(_P)]),
     "tac_bundle_close": (_I, [_P]),
