@@ -376,7 +376,8 @@ int tac_linear_w8a8(const void* X, int x_type, int64_t ldx, const int8_t* Bt, co
  * [num_pages][heads][page_size][head_dim / 2], code 2j in the low and 2j + 1 in
  * the high half of byte j; parameter words [num_pages][heads][page_size], the
  * bits of s above those of z.  A row that holds an infinity or a NaN stands
- * for NaN.  All arrays 16-byte aligned device memory.  The reference's cache is
+ * for NaN.  All arrays 16-byte aligned device memory; fewer than 2^32 rows
+ * (num_pages * heads * page_size).  The reference's cache is
  * INT8 with one scale (the KV-append STOREs of its programs); this form has no
  * counterpart there. */
 typedef struct tac_kv4_cache {

@@ -175,6 +175,8 @@ int take_cache(const tac_kv4_cache* c, Kv4Cache& out) {
   if (c->page_size != 16 && c->page_size != 32 && c->page_size != 64 && c->page_size != 128) return TAC_E_ARGUMENT;
   if (!aligned(c->k_codes, 16) || !aligned(c->v_codes, 16) || !aligned(c->k_params, 16) || !aligned(c->v_params, 16))
     return TAC_E_ARGUMENT;
+  // rows of codes are counted in 32 bits (2^32 rows of 64 values are 128 GB)
+  if (int64_t(c->num_pages) * c->heads * c->page_size >= (int64_t(1) << 32)) return TAC_E_ARGUMENT;
   out = {c->k_codes, c->v_codes, c->k_params, c->v_params, c->num_pages, c->page_size, c->heads, 0};
   while ((1 << out.page_shift) < c->page_size) ++out.page_shift;
   return TAC_OK;
@@ -200,15 +202,31 @@ int rows_tiles(int batch, int total, int group) { return int64_t(total) * group 
 
 // The workspace is sized for the most CTAs that a launch can have, on any device.
 constexpr int kMaxSms = 160;
+static_assert(kMaxSms * rows_ctas(64, 1) <= 1024, "kv4_join_kernel holds a weight for each CTA");
 
-int rows_per_sm(int nt) { return nt == 1 ? 3 : 2; }
+uint64_t rows_workspace(int D, int nt) {
+  const uint64_t grid = uint64_t(kMaxSms) * rows_ctas(D, nt);
+  return grid * 2 * (8 * nt) * (D + 2) * sizeof(float) + grid * sizeof(int4);
+}
 
 template <int D, int NT>
-int launch_rows(const Kv4RowsParams& p, cudaStream_t st) {
-  const int grid = std::min(sm_count(), kMaxSms) * rows_per_sm(NT);
+int launch_rows(Kv4RowsParams p, void* workspace, cudaStream_t st) {
+  const int grid = std::min(sm_count(), kMaxSms) * rows_ctas(D, NT);
+  p.cuts = static_cast<int4*>(workspace);
+  p.part = reinterpret_cast<float*>(p.cuts + grid);
   kv4_rows_kernel<D, NT><<<grid, kRowsThreads, 0, st>>>(p);
-  kv4_join_kernel<D, NT><<<grid - 1, kRowsThreads, 0, st>>>(p, grid);
-  return status();
+  if (int s = status()) return s;
+  // launched while the first kernel still runs; it waits for that kernel's end before it reads
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid - 1, 8 * NT);
+  cfg.blockDim = dim3(D);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kv4_join_kernel<D, NT>, p) == cudaSuccess ? TAC_OK : TAC_E_CUDA;
 }
 
 }  // namespace
@@ -255,7 +273,7 @@ extern "C" uint64_t tac_kv4_attention_workspace_bytes(int batch, int total, int 
       (head_dim != 64 && head_dim != 128))
     return 0;
   const int nt = rows_tiles(batch, total, q_heads / kv_heads);
-  return uint64_t(kMaxSms) * rows_per_sm(nt) * 2 * (8 * nt) * (head_dim + 2) * sizeof(float);
+  return rows_workspace(head_dim, nt);
 }
 
 extern "C" int tac_kv4_attention(const tac_kv4_cache* cache, const int32_t* page_table, const int32_t* lens,
@@ -282,10 +300,10 @@ extern "C" int tac_kv4_attention(const tac_kv4_cache* cache, const int32_t* page
   p.bf16 = type == TAC_BF16;
   p.causal = causal != 0;
   p.scale_log2 = scale * 1.4426950408889634f;
-  p.part = static_cast<float*>(workspace);
+  p.q_vec = aligned(Q, 16) && (q_tok | q_head) % 8 == 0;
   if (sm_count() <= 0) return TAC_E_CUDA;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int nt = rows_tiles(batch, total, p.group);
-  if (cache->head_dim == 64) return nt == 1 ? launch_rows<64, 1>(p, st) : launch_rows<64, 2>(p, st);
-  return nt == 1 ? launch_rows<128, 1>(p, st) : launch_rows<128, 2>(p, st);
+  if (cache->head_dim == 64) return nt == 1 ? launch_rows<64, 1>(p, workspace, st) : launch_rows<64, 2>(p, workspace, st);
+  return nt == 1 ? launch_rows<128, 1>(p, workspace, st) : launch_rows<128, 2>(p, workspace, st);
 }
