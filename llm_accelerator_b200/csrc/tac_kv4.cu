@@ -8,6 +8,10 @@
 #include "tac_kv4.cuh"
 #include "tac_kv4_rows.cuh"
 
+namespace tac {
+int* gemm_fault_word();
+}
+
 namespace {
 
 using namespace tac;
@@ -202,7 +206,7 @@ int rows_tiles(int batch, int total, int group) { return int64_t(total) * group 
 
 // The workspace is sized for the most CTAs that a launch can have, on any device.
 constexpr int kMaxSms = 160;
-static_assert(kMaxSms * rows_ctas(64, 1) <= 1024, "kv4_join_kernel holds a weight for each CTA");
+static_assert(kMaxSms * 2 <= 1024, "kv4_join_kernel holds a weight for each CTA");
 
 uint64_t rows_workspace(int D, int nt) {
   const uint64_t grid = uint64_t(kMaxSms) * rows_ctas(D, nt);
@@ -212,10 +216,25 @@ uint64_t rows_workspace(int D, int nt) {
 template <int D, int NT>
 int launch_rows(Kv4RowsParams p, void* workspace, cudaStream_t st) {
   const int grid = std::min(sm_count(), kMaxSms) * rows_ctas(D, NT);
+  // Contexts of up to four tiles are not worth the second launch that joining pieces takes.
+  // Tiles are counted in 31 bits; a batch that could have more goes by units.
+  const double capacity = double(p.s.width) * p.c.page_size;
+  const double most = (double(p.s.total) * p.hq / (8 * NT) + double(p.s.batch) * p.c.heads) * (capacity / kRowsTile + 1);
+  p.split = capacity > 4 * kRowsTile && most < 2147483648.0;
   p.cuts = static_cast<int4*>(workspace);
   p.part = reinterpret_cast<float*>(p.cuts + grid);
-  kv4_rows_kernel<D, NT><<<grid, kRowsThreads, 0, st>>>(p);
+  static bool smem_set[64] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return TAC_E_CUDA;
+  if (!smem_set[dev]) {
+    if (cudaFuncSetAttribute(kv4_rows_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, rows_smem(D, NT)) !=
+        cudaSuccess)
+      return TAC_E_CUDA;
+    smem_set[dev] = true;
+  }
+  kv4_rows_kernel<D, NT><<<grid, kRowsThreads, rows_smem(D, NT), st>>>(p);
   if (int s = status()) return s;
+  if (!p.split) return TAC_OK;
   // launched while the first kernel still runs; it waits for that kernel's end before it reads
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(grid - 1, 8 * NT);
@@ -300,6 +319,7 @@ extern "C" int tac_kv4_attention(const tac_kv4_cache* cache, const int32_t* page
   p.bf16 = type == TAC_BF16;
   p.causal = causal != 0;
   p.scale_log2 = scale * 1.4426950408889634f;
+  p.o_vec = aligned(O, 16);
   p.q_vec = aligned(Q, 16) && (q_tok | q_head) % 8 == 0;
   if (sm_count() <= 0) return TAC_E_CUDA;
   cudaStream_t st = static_cast<cudaStream_t>(stream);

@@ -6,28 +6,36 @@
 // channels) on its 16 rows and the query rows of one key-value head on its 8
 // columns: S^T = C q^T, O^T = C'^T (p s')^T.  A thread's fragment of C is the
 // 16 or 8 contiguous bytes of one key that it loads, its fragment of C'^T the
-// bytes of the same channels of two keys, interleaved by two PRMTs: the cache
-// goes from global memory to registers to the tensor cores, with no shared
-// memory and no shuffle.  P^T changes from accumulator to operand layout by
-// movmatrix.  Bound by the cache's bytes: 4.5 bits a value at D = 128.
+// bytes of the same channels of two keys, interleaved by two PRMTs: no shuffle
+// and no second pass through shared memory.  P^T changes from accumulator to
+// operand layout by movmatrix.
 //
-// Work is cut into equal shares over all (sequence, head, row block) units
-// laid end to end in tiles of 128 keys, whatever the lengths: a unit that one
-// CTA covers is finished there, the pieces of one that several cover go to
-// the workspace and kv4_join_kernel adds them in order.  The cuts depend on
-// the lengths and the grid only, so results do not change from run to run.
+// Each of eight warps takes 32 keys of a tile of 256 and has a ring of stages
+// of its own, which it fills two or three tiles ahead by 16-byte asynchronous
+// copies; nothing waits for another warp before the unit's end.  (Bulk copies,
+// one for the 512 bytes that a head has of 16 keys, need an instruction for
+// each, lane by lane: 132 us instead of LATER at the 64-sequence case.)
+//
+// Work is laid end to end over all (sequence, head, row block) units.  Where a
+// sequence can be long (p.split), the CTAs take equal shares of its tiles
+// whatever the lengths: a unit that one CTA covers is finished there, the
+// pieces of one that several cover go to the workspace and kv4_join_kernel
+// adds them in order.  Else they take whole units, and there is nothing to
+// join.  The cuts depend on the lengths and the grid only, so results do not
+// change from run to run.
 #pragma once
 #include <type_traits>
 
 #include "tac_kv4.cuh"
+#include "tac_sm100.cuh"
 
 namespace tac {
 
-constexpr int kRowsWarps = 4;
+constexpr int kRowsWarps = 8;
 constexpr int kRowsThreads = kRowsWarps * 32;
 constexpr float kSlack = 8.f;
 constexpr uint32_t kSlackV = 6;
-constexpr int kRowsTile = kRowsWarps * 32;   // keys of a tile, 32 a warp
+constexpr int kRowsTile = kRowsWarps * 32;         // keys of a tile, 32 a warp
 
 struct Kv4RowsParams {
   Kv4Cache c;
@@ -37,9 +45,9 @@ struct Kv4RowsParams {
   float* lse;            // or null
   int64_t q_tok, q_head; // strides in elements
   int hq, group;         // query heads, query heads of one key-value head
-  int bf16, causal;
+  int bf16, causal, split;
+  int q_vec, o_vec;      // q's, o's rows are 16-byte aligned
   float scale_log2;      // softmax scale * log2(e)
-  int q_vec;             // q's rows are 16-byte aligned
   float* part;           // [2 * grid][rows * (D + 2)]
   int4* cuts;            // [grid]: the unit that CTA j's share begins inside of, if it is the first cut of that unit
 };
@@ -93,92 +101,98 @@ __device__ __forceinline__ float exp2_(float x) {
   return y;
 }
 
-// The shares: `total` tiles over `parts` CTAs, CTA j from total * j / parts on.
-struct Shares {
-  int64_t total;
-  int parts;
-  __device__ int64_t at(int64_t j) const { return total * j / parts; }
-};
-
 template <int D, int NT>
 struct RowsCfg {
   static constexpr int kRows = 8 * NT;
   static constexpr int kPart = kRows * (D + 2);   // floats of a piece: O, then m and l of each row
 };
 
-// Tiles of one unit of sequence b, and its units.
-__device__ __forceinline__ void seq_cost(const Kv4Seq& s, int group, int heads, int rows, int& tiles, int64_t& units) {
-  tiles = max(1, (s.len + kRowsTile - 1) / kRowsTile);
-  units = (int64_t(s.n) * group + rows - 1) / rows * heads;
+// Tiles of one unit of sequence b, its units, and its cost in what shares are cut in (units if !p.split, else tiles;
+// the host sees to it that the sum over the sequences fits 31 bits).
+struct SeqCost {
+  uint32_t tiles, units, cost;
+};
+
+__device__ __forceinline__ SeqCost seq_cost(const Kv4RowsParams& p, const Kv4Seq& s, int rows) {
+  SeqCost c;
+  c.tiles = max(1, (s.len + kRowsTile - 1) / kRowsTile);
+  c.units = (uint32_t(s.n) * p.group + rows - 1) / rows * p.c.heads;
+  c.cost = p.split ? c.units * c.tiles : c.units;
+  return c;
 }
 
-// Every thread of the CTA: total tiles, then the sequence that tile `x` of all
-// lies in and its first tile.
-__device__ inline int64_t block_sum(int64_t v, int64_t* red) {
-#pragma unroll
-  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = 0;
-#pragma unroll
-  for (int w = 0; w < kRowsWarps; ++w) v += red[w];
-  return v;
-}
+// `total` cut into `parts` shares, the first `rem` of them one larger.
+struct Cuts {
+  uint32_t total, parts, base, rem;
+  __device__ Cuts() = default;
+  __device__ Cuts(uint32_t total, uint32_t grid) : total(total), parts(min(total, grid)) {
+    base = parts ? total / parts : 0;
+    rem = total - base * parts;
+  }
+  __device__ uint32_t at(uint32_t i) const { return i < parts ? i * base + min(i, rem) : total; }
+  // the share that tile x lies in
+  __device__ uint32_t share(uint32_t x) const {
+    const uint32_t big = rem * (base + 1);
+    return x < big ? x / (base + 1) : rem + (x - big) / base;
+  }
+};
 
-__device__ inline int64_t seq_cost_of(const Kv4RowsParams& p, int b, int rows) {
-  if (b >= p.s.batch) return 0;
-  const Kv4Seq s = kv4_seq(p.s, b, int64_t(p.s.width) * p.c.page_size);
-  int tiles;
-  int64_t units;
-  seq_cost(s, p.group, p.c.heads, rows, tiles, units);
-  return units * tiles;
-}
+// All threads of the CTA: the cuts, and the sequence that share `me` begins in (none for an empty share) with the
+// place where that sequence begins.
+struct Start {
+  Cuts cuts;
+  uint32_t x0, x1, first;
+  int b;
+};
 
-__device__ inline Shares make_shares(const Kv4RowsParams& p, int rows, int grid, int64_t* red) {
-  int64_t v = 0;
-  for (int b = threadIdx.x; b < p.s.batch; b += kRowsThreads) v += seq_cost_of(p, b, rows);
-  Shares sh;
-  sh.total = block_sum(v, red);
-  sh.parts = sh.total < grid ? int(max(sh.total, int64_t(1))) : grid;
-  return sh;
-}
-
-__device__ inline void find_seq(const Kv4RowsParams& p, int rows, int64_t x, int64_t* red, int* found, int& b, int64_t& first) {
-  int64_t base = 0;
-  for (int b0 = 0; b0 < p.s.batch; b0 += kRowsThreads) {
-    const int64_t c = seq_cost_of(p, b0 + threadIdx.x, rows);
-    int64_t inc = c;
+__device__ inline Start find_start(const Kv4RowsParams& p, int rows, uint32_t grid, uint32_t me, uint32_t* red, Start* found) {
+  const int64_t cap = int64_t(p.s.width) * p.c.page_size;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const bool one = p.s.batch <= kRowsThreads;    // a thread for each sequence: one pass does
+  Start st;
+  st.first = 0;
+  st.b = p.s.batch;
+  uint32_t base = 0;
+  for (int pass = one ? 1 : 0; pass < 2; ++pass) {
+    base = 0;
+    for (int b0 = 0; b0 < p.s.batch; b0 += kRowsThreads) {
+      const int b = b0 + threadIdx.x;
+      const uint32_t c = b < p.s.batch ? seq_cost(p, kv4_seq(p.s, b, cap), rows).cost : 0;
+      uint32_t inc = c;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int64_t u = __shfl_up_sync(0xffffffffu, inc, o);
-      if (int(threadIdx.x & 31) >= o) inc += u;
-    }
-    __syncthreads();
-    if ((threadIdx.x & 31) == 31) red[threadIdx.x >> 5] = inc;
-    __syncthreads();
-    int64_t all = 0, before = 0;
-#pragma unroll
-    for (int w = 0; w < kRowsWarps; ++w) {
-      if (w < int(threadIdx.x >> 5)) before += red[w];
-      all += red[w];
-    }
-    if (x < base + all) {
-      const int64_t start = base + before + inc - c;
-      if (x >= start && x < start + c) {
-        found[0] = b0 + threadIdx.x;
-        *reinterpret_cast<int64_t*>(found + 2) = start;
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t u = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += u;
       }
       __syncthreads();
-      b = found[0];
-      first = *reinterpret_cast<int64_t*>(found + 2);
+      if (lane == 31) red[warp] = inc;
       __syncthreads();
-      return;
+      uint32_t all = 0, before = base;
+#pragma unroll
+      for (int w = 0; w < kRowsThreads / 32; ++w) {
+        if (w < warp) before += red[w];
+        all += red[w];
+      }
+      if (one) st.cuts = Cuts(all, grid);
+      if (pass) {
+        if (b0 == 0) st.x0 = st.cuts.at(me), st.x1 = st.cuts.at(me + 1);
+        if (st.x0 >= st.x1) return st;           // an empty share
+        if (st.x0 < base + all) {                // it begins in this chunk
+          const uint32_t start = before + inc - c;
+          if (st.x0 >= start && st.x0 < start + c) {
+            st.first = start;
+            st.b = b;
+            *found = st;
+          }
+          __syncthreads();
+          return *found;
+        }
+      }
+      base += all;
     }
-    base += all;
+    if (!pass) st.cuts = Cuts(base, grid);
   }
-  b = p.s.batch;
-  first = base;
+  return st;                                     // not reached: a share that is not empty begins somewhere
 }
 
 __device__ __forceinline__ float ld_q(const Kv4RowsParams& p, int64_t i) {
@@ -190,8 +204,19 @@ __device__ __forceinline__ void st_o(const Kv4RowsParams& p, int64_t i, float v)
   p.o[i] = p.bf16 ? __bfloat16_as_ushort(__float2bfloat16_rn(v)) : __half_as_ushort(__float2half_rn(v));
 }
 
-// Resident CTAs that the registers are cut for (kv4_rows_kernel).
-__host__ __device__ constexpr int rows_ctas(int D, int NT) { return NT == 1 ? (D == 64 ? 4 : 3) : (D == 64 ? 3 : 2); }
+// Resident CTAs that the registers and the ring are cut for (kv4_rows_kernel).
+__host__ __device__ constexpr int rows_ctas(int D, int NT) { return D == 128 && NT == 2 ? 1 : 2; }
+// A stage: 32 keys' codes of K, then of V, then their words.
+__host__ __device__ constexpr int rows_stage(int D) { return 2 * 32 * (D / 2) + 2 * 32 * 4; }
+__host__ __device__ constexpr int rows_stages(int D, int NT) { return D == 128 && NT == 1 ? 3 : 4; }
+// What one warp hands another: O, mu and l of its rows, a float4 of each lane at a time.  The slots take the rings'
+// place once every warp has done its tiles.
+__host__ __device__ constexpr int rows_slot(int D, int NT) { return 32 * 4 * (NT * D / 4 + 4 * NT); }
+__host__ __device__ constexpr int rows_smem(int D, int NT) { return kRowsWarps * rows_stages(D, NT) * rows_stage(D); }
+
+__device__ __forceinline__ void copy16(void* dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(sm100::smem_u32(dst)), "l"(src) : "memory");
+}
 
 template <int D, int NT>
 __global__ void __launch_bounds__(kRowsThreads, rows_ctas(D, NT)) kv4_rows_kernel(Kv4RowsParams p) {
@@ -199,115 +224,89 @@ __global__ void __launch_bounds__(kRowsThreads, rows_ctas(D, NT)) kv4_rows_kerne
   constexpr int R = Cfg::kRows;
   constexpr int W = D / 32;         // words of one key that a thread converts for S
   constexpr int VW = D / 64;        // words of one key that it converts for O
-  __shared__ int64_t red[kRowsWarps];
-  __shared__ __align__(8) int found[4];
-  __shared__ float sm_o[kRowsWarps][R][D + 4];
-  __shared__ float sm_m[kRowsWarps][R], sm_l[kRowsWarps][R];
+  constexpr int ST = rows_stages(D, NT), kStage = rows_stage(D);
+  static_assert(rows_smem(D, NT) >= 5 * rows_slot(D, NT), "the slots take the rings' place");
+  extern __shared__ __align__(128) uint8_t ring_all[];
+  __shared__ uint32_t red[kRowsThreads / 32];
+  __shared__ Start found;
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const Shares sh = make_shares(p, R, gridDim.x, red);
   asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
-  if (threadIdx.x == 0) p.cuts[blockIdx.x] = make_int4(-1, 0, 0, 0);
-  if (int(blockIdx.x) >= sh.parts || sh.total == 0) return;
-  const int64_t x0 = sh.at(blockIdx.x), x1 = sh.at(blockIdx.x + 1);
-  int b;
-  int64_t off;
-  find_seq(p, R, x0, red, found, b, off);
-  off = x0 - off;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  uint8_t* const ring = ring_all + warp * ST * kStage;
+  if (p.split && threadIdx.x == 0) p.cuts[blockIdx.x] = make_int4(-1, 0, 0, 0);
+  const Start sh = find_start(p, R, gridDim.x, blockIdx.x, red, &found);
+  // Key of a slab's row r and of row r + 8 (less 8): this order keeps both operands' reads of the ring free of bank
+  // conflicts (V's at D = 128 aside: two rows of four share banks in any order).
+  const int key_g = g & 1 ? 7 - (g >> 1) : g >> 1;
 
-  for (int64_t x = x0; x < x1 && b < p.s.batch;) {
+  int b = sh.b;
+  uint32_t off = sh.x0 - sh.first;
+  for (uint32_t x = sh.x0; x < sh.x1 && b < p.s.batch;) {
     const Kv4Seq s = kv4_seq(p.s, b, int64_t(p.s.width) * p.c.page_size);
-    int tiles;
-    int64_t units;
-    seq_cost(s, p.group, p.c.heads, R, tiles, units);
-    if (off >= units * tiles) {
+    const SeqCost sc_b = seq_cost(p, s, R);
+    if (off >= sc_b.cost) {
       ++b;
       off = 0;
       continue;
     }
-    const int64_t unit = off / tiles;
-    const int t0 = int(off - unit * tiles);
-    const int t1 = int(min(int64_t(tiles), t0 + (x1 - x)));
-    const int h = int(unit % p.c.heads), r0 = int(unit / p.c.heads) * R;
+    const uint32_t tiles = sc_b.tiles, unit = p.split ? off / tiles : off;
+    const int t0 = p.split ? off - unit * tiles : 0;
+    const int t1 = p.split ? min(tiles, t0 + (sh.x1 - x)) : tiles;
+    const int step_x = p.split ? t1 - t0 : 1;
+    const bool first_piece = x == sh.x0;
+    const int h = unit % p.c.heads, r0 = unit / p.c.heads * R;
     const int rows_all = s.n * p.group;
+    const int t_end = min(t1, (s.len + kRowsTile - 1) / kRowsTile);   // none for an empty sequence
+    x += step_x;
+    off += step_x;
+
     const int32_t* table = p.s.table + int64_t(b) * p.s.width;
-    if (x == x0 && threadIdx.x == 0) {
+    if (p.split && first_piece && threadIdx.x == 0) {
       // For kv4_join_kernel: this share's first unit, when the cut before it is the first one inside that unit, with
       // the last CTA that has a piece of it and the place of its first piece
-      int4 cut = make_int4(-1, 0, 0, 0);
-      const int64_t u0 = x0 - t0, prev = blockIdx.x ? sh.at(blockIdx.x - 1) : 0;
-      if (t0 > 0 && u0 >= prev) {
-        int last = blockIdx.x;
-        while (last + 1 < sh.parts && sh.at(last + 1) < u0 + tiles) ++last;
-        cut = make_int4(b, r0, last, (u0 == prev ? 0 : 1) | h << 1);
-      }
-      p.cuts[blockIdx.x] = cut;
+      const uint32_t u0 = sh.x0 - t0, prev = blockIdx.x ? sh.cuts.at(blockIdx.x - 1) : 0;
+      if (t0 > 0 && u0 >= prev)
+        p.cuts[blockIdx.x] = make_int4(b, r0, sh.cuts.share(u0 + tiles - 1), (u0 == prev ? 0 : 1) | h << 1);
     }
 
-    // ---- the cache's words of one tile, held in registers a tile ahead ----
-    uint32_t kw[2][2][W] = {}, kpw[2][2] = {}, vw[2][4][VW] = {}, vpw[2][2] = {};
-    int page[2], page1[2];          // of the tile in kw / vw, of the one after it; -1: no keys
+    // ---- copies of this warp's 32 keys of a tile, two slabs of 16 keys that each lie in one page ----
     auto get_page = [&](int tile, int u) -> int {
       const int k0 = tile * kRowsTile + warp * 32 + 16 * u;
-      if (tile >= t1 || k0 >= s.len) return -1;
+      if (tile >= t_end || k0 >= s.len) return -1;
       const int id = __ldg(table + (k0 >> p.c.page_shift));
       return uint32_t(id) < uint32_t(p.c.num_pages) ? id : -1;
     };
-    // Cache row of the first of the 16 keys; the number of rows fits 32 bits (checked on the host).
-    auto row_of = [&](int tile, int u, int pg) -> uint32_t {
-      const uint32_t k0 = tile * kRowsTile + warp * 32 + 16 * u;
-      return (uint32_t(pg) * p.c.heads + h) * p.c.page_size + (k0 & (p.c.page_size - 1));
-    };
-    const uint8_t* const kc = p.c.kc + g * (D / 2) + t * (D / 8);
-    const uint8_t* const vc = p.c.vc + 2 * t * (D / 2) + g * (D / 16);
-    auto load_k = [&](const int (&pg)[2], const uint32_t (&row)[2]) {
+    uint32_t have_bits = 0;         // two bits a stage: which of its slabs hold keys
+    auto fetch = [&](int tile, int st, const int (&pg)[2]) {
+      uint8_t* dst = ring + st * kStage + lane * 16;
+      uint32_t bits = 0;
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         if (pg[u] < 0) continue;
-        const uint8_t* src = kc + uint64_t(row[u]) * (D / 2);
-        const uint32_t* words = p.c.kp + g + uint64_t(row[u]);
+        bits |= 1u << u;
+        const uint32_t k0 = tile * kRowsTile + warp * 32 + 16 * u;
+        const uint64_t row = (uint32_t(pg[u]) * p.c.heads + h) * p.c.page_size + (k0 & (p.c.page_size - 1));   // fits 32 bits
+        const uint8_t *ks = p.c.kc + row * (D / 2) + lane * 16, *vs = p.c.vc + row * (D / 2) + lane * 16;
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          if constexpr (W == 4) {
-            const uint4 v = __ldg(reinterpret_cast<const uint4*>(src + j * 8 * (D / 2)));
-            kw[u][j][0] = v.x, kw[u][j][1] = v.y, kw[u][j][2] = v.z, kw[u][j][3] = v.w;
-          } else {
-            const uint2 v = __ldg(reinterpret_cast<const uint2*>(src + j * 8 * (D / 2)));
-            kw[u][j][0] = v.x, kw[u][j][1] = v.y;
-          }
-          kpw[u][j] = __ldg(words + 8 * j);
+        for (int i = 0; i < D / 64; ++i) {
+          copy16(dst + u * 16 * (D / 2) + i * 512, ks + i * 512);
+          copy16(dst + (32 + u * 16) * (D / 2) + i * 512, vs + i * 512);
+        }
+        if (lane < 8) {               // the words: 64 bytes of K's, 64 of V's
+          const uint32_t* ws = (lane < 4 ? p.c.kp : p.c.vp) + row + (lane & 3) * 4;
+          copy16(ring + st * kStage + 32 * D + (lane >> 2) * 128 + u * 64 + (lane & 3) * 16, ws);
         }
       }
+      asm volatile("cp.async.commit_group;\n" ::: "memory");
+      have_bits = (have_bits & ~(3u << (2 * st))) | bits << (2 * st);
     };
-    auto load_v = [&](const int (&pg)[2], const uint32_t (&row)[2]) {
+    {
+      int pg[ST][2];
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        if (pg[u] < 0) continue;
-        const uint8_t* src = vc + uint64_t(row[u]) * (D / 2);
-        const uint32_t* words = p.c.vp + g + uint64_t(row[u]);
+      for (int i = 0; i < ST; ++i) pg[i][0] = get_page(t0 + i, 0), pg[i][1] = get_page(t0 + i, 1);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {        // keys 2t, 2t + 1, 2t + 8, 2t + 9
-          const uint8_t* sj = src + ((j & 1) + 8 * (j >> 1)) * (D / 2);
-          if constexpr (VW == 2) {
-            const uint2 v = __ldg(reinterpret_cast<const uint2*>(sj));
-            vw[u][j][0] = v.x, vw[u][j][1] = v.y;
-          } else {
-            vw[u][j][0] = __ldg(reinterpret_cast<const uint32_t*>(sj));
-          }
-        }
-#pragma unroll
-        for (int j = 0; j < 2; ++j) vpw[u][j] = __ldg(words + 8 * j);
-      }
-    };
-    uint32_t row1[2];               // cache rows of the tile that the next loads take
-#pragma unroll
-    for (int u = 0; u < 2; ++u) page[u] = get_page(t0, u), page1[u] = get_page(t0 + 1, u);
-#pragma unroll
-    for (int u = 0; u < 2; ++u) row1[u] = row_of(t0, u, page[u]);
-    load_k(page, row1);
-    load_v(page, row1);
-#pragma unroll
-    for (int u = 0; u < 2; ++u) row1[u] = row_of(t0 + 1, u, page1[u]);
+      for (int i = 0; i < ST; ++i) fetch(t0 + i, i, pg[i]);
+    }
 
     // ---- query rows: FP16, each scaled by the power of two that brings its largest magnitude into [1, 2) ----
     uint32_t qf[NT][2 * W][2];
@@ -380,13 +379,39 @@ __global__ void __launch_bounds__(kRowsThreads, rows_ctas(D, NT)) kv4_rows_kerne
 #pragma unroll
     for (int n = 0; n < NT; ++n) ve[n][0] = ve[n][1] = 1;
 
-    auto step = [&](int tile, auto masked_c) {
+    auto step = [&](int tile, int st, auto masked_c) {
       constexpr bool kMasked = decltype(masked_c)::value;
       const int key0 = tile * kRowsTile + warp * 32;
-      const bool have[2] = {page[0] >= 0, page[1] >= 0};
-      auto seen = [&](int u, int j, int n, int i) { return key0 + 16 * u + 8 * j + g < lim[n][i] && have[u]; };
+      const uint32_t have = have_bits >> (2 * st);
+      auto seen = [&](int u, int j, int n, int i) { return key0 + 16 * u + 8 * j + key_g < lim[n][i] && (have >> u & 1); };
+      const uint8_t* stage = ring + st * kStage;
+      uint32_t kpw[2][2], vpw[2][2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const uint32_t* words = reinterpret_cast<const uint32_t*>(stage + 32 * D) + 16 * u + 8 * j + key_g;
+          kpw[u][j] = words[0];
+          vpw[u][j] = words[32];
+          // a slot without a token may hold any bits
+          if (kMasked && !(key0 + 16 * u + 8 * j + key_g < s.len && (have >> u & 1))) kpw[u][j] = vpw[u][j] = 0;
+        }
       // ---- S^T ----
       float sc[2][NT][4] = {};
+      uint32_t kw[2][2][W];
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const uint8_t* src = stage + (16 * u + 8 * j + key_g) * (D / 2) + t * (D / 8);
+          if constexpr (W == 4) {
+            const uint4 v = *reinterpret_cast<const uint4*>(src);
+            kw[u][j][0] = v.x, kw[u][j][1] = v.y, kw[u][j][2] = v.z, kw[u][j][3] = v.w;
+          } else {
+            const uint2 v = *reinterpret_cast<const uint2*>(src);
+            kw[u][j][0] = v.x, kw[u][j][1] = v.y;
+          }
+        }
 #pragma unroll
       for (int w = 0; w < W; ++w)
 #pragma unroll
@@ -417,7 +442,6 @@ __global__ void __launch_bounds__(kRowsThreads, rows_ctas(D, NT)) kv4_rows_kerne
               sc[u][n][2 * j + i] = v;
             }
         }
-      load_k(page1, row1);                          // lands during the rest of this tile
       // ---- softmax over the keys of this warp ----
       const uint32_t vtop = max(max(vpw[0][0], vpw[0][1]), max(vpw[1][0], vpw[1][1]));
       if (__any_sync(0xffffffffu, kMasked || hot > kSlack || vtop >= vlim)) {
@@ -494,13 +518,24 @@ __global__ void __launch_bounds__(kRowsThreads, rows_ctas(D, NT)) kv4_rows_kerne
       }
       // ---- O^T ----
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
+      for (int u = 0; u < 2; ++u) {
+        uint32_t vw[4][VW];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {          // rows 2t, 2t + 1, 2t + 8, 2t + 9 of the slab
+          const uint8_t* src = stage + (32 + 16 * u + 8 * (j >> 1) + (j & 1 ? 7 - t : t)) * (D / 2) + g * (D / 16);
+          if constexpr (VW == 2) {
+            const uint2 v = *reinterpret_cast<const uint2*>(src);
+            vw[j][0] = v.x, vw[j][1] = v.y;
+          } else {
+            vw[j][0] = *reinterpret_cast<const uint32_t*>(src);
+          }
+        }
 #pragma unroll
         for (int w = 0; w < VW; ++w)
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
             const uint32_t sel = half ? 0x7632 : 0x5410;
-            const uint32_t a = __byte_perm(vw[u][0][w], vw[u][1][w], sel), c = __byte_perm(vw[u][2][w], vw[u][3][w], sel);
+            const uint32_t a = __byte_perm(vw[0][w], vw[1][w], sel), c = __byte_perm(vw[2][w], vw[3][w], sel);
             const uint32_t p00 = kv4_pair<0>(a), p01 = kv4_pair<0>(c), p10 = kv4_pair<1>(a), p11 = kv4_pair<1>(c);
             const uint32_t p20 = kv4_pair<2>(a), p21 = kv4_pair<2>(c), p30 = kv4_pair<3>(a), p31 = kv4_pair<3>(c);
 #pragma unroll
@@ -509,78 +544,119 @@ __global__ void __launch_bounds__(kRowsThreads, rows_ctas(D, NT)) kv4_rows_kerne
               mma_16816(o[n][4 * w + 2 * half + 1], p20, p30, p21, p31, pb[u][n][0], pb[u][n][1]);
             }
           }
-      load_v(page1, row1);                          // lands during the next tile's scores
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        page[u] = page1[u];
-        page1[u] = get_page(tile + 2, u);
-        row1[u] = row_of(tile + 2, u, page1[u]);
       }
     };
-    for (int tile = t0; tile < t1; ++tile) {
+    int st = 0;
+    for (int tile = t0; tile < t_end; ++tile) {
       const int key0 = tile * kRowsTile + warp * 32;
       if (key0 >= s.len) break;
-      if (key0 + 32 > lim_min || page[0] < 0 || page[1] < 0) step(tile, std::true_type{});
-      else step(tile, std::false_type{});
+      const int pg[2] = {get_page(tile + ST, 0), get_page(tile + ST, 1)};
+      asm volatile("cp.async.wait_group %0;\n" ::"n"(ST - 1) : "memory");
+      __syncwarp();                 // every lane's copies of this stage have landed
+      if (key0 + 32 > lim_min || (have_bits >> (2 * st) & 3u) != 3u) step(tile, st, std::true_type{});
+      else step(tile, st, std::false_type{});
+      __syncwarp();                 // every lane has read the stage
+      fetch(tile + ST, st, pg);
+      if (++st == ST) st = 0;
     }
+    asm volatile("cp.async.wait_group 0;\n" ::: "memory");
+    __syncthreads();                // every ring is at rest: the slots take their place
 
-    // ---- the warps' pieces of the unit, then the unit's result or this CTA's piece of it ----
-    __syncthreads();                               // the last unit's reads of sm_* are done
+    // ---- the warps' shares of the unit join pairwise: warp w hands its rows to warp w - half ----
+    float mx[NT][2];
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        float v = l[n][i], z = zo[n][i];
 #pragma unroll
         for (int f = 4; f < 32; f <<= 1) {
-          v += __shfl_xor_sync(0xffffffffu, v, f);
-          z += __shfl_xor_sync(0xffffffffu, z, f);
+          l[n][i] += __shfl_xor_sync(0xffffffffu, l[n][i], f);
+          zo[n][i] += __shfl_xor_sync(0xffffffffu, zo[n][i], f);
         }
-        zo[n][i] = z;
-        if (g == 0) {
-          sm_m[warp][n * 8 + 2 * t + i] = v == 0.f ? -INFINITY : mu[n][i];
-          sm_l[warp][n * 8 + 2 * t + i] = v;
+        mx[n][i] = l[n][i] == 0.f ? -INFINITY : mu[n][i];
+        const float up = __uint_as_float(ve[n][i] << 23);
+#pragma unroll
+        for (int d = 0; d < D / 16; ++d) {
+          o[n][d][i] = (o[n][d][i] - zo[n][i]) * up;
+          o[n][d][2 + i] = (o[n][d][2 + i] - zo[n][i]) * up;
         }
       }
+    uint8_t* const slots = ring_all;
 #pragma unroll
-      for (int w = 0; w < VW; ++w)
+    for (int half = 4; half; half >>= 1) {
+      // a slot is written by the warp that has read it last, or after a barrier that its last reader has joined
+      const int slot = half == 4 ? (warp & 3) : half == 2 ? 2 + (warp & 1) : 4;
+      float4* hand = reinterpret_cast<float4*>(slots + slot * rows_slot(D, NT)) + lane;
+      if (warp >= half && warp < 2 * half) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+        for (int n = 0; n < NT; ++n) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            sm_o[warp][n * 8 + 2 * t + (i & 1)][(D / 8) * g + 8 * w + 2 * j + (i >> 1)] =
-                (o[n][4 * w + j][i] - zo[n][i & 1]) * __uint_as_float(ve[n][i & 1] << 23);
+          for (int d = 0; d < D / 16; ++d) hand[(n * (D / 16 + 1) + d) * 32] = make_float4(o[n][d][0], o[n][d][1], o[n][d][2], o[n][d][3]);
+          hand[(n * (D / 16 + 1) + D / 16) * 32] = make_float4(mx[n][0], mx[n][1], l[n][0], l[n][1]);
+        }
+      }
+      __syncthreads();
+      if (warp < half && warp + half < kRowsWarps) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          const float4 ml = hand[(n * (D / 16 + 1) + D / 16) * 32];
+          const float m2[2] = {ml.x, ml.y}, l2[2] = {ml.z, ml.w};
+          float ea[2], eb[2];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const float top = fmaxf(mx[n][i], m2[i]), base = top == -INFINITY ? 0.f : top;
+            ea[i] = exp2_(mx[n][i] - base);
+            eb[i] = exp2_(m2[i] - base);
+            mx[n][i] = top;
+            l[n][i] = l[n][i] * ea[i] + l2[i] * eb[i];
+          }
+#pragma unroll
+          for (int d = 0; d < D / 16; ++d) {
+            const float4 v = hand[(n * (D / 16 + 1) + d) * 32];
+            o[n][d][0] = o[n][d][0] * ea[0] + v.x * eb[0];
+            o[n][d][1] = o[n][d][1] * ea[1] + v.y * eb[1];
+            o[n][d][2] = o[n][d][2] * ea[0] + v.z * eb[0];
+            o[n][d][3] = o[n][d][3] * ea[1] + v.w * eb[1];
+          }
+        }
+      }
     }
-    __syncthreads();
-    const bool whole = t0 == 0 && t1 == tiles;
-    float* part = p.part + (2 * int64_t(blockIdx.x) + (x == x0 ? 0 : 1)) * Cfg::kPart;
-    for (int i = threadIdx.x; i < R * D; i += kRowsThreads) {
-      const int r = i / D, d = i % D;
-      float mx = sm_m[0][r];
+    __syncthreads();                // the slots have been read: the next unit's copies may start
+    if (warp != 0) continue;
+    // ---- the unit's result, or this CTA's piece of it: a lane has D / 8 channels in a row of two rows each ----
+    const bool whole = t0 == 0 && t1 == int(tiles);
+    float* part = p.part + (2 * int64_t(blockIdx.x) + (first_piece ? 0 : 1)) * Cfg::kPart;
 #pragma unroll
-      for (int w = 1; w < kRowsWarps; ++w) mx = fmaxf(mx, sm_m[w][r]);
-      const float mu = mx == -INFINITY ? 0.f : mx;
-      float sum = 0.f, acc = 0.f;
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int w = 0; w < kRowsWarps; ++w) {
-        const float e = exp2_(sm_m[w][r] - mu);
-        sum += sm_l[w][r] * e;
-        acc += sm_o[w][r][d] * e;
-      }
-      if (whole) {
-        const int rr = r0 + r;
-        if (rr < rows_all) {
+      for (int i = 0; i < 2; ++i) {
+        const int r = n * 8 + 2 * t + i, rr = r0 + r;
+        if (!whole) {
+          float4* dst = reinterpret_cast<float4*>(part + r * D + (D / 8) * g);
+#pragma unroll
+          for (int d = 0; d < D / 16; d += 2) dst[d / 2] = make_float4(o[n][d][i], o[n][d][2 + i], o[n][d + 1][i], o[n][d + 1][2 + i]);
+          if (g == 0) part[R * D + r] = mx[n][i], part[R * D + R + r] = l[n][i];
+        } else if (rr < rows_all) {
           const int64_t oi = int64_t(s.q0 + rr / p.group) * p.hq + h * p.group + rr % p.group;
-          st_o(p, oi * D + d, sum == 0.f ? 0.f : acc / sum);
-          if (p.lse && d == 0) p.lse[oi] = sum == 0.f ? -INFINITY : (mx + log2f(sum)) * 0.69314718055994531f;
+          const float inv = l[n][i] == 0.f ? 0.f : 1.f / l[n][i];
+          uint16_t* dst = p.o + oi * D + (D / 8) * g;
+          uint32_t w[D / 16];
+#pragma unroll
+          for (int d = 0; d < D / 16; ++d) {
+            const float a = o[n][d][i] * inv, c = o[n][d][2 + i] * inv;
+            w[d] = p.bf16 ? uint32_t(__bfloat16_as_ushort(__float2bfloat16_rn(a))) | uint32_t(__bfloat16_as_ushort(__float2bfloat16_rn(c))) << 16
+                          : h2_u(__floats2half2_rn(a, c));
+          }
+          if (p.o_vec) {
+#pragma unroll
+            for (int d = 0; d < D / 16; d += 4) reinterpret_cast<uint4*>(dst)[d / 4] = make_uint4(w[d], w[d + 1], w[d + 2], w[d + 3]);
+          } else {
+#pragma unroll
+            for (int d = 0; d < D / 16; ++d) dst[2 * d] = uint16_t(w[d]), dst[2 * d + 1] = uint16_t(w[d] >> 16);
+          }
+          if (p.lse && g == 0) p.lse[oi] = l[n][i] == 0.f ? -INFINITY : (mx[n][i] + log2f(l[n][i])) * 0.69314718055994531f;
         }
-      } else {
-        part[i] = acc;
-        if (d == 0) part[R * D + r] = mx, part[R * D + R + r] = sum;
       }
-    }
-    x += t1 - t0;
-    off += t1 - t0;
   }
 }
 

@@ -170,7 +170,7 @@ def test_what_unused_slots_hold_does_not_matter(new):
     ptr = [0, new, 2 * new, 3 * new]
     q = queries(3 * new, 6, 64, torch.float16)
     outs = []
-    for junk in ((0, 0), (0xFF, 0x7FC0000F), (0xA5, 0x7F800003), (0x13, 0x7F7F000F)):
+    for junk in ((0, 0), (0xFF, 0x7FC0000F), (0xA5, 0x7F800003), (0x13, 0x7F7F000F), (0x77, -1), (0x77, 0x7FFFFFFF)):
         b = Batch(lens, 2, 64, 16, junk=junk)
         outs.append(kv4.attention(q, b.cache, b.d_table, b.d_lens, _i32(ptr), return_lse=True))
     for o, l in outs[1:]:
