@@ -7,6 +7,7 @@
 #include "../../include/taccel_b200.h"
 #include "tac_kv4.cuh"
 #include "tac_kv4_rows.cuh"
+#include "tac_kv4_tc.cuh"
 
 namespace tac {
 int* gemm_fault_word();
@@ -248,6 +249,29 @@ int launch_rows(Kv4RowsParams p, void* workspace, cudaStream_t st) {
   return cudaLaunchKernelEx(&cfg, kv4_join_kernel<D, NT>, p) == cudaSuccess ? TAC_OK : TAC_E_CUDA;
 }
 
+// Prompt chunks: 256 rows a CTA, from 32 rows a sequence and key-value head on.
+bool use_tc(int batch, int total, int group) { return int64_t(total) * group > int64_t(32) * batch; }
+
+template <int D, bool BF16>
+int launch_tc(const Kv4RowsParams& r, cudaStream_t st) {
+  static bool smem_set[64] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return TAC_E_CUDA;
+  if (!smem_set[dev]) {
+    if (cudaFuncSetAttribute(kv4_tc_kernel<D, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, tc_smem(D)) != cudaSuccess)
+      return TAC_E_CUDA;
+    smem_set[dev] = true;
+  }
+  Kv4TcParams p{};
+  p.r = r;
+  p.fault = gemm_fault_word();
+  if (!p.fault) return TAC_E_CUDA;
+  p.blocks = int((int64_t(r.s.total) * r.group + kTcRows - 1) / kTcRows) + r.s.batch;
+  if (int64_t(p.blocks) * r.c.heads > (int64_t(1) << 31) - 1) return TAC_E_ARGUMENT;
+  kv4_tc_kernel<D, BF16><<<p.blocks * r.c.heads, kTcThreads, tc_smem(D), st>>>(p);
+  return status();
+}
+
 }  // namespace
 
 extern "C" int tac_kv4_append(const tac_kv4_cache* cache, const int32_t* page_table, const int32_t* lens,
@@ -323,6 +347,10 @@ extern "C" int tac_kv4_attention(const tac_kv4_cache* cache, const int32_t* page
   p.q_vec = aligned(Q, 16) && (q_tok | q_head) % 8 == 0;
   if (sm_count() <= 0) return TAC_E_CUDA;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (use_tc(batch, total, p.group)) {
+    if (cache->head_dim == 64) return p.bf16 ? launch_tc<64, true>(p, st) : launch_tc<64, false>(p, st);
+    return p.bf16 ? launch_tc<128, true>(p, st) : launch_tc<128, false>(p, st);
+  }
   const int nt = rows_tiles(batch, total, p.group);
   if (cache->head_dim == 64) return nt == 1 ? launch_rows<64, 1>(p, workspace, st) : launch_rows<64, 2>(p, workspace, st);
   return nt == 1 ? launch_rows<128, 1>(p, workspace, st) : launch_rows<128, 2>(p, workspace, st);

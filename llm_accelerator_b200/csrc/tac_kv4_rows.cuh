@@ -124,7 +124,7 @@ __device__ __forceinline__ SeqCost seq_cost(const Kv4RowsParams& p, const Kv4Seq
 // `total` cut into `parts` shares, the first `rem` of them one larger.
 struct Cuts {
   uint32_t total, parts, base, rem;
-  __device__ Cuts() = default;
+  Cuts() = default;
   __device__ Cuts(uint32_t total, uint32_t grid) : total(total), parts(min(total, grid)) {
     base = parts ? total / parts : 0;
     rem = total - base * parts;

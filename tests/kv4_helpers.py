@@ -87,7 +87,9 @@ def reference(batch, q, indptr=None, causal=True, scale=None, half=False):
     numbers, and D products are added in float32 (at most 2 D 2^-24 of their magnitudes' sum, were each addition cut
     off); two float32 factors follow.  exp2 is good to 2^-21.  A weight p s' is rounded once to FP16: 2^-11 of it, or
     2^-25 of the unit that brings the largest s' into [1, 2).  Output sums run in float32 over n tokens.
-    half: weights p and values v are rounded to the output's type, each by half a step (prompt chunks)."""
+    half: weights p and values v are rounded to the output's type, each by half a step (prompt chunks).  A value below
+    the smallest normal number is then off by up to half a subnormal step, and since the weights of a row sum to one,
+    so is the row's result: |sum p (v + e)| - |sum p v| <= sum p |e| <= max |e|."""
     lens, D = batch.lens, batch.D
     q = q.cpu()
     total, hq, _ = q.shape
@@ -129,7 +131,8 @@ def reference(batch, q, indptr=None, causal=True, scale=None, half=False):
             ids = batch.table[b][(batch.table[b] >= 0) & (batch.table[b] < batch.pages)].long()
             big = torch.nan_to_num(vs[ids], nan=0.0).max() if n and ok.any() else 0.0
             tol[a:e, h * group:(h + 1) * group] = rel * (p @ Vc.abs() if n else 0.0) + n * 2.0 ** -24 * 15 * float(big)
-    tol = tol + step * out.abs() * (1 + step) + 2.0 ** (-25 if q.dtype == torch.float16 else -134)
+    tiny = 2.0 ** (-25 if q.dtype == torch.float16 else -134)       # half a subnormal step
+    tol = tol + step * out.abs() * (1 + step) + tiny + (tiny if half else 0)
     return out, lse, tol
 
 
