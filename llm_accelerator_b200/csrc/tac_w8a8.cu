@@ -96,13 +96,14 @@ bool map_rows(CUtensorMap* m, const int8_t* base, int K, int rows, int box_rows)
 
 constexpr int kSkMaxSmem = 200 * 1024;
 
+template <int YT>
 int launch_splitk(const int8_t* A, const int8_t* Bt, W8Params p, cudaStream_t st) {
   static bool smem_set[64] = {};
   int dev = 0;
   const int sms = sm_count();
   if (!sms || cudaGetDevice(&dev) != cudaSuccess) return TAC_E_CUDA;
   if (!smem_set[dev]) {
-    if (cudaFuncSetAttribute(w8_splitk_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSkMaxSmem) != cudaSuccess)
+    if (cudaFuncSetAttribute(w8_splitk_kernel<YT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSkMaxSmem) != cudaSuccess)
       return TAC_E_CUDA;
     smem_set[dev] = true;
   }
@@ -128,7 +129,60 @@ int launch_splitk(const int8_t* A, const int8_t* Bt, W8Params p, cudaStream_t st
   attr[0].val.clusterDim.z = split;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, w8_splitk_kernel, tw, ta, p) == cudaSuccess ? TAC_OK : TAC_E_CUDA;
+  return cudaLaunchKernelEx(&cfg, w8_splitk_kernel<YT>, tw, ta, p) == cudaSuccess ? TAC_OK : TAC_E_CUDA;
+}
+
+// Tokens of a pair tile: the multiple of 32 that leaves the least work on the
+// fullest pair, a tile's time going with its tokens plus a constant share for
+// filling 256 channels of weights.
+int pair_tokens(int M, int N, int clusters, int* waves) {
+  const int64_t wt = (N + 255) / 256;
+  int best = 0;
+  double cost = 0;
+  for (int tn = 256; tn >= 64; tn -= 32) {
+    const int64_t tiles = wt * ((M + tn - 1) / tn);
+    const double c = double((tiles + clusters - 1) / clusters) * (tn + 32);
+    if (!best || c < cost) best = tn, cost = c, *waves = int((tiles + clusters - 1) / clusters);
+  }
+  return best;
+}
+
+// Largest number of CTA pairs that run at once; 0 where none does.
+template <int YT>
+int pair_clusters(int dev) {
+  static int clusters[64];
+  static bool done[64] = {};
+  if (!done[dev]) {
+    int n = 0;
+    const int sms = sm_count();
+    if (cudaFuncSetAttribute(w8_pair_kernel<YT>, cudaFuncAttributeMaxDynamicSharedMemorySize, PairCfg::kSmem) == cudaSuccess) {
+      cudaLaunchConfig_t cfg = {};
+      cfg.gridDim = dim3(2 * (sms / 2));
+      cfg.blockDim = dim3(PairCfg::kThreads);
+      cfg.dynamicSmemBytes = PairCfg::kSmem;
+      if (cudaOccupancyMaxActiveClusters(&n, w8_pair_kernel<YT>, &cfg) != cudaSuccess) n = 0;
+    }
+    cudaGetLastError();
+    clusters[dev] = std::min(n, sms / 2);
+    done[dev] = true;
+  }
+  return clusters[dev];
+}
+
+template <int YT>
+int launch_pair(const int8_t* A, const int8_t* Bt, W8Params p, int clusters, int tn, cudaStream_t st) {
+  W8PairParams pp{};
+  p.tn = tn;
+  p.k_blocks = (p.K + 127) / 128;
+  pp.g = p;
+  pp.w_tiles = (p.N + 255) / 256;
+  pp.t_tiles = (p.M + tn - 1) / tn;
+  CUtensorMap tw, ta;
+  if (!map_rows(&tw, Bt, p.K, p.N, 128) || !map_rows(&ta, A, p.K, p.M, tn / 2)) return TAC_E_CUDA;
+  const int64_t tiles = int64_t(pp.w_tiles) * pp.t_tiles;
+  if (tiles > (1 << 30)) return TAC_E_ARGUMENT;
+  w8_pair_kernel<YT><<<2 * int(std::min<int64_t>(tiles, clusters)), PairCfg::kThreads, PairCfg::kSmem, st>>>(tw, ta, pp);
+  return status();
 }
 
 // Checks that both products share; also the limits of 32-bit sums and of the grid.
@@ -138,6 +192,18 @@ int check_product(const void* Bt, const void* b_scale, int b_type, const void* b
   if ((b_type != TAC_F32 && b_type != TAC_F16) || !type_ok(y_type) || (bias && !type_ok(bias_type))) return TAC_E_ARGUMENT;
   if (K >= (1 << 17) || M > (1 << 20) || !aligned(Bt, 16)) return TAC_E_ARGUMENT;   // |sum| <= K * 128^2 < 2^31
   return TAC_OK;
+}
+
+template <int YT>
+int pick_product(const int8_t* A, const int8_t* Bt, const W8Params& p, cudaStream_t st) {
+  int dev = 0, waves = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return TAC_E_CUDA;
+  const int clusters = pair_clusters<YT>(dev);
+  if (p.M > 128 && clusters > 0) {
+    const int tn = pair_tokens(p.M, p.N, clusters, &waves);
+    if (int64_t((p.N + 255) / 256) * ((p.M + tn - 1) / tn) * 2 >= clusters) return launch_pair<YT>(A, Bt, p, clusters, tn, st);
+  }
+  return launch_splitk<YT>(A, Bt, p, st);
 }
 
 int run_product(const int8_t* A, const int8_t* Bt, const float* a_scale, const void* b_scale, int b_type,
@@ -155,7 +221,7 @@ int run_product(const int8_t* A, const int8_t* Bt, const float* a_scale, const v
   p.K = K;
   p.fault = gemm_fault_word();
   if (!p.fault) return TAC_E_CUDA;
-  return launch_splitk(A, Bt, p, st);
+  return y_type == TAC_F32 ? pick_product<0>(A, Bt, p, st) : y_type == TAC_F16 ? pick_product<1>(A, Bt, p, st) : pick_product<2>(A, Bt, p, st);
 }
 
 uint64_t align256(uint64_t v) { return (v + 255) & ~uint64_t(255); }

@@ -27,9 +27,10 @@ __device__ __forceinline__ float ld_any(const void* p, int type, int64_t i) {
   return type == 1 ? __half2float(__ushort_as_half(b)) : __uint_as_float(uint32_t(b) << 16);
 }
 
-__device__ __forceinline__ void st_any(void* p, int type, int64_t i, float v) {
-  if (type == 0) static_cast<float*>(p)[i] = v;
-  else if (type == 1) static_cast<__half*>(p)[i] = __float2half_rn(v);
+template <int YT>
+__device__ __forceinline__ void st_y(void* p, int64_t i, float v) {
+  if constexpr (YT == 0) static_cast<float*>(p)[i] = v;
+  else if constexpr (YT == 1) static_cast<__half*>(p)[i] = __float2half_rn(v);
   else static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
 }
 
@@ -46,9 +47,73 @@ struct W8Params {
   int* fault;
 };
 
-__device__ __forceinline__ float w8_value(int acc, float as, float bs, float bias, bool has_bias) {
-  const float y = __fmul_rn(__fmul_rn(__int2float_rn(acc), as), bs);
-  return has_bias ? __fadd_rn(y, bias) : y;
+__device__ __forceinline__ float w8_value(int acc, float as, float bs, float bias) {
+  return fmaf(__fmul_rn(__int2float_rn(acc), as), bs, bias);   // bias 0 where there is none
+}
+
+// 32 tokens (m .. m + 31) of a warp's 32 consecutive channels (n its own):
+// v the sums, as their scales (shared memory, 16-byte aligned).  A thread has
+// one channel, so 16-bit results are exchanged with the next lane and stored
+// in pairs: of two tokens, the even lanes store one's pairs and the odd lanes
+// the other's.  Where N is odd every second row begins between two words; its
+// pairs are those of an odd lane and the next, its first and last channel go
+// alone.  (Four warps with an element's own 16-bit store and 30 instructions
+// each took 91 us at 4096^3, the MMAs 34.)
+template <int YT>
+__device__ __forceinline__ void w8_store32(const W8Params& p, const uint32_t (&v)[32], const float* as, int m, int n,
+                                           float bs, float bias) {
+  const int lane = threadIdx.x & 31, n_warp = n - lane;
+  const bool inside = m + 32 <= p.M && n_warp + 32 <= p.N;
+  const uint32_t base_odd = uint32_t(reinterpret_cast<uintptr_t>(p.y) >> 1) & 1;
+  if (YT == 0 && inside) {
+    float* dst = static_cast<float*>(p.y) + int64_t(m) * p.N + n;
+#pragma unroll
+    for (int j = 0; j < 32; j += 4) {
+      const float4 a = *reinterpret_cast<const float4*>(as + j);
+      const float aa[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i, dst += p.N) *dst = w8_value(int(v[j + i]), aa[i], bs, bias);
+    }
+  } else if (YT != 0 && inside && ((p.N & 1) || !base_odd)) {
+    // the token of a pair whose row is word-aligned at an even channel: the first one, or with an odd N that of that parity
+    const bool odd_n = p.N & 1;
+    const uint32_t first = odd_n ? (base_odd ^ uint32_t(m & 1)) : 0u;   // n_warp is even
+    const bool mine_first = (lane & 1) == 0;                            // even lanes store the aligned token
+    const int tok = mine_first ? int(first) : int(first ^ 1u);
+    uint16_t* dst = static_cast<uint16_t*>(p.y) + int64_t(m + tok) * p.N + n - (mine_first || odd_n ? 0 : 1);
+    uint16_t* edge = static_cast<uint16_t*>(p.y) + int64_t(m + int(first ^ 1u)) * p.N + n;
+    const int64_t step = 2 * int64_t(p.N);
+#pragma unroll
+    for (int j = 0; j < 32; j += 4) {
+      const float4 a = *reinterpret_cast<const float4*>(as + j);
+      const float aa[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+      for (int i = 0; i < 4; i += 2, dst += step, edge += step) {
+        const float y0 = w8_value(int(v[j + i]), aa[i], bs, bias), y1 = w8_value(int(v[j + i + 1]), aa[i + 1], bs, bias);
+        uint32_t mine;               // the first token's result low, the second's high
+        if constexpr (YT == 1) {
+          const __half2 h = __floats2half2_rn(y0, y1);
+          mine = *reinterpret_cast<const uint32_t*>(&h);
+        } else {
+          const __nv_bfloat162 h = __floats2bfloat162_rn(y0, y1);
+          mine = *reinterpret_cast<const uint32_t*>(&h);
+        }
+        if (!odd_n) {
+          const uint32_t other = __shfl_xor_sync(0xffffffffu, mine, 1);
+          *reinterpret_cast<uint32_t*>(dst) = mine_first ? __byte_perm(mine, other, 0x5410) : __byte_perm(other, mine, 0x7632);
+        } else {
+          const uint32_t other = __shfl_down_sync(0xffffffffu, mine, 1);
+          const uint32_t sel = tok ? 0x7632 : 0x5410;
+          if (lane != 31) *reinterpret_cast<uint32_t*>(dst) = __byte_perm(mine, other, sel);
+          if (lane == 0 || lane == 31) *edge = uint16_t(first ? mine : mine >> 16);
+        }
+      }
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 32; ++j)
+      if (m + j < p.M && n < p.N) st_y<YT>(p.y, int64_t(m + j) * p.N + n, w8_value(int(v[j]), as[j], bs, bias));
+  }
 }
 
 // ---- split-K over a cluster -----------------------------------------------------------------------------------------
@@ -63,6 +128,7 @@ constexpr int kSkWBytes = 128 * 128;
 
 __host__ __device__ constexpr int sk_stage_bytes(int tn) { return kSkWBytes + tn * 128; }
 
+template <int YT>
 __global__ void __launch_bounds__(kSkThreads)
     w8_splitk_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_a, W8Params p) {
   constexpr int kMaxStages = 8;
@@ -70,7 +136,7 @@ __global__ void __launch_bounds__(kSkThreads)
   __shared__ __align__(8) uint64_t full_bar[kMaxStages], empty_bar[kMaxStages], acc_bar;
   __shared__ uint32_t tmem_base;
   __shared__ int abort_flag;
-  __shared__ float as_s[256];
+  __shared__ __align__(16) float as_s[256];
 
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(dyn_smem) + 1023) & ~uintptr_t(1023));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -143,12 +209,11 @@ __global__ void __launch_bounds__(kSkThreads)
   const int row = (warp & 3) * 32 + lane;     // TMEM lane = channel of the tile (warps 2..5)
   const int n = n0 + row;
   float bs = 0.f, bias = 0.f;
-  const bool has_bias = p.bias != nullptr;
   bool acc_ok = false;
   if (warp >= 2) {
     if (n < p.N) {
       bs = ld_any(p.b_scale, p.b_type, n);
-      if (has_bias) bias = ld_any(p.bias, p.bias_type, n);
+      if (p.bias) bias = ld_any(p.bias, p.bias_type, n);
     }
     for (int i = threadIdx.x - 64; i < p.tn; i += 128) as_s[i] = m0 + i < p.M ? __ldg(p.a_scale + m0 + i) : 0.f;
     asm volatile("bar.sync 1, 128;\n" ::: "memory");   // as_s, among the epilogue's warps
@@ -163,12 +228,8 @@ __global__ void __launch_bounds__(kSkThreads)
         uint32_t v[32];
         __syncwarp();
         sm100::tmem_ld32(t_addr + c, v);
-#pragma unroll
-        for (int j = 0; j < 32; ++j) {
-          const int m = m0 + c + j;
-          if (c + j < p.tn && m < p.M && n < p.N)
-            st_any(p.y, p.y_type, int64_t(m) * p.N + n, w8_value(int(v[j]), as_s[c + j], bs, bias, has_bias));
-        }
+        // a tile of 16 tokens has no more than 16 rows before M
+        w8_store32<YT>(p, v, as_s + c, m0 + c, n, bs, bias);
       }
     }
   } else {
@@ -194,7 +255,7 @@ __global__ void __launch_bounds__(kSkThreads)
           asm volatile("ld.shared::cluster.s32 %0, [%1];\n" : "=r"(v) : "r"(sm100::mapa_shared(part + c * 128 + row, r)));
           acc += v;
         }
-        if (n < p.N) st_any(p.y, p.y_type, int64_t(m) * p.N + n, w8_value(acc, as_s[c], bs, bias, has_bias));
+        if (n < p.N) st_y<YT>(p.y, int64_t(m) * p.N + n, w8_value(acc, as_s[c], bs, bias));
       }
     }
     sm100::cluster_sync();   // no CTA leaves while another reads its partial sums
@@ -205,6 +266,170 @@ __global__ void __launch_bounds__(kSkThreads)
     __syncwarp();
     sm100::tc_fence_after();
     sm100::tmem_dealloc(tmem, cols);
+  }
+}
+
+// ---- CTA pairs ------------------------------------------------------------------------------------------------------
+// 256 channels x tn tokens a pair of CTAs (cta_group::2): each CTA stages 128
+// channels of the weights and half of the tokens, 32 KB a 128-byte K block at
+// most, and gets its 128 channels of the result in its own TMEM.  Persistent,
+// two accumulators, the last tile's epilogue under the next one's MMAs.  Roles
+// and waits as in tac_gemm_tc2.cuh; no load uses multicast.
+struct PairCfg {
+  static constexpr int kStages = 6;
+  static constexpr int kStageBytes = 2 * 16384;
+  static constexpr int kSmem = kStages * kStageBytes + 1024;
+  static constexpr int kEpi = 256;     // epilogue threads: two warps a quadrant of TMEM, half of the tokens each
+  static constexpr int kThreads = 64 + kEpi;
+};
+
+struct W8PairParams {
+  W8Params g;
+  int w_tiles, t_tiles;      // 256-channel tiles, token tiles
+};
+
+template <int YT>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg::kThreads, 1)
+    w8_pair_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_a, W8PairParams pp) {
+  constexpr int S = PairCfg::kStages;
+  const W8Params& p = pp.g;
+  extern __shared__ uint8_t dyn_smem[];
+  __shared__ __align__(8) uint64_t full_bar[S], empty_bar[S], acc_full[2], acc_empty[2], drain_bar;
+  __shared__ uint32_t tmem_base;
+  __shared__ int abort_flag;
+  __shared__ __align__(16) float as_s[2][256];
+
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(dyn_smem) + 1023) & ~uintptr_t(1023));
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = sm100::cluster_ctarank();
+  const int cid = blockIdx.x >> 1, ncl = gridDim.x >> 1;
+  const int half = p.tn / 2, total = pp.w_tiles * pp.t_tiles;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S; ++s) {
+      sm100::mbar_init(&full_bar[s], 1);
+      sm100::mbar_init(&empty_bar[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      sm100::mbar_init(&acc_full[b], 1);
+      sm100::mbar_init(&acc_empty[b], 2 * PairCfg::kEpi / 32);   // the epilogue warps of both CTAs
+    }
+    sm100::mbar_init(&drain_bar, 1);
+    abort_flag = 0;
+    sm100::mbar_fence_init();
+  }
+  if (warp == 1) sm100::tmem_alloc_pair(&tmem_base, 512);
+  sm100::tc_fence_before();
+  sm100::cluster_sync();   // barriers and TMEM of both CTAs exist before any remote use
+  sm100::tc_fence_after();
+  const uint32_t tmem = tmem_base;
+  volatile int* abort_v = &abort_flag;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      uint32_t it = 0;
+      for (int tile = cid; tile < total && !*abort_v; tile += ncl) {
+        const int n0 = tile / pp.t_tiles * 256 + int(rank) * 128, m0 = tile % pp.t_tiles * p.tn + int(rank) * half;
+        for (int kb = 0; kb < p.k_blocks; ++kb, ++it) {
+          const uint32_t s = it % S, ph = (it / S) & 1;
+          if (!sm100::mbar_wait(&empty_bar[s], ph ^ 1, p.fault, W8_TIMEOUT_EMPTY) || *abort_v) {
+            *abort_v = 1;
+            break;
+          }
+          if (rank == 0) sm100::mbar_arrive_expect_tx(&full_bar[s], 2 * (16384 + half * 128));
+          const uint32_t bar0 = sm100::mapa_shared(&full_bar[s], 0);
+          uint8_t* st = smem + s * PairCfg::kStageBytes;
+          sm100::tma_load_2d_pair(st, &tm_w, kb * 128, n0, bar0);
+          sm100::tma_load_2d_pair(st + 16384, &tm_a, kb * 128, m0, bar0);
+        }
+        if (*abort_v) break;
+      }
+      if (rank == 0) {
+        // both CTAs' copies of the stages still in flight land on these barriers
+        const uint32_t first = it > uint32_t(S) ? it - S : 0;
+        for (uint32_t j = first; j < it; ++j)
+          sm100::mbar_wait(&full_bar[j % S], (j / S) & 1, p.fault, W8_TIMEOUT_DRAIN);
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      if (rank == 0) {
+        const uint32_t idesc = sm100::idesc_i8(256, p.tn, 0);
+        uint32_t it = 0, local = 0;
+        for (int tile = cid; tile < total && !*abort_v; tile += ncl, ++local) {
+          const uint32_t b = local & 1, aph = (local >> 1) & 1;
+          if (!sm100::mbar_wait(&acc_empty[b], aph ^ 1, p.fault, W8_TIMEOUT_ACC)) {
+            *abort_v = 1;
+            break;
+          }
+          sm100::tc_fence_after();
+          bool ok = true;
+          for (int kb = 0; kb < p.k_blocks; ++kb, ++it) {
+            const uint32_t s = it % S, ph = (it / S) & 1;
+            if (!sm100::mbar_wait(&full_bar[s], ph, p.fault, W8_TIMEOUT_FULL) || *abort_v) {
+              *abort_v = 1;
+              ok = false;
+              break;
+            }
+            sm100::tc_fence_after();
+            const uint32_t w_addr = sm100::smem_u32(smem + s * PairCfg::kStageBytes);
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              sm100::mma_i8_pair(tmem + b * 256, sm100::smem_desc_sw128(w_addr + k * 32, 16, 1024),
+                                 sm100::smem_desc_sw128(w_addr + 16384 + k * 32, 16, 1024), idesc, (kb | k) != 0);
+            sm100::mma_commit_pair(&empty_bar[s], 0x3);
+          }
+          if (!ok) break;
+          sm100::mma_commit_pair(&acc_full[b], 0x3);
+        }
+        // every MMA issued must finish before either CTA releases TMEM
+        sm100::mma_commit_pair(&drain_bar, 0x3);
+      }
+      sm100::mbar_wait(&drain_bar, 0, p.fault, W8_TIMEOUT_DRAIN);
+    }
+  } else {
+    const int row = (warp & 3) * 32 + lane;
+    const uint32_t acc_empty0_0 = sm100::mapa_shared(&acc_empty[0], 0), acc_empty0_1 = sm100::mapa_shared(&acc_empty[1], 0);
+    const int part = (warp - 2) >> 2;
+    uint32_t local = 0;
+    for (int tile = cid; tile < total; tile += ncl, ++local) {
+      const uint32_t b = local & 1, aph = (local >> 1) & 1;
+      const int n = tile / pp.t_tiles * 256 + int(rank) * 128 + row, m0 = tile % pp.t_tiles * p.tn;
+      float bs = 0.f, bias = 0.f;
+      if (n < p.N) {
+        bs = ld_any(p.b_scale, p.b_type, n);
+        if (p.bias) bias = ld_any(p.bias, p.bias_type, n);
+      }
+      for (int i = threadIdx.x - 64; i < p.tn; i += PairCfg::kEpi) as_s[b][i] = m0 + i < p.M ? __ldg(p.a_scale + m0 + i) : 0.f;
+      asm volatile("bar.sync 1, %0;\n" ::"n"(PairCfg::kEpi) : "memory");   // as_s[b]: its readers two tiles ago are past the last one
+      if (*abort_v) break;
+      if (!sm100::mbar_wait(&acc_full[b], aph, p.fault, W8_TIMEOUT_ACC)) {
+        *abort_v = 1;
+        break;
+      }
+      __syncwarp();
+      sm100::tc_fence_after();
+#pragma unroll 1
+      for (int c = part * 32; c < p.tn; c += 64) {
+        if (m0 + c >= p.M) break;
+        uint32_t v[32];
+        __syncwarp();
+        sm100::tmem_ld32(tmem + (uint32_t((warp & 3) * 32) << 16) + b * 256 + c, v);
+        w8_store32<YT>(p, v, as_s[b] + c, m0 + c, n, bs, bias);
+      }
+      sm100::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) sm100::mbar_arrive_remote(b ? acc_empty0_1 : acc_empty0_0);
+    }
+  }
+
+  sm100::tc_fence_before();
+  __syncwarp();
+  sm100::cluster_sync();   // no CTA leaves while its peer may still touch its shared memory or TMEM
+  if (warp == 1) {
+    __syncwarp();
+    sm100::tc_fence_after();
+    sm100::tmem_dealloc_pair(tmem, 512);
   }
 }
 
