@@ -300,7 +300,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg::kThreads, 1
   __shared__ __align__(16) float as_s[2][256];
 
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(dyn_smem) + 1023) & ~uintptr_t(1023));
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const uint32_t rank = sm100::cluster_ctarank();
   const int cid = blockIdx.x >> 1, ncl = gridDim.x >> 1;
   const int half = p.tn / 2, total = pp.w_tiles * pp.t_tiles;
@@ -326,67 +326,70 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg::kThreads, 1
   volatile int* abort_v = &abort_flag;
 
   if (warp == 0) {
-    if (lane == 0) {
-      uint32_t it = 0;
-      for (int tile = cid; tile < total && !*abort_v; tile += ncl) {
-        const int n0 = tile / pp.t_tiles * 256 + int(rank) * 128, m0 = tile % pp.t_tiles * p.tn + int(rank) * half;
-        for (int kb = 0; kb < p.k_blocks; ++kb, ++it) {
-          const uint32_t s = it % S, ph = (it / S) & 1;
-          if (!sm100::mbar_wait(&empty_bar[s], ph ^ 1, p.fault, W8_TIMEOUT_EMPTY) || *abort_v) {
-            *abort_v = 1;
-            break;
-          }
+    uint32_t s = 0, ph = 1, issued = 0;
+    for (int tile = cid; tile < total && !*abort_v; tile += ncl) {
+      const int n0 = tile / pp.t_tiles * 256 + int(rank) * 128, m0 = tile % pp.t_tiles * p.tn + int(rank) * half;
+      for (int kb = 0; kb < p.k_blocks; ++kb) {
+        if (!sm100::mbar_wait(&empty_bar[s], ph, p.fault, W8_TIMEOUT_EMPTY) || *abort_v) {
+          *abort_v = 1;
+          break;
+        }
+        if (sm100::elect_one()) {
           if (rank == 0) sm100::mbar_arrive_expect_tx(&full_bar[s], 2 * (16384 + half * 128));
           const uint32_t bar0 = sm100::mapa_shared(&full_bar[s], 0);
           uint8_t* st = smem + s * PairCfg::kStageBytes;
           sm100::tma_load_2d_pair(st, &tm_w, kb * 128, n0, bar0);
           sm100::tma_load_2d_pair(st + 16384, &tm_a, kb * 128, m0, bar0);
         }
-        if (*abort_v) break;
-      }
-      if (rank == 0) {
-        // both CTAs' copies of the stages still in flight land on these barriers
-        const uint32_t first = it > uint32_t(S) ? it - S : 0;
-        for (uint32_t j = first; j < it; ++j)
-          sm100::mbar_wait(&full_bar[j % S], (j / S) & 1, p.fault, W8_TIMEOUT_DRAIN);
+        __syncwarp();
+        ++issued;
+        if (++s == S) s = 0, ph ^= 1;
       }
     }
+    if (rank == 0) {
+      // both CTAs' copies of the stages still in flight land on these barriers
+      for (uint32_t j = issued > uint32_t(S) ? issued - S : 0; j < issued; ++j)
+        sm100::mbar_wait(&full_bar[j % S], (j / S) & 1, p.fault, W8_TIMEOUT_DRAIN);
+    }
   } else if (warp == 1) {
-    if (lane == 0) {
-      if (rank == 0) {
-        const uint32_t idesc = sm100::idesc_i8(256, p.tn, 0);
-        uint32_t it = 0, local = 0;
-        for (int tile = cid; tile < total && !*abort_v; tile += ncl, ++local) {
-          const uint32_t b = local & 1, aph = (local >> 1) & 1;
-          if (!sm100::mbar_wait(&acc_empty[b], aph ^ 1, p.fault, W8_TIMEOUT_ACC)) {
+    if (rank == 0) {
+      const uint32_t idesc = sm100::idesc_i8(256, p.tn, 0);
+      const uint64_t w0 = sm100::smem_desc_sw128(sm100::smem_u32(smem), 16, 1024);
+      uint32_t s = 0, ph = 0, local = 0;
+      for (int tile = cid; tile < total && !*abort_v; tile += ncl, ++local) {
+        const uint32_t b = local & 1, aph = (local >> 1) & 1;
+        if (!sm100::mbar_wait(&acc_empty[b], aph ^ 1, p.fault, W8_TIMEOUT_ACC)) {
+          *abort_v = 1;
+          break;
+        }
+        sm100::tc_fence_after();
+        bool ok = true;
+        for (int kb = 0; kb < p.k_blocks; ++kb) {
+          if (!sm100::mbar_wait(&full_bar[s], ph, p.fault, W8_TIMEOUT_FULL) || *abort_v) {
             *abort_v = 1;
+            ok = false;
             break;
           }
           sm100::tc_fence_after();
-          bool ok = true;
-          for (int kb = 0; kb < p.k_blocks; ++kb, ++it) {
-            const uint32_t s = it % S, ph = (it / S) & 1;
-            if (!sm100::mbar_wait(&full_bar[s], ph, p.fault, W8_TIMEOUT_FULL) || *abort_v) {
-              *abort_v = 1;
-              ok = false;
-              break;
-            }
-            sm100::tc_fence_after();
-            const uint32_t w_addr = sm100::smem_u32(smem + s * PairCfg::kStageBytes);
+          const uint64_t dw = w0 + s * (PairCfg::kStageBytes >> 4);
+          if (sm100::elect_one()) {
 #pragma unroll
             for (int k = 0; k < 4; ++k)
-              sm100::mma_i8_pair(tmem + b * 256, sm100::smem_desc_sw128(w_addr + k * 32, 16, 1024),
-                                 sm100::smem_desc_sw128(w_addr + 16384 + k * 32, 16, 1024), idesc, (kb | k) != 0);
+              sm100::mma_i8_pair(tmem + b * 256, dw + 2 * k, dw + (16384 >> 4) + 2 * k, idesc, (kb | k) != 0);
             sm100::mma_commit_pair(&empty_bar[s], 0x3);
           }
-          if (!ok) break;
-          sm100::mma_commit_pair(&acc_full[b], 0x3);
+          __syncwarp();
+          if (++s == S) s = 0, ph ^= 1;
         }
-        // every MMA issued must finish before either CTA releases TMEM
-        sm100::mma_commit_pair(&drain_bar, 0x3);
+        if (!ok) break;
+        if (sm100::elect_one()) sm100::mma_commit_pair(&acc_full[b], 0x3);
+        __syncwarp();
       }
-      sm100::mbar_wait(&drain_bar, 0, p.fault, W8_TIMEOUT_DRAIN);
+      // every MMA issued must finish before either CTA releases TMEM
+      if (sm100::elect_one()) sm100::mma_commit_pair(&drain_bar, 0x3);
+      __syncwarp();
     }
+    sm100::mbar_wait(&drain_bar, 0, p.fault, W8_TIMEOUT_DRAIN);
   } else {
     const int row = (warp & 3) * 32 + lane;
     const uint32_t acc_empty0_0 = sm100::mapa_shared(&acc_empty[0], 0), acc_empty0_1 = sm100::mapa_shared(&acc_empty[1], 0);
