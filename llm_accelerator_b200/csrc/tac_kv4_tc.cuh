@@ -138,7 +138,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv4_tc_kernel(Kv4TcParams pp) {
   __shared__ __align__(16) float ks_s[4][kTcKeys];
   __shared__ uint32_t present_s[4][4];
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   // ---- this CTA's rows: later row blocks, which see more keys, come first ----
   const int h = blockIdx.x % p.c.heads;
   int blk = pp.blocks - 1 - int(blockIdx.x / p.c.heads), b = 0;
@@ -197,44 +197,53 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv4_tc_kernel(Kv4TcParams pp) {
 
   if (warp == 12) {
     // ---- MMA issue ----
-    if (lane == 0 && tiles) {
+    // The whole warp runs these loops and one elected lane issues, so that descriptors stay in uniform registers.
+    if (tiles) {
       constexpr uint32_t kIdS = tc_idesc(kTcKeys, false, false), kIdO = tc_idesc(D, BF16, true);
-      const uint32_t qa = sm100::smem_u32(q_sm), ka = sm100::smem_u32(k_sm), va = sm100::smem_u32(v_sm);
+      // K-major rows of 128 bytes (64 values), blocks of 64 values 16 KB apart
+      const uint64_t qd = sm100::smem_desc_sw128(sm100::smem_u32(q_sm), 16, 1024), kd = sm100::smem_desc_sw128(sm100::smem_u32(k_sm), 16, 1024);
+      // MN-major: a key's 64 values a row of 128 bytes, 8 keys 1024 bytes, blocks of 64 values 16 KB apart
+      const uint64_t vd = sm100::smem_desc_sw128(sm100::smem_u32(v_sm), kTcKeys * 128, 1024);
       auto qk = [&](int i, int g) {
-        if (*abort_v) return;
+        const uint64_t qg = qd + g * (kTile >> 4), ki = kd + (i & 1) * (kTile >> 4);
+        if (!*abort_v && sm100::elect_one()) {
 #pragma unroll
-        for (int k = 0; k < D / 16; ++k) {
-          // K-major rows of 128 bytes (64 values), blocks of 64 values 16 KB apart
-          const uint32_t o = (k >> 2) * (kTcKeys * 128) + (k & 3) * 32;
-          mma_f16_ss(tmem + g * 128, sm100::smem_desc_sw128(qa + g * kTile + o, 16, 1024),
-                     sm100::smem_desc_sw128(ka + (i & 1) * kTile + o, 16, 1024), kIdS, k != 0);
+          for (int k = 0; k < D / 16; ++k) {
+            const uint32_t o = ((k >> 2) * (kTcKeys * 128) + (k & 3) * 32) >> 4;
+            mma_f16_ss(tmem + g * 128, qg + o, ki + o, kIdS, k != 0);
+          }
+          sm100::mma_commit(&s_full[g]);
         }
-        sm100::mma_commit(&s_full[g]);
+        __syncwarp();
+      };
+      auto commit = [&](uint64_t* bar) {
+        if (sm100::elect_one()) sm100::mma_commit(bar);
+        __syncwarp();
       };
       wait(&q_full, 0, KV4_TIMEOUT_TILE);
       wait(&k_full[0], 0, KV4_TIMEOUT_TILE);
       sm100::tc_fence_after();
       for (int g = 0; g < groups; ++g) qk(0, g);
-      sm100::mma_commit(&k_empty[0]);
+      commit(&k_empty[0]);
       for (int i = 0; i < tiles; ++i) {
         wait(&v_full[i & 1], (i >> 1) & 1, KV4_TIMEOUT_TILE);
         if (i + 1 < tiles) wait(&k_full[(i + 1) & 1], ((i + 1) >> 1) & 1, KV4_TIMEOUT_TILE);
+        const uint64_t vi = vd + (i & 1) * (kTile >> 4);
         for (int g = 0; g < groups; ++g) {
           wait(&p_full[g], i & 1, KV4_TIMEOUT_P);
           sm100::tc_fence_after();
-          if (!*abort_v) {
+          if (!*abort_v && sm100::elect_one()) {
 #pragma unroll
             for (int k = 0; k < kTcKeys / 16; ++k)
-              // MN-major: a key's 64 values a row of 128 bytes, 8 keys 1024 bytes, blocks of 64 values 16 KB apart
-              mma_f16_ts(tmem + 256 + g * 128, tmem + g * 128 + k * 8,
-                         sm100::smem_desc_sw128(va + (i & 1) * kTile + k * 2048, kTcKeys * 128, 1024), kIdO, i || k);
+              mma_f16_ts(tmem + 256 + g * 128, tmem + g * 128 + k * 8, vi + k * (2048 >> 4), kIdO, i || k);
           }
+          __syncwarp();
           if (i + 1 < tiles) qk(i + 1, g);
         }
-        sm100::mma_commit(&v_empty[i & 1]);
-        if (i + 1 < tiles) sm100::mma_commit(&k_empty[(i + 1) & 1]);
+        commit(&v_empty[i & 1]);
+        if (i + 1 < tiles) commit(&k_empty[(i + 1) & 1]);
       }
-      sm100::mma_commit(&o_full);                // every MMA has completed, before TMEM is read for the last time and freed
+      commit(&o_full);                           // every MMA has completed, before TMEM is read for the last time and freed
       sm100::mbar_wait(&o_full, 0, pp.fault, KV4_TIMEOUT_DRAIN);
     }
   } else if (warp >= 8) {

@@ -139,7 +139,7 @@ __global__ void __launch_bounds__(kSkThreads)
   __shared__ __align__(16) float as_s[256];
 
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(dyn_smem) + 1023) & ~uintptr_t(1023));
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int n0 = blockIdx.x * 128, m0 = blockIdx.y * p.tn;
   const int nsplit = gridDim.z, rank = blockIdx.z;
   const int kb0 = int(int64_t(p.k_blocks) * rank / nsplit), kb1 = int(int64_t(p.k_blocks) * (rank + 1) / nsplit);
@@ -163,48 +163,49 @@ __global__ void __launch_bounds__(kSkThreads)
   volatile int* abort_v = &abort_flag;
 
   if (warp == 0) {
-    if (lane == 0) {
-      uint32_t it = 0;
-      for (int kb = kb0; kb < kb1; ++kb, ++it) {
-        const uint32_t s = it % S, ph = (it / S) & 1;
-        if (!sm100::mbar_wait(&empty_bar[s], ph ^ 1, p.fault, W8_TIMEOUT_EMPTY) || *abort_v) {
-          *abort_v = 1;
-          break;
-        }
+    uint32_t s = 0, ph = 1, issued = 0;
+    for (int kb = kb0; kb < kb1; ++kb) {
+      if (!sm100::mbar_wait(&empty_bar[s], ph, p.fault, W8_TIMEOUT_EMPTY) || *abort_v) {
+        *abort_v = 1;
+        break;
+      }
+      if (sm100::elect_one()) {
         uint8_t* st = smem + s * stage_bytes;
         sm100::mbar_arrive_expect_tx(&full_bar[s], stage_bytes);
         sm100::tma_load_2d(st, &tm_w, kb * 128, n0, &full_bar[s]);
         sm100::tma_load_2d(st + kSkWBytes, &tm_a, kb * 128, m0, &full_bar[s]);
       }
-      // the copies still in flight land before the CTA goes on
-      const uint32_t first = it > uint32_t(S) ? it - S : 0;
-      for (uint32_t j = first; j < it; ++j)
-        sm100::mbar_wait(&full_bar[j % S], (j / S) & 1, p.fault, W8_TIMEOUT_DRAIN);
+      __syncwarp();
+      ++issued;
+      if (++s == uint32_t(S)) s = 0, ph ^= 1;
     }
-    __syncwarp();
+    // the copies still in flight land before the CTA goes on
+    for (uint32_t j = issued > uint32_t(S) ? issued - S : 0; j < issued; ++j)
+      sm100::mbar_wait(&full_bar[j % S], (j / S) & 1, p.fault, W8_TIMEOUT_DRAIN);
   } else if (warp == 1) {
-    if (lane == 0) {
-      const uint32_t idesc = sm100::idesc_i8(128, p.tn, 0);
-      uint32_t it = 0;
-      for (int kb = kb0; kb < kb1; ++kb, ++it) {
-        const uint32_t s = it % S, ph = (it / S) & 1;
-        if (!sm100::mbar_wait(&full_bar[s], ph, p.fault, W8_TIMEOUT_FULL) || *abort_v) {
-          *abort_v = 1;
-          break;
-        }
-        sm100::tc_fence_after();
-        const uint32_t w_addr = sm100::smem_u32(smem + s * stage_bytes);
+    const uint32_t idesc = sm100::idesc_i8(128, p.tn, 0);
+    const uint64_t w0 = sm100::smem_desc_sw128(sm100::smem_u32(smem), 16, 1024);
+    uint32_t s = 0, ph = 0;
+    for (int kb = kb0; kb < kb1; ++kb) {
+      if (!sm100::mbar_wait(&full_bar[s], ph, p.fault, W8_TIMEOUT_FULL) || *abort_v) {
+        *abort_v = 1;
+        break;
+      }
+      sm100::tc_fence_after();
+      const uint64_t dw = w0 + s * (stage_bytes >> 4);
+      if (sm100::elect_one()) {
 #pragma unroll
         for (int k = 0; k < 4; ++k)
-          sm100::mma_i8(tmem, sm100::smem_desc_sw128(w_addr + k * 32, 16, 1024),
-                        sm100::smem_desc_sw128(w_addr + kSkWBytes + k * 32, 16, 1024), idesc, (kb > kb0) || k);
+          sm100::mma_i8(tmem, dw + 2 * k, dw + (kSkWBytes >> 4) + 2 * k, idesc, (kb > kb0) || k);
         sm100::mma_commit(&empty_bar[s]);
       }
-      // arrives once every MMA has completed, also after a failed wait
-      sm100::mma_commit(&acc_bar);
-      sm100::mbar_wait(&acc_bar, 0, p.fault, W8_TIMEOUT_DRAIN);
+      __syncwarp();
+      if (++s == uint32_t(S)) s = 0, ph ^= 1;
     }
+    // arrives once every MMA has completed, also after a failed wait
+    if (sm100::elect_one()) sm100::mma_commit(&acc_bar);
     __syncwarp();
+    sm100::mbar_wait(&acc_bar, 0, p.fault, W8_TIMEOUT_DRAIN);
   }
   const int row = (warp & 3) * 32 + lane;     // TMEM lane = channel of the tile (warps 2..5)
   const int n = n0 + row;
