@@ -5,10 +5,12 @@
 // query heads of a token side by side, so one unpacking of a key serves them
 // all) and walks the keys up to its last row's position in tiles of 128:
 //   warps 0..3, 4..7  two row groups of 128, a thread a row: Q to shared
-//                     memory, softmax of S out of TMEM, P into TMEM, O out
-//   warps 8..11       unpack the tile's keys and values, a thread a key,
-//                     into the swizzled layouts that the MMAs read
-//   warp 12           issues the MMAs: S = Q C^T (FP16), O += P V
+//                     memory, softmax of S out of TMEM, P into TMEM, O out;
+//                     a group's first warp issues its MMAs,
+//                     S = Q C^T (FP16) and O += P V
+//   warps 8..11       unpack the tile's keys, a thread a key, into the
+//                     swizzled layout that the MMAs read
+//   warps 12..15      unpack its values
 // While one group does its softmax the tensor core works for the other: per
 // tile and group D = 128 needs 1024 tensor clocks, and 1024 clocks of the
 // exponential unit.
@@ -27,7 +29,9 @@ enum Kv4TcFault : int { KV4_TIMEOUT_TILE = 21, KV4_TIMEOUT_S = 22, KV4_TIMEOUT_P
 
 constexpr int kTcKeys = 128;
 constexpr int kTcRows = 256;
-constexpr int kTcThreads = 13 * 32;
+constexpr int kTcThreads = 16 * 32;
+// Registers a thread: 128 at launch, then shared out by warpgroup (rows, rows, keys, values: their sum is 4 * 128).
+constexpr int kTcRegsRows = 184, kTcRegsUnpack = 72;
 
 __host__ __device__ constexpr int tc_tile_bytes(int D) { return kTcKeys * D * 2; }
 // Q of two groups, two K tiles, two V tiles
@@ -64,17 +68,70 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
       : "memory");
 }
 
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
   asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "
-      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};\n" ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]),
-      "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]),
-      "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]),
-      "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]),
-      "r"(taddr)
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n"
+      "tcgen05.wait::ld.sync.aligned;\n"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
       : "memory");
 }
+
+// 32 columns of this thread's lane; the registers may be used after tmem_landed.
+__device__ __forceinline__ void tmem_ld32_start(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+}
+// Names the registers, so that no use of them moves ahead of the wait.
+__device__ __forceinline__ void tmem_landed(uint32_t* r) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;\n"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])::"memory");
+  asm volatile(""
+               : "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
+                 "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])::"memory");
+}
+
+// Two float32 operations an instruction.
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpack2(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+template <int N>
+__device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(N)); }
 
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory"); }
 
@@ -96,10 +153,6 @@ enum TcUnpack { UNPACK_CODES, UNPACK_BF16, UNPACK_F16, UNPACK_F32 };
 
 template <int MODE>
 __device__ __forceinline__ uint32_t tc_finish(__half2 v, float s) {
-  if (MODE == UNPACK_BF16) {
-    const __nv_bfloat162 r = __hmul2(__floats2bfloat162_rn(__low2float(v), __high2float(v)), __float2bfloat162_rn(s));
-    return *reinterpret_cast<const uint32_t*>(&r);
-  }
   if (MODE == UNPACK_F16) return h2_u(__hmul2(v, __float2half2_rn(s)));
   if (MODE == UNPACK_F32) return h2_u(__floats2half2_rn(__low2float(v) * s, __high2float(v) * s));
   return h2_u(v);
@@ -116,6 +169,18 @@ __device__ __forceinline__ void tc_unpack(uint8_t* dst, uint32_t key, const uint
       const int w = 4 * q + j;
       const uint32_t x = x4[j], y = x >> 8;
       uint4 o;
+      if (MODE == UNPACK_BF16) {
+        // a code under the exponent of 128 is 128 + c; less 128 + z it is exact, and the product is rounded once
+        auto b2 = [](uint32_t u) { return *reinterpret_cast<__nv_bfloat162*>(&u); };
+        const __nv_bfloat162 zb = b2(0x43004300u + z * 0x10001u), sb = __float2bfloat162_rn(s);
+        auto value = [&](uint32_t u) {
+          const __nv_bfloat162 r = __hmul2(__hsub2(b2(and_or(u, 0x000f000fu, 0x43004300u)), zb), sb);
+          return *reinterpret_cast<const uint32_t*>(&r);
+        };
+        o = make_uint4(value(x), value(x >> 4), value(y), value(x >> 12));
+        *reinterpret_cast<uint4*>(dst + (w >> 3) * (kTcKeys * 128) + sw128(key, w & 7)) = o;
+        continue;
+      }
       o.x = tc_finish<MODE>(__hsub2(u_h2(and_or(x, 0x000f000fu, 0x64006400u)), zlo), s);
       o.y = tc_finish<MODE>(__hsub2(u_h2(and_or(x, 0x00f000f0u, 0x54005400u)), zhi), s);
       o.z = tc_finish<MODE>(__hsub2(u_h2(and_or(y, 0x000f000fu, 0x64006400u)), zlo), s);
@@ -131,12 +196,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv4_tc_kernel(Kv4TcParams pp) {
   constexpr int W = D / 8;                       // words of codes a key
   constexpr int kTile = tc_tile_bytes(D);
   extern __shared__ uint8_t dyn_smem[];
-  __shared__ __align__(8) uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_full;
+  __shared__ __align__(8) uint64_t k_full[2], k_empty[2], ks_full[4], v_full[2], v_empty[2], s_full[2], o_full[2];
   __shared__ uint32_t tmem_base;
   __shared__ int abort_flag;
   // scale and presence of a tile's keys; a slot is written again when both groups are past the tile after it
   __shared__ __align__(16) float ks_s[4][kTcKeys];
   __shared__ uint32_t present_s[4][4];
+  __shared__ float rf_s[kTcRows];
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   // ---- this CTA's rows: later row blocks, which see more keys, come first ----
@@ -171,20 +237,19 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv4_tc_kernel(Kv4TcParams pp) {
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(dyn_smem) + 1023) & ~uintptr_t(1023));
   uint8_t *const q_sm = smem, *const k_sm = smem + 2 * kTile, *const v_sm = smem + 4 * kTile;
   if (threadIdx.x == 0) {
-    sm100::mbar_init(&q_full, groups * 128);
     for (int i = 0; i < 2; ++i) {
-      sm100::mbar_init(&k_full[i], 128);
-      sm100::mbar_init(&v_full[i], 128);
-      sm100::mbar_init(&k_empty[i], 1);
-      sm100::mbar_init(&v_empty[i], 1);
+      sm100::mbar_init(&k_full[i], 4);      // a warp each of those that unpack
+      sm100::mbar_init(&v_full[i], 4);
+      sm100::mbar_init(&k_empty[i], groups);
+      sm100::mbar_init(&v_empty[i], groups);
       sm100::mbar_init(&s_full[i], 1);
-      sm100::mbar_init(&p_full[i], 128);
+      sm100::mbar_init(&o_full[i], 1);
     }
-    sm100::mbar_init(&o_full, 1);
+    for (int i = 0; i < 4; ++i) sm100::mbar_init(&ks_full[i], 4);
     abort_flag = 0;
     sm100::mbar_fence_init();
   }
-  if (warp == 12) sm100::tmem_alloc(&tmem_base, 512);
+  if (warp == 8) sm100::tmem_alloc(&tmem_base, 512);
   sm100::tc_fence_before();
   __syncthreads();
   sm100::tc_fence_after();
@@ -195,164 +260,168 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv4_tc_kernel(Kv4TcParams pp) {
     if (!*abort_v && !sm100::mbar_wait(bar, parity, pp.fault, code)) *abort_v = 1;
   };
 
-  if (warp == 12) {
-    // ---- MMA issue ----
-    // The whole warp runs these loops and one elected lane issues, so that descriptors stay in uniform registers.
-    if (tiles) {
+  if (warp >= 8) {
+    // ---- unpacking: thread = key of the tile, keys or values ----
+    regs_down<kTcRegsUnpack>();
+    const bool values = warp >= 12;
+    const int key = threadIdx.x & 127;
+    const int32_t* table = p.s.table + int64_t(b) * p.s.width;
+    const uint8_t* codes = values ? p.c.vc : p.c.kc;
+    // row of the cache that holds this thread's key of tile i, -1 where none does
+    auto row_of = [&](int i) -> int64_t {
+      const int pos = i * kTcKeys + key;
+      if (i >= tiles || pos >= s.len) return -1;
+      const int pg = __ldg(table + (pos >> p.c.page_shift));
+      if (uint32_t(pg) >= uint32_t(p.c.num_pages)) return -1;
+      return int64_t(uint32_t(pg) * p.c.heads + h) * p.c.page_size + (pos & (p.c.page_size - 1));
+    };
+    uint4 cw[W / 4];
+    uint32_t kp = 0, vp = 0;
+    auto load = [&](int64_t row) {
+      if (row < 0) return;
+      const uint4* src = reinterpret_cast<const uint4*>(codes + row * (D / 2));
+#pragma unroll
+      for (int w = 0; w < W / 4; ++w) cw[w] = __ldg(src + w);
+      kp = __ldg(p.c.kp + row);
+      vp = __ldg(p.c.vp + row);
+    };
+    int64_t row = row_of(0), row1 = row_of(1);
+    load(row);
+    for (int i = 0; i < tiles; ++i) {
+      const int slot = i & 1;
+      const uint32_t par = ((i >> 1) & 1) ^ 1;
+      const bool here = row >= 0;
+      uint8_t* dst = (values ? v_sm : k_sm) + slot * kTile;
+      if (!values) {
+        // K: c - z
+        wait(&k_empty[slot], par, KV4_TIMEOUT_TILE);
+        const float vs = kv4_scale(vp);
+        // a row of NaN, of K or of V, reaches the rows that see it through their scores
+        ks_s[i & 3][key] = !here ? 0.f : vs != vs ? vs : kv4_scale(kp);
+        const uint32_t there = __ballot_sync(0xffffffffu, here);
+        if (lane == 0) present_s[i & 3][warp - 8] = there;
+        tc_unpack<W, UNPACK_CODES>(dst, key, cw, kp & 15u, 0.f);
+      } else {
+        // V: s (c - z), rounded once
+        wait(&v_empty[slot], par, KV4_TIMEOUT_TILE);
+        const float vs = kv4_scale(vp);
+        if (!here || vs != vs) {
+#pragma unroll
+          for (int w = 0; w < W; ++w)
+            *reinterpret_cast<uint4*>(dst + (w >> 3) * (kTcKeys * 128) + sw128(key, w & 7)) = make_uint4(0, 0, 0, 0);
+        } else if (BF16) {
+          tc_unpack<W, UNPACK_BF16>(dst, key, cw, vp & 15u, vs);
+        } else if (vs >= 0x1p-17f && vs < 65504.f) {
+          tc_unpack<W, UNPACK_F16>(dst, key, cw, vp & 15u, vs);
+        } else {
+          tc_unpack<W, UNPACK_F32>(dst, key, cw, vp & 15u, vs);
+        }
+      }
+      sm100::fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) {
+        sm100::mbar_arrive(values ? &v_full[slot] : &k_full[slot]);
+        if (!values) sm100::mbar_arrive(&ks_full[i & 3]);
+      }
+      load(row1);                                // after the fence, which would wait for it
+      row = row1;
+      row1 = row_of(i + 2);
+    }
+  } else {
+    // ---- rows ----
+    regs_up<kTcRegsRows>();
+    const int g = warp >> 2, row = threadIdx.x & 127;
+    const int rr = r0 + g * 128 + row;
+    const bool ok = rr < rows_all;
+    if (g < groups) {
+      uint8_t* const q_mine = q_sm + g * kTile;
+      auto group_sync = [&] { asm volatile("bar.sync %0, 128;\n" ::"r"(1 + g) : "memory"); };
+      // ---- Q: D / 8 lanes a row; each row scaled by the power of two that brings its largest magnitude into [1, 2),
+      // with the softmax scale's sign ----
+      {
+        constexpr int L = D / 8, R = 32 / L;     // lanes a row, rows at a time
+        const int c = lane % L;
+        uint4 qw[32 / R];
+#pragma unroll
+        for (int j = 0; j < 32 / R; ++j) {
+          const int r = r0 + warp * 32 + j * R + lane / L;
+          qw[j] = make_uint4(0, 0, 0, 0);
+          if (r < rows_all) {
+            const uint16_t* src = p.q + (s.q0 + r / p.group) * p.q_tok + (h * p.group + r % p.group) * p.q_head + c * 8;
+            if (p.q_vec) {
+              qw[j] = __ldg(reinterpret_cast<const uint4*>(src));
+            } else {
+              uint32_t e[4];
+#pragma unroll
+              for (int k = 0; k < 4; ++k) e[k] = uint32_t(__ldg(src + 2 * k)) | uint32_t(__ldg(src + 2 * k + 1)) << 16;
+              qw[j] = make_uint4(e[0], e[1], e[2], e[3]);
+            }
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < 32 / R; ++j) {
+          const uint32_t ww[4] = {qw[j].x, qw[j].y, qw[j].z, qw[j].w};
+          float v[8];
+          uint32_t mx = 0;
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const uint16_t e = uint16_t(ww[k / 2] >> (16 * (k & 1)));
+            v[k] = BF16 ? __uint_as_float(uint32_t(e) << 16) : __half2float(__ushort_as_half(e));
+            mx = max(mx, __float_as_uint(v[k]) & 0x7fffffffu);
+          }
+#pragma unroll
+          for (int o = 1; o < L; o <<= 1) mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+          int e = int(mx >> 23);                 // infinities and NaN stay what they are
+          e = e == 255 ? 127 : e < 1 ? 1 : e > 253 ? 253 : e;
+          const float down = copysignf(__uint_as_float(uint32_t(254 - e) << 23), p.scale_log2);
+          const int q_row = (warp & 3) * 32 + j * R + lane / L;
+          if (c == 0) rf_s[g * 128 + q_row] = __uint_as_float(uint32_t(e) << 23) * fabsf(p.scale_log2);
+          uint32_t w[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) w[k] = h2_u(__floats2half2_rn(v[k] * down, v[k + 4] * down));
+          *reinterpret_cast<uint4*>(q_mine + (c >> 3) * (kTcKeys * 128) + sw128(q_row, c & 7)) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+      }
+      sm100::fence_proxy_async();
+      group_sync();
+      const float rf = rf_s[g * 128 + row];
+
+      // ---- MMA issue, by the group's first warp: all of it runs this code and one elected lane issues, so that
+      // descriptors stay in uniform registers ----
       constexpr uint32_t kIdS = tc_idesc(kTcKeys, false, false), kIdO = tc_idesc(D, BF16, true);
+      const bool issuer = (warp & 3) == 0;
       // K-major rows of 128 bytes (64 values), blocks of 64 values 16 KB apart
-      const uint64_t qd = sm100::smem_desc_sw128(sm100::smem_u32(q_sm), 16, 1024), kd = sm100::smem_desc_sw128(sm100::smem_u32(k_sm), 16, 1024);
+      const uint64_t qd = sm100::smem_desc_sw128(sm100::smem_u32(q_mine), 16, 1024), kd = sm100::smem_desc_sw128(sm100::smem_u32(k_sm), 16, 1024);
       // MN-major: a key's 64 values a row of 128 bytes, 8 keys 1024 bytes, blocks of 64 values 16 KB apart
       const uint64_t vd = sm100::smem_desc_sw128(sm100::smem_u32(v_sm), kTcKeys * 128, 1024);
-      auto qk = [&](int i, int g) {
-        const uint64_t qg = qd + g * (kTile >> 4), ki = kd + (i & 1) * (kTile >> 4);
+      auto qk = [&](int i) {
+        wait(&k_full[i & 1], (i >> 1) & 1, KV4_TIMEOUT_TILE);
+        sm100::tc_fence_after();
+        const uint64_t ki = kd + (i & 1) * (kTile >> 4);
         if (!*abort_v && sm100::elect_one()) {
 #pragma unroll
           for (int k = 0; k < D / 16; ++k) {
             const uint32_t o = ((k >> 2) * (kTcKeys * 128) + (k & 3) * 32) >> 4;
-            mma_f16_ss(tmem + g * 128, qg + o, ki + o, kIdS, k != 0);
+            mma_f16_ss(tmem + g * 128, qd + o, ki + o, kIdS, k != 0);
           }
           sm100::mma_commit(&s_full[g]);
+          sm100::mma_commit(&k_empty[i & 1]);
         }
         __syncwarp();
       };
-      auto commit = [&](uint64_t* bar) {
-        if (sm100::elect_one()) sm100::mma_commit(bar);
-        __syncwarp();
-      };
-      wait(&q_full, 0, KV4_TIMEOUT_TILE);
-      wait(&k_full[0], 0, KV4_TIMEOUT_TILE);
-      sm100::tc_fence_after();
-      for (int g = 0; g < groups; ++g) qk(0, g);
-      commit(&k_empty[0]);
-      for (int i = 0; i < tiles; ++i) {
+      auto pv = [&](int i) {
         wait(&v_full[i & 1], (i >> 1) & 1, KV4_TIMEOUT_TILE);
-        if (i + 1 < tiles) wait(&k_full[(i + 1) & 1], ((i + 1) >> 1) & 1, KV4_TIMEOUT_TILE);
+        sm100::tc_fence_after();
         const uint64_t vi = vd + (i & 1) * (kTile >> 4);
-        for (int g = 0; g < groups; ++g) {
-          wait(&p_full[g], i & 1, KV4_TIMEOUT_P);
-          sm100::tc_fence_after();
-          if (!*abort_v && sm100::elect_one()) {
+        if (!*abort_v && sm100::elect_one()) {
 #pragma unroll
-            for (int k = 0; k < kTcKeys / 16; ++k)
-              mma_f16_ts(tmem + 256 + g * 128, tmem + g * 128 + k * 8, vi + k * (2048 >> 4), kIdO, i || k);
-          }
-          __syncwarp();
-          if (i + 1 < tiles) qk(i + 1, g);
+          for (int k = 0; k < kTcKeys / 16; ++k)
+            mma_f16_ts(tmem + 256 + g * 128, tmem + g * 128 + k * 8, vi + k * (2048 >> 4), kIdO, i || k);
+          sm100::mma_commit(&v_empty[i & 1]);
         }
-        commit(&v_empty[i & 1]);
-        if (i + 1 < tiles) commit(&k_empty[(i + 1) & 1]);
-      }
-      commit(&o_full);                           // every MMA has completed, before TMEM is read for the last time and freed
-      sm100::mbar_wait(&o_full, 0, pp.fault, KV4_TIMEOUT_DRAIN);
-    }
-  } else if (warp >= 8) {
-    // ---- unpacking: thread = key of the tile; the next tile's codes are on their way meanwhile ----
-    const int key = threadIdx.x - 256;
-    const int32_t* table = p.s.table + int64_t(b) * p.s.width;
-    uint4 kw[W / 4], vw[W / 4], kn[W / 4], vn[W / 4];
-    uint32_t kp = 0, vp = 0, kpn = 0, vpn = 0;
-    bool here = false, here_n = false;
-    auto load = [&](int i) {
-      const int pos = i * kTcKeys + key;
-      here_n = false;
-      if (i < tiles && pos < s.len) {
-        const int pg = __ldg(table + (pos >> p.c.page_shift));
-        if (uint32_t(pg) < uint32_t(p.c.num_pages)) {
-          here_n = true;
-          const uint64_t row = (uint32_t(pg) * p.c.heads + h) * p.c.page_size + (pos & (p.c.page_size - 1));   // fits 32 bits
-          const uint4* ks = reinterpret_cast<const uint4*>(p.c.kc + row * (D / 2));
-          const uint4* vs = reinterpret_cast<const uint4*>(p.c.vc + row * (D / 2));
-#pragma unroll
-          for (int w = 0; w < W / 4; ++w) kn[w] = __ldg(ks + w), vn[w] = __ldg(vs + w);
-          kpn = __ldg(p.c.kp + row);
-          vpn = __ldg(p.c.vp + row);
-        }
-      }
-    };
-    load(0);
-    for (int i = 0; i < tiles; ++i) {
-#pragma unroll
-      for (int w = 0; w < W / 4; ++w) kw[w] = kn[w], vw[w] = vn[w];
-      kp = kpn, vp = vpn, here = here_n;
-      load(i + 1);
-      const uint32_t par = ((i >> 1) & 1) ^ 1;
-      // K: c - z
-      wait(&k_empty[i & 1], par, KV4_TIMEOUT_TILE);
-      const float vs = here ? kv4_scale(vp) : 0.f;
-      // a row of NaN, of K or of V, reaches the rows that see it through their scores
-      const bool v_nan = vs != vs;
-      ks_s[i & 3][key] = !here ? 0.f : v_nan ? vs : kv4_scale(kp);
-      const uint32_t there = __ballot_sync(0xffffffffu, here);
-      if (lane == 0) present_s[i & 3][warp - 8] = there;
-      uint8_t* dst = k_sm + (i & 1) * kTile;
-      tc_unpack<W, UNPACK_CODES>(dst, key, kw, kp & 15u, 0.f);
-      sm100::fence_proxy_async();
-      sm100::mbar_arrive(&k_full[i & 1]);
-      // V: s (c - z), rounded once
-      wait(&v_empty[i & 1], par, KV4_TIMEOUT_TILE);
-      dst = v_sm + (i & 1) * kTile;
-      if (!here || v_nan) {
-#pragma unroll
-        for (int w = 0; w < W; ++w)
-          *reinterpret_cast<uint4*>(dst + (w >> 3) * (kTcKeys * 128) + sw128(key, w & 7)) = make_uint4(0, 0, 0, 0);
-      } else if (BF16) {
-        tc_unpack<W, UNPACK_BF16>(dst, key, vw, vp & 15u, vs);
-      } else if (vs >= 0x1p-17f && vs < 65504.f) {
-        tc_unpack<W, UNPACK_F16>(dst, key, vw, vp & 15u, vs);
-      } else {
-        tc_unpack<W, UNPACK_F32>(dst, key, vw, vp & 15u, vs);
-      }
-      sm100::fence_proxy_async();
-      sm100::mbar_arrive(&v_full[i & 1]);
-    }
-  } else {
-    // ---- rows ----
-    const int g = warp >> 2, row = threadIdx.x & 127;
-    const int rr = r0 + g * 128 + row;
-    const bool ok = rr < rows_all;
-    const int64_t oi = ok ? int64_t(s.q0 + rr / p.group) * p.hq + h * p.group + rr % p.group : 0;
-    float rf = 0.f;
-    if (g < groups) {
-      const int64_t qi = ok ? (s.q0 + rr / p.group) * p.q_tok + (h * p.group + rr % p.group) * p.q_head : 0;
-      uint32_t mx = 0;
-      auto chunk = [&](int c, float (&v)[8]) {
-        if (ok && p.q_vec) {
-          const uint4 w = __ldg(reinterpret_cast<const uint4*>(p.q + qi) + c);
-          const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const uint16_t e = uint16_t(ww[j / 2] >> (16 * (j & 1)));
-            v[j] = BF16 ? __uint_as_float(uint32_t(e) << 16) : __half2float(__ushort_as_half(e));
-          }
-        } else {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) v[j] = ok ? ld_q(p, qi + 8 * c + j) : 0.f;
-        }
+        __syncwarp();
       };
-#pragma unroll 4
-      for (int c = 0; c < D / 8; ++c) {
-        float v[8];
-        chunk(c, v);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) mx = max(mx, __float_as_uint(v[j]) & 0x7fffffffu);
-      }
-      int e = int(mx >> 23);
-      e = e == 255 ? 127 : e < 1 ? 1 : e > 253 ? 253 : e;
-      // the power of two that brings the row's largest magnitude into [1, 2), with the softmax scale's sign
-      const float down = copysignf(__uint_as_float(uint32_t(254 - e) << 23), p.scale_log2);
-      rf = __uint_as_float(uint32_t(e) << 23) * fabsf(p.scale_log2);
-#pragma unroll 4
-      for (int c = 0; c < D / 8; ++c) {
-        float v[8];
-        chunk(c, v);
-        uint32_t w[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) w[j] = h2_u(__floats2half2_rn(v[j] * down, v[j + 4] * down));
-        *reinterpret_cast<uint4*>(q_sm + g * kTile + (c >> 3) * (kTcKeys * 128) + sw128(row, c & 7)) = make_uint4(w[0], w[1], w[2], w[3]);
-      }
-      sm100::fence_proxy_async();
-      sm100::mbar_arrive(&q_full);
+      if (issuer && tiles) qk(0);
       const int lim = ok ? (p.causal ? min(s.len, s.p0 + rr / p.group + 1) : s.len) : 0;
       const uint32_t lanes = uint32_t((warp & 3) * 32) << 16, t_s = tmem + lanes + g * 128, t_o = tmem + lanes + 256 + g * 128;
       float mu = 0.f, l = 0.f;
@@ -360,33 +429,38 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv4_tc_kernel(Kv4TcParams pp) {
 
       auto tile = [&](int i, auto masked_c) {
         constexpr bool kMasked = decltype(masked_c)::value;
-        const float4* ks = reinterpret_cast<const float4*>(ks_s[i & 3]);
-        auto score = [&](const uint32_t (&v)[32], int c, float (&y)[32]) {
-          const uint32_t present = kMasked ? present_s[i & 3][c] : 0u;
+        const ulonglong2* ks = reinterpret_cast<const ulonglong2*>(ks_s[i & 3]);
+        uint32_t v[kTcKeys];
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const float4 k4 = ks[c * 8 + j];
-            y[4 * j] = __uint_as_float(v[4 * j]) * k4.x;
-            y[4 * j + 1] = __uint_as_float(v[4 * j + 1]) * k4.y;
-            y[4 * j + 2] = __uint_as_float(v[4 * j + 2]) * k4.z;
-            y[4 * j + 3] = __uint_as_float(v[4 * j + 3]) * k4.w;
-          }
+        for (int c = 0; c < 4; ++c) tmem_ld32_start(t_s + c * 32, v + c * 32);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_landed(v + c * 32);
+        // scores, but for the row's factor
+        uint64_t y[kTcKeys / 2];
+        float top4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int j = 0; j < kTcKeys / 4; ++j) {
+          const ulonglong2 k4 = ks[j];
+          y[2 * j] = mul2(pack2(__uint_as_float(v[4 * j]), __uint_as_float(v[4 * j + 1])), k4.x);
+          y[2 * j + 1] = mul2(pack2(__uint_as_float(v[4 * j + 2]), __uint_as_float(v[4 * j + 3])), k4.y);
           if (kMasked) {
+            const uint32_t present = present_s[i & 3][j / 8];
+            float f[4];
+            unpack2(y[2 * j], f[0], f[1]);
+            unpack2(y[2 * j + 1], f[2], f[3]);
 #pragma unroll
-            for (int j = 0; j < 32; ++j)
-              if (!(i * kTcKeys + c * 32 + j < lim && (present >> j & 1))) y[j] = -INFINITY;
+            for (int e = 0; e < 4; ++e)
+              if (!(i * kTcKeys + 4 * j + e < lim && (present >> (4 * (j % 8) + e) & 1))) f[e] = -INFINITY;
+            y[2 * j] = pack2(f[0], f[1]);
+            y[2 * j + 1] = pack2(f[2], f[3]);
           }
-        };
-        float mx = -INFINITY;
-#pragma unroll 1
-        for (int c = 0; c < 4; ++c) {
-          uint32_t v[32];
-          float y[32];
-          sm100::tmem_ld32(t_s + c * 32, v);
-          score(v, c, y);
-#pragma unroll
-          for (int j = 0; j < 32; ++j) mx = fmaxf(mx, y[j]);
+          float f[4];
+          unpack2(y[2 * j], f[0], f[1]);
+          unpack2(y[2 * j + 1], f[2], f[3]);
+          top4[(2 * j) & 3] = max3(top4[(2 * j) & 3], f[0], f[1]);
+          top4[(2 * j + 1) & 3] = max3(top4[(2 * j + 1) & 3], f[2], f[3]);
         }
+        const float mx = fmaxf(max3(top4[0], top4[1], top4[2]), top4[3]);
         const float top = mx == -INFINITY ? -INFINITY : mx * rf;
         const bool up = begun ? top > mu + kSlack : mx != -INFINITY;
         if (__any_sync(0xffffffffu, up)) {
@@ -400,45 +474,61 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv4_tc_kernel(Kv4TcParams pp) {
           l *= corr;
           if (i) {                               // P V of the tiles before has ended: it was issued before this S
 #pragma unroll 1
-            for (int c = 0; c < D / 32; ++c) {
-              uint32_t v[32];
-              sm100::tmem_ld32(t_o + c * 32, v);
+            for (int c = 0; c < D / 16; ++c) {
+              uint32_t u[16];
+              tmem_ld16(t_o + c * 16, u);
 #pragma unroll
-              for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) * corr);
-              tmem_st32(t_o + c * 32, v);
+              for (int j = 0; j < 16; ++j) u[j] = __float_as_uint(__uint_as_float(u[j]) * corr);
+              tmem_st16(t_o + c * 16, u);
             }
           }
         }
-#pragma unroll 1
-        for (int c = 0; c < 4; ++c) {
-          uint32_t v[32], w[16];
-          float y[32];
-          sm100::tmem_ld32(t_s + c * 32, v);
-          score(v, c, y);
-          float sum[4] = {};
+        const uint64_t rf2 = pack2(rf, rf), mu2 = pack2(-mu, -mu);
+        uint64_t sum2[2] = {0, 0};
 #pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            y[j] = kMasked && y[j] == -INFINITY ? 0.f : exp2_(fmaf(y[j], rf, -mu));
-            sum[j & 3] += y[j];
-          }
-          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        for (int c = 0; c < 4; ++c) {
+          uint32_t w[16];
+          float x[32];
 #pragma unroll
           for (int j = 0; j < 16; ++j) {
+            unpack2(fma2(y[16 * c + j], rf2, mu2), x[2 * j], x[2 * j + 1]);
+            if (kMasked) {                       // a row of factor 0 must not turn -inf into a NaN
+              float ya, ye;
+              unpack2(y[16 * c + j], ya, ye);
+              x[2 * j] = ya == -INFINITY ? -INFINITY : x[2 * j];
+              x[2 * j + 1] = ye == -INFINITY ? -INFINITY : x[2 * j + 1];
+            }
+          }
+#pragma unroll
+          for (int j = 0; j < 32; ++j) x[j] = exp2_(x[j]);
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            sum2[j & 1] = add2(sum2[j & 1], pack2(x[2 * j], x[2 * j + 1]));
             if (BF16) {
-              const __nv_bfloat162 r = __floats2bfloat162_rn(y[2 * j], y[2 * j + 1]);
+              const __nv_bfloat162 r = __floats2bfloat162_rn(x[2 * j], x[2 * j + 1]);
               w[j] = *reinterpret_cast<const uint32_t*>(&r);
             } else {
-              w[j] = h2_u(__floats2half2_rn(y[2 * j], y[2 * j + 1]));
+              w[j] = h2_u(__floats2half2_rn(x[2 * j], x[2 * j + 1]));
             }
           }
           tmem_st16(t_s + c * 16, w);            // over S columns that have been read
         }
+        float a, e;
+        unpack2(add2(sum2[0], sum2[1]), a, e);
+        l += a + e;
         tmem_wait_st();
         sm100::tc_fence_before();
-        sm100::mbar_arrive(&p_full[g]);
+        group_sync();
+        if (issuer) {
+          sm100::tc_fence_after();
+          pv(i);
+          if (i + 1 < tiles) qk(i + 1);
+        }
       };
       for (int i = 0; i < tiles; ++i) {
-        wait(&k_full[i & 1], (i >> 1) & 1, KV4_TIMEOUT_TILE);   // ks_s, present_s
+        // ks_s, present_s: their slot is not filled again before this group is past the tile, so its barrier cannot
+        // run a phase ahead
+        wait(&ks_full[i & 3], (i >> 2) & 1, KV4_TIMEOUT_TILE);
         wait(&s_full[g], i & 1, KV4_TIMEOUT_S);
         __syncwarp();
         sm100::tc_fence_after();
@@ -446,8 +536,17 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv4_tc_kernel(Kv4TcParams pp) {
         if (__any_sync(0xffffffffu, (i + 1) * kTcKeys > lim || all != 0xffffffffu)) tile(i, std::true_type{});
         else tile(i, std::false_type{});
       }
-      // ---- the rows' results ----
-      if (tiles) wait(&o_full, 0, KV4_TIMEOUT_S);
+      // ---- the rows' results, through the group's Q buffer so that a row leaves in one run ----
+      if (tiles) {
+        if (issuer) {
+          if (sm100::elect_one()) sm100::mma_commit(&o_full[g]);
+          __syncwarp();
+          // every MMA of the group has ended before TMEM is freed, also after a failed wait
+          sm100::mbar_wait(&o_full[g], 0, pp.fault, KV4_TIMEOUT_DRAIN);
+        } else {
+          wait(&o_full[g], 0, KV4_TIMEOUT_S);
+        }
+      }
       __syncwarp();
       sm100::tc_fence_after();
       const float inv = l == 0.f ? 0.f : 1.f / l;
@@ -455,8 +554,6 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv4_tc_kernel(Kv4TcParams pp) {
       for (int c = 0; c < D / 32; ++c) {
         uint32_t v[32];
         if (tiles) sm100::tmem_ld32(t_o + c * 32, v);
-        if (!ok) continue;
-        uint16_t* dst = p.o + oi * D + c * 32;
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           uint32_t w[4];
@@ -467,20 +564,37 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv4_tc_kernel(Kv4TcParams pp) {
             w[j] = BF16 ? uint32_t(__bfloat16_as_ushort(__float2bfloat16_rn(x))) | uint32_t(__bfloat16_as_ushort(__float2bfloat16_rn(z))) << 16
                         : h2_u(__floats2half2_rn(x, z));
           }
+          const int ch = c * 4 + q;
+          *reinterpret_cast<uint4*>(q_mine + (ch >> 3) * (kTcKeys * 128) + sw128(row, ch & 7)) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+      }
+      if (ok && p.lse)
+        p.lse[int64_t(s.q0 + rr / p.group) * p.hq + h * p.group + rr % p.group] =
+            l == 0.f ? -INFINITY : (mu + log2f(l)) * 0.69314718055994531f;
+      __syncwarp();                              // a warp stores its own rows
+      {
+        constexpr int L = D / 8, R = 32 / L;
+        const int ch = lane % L;
+#pragma unroll 4
+        for (int j = 0; j < 32 / R; ++j) {
+          const int q_row = (warp & 3) * 32 + j * R + lane / L, r = r0 + g * 128 + q_row;
+          if (r >= rows_all) continue;
+          const uint4 w = *reinterpret_cast<const uint4*>(q_mine + (ch >> 3) * (kTcKeys * 128) + sw128(q_row, ch & 7));
+          uint16_t* dst = p.o + (int64_t(s.q0 + r / p.group) * p.hq + h * p.group + r % p.group) * D + ch * 8;
           if (p.o_vec) {
-            reinterpret_cast<uint4*>(dst)[q] = make_uint4(w[0], w[1], w[2], w[3]);
+            *reinterpret_cast<uint4*>(dst) = w;
           } else {
+            const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-            for (int j = 0; j < 4; ++j) dst[8 * q + 2 * j] = uint16_t(w[j]), dst[8 * q + 2 * j + 1] = uint16_t(w[j] >> 16);
+            for (int k = 0; k < 8; ++k) dst[k] = uint16_t(ww[k / 2] >> (16 * (k & 1)));
           }
         }
       }
-      if (ok && p.lse) p.lse[oi] = l == 0.f ? -INFINITY : (mu + log2f(l)) * 0.69314718055994531f;
     }
   }
   sm100::tc_fence_before();
   __syncthreads();
-  if (warp == 12) {
+  if (warp == 8) {
     __syncwarp();
     sm100::tc_fence_after();
     sm100::tmem_dealloc(tmem, 512);
