@@ -5,12 +5,11 @@
 // query heads of a token side by side, so one unpacking of a key serves them
 // all) and walks the keys up to its last row's position in tiles of 128:
 //   warps 0..3, 4..7  two row groups of 128, a thread a row: Q to shared
-//                     memory, softmax of S out of TMEM, P into TMEM, O out;
-//                     a group's first warp issues its MMAs,
-//                     S = Q C^T (FP16) and O += P V
+//                     memory, softmax of S out of TMEM, P into TMEM, O out
 //   warps 8..11       unpack the tile's keys, a thread a key, into the
 //                     swizzled layout that the MMAs read
-//   warps 12..15      unpack its values
+//   warp 12           issues the MMAs: S = Q C^T (FP16), O += P V
+//   warps 13..15      unpack its values, a thread half a key at a time
 // While one group does its softmax the tensor core works for the other: per
 // tile and group D = 128 needs 1024 tensor clocks, and 1024 clocks of the
 // exponential unit.
@@ -30,7 +29,7 @@ enum Kv4TcFault : int { KV4_TIMEOUT_TILE = 21, KV4_TIMEOUT_S = 22, KV4_TIMEOUT_P
 constexpr int kTcKeys = 128;
 constexpr int kTcRows = 256;
 constexpr int kTcThreads = 16 * 32;
-// Registers a thread: 128 at launch, then shared out by warpgroup (rows, rows, keys, values: their sum is 4 * 128).
+// Registers a thread: 128 at launch, then shared out by warpgroup (rows, rows, keys, MMA and values: their sum is 4 * 128).
 constexpr int kTcRegsRows = 184, kTcRegsUnpack = 72;
 
 __host__ __device__ constexpr int tc_tile_bytes(int D) { return kTcKeys * D * 2; }
@@ -159,14 +158,14 @@ __device__ __forceinline__ uint32_t tc_finish(__half2 v, float s) {
 }
 
 template <int W, int MODE>
-__device__ __forceinline__ void tc_unpack(uint8_t* dst, uint32_t key, const uint4 (&words)[W / 4], uint32_t z, float s) {
+__device__ __forceinline__ void tc_unpack(uint8_t* dst, uint32_t key, int first, const uint4 (&words)[W / 4], uint32_t z, float s) {
   const __half2 zlo = u_h2(0x64006400u + z * 0x10001u), zhi = u_h2(0x54005400u + z * 0x100010u);   // 1024 + z, 64 + z
 #pragma unroll
   for (int q = 0; q < W / 4; ++q) {
     const uint32_t x4[4] = {words[q].x, words[q].y, words[q].z, words[q].w};
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const int w = 4 * q + j;
+      const int w = first + 4 * q + j;
       const uint32_t x = x4[j], y = x >> 8;
       uint4 o;
       if (MODE == UNPACK_BF16) {
@@ -196,7 +195,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv4_tc_kernel(Kv4TcParams pp) {
   constexpr int W = D / 8;                       // words of codes a key
   constexpr int kTile = tc_tile_bytes(D);
   extern __shared__ uint8_t dyn_smem[];
-  __shared__ __align__(8) uint64_t k_full[2], k_empty[2], ks_full[4], v_full[2], v_empty[2], s_full[2], o_full[2];
+  __shared__ __align__(8) uint64_t q_full, k_full[2], k_empty[2], ks_full[4], v_full[2], v_empty[2], s_full[2], p_full[2], o_full;
   __shared__ uint32_t tmem_base;
   __shared__ int abort_flag;
   // scale and presence of a tile's keys; a slot is written again when both groups are past the tile after it
@@ -237,14 +236,16 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv4_tc_kernel(Kv4TcParams pp) {
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(dyn_smem) + 1023) & ~uintptr_t(1023));
   uint8_t *const q_sm = smem, *const k_sm = smem + 2 * kTile, *const v_sm = smem + 4 * kTile;
   if (threadIdx.x == 0) {
+    sm100::mbar_init(&q_full, 4 * groups);   // a warp each of those that write
     for (int i = 0; i < 2; ++i) {
-      sm100::mbar_init(&k_full[i], 4);      // a warp each of those that unpack
-      sm100::mbar_init(&v_full[i], 4);
-      sm100::mbar_init(&k_empty[i], groups);
-      sm100::mbar_init(&v_empty[i], groups);
+      sm100::mbar_init(&k_full[i], 4);
+      sm100::mbar_init(&v_full[i], 3);
+      sm100::mbar_init(&p_full[i], 4);
+      sm100::mbar_init(&k_empty[i], 1);
+      sm100::mbar_init(&v_empty[i], 1);
       sm100::mbar_init(&s_full[i], 1);
-      sm100::mbar_init(&o_full[i], 1);
     }
+    sm100::mbar_init(&o_full, 1);
     for (int i = 0; i < 4; ++i) sm100::mbar_init(&ks_full[i], 4);
     abort_flag = 0;
     sm100::mbar_fence_init();
@@ -260,72 +261,149 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv4_tc_kernel(Kv4TcParams pp) {
     if (!*abort_v && !sm100::mbar_wait(bar, parity, pp.fault, code)) *abort_v = 1;
   };
 
-  if (warp >= 8) {
-    // ---- unpacking: thread = key of the tile, keys or values ----
+  const int32_t* table = p.s.table + int64_t(b) * p.s.width;
+  // row of the cache that holds key `key` of tile i, -1 where none does
+  auto row_of = [&](int i, int key) -> int64_t {
+    const int pos = i * kTcKeys + key;
+    if (i >= tiles || pos >= s.len) return -1;
+    const int pg = __ldg(table + (pos >> p.c.page_shift));
+    if (uint32_t(pg) >= uint32_t(p.c.num_pages)) return -1;
+    return int64_t(uint32_t(pg) * p.c.heads + h) * p.c.page_size + (pos & (p.c.page_size - 1));
+  };
+  if (warp == 12) {
+    // ---- MMA issue: the whole warp runs these loops and one elected lane issues, so that descriptors stay in uniform
+    // registers ----
     regs_down<kTcRegsUnpack>();
-    const bool values = warp >= 12;
-    const int key = threadIdx.x & 127;
-    const int32_t* table = p.s.table + int64_t(b) * p.s.width;
-    const uint8_t* codes = values ? p.c.vc : p.c.kc;
-    // row of the cache that holds this thread's key of tile i, -1 where none does
-    auto row_of = [&](int i) -> int64_t {
-      const int pos = i * kTcKeys + key;
-      if (i >= tiles || pos >= s.len) return -1;
-      const int pg = __ldg(table + (pos >> p.c.page_shift));
-      if (uint32_t(pg) >= uint32_t(p.c.num_pages)) return -1;
-      return int64_t(uint32_t(pg) * p.c.heads + h) * p.c.page_size + (pos & (p.c.page_size - 1));
+    if (tiles) {
+      constexpr uint32_t kIdS = tc_idesc(kTcKeys, false, false), kIdO = tc_idesc(D, BF16, true);
+      // K-major rows of 128 bytes (64 values), blocks of 64 values 16 KB apart
+      const uint64_t qd = sm100::smem_desc_sw128(sm100::smem_u32(q_sm), 16, 1024), kd = sm100::smem_desc_sw128(sm100::smem_u32(k_sm), 16, 1024);
+      // MN-major: a key's 64 values a row of 128 bytes, 8 keys 1024 bytes, blocks of 64 values 16 KB apart
+      const uint64_t vd = sm100::smem_desc_sw128(sm100::smem_u32(v_sm), kTcKeys * 128, 1024);
+      auto qk = [&](int i, int g) {
+        const uint64_t qg = qd + g * (kTile >> 4), ki = kd + (i & 1) * (kTile >> 4);
+        if (!*abort_v && sm100::elect_one()) {
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k) {
+            const uint32_t o = ((k >> 2) * (kTcKeys * 128) + (k & 3) * 32) >> 4;
+            mma_f16_ss(tmem + g * 128, qg + o, ki + o, kIdS, k != 0);
+          }
+          sm100::mma_commit(&s_full[g]);
+          if (g == groups - 1) sm100::mma_commit(&k_empty[i & 1]);
+        }
+        __syncwarp();
+      };
+      wait(&q_full, 0, KV4_TIMEOUT_TILE);
+      wait(&k_full[0], 0, KV4_TIMEOUT_TILE);
+      sm100::tc_fence_after();
+      for (int g = 0; g < groups; ++g) qk(0, g);
+      for (int i = 0; i < tiles; ++i) {
+        wait(&v_full[i & 1], (i >> 1) & 1, KV4_TIMEOUT_TILE);
+        if (i + 1 < tiles) wait(&k_full[(i + 1) & 1], ((i + 1) >> 1) & 1, KV4_TIMEOUT_TILE);
+        const uint64_t vi = vd + (i & 1) * (kTile >> 4);
+        for (int g = 0; g < groups; ++g) {
+          wait(&p_full[g], i & 1, KV4_TIMEOUT_P);
+          sm100::tc_fence_after();
+          if (!*abort_v && sm100::elect_one()) {
+#pragma unroll
+            for (int k = 0; k < kTcKeys / 16; ++k)
+              mma_f16_ts(tmem + 256 + g * 128, tmem + g * 128 + k * 8, vi + k * (2048 >> 4), kIdO, i || k);
+            if (g == groups - 1) sm100::mma_commit(&v_empty[i & 1]);
+          }
+          __syncwarp();
+          if (i + 1 < tiles) qk(i + 1, g);
+        }
+      }
+      if (sm100::elect_one()) sm100::mma_commit(&o_full);
+      __syncwarp();
+      // every MMA has ended before TMEM is freed, also after a failed wait
+      sm100::mbar_wait(&o_full, 0, pp.fault, KV4_TIMEOUT_DRAIN);
+    }
+  } else if (warp > 12) {
+    // ---- values: s (c - z), rounded once; items of half a key, thread t takes t, t + 96, t + 192 ----
+    regs_down<kTcRegsUnpack>();
+    constexpr int H = W / 2, kItems = 3;
+    const int t = threadIdx.x - 13 * 32;
+    uint4 cw[kItems][H / 4];
+    uint32_t vp[kItems] = {};
+    int64_t row[kItems], row1[kItems];
+    auto load = [&](int j) {
+      if (row[j] < 0) return;
+      const uint4* src = reinterpret_cast<const uint4*>(p.c.vc + row[j] * (D / 2) + ((t + 96 * j) >> 7) * (D / 4));
+#pragma unroll
+      for (int w = 0; w < H / 4; ++w) cw[j][w] = __ldg(src + w);
+      vp[j] = __ldg(p.c.vp + row[j]);
     };
+    auto row_item = [&](int i, int j) { return t + 96 * j < 256 ? row_of(i, (t + 96 * j) & 127) : int64_t(-1); };
+#pragma unroll
+    for (int j = 0; j < kItems; ++j) row[j] = row_item(0, j), row1[j] = row_item(1, j);
+#pragma unroll
+    for (int j = 0; j < kItems; ++j) load(j);
+    for (int i = 0; i < tiles; ++i) {
+      uint8_t* const dst = v_sm + (i & 1) * kTile;
+      wait(&v_empty[i & 1], ((i >> 1) & 1) ^ 1, KV4_TIMEOUT_TILE);
+#pragma unroll
+      for (int j = 0; j < kItems; ++j) {
+        const int item = t + 96 * j, key = item & 127, first = (item >> 7) * H;
+        if (item >= 256) continue;
+        const float vs = kv4_scale(vp[j]);
+        if (row[j] < 0 || vs != vs) {
+#pragma unroll
+          for (int w = 0; w < H; ++w)
+            *reinterpret_cast<uint4*>(dst + ((first + w) >> 3) * (kTcKeys * 128) + sw128(key, (first + w) & 7)) = make_uint4(0, 0, 0, 0);
+        } else if (BF16) {
+          tc_unpack<H, UNPACK_BF16>(dst, key, first, cw[j], vp[j] & 15u, vs);
+        } else if (vs >= 0x1p-17f && vs < 65504.f) {
+          tc_unpack<H, UNPACK_F16>(dst, key, first, cw[j], vp[j] & 15u, vs);
+        } else {
+          tc_unpack<H, UNPACK_F32>(dst, key, first, cw[j], vp[j] & 15u, vs);
+        }
+      }
+      sm100::fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) sm100::mbar_arrive(&v_full[i & 1]);
+      // after the fence, which would wait for them
+#pragma unroll
+      for (int j = 0; j < kItems; ++j) row[j] = row1[j];
+#pragma unroll
+      for (int j = 0; j < kItems; ++j) load(j);
+#pragma unroll
+      for (int j = 0; j < kItems; ++j) row1[j] = row_item(i + 2, j);
+    }
+  } else if (warp >= 8) {
+    // ---- keys: c - z; thread = key of the tile ----
+    regs_down<kTcRegsUnpack>();
+    const int key = threadIdx.x & 127;
     uint4 cw[W / 4];
     uint32_t kp = 0, vp = 0;
     auto load = [&](int64_t row) {
       if (row < 0) return;
-      const uint4* src = reinterpret_cast<const uint4*>(codes + row * (D / 2));
+      const uint4* src = reinterpret_cast<const uint4*>(p.c.kc + row * (D / 2));
 #pragma unroll
       for (int w = 0; w < W / 4; ++w) cw[w] = __ldg(src + w);
       kp = __ldg(p.c.kp + row);
       vp = __ldg(p.c.vp + row);
     };
-    int64_t row = row_of(0), row1 = row_of(1);
+    int64_t row = row_of(0, key), row1 = row_of(1, key);
     load(row);
     for (int i = 0; i < tiles; ++i) {
-      const int slot = i & 1;
-      const uint32_t par = ((i >> 1) & 1) ^ 1;
+      wait(&k_empty[i & 1], ((i >> 1) & 1) ^ 1, KV4_TIMEOUT_TILE);
       const bool here = row >= 0;
-      uint8_t* dst = (values ? v_sm : k_sm) + slot * kTile;
-      if (!values) {
-        // K: c - z
-        wait(&k_empty[slot], par, KV4_TIMEOUT_TILE);
-        const float vs = kv4_scale(vp);
-        // a row of NaN, of K or of V, reaches the rows that see it through their scores
-        ks_s[i & 3][key] = !here ? 0.f : vs != vs ? vs : kv4_scale(kp);
-        const uint32_t there = __ballot_sync(0xffffffffu, here);
-        if (lane == 0) present_s[i & 3][warp - 8] = there;
-        tc_unpack<W, UNPACK_CODES>(dst, key, cw, kp & 15u, 0.f);
-      } else {
-        // V: s (c - z), rounded once
-        wait(&v_empty[slot], par, KV4_TIMEOUT_TILE);
-        const float vs = kv4_scale(vp);
-        if (!here || vs != vs) {
-#pragma unroll
-          for (int w = 0; w < W; ++w)
-            *reinterpret_cast<uint4*>(dst + (w >> 3) * (kTcKeys * 128) + sw128(key, w & 7)) = make_uint4(0, 0, 0, 0);
-        } else if (BF16) {
-          tc_unpack<W, UNPACK_BF16>(dst, key, cw, vp & 15u, vs);
-        } else if (vs >= 0x1p-17f && vs < 65504.f) {
-          tc_unpack<W, UNPACK_F16>(dst, key, cw, vp & 15u, vs);
-        } else {
-          tc_unpack<W, UNPACK_F32>(dst, key, cw, vp & 15u, vs);
-        }
-      }
+      const float vs = kv4_scale(vp);
+      // a row of NaN, of K or of V, reaches the rows that see it through their scores
+      ks_s[i & 3][key] = !here ? 0.f : vs != vs ? vs : kv4_scale(kp);
+      const uint32_t there = __ballot_sync(0xffffffffu, here);
+      if (lane == 0) present_s[i & 3][warp - 8] = there;
+      tc_unpack<W, UNPACK_CODES>(k_sm + (i & 1) * kTile, key, 0, cw, kp & 15u, 0.f);
       sm100::fence_proxy_async();
       __syncwarp();
       if (lane == 0) {
-        sm100::mbar_arrive(values ? &v_full[slot] : &k_full[slot]);
-        if (!values) sm100::mbar_arrive(&ks_full[i & 3]);
+        sm100::mbar_arrive(&k_full[i & 1]);
+        sm100::mbar_arrive(&ks_full[i & 3]);
       }
-      load(row1);                                // after the fence, which would wait for it
+      load(row1);
       row = row1;
-      row1 = row_of(i + 2);
+      row1 = row_of(i + 2, key);
     }
   } else {
     // ---- rows ----
@@ -335,7 +413,6 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv4_tc_kernel(Kv4TcParams pp) {
     const bool ok = rr < rows_all;
     if (g < groups) {
       uint8_t* const q_mine = q_sm + g * kTile;
-      auto group_sync = [&] { asm volatile("bar.sync %0, 128;\n" ::"r"(1 + g) : "memory"); };
       // ---- Q: D / 8 lanes a row; each row scaled by the power of two that brings its largest magnitude into [1, 2),
       // with the softmax scale's sign ----
       {
@@ -383,45 +460,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv4_tc_kernel(Kv4TcParams pp) {
         }
       }
       sm100::fence_proxy_async();
-      group_sync();
+      __syncwarp();                              // rf_s: a warp reads what it wrote
+      if (lane == 0) sm100::mbar_arrive(&q_full);
       const float rf = rf_s[g * 128 + row];
-
-      // ---- MMA issue, by the group's first warp: all of it runs this code and one elected lane issues, so that
-      // descriptors stay in uniform registers ----
-      constexpr uint32_t kIdS = tc_idesc(kTcKeys, false, false), kIdO = tc_idesc(D, BF16, true);
-      const bool issuer = (warp & 3) == 0;
-      // K-major rows of 128 bytes (64 values), blocks of 64 values 16 KB apart
-      const uint64_t qd = sm100::smem_desc_sw128(sm100::smem_u32(q_mine), 16, 1024), kd = sm100::smem_desc_sw128(sm100::smem_u32(k_sm), 16, 1024);
-      // MN-major: a key's 64 values a row of 128 bytes, 8 keys 1024 bytes, blocks of 64 values 16 KB apart
-      const uint64_t vd = sm100::smem_desc_sw128(sm100::smem_u32(v_sm), kTcKeys * 128, 1024);
-      auto qk = [&](int i) {
-        wait(&k_full[i & 1], (i >> 1) & 1, KV4_TIMEOUT_TILE);
-        sm100::tc_fence_after();
-        const uint64_t ki = kd + (i & 1) * (kTile >> 4);
-        if (!*abort_v && sm100::elect_one()) {
-#pragma unroll
-          for (int k = 0; k < D / 16; ++k) {
-            const uint32_t o = ((k >> 2) * (kTcKeys * 128) + (k & 3) * 32) >> 4;
-            mma_f16_ss(tmem + g * 128, qd + o, ki + o, kIdS, k != 0);
-          }
-          sm100::mma_commit(&s_full[g]);
-          sm100::mma_commit(&k_empty[i & 1]);
-        }
-        __syncwarp();
-      };
-      auto pv = [&](int i) {
-        wait(&v_full[i & 1], (i >> 1) & 1, KV4_TIMEOUT_TILE);
-        sm100::tc_fence_after();
-        const uint64_t vi = vd + (i & 1) * (kTile >> 4);
-        if (!*abort_v && sm100::elect_one()) {
-#pragma unroll
-          for (int k = 0; k < kTcKeys / 16; ++k)
-            mma_f16_ts(tmem + 256 + g * 128, tmem + g * 128 + k * 8, vi + k * (2048 >> 4), kIdO, i || k);
-          sm100::mma_commit(&v_empty[i & 1]);
-        }
-        __syncwarp();
-      };
-      if (issuer && tiles) qk(0);
       const int lim = ok ? (p.causal ? min(s.len, s.p0 + rr / p.group + 1) : s.len) : 0;
       const uint32_t lanes = uint32_t((warp & 3) * 32) << 16, t_s = tmem + lanes + g * 128, t_o = tmem + lanes + 256 + g * 128;
       float mu = 0.f, l = 0.f;
@@ -518,12 +559,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv4_tc_kernel(Kv4TcParams pp) {
         l += a + e;
         tmem_wait_st();
         sm100::tc_fence_before();
-        group_sync();
-        if (issuer) {
-          sm100::tc_fence_after();
-          pv(i);
-          if (i + 1 < tiles) qk(i + 1);
-        }
+        __syncwarp();
+        if (lane == 0) sm100::mbar_arrive(&p_full[g]);
       };
       for (int i = 0; i < tiles; ++i) {
         // ks_s, present_s: their slot is not filled again before this group is past the tile, so its barrier cannot
@@ -537,16 +574,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv4_tc_kernel(Kv4TcParams pp) {
         else tile(i, std::false_type{});
       }
       // ---- the rows' results, through the group's Q buffer so that a row leaves in one run ----
-      if (tiles) {
-        if (issuer) {
-          if (sm100::elect_one()) sm100::mma_commit(&o_full[g]);
-          __syncwarp();
-          // every MMA of the group has ended before TMEM is freed, also after a failed wait
-          sm100::mbar_wait(&o_full[g], 0, pp.fault, KV4_TIMEOUT_DRAIN);
-        } else {
-          wait(&o_full[g], 0, KV4_TIMEOUT_S);
-        }
-      }
+      if (tiles) wait(&o_full, 0, KV4_TIMEOUT_S);
       __syncwarp();
       sm100::tc_fence_after();
       const float inv = l == 0.f ? 0.f : 1.f / l;
