@@ -340,6 +340,7 @@ extern "C" int tac_kv4_attention(const tac_kv4_cache* cache, const int32_t* page
   p.q_head = q_head;
   p.hq = q_heads;
   p.group = q_heads / p.c.heads;
+  p.div = make_divider(p.group);
   p.bf16 = type == TAC_BF16;
   p.causal = causal != 0;
   p.scale_log2 = scale * 1.4426950408889634f;

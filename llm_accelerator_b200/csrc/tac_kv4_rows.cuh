@@ -37,6 +37,19 @@ constexpr float kSlack = 8.f;
 constexpr uint32_t kSlackV = 6;
 constexpr int kRowsTile = kRowsWarps * 32;         // keys of a tile, 32 a warp
 
+// n / d and n % d for n below 2^31: with 2^(s - 1) < d <= 2^s, m = ceil(2^(31 + s) / d) is less than one above the
+// quotient, so n m / 2^(31 + s) exceeds n / d by less than 1 / d.
+struct Divider {
+  uint32_t d, m, s;
+  __host__ __device__ int of(int n) const { return int((uint64_t(uint32_t(n)) * m) >> (31 + s)); }
+  __host__ __device__ int rest(int n) const { return n - of(n) * int(d); }
+};
+inline Divider make_divider(uint32_t d) {
+  uint32_t s = 0;
+  while ((uint32_t(1) << s) < d) ++s;
+  return {d, uint32_t(((uint64_t(1) << (31 + s)) + d - 1) / d), s};
+}
+
 struct Kv4RowsParams {
   Kv4Cache c;
   Kv4Seqs s;
@@ -45,6 +58,7 @@ struct Kv4RowsParams {
   float* lse;            // or null
   int64_t q_tok, q_head; // strides in elements
   int hq, group;         // query heads, query heads of one key-value head
+  Divider div;           // by group
   int bf16, causal, split;
   int q_vec, o_vec;      // q's, o's rows are 16-byte aligned
   float scale_log2;      // softmax scale * log2(e)
@@ -317,7 +331,7 @@ __global__ void __launch_bounds__(kRowsThreads, rows_ctas(D, NT)) kv4_rows_kerne
     for (int n = 0; n < NT; ++n) {
       const int r = r0 + n * 8 + g;
       const bool ok = r < rows_all;
-      const int64_t qi = ok ? (s.q0 + r / p.group) * p.q_tok + (h * p.group + r % p.group) * p.q_head + (D / 4) * t : 0;
+      const int64_t qi = ok ? (s.q0 + p.div.of(r)) * p.q_tok + (h * p.group + p.div.rest(r)) * p.q_head + (D / 4) * t : 0;
       float v[D / 4];
       uint32_t mx = 0;
       if (ok && p.q_vec) {
@@ -361,7 +375,7 @@ __global__ void __launch_bounds__(kRowsThreads, rows_ctas(D, NT)) kv4_rows_kerne
         qs[n][i] = __shfl_sync(0xffffffffu, up, (2 * t + i) * 4);
         qsum[n][i] = __shfl_sync(0xffffffffu, sum, (2 * t + i) * 4);
         const int rr = r0 + n * 8 + 2 * t + i;
-        lim[n][i] = rr >= rows_all ? 0 : p.causal ? min(s.len, s.p0 + rr / p.group + 1) : s.len;   // keys below it are seen
+        lim[n][i] = rr >= rows_all ? 0 : p.causal ? min(s.len, s.p0 + p.div.of(rr) + 1) : s.len;   // keys below it are seen
         if (rr < rows_all) lim_min = min(lim_min, lim[n][i]);
       }
     }
@@ -637,7 +651,7 @@ __global__ void __launch_bounds__(kRowsThreads, rows_ctas(D, NT)) kv4_rows_kerne
           for (int d = 0; d < D / 16; d += 2) dst[d / 2] = make_float4(o[n][d][i], o[n][d][2 + i], o[n][d + 1][i], o[n][d + 1][2 + i]);
           if (g == 0) part[R * D + r] = mx[n][i], part[R * D + R + r] = l[n][i];
         } else if (rr < rows_all) {
-          const int64_t oi = int64_t(s.q0 + rr / p.group) * p.hq + h * p.group + rr % p.group;
+          const int64_t oi = int64_t(s.q0 + p.div.of(rr)) * p.hq + h * p.group + p.div.rest(rr);
           const float inv = l[n][i] == 0.f ? 0.f : 1.f / l[n][i];
           uint16_t* dst = p.o + oi * D + (D / 8) * g;
           uint32_t w[D / 16];
@@ -702,7 +716,7 @@ __global__ void __launch_bounds__(D) kv4_join_kernel(Kv4RowsParams p) {
   float acc = 0.f;
 #pragma unroll 8
   for (int i = 0; i < pieces; ++i) acc += piece(i)[r * D + threadIdx.x] * wt[i];
-  const int64_t oi = int64_t(s.q0 + rr / p.group) * p.hq + h * p.group + rr % p.group;
+  const int64_t oi = int64_t(s.q0 + p.div.of(rr)) * p.hq + h * p.group + p.div.rest(rr);
   st_o(p, oi * D + threadIdx.x, sum == 0.f ? 0.f : acc / sum);
   if (p.lse && threadIdx.x == 0) p.lse[oi] = sum == 0.f ? -INFINITY : (mx + log2f(sum)) * 0.69314718055994531f;
 }

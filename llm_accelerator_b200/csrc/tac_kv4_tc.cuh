@@ -9,16 +9,20 @@
 //   warps 8..11       unpack the tile's keys, a thread a key, into the
 //                     swizzled layout that the MMAs read
 //   warp 12           issues the MMAs: S = Q C^T (FP16), O += P V
-//   warps 13..15      unpack its values, a thread half a key at a time
-// While one group does its softmax the tensor core works for the other: per
+//   warps 16..23      unpack its values, a thread half a key (13..15 idle)
+// S, P and the MMAs go in steps of 64 keys, two steps in flight for each
+// group: while a group's threads are at one step's softmax the tensor core
+// does P V of the step before and S of the step after it.  (Whole tiles of 128
+// keys, one S a group, left a group's threads and the tensor core waiting for
+// each other: 353 us for the ragged chunks of which this takes LATER.)  Per
 // tile and group D = 128 needs 1024 tensor clocks, and 1024 clocks of the
 // exponential unit.
 //
 // S comes from whole numbers (codes less zero point, exact in FP16) and the
 // FP16 query scaled by a power of two for each row; the keys' scales multiply
 // it in float32.  V is rounded once to the query's type, P as well.
-// TMEM: S of both groups (128 columns each; P takes the first half of its S),
-// then O of both.
+// TMEM: two S of each group (64 columns; P takes the first half of its S), then
+// O of both.
 #pragma once
 #include "tac_kv4_rows.cuh"
 
@@ -28,9 +32,9 @@ enum Kv4TcFault : int { KV4_TIMEOUT_TILE = 21, KV4_TIMEOUT_S = 22, KV4_TIMEOUT_P
 
 constexpr int kTcKeys = 128;
 constexpr int kTcRows = 256;
-constexpr int kTcThreads = 16 * 32;
-// Registers a thread: 128 at launch, then shared out by warpgroup (rows, rows, keys, MMA and values: their sum is 4 * 128).
-constexpr int kTcRegsRows = 184, kTcRegsUnpack = 72;
+constexpr int kTcThreads = 24 * 32;
+// Registers a thread: 80 at launch, then shared out by warpgroup (two of rows, four others: 2 * 144 + 4 * 48 = 6 * 80).
+constexpr int kTcRegsRows = 144, kTcRegsRest = 48;
 
 __host__ __device__ constexpr int tc_tile_bytes(int D) { return kTcKeys * D * 2; }
 // Q of two groups, two K tiles, two V tiles
@@ -195,7 +199,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv4_tc_kernel(Kv4TcParams pp) {
   constexpr int W = D / 8;                       // words of codes a key
   constexpr int kTile = tc_tile_bytes(D);
   extern __shared__ uint8_t dyn_smem[];
-  __shared__ __align__(8) uint64_t q_full, k_full[2], k_empty[2], ks_full[4], v_full[2], v_empty[2], s_full[2], p_full[2], o_full;
+  __shared__ __align__(8) uint64_t q_full, k_full[2], k_empty[2], ks_full[4], v_full[2], v_empty[2], s_full[2][2], p_full[2][2], pv_done[2], o_full;
   __shared__ uint32_t tmem_base;
   __shared__ int abort_flag;
   // scale and presence of a tile's keys; a slot is written again when both groups are past the tile after it
@@ -230,7 +234,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv4_tc_kernel(Kv4TcParams pp) {
   const int rows_all = s.n * p.group, r0 = blk * kTcRows;
   const int r_last = min(rows_all, r0 + kTcRows) - 1;
   const int groups = rows_all - r0 > 128 ? 2 : 1;
-  const int key_end = max(0, p.causal ? min(s.len, s.p0 + r_last / p.group + 1) : s.len);
+  const int key_end = max(0, p.causal ? min(s.len, s.p0 + p.div.of(r_last) + 1) : s.len);
   const int tiles = (key_end + kTcKeys - 1) / kTcKeys;
 
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(dyn_smem) + 1023) & ~uintptr_t(1023));
@@ -239,11 +243,14 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv4_tc_kernel(Kv4TcParams pp) {
     sm100::mbar_init(&q_full, 4 * groups);   // a warp each of those that write
     for (int i = 0; i < 2; ++i) {
       sm100::mbar_init(&k_full[i], 4);
-      sm100::mbar_init(&v_full[i], 3);
-      sm100::mbar_init(&p_full[i], 4);
+      sm100::mbar_init(&v_full[i], 8);
+      for (int j = 0; j < 2; ++j) {
+        sm100::mbar_init(&p_full[i][j], 4);
+        sm100::mbar_init(&s_full[i][j], 1);
+      }
+      sm100::mbar_init(&pv_done[i], 1);
       sm100::mbar_init(&k_empty[i], 1);
       sm100::mbar_init(&v_empty[i], 1);
-      sm100::mbar_init(&s_full[i], 1);
     }
     sm100::mbar_init(&o_full, 1);
     for (int i = 0; i < 4; ++i) sm100::mbar_init(&ks_full[i], 4);
@@ -258,60 +265,68 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv4_tc_kernel(Kv4TcParams pp) {
   volatile int* abort_v = &abort_flag;
   // After a wait that ran out nothing waits any more (and no MMA is issued): the CTA runs to its end.
   auto wait = [&](uint64_t* bar, uint32_t parity, int code) {
+    if (sm100::mbar_try_wait(bar, parity)) return;
     if (!*abort_v && !sm100::mbar_wait(bar, parity, pp.fault, code)) *abort_v = 1;
   };
 
   const int32_t* table = p.s.table + int64_t(b) * p.s.width;
-  // row of the cache that holds key `key` of tile i, -1 where none does
-  auto row_of = [&](int i, int key) -> int64_t {
+  // row of the cache that holds key `key` of tile i, kNone where none does
+  constexpr uint32_t kNone = 0xffffffffu;        // no row: there are fewer than 2^32
+  auto row_of = [&](int i, int key) -> uint32_t {
     const int pos = i * kTcKeys + key;
-    if (i >= tiles || pos >= s.len) return -1;
+    if (i >= tiles || pos >= s.len) return kNone;
     const int pg = __ldg(table + (pos >> p.c.page_shift));
-    if (uint32_t(pg) >= uint32_t(p.c.num_pages)) return -1;
-    return int64_t(uint32_t(pg) * p.c.heads + h) * p.c.page_size + (pos & (p.c.page_size - 1));
+    if (uint32_t(pg) >= uint32_t(p.c.num_pages)) return kNone;
+    return (uint32_t(pg) * p.c.heads + h) * p.c.page_size + (pos & (p.c.page_size - 1));
   };
-  if (warp == 12) {
+  if (warp >= 12 && warp < 16) {
     // ---- MMA issue: the whole warp runs these loops and one elected lane issues, so that descriptors stay in uniform
     // registers ----
-    regs_down<kTcRegsUnpack>();
-    if (tiles) {
-      constexpr uint32_t kIdS = tc_idesc(kTcKeys, false, false), kIdO = tc_idesc(D, BF16, true);
+    regs_down<kTcRegsRest>();
+    if (warp == 12 && tiles) {
+      constexpr uint32_t kIdS = tc_idesc(64, false, false), kIdO = tc_idesc(D, BF16, true);
       // K-major rows of 128 bytes (64 values), blocks of 64 values 16 KB apart
       const uint64_t qd = sm100::smem_desc_sw128(sm100::smem_u32(q_sm), 16, 1024), kd = sm100::smem_desc_sw128(sm100::smem_u32(k_sm), 16, 1024);
       // MN-major: a key's 64 values a row of 128 bytes, 8 keys 1024 bytes, blocks of 64 values 16 KB apart
       const uint64_t vd = sm100::smem_desc_sw128(sm100::smem_u32(v_sm), kTcKeys * 128, 1024);
-      auto qk = [&](int i, int g) {
-        const uint64_t qg = qd + g * (kTile >> 4), ki = kd + (i & 1) * (kTile >> 4);
+      const int steps = 2 * tiles;
+      auto qk = [&](int j, int g) {              // S of step j: 64 keys are 8 KB of each block
+        const uint64_t qg = qd + g * (kTile >> 4), ki = kd + ((j >> 1) & 1) * (kTile >> 4) + (j & 1) * (8192 >> 4);
         if (!*abort_v && sm100::elect_one()) {
 #pragma unroll
           for (int k = 0; k < D / 16; ++k) {
             const uint32_t o = ((k >> 2) * (kTcKeys * 128) + (k & 3) * 32) >> 4;
-            mma_f16_ss(tmem + g * 128, qg + o, ki + o, kIdS, k != 0);
+            mma_f16_ss(tmem + g * 128 + (j & 1) * 64, qg + o, ki + o, kIdS, k != 0);
           }
-          sm100::mma_commit(&s_full[g]);
-          if (g == groups - 1) sm100::mma_commit(&k_empty[i & 1]);
+          sm100::mma_commit(&s_full[g][j & 1]);
+          if ((j & 1) && g == groups - 1) sm100::mma_commit(&k_empty[(j >> 1) & 1]);
         }
         __syncwarp();
       };
       wait(&q_full, 0, KV4_TIMEOUT_TILE);
       wait(&k_full[0], 0, KV4_TIMEOUT_TILE);
       sm100::tc_fence_after();
-      for (int g = 0; g < groups; ++g) qk(0, g);
-      for (int i = 0; i < tiles; ++i) {
-        wait(&v_full[i & 1], (i >> 1) & 1, KV4_TIMEOUT_TILE);
-        if (i + 1 < tiles) wait(&k_full[(i + 1) & 1], ((i + 1) >> 1) & 1, KV4_TIMEOUT_TILE);
-        const uint64_t vi = vd + (i & 1) * (kTile >> 4);
+      for (int j = 0; j < 2; ++j)
+        for (int g = 0; g < groups; ++g) qk(j, g);
+      for (int j = 0; j < steps; ++j) {
+        if (!(j & 1)) {
+          const int i = j >> 1;
+          wait(&v_full[i & 1], (i >> 1) & 1, KV4_TIMEOUT_TILE);
+          if (i + 1 < tiles) wait(&k_full[(i + 1) & 1], ((i + 1) >> 1) & 1, KV4_TIMEOUT_TILE);
+        }
+        const uint64_t vi = vd + ((j >> 1) & 1) * (kTile >> 4) + (j & 1) * (4 * 2048 >> 4);
         for (int g = 0; g < groups; ++g) {
-          wait(&p_full[g], i & 1, KV4_TIMEOUT_P);
+          wait(&p_full[g][j & 1], (j >> 1) & 1, KV4_TIMEOUT_P);
           sm100::tc_fence_after();
           if (!*abort_v && sm100::elect_one()) {
 #pragma unroll
-            for (int k = 0; k < kTcKeys / 16; ++k)
-              mma_f16_ts(tmem + 256 + g * 128, tmem + g * 128 + k * 8, vi + k * (2048 >> 4), kIdO, i || k);
-            if (g == groups - 1) sm100::mma_commit(&v_empty[i & 1]);
+            for (int k = 0; k < 4; ++k)
+              mma_f16_ts(tmem + 256 + g * 128, tmem + g * 128 + (j & 1) * 64 + k * 8, vi + k * (2048 >> 4), kIdO, j || k);
+            sm100::mma_commit(&pv_done[g]);
+            if ((j & 1) && g == groups - 1) sm100::mma_commit(&v_empty[(j >> 1) & 1]);
           }
           __syncwarp();
-          if (i + 1 < tiles) qk(i + 1, g);
+          if (j + 2 < steps) qk(j + 2, g);
         }
       }
       if (sm100::elect_one()) sm100::mma_commit(&o_full);
@@ -319,76 +334,63 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv4_tc_kernel(Kv4TcParams pp) {
       // every MMA has ended before TMEM is freed, also after a failed wait
       sm100::mbar_wait(&o_full, 0, pp.fault, KV4_TIMEOUT_DRAIN);
     }
-  } else if (warp > 12) {
-    // ---- values: s (c - z), rounded once; items of half a key, thread t takes t, t + 96, t + 192 ----
-    regs_down<kTcRegsUnpack>();
-    constexpr int H = W / 2, kItems = 3;
-    const int t = threadIdx.x - 13 * 32;
-    uint4 cw[kItems][H / 4];
-    uint32_t vp[kItems] = {};
-    int64_t row[kItems], row1[kItems];
-    auto load = [&](int j) {
-      if (row[j] < 0) return;
-      const uint4* src = reinterpret_cast<const uint4*>(p.c.vc + row[j] * (D / 2) + ((t + 96 * j) >> 7) * (D / 4));
+  } else if (warp >= 16) {
+    // ---- values: s (c - z), rounded once; thread = half of a key's ----
+    regs_down<kTcRegsRest>();
+    constexpr int H = W / 2;
+    const int key = threadIdx.x & 127, half = (threadIdx.x >> 7) & 1;
+    uint4 cw[H / 4];
+    uint32_t vp = 0;
+    auto load = [&](uint32_t row) {
+      if (row == kNone) return;
+      const uint4* src = reinterpret_cast<const uint4*>(p.c.vc + uint64_t(row) * (D / 2) + half * (D / 4));
 #pragma unroll
-      for (int w = 0; w < H / 4; ++w) cw[j][w] = __ldg(src + w);
-      vp[j] = __ldg(p.c.vp + row[j]);
+      for (int w = 0; w < H / 4; ++w) cw[w] = __ldg(src + w);
+      vp = __ldg(p.c.vp + row);
     };
-    auto row_item = [&](int i, int j) { return t + 96 * j < 256 ? row_of(i, (t + 96 * j) & 127) : int64_t(-1); };
-#pragma unroll
-    for (int j = 0; j < kItems; ++j) row[j] = row_item(0, j), row1[j] = row_item(1, j);
-#pragma unroll
-    for (int j = 0; j < kItems; ++j) load(j);
+    uint32_t row = row_of(0, key), row1 = row_of(1, key);
+    load(row);
     for (int i = 0; i < tiles; ++i) {
       uint8_t* const dst = v_sm + (i & 1) * kTile;
       wait(&v_empty[i & 1], ((i >> 1) & 1) ^ 1, KV4_TIMEOUT_TILE);
+      const float vs = kv4_scale(vp);
+      if (row == kNone || vs != vs) {
 #pragma unroll
-      for (int j = 0; j < kItems; ++j) {
-        const int item = t + 96 * j, key = item & 127, first = (item >> 7) * H;
-        if (item >= 256) continue;
-        const float vs = kv4_scale(vp[j]);
-        if (row[j] < 0 || vs != vs) {
-#pragma unroll
-          for (int w = 0; w < H; ++w)
-            *reinterpret_cast<uint4*>(dst + ((first + w) >> 3) * (kTcKeys * 128) + sw128(key, (first + w) & 7)) = make_uint4(0, 0, 0, 0);
-        } else if (BF16) {
-          tc_unpack<H, UNPACK_BF16>(dst, key, first, cw[j], vp[j] & 15u, vs);
-        } else if (vs >= 0x1p-17f && vs < 65504.f) {
-          tc_unpack<H, UNPACK_F16>(dst, key, first, cw[j], vp[j] & 15u, vs);
-        } else {
-          tc_unpack<H, UNPACK_F32>(dst, key, first, cw[j], vp[j] & 15u, vs);
-        }
+        for (int w = half * H; w < half * H + H; ++w)
+          *reinterpret_cast<uint4*>(dst + (w >> 3) * (kTcKeys * 128) + sw128(key, w & 7)) = make_uint4(0, 0, 0, 0);
+      } else if (BF16) {
+        tc_unpack<H, UNPACK_BF16>(dst, key, half * H, cw, vp & 15u, vs);
+      } else if (vs >= 0x1p-17f && vs < 65504.f) {
+        tc_unpack<H, UNPACK_F16>(dst, key, half * H, cw, vp & 15u, vs);
+      } else {
+        tc_unpack<H, UNPACK_F32>(dst, key, half * H, cw, vp & 15u, vs);
       }
       sm100::fence_proxy_async();
       __syncwarp();
       if (lane == 0) sm100::mbar_arrive(&v_full[i & 1]);
-      // after the fence, which would wait for them
-#pragma unroll
-      for (int j = 0; j < kItems; ++j) row[j] = row1[j];
-#pragma unroll
-      for (int j = 0; j < kItems; ++j) load(j);
-#pragma unroll
-      for (int j = 0; j < kItems; ++j) row1[j] = row_item(i + 2, j);
+      load(row1);                                // after the fence, which would wait for it
+      row = row1;
+      row1 = row_of(i + 2, key);
     }
   } else if (warp >= 8) {
     // ---- keys: c - z; thread = key of the tile ----
-    regs_down<kTcRegsUnpack>();
+    regs_down<kTcRegsRest>();
     const int key = threadIdx.x & 127;
     uint4 cw[W / 4];
     uint32_t kp = 0, vp = 0;
-    auto load = [&](int64_t row) {
-      if (row < 0) return;
-      const uint4* src = reinterpret_cast<const uint4*>(p.c.kc + row * (D / 2));
+    auto load = [&](uint32_t row) {
+      if (row == kNone) return;
+      const uint4* src = reinterpret_cast<const uint4*>(p.c.kc + uint64_t(row) * (D / 2));
 #pragma unroll
       for (int w = 0; w < W / 4; ++w) cw[w] = __ldg(src + w);
       kp = __ldg(p.c.kp + row);
       vp = __ldg(p.c.vp + row);
     };
-    int64_t row = row_of(0, key), row1 = row_of(1, key);
+    uint32_t row = row_of(0, key), row1 = row_of(1, key);
     load(row);
     for (int i = 0; i < tiles; ++i) {
       wait(&k_empty[i & 1], ((i >> 1) & 1) ^ 1, KV4_TIMEOUT_TILE);
-      const bool here = row >= 0;
+      const bool here = row != kNone;
       const float vs = kv4_scale(vp);
       // a row of NaN, of K or of V, reaches the rows that see it through their scores
       ks_s[i & 3][key] = !here ? 0.f : vs != vs ? vs : kv4_scale(kp);
@@ -424,7 +426,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv4_tc_kernel(Kv4TcParams pp) {
           const int r = r0 + warp * 32 + j * R + lane / L;
           qw[j] = make_uint4(0, 0, 0, 0);
           if (r < rows_all) {
-            const uint16_t* src = p.q + (s.q0 + r / p.group) * p.q_tok + (h * p.group + r % p.group) * p.q_head + c * 8;
+            const uint16_t* src = p.q + (s.q0 + p.div.of(r)) * p.q_tok + (h * p.group + p.div.rest(r)) * p.q_head + c * 8;
             if (p.q_vec) {
               qw[j] = __ldg(reinterpret_cast<const uint4*>(src));
             } else {
@@ -463,43 +465,42 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv4_tc_kernel(Kv4TcParams pp) {
       __syncwarp();                              // rf_s: a warp reads what it wrote
       if (lane == 0) sm100::mbar_arrive(&q_full);
       const float rf = rf_s[g * 128 + row];
-      const int lim = ok ? (p.causal ? min(s.len, s.p0 + rr / p.group + 1) : s.len) : 0;
+      const int lim = ok ? (p.causal ? min(s.len, s.p0 + p.div.of(rr) + 1) : s.len) : 0;
       const uint32_t lanes = uint32_t((warp & 3) * 32) << 16, t_s = tmem + lanes + g * 128, t_o = tmem + lanes + 256 + g * 128;
       float mu = 0.f, l = 0.f;
       bool begun = false;
 
-      auto tile = [&](int i, auto masked_c) {
+      auto step = [&](int j, auto masked_c) {
         constexpr bool kMasked = decltype(masked_c)::value;
-        const ulonglong2* ks = reinterpret_cast<const ulonglong2*>(ks_s[i & 3]);
-        uint32_t v[kTcKeys];
-#pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_ld32_start(t_s + c * 32, v + c * 32);
-#pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_landed(v + c * 32);
+        const int slot = (j >> 1) & 3, key0 = j * 64;
+        const uint32_t t_sj = t_s + (j & 1) * 64;
+        const ulonglong2* ks = reinterpret_cast<const ulonglong2*>(ks_s[slot] + (j & 1) * 64);
+        uint32_t v[64];
+        tmem_ld32_start(t_sj, v);
+        tmem_ld32_start(t_sj + 32, v + 32);
+        tmem_landed(v);
+        tmem_landed(v + 32);
         // scores, but for the row's factor
-        uint64_t y[kTcKeys / 2];
+        uint64_t y[32];
         float top4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int j = 0; j < kTcKeys / 4; ++j) {
-          const ulonglong2 k4 = ks[j];
-          y[2 * j] = mul2(pack2(__uint_as_float(v[4 * j]), __uint_as_float(v[4 * j + 1])), k4.x);
-          y[2 * j + 1] = mul2(pack2(__uint_as_float(v[4 * j + 2]), __uint_as_float(v[4 * j + 3])), k4.y);
+        for (int q = 0; q < 16; ++q) {
+          const ulonglong2 k4 = ks[q];
+          y[2 * q] = mul2(pack2(__uint_as_float(v[4 * q]), __uint_as_float(v[4 * q + 1])), k4.x);
+          y[2 * q + 1] = mul2(pack2(__uint_as_float(v[4 * q + 2]), __uint_as_float(v[4 * q + 3])), k4.y);
+          float f[4];
+          unpack2(y[2 * q], f[0], f[1]);
+          unpack2(y[2 * q + 1], f[2], f[3]);
           if (kMasked) {
-            const uint32_t present = present_s[i & 3][j / 8];
-            float f[4];
-            unpack2(y[2 * j], f[0], f[1]);
-            unpack2(y[2 * j + 1], f[2], f[3]);
+            const uint32_t present = present_s[slot][(j & 1) * 2 + q / 8];
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-              if (!(i * kTcKeys + 4 * j + e < lim && (present >> (4 * (j % 8) + e) & 1))) f[e] = -INFINITY;
-            y[2 * j] = pack2(f[0], f[1]);
-            y[2 * j + 1] = pack2(f[2], f[3]);
+              if (!(key0 + 4 * q + e < lim && (present >> (4 * (q % 8) + e) & 1))) f[e] = -INFINITY;
+            y[2 * q] = pack2(f[0], f[1]);
+            y[2 * q + 1] = pack2(f[2], f[3]);
           }
-          float f[4];
-          unpack2(y[2 * j], f[0], f[1]);
-          unpack2(y[2 * j + 1], f[2], f[3]);
-          top4[(2 * j) & 3] = max3(top4[(2 * j) & 3], f[0], f[1]);
-          top4[(2 * j + 1) & 3] = max3(top4[(2 * j + 1) & 3], f[2], f[3]);
+          top4[(2 * q) & 3] = max3(top4[(2 * q) & 3], f[0], f[1]);
+          top4[(2 * q + 1) & 3] = max3(top4[(2 * q + 1) & 3], f[2], f[3]);
         }
         const float mx = fmaxf(max3(top4[0], top4[1], top4[2]), top4[3]);
         const float top = mx == -INFINITY ? -INFINITY : mx * rf;
@@ -513,13 +514,16 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv4_tc_kernel(Kv4TcParams pp) {
             begun = true;
           }
           l *= corr;
-          if (i) {                               // P V of the tiles before has ended: it was issued before this S
+          if (j) {
+            wait(&pv_done[g], (j - 1) & 1, KV4_TIMEOUT_S);   // P V of the step before; the next one waits for this step's P
+            __syncwarp();
+            sm100::tc_fence_after();
 #pragma unroll 1
             for (int c = 0; c < D / 16; ++c) {
               uint32_t u[16];
               tmem_ld16(t_o + c * 16, u);
 #pragma unroll
-              for (int j = 0; j < 16; ++j) u[j] = __float_as_uint(__uint_as_float(u[j]) * corr);
+              for (int k = 0; k < 16; ++k) u[k] = __float_as_uint(__uint_as_float(u[k]) * corr);
               tmem_st16(t_o + c * 16, u);
             }
           }
@@ -527,32 +531,32 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv4_tc_kernel(Kv4TcParams pp) {
         const uint64_t rf2 = pack2(rf, rf), mu2 = pack2(-mu, -mu);
         uint64_t sum2[2] = {0, 0};
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
+        for (int c = 0; c < 2; ++c) {
           uint32_t w[16];
           float x[32];
 #pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            unpack2(fma2(y[16 * c + j], rf2, mu2), x[2 * j], x[2 * j + 1]);
+          for (int k = 0; k < 16; ++k) {
+            unpack2(fma2(y[16 * c + k], rf2, mu2), x[2 * k], x[2 * k + 1]);
             if (kMasked) {                       // a row of factor 0 must not turn -inf into a NaN
               float ya, ye;
-              unpack2(y[16 * c + j], ya, ye);
-              x[2 * j] = ya == -INFINITY ? -INFINITY : x[2 * j];
-              x[2 * j + 1] = ye == -INFINITY ? -INFINITY : x[2 * j + 1];
+              unpack2(y[16 * c + k], ya, ye);
+              x[2 * k] = ya == -INFINITY ? -INFINITY : x[2 * k];
+              x[2 * k + 1] = ye == -INFINITY ? -INFINITY : x[2 * k + 1];
             }
           }
 #pragma unroll
-          for (int j = 0; j < 32; ++j) x[j] = exp2_(x[j]);
+          for (int k = 0; k < 32; ++k) x[k] = exp2_(x[k]);
 #pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            sum2[j & 1] = add2(sum2[j & 1], pack2(x[2 * j], x[2 * j + 1]));
+          for (int k = 0; k < 16; ++k) {
+            sum2[k & 1] = add2(sum2[k & 1], pack2(x[2 * k], x[2 * k + 1]));
             if (BF16) {
-              const __nv_bfloat162 r = __floats2bfloat162_rn(x[2 * j], x[2 * j + 1]);
-              w[j] = *reinterpret_cast<const uint32_t*>(&r);
+              const __nv_bfloat162 r = __floats2bfloat162_rn(x[2 * k], x[2 * k + 1]);
+              w[k] = *reinterpret_cast<const uint32_t*>(&r);
             } else {
-              w[j] = h2_u(__floats2half2_rn(x[2 * j], x[2 * j + 1]));
+              w[k] = h2_u(__floats2half2_rn(x[2 * k], x[2 * k + 1]));
             }
           }
-          tmem_st16(t_s + c * 16, w);            // over S columns that have been read
+          tmem_st16(t_sj + c * 16, w);           // over S columns that have been read
         }
         float a, e;
         unpack2(add2(sum2[0], sum2[1]), a, e);
@@ -560,18 +564,22 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv4_tc_kernel(Kv4TcParams pp) {
         tmem_wait_st();
         sm100::tc_fence_before();
         __syncwarp();
-        if (lane == 0) sm100::mbar_arrive(&p_full[g]);
+        if (lane == 0) sm100::mbar_arrive(&p_full[g][j & 1]);
       };
       for (int i = 0; i < tiles; ++i) {
         // ks_s, present_s: their slot is not filled again before this group is past the tile, so its barrier cannot
         // run a phase ahead
         wait(&ks_full[i & 3], (i >> 2) & 1, KV4_TIMEOUT_TILE);
-        wait(&s_full[g], i & 1, KV4_TIMEOUT_S);
-        __syncwarp();
-        sm100::tc_fence_after();
         const uint32_t all = present_s[i & 3][0] & present_s[i & 3][1] & present_s[i & 3][2] & present_s[i & 3][3];
-        if (__any_sync(0xffffffffu, (i + 1) * kTcKeys > lim || all != 0xffffffffu)) tile(i, std::true_type{});
-        else tile(i, std::false_type{});
+        const bool masked = __any_sync(0xffffffffu, (i + 1) * kTcKeys > lim || all != 0xffffffffu);
+#pragma unroll
+        for (int hh = 0; hh < 2; ++hh) {
+          wait(&s_full[g][hh], i & 1, KV4_TIMEOUT_S);
+          __syncwarp();
+          sm100::tc_fence_after();
+          if (masked) step(2 * i + hh, std::true_type{});
+          else step(2 * i + hh, std::false_type{});
+        }
       }
       // ---- the rows' results, through the group's Q buffer so that a row leaves in one run ----
       if (tiles) wait(&o_full, 0, KV4_TIMEOUT_S);
@@ -597,7 +605,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv4_tc_kernel(Kv4TcParams pp) {
         }
       }
       if (ok && p.lse)
-        p.lse[int64_t(s.q0 + rr / p.group) * p.hq + h * p.group + rr % p.group] =
+        p.lse[int64_t(s.q0 + p.div.of(rr)) * p.hq + h * p.group + p.div.rest(rr)] =
             l == 0.f ? -INFINITY : (mu + log2f(l)) * 0.69314718055994531f;
       __syncwarp();                              // a warp stores its own rows
       {
@@ -608,7 +616,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv4_tc_kernel(Kv4TcParams pp) {
           const int q_row = (warp & 3) * 32 + j * R + lane / L, r = r0 + g * 128 + q_row;
           if (r >= rows_all) continue;
           const uint4 w = *reinterpret_cast<const uint4*>(q_mine + (ch >> 3) * (kTcKeys * 128) + sw128(q_row, ch & 7));
-          uint16_t* dst = p.o + (int64_t(s.q0 + r / p.group) * p.hq + h * p.group + r % p.group) * D + ch * 8;
+          uint16_t* dst = p.o + (int64_t(s.q0 + p.div.of(r)) * p.hq + h * p.group + p.div.rest(r)) * D + ch * 8;
           if (p.o_vec) {
             *reinterpret_cast<uint4*>(dst) = w;
           } else {
