@@ -83,6 +83,8 @@ __device__ __forceinline__ void w8_store32(const W8Params& p, const uint32_t (&v
     uint16_t* dst = static_cast<uint16_t*>(p.y) + int64_t(m + tok) * p.N + n - (mine_first || odd_n ? 0 : 1);
     uint16_t* edge = static_cast<uint16_t*>(p.y) + int64_t(m + int(first ^ 1u)) * p.N + n;
     const int64_t step = 2 * int64_t(p.N);
+    const uint32_t has_next = lane != 31, is_edge = lane == 0 || lane == 31, edge_shift = first ? 0 : 16;
+    const uint32_t sel = tok ? 0x7632 : 0x5410;
 #pragma unroll
     for (int j = 0; j < 32; j += 4) {
       const float4 a = *reinterpret_cast<const float4*>(as + j);
@@ -103,9 +105,13 @@ __device__ __forceinline__ void w8_store32(const W8Params& p, const uint32_t (&v
           *reinterpret_cast<uint32_t*>(dst) = mine_first ? __byte_perm(mine, other, 0x5410) : __byte_perm(other, mine, 0x7632);
         } else {
           const uint32_t other = __shfl_down_sync(0xffffffffu, mine, 1);
-          const uint32_t sel = tok ? 0x7632 : 0x5410;
-          if (lane != 31) *reinterpret_cast<uint32_t*>(dst) = __byte_perm(mine, other, sel);
-          if (lane == 0 || lane == 31) *edge = uint16_t(first ? mine : mine >> 16);
+          // predicated: a branch for each costs more than the store
+          asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %2, 0;\n\t@p st.global.b32 [%0], %1;\n\t}\n" ::"l"(dst),
+                       "r"(__byte_perm(mine, other, sel)), "r"(has_next)
+                       : "memory");
+          asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %2, 0;\n\t@p st.global.b16 [%0], %1;\n\t}\n" ::"l"(edge),
+                       "h"(uint16_t(mine >> edge_shift)), "r"(is_edge)
+                       : "memory");
         }
       }
     }
@@ -280,7 +286,7 @@ struct PairCfg {
   static constexpr int kStages = 6;
   static constexpr int kStageBytes = 2 * 16384;
   static constexpr int kSmem = kStages * kStageBytes + 1024;
-  static constexpr int kEpi = 256;     // epilogue threads: two warps a quadrant of TMEM, half of the tokens each
+  static constexpr int kEpi = 512;     // epilogue threads: four warps a quadrant of TMEM, a fourth of the tokens each
   static constexpr int kThreads = 64 + kEpi;
 };
 
@@ -414,7 +420,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg::kThreads, 1
       __syncwarp();
       sm100::tc_fence_after();
 #pragma unroll 1
-      for (int c = part * 32; c < p.tn; c += 64) {
+      for (int c = part * 32; c < p.tn; c += PairCfg::kEpi / 4) {
         if (m0 + c >= p.M) break;
         uint32_t v[32];
         __syncwarp();
