@@ -5,6 +5,7 @@
 
 #include <algorithm>
 #include <cstdint>
+#include <type_traits>
 
 #include "../../include/taccel_b200.h"
 #include "tac_tmap.h"
@@ -50,11 +51,32 @@ __device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
 template <>
 __device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
 
+struct RowScale {
+  float inv, scale;
+  bool finite;
+};
+__device__ __forceinline__ RowScale row_scale(uint32_t max_bits) {
+  RowScale r;
+  r.finite = max_bits < 0x7f800000u;
+  const float t = fmaxf(__uint_as_float(max_bits), 1e-8f);
+  r.inv = r.finite ? __fdiv_rn(127.0f, t) : 0.f;
+  r.scale = r.finite ? __fdiv_rn(t, 127.0f) : __uint_as_float(0x7fc00000u);
+  return r;
+}
+
+// Lets the product that follows start early: at once when these rows leave SMs free, else when they are done (its
+// CTAs would take the registers that the rest of this grid needs).
+__device__ __forceinline__ void release_dependents(bool early) {
+  if (early == (gridDim.x <= 148)) asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
+}
+
+// Any alignment and length: two reads of the row.
 template <typename T>
 __global__ void __launch_bounds__(kQrThreads) quant_rows_kernel(const T* __restrict__ X, int64_t ldx,
                                                                 int8_t* __restrict__ Q, int ldq,
                                                                 float* __restrict__ scale, int K) {
   __shared__ uint32_t red[kQrThreads / 32];
+  release_dependents(true);
   const int64_t row = blockIdx.x;
   const T* x = X + row * ldx;
   int8_t* q = Q + row * ldq;
@@ -65,15 +87,85 @@ __global__ void __launch_bounds__(kQrThreads) quant_rows_kernel(const T* __restr
   __syncthreads();
 #pragma unroll
   for (int w = 0; w < kQrThreads / 32; ++w) mb = max(mb, red[w]);
-  const bool finite = mb < 0x7f800000u;
-  const float t = fmaxf(__uint_as_float(mb), 1e-8f);
-  const float inv = finite ? __fdiv_rn(127.0f, t) : 0.f;
-  if (threadIdx.x == 0) scale[row] = finite ? __fdiv_rn(t, 127.0f) : __uint_as_float(0x7fc00000u);
+  const RowScale r = row_scale(mb);
+  if (threadIdx.x == 0) scale[row] = r.scale;
   for (int k = threadIdx.x; k < ldq; k += kQrThreads) {
     int v = 0;
-    if (k < K && finite) v = __float2int_rn(__fmul_rn(to_f(x[k]), inv));
+    if (k < K && r.finite) v = __float2int_rn(__fmul_rn(to_f(x[k]), r.inv));
     q[k] = int8_t(v);
   }
+  release_dependents(false);
+}
+
+// 16-bit rows of whole 16-byte chunks: a row is read once, eight chunks a
+// thread at most, by one warp (K up to 2048) or four.  Bound by the bytes,
+// 2 read and 1 written a value; the rounding is one addition of 1.5 * 2^23,
+// after which the low byte is the code, and a byte permutation packs four
+// (a convert instruction a value alone took as long as the memory).
+template <typename T, int WPR>
+__global__ void __launch_bounds__(kQrThreads) quant_rows_vec_kernel(const T* __restrict__ X, int64_t ldx,
+                                                                    int8_t* __restrict__ Q, int ldq,
+                                                                    float* __restrict__ scale, int M, int K) {
+  constexpr int kChunks = 8, kLanes = 32 * WPR, kRows = kQrThreads / kLanes;
+  __shared__ uint32_t red[kQrThreads / 32];
+  release_dependents(true);
+  const int64_t row = int64_t(blockIdx.x) * kRows + threadIdx.x / kLanes;
+  const int t = threadIdx.x % kLanes, chunks = K / 8;
+  if (WPR == 1 && row >= M) return;              // a whole warp
+  const uint4* x = reinterpret_cast<const uint4*>(X + row * ldx);
+  uint4 v[kChunks];
+  uint32_t m2 = 0;
+#pragma unroll
+  for (int i = 0; i < kChunks; ++i) {
+    v[i] = make_uint4(0, 0, 0, 0);
+    if (t + i * kLanes < chunks) v[i] = __ldg(x + t + i * kLanes);
+  }
+#pragma unroll
+  for (int i = 0; i < kChunks; ++i) {
+    m2 = __vmaxu2(m2, __vmaxu2(__vmaxu2(v[i].x & 0x7fff7fffu, v[i].y & 0x7fff7fffu),
+                               __vmaxu2(v[i].z & 0x7fff7fffu, v[i].w & 0x7fff7fffu)));
+  }
+  uint32_t mb = __reduce_max_sync(0xffffffffu, max(m2 & 0xffffu, m2 >> 16));
+  if (WPR > 1) {
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = mb;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kQrThreads / 32; ++w) mb = max(mb, red[w]);
+  }
+  // a 16-bit magnitude as float32: infinities and NaN stay above every finite value
+  auto f32 = [](uint32_t h) {
+    return sizeof(T) == 2 && std::is_same<T, __half>::value ? __half2float(__ushort_as_half(uint16_t(h))) : __uint_as_float(h << 16);
+  };
+  const RowScale r = row_scale(__float_as_uint(f32(mb)) & 0x7fffffffu);
+  if (t == 0) scale[row] = r.scale;
+  auto code = [&](uint32_t h) { return __float_as_uint(__fadd_rn(__fmul_rn(f32(h & 0xffffu), r.inv), 12582912.f)); };
+  uint2* q = reinterpret_cast<uint2*>(Q + row * ldq);
+#pragma unroll
+  for (int i = 0; i < kChunks; ++i) {
+    if (t + i * kLanes >= chunks) break;
+    const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+    uint32_t o[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const uint32_t a = __byte_perm(code(w[2 * j]), code(w[2 * j] >> 16), 0x0040);
+      const uint32_t b = __byte_perm(code(w[2 * j + 1]), code(w[2 * j + 1] >> 16), 0x0040);
+      o[j] = r.finite ? __byte_perm(a, b, 0x5410) : 0u;
+    }
+    q[t + i * kLanes] = make_uint2(o[0], o[1]);
+  }
+  if (K % 16 && t == 0) q[chunks] = make_uint2(0, 0);   // the padding columns
+  release_dependents(false);
+}
+
+template <typename T>
+void quant_rows_16(const T* X, int64_t ldx, int8_t* Q, int ldq, float* scale, int M, int K, cudaStream_t st) {
+  const bool vec = K % 8 == 0 && K <= 8192 && aligned(X, 16) && (M == 1 || ldx % 8 == 0);
+  if (vec && K <= 2048)
+    quant_rows_vec_kernel<T, 1><<<(M + 3) / 4, kQrThreads, 0, st>>>(X, ldx, Q, ldq, scale, M, K);
+  else if (vec)
+    quant_rows_vec_kernel<T, 4><<<M, kQrThreads, 0, st>>>(X, ldx, Q, ldq, scale, M, K);
+  else
+    quant_rows_kernel<<<M, kQrThreads, 0, st>>>(X, ldx, Q, ldq, scale, K);
 }
 
 int launch_quant_rows(const void* X, int type, int64_t ldx, int8_t* Q, float* scale, int M, int K, cudaStream_t st) {
@@ -81,9 +173,9 @@ int launch_quant_rows(const void* X, int type, int64_t ldx, int8_t* Q, float* sc
   if (type == TAC_F32)
     quant_rows_kernel<<<M, kQrThreads, 0, st>>>(static_cast<const float*>(X), ldx, Q, ldq, scale, K);
   else if (type == TAC_F16)
-    quant_rows_kernel<<<M, kQrThreads, 0, st>>>(static_cast<const __half*>(X), ldx, Q, ldq, scale, K);
+    quant_rows_16(static_cast<const __half*>(X), ldx, Q, ldq, scale, M, K, st);
   else
-    quant_rows_kernel<<<M, kQrThreads, 0, st>>>(static_cast<const __nv_bfloat16*>(X), ldx, Q, ldq, scale, K);
+    quant_rows_16(static_cast<const __nv_bfloat16*>(X), ldx, Q, ldq, scale, M, K, st);
   return status();
 }
 
@@ -122,13 +214,15 @@ int launch_splitk(const int8_t* A, const int8_t* Bt, W8Params p, cudaStream_t st
   cfg.blockDim = dim3(kSkThreads);
   cfg.dynamicSmemBytes = std::max(p.stages * sb, part) + 1024;
   cfg.stream = st;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = 1;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = split;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = p.after_rows ? 2 : 1;
   return cudaLaunchKernelEx(&cfg, w8_splitk_kernel<YT>, tw, ta, p) == cudaSuccess ? TAC_OK : TAC_E_CUDA;
 }
 
@@ -181,8 +275,17 @@ int launch_pair(const int8_t* A, const int8_t* Bt, W8Params p, int clusters, int
   if (!map_rows(&tw, Bt, p.K, p.N, 128) || !map_rows(&ta, A, p.K, p.M, tn / 2)) return TAC_E_CUDA;
   const int64_t tiles = int64_t(pp.w_tiles) * pp.t_tiles;
   if (tiles > (1 << 30)) return TAC_E_ARGUMENT;
-  w8_pair_kernel<YT><<<2 * int(std::min<int64_t>(tiles, clusters)), PairCfg::kThreads, PairCfg::kSmem, st>>>(tw, ta, pp);
-  return status();
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(2 * int(std::min<int64_t>(tiles, clusters)));
+  cfg.blockDim = dim3(PairCfg::kThreads);
+  cfg.dynamicSmemBytes = PairCfg::kSmem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = p.after_rows ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, w8_pair_kernel<YT>, tw, ta, pp) == cudaSuccess ? TAC_OK : TAC_E_CUDA;
 }
 
 // Checks that both products share; also the limits of 32-bit sums and of the grid.
@@ -207,8 +310,9 @@ int pick_product(const int8_t* A, const int8_t* Bt, const W8Params& p, cudaStrea
 }
 
 int run_product(const int8_t* A, const int8_t* Bt, const float* a_scale, const void* b_scale, int b_type,
-                const void* bias, int bias_type, void* Y, int y_type, int M, int N, int K, cudaStream_t st) {
+                const void* bias, int bias_type, void* Y, int y_type, int M, int N, int K, bool after_rows, cudaStream_t st) {
   W8Params p{};
+  p.after_rows = after_rows;
   p.a_scale = a_scale;
   p.b_scale = b_scale;
   p.bias = bias;
@@ -240,7 +344,7 @@ extern "C" int tac_gemm_i8_scaled(const int8_t* A, const int8_t* Bt, const float
                                   int K, void* stream) {
   if (!A || !a_scale || K % 16 || !aligned(A, 16)) return TAC_E_ARGUMENT;
   if (int s = check_product(Bt, b_scale, b_scale_type, bias, bias_type, Y, y_type, M, N, K)) return s;
-  return run_product(A, Bt, a_scale, b_scale, b_scale_type, bias, bias_type, Y, y_type, M, N, K,
+  return run_product(A, Bt, a_scale, b_scale, b_scale_type, bias, bias_type, Y, y_type, M, N, K, false,
                      static_cast<cudaStream_t>(stream));
 }
 
@@ -260,5 +364,5 @@ extern "C" int tac_linear_w8a8(const void* X, int x_type, int64_t ldx, const int
   int8_t* q = static_cast<int8_t*>(workspace);
   float* s = reinterpret_cast<float*>(q + align256(uint64_t(M) * Kp));
   if (int e = launch_quant_rows(X, x_type, ldx, q, s, M, K, st)) return e;
-  return run_product(q, Bt, s, b_scale, b_scale_type, bias, bias_type, Y, y_type, M, N, Kp, st);
+  return run_product(q, Bt, s, b_scale, b_scale_type, bias, bias_type, Y, y_type, M, N, Kp, true, st);
 }

@@ -45,7 +45,10 @@ struct W8Params {
   int tn;                    // tokens of a tile
   int stages;
   int* fault;
+  int after_rows;            // launched while the row quantiser may still run: A and a_scale wait for its end
 };
+
+__device__ __forceinline__ void wait_rows() { asm volatile("griddepcontrol.wait;\n" ::: "memory"); }
 
 __device__ __forceinline__ float w8_value(int acc, float as, float bs, float bias) {
   return fmaf(__fmul_rn(__int2float_rn(acc), as), bs, bias);   // bias 0 where there is none
@@ -170,6 +173,15 @@ __global__ void __launch_bounds__(kSkThreads)
 
   if (warp == 0) {
     uint32_t s = 0, ph = 1, issued = 0;
+    // the first stages' weights need not wait for the rows
+    const int early = min(S, kb1 - kb0);
+    if (sm100::elect_one())
+      for (int i = 0; i < early; ++i) {
+        sm100::mbar_arrive_expect_tx(&full_bar[i], stage_bytes);
+        sm100::tma_load_2d(smem + i * stage_bytes, &tm_w, (kb0 + i) * 128, n0, &full_bar[i]);
+      }
+    __syncwarp();
+    wait_rows();
     for (int kb = kb0; kb < kb1; ++kb) {
       if (!sm100::mbar_wait(&empty_bar[s], ph, p.fault, W8_TIMEOUT_EMPTY) || *abort_v) {
         *abort_v = 1;
@@ -177,8 +189,10 @@ __global__ void __launch_bounds__(kSkThreads)
       }
       if (sm100::elect_one()) {
         uint8_t* st = smem + s * stage_bytes;
-        sm100::mbar_arrive_expect_tx(&full_bar[s], stage_bytes);
-        sm100::tma_load_2d(st, &tm_w, kb * 128, n0, &full_bar[s]);
+        if (kb - kb0 >= early) {
+          sm100::mbar_arrive_expect_tx(&full_bar[s], stage_bytes);
+          sm100::tma_load_2d(st, &tm_w, kb * 128, n0, &full_bar[s]);
+        }
         sm100::tma_load_2d(st + kSkWBytes, &tm_a, kb * 128, m0, &full_bar[s]);
       }
       __syncwarp();
@@ -222,6 +236,7 @@ __global__ void __launch_bounds__(kSkThreads)
       bs = ld_any(p.b_scale, p.b_type, n);
       if (p.bias) bias = ld_any(p.bias, p.bias_type, n);
     }
+    wait_rows();
     for (int i = threadIdx.x - 64; i < p.tn; i += 128) as_s[i] = m0 + i < p.M ? __ldg(p.a_scale + m0 + i) : 0.f;
     asm volatile("bar.sync 1, 128;\n" ::: "memory");   // as_s, among the epilogue's warps
     acc_ok = sm100::mbar_wait(&acc_bar, 0, p.fault, W8_TIMEOUT_ACC);
@@ -334,6 +349,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg::kThreads, 1
 
   if (warp == 0) {
     uint32_t s = 0, ph = 1, issued = 0;
+    wait_rows();
     for (int tile = cid; tile < total && !*abort_v; tile += ncl) {
       const int n0 = tile / pp.t_tiles * 256 + int(rank) * 128, m0 = tile % pp.t_tiles * p.tn + int(rank) * half;
       for (int kb = 0; kb < p.k_blocks; ++kb) {
@@ -402,6 +418,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg::kThreads, 1
     const uint32_t acc_empty0_0 = sm100::mapa_shared(&acc_empty[0], 0), acc_empty0_1 = sm100::mapa_shared(&acc_empty[1], 0);
     const int part = (warp - 2) >> 2;
     uint32_t local = 0;
+    wait_rows();
     for (int tile = cid; tile < total; tile += ncl, ++local) {
       const uint32_t b = local & 1, aph = (local >> 1) & 1;
       const int n = tile / pp.t_tiles * 256 + int(rank) * 128 + row, m0 = tile % pp.t_tiles * p.tn;
