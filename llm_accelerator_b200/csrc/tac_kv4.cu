@@ -33,7 +33,11 @@ int sm_count() {
 }
 
 // ---- append and read ------------------------------------------------------------------------------------------------
-// D / 8 lanes a row, eight values (one word of codes) a lane.
+// A CTA takes a run of tokens.  Each lane of a warp finds the place of one of
+// them (a search in indptr, the length, the page), all at once; then the
+// tokens' 2 * heads rows go by, a few lanes a row, two tokens' loads in
+// flight.  Bound by the bytes: D values in and D / 2 + 4 bytes out a row
+// (append), D / 2 + 4 in and 4 D out (read).
 constexpr int kRowThreads = 256;
 
 struct RowArgs {
@@ -43,13 +47,17 @@ struct RowArgs {
   int64_t tok[2], head[2];
   float* out[2];
   int type, vec;
+  int run;                // tokens of a CTA, at most 32
 };
 
-// Position of new token `tok` and its sequence; false where it has none.
-__device__ __forceinline__ bool token_place(const Kv4Seqs& s, int tok, int64_t cap, int& b, int64_t& pos) {
-  b = tok;
+constexpr uint32_t kNoRow = 0xffffffffu;        // there are fewer than 2^32 rows
+
+// Cache row of head 0 of new token `tok`, kNoRow where it has no place.
+__device__ __forceinline__ uint32_t token_row(const Kv4Cache& c, const Kv4Seqs& s, int tok) {
+  if (tok >= s.total) return kNoRow;
+  int b = tok;
   if (s.indptr) {
-    int lo = 0, hi = s.batch;          // the last b with indptr[b] <= tok
+    int lo = 0, hi = s.batch;                    // the last b with indptr[b] <= tok
     while (lo < hi) {
       const int mid = (lo + hi + 1) >> 1;
       if (__ldg(s.indptr + mid) <= tok) lo = mid;
@@ -57,18 +65,15 @@ __device__ __forceinline__ bool token_place(const Kv4Seqs& s, int tok, int64_t c
     }
     b = lo;
   }
-  if (b >= s.batch) return false;
+  if (b >= s.batch) return kNoRow;
+  const int64_t cap = int64_t(s.width) * c.page_size;
   const Kv4Seq q = kv4_seq(s, b, cap);
-  if (tok < q.q0 || tok >= q.q0 + q.n) return false;
-  pos = int64_t(q.p0) + (tok - q.q0);
-  return pos >= 0 && pos < cap;
-}
-
-// Index of the cache row of (b, pos, head), or -1.
-__device__ __forceinline__ int64_t cache_row(const Kv4Cache& c, const Kv4Seqs& s, int b, int64_t pos, int head) {
+  if (tok < q.q0 || tok >= q.q0 + q.n) return kNoRow;
+  const int64_t pos = int64_t(q.p0) + (tok - q.q0);
+  if (pos < 0 || pos >= cap) return kNoRow;
   const int page = __ldg(s.table + int64_t(b) * s.width + (pos >> c.page_shift));
-  if (page < 0 || page >= c.num_pages) return -1;
-  return (int64_t(page) * c.heads + head) * c.page_size + (pos & (c.page_size - 1));
+  if (uint32_t(page) >= uint32_t(c.num_pages)) return kNoRow;
+  return uint32_t(page) * c.heads * c.page_size + (uint32_t(pos) & (c.page_size - 1));
 }
 
 __device__ __forceinline__ float elem(const void* p, int type, int64_t i) {
@@ -77,98 +82,184 @@ __device__ __forceinline__ float elem(const void* p, int type, int64_t i) {
   return type == TAC_F16 ? __half2float(__ushort_as_half(u)) : __uint_as_float(uint32_t(u) << 16);
 }
 
-template <int D>
+// Codes of 16 values of a lane and the row's parameter word, from the row's
+// extremes.  SHORT: the values have 11 significant bits at most (FP16, BF16).
+template <bool SHORT>
+__device__ __forceinline__ uint2 codes16(const float (&v)[16], float lo, float hi, uint32_t& word) {
+  const float s = __bfloat162float(__float2bfloat16_rn(__fdiv_rn(__fsub_rn(hi, lo), 15.f)));
+  uint2 out = make_uint2(0, 0);
+  if (!(s <= 3.3e38f)) {                         // an infinity, a NaN or a range beyond float32: the row reads as NaN
+    word = 0x7fc00000u;
+  } else if (s == 0.f) {
+    word = 0;
+  } else if (SHORT && s >= 0x1p-100f) {
+    // x / s by one residual correction of x * (1 / s) (Markstein's): x has 11 bits at most and s 8, so x - q s is exact
+    // and the corrected q within 2^-47 of the quotient, relative; a quotient halfway between two whole numbers is
+    // representable and comes out exactly, and no other lies within 2^-13 of one.  Adding 1.5 * 2^23 rounds it to a
+    // whole number, half to even; z and the clamp are exact there.  No code is below 0: z is lo's rounding.
+    constexpr float kMagic = 12582912.f;
+    const float r = __frcp_rn(s);
+    auto quotient = [&](float x) {
+      const float q = __fmul_rn(x, r);
+      return __fmaf_rn(__fmaf_rn(-q, s, x), r, q);
+    };
+    const float z = -__fsub_rn(__fadd_rn(quotient(lo), kMagic), kMagic);
+    uint32_t acc[2] = {0, 0};                    // sum of 16^j (bits of kMagic + code)
+#pragma unroll
+    for (int j = 15; j >= 0; --j) {
+      const float c = fminf(__fadd_rn(__fadd_rn(quotient(v[j]), kMagic), z), kMagic + 15.f);
+      acc[j / 8] = acc[j / 8] * 16u + __float_as_uint(c);
+    }
+    const uint32_t off = __float_as_uint(kMagic) * 0x11111111u;
+    out = make_uint2(acc[0] - off, acc[1] - off);
+    word = __float_as_uint(s) | uint32_t(z);
+  } else {
+    const float z = fminf(rintf(__fdiv_rn(-lo, s)), 15.f);   // a subnormal s may be far from (hi - lo) / 15
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      const float c = fminf(fmaxf(rintf(__fdiv_rn(v[j], s)) + z, 0.f), 15.f);
+      (j < 8 ? out.x : out.y) |= uint32_t(c) << (4 * (j & 7));
+    }
+    word = __float_as_uint(s) | uint32_t(z);
+  }
+  return out;
+}
+
+// Extremes of packed 16-bit values; a NaN stays.
+__device__ __forceinline__ uint32_t min2(uint32_t a, uint32_t b, bool f16) {
+  uint32_t r;
+  if (f16) asm("min.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  else asm("min.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+__device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b, bool f16) {
+  uint32_t r;
+  if (f16) asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  else asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+
+// TYPE: TAC_F16 or TAC_BF16 with 16-byte aligned rows; -1: any type and alignment.
+template <int D, int TYPE>
 __global__ void __launch_bounds__(kRowThreads) kv4_append_kernel(RowArgs a) {
-  constexpr int L = D / 8;
-  const int sub = threadIdx.x % L;
-  const int64_t rows = int64_t(a.s.total) * a.c.heads * 2;
-  const int64_t cap = int64_t(a.s.width) * a.c.page_size;
-  const int64_t step = int64_t(gridDim.x) * (kRowThreads / L);
-  // whole warps stay in the loop together: its shuffles name every lane
-  for (int64_t i0 = int64_t(blockIdx.x) * (kRowThreads / L); i0 < rows; i0 += step) {
-    const int64_t i = i0 + threadIdx.x / L;
-    int64_t row = -1;
-    float v[8] = {};
-    const int which = int(i & 1);
-    if (i < rows) {
-      const int head = int((i >> 1) % a.c.heads), tok = int((i >> 1) / a.c.heads);
-      int b;
-      int64_t pos;
-      if (token_place(a.s, tok, cap, b, pos)) row = cache_row(a.c, a.s, b, pos, head);
-      if (row >= 0) {
-        const int64_t e = tok * a.tok[which] + head * a.head[which] + sub * 8;
-        if (a.vec && a.type != TAC_F32) {
-          const uint4 u = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.x[which]) + e));
-          const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+  constexpr int L = D / 16, kRows = kRowThreads / L, kPair = 2;
+  const int sub = threadIdx.x % L, lane = threadIdx.x & 31;
+  const int64_t t0 = int64_t(blockIdx.x) * a.run;
+  const uint32_t mine = lane < a.run && t0 + lane < a.s.total ? token_row(a.c, a.s, int(t0 + lane)) : kNoRow;
+  // whole warps take part in every pass: its shuffles name every lane
+  for (int r0 = 0; r0 < 2 * a.c.heads; r0 += kRows) {
+    const int r = r0 + int(threadIdx.x) / L;
+    const bool in = r < 2 * a.c.heads;
+    const int which = r >= a.c.heads, head = in ? r - (which ? a.c.heads : 0) : 0;
+    const void* src = which ? a.x[1] : a.x[0];
+    const int64_t tok = which ? a.tok[1] : a.tok[0];
+    const int64_t e0 = t0 * tok + head * (which ? a.head[1] : a.head[0]) + sub * 16;
+    uint8_t* const codes = (which ? a.c.vc : a.c.kc) + sub * 8;
+    uint32_t* const words = which ? a.c.vp : a.c.kp;
+    for (int k0 = 0; k0 < a.run; k0 += kPair) {
+      uint32_t base[kPair];
+      uint4 raw[kPair][2];
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const uint16_t h = uint16_t(w[j / 2] >> (16 * (j & 1)));
-            v[j] = a.type == TAC_F16 ? __half2float(__ushort_as_half(h)) : __uint_as_float(uint32_t(h) << 16);
+      for (int k = 0; k < kPair; ++k) {
+        base[k] = k0 + k < a.run ? __shfl_sync(0xffffffffu, mine, k0 + k) : kNoRow;
+        raw[k][0] = raw[k][1] = make_uint4(0, 0, 0, 0);
+        if (TYPE >= 0 && in && base[k] != kNoRow) {
+          const uint4* q = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(src) + e0 + (k0 + k) * tok);
+          raw[k][0] = __ldg(q);
+          raw[k][1] = __ldg(q + 1);
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < kPair; ++k) {
+        if (base[k] == kNoRow) continue;         // the whole CTA
+        float v[16] = {}, lo, hi;
+        if (TYPE >= 0) {
+          constexpr bool kF16 = TYPE == TAC_F16;
+          const uint32_t w[8] = {raw[k][0].x, raw[k][0].y, raw[k][0].z, raw[k][0].w, raw[k][1].x, raw[k][1].y, raw[k][1].z, raw[k][1].w};
+          uint32_t mn = 0, mx = 0;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) mn = min2(mn, w[j], kF16), mx = max2(mx, w[j], kF16);
+#pragma unroll
+          for (int o = 1; o < L; o <<= 1) {
+            mn = min2(mn, __shfl_xor_sync(0xffffffffu, mn, o), kF16);
+            mx = max2(mx, __shfl_xor_sync(0xffffffffu, mx, o), kF16);
           }
-        } else {
+          mn = min2(mn, mn >> 16, kF16);
+          mx = max2(mx, mx >> 16, kF16);
+          auto f32 = [](uint32_t h) { return kF16 ? __half2float(__ushort_as_half(uint16_t(h))) : __uint_as_float(h << 16); };
+          lo = f32(mn & 0xffffu);
+          hi = f32(mx & 0xffffu);
 #pragma unroll
-          for (int j = 0; j < 8; ++j) v[j] = elem(a.x[which], a.type, e + j);
+          for (int j = 0; j < 16; ++j) v[j] = f32((w[j / 2] >> (16 * (j & 1))) & 0xffffu);
+        } else {
+          bool nan = false;
+          lo = hi = 0.f;
+          if (in) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) v[j] = elem(src, a.type, e0 + (k0 + k) * tok + j);
+          }
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            lo = fminf(lo, v[j]);
+            hi = fmaxf(hi, v[j]);
+            nan |= v[j] != v[j];
+          }
+          if (nan) hi = __uint_as_float(0x7f800000u);
+#pragma unroll
+          for (int o = 1; o < L; o <<= 1) {
+            lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+            hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+          }
+        }
+        uint32_t word;
+        const uint2 c = codes16<TYPE >= 0>(v, lo, hi, word);
+        if (in) {
+          const uint64_t row = base[k] + uint32_t(head) * a.c.page_size;
+          *reinterpret_cast<uint2*>(codes + row * (D / 2)) = c;
+          if (sub == 0) words[row] = word;
         }
       }
     }
-    float lo = 0.f, hi = 0.f;
-    uint32_t mag = 0;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      lo = fminf(lo, v[j]);
-      hi = fmaxf(hi, v[j]);
-      mag = max(mag, __float_as_uint(v[j]) & 0x7fffffffu);
-    }
-#pragma unroll
-    for (int o = 1; o < L; o <<= 1) {
-      lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-      hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-      mag = max(mag, __shfl_xor_sync(0xffffffffu, mag, o));
-    }
-    if (row < 0) continue;
-    const float s = __bfloat162float(__float2bfloat16_rn(__fdiv_rn(__fsub_rn(hi, lo), 15.f)));
-    uint32_t word, codes = 0;
-    if (mag >= 0x7f800000u || s > 3.3e38f) {     // not finite: the row reads as NaN
-      word = 0x7fc00000u;
-    } else if (s == 0.f) {
-      word = 0;
-    } else {
-      const float z = fminf(rintf(__fdiv_rn(-lo, s)), 15.f);   // a subnormal s may be far from (hi - lo) / 15
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float c = fminf(fmaxf(rintf(__fdiv_rn(v[j], s)) + z, 0.f), 15.f);
-        codes |= uint32_t(c) << (4 * j);
-      }
-      word = __float_as_uint(s) | uint32_t(z);
-    }
-    reinterpret_cast<uint32_t*>((which ? a.c.vc : a.c.kc) + row * (D / 2))[sub] = codes;
-    if (sub == 0) (which ? a.c.vp : a.c.kp)[row] = word;
   }
 }
 
 template <int D>
 __global__ void __launch_bounds__(kRowThreads) kv4_read_kernel(RowArgs a) {
-  constexpr int L = D / 8;
-  const int sub = threadIdx.x % L;
-  const int64_t rows = int64_t(a.s.total) * a.c.heads * 2;
-  const int64_t cap = int64_t(a.s.width) * a.c.page_size;
-  for (int64_t i = int64_t(blockIdx.x) * (kRowThreads / L) + threadIdx.x / L; i < rows;
-       i += int64_t(gridDim.x) * (kRowThreads / L)) {
-    const int which = int(i & 1), head = int((i >> 1) % a.c.heads), tok = int((i >> 1) / a.c.heads);
-    int b;
-    int64_t pos, row = -1;
-    if (token_place(a.s, tok, cap, b, pos)) row = cache_row(a.c, a.s, b, pos, head);
-    float v[8] = {};
-    if (row >= 0) {
-      const uint32_t codes = __ldg(reinterpret_cast<const uint32_t*>((which ? a.c.vc : a.c.kc) + row * (D / 2)) + sub);
-      const uint32_t word = __ldg((which ? a.c.vp : a.c.kp) + row);
-      const float s = kv4_scale(word), z = float(word & 0xffffu);
+  constexpr int L = D / 4, kRows = kRowThreads / L, kQuad = 4;   // four values a lane: a warp writes 512 bytes in one run
+  const int sub = threadIdx.x % L, lane = threadIdx.x & 31;
+  const int64_t t0 = int64_t(blockIdx.x) * a.run;
+  const uint32_t mine = lane < a.run && t0 + lane < a.s.total ? token_row(a.c, a.s, int(t0 + lane)) : kNoRow;
+  for (int r0 = 0; r0 < 2 * a.c.heads; r0 += kRows) {
+    const int r = r0 + int(threadIdx.x) / L;
+    const bool in = r < 2 * a.c.heads;
+    const int which = r >= a.c.heads, head = in ? r - (which ? a.c.heads : 0) : 0;
+    const uint8_t* const codes = (which ? a.c.vc : a.c.kc) + sub * 2;
+    const uint32_t* const words = which ? a.c.vp : a.c.kp;
+    float* const dst = (which ? a.out[1] : a.out[0]) + (t0 * a.c.heads + head) * D + sub * 4;
+    for (int k0 = 0; k0 < a.run; k0 += kQuad) {
+      uint32_t code[kQuad], word[kQuad];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = __fmul_rn(s, float((codes >> (4 * j)) & 15u) - z);
+      for (int k = 0; k < kQuad; ++k) {
+        code[k] = word[k] = 0;                   // a row without a place reads as zeros
+        const uint32_t base = k0 + k < a.run ? __shfl_sync(0xffffffffu, mine, k0 + k) : kNoRow;
+        if (in && base != kNoRow) {
+          const uint64_t row = base + uint32_t(head) * a.c.page_size;
+          code[k] = __ldg(reinterpret_cast<const uint16_t*>(codes + row * (D / 2)));
+          word[k] = __ldg(words + row);
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < kQuad; ++k) {
+        if (!in || k0 + k >= a.run || t0 + k0 + k >= a.s.total) break;
+        const float s = kv4_scale(word[k]), z = float(word[k] & 0xffffu);
+        float4 o;
+        o.x = __fmul_rn(s, float(code[k] & 15u) - z);
+        o.y = __fmul_rn(s, float((code[k] >> 4) & 15u) - z);
+        o.z = __fmul_rn(s, float((code[k] >> 8) & 15u) - z);
+        o.w = __fmul_rn(s, float(code[k] >> 12) - z);
+        *reinterpret_cast<float4*>(dst + int64_t(k0 + k) * a.c.heads * D) = o;
+      }
     }
-    float4* dst = reinterpret_cast<float4*>(a.out[which] + (int64_t(tok) * a.c.heads + head) * D + sub * 8);
-    dst[0] = make_float4(v[0], v[1], v[2], v[3]);
-    dst[1] = make_float4(v[4], v[5], v[6], v[7]);
   }
 }
 
@@ -196,9 +287,18 @@ int take_seqs(const int32_t* table, const int32_t* lens, const int32_t* indptr, 
   return TAC_OK;
 }
 
-int rows_grid(const RowArgs& a, int D) {
-  const int64_t rows = int64_t(a.s.total) * a.c.heads * 2, per = kRowThreads / (D / 8);
-  return int(std::min<int64_t>((rows + per - 1) / per, int64_t(sm_count()) * 8));
+// Tokens of a CTA: one while every token finds an SM to itself, then as many as keep six CTAs an SM, to the lanes' 32.
+void set_run(RowArgs& a, int* grid) {
+  const int64_t ctas = int64_t(sm_count()) * 6;
+  a.run = ctas > 0 ? int(std::max<int64_t>(1, std::min<int64_t>(32, (a.s.total + ctas - 1) / ctas))) : 0;
+  *grid = a.run ? int((int64_t(a.s.total) + a.run - 1) / a.run) : 0;
+}
+
+template <int D>
+void launch_append(const RowArgs& a, int grid, cudaStream_t st) {
+  if (a.vec && a.type == TAC_F16) kv4_append_kernel<D, TAC_F16><<<grid, kRowThreads, 0, st>>>(a);
+  else if (a.vec && a.type == TAC_BF16) kv4_append_kernel<D, TAC_BF16><<<grid, kRowThreads, 0, st>>>(a);
+  else kv4_append_kernel<D, -1><<<grid, kRowThreads, 0, st>>>(a);
 }
 
 // ---- attention ------------------------------------------------------------------------------------------------------
@@ -288,11 +388,12 @@ extern "C" int tac_kv4_append(const tac_kv4_cache* cache, const int32_t* page_ta
   a.head[0] = k_head, a.head[1] = v_head;
   a.type = type;
   a.vec = aligned(K, 16) && aligned(V, 16) && (k_tok | k_head | v_tok | v_head) % 8 == 0;
-  const int grid = rows_grid(a, cache->head_dim);
+  int grid;
+  set_run(a, &grid);
   if (grid <= 0) return TAC_E_CUDA;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (cache->head_dim == 64) kv4_append_kernel<64><<<grid, kRowThreads, 0, st>>>(a);
-  else kv4_append_kernel<128><<<grid, kRowThreads, 0, st>>>(a);
+  if (cache->head_dim == 64) launch_append<64>(a, grid, st);
+  else launch_append<128>(a, grid, st);
   return status();
 }
 
@@ -303,7 +404,8 @@ extern "C" int tac_kv4_read(const tac_kv4_cache* cache, const int32_t* page_tabl
   if (int s = take_seqs(page_table, lens, indptr, batch, width, total, a.c, a.s)) return s;
   if (!K || !V || !aligned(K, 16) || !aligned(V, 16)) return TAC_E_ARGUMENT;
   a.out[0] = K, a.out[1] = V;
-  const int grid = rows_grid(a, cache->head_dim);
+  int grid;
+  set_run(a, &grid);
   if (grid <= 0) return TAC_E_CUDA;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (cache->head_dim == 64) kv4_read_kernel<64><<<grid, kRowThreads, 0, st>>>(a);
