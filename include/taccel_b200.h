@@ -360,8 +360,9 @@ int tac_gemm_i8_scaled(const int8_t* A, const int8_t* Bt, const float* a_scale, 
 /* The same product of floating-point rows, quantised in the call as
  * tac_quantize_rows_i8 does: Y = linear(X[M,K]) with Bt [N, K_pad] int8, K_pad
  * = K rounded up to 16.  A multiplier in columns K .. K_pad of Bt meets a zero.
- * Calls that share a workspace (256-byte aligned, at least
- * tac_linear_w8a8_workspace_bytes) must not overlap. */
+ * Up to 16 rows of up to 8192 columns take one launch and no workspace (the
+ * query gives 0, workspace may be null).  Calls that share a workspace
+ * (256-byte aligned, at least the queried bytes) must not overlap. */
 uint64_t tac_linear_w8a8_workspace_bytes(int M, int K);
 int tac_linear_w8a8(const void* X, int x_type, int64_t ldx, const int8_t* Bt, const void* b_scale,
                     int b_scale_type, const void* bias, int bias_type, void* Y, int y_type, void* workspace,
@@ -423,8 +424,9 @@ int tac_kv4_read(const tac_kv4_cache* cache, const int32_t* page_table, const in
  * float32 [total][q_heads] gets log sum_j exp(scale * Q . k_j).  A row that
  * sees no token gets zeros and an lse of -inf; rows of no sequence are left as
  * they are.  The workspace (256-byte aligned, at least the bytes of the query
- * below on the same device) must not be shared by calls that overlap. */
-uint64_t tac_kv4_attention_workspace_bytes(int batch, int total, int q_heads, int kv_heads, int head_dim);
+ * below; null where that gives 0) must not be shared by calls that overlap. */
+uint64_t tac_kv4_attention_workspace_bytes(int batch, int width, int page_size, int total, int q_heads, int kv_heads,
+                                           int head_dim);
 int tac_kv4_attention(const tac_kv4_cache* cache, const int32_t* page_table, const int32_t* lens,
                       const int32_t* indptr, int batch, int width, int total, const void* Q, int64_t q_tok,
                       int64_t q_head, int q_heads, int type, float scale, int causal, void* O, float* lse,

@@ -123,7 +123,7 @@ SIGNATURES = {
     "tac_linear_w8a8": (_I, [_P, _I, _I64, _P, _P, _I, _P, _I, _P, _I, _P, _U64, _I, _I, _I, _P]),
     "tac_kv4_append": (_I, [_P, _P, _P, _P, _I, _I, _I, _P, _I64, _I64, _P, _I64, _I64, _I, _P]),
     "tac_kv4_read": (_I, [_P, _P, _P, _P, _I, _I, _I, _P, _P, _P]),
-    "tac_kv4_attention_workspace_bytes": (_U64, [_I, _I, _I, _I, _I]),
+    "tac_kv4_attention_workspace_bytes": (_U64, [_I, _I, _I, _I, _I, _I, _I]),
     "tac_kv4_attention": (_I, [_P, _P, _P, _P, _I, _I, _I, _P, _I64, _I64, _I, _I, C.c_float, _I, _P, _P, _P, _U64,
                                _P]),
     "tac_quantize_weight_i8": (_I, [_P, _I, _I, _I, _P, _P, _P, _P]),

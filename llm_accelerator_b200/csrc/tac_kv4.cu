@@ -309,6 +309,14 @@ int rows_tiles(int batch, int total, int group) { return int64_t(total) * group 
 constexpr int kMaxSms = 160;
 static_assert(kMaxSms * 2 <= 1024, "kv4_join_kernel holds a weight for each CTA");
 
+// Whether CTAs share the units of long sequences.  Contexts of up to four tiles are not worth the second launch that
+// joining pieces takes.  Tiles are counted in 31 bits; a batch that could have more goes by units.
+bool rows_split(int batch, int width, int page_size, int total, int q_heads, int kv_heads, int nt) {
+  const double capacity = double(width) * page_size;
+  const double most = (double(total) * q_heads / (8 * nt) + double(batch) * kv_heads) * (capacity / kRowsTile + 1);
+  return capacity > 4 * kRowsTile && most < 2147483648.0;
+}
+
 uint64_t rows_workspace(int D, int nt) {
   const uint64_t grid = uint64_t(kMaxSms) * rows_ctas(D, nt);
   return grid * 2 * (8 * nt) * (D + 2) * sizeof(float) + grid * sizeof(int4);
@@ -317,11 +325,7 @@ uint64_t rows_workspace(int D, int nt) {
 template <int D, int NT>
 int launch_rows(Kv4RowsParams p, void* workspace, cudaStream_t st) {
   const int grid = std::min(sm_count(), kMaxSms) * rows_ctas(D, NT);
-  // Contexts of up to four tiles are not worth the second launch that joining pieces takes.
-  // Tiles are counted in 31 bits; a batch that could have more goes by units.
-  const double capacity = double(p.s.width) * p.c.page_size;
-  const double most = (double(p.s.total) * p.hq / (8 * NT) + double(p.s.batch) * p.c.heads) * (capacity / kRowsTile + 1);
-  p.split = capacity > 4 * kRowsTile && most < 2147483648.0;
+  p.split = rows_split(p.s.batch, p.s.width, p.c.page_size, p.s.total, p.hq, p.c.heads, NT);
   p.cuts = static_cast<int4*>(workspace);
   p.part = reinterpret_cast<float*>(p.cuts + grid);
   static bool smem_set[64] = {};
@@ -413,11 +417,13 @@ extern "C" int tac_kv4_read(const tac_kv4_cache* cache, const int32_t* page_tabl
   return status();
 }
 
-extern "C" uint64_t tac_kv4_attention_workspace_bytes(int batch, int total, int q_heads, int kv_heads, int head_dim) {
-  if (batch <= 0 || total <= 0 || q_heads <= 0 || kv_heads <= 0 || q_heads % kv_heads ||
+extern "C" uint64_t tac_kv4_attention_workspace_bytes(int batch, int width, int page_size, int total, int q_heads,
+                                                      int kv_heads, int head_dim) {
+  if (batch <= 0 || width <= 0 || page_size <= 0 || total <= 0 || q_heads <= 0 || kv_heads <= 0 || q_heads % kv_heads ||
       (head_dim != 64 && head_dim != 128))
     return 0;
-  const int nt = rows_tiles(batch, total, q_heads / kv_heads);
+  const int group = q_heads / kv_heads, nt = rows_tiles(batch, total, group);
+  if (use_tc(batch, total, group) || !rows_split(batch, width, page_size, total, q_heads, kv_heads, nt)) return 0;
   return rows_workspace(head_dim, nt);
 }
 
@@ -432,9 +438,9 @@ extern "C" int tac_kv4_attention(const tac_kv4_cache* cache, const int32_t* page
       q_heads % p.c.heads || q_heads > 65536 || int64_t(total) * q_heads > (int64_t(1) << 31) - 1)
     return TAC_E_ARGUMENT;
   if (!aligned(Q, 2) || !aligned(O, 2) || (lse && !aligned(lse, 4))) return TAC_E_ARGUMENT;
-  if (!workspace || !aligned(workspace, 256) ||
-      workspace_bytes < tac_kv4_attention_workspace_bytes(batch, total, q_heads, p.c.heads, cache->head_dim))
-    return TAC_E_ARGUMENT;
+  const uint64_t need =
+      tac_kv4_attention_workspace_bytes(batch, width, cache->page_size, total, q_heads, p.c.heads, cache->head_dim);
+  if (need && (!workspace || !aligned(workspace, 256) || workspace_bytes < need)) return TAC_E_ARGUMENT;
   p.q = static_cast<const uint16_t*>(Q);
   p.o = static_cast<uint16_t*>(O);
   p.lse = lse;

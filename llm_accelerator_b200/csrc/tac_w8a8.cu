@@ -35,6 +35,14 @@ int sm_count() {
   return sms[dev];
 }
 
+int* fault_word() {
+  static int* words[64] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return nullptr;
+  if (!words[dev]) words[dev] = gemm_fault_word();
+  return words[dev];
+}
+
 // ---- row quantiser --------------------------------------------------------------------------------------------------
 // t = max(max |x|, 1e-8), scale = t / 127, q = rint(x * (127 / t)) in float32;
 // a row that holds an infinity or a NaN gets the scale NaN.  The maximum is
@@ -323,9 +331,47 @@ int run_product(const int8_t* A, const int8_t* Bt, const float* a_scale, const v
   p.M = M;
   p.N = N;
   p.K = K;
-  p.fault = gemm_fault_word();
-  if (!p.fault) return TAC_E_CUDA;
+  if (!(p.fault = fault_word())) return TAC_E_CUDA;
   return y_type == TAC_F32 ? pick_product<0>(A, Bt, p, st) : y_type == TAC_F16 ? pick_product<1>(A, Bt, p, st) : pick_product<2>(A, Bt, p, st);
+}
+
+// Few rows: one launch, no workspace.
+bool few_rows(int M, int K) { return M <= kRowsMost && K <= kRowsMostK; }
+
+template <int YT>
+int launch_rows(W8RowsParams pp, const int8_t* Bt, cudaStream_t st) {
+  static bool smem_set[64] = {};
+  int dev = 0;
+  const int sms = sm_count();
+  if (!sms || cudaGetDevice(&dev) != cudaSuccess) return TAC_E_CUDA;
+  if (!smem_set[dev]) {
+    if (cudaFuncSetAttribute(w8_rows_kernel<YT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSkMaxSmem) != cudaSuccess)
+      return TAC_E_CUDA;
+    smem_set[dev] = true;
+  }
+  W8Params& p = pp.g;
+  p.tn = kRowsMost;
+  p.k_blocks = (p.K + 127) / 128;
+  const int64_t tiles = (p.N + 127) / 128;
+  int split = 1;
+  while (split < 8 && 2 * split <= p.k_blocks && tiles * split * 2 <= 2 * sms) split *= 2;
+  const int per = (p.k_blocks + split - 1) / split;
+  p.stages = std::min(per, 4);
+  CUtensorMap tw;
+  if (!map_rows(&tw, Bt, p.K, p.N, 128)) return TAC_E_CUDA;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(uint32_t(tiles), 1, split);
+  cfg.blockDim = dim3(kSkThreads);
+  cfg.dynamicSmemBytes = p.stages * kSkWBytes + per * kRowsMost * 128 + 1024;   // the partial sums (8 KB) fit the first stage
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 1;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = split;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, w8_rows_kernel<YT>, tw, pp) == cudaSuccess ? TAC_OK : TAC_E_CUDA;
 }
 
 uint64_t align256(uint64_t v) { return (v + 255) & ~uint64_t(255); }
@@ -349,18 +395,29 @@ extern "C" int tac_gemm_i8_scaled(const int8_t* A, const int8_t* Bt, const float
 }
 
 extern "C" uint64_t tac_linear_w8a8_workspace_bytes(int M, int K) {
-  if (M <= 0 || K <= 0) return 0;
+  if (M <= 0 || K <= 0 || few_rows(M, K)) return 0;
   return align256(uint64_t(M) * ((uint64_t(K) + 15) / 16 * 16)) + align256(uint64_t(M) * 4);
 }
 
 extern "C" int tac_linear_w8a8(const void* X, int x_type, int64_t ldx, const int8_t* Bt, const void* b_scale,
                                int b_scale_type, const void* bias, int bias_type, void* Y, int y_type, void* workspace,
                                uint64_t workspace_bytes, int M, int N, int K, void* stream) {
-  if (!X || !type_ok(x_type) || !workspace || !aligned(workspace, 256) || (M > 1 && ldx < K)) return TAC_E_ARGUMENT;
+  if (!X || !type_ok(x_type) || (M > 1 && ldx < K)) return TAC_E_ARGUMENT;
   if (int s = check_product(Bt, b_scale, b_scale_type, bias, bias_type, Y, y_type, M, N, K)) return s;
-  if (workspace_bytes < tac_linear_w8a8_workspace_bytes(M, K)) return TAC_E_ARGUMENT;
   const int Kp = (K + 15) / 16 * 16;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (few_rows(M, K)) {
+    W8RowsParams pp{};
+    pp.g.b_scale = b_scale, pp.g.b_type = b_scale_type;
+    pp.g.bias = bias, pp.g.bias_type = bias_type;
+    pp.g.y = Y, pp.g.y_type = y_type;
+    pp.g.M = M, pp.g.N = N, pp.g.K = Kp;
+    if (!(pp.g.fault = fault_word())) return TAC_E_CUDA;
+    pp.x = X, pp.x_type = x_type, pp.ldx = ldx, pp.k_real = K;
+    pp.x_vec = x_type != TAC_F32 && aligned(X, 16) && (M == 1 || ldx % 8 == 0);
+    return y_type == TAC_F32 ? launch_rows<0>(pp, Bt, st) : y_type == TAC_F16 ? launch_rows<1>(pp, Bt, st) : launch_rows<2>(pp, Bt, st);
+  }
+  if (!workspace || !aligned(workspace, 256) || workspace_bytes < tac_linear_w8a8_workspace_bytes(M, K)) return TAC_E_ARGUMENT;
   int8_t* q = static_cast<int8_t*>(workspace);
   float* s = reinterpret_cast<float*>(q + align256(uint64_t(M) * Kp));
   if (int e = launch_quant_rows(X, x_type, ldx, q, s, M, K, st)) return e;

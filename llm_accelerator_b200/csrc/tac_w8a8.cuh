@@ -137,6 +137,53 @@ constexpr int kSkWBytes = 128 * 128;
 
 __host__ __device__ constexpr int sk_stage_bytes(int tn) { return kSkWBytes + tn * 128; }
 
+// The end of both split-K kernels: the tile's results, or the CTA's partial sums to shared memory (over its stages: every
+// copy and MMA has ended) and every nsplit-th token from all partials.  All threads of the CTA.
+template <int YT>
+__device__ __forceinline__ void w8_splitk_finish(const W8Params& p, uint8_t* smem, uint32_t tmem, const float* as_s, int warp,
+                                                 int row, int n, int m0, int rank, int nsplit, float bs, float bias,
+                                                 bool acc_ok) {
+  const uint32_t t_addr = tmem + (uint32_t((warp & 3) * 32) << 16);
+  if (nsplit == 1) {
+    if (warp >= 2 && acc_ok) {
+      for (int c = 0; c < p.tn; c += 32) {
+        uint32_t v[32];
+        __syncwarp();
+        sm100::tmem_ld32(t_addr + c, v);
+        // a tile of 16 tokens has no more than 16 rows before M
+        w8_store32<YT>(p, v, as_s + c, m0 + c, n, bs, bias);
+      }
+    }
+  } else {
+    int* part = reinterpret_cast<int*>(smem);            // [tn][128]
+    if (warp >= 2) {
+      for (int c = 0; c < p.tn; c += 32) {
+        uint32_t v[32];
+        __syncwarp();
+        sm100::tmem_ld32(t_addr + c, v);
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+          if (c + j < p.tn) part[(c + j) * 128 + row] = int(v[j]);
+      }
+    }
+    sm100::cluster_sync();
+    if (warp >= 2) {
+      for (int c = rank; c < p.tn; c += nsplit) {
+        const int m = m0 + c;
+        if (m >= p.M) break;
+        int acc = 0;
+        for (int r = 0; r < nsplit; ++r) {
+          int v;
+          asm volatile("ld.shared::cluster.s32 %0, [%1];\n" : "=r"(v) : "r"(sm100::mapa_shared(part + c * 128 + row, r)));
+          acc += v;
+        }
+        if (n < p.N) st_y<YT>(p.y, int64_t(m) * p.N + n, w8_value(acc, as_s[c], bs, bias));
+      }
+    }
+    sm100::cluster_sync();   // no CTA leaves while another reads its partial sums
+  }
+}
+
 template <int YT>
 __global__ void __launch_bounds__(kSkThreads)
     w8_splitk_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_a, W8Params p) {
@@ -243,51 +290,210 @@ __global__ void __launch_bounds__(kSkThreads)
     __syncwarp();
     sm100::tc_fence_after();
   }
-  const uint32_t t_addr = tmem + (uint32_t((warp & 3) * 32) << 16);
-  if (nsplit == 1) {
-    if (warp >= 2 && acc_ok) {
-      for (int c = 0; c < p.tn; c += 32) {
-        uint32_t v[32];
-        __syncwarp();
-        sm100::tmem_ld32(t_addr + c, v);
-        // a tile of 16 tokens has no more than 16 rows before M
-        w8_store32<YT>(p, v, as_s + c, m0 + c, n, bs, bias);
-      }
-    }
-  } else {
-    int* part = reinterpret_cast<int*>(smem);            // [tn][128], over the stages: every copy and MMA has ended
-    if (warp >= 2) {
-      for (int c = 0; c < p.tn; c += 32) {
-        uint32_t v[32];
-        __syncwarp();
-        sm100::tmem_ld32(t_addr + c, v);
-#pragma unroll
-        for (int j = 0; j < 32; ++j)
-          if (c + j < p.tn) part[(c + j) * 128 + row] = int(v[j]);
-      }
-    }
-    sm100::cluster_sync();
-    if (warp >= 2) {
-      for (int c = rank; c < p.tn; c += nsplit) {
-        const int m = m0 + c;
-        if (m >= p.M) break;
-        int acc = 0;
-        for (int r = 0; r < nsplit; ++r) {
-          int v;
-          asm volatile("ld.shared::cluster.s32 %0, [%1];\n" : "=r"(v) : "r"(sm100::mapa_shared(part + c * 128 + row, r)));
-          acc += v;
-        }
-        if (n < p.N) st_y<YT>(p.y, int64_t(m) * p.N + n, w8_value(acc, as_s[c], bs, bias));
-      }
-    }
-    sm100::cluster_sync();   // no CTA leaves while another reads its partial sums
-  }
+  w8_splitk_finish<YT>(p, smem, tmem, as_s, warp, row, n, m0, rank, nsplit, bs, bias, acc_ok);
   sm100::tc_fence_before();
   __syncthreads();
   if (warp == 1) {
     __syncwarp();
     sm100::tc_fence_after();
     sm100::tmem_dealloc(tmem, cols);
+  }
+}
+
+// ---- the same for few floating-point rows, quantised in the kernel ----------------------------------------------------
+// One launch for a decode step: while the first stages of weights are on their
+// way, the epilogue's warps take the largest magnitude of each row over this
+// CTA's K blocks, the cluster's CTAs tell each other theirs, and the rows'
+// codes go straight into the swizzled operand, which stays in shared memory.
+// A launch of its own for the quantiser costs more than reading the few rows
+// once for each 128 channels.
+constexpr int kRowsMost = 16, kRowsMostK = 8192;
+
+struct W8RowsParams {
+  W8Params g;
+  const void* x;
+  int x_type, x_vec;         // x_vec: 16-bit rows of whole 16-byte chunks
+  int64_t ldx;
+  int k_real;                // columns of x
+};
+
+__device__ __forceinline__ void load8(const W8RowsParams& p, int m, int k, float (&v)[8]) {
+  const int64_t i = m * p.ldx + k;
+  if (p.x_vec && k + 8 <= p.k_real) {
+    const uint4 u = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.x) + i));
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const uint32_t h = (w[j / 2] >> (16 * (j & 1))) & 0xffffu;
+      v[j] = p.x_type == 1 ? __half2float(__ushort_as_half(uint16_t(h))) : __uint_as_float(h << 16);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = k + j < p.k_real ? ld_any(p.x, p.x_type, i + j) : 0.f;
+  }
+}
+
+template <int YT>
+__global__ void __launch_bounds__(kSkThreads) w8_rows_kernel(const __grid_constant__ CUtensorMap tm_w, W8RowsParams pp) {
+  constexpr int kMaxStages = 8, kTn = kRowsMost;
+  const W8Params& p = pp.g;
+  extern __shared__ uint8_t dyn_smem[];
+  __shared__ __align__(8) uint64_t full_bar[kMaxStages], empty_bar[kMaxStages], acc_bar, rows_bar;
+  __shared__ uint32_t tmem_base, row_max[kTn], all_max[8][kTn];
+  __shared__ int abort_flag;
+  __shared__ __align__(16) float as_s[32];       // a chunk of the epilogue is 32 tokens wide
+
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(dyn_smem) + 1023) & ~uintptr_t(1023));
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  const int n0 = blockIdx.x * 128, nsplit = gridDim.z, rank = blockIdx.z;
+  const int kb0 = int(int64_t(p.k_blocks) * rank / nsplit), kb1 = int(int64_t(p.k_blocks) * (rank + 1) / nsplit);
+  const int S = p.stages;
+  uint8_t* const rows_sm = smem + S * kSkWBytes;  // [K block][16 rows][128 bytes], swizzled
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S; ++s) {
+      sm100::mbar_init(&full_bar[s], 1);
+      sm100::mbar_init(&empty_bar[s], 1);
+    }
+    sm100::mbar_init(&acc_bar, 1);
+    sm100::mbar_init(&rows_bar, 4);
+    abort_flag = 0;
+    sm100::mbar_fence_init();
+  }
+  if (threadIdx.x < kTn) row_max[threadIdx.x] = 0;
+  if (threadIdx.x < 32) as_s[threadIdx.x] = 0.f;
+  if (warp == 1) sm100::tmem_alloc(&tmem_base, 32);
+  sm100::tc_fence_before();
+  __syncthreads();
+  sm100::tc_fence_after();
+  const uint32_t tmem = tmem_base;
+  volatile int* abort_v = &abort_flag;
+
+  const int early = min(S, kb1 - kb0);
+  const int t = threadIdx.x - 64, per = (kb1 - kb0) * 16, items = p.M * per;   // 8-value chunks of this CTA's columns
+  if (warp == 0) {
+    if (sm100::elect_one())
+      for (int i = 0; i < early; ++i) {
+        sm100::mbar_arrive_expect_tx(&full_bar[i], kSkWBytes);
+        sm100::tma_load_2d(smem + i * kSkWBytes, &tm_w, (kb0 + i) * 128, n0, &full_bar[i]);
+      }
+    __syncwarp();
+  } else if (warp >= 2) {
+    for (int i = t; i < items; i += 128) {
+      float v[8];
+      const int m = i / per;
+      load8(pp, m, kb0 * 128 + (i - m * per) * 8, v);
+      uint32_t mb = 0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) mb = max(mb, __float_as_uint(v[j]) & 0x7fffffffu);
+      // lanes of one row first: a row has a multiple of 16 chunks
+      mb = max(mb, __shfl_xor_sync(__activemask(), mb, 1));
+      mb = max(mb, __shfl_xor_sync(__activemask(), mb, 2));
+      mb = max(mb, __shfl_xor_sync(__activemask(), mb, 4));
+      mb = max(mb, __shfl_xor_sync(__activemask(), mb, 8));
+      if ((lane & 15) == 0) atomicMax(&row_max[m], mb);
+    }
+    asm volatile("bar.sync 1, 128;\n" ::: "memory");
+    for (int i = t; i < kTn * nsplit; i += 128) {
+      const int m = i % kTn;
+      asm volatile("st.shared::cluster.u32 [%0], %1;\n" ::"r"(sm100::mapa_shared(&all_max[rank][m], i / kTn)), "r"(row_max[m]) : "memory");
+    }
+  }
+  __syncwarp();
+  if (nsplit > 1) sm100::cluster_sync();
+  else __syncthreads();
+
+  if (warp == 0) {
+    uint32_t s = 0, ph = 1, issued = 0;
+    for (int kb = kb0; kb < kb1; ++kb) {
+      if (!sm100::mbar_wait(&empty_bar[s], ph, p.fault, W8_TIMEOUT_EMPTY) || *abort_v) {
+        *abort_v = 1;
+        break;
+      }
+      if (kb - kb0 >= early && sm100::elect_one()) {
+        sm100::mbar_arrive_expect_tx(&full_bar[s], kSkWBytes);
+        sm100::tma_load_2d(smem + s * kSkWBytes, &tm_w, kb * 128, n0, &full_bar[s]);
+      }
+      __syncwarp();
+      ++issued;
+      if (++s == uint32_t(S)) s = 0, ph ^= 1;
+    }
+    // the copies still in flight land before the CTA goes on
+    for (uint32_t j = issued > uint32_t(S) ? issued - S : 0; j < issued; ++j)
+      sm100::mbar_wait(&full_bar[j % S], (j / S) & 1, p.fault, W8_TIMEOUT_DRAIN);
+  } else if (warp == 1) {
+    const uint32_t idesc = sm100::idesc_i8(128, kTn, 0);
+    const uint64_t w0 = sm100::smem_desc_sw128(sm100::smem_u32(smem), 16, 1024);
+    const uint64_t r0 = sm100::smem_desc_sw128(sm100::smem_u32(rows_sm), 16, 1024);
+    if (!sm100::mbar_wait(&rows_bar, 0, p.fault, W8_TIMEOUT_FULL)) *abort_v = 1;
+    uint32_t s = 0, ph = 0;
+    for (int kb = kb0; kb < kb1; ++kb) {
+      if (*abort_v || !sm100::mbar_wait(&full_bar[s], ph, p.fault, W8_TIMEOUT_FULL)) {
+        *abort_v = 1;
+        break;
+      }
+      sm100::tc_fence_after();
+      const uint64_t dw = w0 + s * (kSkWBytes >> 4), dr = r0 + (kb - kb0) * (kTn * 128 >> 4);
+      if (sm100::elect_one()) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) sm100::mma_i8(tmem, dw + 2 * k, dr + 2 * k, idesc, (kb > kb0) || k);
+        sm100::mma_commit(&empty_bar[s]);
+      }
+      __syncwarp();
+      if (++s == uint32_t(S)) s = 0, ph ^= 1;
+    }
+    // arrives once every MMA has completed, also after a failed wait
+    if (sm100::elect_one()) sm100::mma_commit(&acc_bar);
+    __syncwarp();
+    sm100::mbar_wait(&acc_bar, 0, p.fault, W8_TIMEOUT_DRAIN);
+  }
+  const int row = (warp & 3) * 32 + lane;
+  const int n = n0 + row;
+  float bs = 0.f, bias = 0.f;
+  bool acc_ok = false;
+  if (warp >= 2) {
+    // ---- codes of all 16 rows (zeros past M) ----
+    for (int i = t; i < kTn * per; i += 128) {
+      const int m = i / per, c = i - m * per;    // c: 8-value chunk of the row
+      uint2 codes = make_uint2(0, 0);
+      if (m < p.M) {
+        uint32_t mb = 0;
+        for (int r = 0; r < nsplit; ++r) mb = max(mb, all_max[r][m]);
+        const bool finite = mb < 0x7f800000u;
+        const float top = fmaxf(__uint_as_float(mb), 1e-8f), inv = finite ? __fdiv_rn(127.0f, top) : 0.f;
+        if (c == 0) as_s[m] = finite ? __fdiv_rn(top, 127.0f) : __uint_as_float(0x7fc00000u);
+        if (finite) {
+          float v[8];
+          load8(pp, m, kb0 * 128 + c * 8, v);
+          uint32_t b[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) b[j] = __float_as_uint(__fadd_rn(__fmul_rn(v[j], inv), 12582912.f));   // rounds; low byte = code
+          codes.x = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
+          codes.y = __byte_perm(__byte_perm(b[4], b[5], 0x0040), __byte_perm(b[6], b[7], 0x0040), 0x5410);
+        }
+      }
+      // block c / 16, 16-byte chunk (c / 2) % 8, its half c % 2
+      *reinterpret_cast<uint2*>(rows_sm + (c >> 4) * (kTn * 128) + (m >> 3) * 1024 + (m & 7) * 128 + ((((c >> 1) & 7) ^ (m & 7)) << 4) + (c & 1) * 8) = codes;
+    }
+    sm100::fence_proxy_async();
+    __syncwarp();
+    if (lane == 0) sm100::mbar_arrive(&rows_bar);
+    if (n < p.N) {
+      bs = ld_any(p.b_scale, p.b_type, n);
+      if (p.bias) bias = ld_any(p.bias, p.bias_type, n);
+    }
+    asm volatile("bar.sync 1, 128;\n" ::: "memory");   // as_s, among the epilogue's warps
+    acc_ok = sm100::mbar_wait(&acc_bar, 0, p.fault, W8_TIMEOUT_ACC);
+    __syncwarp();
+    sm100::tc_fence_after();
+  }
+  w8_splitk_finish<YT>(p, smem, tmem, as_s, warp, row, n, 0, rank, nsplit, bs, bias, acc_ok);
+  sm100::tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    __syncwarp();
+    sm100::tc_fence_after();
+    sm100::tmem_dealloc(tmem, 32);
   }
 }
 

@@ -13,6 +13,7 @@
 from __future__ import annotations
 
 from . import _lib as L
+from .w8a8 import gemm_i8_scaled, linear_w8a8, linear_workspace, pad_k16  # noqa: F401
 
 
 def _ptr(t):
@@ -111,136 +112,6 @@ def gemm_wo_f16_i8(X, Q, scale, bias=None, out=None):
     L.check(L.lib.tac_gemm_wo_f16_i8(_ptr(X), _ptr(Q), _ptr(scale), None if bias is None else _ptr(bias), _ptr(out),
                                      M, N, K, _stream()), "tac_gemm_wo_f16_i8")
     return out
-
-
-def _types():
-    import torch
-    return {torch.float32: L.TYPE_F32, torch.float16: L.TYPE_F16, torch.bfloat16: L.TYPE_BF16}
-
-
-_TYPES: dict = {}
-
-
-def _type(dtype, what):
-    """enum tac_type of a torch dtype."""
-    if not _TYPES:
-        _TYPES.update(_types())
-    try:
-        return _TYPES[dtype]
-    except KeyError:
-        raise TypeError(f"{what} must be float32, float16 or bfloat16, got {dtype}") from None
-
-
-def _on_device(device, call):
-    """call(raw stream) with `device` current: its current stream, whichever device was current before."""
-    import torch
-    index = device.index
-    if index == torch._C._cuda_getDevice():
-        return call(torch._C._cuda_getCurrentRawStream(index))
-    with torch.cuda.device(index):
-        return call(torch._C._cuda_getCurrentRawStream(index))
-
-
-def _check_scaled(rows, Bt, b_scale, bias, out, out_dtype, M, K):
-    """Checks of what gemm_i8_scaled and linear_w8a8 share; (N, out, bias pointer, bias type)."""
-    import torch
-    if Bt.dtype != torch.int8 or b_scale.dtype not in (torch.float32, torch.float16):
-        raise TypeError("Bt must be int8 and b_scale float32 or float16")
-    if Bt.dim() != 2 or Bt.shape[1] != K:
-        raise ValueError(f"Bt must be [N, {K}], got {tuple(Bt.shape)}")
-    N = Bt.shape[0]
-    if b_scale.dim() != 1 or b_scale.shape[0] != N:
-        raise ValueError(f"b_scale must be [{N}], got {tuple(b_scale.shape)}")
-    if not (Bt.is_contiguous() and b_scale.is_contiguous()):
-        raise ValueError("Bt and b_scale must be contiguous")
-    dev = rows.device
-    if dev.type != "cuda" or Bt.device != dev or b_scale.device != dev:
-        raise ValueError("the operands must be on one CUDA device")
-    bp, bt = None, 0
-    if bias is not None:
-        bt = _type(bias.dtype, "bias")
-        if bias.dim() != 1 or bias.shape[0] != N or not bias.is_contiguous() or bias.device != dev:
-            raise ValueError(f"bias must be a contiguous [{N}] tensor on the operands' device")
-        bp = bias.data_ptr()
-    if out is None:
-        out = torch.empty((M, N), dtype=out_dtype, device=dev)
-    elif out.dtype != out_dtype or tuple(out.shape) != (M, N) or not out.is_contiguous() or out.device != dev:
-        raise ValueError(f"out must be a contiguous {out_dtype} [{M}, {N}] tensor on the operands' device")
-    return N, out, bp, bt
-
-
-def gemm_i8_scaled(A, Bt, a_scale, b_scale, bias=None, out_dtype=None, out=None):
-    """Y [M, N] = (A int8 [M, K] @ Bt int8 [N, K]^T) * a_scale[m] * b_scale[n] (+ bias[n]).
-
-    a_scale float32 [M], b_scale float32 or float16 [N] (``ptq.quantize_tensor`` gives Bt and b_scale), bias and
-    output float32, float16 or bfloat16 (default: out's type, else float16).  K a multiple of 16 (pad both
-    operands with zero columns: ``pad_k16``), any M and N.  M or N of zero gives an empty result."""
-    import torch
-    if A.dtype != torch.int8 or a_scale.dtype != torch.float32:
-        raise TypeError("A must be int8 and a_scale float32")
-    if A.dim() != 2 or a_scale.dim() != 1 or a_scale.shape[0] != A.shape[0]:
-        raise ValueError(f"A must be [M, K] with a_scale [M], got {tuple(A.shape)} and {tuple(a_scale.shape)}")
-    if not (A.is_contiguous() and a_scale.is_contiguous()):
-        raise ValueError("A and a_scale must be contiguous")
-    M, K = A.shape
-    if out_dtype is None:
-        out_dtype = torch.float16 if out is None else out.dtype
-    yt = _type(out_dtype, "out_dtype")
-    if a_scale.device != A.device:
-        raise ValueError("the operands must be on one CUDA device")
-    N, out, bp, bt = _check_scaled(A, Bt, b_scale, bias, out, out_dtype, M, K)
-    if K == 0 or K % 16:
-        raise ValueError(f"K must be a positive multiple of 16, got {K} (pad_k16 pads with zero columns)")
-    if M and N:
-        L.check(_on_device(A.device, lambda st: L.lib.tac_gemm_i8_scaled(
-            A.data_ptr(), Bt.data_ptr(), a_scale.data_ptr(), b_scale.data_ptr(), _type(b_scale.dtype, ""), bp, bt,
-            out.data_ptr(), yt, M, N, K, st)), "tac_gemm_i8_scaled")
-    return out
-
-
-def pad_k16(Q):
-    """Q int8 [N, K] with zero columns appended up to a multiple of 16 (Q itself when there is nothing to add)."""
-    import torch
-    pad = -Q.shape[1] % 16
-    return torch.nn.functional.pad(Q, (0, pad)).contiguous() if pad else Q
-
-
-def linear_w8a8(X, Bt, b_scale, bias=None, out=None, ws=None):
-    """Y [M, N] in X's type = X [M, K] @ (Bt [N, K] * b_scale[n])^T (+ bias[n]) with INT8 products: each row of X is
-    quantised by its own maximum (``ptq.quantize_rows``) in the call.
-
-    X float32, float16 or bfloat16 with contiguous rows at any row stride; Bt int8 [N, K_pad], K_pad = K rounded up
-    to 16 (``pad_k16``); b_scale and bias as in ``gemm_i8_scaled``.  Rotate X first (``quarot.fwht_f16``) where the
-    weights are rotated.  ws: a ``linear_workspace`` to reuse across calls on one stream; by default a call
-    allocates its own.  A row with an infinity or a NaN gives a row of NaN."""
-    import torch
-    xt = _type(X.dtype, "X")
-    if X.dim() != 2 or (X.shape[1] > 1 and X.stride(1) != 1):
-        raise ValueError(f"X must be [M, K] with contiguous rows, got shape {tuple(X.shape)}, stride {X.stride()}")
-    M, K = X.shape
-    if K == 0:
-        raise ValueError("K must be positive")
-    ldx = X.stride(0) if M > 1 else K
-    if ldx < K:
-        raise ValueError(f"rows of X overlap (stride {ldx}, {K} columns)")
-    N, out, bp, bt = _check_scaled(X, Bt, b_scale, bias, out, X.dtype, M, (K + 15) // 16 * 16)
-    if M and N:
-        if ws is None:
-            ws = linear_workspace(M, K, X.device)
-        elif ws.device != X.device or ws.dtype != torch.uint8 or not ws.is_contiguous():
-            raise ValueError("ws must be a linear_workspace on X's device")
-        wp = (ws.data_ptr() + 255) & ~255
-        wn = ws.numel() - (wp - ws.data_ptr())
-        L.check(_on_device(X.device, lambda st: L.lib.tac_linear_w8a8(
-            X.data_ptr(), xt, ldx, Bt.data_ptr(), b_scale.data_ptr(), _type(b_scale.dtype, ""), bp, bt,
-            out.data_ptr(), xt, wp, max(wn, 0), M, N, K, st)), "tac_linear_w8a8")
-    return out
-
-
-def linear_workspace(M: int, K: int, device="cuda"):
-    """A workspace for linear_w8a8 calls of at most M rows of K columns (calls that share one must not overlap)."""
-    import torch
-    return torch.empty(int(L.lib.tac_linear_w8a8_workspace_bytes(M, K)) + 256, dtype=torch.uint8, device=device)
 
 
 def time_gemm_wo(M: int = 1024, N: int = 3072, K: int = 768, iters: int = 20, warmup: int = 5, seed: int = 0,

@@ -18,8 +18,16 @@ are device tensors that are read when the call runs, so a captured call follows 
 """
 from __future__ import annotations
 
+from functools import lru_cache
+
+import torch
+
 from . import _lib as L
-from .gemm import _on_device, _type
+from ._tensors import TYPES, call, type_code
+
+_I32, _F32 = torch.int32, torch.float32
+_append, _read, _attention = L.lib.tac_kv4_append, L.lib.tac_kv4_read, L.lib.tac_kv4_attention
+_workspace_bytes = lru_cache(maxsize=1024)(L.lib.tac_kv4_attention_workspace_bytes)   # sizes alone decide
 
 PAGE_SIZES = (16, 32, 64, 128)
 HEAD_DIMS = (64, 128)
@@ -32,7 +40,6 @@ class Kv4Cache:
     byte j), k_params, v_params int32 [pages, heads, page_size] (the bits of s above those of z)."""
 
     def __init__(self, num_pages: int, page_size: int, heads: int, head_dim: int, device="cuda"):
-        import torch
         if page_size not in PAGE_SIZES or head_dim not in HEAD_DIMS:
             raise ValueError(f"page_size must be one of {PAGE_SIZES} and head_dim of {HEAD_DIMS}, got {page_size} "
                              f"and {head_dim}")
@@ -52,7 +59,6 @@ class Kv4Cache:
         return self
 
     def _set(self, k_codes, k_params, v_codes, v_params):
-        import torch
         for c, p in ((k_codes, k_params), (v_codes, v_params)):
             if c.dtype != torch.uint8 or p.dtype != torch.int32:
                 raise TypeError("codes must be uint8 and parameter words int32")
@@ -76,14 +82,13 @@ class Kv4Cache:
 
 def _batch(cache, page_table, lens, indptr, total):
     """Checks of the batch's description; (page_table, lens, indptr, batch, width, total) as the C calls take them."""
-    import torch
-    i32 = torch.int32
-    if page_table.dtype != i32 or lens.dtype != i32 or (indptr is not None and indptr.dtype != i32):
+    if page_table.dtype is not _I32 or lens.dtype is not _I32 or (indptr is not None and indptr.dtype is not _I32):
         raise TypeError("page_table, lens and indptr must be int32")
-    if page_table.dim() != 2 or lens.dim() != 1 or lens.shape[0] != page_table.shape[0]:
-        raise ValueError(f"page_table must be [batch, width] and lens [batch], got {tuple(page_table.shape)} and "
+    shape = page_table.shape
+    if len(shape) != 2 or lens.shape != shape[:1]:
+        raise ValueError(f"page_table must be [batch, width] and lens [batch], got {tuple(shape)} and "
                          f"{tuple(lens.shape)}")
-    batch, width = page_table.shape
+    batch, width = shape
     if width == 0:
         raise ValueError("page_table must have a column")
     if not (page_table.is_contiguous() and lens.is_contiguous()):
@@ -95,18 +100,21 @@ def _batch(cache, page_table, lens, indptr, total):
         if total != batch:
             raise ValueError(f"without indptr there is one row a sequence: {batch} sequences, {total} rows")
         return page_table.data_ptr(), lens.data_ptr(), None, batch, width, total
-    if indptr.dim() != 1 or indptr.shape[0] != batch + 1 or not indptr.is_contiguous() or indptr.device != dev:
+    if indptr.shape != (batch + 1,) or not indptr.is_contiguous() or indptr.device != dev:
         raise ValueError(f"indptr must be a contiguous [{batch + 1}] tensor on the cache's device")
     return page_table.data_ptr(), lens.data_ptr(), indptr.data_ptr(), batch, width, total
 
 
-def _rows(x, heads, cache, what):
-    if x.dim() != 3 or x.shape[2] != cache.head_dim or (heads is not None and x.shape[1] != heads):
-        raise ValueError(f"{what} must be [rows, {heads or 'heads'}, {cache.head_dim}], got {tuple(x.shape)}")
-    if x.stride(2) != 1:
-        raise ValueError(f"the values of a head must be contiguous in {what}, got strides {x.stride()}")
+def _rows(x, shape, heads, cache, what):
+    """Checks of rows [rows, heads, head_dim]; their strides."""
+    if len(shape) != 3 or shape[2] != cache.head_dim or (heads is not None and shape[1] != heads):
+        raise ValueError(f"{what} must be [rows, {heads or 'heads'}, {cache.head_dim}], got {tuple(shape)}")
+    stride = x.stride()
+    if stride[2] != 1:
+        raise ValueError(f"the values of a head must be contiguous in {what}, got strides {stride}")
     if x.device != cache.device:
         raise ValueError(f"{what} must be on the cache's device")
+    return stride
 
 
 def append(cache: Kv4Cache, k, v, page_table, lens, indptr=None) -> None:
@@ -114,39 +122,37 @@ def append(cache: Kv4Cache, k, v, page_table, lens, indptr=None) -> None:
     strides: slices of a fused projection will do) into the cache.  Rows without a place (before position 0, past
     the table, on a page number outside the cache, or of no sequence) are skipped.  No two rows of a call may have
     the same place, which only sequences that share a page could bring about."""
-    t = _type(k.dtype, "k")
-    if v.dtype != k.dtype:
+    t = type_code(k.dtype, "k")
+    if v.dtype is not k.dtype:
         raise TypeError(f"k and v must have one type, got {k.dtype} and {v.dtype}")
-    _rows(k, cache.heads, cache, "k")
-    _rows(v, cache.heads, cache, "v")
-    if v.shape != k.shape:
-        raise ValueError(f"k and v must have one shape, got {tuple(k.shape)} and {tuple(v.shape)}")
-    args = _batch(cache, page_table, lens, indptr, k.shape[0])
-    if k.shape[0] == 0 or args[3] == 0:
-        return
-    ks, vs = k.stride(), v.stride()
-    L.check(_on_device(cache.device, lambda st: L.lib.tac_kv4_append(
-        cache._ref, *args, k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], t, st)), "tac_kv4_append")
+    shape = k.shape
+    if v.shape != shape:
+        raise ValueError(f"k and v must have one shape, got {tuple(shape)} and {tuple(v.shape)}")
+    ks = _rows(k, shape, cache.heads, cache, "k")
+    vs = _rows(v, shape, cache.heads, cache, "v")
+    total = shape[0]
+    args = _batch(cache, page_table, lens, indptr, total)
+    if total and args[3]:
+        call("tac_kv4_append", _append, cache.device.index, cache._ref, *args, k.data_ptr(), ks[0], ks[1], v.data_ptr(),
+             vs[0], vs[1], t)
 
 
 def read(cache: Kv4Cache, page_table, lens, indptr=None, total=None):
     """(k, v) float32 [rows, heads, head_dim] that the new tokens' rows of the cache stand for; zeros for rows without
     a place.  total: the number of rows with indptr (a captured call cannot ask the device for it).  A whole prefix
     is read with indptr = 0, lens[0], lens[0] + lens[1], ..."""
-    import torch
     if total is None:
         if indptr is not None:
             raise ValueError("total is needed with indptr")
         total = lens.shape[0]
     args = _batch(cache, page_table, lens, indptr, total)
-    k = torch.empty((total, cache.heads, cache.head_dim), dtype=torch.float32, device=cache.device)
-    v = torch.empty_like(k)
-    if total and args[3]:
-        L.check(_on_device(cache.device, lambda st: L.lib.tac_kv4_read(cache._ref, *args, k.data_ptr(), v.data_ptr(),
-                                                                       st)), "tac_kv4_read")
-    elif total:
-        k.zero_()
-        v.zero_()
+    kv = torch.empty((2, total, cache.heads, cache.head_dim), dtype=_F32, device=cache.device)
+    k, v = kv.unbind(0)
+    if total:
+        if args[3]:
+            call("tac_kv4_read", _read, cache.device.index, cache._ref, *args, k.data_ptr(), v.data_ptr())
+        else:
+            kv.zero_()
     return k, v
 
 
@@ -160,29 +166,24 @@ def attention(q, cache: Kv4Cache, page_table, lens, indptr=None, *, scale=None, 
     h // (q_heads // heads).  scale defaults to head_dim ** -0.5.  The result has q's type; with return_lse also
     float32 [rows, q_heads] log sum_j exp(scale q . k_j), by which parts of one attention can be joined.  A row that
     sees no token is zero (lse -inf); rows of no sequence are left as they are in `out`."""
-    import torch
-    if q.dtype not in (torch.float16, torch.bfloat16):
-        raise TypeError(f"q must be float16 or bfloat16, got {q.dtype}")
-    _rows(q, None, cache, "q")
-    total, hq, D = q.shape
+    dt = q.dtype
+    if dt is not torch.float16 and dt is not torch.bfloat16:
+        raise TypeError(f"q must be float16 or bfloat16, got {dt}")
+    shape = q.shape
+    qs = _rows(q, shape, None, cache, "q")
+    total, hq, D = shape
     if hq == 0 or hq % cache.heads:
         raise ValueError(f"{hq} query heads over {cache.heads} key-value heads")
     args = _batch(cache, page_table, lens, indptr, total)
     if out is None:
-        out = torch.empty((total, hq, D), dtype=q.dtype, device=q.device)
-    elif out.dtype != q.dtype or out.shape != q.shape or not out.is_contiguous() or out.device != q.device:
-        raise ValueError(f"out must be a contiguous {q.dtype} {tuple(q.shape)} tensor on q's device")
-    lse = torch.empty((total, hq), dtype=torch.float32, device=q.device) if return_lse else None
+        out = torch.empty(shape, dtype=dt, device=cache.device)
+    elif out.dtype is not dt or out.shape != shape or not out.is_contiguous() or out.device != cache.device:
+        raise ValueError(f"out must be a contiguous {dt} {tuple(shape)} tensor on q's device")
+    lse = torch.empty((total, hq), dtype=_F32, device=cache.device) if return_lse else None
     if total and args[3]:
-        qs = q.stride()
-
-        def call(st):
-            need = L.lib.tac_kv4_attention_workspace_bytes(args[3], total, hq, cache.heads, D)
-            ws = torch.empty(need, dtype=torch.uint8, device=cache.device)
-            return L.lib.tac_kv4_attention(
-                cache._ref, *args, q.data_ptr(), qs[0], qs[1], hq, _type(q.dtype, "q"),
-                D ** -0.5 if scale is None else scale, causal, out.data_ptr(), None if lse is None else lse.data_ptr(),
-                ws.data_ptr(), need, st)
-
-        L.check(_on_device(cache.device, call), "tac_kv4_attention")
+        need = _workspace_bytes(args[3], args[4], cache.page_size, total, hq, cache.heads, D)
+        ws = torch.empty(need, dtype=torch.uint8, device=cache.device) if need else None
+        call("tac_kv4_attention", _attention, cache.device.index, cache._ref, *args, q.data_ptr(), qs[0], qs[1], hq,
+             TYPES[dt], D ** -0.5 if scale is None else scale, causal, out.data_ptr(),
+             None if lse is None else lse.data_ptr(), None if ws is None else ws.data_ptr(), need)
     return (out, lse) if return_lse else out

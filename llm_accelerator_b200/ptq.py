@@ -62,8 +62,8 @@ def quantize_rows(X):
     stride): t = max(max |x|, 1e-8), scale = t / 127, q = rint(x * (127 / t)); K_pad = K rounded up to 16, padding
     columns zero.  A row that holds an infinity or a NaN gets the scale NaN."""
     import torch
-    from .gemm import _on_device, _type
-    xt = _type(X.dtype, "X")
+    from ._tensors import call, type_code
+    xt = type_code(X.dtype, "X")
     if not X.is_cuda:
         raise TypeError("X must be a CUDA tensor")
     if X.dim() != 2 or X.shape[1] == 0 or (X.shape[1] > 1 and X.stride(1) != 1):
@@ -75,9 +75,8 @@ def quantize_rows(X):
     q = torch.empty((M, -(-K // 16) * 16), dtype=torch.int8, device=X.device)
     scale = torch.empty(M, dtype=torch.float32, device=X.device)
     if M:
-        L.check(_on_device(X.device, lambda st: L.lib.tac_quantize_rows_i8(X.data_ptr(), xt, ldx, q.data_ptr(),
-                                                                           scale.data_ptr(), M, K, st)),
-                "tac_quantize_rows_i8")
+        call("tac_quantize_rows_i8", L.lib.tac_quantize_rows_i8, X.get_device(), X.data_ptr(), xt, ldx, q.data_ptr(),
+             scale.data_ptr(), M, K)
     return q, scale
 
 

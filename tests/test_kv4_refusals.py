@@ -18,7 +18,7 @@ def _cache(**bad):
     return L.Kv4CacheRecord(*(f[n] for n, _ in L.Kv4CacheRecord._fields_))
 
 
-def _seqs(table=P, lens=P, indptr=P, batch=2, width=3, total=5):
+def _seqs(table=P, lens=P, indptr=P, batch=2, width=300, total=5):
     return table, lens, indptr, batch, width, total
 
 
@@ -68,7 +68,11 @@ def test_attention(bad):
 
 def test_workspace_query():
     f = L.lib.tac_kv4_attention_workspace_bytes
-    assert f(0, 1, 4, 2, 64) == 0 and f(1, 0, 4, 2, 64) == 0 and f(1, 1, 3, 2, 64) == 0 and f(1, 1, 4, 2, 80) == 0
+    assert f(0, 99, 64, 1, 4, 2, 64) == 0 and f(1, 99, 64, 0, 4, 2, 64) == 0 and f(1, 99, 64, 1, 3, 2, 64) == 0
+    assert f(1, 99, 64, 1, 4, 2, 80) == 0
+    assert f(1, 16, 64, 1, 4, 2, 64) == 0            # short contexts are not split
+    assert f(1, 99, 64, 99, 4, 2, 64) == 0           # nor are prompts
+    assert f(1, 99, 64, 1, 4, 2, 64) > 0
 
 
 def test_record_matches_the_header():

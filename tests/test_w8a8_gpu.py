@@ -117,7 +117,7 @@ def test_quantize_rows_of_slices():
 
 
 # (M, K): decode rows, K past one 16-byte group, K that no vector load divides, prompts
-LINEAR = [(1, 1024), (1, 33), (4, 768), (16, 4096), (17, 100), (40, 2048), (64, 1023), (130, 768), (600, 1040)]
+LINEAR = [(1, 1024), (1, 33), (1, 1), (3, 8192), (5, 8208), (15, 1000), (4, 768), (16, 4096), (17, 100), (40, 2048), (64, 1023), (130, 768), (600, 1040)]
 
 
 @pytest.mark.parametrize("dtype", ["float16", "bfloat16", "float32"])

@@ -18,7 +18,7 @@ def _gemm(A=P, Bt=P, sa=P, sb=P, sbt=L.TYPE_F32, bias=None, bt=0, Y=P, yt=L.TYPE
 
 
 def _linear(X=P, xt=L.TYPE_F16, ldx=32, Bt=P, sb=P, sbt=L.TYPE_F16, bias=None, bt=0, Y=P, yt=L.TYPE_F16, ws=P,
-            wn=1 << 20, M=4, N=8, K=32):
+            wn=1 << 20, M=40, N=8, K=32):
     return L.lib.tac_linear_w8a8(X, xt, ldx, Bt, sb, sbt, bias, bt, Y, yt, ws, wn, M, N, K, None)
 
 
@@ -48,7 +48,9 @@ def test_quantize_rows_refusals(bad):
 
 def test_workspace_bytes():
     assert L.lib.tac_linear_w8a8_workspace_bytes(0, 5) == 0
-    assert L.lib.tac_linear_w8a8_workspace_bytes(3, 17) >= 3 * 32 + 12
+    assert L.lib.tac_linear_w8a8_workspace_bytes(16, 8192) == 0          # few rows need none
+    assert L.lib.tac_linear_w8a8_workspace_bytes(17, 17) >= 17 * 32 + 17 * 4
+    assert L.lib.tac_linear_w8a8_workspace_bytes(16, 8193) >= 16 * 8208 + 64
     assert L.lib.tac_linear_w8a8_workspace_bytes(1 << 20, 131071) > 1 << 36
 
 
