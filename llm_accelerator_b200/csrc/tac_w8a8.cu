@@ -194,7 +194,16 @@ bool map_rows(CUtensorMap* m, const int8_t* base, int K, int rows, int box_rows)
   return tmap_encode_u8(m, base, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
-constexpr int kSkMaxSmem = 200 * 1024;
+constexpr int kSkMaxSmem = 224 * 1024;
+
+// CTAs that share a tile's K blocks: as many as find an SM each, with eight K blocks or more a CTA (two for 16 tokens,
+// whose partial sums are few).  Measured: 64 x 4096 x 1024 takes 7.2 us whole and 8.3 us in four, 64 x 4096 x 4096 12.1
+// and 10.9, 1 x 4096 x 4096 10.0 and 7.7; more CTAs than SMs cost 1 x 4096 x 1024 1.7 us.
+int splits(int64_t tiles, int k_blocks, int tn, int sms) {
+  int split = 1;
+  while (split < 8 && 2 * split * (tn > 16 ? 8 : 2) <= k_blocks && tiles * split * 2 <= sms) split *= 2;
+  return split;
+}
 
 template <int YT>
 int launch_splitk(const int8_t* A, const int8_t* Bt, W8Params p, cudaStream_t st) {
@@ -210,11 +219,11 @@ int launch_splitk(const int8_t* A, const int8_t* Bt, W8Params p, cudaStream_t st
   p.k_blocks = (p.K + 127) / 128;
   p.tn = p.M <= 16 ? 16 : p.M <= 32 ? 32 : p.M <= 64 ? 64 : 128;
   const int64_t tiles = int64_t((p.N + 127) / 128) * ((p.M + p.tn - 1) / p.tn);
-  int split = 1;
-  while (split < 8 && 2 * split <= p.k_blocks && tiles * split * 2 <= 2 * sms) split *= 2;
+  const int split = splits(tiles, p.k_blocks, p.tn, sms);
   const int per = (p.k_blocks + split - 1) / split, sb = sk_stage_bytes(p.tn);
-  p.stages = std::min(std::min(per, 8), std::max(2, 96 * 1024 / sb));
-  const int part = split > 1 ? p.tn * 512 : 0;
+  // in flight: 96 KB where two CTAs share an SM, else twice that
+  p.stages = std::min(std::min(per, 8), std::max(2, (tiles * split > sms ? 96 : 190) * 1024 / sb));
+  const int part = split > 1 ? sk_part_bytes(p.tn) : 0;
   CUtensorMap tw, ta;
   if (!map_rows(&tw, Bt, p.K, p.N, 128) || !map_rows(&ta, A, p.K, p.M, p.tn)) return TAC_E_CUDA;
   cudaLaunchConfig_t cfg = {};
@@ -353,16 +362,15 @@ int launch_rows(W8RowsParams pp, const int8_t* Bt, cudaStream_t st) {
   p.tn = kRowsMost;
   p.k_blocks = (p.K + 127) / 128;
   const int64_t tiles = (p.N + 127) / 128;
-  int split = 1;
-  while (split < 8 && 2 * split <= p.k_blocks && tiles * split * 2 <= 2 * sms) split *= 2;
+  const int split = splits(tiles, p.k_blocks, p.tn, sms);
   const int per = (p.k_blocks + split - 1) / split;
-  p.stages = std::min(per, 4);
+  p.stages = std::min(per, tiles * split > sms ? 4 : 8);
   CUtensorMap tw;
   if (!map_rows(&tw, Bt, p.K, p.N, 128)) return TAC_E_CUDA;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(uint32_t(tiles), 1, split);
   cfg.blockDim = dim3(kSkThreads);
-  cfg.dynamicSmemBytes = p.stages * kSkWBytes + per * kRowsMost * 128 + 1024;   // the partial sums (8 KB) fit the first stage
+  cfg.dynamicSmemBytes = p.stages * kSkWBytes + per * kRowsMost * 128 + 1024;   // the partial sums (10 KB) fit the first stage
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;

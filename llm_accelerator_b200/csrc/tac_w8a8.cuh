@@ -137,8 +137,14 @@ constexpr int kSkWBytes = 128 * 128;
 
 __host__ __device__ constexpr int sk_stage_bytes(int tn) { return kSkWBytes + tn * 128; }
 
-// The end of both split-K kernels: the tile's results, or the CTA's partial sums to shared memory (over its stages: every
-// copy and MMA has ended) and every nsplit-th token from all partials.  All threads of the CTA.
+// Partial sums of a split tile in shared memory: [128 channels][tn + 4], so that a channel's tokens are read 16 bytes at
+// a time from the other CTAs and the padding spreads the channels over the banks.
+__host__ __device__ constexpr int sk_part_bytes(int tn) { return 128 * (tn + 4) * 4; }
+
+// The end of both split-K kernels: the tile's results, or the CTA's partial sums to shared memory (over its stages:
+// every copy and MMA has ended) and, after the cluster's barrier, CTA r's share of the tokens from all partials.
+// (Reading the others' partials a word at a time took 12 us where one CTA alone took 7; pushing them a word at a time
+// was no better.)  All threads of the CTA.
 template <int YT>
 __device__ __forceinline__ void w8_splitk_finish(const W8Params& p, uint8_t* smem, uint32_t tmem, const float* as_s, int warp,
                                                  int row, int n, int m0, int rank, int nsplit, float bs, float bias,
@@ -154,34 +160,50 @@ __device__ __forceinline__ void w8_splitk_finish(const W8Params& p, uint8_t* sme
         w8_store32<YT>(p, v, as_s + c, m0 + c, n, bs, bias);
       }
     }
-  } else {
-    int* part = reinterpret_cast<int*>(smem);            // [tn][128]
-    if (warp >= 2) {
-      for (int c = 0; c < p.tn; c += 32) {
-        uint32_t v[32];
-        __syncwarp();
-        sm100::tmem_ld32(t_addr + c, v);
-#pragma unroll
-        for (int j = 0; j < 32; ++j)
-          if (c + j < p.tn) part[(c + j) * 128 + row] = int(v[j]);
-      }
-    }
-    sm100::cluster_sync();
-    if (warp >= 2) {
-      for (int c = rank; c < p.tn; c += nsplit) {
-        const int m = m0 + c;
-        if (m >= p.M) break;
-        int acc = 0;
-        for (int r = 0; r < nsplit; ++r) {
-          int v;
-          asm volatile("ld.shared::cluster.s32 %0, [%1];\n" : "=r"(v) : "r"(sm100::mapa_shared(part + c * 128 + row, r)));
-          acc += v;
-        }
-        if (n < p.N) st_y<YT>(p.y, int64_t(m) * p.N + n, w8_value(acc, as_s[c], bs, bias));
-      }
-    }
-    sm100::cluster_sync();   // no CTA leaves while another reads its partial sums
+    return;
   }
+  int* const mine = reinterpret_cast<int*>(smem) + row * (p.tn + 4);
+  if (warp >= 2) {
+    for (int c = 0; c < p.tn; c += 32) {
+      uint32_t v[32];
+      __syncwarp();
+      sm100::tmem_ld32(t_addr + c, v);
+#pragma unroll
+      for (int j = 0; j < 32; j += 4)
+        if (c + j < p.tn) *reinterpret_cast<int4*>(mine + c + j) = make_int4(int(v[j]), int(v[j + 1]), int(v[j + 2]), int(v[j + 3]));
+    }
+  }
+  __syncwarp();
+  sm100::cluster_sync();
+  const int per = max(4, p.tn / nsplit), first = rank * per;    // tokens of this CTA
+  if (warp >= 2 && first < p.tn) {
+    uint32_t base[8];
+#pragma unroll
+    for (int r = 0; r < 8; ++r) base[r] = sm100::mapa_shared(mine + first, r < nsplit ? r : 0);
+    for (int k = 0; k < per; k += 4) {
+      if (m0 + first + k >= p.M) break;
+      int4 v[8];
+#pragma unroll
+      for (int r = 0; r < 8; ++r) {
+        v[r] = make_int4(0, 0, 0, 0);
+        if (r < nsplit)
+          asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];\n"
+                       : "=r"(v[r].x), "=r"(v[r].y), "=r"(v[r].z), "=r"(v[r].w)
+                       : "r"(base[r] + k * 4)
+                       : "memory");
+      }
+      int acc[4] = {};
+#pragma unroll
+      for (int r = 0; r < 8; ++r) acc[0] += v[r].x, acc[1] += v[r].y, acc[2] += v[r].z, acc[3] += v[r].w;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int tok = first + k + j, m = m0 + tok;
+        if (m < p.M && n < p.N) st_y<YT>(p.y, int64_t(m) * p.N + n, w8_value(acc[j], as_s[tok], bs, bias));
+      }
+    }
+  }
+  __syncwarp();
+  sm100::cluster_sync();                         // no CTA leaves while another reads its partial sums
 }
 
 template <int YT>
@@ -342,6 +364,7 @@ __global__ void __launch_bounds__(kSkThreads) w8_rows_kernel(const __grid_consta
   __shared__ uint32_t tmem_base, row_max[kTn], all_max[8][kTn];
   __shared__ int abort_flag;
   __shared__ __align__(16) float as_s[32];       // a chunk of the epilogue is 32 tokens wide
+  __shared__ float inv_s[kTn];
 
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(dyn_smem) + 1023) & ~uintptr_t(1023));
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
@@ -371,6 +394,23 @@ __global__ void __launch_bounds__(kSkThreads) w8_rows_kernel(const __grid_consta
 
   const int early = min(S, kb1 - kb0);
   const int t = threadIdx.x - 64, per = (kb1 - kb0) * 16, items = p.M * per;   // 8-value chunks of this CTA's columns
+  constexpr int kHeld = 4;                       // chunks that a thread keeps from the maximum to the codes; it reads the rest again
+  float held[kHeld][8];
+  auto item = [&](int i, float (&v)[8]) {
+    const int m = i / per;
+    load8(pp, m, kb0 * 128 + (i - m * per) * 8, v);
+    return m;
+  };
+  auto largest = [&](int m, const float (&v)[8]) {
+    uint32_t mb = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) mb = max(mb, __float_as_uint(v[j]) & 0x7fffffffu);
+    // 16 lanes of one row first: a row has a multiple of 16 chunks
+    const uint32_t lanes = __activemask();
+#pragma unroll
+    for (int o = 1; o < 16; o <<= 1) mb = max(mb, __shfl_xor_sync(lanes, mb, o));
+    if ((lane & 15) == 0) atomicMax(&row_max[m], mb);
+  };
   if (warp == 0) {
     if (sm100::elect_one())
       for (int i = 0; i < early; ++i) {
@@ -379,25 +419,23 @@ __global__ void __launch_bounds__(kSkThreads) w8_rows_kernel(const __grid_consta
       }
     __syncwarp();
   } else if (warp >= 2) {
-    for (int i = t; i < items; i += 128) {
-      float v[8];
-      const int m = i / per;
-      load8(pp, m, kb0 * 128 + (i - m * per) * 8, v);
-      uint32_t mb = 0;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) mb = max(mb, __float_as_uint(v[j]) & 0x7fffffffu);
-      // lanes of one row first: a row has a multiple of 16 chunks
-      mb = max(mb, __shfl_xor_sync(__activemask(), mb, 1));
-      mb = max(mb, __shfl_xor_sync(__activemask(), mb, 2));
-      mb = max(mb, __shfl_xor_sync(__activemask(), mb, 4));
-      mb = max(mb, __shfl_xor_sync(__activemask(), mb, 8));
-      if ((lane & 15) == 0) atomicMax(&row_max[m], mb);
+    for (int k = 0; k < kHeld; ++k)
+      if (t + k * 128 < items) item(t + k * 128, held[k]);
+    for (int i = t; i < per * 8; i += 128) reinterpret_cast<uint4*>(rows_sm)[i] = make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (int k = 0; k < kHeld; ++k)
+      if (t + k * 128 < items) largest((t + k * 128) / per, held[k]);
+    for (int i = t + kHeld * 128; i < items; i += 128) {
+      float v[8];
+      const int m = item(i, v);
+      largest(m, v);
     }
     asm volatile("bar.sync 1, 128;\n" ::: "memory");
-    for (int i = t; i < kTn * nsplit; i += 128) {
-      const int m = i % kTn;
-      asm volatile("st.shared::cluster.u32 [%0], %1;\n" ::"r"(sm100::mapa_shared(&all_max[rank][m], i / kTn)), "r"(row_max[m]) : "memory");
-    }
+    // this CTA's maxima to every CTA of the cluster
+    for (int i = t; i < kTn * nsplit; i += 128)
+      asm volatile("st.shared::cluster.u32 [%0], %1;\n" ::"r"(sm100::mapa_shared(&all_max[rank][i % kTn], i / kTn)), "r"(row_max[i % kTn])
+                   : "memory");
   }
   __syncwarp();
   if (nsplit > 1) sm100::cluster_sync();
@@ -452,28 +490,35 @@ __global__ void __launch_bounds__(kSkThreads) w8_rows_kernel(const __grid_consta
   float bs = 0.f, bias = 0.f;
   bool acc_ok = false;
   if (warp >= 2) {
-    // ---- codes of all 16 rows (zeros past M) ----
-    for (int i = t; i < kTn * per; i += 128) {
+    if (t < p.M) {
+      uint32_t mb = 0;
+      for (int r = 0; r < nsplit; ++r) mb = max(mb, all_max[r][t]);
+      const bool finite = mb < 0x7f800000u;
+      const float top = fmaxf(__uint_as_float(mb), 1e-8f);
+      inv_s[t] = finite ? __fdiv_rn(127.0f, top) : __uint_as_float(0x7fc00000u);
+      as_s[t] = finite ? __fdiv_rn(top, 127.0f) : __uint_as_float(0x7fc00000u);
+    }
+    asm volatile("bar.sync 1, 128;\n" ::: "memory");   // inv_s, as_s, and the zeros of rows_sm
+    auto codes = [&](int i, const float (&v)[8]) {
       const int m = i / per, c = i - m * per;    // c: 8-value chunk of the row
-      uint2 codes = make_uint2(0, 0);
-      if (m < p.M) {
-        uint32_t mb = 0;
-        for (int r = 0; r < nsplit; ++r) mb = max(mb, all_max[r][m]);
-        const bool finite = mb < 0x7f800000u;
-        const float top = fmaxf(__uint_as_float(mb), 1e-8f), inv = finite ? __fdiv_rn(127.0f, top) : 0.f;
-        if (c == 0) as_s[m] = finite ? __fdiv_rn(top, 127.0f) : __uint_as_float(0x7fc00000u);
-        if (finite) {
-          float v[8];
-          load8(pp, m, kb0 * 128 + c * 8, v);
-          uint32_t b[8];
+      const float inv = inv_s[m];
+      if (!(inv == inv)) return;                 // a row without a scale: its codes stay 0
+      uint32_t b[8];
 #pragma unroll
-          for (int j = 0; j < 8; ++j) b[j] = __float_as_uint(__fadd_rn(__fmul_rn(v[j], inv), 12582912.f));   // rounds; low byte = code
-          codes.x = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
-          codes.y = __byte_perm(__byte_perm(b[4], b[5], 0x0040), __byte_perm(b[6], b[7], 0x0040), 0x5410);
-        }
-      }
+      for (int j = 0; j < 8; ++j) b[j] = __float_as_uint(__fadd_rn(__fmul_rn(v[j], inv), 12582912.f));   // rounds; low byte = code
       // block c / 16, 16-byte chunk (c / 2) % 8, its half c % 2
-      *reinterpret_cast<uint2*>(rows_sm + (c >> 4) * (kTn * 128) + (m >> 3) * 1024 + (m & 7) * 128 + ((((c >> 1) & 7) ^ (m & 7)) << 4) + (c & 1) * 8) = codes;
+      *reinterpret_cast<uint2*>(rows_sm + (c >> 4) * (kTn * 128) + (m >> 3) * 1024 + (m & 7) * 128 + ((((c >> 1) & 7) ^ (m & 7)) << 4) +
+                                (c & 1) * 8) =
+          make_uint2(__byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410),
+                     __byte_perm(__byte_perm(b[4], b[5], 0x0040), __byte_perm(b[6], b[7], 0x0040), 0x5410));
+    };
+#pragma unroll
+    for (int k = 0; k < kHeld; ++k)
+      if (t + k * 128 < items) codes(t + k * 128, held[k]);
+    for (int i = t + kHeld * 128; i < items; i += 128) {
+      float v[8];
+      item(i, v);
+      codes(i, v);
     }
     sm100::fence_proxy_async();
     __syncwarp();
@@ -482,7 +527,6 @@ __global__ void __launch_bounds__(kSkThreads) w8_rows_kernel(const __grid_consta
       bs = ld_any(p.b_scale, p.b_type, n);
       if (p.bias) bias = ld_any(p.bias, p.bias_type, n);
     }
-    asm volatile("bar.sync 1, 128;\n" ::: "memory");   // as_s, among the epilogue's warps
     acc_ok = sm100::mbar_wait(&acc_bar, 0, p.fault, W8_TIMEOUT_ACC);
     __syncwarp();
     sm100::tc_fence_after();

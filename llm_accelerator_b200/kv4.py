@@ -146,13 +146,14 @@ def read(cache: Kv4Cache, page_table, lens, indptr=None, total=None):
             raise ValueError("total is needed with indptr")
         total = lens.shape[0]
     args = _batch(cache, page_table, lens, indptr, total)
-    kv = torch.empty((2, total, cache.heads, cache.head_dim), dtype=_F32, device=cache.device)
-    k, v = kv.unbind(0)
+    k = torch.empty((total, cache.heads, cache.head_dim), dtype=_F32, device=cache.device)
+    v = torch.empty_like(k)
     if total:
         if args[3]:
             call("tac_kv4_read", _read, cache.device.index, cache._ref, *args, k.data_ptr(), v.data_ptr())
         else:
-            kv.zero_()
+            k.zero_()
+            v.zero_()
     return k, v
 
 
@@ -176,7 +177,7 @@ def attention(q, cache: Kv4Cache, page_table, lens, indptr=None, *, scale=None, 
         raise ValueError(f"{hq} query heads over {cache.heads} key-value heads")
     args = _batch(cache, page_table, lens, indptr, total)
     if out is None:
-        out = torch.empty(shape, dtype=dt, device=cache.device)
+        out = q.new_empty(shape)
     elif out.dtype is not dt or out.shape != shape or not out.is_contiguous() or out.device != cache.device:
         raise ValueError(f"out must be a contiguous {dt} {tuple(shape)} tensor on q's device")
     lse = torch.empty((total, hq), dtype=_F32, device=cache.device) if return_lse else None

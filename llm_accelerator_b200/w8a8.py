@@ -38,7 +38,7 @@ def _check(rows, Bt, b_scale, bias, out, out_dtype, M, K):
             raise ValueError(f"bias must be a contiguous [{N}] tensor on the operands' device")
         bp = bias.data_ptr()
     if out is None:
-        out = torch.empty((M, N), dtype=out_dtype, device=dev)
+        out = rows.new_empty((M, N), dtype=out_dtype)
     elif out.dtype is not out_dtype or out.shape != (M, N) or not out.is_contiguous() or out.device != dev:
         raise ValueError(f"out must be a contiguous {out_dtype} [{M}, {N}] tensor on the operands' device")
     return N, out, bp, bt
