@@ -83,14 +83,18 @@ __device__ __forceinline__ uint32_t movmatrix(uint32_t x) {
   return y;
 }
 
-// Codes 0 and 4 (N = 0), 1 and 5, 2 and 6, 3 and 7 of a word as FP16 64 + c:
+// Codes 0 and 4 (N = 0), 1 and 5, 2 and 6, 3 and 7 of a word as FP16 numbers:
 // a code in bits 4..7 of a half with the exponent of 64 is 64 + c, one in bits
-// 0..3 with that of 1024 is 1024 + c, and 960 less is exact.  The common 64
-// (and the zero point with it) is taken off the sums, once a score and once an
-// output, where it costs 2^-24 * 64 of the operand's sum, not once a code.
-// Of the two instructions that a pair takes, the masks run on the integer
-// pipe, which bounds this kernel once the loads overlap, the additions beside
-// them on the other.
+// 0..3 with that of 1024 is 1024 + c.  Of the instructions that a pair takes,
+// the masks run on the integer pipe, which bounds this kernel once the loads
+// overlap, the additions beside them on the other.
+//
+// For the scores all become 64 + c (960 less is exact): the common 64, and the
+// zero point with it, is taken off the sum of a score, where it costs 2^-24 *
+// 64 times the query's sum, far below what the weight's rounding to FP16 does.
+// For the outputs that would not do: thousands of weights cancel there (64 in
+// the sums of 131,072 flat weights cost ten times the output's rounding).
+// They get c - 8, and the sum of weights * (z - 8), small as well, is taken off.
 // The mask and the exponent go in by one three-input instruction, written out
 // because the compiler makes two of them.
 __device__ __forceinline__ uint32_t and_or(uint32_t x, uint32_t mask, uint32_t bits) {
@@ -100,10 +104,17 @@ __device__ __forceinline__ uint32_t and_or(uint32_t x, uint32_t mask, uint32_t b
 }
 
 template <int N>
-__device__ __forceinline__ uint32_t kv4_pair(uint32_t x) {
+__device__ __forceinline__ uint32_t kv4_pair64(uint32_t x) {
   const uint32_t y = N >= 2 ? x >> 8 : x;
   if (N & 1) return and_or(y, 0x00f000f0u, 0x54005400u);
   return h2_u(__hadd2(u_h2(and_or(y, 0x000f000fu, 0x64006400u)), __float2half2_rn(-960.f)));
+}
+
+template <int N>
+__device__ __forceinline__ uint32_t kv4_pair8(uint32_t x) {
+  const uint32_t y = N >= 2 ? x >> 8 : x;
+  if (N & 1) return h2_u(__hadd2(u_h2(and_or(y, 0x00f000f0u, 0x54005400u)), __float2half2_rn(-72.f)));
+  return h2_u(__hadd2(u_h2(and_or(y, 0x000f000fu, 0x64006400u)), __float2half2_rn(-1032.f)));
 }
 
 // 64 + z of a parameter word as a float: z in the bits worth 1 .. 8 at 64.
@@ -384,7 +395,7 @@ __global__ void __launch_bounds__(kRowsThreads, rows_ctas(D, NT)) kv4_rows_kerne
     // Softmax state of a row, per warp.  Weights are exp2(s - mu): mu follows the largest score only when one is more
     // than kSlack above it, so that most tiles need neither the maximum over the warp nor a rescaling.
     float o[NT][D / 16][4] = {};
-    float mu[NT][2] = {}, l[NT][2] = {}, zo[NT][2] = {};   // zo: sum of weights * (64 + z), to be taken off o
+    float mu[NT][2] = {}, l[NT][2] = {}, zo[NT][2] = {};   // zo: sum of weights * (z - 8), to be taken off o
     // A row's O is held in units of 2^(ve - 127), ve following the exponent of the largest s' among the keys that it
     // has seen (a NaN aside) in the same manner, so that its weights p s' fit FP16 whatever the values' magnitude, and
     // whatever it does not see: they stay below 2^kSlack 2^(kSlackV + 1).
@@ -431,8 +442,8 @@ __global__ void __launch_bounds__(kRowsThreads, rows_ctas(D, NT)) kv4_rows_kerne
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
           const uint32_t a = kw[u][0][w], c = kw[u][1][w];
-          const uint32_t p00 = kv4_pair<0>(a), p01 = kv4_pair<0>(c), p10 = kv4_pair<1>(a), p11 = kv4_pair<1>(c);
-          const uint32_t p20 = kv4_pair<2>(a), p21 = kv4_pair<2>(c), p30 = kv4_pair<3>(a), p31 = kv4_pair<3>(c);
+          const uint32_t p00 = kv4_pair64<0>(a), p01 = kv4_pair64<0>(c), p10 = kv4_pair64<1>(a), p11 = kv4_pair64<1>(c);
+          const uint32_t p20 = kv4_pair64<2>(a), p21 = kv4_pair64<2>(c), p30 = kv4_pair64<3>(a), p31 = kv4_pair64<3>(c);
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
             mma_16816(sc[u][n], p00, p01, p10, p11, qf[n][2 * w][0], qf[n][2 * w][1]);
@@ -515,7 +526,7 @@ __global__ void __launch_bounds__(kRowsThreads, rows_ctas(D, NT)) kv4_rows_kerne
         for (int u = 0; u < 2; ++u)
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            const float vs = kv4_scale(vpw[u][j]), vz = kv4_zero64(vpw[u][j]);
+            const float vs = kv4_scale(vpw[u][j]), vz = kv4_zero64(vpw[u][j]) - 72.f;
             float w[2];
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
@@ -550,8 +561,8 @@ __global__ void __launch_bounds__(kRowsThreads, rows_ctas(D, NT)) kv4_rows_kerne
           for (int half = 0; half < 2; ++half) {
             const uint32_t sel = half ? 0x7632 : 0x5410;
             const uint32_t a = __byte_perm(vw[0][w], vw[1][w], sel), c = __byte_perm(vw[2][w], vw[3][w], sel);
-            const uint32_t p00 = kv4_pair<0>(a), p01 = kv4_pair<0>(c), p10 = kv4_pair<1>(a), p11 = kv4_pair<1>(c);
-            const uint32_t p20 = kv4_pair<2>(a), p21 = kv4_pair<2>(c), p30 = kv4_pair<3>(a), p31 = kv4_pair<3>(c);
+            const uint32_t p00 = kv4_pair8<0>(a), p01 = kv4_pair8<0>(c), p10 = kv4_pair8<1>(a), p11 = kv4_pair8<1>(c);
+            const uint32_t p20 = kv4_pair8<2>(a), p21 = kv4_pair8<2>(c), p30 = kv4_pair8<3>(a), p31 = kv4_pair8<3>(c);
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
               mma_16816(o[n][4 * w + 2 * half], p00, p10, p01, p11, pb[u][n][0], pb[u][n][1]);

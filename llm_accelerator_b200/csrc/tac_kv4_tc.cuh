@@ -18,9 +18,10 @@
 // tile and group D = 128 needs 1024 tensor clocks, and 1024 clocks of the
 // exponential unit.
 //
-// S comes from whole numbers (codes less zero point, exact in FP16) and the
-// FP16 query scaled by a power of two for each row; the keys' scales multiply
-// it in float32.  V is rounded once to the query's type, P as well.
+// Both products have whole numbers (codes less zero point, exact in FP16) for
+// the cache's side.  The keys' scales multiply S in float32, the values' scales
+// the weights before these are rounded to FP16, once; the query is FP16, scaled
+// by a power of two for each row.  So nothing is rounded to BF16 but the result.
 // TMEM: two S of each group (64 columns; P takes the first half of its S), then
 // O of both.
 #pragma once
@@ -40,10 +41,9 @@ __host__ __device__ constexpr int tc_tile_bytes(int D) { return kTcKeys * D * 2;
 // Q of two groups, two K tiles, two V tiles
 __host__ __device__ constexpr int tc_smem(int D) { return 6 * tc_tile_bytes(D) + 1024; }
 
-// kind::f16 with float32 accumulation; b_mn: B is MN-major (one row a K step).
-__host__ __device__ constexpr uint32_t tc_idesc(uint32_t N, bool bf16, bool b_mn) {
-  return (1u << 4) | (uint32_t(bf16) << 7) | (uint32_t(bf16) << 10) | (uint32_t(b_mn) << 16) | ((N >> 3) << 17) |
-         ((128u >> 4) << 24);
+// kind::f16, FP16 operands, float32 accumulation; b_mn: B is MN-major (one row a K step).
+__host__ __device__ constexpr uint32_t tc_idesc(uint32_t N, bool b_mn) {
+  return (1u << 4) | (uint32_t(b_mn) << 16) | ((N >> 3) << 17) | ((128u >> 4) << 24);
 }
 
 __device__ __forceinline__ void mma_f16_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
@@ -149,20 +149,10 @@ __device__ __forceinline__ uint32_t sw128(uint32_t r, uint32_t c) {
   return (r >> 3) * 1024 + (r & 7) * 128 + ((c ^ (r & 7)) << 4);
 }
 
-// Codes of a key to shared memory as c - z (FP16), or s (c - z) rounded once: to BF16, to FP16 by an FP16 product (the
-// eight bits of a scale down to 2^-17 are exact in FP16), to FP16 by a float32 product (any scale).  A chunk of eight
-// values is stored in the order 0 4 1 5 2 6 3 7.
-enum TcUnpack { UNPACK_CODES, UNPACK_BF16, UNPACK_F16, UNPACK_F32 };
-
-template <int MODE>
-__device__ __forceinline__ uint32_t tc_finish(__half2 v, float s) {
-  if (MODE == UNPACK_F16) return h2_u(__hmul2(v, __float2half2_rn(s)));
-  if (MODE == UNPACK_F32) return h2_u(__floats2half2_rn(__low2float(v) * s, __high2float(v) * s));
-  return h2_u(v);
-}
-
-template <int W, int MODE>
-__device__ __forceinline__ void tc_unpack(uint8_t* dst, uint32_t key, int first, const uint4 (&words)[W / 4], uint32_t z, float s) {
+// Codes of a key to shared memory as c - z in FP16, chunks from `first` on.  A chunk of eight values is stored in the
+// order 0 4 1 5 2 6 3 7.
+template <int W>
+__device__ __forceinline__ void tc_unpack(uint8_t* dst, uint32_t key, int first, const uint4 (&words)[W / 4], uint32_t z) {
   const __half2 zlo = u_h2(0x64006400u + z * 0x10001u), zhi = u_h2(0x54005400u + z * 0x100010u);   // 1024 + z, 64 + z
 #pragma unroll
   for (int q = 0; q < W / 4; ++q) {
@@ -171,24 +161,9 @@ __device__ __forceinline__ void tc_unpack(uint8_t* dst, uint32_t key, int first,
     for (int j = 0; j < 4; ++j) {
       const int w = first + 4 * q + j;
       const uint32_t x = x4[j], y = x >> 8;
-      uint4 o;
-      if (MODE == UNPACK_BF16) {
-        // a code under the exponent of 128 is 128 + c; less 128 + z it is exact, and the product is rounded once
-        auto b2 = [](uint32_t u) { return *reinterpret_cast<__nv_bfloat162*>(&u); };
-        const __nv_bfloat162 zb = b2(0x43004300u + z * 0x10001u), sb = __float2bfloat162_rn(s);
-        auto value = [&](uint32_t u) {
-          const __nv_bfloat162 r = __hmul2(__hsub2(b2(and_or(u, 0x000f000fu, 0x43004300u)), zb), sb);
-          return *reinterpret_cast<const uint32_t*>(&r);
-        };
-        o = make_uint4(value(x), value(x >> 4), value(y), value(x >> 12));
-        *reinterpret_cast<uint4*>(dst + (w >> 3) * (kTcKeys * 128) + sw128(key, w & 7)) = o;
-        continue;
-      }
-      o.x = tc_finish<MODE>(__hsub2(u_h2(and_or(x, 0x000f000fu, 0x64006400u)), zlo), s);
-      o.y = tc_finish<MODE>(__hsub2(u_h2(and_or(x, 0x00f000f0u, 0x54005400u)), zhi), s);
-      o.z = tc_finish<MODE>(__hsub2(u_h2(and_or(y, 0x000f000fu, 0x64006400u)), zlo), s);
-      o.w = tc_finish<MODE>(__hsub2(u_h2(and_or(y, 0x00f000f0u, 0x54005400u)), zhi), s);
-      *reinterpret_cast<uint4*>(dst + (w >> 3) * (kTcKeys * 128) + sw128(key, w & 7)) = o;
+      *reinterpret_cast<uint4*>(dst + (w >> 3) * (kTcKeys * 128) + sw128(key, w & 7)) =
+          make_uint4(h2_u(__hsub2(u_h2(and_or(x, 0x000f000fu, 0x64006400u)), zlo)), h2_u(__hsub2(u_h2(and_or(x, 0x00f000f0u, 0x54005400u)), zhi)),
+                     h2_u(__hsub2(u_h2(and_or(y, 0x000f000fu, 0x64006400u)), zlo)), h2_u(__hsub2(u_h2(and_or(y, 0x00f000f0u, 0x54005400u)), zhi)));
     }
   }
 }
@@ -202,9 +177,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv4_tc_kernel(Kv4TcParams pp) {
   __shared__ __align__(8) uint64_t q_full, k_full[2], k_empty[2], ks_full[4], v_full[2], v_empty[2], s_full[2][2], p_full[2][2], pv_done[2], o_full;
   __shared__ uint32_t tmem_base;
   __shared__ int abort_flag;
-  // scale and presence of a tile's keys; a slot is written again when both groups are past the tile after it
-  __shared__ __align__(16) float ks_s[4][kTcKeys];
-  __shared__ uint32_t present_s[4][4];
+  // scales and presence of a tile's keys, and the largest exponent of the values' scales (a NaN aside) for each 32 of
+  // them; a slot is written again when both groups are past the tile after it
+  __shared__ __align__(16) float ks_s[4][kTcKeys], vs_s[4][kTcKeys];
+  __shared__ uint32_t present_s[4][4], vexp_s[4][4];
   __shared__ float rf_s[kTcRows];
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
@@ -284,7 +260,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv4_tc_kernel(Kv4TcParams pp) {
     // registers ----
     regs_down<kTcRegsRest>();
     if (warp == 12 && tiles) {
-      constexpr uint32_t kIdS = tc_idesc(64, false, false), kIdO = tc_idesc(D, BF16, true);
+      constexpr uint32_t kIdS = tc_idesc(64, false), kIdO = tc_idesc(D, true);
       // K-major rows of 128 bytes (64 values), blocks of 64 values 16 KB apart
       const uint64_t qd = sm100::smem_desc_sw128(sm100::smem_u32(q_sm), 16, 1024), kd = sm100::smem_desc_sw128(sm100::smem_u32(k_sm), 16, 1024);
       // MN-major: a key's 64 values a row of 128 bytes, 8 keys 1024 bytes, blocks of 64 values 16 KB apart
@@ -335,7 +311,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv4_tc_kernel(Kv4TcParams pp) {
       sm100::mbar_wait(&o_full, 0, pp.fault, KV4_TIMEOUT_DRAIN);
     }
   } else if (warp >= 16) {
-    // ---- values: s (c - z), rounded once; thread = half of a key's ----
+    // ---- values: c - z; thread = half of a key's ----
     regs_down<kTcRegsRest>();
     constexpr int H = W / 2;
     const int key = threadIdx.x & 127, half = (threadIdx.x >> 7) & 1;
@@ -353,17 +329,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv4_tc_kernel(Kv4TcParams pp) {
     for (int i = 0; i < tiles; ++i) {
       uint8_t* const dst = v_sm + (i & 1) * kTile;
       wait(&v_empty[i & 1], ((i >> 1) & 1) ^ 1, KV4_TIMEOUT_TILE);
-      const float vs = kv4_scale(vp);
-      if (row == kNone || vs != vs) {
+      if (row == kNone) {
 #pragma unroll
         for (int w = half * H; w < half * H + H; ++w)
           *reinterpret_cast<uint4*>(dst + (w >> 3) * (kTcKeys * 128) + sw128(key, w & 7)) = make_uint4(0, 0, 0, 0);
-      } else if (BF16) {
-        tc_unpack<H, UNPACK_BF16>(dst, key, half * H, cw, vp & 15u, vs);
-      } else if (vs >= 0x1p-17f && vs < 65504.f) {
-        tc_unpack<H, UNPACK_F16>(dst, key, half * H, cw, vp & 15u, vs);
       } else {
-        tc_unpack<H, UNPACK_F32>(dst, key, half * H, cw, vp & 15u, vs);
+        tc_unpack<H>(dst, key, half * H, cw, vp & 15u);
       }
       sm100::fence_proxy_async();
       __syncwarp();
@@ -391,12 +362,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv4_tc_kernel(Kv4TcParams pp) {
     for (int i = 0; i < tiles; ++i) {
       wait(&k_empty[i & 1], ((i >> 1) & 1) ^ 1, KV4_TIMEOUT_TILE);
       const bool here = row != kNone;
-      const float vs = kv4_scale(vp);
-      // a row of NaN, of K or of V, reaches the rows that see it through their scores
-      ks_s[i & 3][key] = !here ? 0.f : vs != vs ? vs : kv4_scale(kp);
-      const uint32_t there = __ballot_sync(0xffffffffu, here);
-      if (lane == 0) present_s[i & 3][warp - 8] = there;
-      tc_unpack<W, UNPACK_CODES>(k_sm + (i & 1) * kTile, key, 0, cw, kp & 15u, 0.f);
+      const int slot = i & 3;
+      ks_s[slot][key] = here ? kv4_scale(kp) : 0.f;
+      vs_s[slot][key] = here ? kv4_scale(vp) : 0.f;
+      const uint32_t there = __ballot_sync(0xffffffffu, here), ve = here ? (vp >> 23) & 0xffu : 0u;
+      const uint32_t top = __reduce_max_sync(0xffffffffu, ve == 255u ? 0u : ve);
+      if (lane == 0) present_s[slot][warp - 8] = there, vexp_s[slot][warp - 8] = top;
+      tc_unpack<W>(k_sm + (i & 1) * kTile, key, 0, cw, kp & 15u);
       sm100::fence_proxy_async();
       __syncwarp();
       if (lane == 0) {
@@ -467,9 +439,14 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv4_tc_kernel(Kv4TcParams pp) {
       const float rf = rf_s[g * 128 + row];
       const int lim = ok ? (p.causal ? min(s.len, s.p0 + p.div.of(rr) + 1) : s.len) : 0;
       const uint32_t lanes = uint32_t((warp & 3) * 32) << 16, t_s = tmem + lanes + g * 128, t_o = tmem + lanes + 256 + g * 128;
+      // Weights are exp2(s - mu) times the value's scale, l their sum without it, all in units of 2^(127 - ve): ve follows
+      // the exponent of the largest scale among the keys that the row has seen, so that the products fit FP16 whatever
+      // the values' magnitude.  mu and ve move only when a score or a scale passes them by kSlack or kSlackV.
       float mu = 0.f, l = 0.f;
+      int ve = 127;
       bool begun = false;
 
+      int vtop = 0;                              // largest exponent of the values' scales in the tile
       auto step = [&](int j, auto masked_c) {
         constexpr bool kMasked = decltype(masked_c)::value;
         const int slot = (j >> 1) & 3, key0 = j * 64;
@@ -504,13 +481,24 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv4_tc_kernel(Kv4TcParams pp) {
         }
         const float mx = fmaxf(max3(top4[0], top4[1], top4[2]), top4[3]);
         const float top = mx == -INFINITY ? -INFINITY : mx * rf;
-        const bool up = begun ? top > mu + kSlack : mx != -INFINITY;
+        const bool up = begun ? top > mu + kSlack || vtop >= ve + int(kSlackV) : mx != -INFINITY;
         if (__any_sync(0xffffffffu, up)) {
           float corr = 1.f;
           if (mx != -INFINITY) {
+            int v_new = vtop;
+            if (kMasked) {                       // of the keys that this row sees
+              v_new = 0;
+              for (int k = 0; k < 64; ++k) {
+                const int e = (__float_as_uint(vs_s[slot][(j & 1) * 64 + k]) >> 23) & 0xff;
+                if (key0 + k < lim && (present_s[slot][(j & 1) * 2 + k / 32] >> (k & 31) & 1) && e != 255) v_new = max(v_new, e);
+              }
+            }
+            v_new = min(max(v_new, 27), 227);
+            if (begun) v_new = max(v_new, ve);
             const float to = begun ? fmaxf(mu, top) : top;
-            if (begun) corr = exp2_(mu - to);
+            if (begun) corr = exp2_((mu - to) + float(ve - v_new));
             mu = to;
+            ve = v_new;
             begun = true;
           }
           l *= corr;
@@ -528,7 +516,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv4_tc_kernel(Kv4TcParams pp) {
             }
           }
         }
-        const uint64_t rf2 = pack2(rf, rf), mu2 = pack2(-mu, -mu);
+        const float shift = -(mu + float(ve - 127));
+        const uint64_t rf2 = pack2(rf, rf), mu2 = pack2(shift, shift);
+        const ulonglong2* vs = reinterpret_cast<const ulonglong2*>(vs_s[slot] + (j & 1) * 64);
         uint64_t sum2[2] = {0, 0};
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
@@ -547,13 +537,19 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv4_tc_kernel(Kv4TcParams pp) {
 #pragma unroll
           for (int k = 0; k < 32; ++k) x[k] = exp2_(x[k]);
 #pragma unroll
-          for (int k = 0; k < 16; ++k) {
-            sum2[k & 1] = add2(sum2[k & 1], pack2(x[2 * k], x[2 * k + 1]));
-            if (BF16) {
-              const __nv_bfloat162 r = __floats2bfloat162_rn(x[2 * k], x[2 * k + 1]);
-              w[k] = *reinterpret_cast<const uint32_t*>(&r);
-            } else {
-              w[k] = h2_u(__floats2half2_rn(x[2 * k], x[2 * k + 1]));
+          for (int k = 0; k < 16; k += 2) {
+            const ulonglong2 v4 = vs[8 * c + k / 2];
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+              const uint64_t e2 = pack2(x[2 * (k + q)], x[2 * (k + q) + 1]);
+              sum2[q] = add2(sum2[q], e2);
+              float a, e;
+              unpack2(mul2(e2, q ? v4.y : v4.x), a, e);
+              if (kMasked) {                     // a hidden key may hold a NaN scale
+                a = x[2 * (k + q)] == 0.f ? 0.f : a;
+                e = x[2 * (k + q) + 1] == 0.f ? 0.f : e;
+              }
+              w[k + q] = h2_u(__floats2half2_rn(a, e));
             }
           }
           tmem_st16(t_sj + c * 16, w);           // over S columns that have been read
@@ -572,6 +568,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv4_tc_kernel(Kv4TcParams pp) {
         wait(&ks_full[i & 3], (i >> 2) & 1, KV4_TIMEOUT_TILE);
         const uint32_t all = present_s[i & 3][0] & present_s[i & 3][1] & present_s[i & 3][2] & present_s[i & 3][3];
         const bool masked = __any_sync(0xffffffffu, (i + 1) * kTcKeys > lim || all != 0xffffffffu);
+        vtop = max(max(vexp_s[i & 3][0], vexp_s[i & 3][1]), max(vexp_s[i & 3][2], vexp_s[i & 3][3]));
 #pragma unroll
         for (int hh = 0; hh < 2; ++hh) {
           wait(&s_full[g][hh], i & 1, KV4_TIMEOUT_S);
@@ -606,7 +603,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv4_tc_kernel(Kv4TcParams pp) {
       }
       if (ok && p.lse)
         p.lse[int64_t(s.q0 + p.div.of(rr)) * p.hq + h * p.group + p.div.rest(rr)] =
-            l == 0.f ? -INFINITY : (mu + log2f(l)) * 0.69314718055994531f;
+            l == 0.f ? -INFINITY : (mu + float(ve - 127) + log2f(l)) * 0.69314718055994531f;
       __syncwarp();                              // a warp stores its own rows
       {
         constexpr int L = D / 8, R = 32 / L;

@@ -80,16 +80,13 @@ class Batch:
         return x, ok
 
 
-def reference(batch, q, indptr=None, causal=True, scale=None, half=False):
+def reference(batch, q, indptr=None, causal=True, scale=None):
     """(out, lse, tol) float64: the definition, and how far a kernel may be from it before the last rounding.
 
     A score is an FP16 product sum: q is exact in FP16 up to 2^-25 of its row's largest magnitude, codes are whole
     numbers, and D products are added in float32 (at most 2 D 2^-24 of their magnitudes' sum, were each addition cut
     off); two float32 factors follow.  exp2 is good to 2^-21.  A weight p s' is rounded once to FP16: 2^-11 of it, or
-    2^-25 of the unit that brings the largest s' into [1, 2).  Output sums run in float32 over n tokens.
-    half: weights p and values v are rounded to the output's type, each by half a step (prompt chunks).  A value below
-    the smallest normal number is then off by up to half a subnormal step, and since the weights of a row sum to one,
-    so is the row's result: |sum p (v + e)| - |sum p v| <= sum p |e| <= max |e|."""
+    2^-25 of the unit that brings the largest s' into [1, 2).  Output sums run in float32 over n tokens."""
     lens, D = batch.lens, batch.D
     q = q.cpu()
     total, hq, _ = q.shape
@@ -123,8 +120,6 @@ def reference(batch, q, indptr=None, causal=True, scale=None, half=False):
             p = torch.where(z > 0, p / z, p)
             dmax = torch.where(seen[:, None, :], ds, torch.zeros_like(ds)).amax(-1, keepdim=True) if n else 0 * top
             rel = 2.0 ** -11 + 2.0 ** -19 + 2 * dmax + max(n, 1) * 2.0 ** -24
-            if half:
-                rel = rel + 2 * step * (1 + step)
             Vc = torch.where(ok[:, None], V, torch.zeros_like(V))
             out[a:e, h * group:(h + 1) * group] = torch.where(z > 0, p @ Vc, torch.zeros(()).double()) if n else 0.0
             lse[a:e, h * group:(h + 1) * group] = (top + torch.log(z))[..., 0]
@@ -132,7 +127,7 @@ def reference(batch, q, indptr=None, causal=True, scale=None, half=False):
             big = torch.nan_to_num(vs[ids], nan=0.0).max() if n and ok.any() else 0.0
             tol[a:e, h * group:(h + 1) * group] = rel * (p @ Vc.abs() if n else 0.0) + n * 2.0 ** -24 * 15 * float(big)
     tiny = 2.0 ** (-25 if q.dtype == torch.float16 else -134)       # half a subnormal step
-    tol = tol + step * out.abs() * (1 + step) + tiny + (tiny if half else 0)
+    tol = tol + step * out.abs() * (1 + step) + tiny
     return out, lse, tol
 
 

@@ -157,7 +157,7 @@ def test_several_tokens(D, heads, group, page, lens, new, dtype, causal):
     out = torch.full(q.shape, 7.0, dtype=q.dtype, device="cuda")
     got, lse = kv4.attention(q, b.cache, b.d_table, b.d_lens, _i32(ptr), causal=causal, return_lse=True, out=out)
     assert got is out and (out[ptr[-1]:] == 7).all()
-    want, wlse, tol = reference(b, q, ptr, causal, half=True)
+    want, wlse, tol = reference(b, q, ptr, causal)
     check(out, want, tol)
     check_lse(lse, wlse)
 
@@ -207,7 +207,7 @@ def test_pages_without_tokens(new):
     ptr = [0, new, new + 1, new + 2, new + 3]
     q = queries(new + 3, 2, 64, torch.float16)
     out, lse = kv4.attention(q, b.cache, b.d_table, b.d_lens, _i32(ptr), return_lse=True)
-    want, wlse, tol = reference(b, q, ptr, half=True)
+    want, wlse, tol = reference(b, q, ptr)
     check(out, want, tol)
     check_lse(lse, wlse)
     assert not out[new + 1].any()
@@ -222,7 +222,7 @@ def test_magnitudes(dtype, qmul, vmul, new):
     b = Batch([500, 333], 2, 64, 32, vscale=vmul)
     q = queries(2 * new, 4, 64, DT[dtype], mul=qmul)
     out = kv4.attention(q, b.cache, b.d_table, b.d_lens, _i32([0, new, 2 * new]))
-    want, _, tol = reference(b, q, [0, new, 2 * new], half=True)
+    want, _, tol = reference(b, q, [0, new, 2 * new])
     check(out, want, tol)
 
 
@@ -237,7 +237,7 @@ def test_a_loud_token_among_quiet_ones(new):
             t[p, 0, slot] += 20 << 23
         q = queries(new, 1, 64, torch.bfloat16)
         out = kv4.attention(q, b.cache, b.d_table, b.d_lens, _i32([0, new]))
-        want, _, tol = reference(b, q, [0, new], half=True)
+        want, _, tol = reference(b, q, [0, new])
         check(out, want, tol)
 
 
@@ -248,7 +248,7 @@ def test_scale(scale):
     for ptr in ([0, 1, 2], [0, 150, 152]):
         q = queries(ptr[-1], 4, 64, torch.float16)
         out = kv4.attention(q, b.cache, b.d_table, b.d_lens, _i32(ptr), scale=scale)
-        want, _, tol = reference(b, q, ptr, scale=scale, half=True)
+        want, _, tol = reference(b, q, ptr, scale=scale)
         check(out, want, tol)
 
 
