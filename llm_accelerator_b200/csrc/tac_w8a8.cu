@@ -232,14 +232,17 @@ int launch_splitk(const int8_t* A, const int8_t* Bt, W8Params p, cudaStream_t st
   cfg.dynamicSmemBytes = std::max(p.stages * sb, part) + 1024;
   cfg.stream = st;
   cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = 1;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = split;
-  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = p.after_rows ? 2 : 1;
+  if (split > 1) {
+    attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+    attr[cfg.numAttrs].val.clusterDim.x = 1;
+    attr[cfg.numAttrs].val.clusterDim.y = 1;
+    attr[cfg.numAttrs++].val.clusterDim.z = split;
+  }
+  if (p.after_rows) {
+    attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
+  }
   return cudaLaunchKernelEx(&cfg, w8_splitk_kernel<YT>, tw, ta, p) == cudaSuccess ? TAC_OK : TAC_E_CUDA;
 }
 
@@ -378,7 +381,7 @@ int launch_rows(W8RowsParams pp, const int8_t* Bt, cudaStream_t st) {
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = split;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = split > 1;
   return cudaLaunchKernelEx(&cfg, w8_rows_kernel<YT>, tw, pp) == cudaSuccess ? TAC_OK : TAC_E_CUDA;
 }
 

@@ -74,7 +74,7 @@ class Kv4Cache:
                              f"{HEAD_DIMS}")
         self.k_codes, self.k_params, self.v_codes, self.v_params = k_codes, k_params, v_codes, v_params
         self.num_pages, self.heads, self.page_size, self.head_dim = pages, heads, page_size, 2 * half
-        self.device = k_codes.device
+        self.device, self._index = k_codes.device, k_codes.get_device()
         self._record = L.Kv4CacheRecord(k_codes.data_ptr(), v_codes.data_ptr(), k_params.data_ptr(),
                                         v_params.data_ptr(), pages, page_size, heads, 2 * half)
         self._ref = L.C.addressof(self._record)
@@ -93,14 +93,14 @@ def _batch(cache, page_table, lens, indptr, total):
         raise ValueError("page_table must have a column")
     if not (page_table.is_contiguous() and lens.is_contiguous()):
         raise ValueError("page_table and lens must be contiguous")
-    dev = cache.device
-    if page_table.device != dev or lens.device != dev:
+    dev = cache._index
+    if page_table.get_device() != dev or lens.get_device() != dev:
         raise ValueError("page_table and lens must be on the cache's device")
     if indptr is None:
         if total != batch:
             raise ValueError(f"without indptr there is one row a sequence: {batch} sequences, {total} rows")
         return page_table.data_ptr(), lens.data_ptr(), None, batch, width, total
-    if indptr.shape != (batch + 1,) or not indptr.is_contiguous() or indptr.device != dev:
+    if indptr.shape != (batch + 1,) or not indptr.is_contiguous() or indptr.get_device() != dev:
         raise ValueError(f"indptr must be a contiguous [{batch + 1}] tensor on the cache's device")
     return page_table.data_ptr(), lens.data_ptr(), indptr.data_ptr(), batch, width, total
 
@@ -112,7 +112,7 @@ def _rows(x, shape, heads, cache, what):
     stride = x.stride()
     if stride[2] != 1:
         raise ValueError(f"the values of a head must be contiguous in {what}, got strides {stride}")
-    if x.device != cache.device:
+    if x.get_device() != cache._index:
         raise ValueError(f"{what} must be on the cache's device")
     return stride
 
@@ -133,7 +133,7 @@ def append(cache: Kv4Cache, k, v, page_table, lens, indptr=None) -> None:
     total = shape[0]
     args = _batch(cache, page_table, lens, indptr, total)
     if total and args[3]:
-        call("tac_kv4_append", _append, cache.device.index, cache._ref, *args, k.data_ptr(), ks[0], ks[1], v.data_ptr(),
+        call("tac_kv4_append", _append, cache._index, cache._ref, *args, k.data_ptr(), ks[0], ks[1], v.data_ptr(),
              vs[0], vs[1], t)
 
 
@@ -150,7 +150,7 @@ def read(cache: Kv4Cache, page_table, lens, indptr=None, total=None):
     v = torch.empty_like(k)
     if total:
         if args[3]:
-            call("tac_kv4_read", _read, cache.device.index, cache._ref, *args, k.data_ptr(), v.data_ptr())
+            call("tac_kv4_read", _read, cache._index, cache._ref, *args, k.data_ptr(), v.data_ptr())
         else:
             k.zero_()
             v.zero_()
@@ -178,13 +178,13 @@ def attention(q, cache: Kv4Cache, page_table, lens, indptr=None, *, scale=None, 
     args = _batch(cache, page_table, lens, indptr, total)
     if out is None:
         out = q.new_empty(shape)
-    elif out.dtype is not dt or out.shape != shape or not out.is_contiguous() or out.device != cache.device:
+    elif out.dtype is not dt or out.shape != shape or not out.is_contiguous() or out.get_device() != cache._index:
         raise ValueError(f"out must be a contiguous {dt} {tuple(shape)} tensor on q's device")
     lse = torch.empty((total, hq), dtype=_F32, device=cache.device) if return_lse else None
     if total and args[3]:
         need = _workspace_bytes(args[3], args[4], cache.page_size, total, hq, cache.heads, D)
         ws = torch.empty(need, dtype=torch.uint8, device=cache.device) if need else None
-        call("tac_kv4_attention", _attention, cache.device.index, cache._ref, *args, q.data_ptr(), qs[0], qs[1], hq,
+        call("tac_kv4_attention", _attention, cache._index, cache._ref, *args, q.data_ptr(), qs[0], qs[1], hq,
              TYPES[dt], D ** -0.5 if scale is None else scale, causal, out.data_ptr(),
              None if lse is None else lse.data_ptr(), None if ws is None else ws.data_ptr(), need)
     return (out, lse) if return_lse else out

@@ -28,18 +28,18 @@ def _check(rows, Bt, b_scale, bias, out, out_dtype, M, K):
         raise ValueError(f"b_scale must be [{N}], got {tuple(b_scale.shape)}")
     if not (Bt.is_contiguous() and b_scale.is_contiguous()):
         raise ValueError("Bt and b_scale must be contiguous")
-    dev = rows.device
-    if dev.type != "cuda" or Bt.device != dev or b_scale.device != dev:
+    dev = rows.get_device()                       # -1 on the CPU
+    if dev < 0 or Bt.get_device() != dev or b_scale.get_device() != dev:
         raise ValueError("the operands must be on one CUDA device")
     bp, bt = None, 0
     if bias is not None:
         bt = type_code(bias.dtype, "bias")
-        if bias.shape != (N,) or not bias.is_contiguous() or bias.device != dev:
+        if bias.shape != (N,) or not bias.is_contiguous() or bias.get_device() != dev:
             raise ValueError(f"bias must be a contiguous [{N}] tensor on the operands' device")
         bp = bias.data_ptr()
     if out is None:
         out = rows.new_empty((M, N), dtype=out_dtype)
-    elif out.dtype is not out_dtype or out.shape != (M, N) or not out.is_contiguous() or out.device != dev:
+    elif out.dtype is not out_dtype or out.shape != (M, N) or not out.is_contiguous() or out.get_device() != dev:
         raise ValueError(f"out must be a contiguous {out_dtype} [{M}, {N}] tensor on the operands' device")
     return N, out, bp, bt
 
@@ -62,7 +62,7 @@ def gemm_i8_scaled(A, Bt, a_scale, b_scale, bias=None, out_dtype=None, out=None)
     if out_dtype is None:
         out_dtype = _F16 if out is None else out.dtype
     yt = type_code(out_dtype, "out_dtype")
-    if a_scale.device != A.device:
+    if a_scale.get_device() != A.get_device():
         raise ValueError("the operands must be on one CUDA device")
     N, out, bp, bt = _check(A, Bt, b_scale, bias, out, out_dtype, M, K)
     if K == 0 or K % 16:
@@ -101,7 +101,7 @@ def linear_w8a8(X, Bt, b_scale, bias=None, out=None, ws=None):
     if M and N:
         wp, wn = None, 0
         if ws is not None:
-            if ws.device != X.device or ws.dtype is not torch.uint8 or not ws.is_contiguous():
+            if ws.get_device() != X.get_device() or ws.dtype is not torch.uint8 or not ws.is_contiguous():
                 raise ValueError("ws must be a linear_workspace on X's device")
         elif M > 16 or _ws_bytes(M, K):
             ws = linear_workspace(M, K, X.device)

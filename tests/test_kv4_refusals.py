@@ -81,7 +81,7 @@ def test_record_matches_the_header():
 
 class _Fake:
     """What the checks read of a cache, without a GPU."""
-    heads, head_dim, page_size, device = 2, 64, 16, torch.device("cpu")
+    heads, head_dim, page_size, device, _index = 2, 64, 16, torch.device("cpu"), -1
 
 
 def test_python_checks():
