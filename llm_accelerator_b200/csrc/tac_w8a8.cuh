@@ -54,6 +54,52 @@ __device__ __forceinline__ float w8_value(int acc, float as, float bs, float bia
   return fmaf(__fmul_rn(__int2float_rn(acc), as), bs, bias);   // bias 0 where there is none
 }
 
+// The 16-bit case of w8_store32.
+template <int YT, bool ODD>
+__device__ __forceinline__ void w8_store_pairs(const W8Params& p, const uint32_t (&v)[32], const float* as, int m, int n,
+                                               float bs, float bias, uint32_t base_odd) {
+  const int lane = threadIdx.x & 31;
+  // the token of a pair whose row is word-aligned at an even channel: the first one, or with an odd N that of that parity
+  const uint32_t first = ODD ? (base_odd ^ uint32_t(m & 1)) : 0u;   // the warp's first channel is even
+  const bool mine_first = (lane & 1) == 0;                          // even lanes store the aligned token
+  const int tok = mine_first ? int(first) : int(first ^ 1u);
+  uint16_t* dst = static_cast<uint16_t*>(p.y) + int64_t(m + tok) * p.N + n - (mine_first || ODD ? 0 : 1);
+  uint16_t* edge = static_cast<uint16_t*>(p.y) + int64_t(m + int(first ^ 1u)) * p.N + n;
+  const int64_t step = 2 * int64_t(p.N);
+  const uint32_t has_next = lane != 31, is_edge = lane == 0 || lane == 31, edge_shift = first ? 0 : 16;
+  const uint32_t sel = ODD ? (tok ? 0x7632 : 0x5410) : (mine_first ? 0x5410 : 0x3276);
+#pragma unroll
+  for (int j = 0; j < 32; j += 4) {
+    const float4 a = *reinterpret_cast<const float4*>(as + j);
+    const float aa[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+    for (int i = 0; i < 4; i += 2, dst += step, edge += step) {
+      const float y0 = w8_value(int(v[j + i]), aa[i], bs, bias), y1 = w8_value(int(v[j + i + 1]), aa[i + 1], bs, bias);
+      uint32_t mine;                 // the first token's result low, the second's high
+      if constexpr (YT == 1) {
+        const __half2 h = __floats2half2_rn(y0, y1);
+        mine = *reinterpret_cast<const uint32_t*>(&h);
+      } else {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(y0, y1);
+        mine = *reinterpret_cast<const uint32_t*>(&h);
+      }
+      if constexpr (!ODD) {
+        const uint32_t other = __shfl_xor_sync(0xffffffffu, mine, 1);
+        *reinterpret_cast<uint32_t*>(dst) = __byte_perm(mine, other, sel);
+      } else {
+        const uint32_t other = __shfl_down_sync(0xffffffffu, mine, 1);
+        // predicated: a branch for each costs more than the store
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %2, 0;\n\t@p st.global.b32 [%0], %1;\n\t}\n" ::"l"(dst),
+                     "r"(__byte_perm(mine, other, sel)), "r"(has_next)
+                     : "memory");
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %2, 0;\n\t@p st.global.b16 [%0], %1;\n\t}\n" ::"l"(edge),
+                     "h"(uint16_t(mine >> edge_shift)), "r"(is_edge)
+                     : "memory");
+      }
+    }
+  }
+}
+
 // 32 tokens (m .. m + 31) of a warp's 32 consecutive channels (n its own):
 // v the sums, as their scales (shared memory, 16-byte aligned).  A thread has
 // one channel, so 16-bit results are exchanged with the next lane and stored
@@ -78,46 +124,8 @@ __device__ __forceinline__ void w8_store32(const W8Params& p, const uint32_t (&v
       for (int i = 0; i < 4; ++i, dst += p.N) *dst = w8_value(int(v[j + i]), aa[i], bs, bias);
     }
   } else if (YT != 0 && inside && ((p.N & 1) || !base_odd)) {
-    // the token of a pair whose row is word-aligned at an even channel: the first one, or with an odd N that of that parity
-    const bool odd_n = p.N & 1;
-    const uint32_t first = odd_n ? (base_odd ^ uint32_t(m & 1)) : 0u;   // n_warp is even
-    const bool mine_first = (lane & 1) == 0;                            // even lanes store the aligned token
-    const int tok = mine_first ? int(first) : int(first ^ 1u);
-    uint16_t* dst = static_cast<uint16_t*>(p.y) + int64_t(m + tok) * p.N + n - (mine_first || odd_n ? 0 : 1);
-    uint16_t* edge = static_cast<uint16_t*>(p.y) + int64_t(m + int(first ^ 1u)) * p.N + n;
-    const int64_t step = 2 * int64_t(p.N);
-    const uint32_t has_next = lane != 31, is_edge = lane == 0 || lane == 31, edge_shift = first ? 0 : 16;
-    const uint32_t sel = tok ? 0x7632 : 0x5410;
-#pragma unroll
-    for (int j = 0; j < 32; j += 4) {
-      const float4 a = *reinterpret_cast<const float4*>(as + j);
-      const float aa[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-      for (int i = 0; i < 4; i += 2, dst += step, edge += step) {
-        const float y0 = w8_value(int(v[j + i]), aa[i], bs, bias), y1 = w8_value(int(v[j + i + 1]), aa[i + 1], bs, bias);
-        uint32_t mine;               // the first token's result low, the second's high
-        if constexpr (YT == 1) {
-          const __half2 h = __floats2half2_rn(y0, y1);
-          mine = *reinterpret_cast<const uint32_t*>(&h);
-        } else {
-          const __nv_bfloat162 h = __floats2bfloat162_rn(y0, y1);
-          mine = *reinterpret_cast<const uint32_t*>(&h);
-        }
-        if (!odd_n) {
-          const uint32_t other = __shfl_xor_sync(0xffffffffu, mine, 1);
-          *reinterpret_cast<uint32_t*>(dst) = mine_first ? __byte_perm(mine, other, 0x5410) : __byte_perm(other, mine, 0x7632);
-        } else {
-          const uint32_t other = __shfl_down_sync(0xffffffffu, mine, 1);
-          // predicated: a branch for each costs more than the store
-          asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %2, 0;\n\t@p st.global.b32 [%0], %1;\n\t}\n" ::"l"(dst),
-                       "r"(__byte_perm(mine, other, sel)), "r"(has_next)
-                       : "memory");
-          asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %2, 0;\n\t@p st.global.b16 [%0], %1;\n\t}\n" ::"l"(edge),
-                       "h"(uint16_t(mine >> edge_shift)), "r"(is_edge)
-                       : "memory");
-        }
-      }
-    }
+    if (p.N & 1) w8_store_pairs<YT, true>(p, v, as, m, n, bs, bias, base_odd);
+    else w8_store_pairs<YT, false>(p, v, as, m, n, bs, bias, 0u);
   } else {
 #pragma unroll
     for (int j = 0; j < 32; ++j)
@@ -569,7 +577,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg::kThreads, 1
   __shared__ __align__(8) uint64_t full_bar[S], empty_bar[S], acc_full[2], acc_empty[2], drain_bar;
   __shared__ uint32_t tmem_base;
   __shared__ int abort_flag;
-  __shared__ __align__(16) float as_s[2][256];
+  __shared__ __align__(16) float as_s[PairCfg::kEpi / 32][64];
 
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(dyn_smem) + 1023) & ~uintptr_t(1023));
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
@@ -669,16 +677,32 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg::kThreads, 1
     const int part = (warp - 2) >> 2;
     uint32_t local = 0;
     wait_rows();
-    for (int tile = cid; tile < total; tile += ncl, ++local) {
-      const uint32_t b = local & 1, aph = (local >> 1) & 1;
+    // a tile's scales are loaded while the tile before it is finished: its channel's, and a token's of each of the
+    // warp's (at most two) chunks of 32, which go through the warp's own piece of shared memory
+    float bs = 0.f, bias = 0.f, as[2] = {0.f, 0.f};
+    auto scales = [&](int tile) {
       const int n = tile / pp.t_tiles * 256 + int(rank) * 128 + row, m0 = tile % pp.t_tiles * p.tn;
-      float bs = 0.f, bias = 0.f;
+      bs = bias = 0.f;
       if (n < p.N) {
         bs = ld_any(p.b_scale, p.b_type, n);
         if (p.bias) bias = ld_any(p.bias, p.bias_type, n);
       }
-      for (int i = threadIdx.x - 64; i < p.tn; i += PairCfg::kEpi) as_s[b][i] = m0 + i < p.M ? __ldg(p.a_scale + m0 + i) : 0.f;
-      asm volatile("bar.sync 1, %0;\n" ::"n"(PairCfg::kEpi) : "memory");   // as_s[b]: its readers two tiles ago are past the last one
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const int tok = part * 32 + k * (PairCfg::kEpi / 4) + lane;
+        as[k] = tok < p.tn && m0 + tok < p.M ? __ldg(p.a_scale + m0 + tok) : 0.f;
+      }
+    };
+    if (cid < total) scales(cid);
+    for (int tile = cid; tile < total; tile += ncl, ++local) {
+      const uint32_t b = local & 1, aph = (local >> 1) & 1;
+      const int n = tile / pp.t_tiles * 256 + int(rank) * 128 + row, m0 = tile % pp.t_tiles * p.tn;
+      const float bs_now = bs, bias_now = bias;
+      __syncwarp();                              // the warp is done with its last scales
+      as_s[warp - 2][lane] = as[0];
+      as_s[warp - 2][32 + lane] = as[1];
+      __syncwarp();
+      if (tile + ncl < total) scales(tile + ncl);
       if (*abort_v) break;
       if (!sm100::mbar_wait(&acc_full[b], aph, p.fault, W8_TIMEOUT_ACC)) {
         *abort_v = 1;
@@ -686,17 +710,25 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg::kThreads, 1
       }
       __syncwarp();
       sm100::tc_fence_after();
+      // The accumulator is free once its values are in registers.  The arrival is relaxed: as a release it would wait
+      // for the warp's stores of this tile and the last.
+      auto release = [&] {
+        sm100::tc_fence_before();
+        __syncwarp();
+        if (lane == 0)
+          asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];\n" ::"r"(b ? acc_empty0_1 : acc_empty0_0) : "memory");
+      };
+      const int chunks = min(2, max(0, (min(p.tn, p.M - m0) - part * 32 + PairCfg::kEpi / 4 - 1) / (PairCfg::kEpi / 4)));
+      if (chunks == 0) release();
 #pragma unroll 1
-      for (int c = part * 32; c < p.tn; c += PairCfg::kEpi / 4) {
-        if (m0 + c >= p.M) break;
+      for (int k = 0; k < chunks; ++k) {
+        const int c = part * 32 + k * (PairCfg::kEpi / 4);
         uint32_t v[32];
         __syncwarp();
         sm100::tmem_ld32(tmem + (uint32_t((warp & 3) * 32) << 16) + b * 256 + c, v);
-        w8_store32<YT>(p, v, as_s[b] + c, m0 + c, n, bs, bias);
+        if (k == chunks - 1) release();
+        w8_store32<YT>(p, v, as_s[warp - 2] + 32 * k, m0 + c, n, bs_now, bias_now);
       }
-      sm100::tc_fence_before();
-      __syncwarp();
-      if (lane == 0) sm100::mbar_arrive_remote(b ? acc_empty0_1 : acc_empty0_0);
     }
   }
 
