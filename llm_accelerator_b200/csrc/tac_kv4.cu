@@ -142,12 +142,13 @@ __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b, bool f16) {
 // TYPE: TAC_F16 or TAC_BF16 with 16-byte aligned rows; -1: any type and alignment.
 template <int D, int TYPE>
 __global__ void __launch_bounds__(kRowThreads) kv4_append_kernel(RowArgs a) {
-  constexpr int L = D / 16, kRows = kRowThreads / L, kPair = 2;
+  constexpr int L = D / 16, kPair = 2;
+  const int rows = blockDim.x / L;
   const int sub = threadIdx.x % L, lane = threadIdx.x & 31;
   const int64_t t0 = int64_t(blockIdx.x) * a.run;
   const uint32_t mine = lane < a.run && t0 + lane < a.s.total ? token_row(a.c, a.s, int(t0 + lane)) : kNoRow;
   // whole warps take part in every pass: its shuffles name every lane
-  for (int r0 = 0; r0 < 2 * a.c.heads; r0 += kRows) {
+  for (int r0 = 0; r0 < 2 * a.c.heads; r0 += rows) {
     const int r = r0 + int(threadIdx.x) / L;
     const bool in = r < 2 * a.c.heads;
     const int which = r >= a.c.heads, head = in ? r - (which ? a.c.heads : 0) : 0;
@@ -287,18 +288,20 @@ int take_seqs(const int32_t* table, const int32_t* lens, const int32_t* indptr, 
   return TAC_OK;
 }
 
-// Tokens of a CTA: one while every token finds an SM to itself, then as many as keep six CTAs an SM, to the lanes' 32.
+// Tokens of a CTA: one while every token finds an SM to itself, then as many as keep twelve CTAs an SM, to the lanes' 32.
 void set_run(RowArgs& a, int* grid) {
-  const int64_t ctas = int64_t(sm_count()) * 6;
+  const int64_t ctas = int64_t(sm_count()) * 12;
   a.run = ctas > 0 ? int(std::max<int64_t>(1, std::min<int64_t>(32, (a.s.total + ctas - 1) / ctas))) : 0;
   *grid = a.run ? int((int64_t(a.s.total) + a.run - 1) / a.run) : 0;
 }
 
 template <int D>
 void launch_append(const RowArgs& a, int grid, cudaStream_t st) {
-  if (a.vec && a.type == TAC_F16) kv4_append_kernel<D, TAC_F16><<<grid, kRowThreads, 0, st>>>(a);
-  else if (a.vec && a.type == TAC_BF16) kv4_append_kernel<D, TAC_BF16><<<grid, kRowThreads, 0, st>>>(a);
-  else kv4_append_kernel<D, -1><<<grid, kRowThreads, 0, st>>>(a);
+  // no more threads than a token's rows keep busy
+  const int threads = std::min(kRowThreads, (2 * a.c.heads * (D / 16) + 31) / 32 * 32);
+  if (a.vec && a.type == TAC_F16) kv4_append_kernel<D, TAC_F16><<<grid, threads, 0, st>>>(a);
+  else if (a.vec && a.type == TAC_BF16) kv4_append_kernel<D, TAC_BF16><<<grid, threads, 0, st>>>(a);
+  else kv4_append_kernel<D, -1><<<grid, threads, 0, st>>>(a);
 }
 
 // ---- attention ------------------------------------------------------------------------------------------------------

@@ -120,6 +120,35 @@ __device__ __forceinline__ uint32_t kv4_pair8(uint32_t x) {
 // 64 + z of a parameter word as a float: z in the bits worth 1 .. 8 at 64.
 __device__ __forceinline__ float kv4_zero64(uint32_t word) { return __uint_as_float(word * (1u << 17) + 0x42800000u); }
 
+// Two float32 operations an instruction.
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpack2(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
 __device__ __forceinline__ float exp2_(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -450,23 +479,26 @@ __global__ void __launch_bounds__(kRowsThreads, rows_ctas(D, NT)) kv4_rows_kerne
             mma_16816(sc[u][n], p20, p21, p30, p31, qf[n][2 * w + 1][0], qf[n][2 * w + 1][1]);
           }
         }
-      // scores less mu (0 for a row that has seen no key yet)
+      // scores less mu (0 for a row that has seen no key yet), two rows at a time
       float hot = -INFINITY;
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
+      for (int n = 0; n < NT; ++n) {
+        const uint64_t qs2 = pack2(qs[n][0], qs[n][1]), qsum2 = pack2(qsum[n][0], qsum[n][1]), mu2 = pack2(-mu[n][0], -mu[n][1]);
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const float ks = kv4_scale(kpw[u][j]), kz = kv4_zero64(kpw[u][j]);
+        for (int u = 0; u < 2; ++u)
 #pragma unroll
-          for (int n = 0; n < NT; ++n)
+          for (int j = 0; j < 2; ++j) {
+            const float ks = kv4_scale(kpw[u][j]), kz = -kv4_zero64(kpw[u][j]);
+            float v[2];
+            unpack2(fma2(fma2(pack2(kz, kz), qsum2, pack2(sc[u][n][2 * j], sc[u][n][2 * j + 1])), mul2(pack2(ks, ks), qs2), mu2), v[0], v[1]);
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-              float v = fmaf(sc[u][n][2 * j + i] - kz * qsum[n][i], ks * qs[n][i], -mu[n][i]);
-              if (kMasked && !seen(u, j, n, i)) v = -INFINITY;
-              hot = fmaxf(hot, v);
-              sc[u][n][2 * j + i] = v;
+              if (kMasked && !seen(u, j, n, i)) v[i] = -INFINITY;
+              sc[u][n][2 * j + i] = v[i];
             }
-        }
+            hot = max3(hot, v[0], v[1]);
+          }
+      }
       // ---- softmax over the keys of this warp ----
       const uint32_t vtop = max(max(vpw[0][0], vpw[0][1]), max(vpw[1][0], vpw[1][1]));
       if (__any_sync(0xffffffffu, kMasked || hot > kSlack || vtop >= vlim)) {
@@ -521,25 +553,27 @@ __global__ void __launch_bounds__(kRowsThreads, rows_ctas(D, NT)) kv4_rows_kerne
       uint32_t pb[2][NT][2];
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        const float down[2] = {__uint_as_float((254u - ve[n][0]) << 23), __uint_as_float((254u - ve[n][1]) << 23)};
+        const uint64_t down2 = pack2(__uint_as_float((254u - ve[n][0]) << 23), __uint_as_float((254u - ve[n][1]) << 23));
+        uint64_t l2 = pack2(l[n][0], l[n][1]), zo2 = pack2(zo[n][0], zo[n][1]);
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
             const float vs = kv4_scale(vpw[u][j]), vz = kv4_zero64(vpw[u][j]) - 72.f;
+            const uint64_t e2 = pack2(exp2_(sc[u][n][2 * j]), exp2_(sc[u][n][2 * j + 1]));
+            l2 = add2(l2, e2);
             float w[2];
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              const float e = exp2_(sc[u][n][2 * j + i]);
-              l[n][i] += e;
-              w[i] = e * (vs * down[i]);
-              if (kMasked && !seen(u, j, n, i)) w[i] = 0.f;   // a key that this row does not see may hold a NaN scale
+            unpack2(mul2(e2, mul2(pack2(vs, vs), down2)), w[0], w[1]);
+            if (kMasked) {                          // a key that this row does not see may hold a NaN scale
+              if (!seen(u, j, n, 0)) w[0] = 0.f;
+              if (!seen(u, j, n, 1)) w[1] = 0.f;
             }
             const __half2 w2 = __floats2half2_rn(w[0], w[1]);
-            zo[n][0] += __low2float(w2) * vz;
-            zo[n][1] += __high2float(w2) * vz;
+            zo2 = fma2(pack2(__low2float(w2), __high2float(w2)), pack2(vz, vz), zo2);
             pb[u][n][j] = movmatrix(h2_u(w2));
           }
+        unpack2(l2, l[n][0], l[n][1]);
+        unpack2(zo2, zo[n][0], zo[n][1]);
       }
       // ---- O^T ----
 #pragma unroll
