@@ -2,6 +2,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <cmath>
 #include <cstdint>
 
 #include "../../include/taccel_b200.h"
@@ -356,8 +357,15 @@ int launch_rows(Kv4RowsParams p, void* workspace, cudaStream_t st) {
   return cudaLaunchKernelEx(&cfg, kv4_join_kernel<D, NT>, p) == cudaSuccess ? TAC_OK : TAC_E_CUDA;
 }
 
-// Prompt chunks: 256 rows a CTA, from 32 rows a sequence and key-value head on.
-bool use_tc(int batch, int total, int group) { return int64_t(total) * group > int64_t(32) * batch; }
+// The prompt kernel (256 rows a CTA, one CTA an SM) where it is faster than the row kernel, whose time goes with all
+// rows: measured per key, 3.6e-6 us a row and key-value head against 0.025 us a round of CTAs over the SMs at D = 128,
+// 2.3e-6 against 0.021 at D = 64 (64 rows for each of 64 heads: 63 us by rows, 136 by the prompt kernel; 512 rows for
+// each of 16: 113 and 103).  The rows of a sequence are taken at their mean.
+bool use_tc(int batch, int total, int group, int kv_heads, int head_dim) {
+  const double rows = double(total) * group / batch, units = double(batch) * kv_heads;
+  const double rounds = std::max(1.0, units * std::ceil(rows / kTcRows) / 148);
+  return units * rows > (head_dim == 128 ? 8000 : 10500) * rounds;
+}
 
 template <int D, bool BF16>
 int launch_tc(const Kv4RowsParams& r, cudaStream_t st) {
@@ -426,7 +434,7 @@ extern "C" uint64_t tac_kv4_attention_workspace_bytes(int batch, int width, int 
       (head_dim != 64 && head_dim != 128))
     return 0;
   const int group = q_heads / kv_heads, nt = rows_tiles(batch, total, group);
-  if (use_tc(batch, total, group) || !rows_split(batch, width, page_size, total, q_heads, kv_heads, nt)) return 0;
+  if (use_tc(batch, total, group, kv_heads, head_dim) || !rows_split(batch, width, page_size, total, q_heads, kv_heads, nt)) return 0;
   return rows_workspace(head_dim, nt);
 }
 
@@ -459,7 +467,7 @@ extern "C" int tac_kv4_attention(const tac_kv4_cache* cache, const int32_t* page
   p.q_vec = aligned(Q, 16) && (q_tok | q_head) % 8 == 0;
   if (sm_count() <= 0) return TAC_E_CUDA;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (use_tc(batch, total, p.group)) {
+  if (use_tc(batch, total, p.group, p.c.heads, cache->head_dim)) {
     if (cache->head_dim == 64) return p.bf16 ? launch_tc<64, true>(p, st) : launch_tc<64, false>(p, st);
     return p.bf16 ? launch_tc<128, true>(p, st) : launch_tc<128, false>(p, st);
   }

@@ -409,7 +409,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv4_tc_kernel(Kv4TcParams pp) {
       __syncwarp();                              // rf_s: a warp reads what it wrote
       if (lane == 0) sm100::mbar_arrive(&q_full);
       const float rf = rf_s[g * 128 + row];
-      const int lim = ok ? (p.causal ? min(s.len, s.p0 + p.div.of(rr) + 1) : s.len) : 0;
+      // keys below it are seen; a row past the last one is a row of zeros that nothing stores, and needs no mask
+      const int lim = ok && p.causal ? min(s.len, s.p0 + p.div.of(rr) + 1) : s.len;
       const uint32_t lanes = uint32_t((warp & 3) * 32) << 16, t_s = tmem + lanes + g * 128, t_o = tmem + lanes + 256 + g * 128;
       // Weights are exp2(s - mu) times the value's scale, l their sum without it, all in units of 2^(127 - ve): ve follows
       // the exponent of the largest scale among the keys that the row has seen, so that the products fit FP16 whatever

@@ -2,12 +2,18 @@
 (tests/kv4_helpers.py derives the tolerances)."""
 from __future__ import annotations
 
+import subprocess
+import sys
+import textwrap
+from pathlib import Path
+
 import pytest
 import torch
 
 from kv4_helpers import Batch, check, check_lse, pack, quantise, queries, reference, values
 
 pytestmark = pytest.mark.gpu
+ROOT = Path(__file__).resolve().parent.parent
 DT = {"f16": torch.float16, "bf16": torch.bfloat16, "f32": torch.float32}
 
 
@@ -117,6 +123,8 @@ DECODE = [
     (128, 8, 4, 64, [127, 128, 129, 1000, 0, 64]), (128, 4, 8, 128, [5000, 1]), (128, 2, 7, 16, [300, 77]),
     (64, 1, 16, 32, [500, 1, 0]), (128, 1, 32, 64, [513, 40]), (64, 3, 9, 64, [256, 255]), (64, 12, 1, 16, [64] * 9),
     (128, 1, 1, 16, [20011]), (64, 2, 2, 16, list(range(0, 150))),
+    # more sequences than threads of a CTA, with and without a context that is shared out
+    (64, 1, 2, 16, [i * 7 % 60 for i in range(600)]), (64, 1, 1, 16, [i * 7 % 60 for i in range(599)] + [5000]),
 ]
 
 
@@ -139,6 +147,10 @@ SEVERAL = [
     (128, 1, 5, 16, [500, 0, 20], [17, 0, 20]), (64, 2, 8, 128, [300, 10], [2, 7]), (64, 4, 2, 16, [33, 1], [33, 1]),
     (128, 8, 4, 64, [700, 333], [260, 333]), (64, 3, 1, 32, [1030], [513]), (128, 1, 16, 128, [260], [130]),
     (64, 2, 3, 64, [5, 9, 200], [8, 9, 130]),       # more rows than positions: the first rows see nothing
+    # enough rows for the prompt kernel: partial row blocks and tiles, one and two row groups, many sequences
+    (128, 8, 4, 64, [300, 333], [300, 200]), (64, 8, 2, 16, [700, 129, 64], [700, 100, 64]), (64, 16, 1, 128, [1030], [900]),
+    (128, 2, 5, 32, [900], [850]), (64, 2, 3, 64, [500, 9, 1100], [600, 11, 1101]), (128, 1, 16, 16, [640, 0], [640, 0]),
+    (64, 2, 8, 16, list(range(20, 90)), [20] * 70),
 ]
 
 
@@ -162,11 +174,11 @@ def test_several_tokens(D, heads, group, page, lens, new, dtype, causal):
     check_lse(lse, wlse)
 
 
-@pytest.mark.parametrize("new", [1, 3, 200])
+@pytest.mark.parametrize("new", [1, 3, 200, 1500])
 def test_what_unused_slots_hold_does_not_matter(new):
     """Slots past a sequence's end and pages of no sequence: zeros, NaN words and infinities give the same bits."""
     from llm_accelerator_b200 import kv4
-    lens = [230, 201, 300]
+    lens = [230, 201, 300] if new <= 200 else [1530, 1501, 1600]
     ptr = [0, new, 2 * new, 3 * new]
     q = queries(3 * new, 6, 64, torch.float16)
     outs = []
@@ -177,10 +189,10 @@ def test_what_unused_slots_hold_does_not_matter(new):
         assert torch.equal(o, outs[0][0]) and torch.equal(l, outs[0][1])
 
 
-@pytest.mark.parametrize("new", [1, 4, 150])
+@pytest.mark.parametrize("new", [1, 4, 150, 2300])
 def test_a_nan_token_reaches_only_the_rows_that_see_it(new):
     from llm_accelerator_b200 import kv4
-    n = 400
+    n = 400 if new < 400 else 2500
     for which in (0, 1):
         b = Batch([n], 2, 128, 32)
         pos = n - (new + 1) // 2                       # among the new tokens, seen by the rows from there on
@@ -193,12 +205,12 @@ def test_a_nan_token_reaches_only_the_rows_that_see_it(new):
         assert torch.equal(got[:first], clean[:first]) and torch.equal(got[:, :2], clean[:, :2])
 
 
-@pytest.mark.parametrize("new", [1, 200])
+@pytest.mark.parametrize("new", [1, 200, 5400])
 def test_pages_without_tokens(new):
     """Page numbers outside the cache, inside and at the ends of a sequence, hold no keys; a sequence of none of them
     gives zeros."""
     from llm_accelerator_b200 import kv4
-    b = Batch([400, 400, 300, 33], 2, 64, 16)
+    b = Batch([400 if new < 400 else 6000, 400, 300, 33], 2, 64, 16)
     b.table[0, 0] = -1
     b.table[0, 7:11] = b.pages
     b.table[1, 12:] = 2 ** 31 - 1
@@ -213,25 +225,25 @@ def test_pages_without_tokens(new):
     assert not out[new + 1].any()
 
 
-@pytest.mark.parametrize("new", [1, 140])
+@pytest.mark.parametrize("new", [1, 140, 1500])
 @pytest.mark.parametrize("dtype,qmul,vmul", [("f16", 1.0, 1e-6), ("f16", 60.0, 1.0), ("bf16", 1.0, 1e30),
                                              ("bf16", 1e-20, 1e-30), ("f16", 1e-6, 4000.0), ("bf16", 40.0, 1e-3)])
 def test_magnitudes(dtype, qmul, vmul, new):
     """Values near the ends of the types' ranges, and scores of some hundreds (one key takes it all)."""
     from llm_accelerator_b200 import kv4
-    b = Batch([500, 333], 2, 64, 32, vscale=vmul)
+    b = Batch([500, 333] if new < 300 else [1600, 1520], 2, 64, 32, vscale=vmul)
     q = queries(2 * new, 4, 64, DT[dtype], mul=qmul)
     out = kv4.attention(q, b.cache, b.d_table, b.d_lens, _i32([0, new, 2 * new]))
     want, _, tol = reference(b, q, [0, new, 2 * new])
     check(out, want, tol)
 
 
-@pytest.mark.parametrize("new", [1, 130])
+@pytest.mark.parametrize("new", [1, 130, 10600])
 def test_a_loud_token_among_quiet_ones(new):
     """One token with values 2^20 times the others', early and late: no weight is lost on either side of it."""
     from llm_accelerator_b200 import kv4
-    for pos in (3, 250, 580):
-        b = Batch([700], 1, 64, 16)
+    for pos in (3, 250, 580) if new < 700 else (3, 5000, 10690):
+        b = Batch([700 if new < 700 else 10700], 1, 64, 16)
         p, slot = int(b.table[0, pos // 16]), pos % 16
         for t in (b.host[3], b.cache.v_params):
             t[p, 0, slot] += 20 << 23
@@ -245,7 +257,7 @@ def test_a_loud_token_among_quiet_ones(new):
 def test_scale(scale):
     from llm_accelerator_b200 import kv4
     b = Batch([200, 90], 2, 64, 16)
-    for ptr in ([0, 1, 2], [0, 150, 152]):
+    for ptr in ([0, 1, 2], [0, 150, 152], [0, 3000, 3002]):
         q = queries(ptr[-1], 4, 64, torch.float16)
         out = kv4.attention(q, b.cache, b.d_table, b.d_lens, _i32(ptr), scale=scale)
         want, _, tol = reference(b, q, ptr, scale=scale)
@@ -351,6 +363,41 @@ def test_malformed_offsets_stay_inside():
         kv4.append(b.cache, x, x, b.d_table, _i32(lens), _i32(ptr))
         kv4.read(b.cache, b.d_table, _i32(lens), _i32(ptr), total=10)
     torch.cuda.synchronize()
+
+
+def test_first_calls_inside_a_capture():
+    """In a fresh process the first append, attention (both kernels) and products are captured, then replayed."""
+    code = textwrap.dedent(f"""
+        import sys
+        sys.path[:0] = [{str(ROOT)!r}, {str(ROOT / 'tests')!r}]
+        import torch
+        from llm_accelerator_b200 import gemm, kv4
+        i32 = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")
+        g = torch.Generator(device="cuda").manual_seed(0)
+        cache = kv4.Kv4Cache(80, 16, 4, 64)
+        table = torch.arange(80, dtype=torch.int32, device="cuda").view(1, 80)
+        k = torch.randn((1200, 4, 64), generator=g, device="cuda").half()
+        q = torch.randn((1200, 16, 64), generator=g, device="cuda").half()
+        lens, ptr = i32([1200]), i32([0, 1200])
+        xs = [torch.randn((m, 256), generator=g, device="cuda").half() for m in (1, 40, 1024)]
+        w, s = torch.randint(-127, 128, (5000, 256), dtype=torch.int8, device="cuda", generator=g), torch.rand(5000, generator=g, device="cuda")
+        def calls():
+            kv4.append(cache, k, k, table, lens, ptr)
+            a = kv4.attention(q, cache, table, lens, ptr)
+            return [a, kv4.attention(q[-1:], cache, table, lens), *(gemm.linear_w8a8(x, w, s) for x in xs)]
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = calls()
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in got]
+        assert all(torch.equal(a, b) for a, b in zip(got, calls()))
+        assert all(t.isfinite().all() for t in got)
+        print("ok")
+    """)
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and r.stdout.strip().endswith("ok"), r.stdout + r.stderr
 
 
 def test_nothing_to_do():

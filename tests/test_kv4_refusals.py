@@ -71,8 +71,8 @@ def test_workspace_query():
     assert f(0, 99, 64, 1, 4, 2, 64) == 0 and f(1, 99, 64, 0, 4, 2, 64) == 0 and f(1, 99, 64, 1, 3, 2, 64) == 0
     assert f(1, 99, 64, 1, 4, 2, 80) == 0
     assert f(1, 16, 64, 1, 4, 2, 64) == 0            # short contexts are not split
-    assert f(1, 99, 64, 99, 4, 2, 64) == 0           # nor are prompts
-    assert f(1, 99, 64, 1, 4, 2, 64) > 0
+    assert f(1, 99, 64, 4000, 32, 8, 64) == 0        # nor are prompts
+    assert f(1, 99, 64, 1, 4, 2, 64) > 0 and f(1, 99, 64, 99, 4, 2, 64) > 0
 
 
 def test_record_matches_the_header():
