@@ -9,7 +9,9 @@ classes keep the reference interfaces:
 * ``HostRunner``     - drop-in for ``taccel.runtime.host_runner.HostRunner``
 * ``BatchedRunner``  - many sequences per GPU, greedy decode on device
 * ``ProgramBundle``  - the reference bundle format, with file I/O
-* ``gemm``           - stand-alone INT8 GEMM kernels with requant epilogues
+* ``gemm``           - stand-alone INT8 GEMM kernels with requant epilogues, INT8 linear layers with a scale for
+  each token and channel
+* ``kv4``            - 4-bit paged key / value cache and attention over it
 """
 from .bundle import ProgramBundle, RelocationSite, RuntimeConfigAttnSite, RuntimePatchSite  # noqa: F401
 from .errors import (ConfigError, DRAMAccessError, EngineError, IllegalBufferError,  # noqa: F401
@@ -25,6 +27,6 @@ def __getattr__(name):
     import importlib
     if name in _LAZY:
         return getattr(importlib.import_module(f".{_LAZY[name]}", __name__), name)
-    if name == "gemm":
-        return importlib.import_module(".gemm", __name__)
+    if name in ("gemm", "kv4"):
+        return importlib.import_module(f".{name}", __name__)
     raise AttributeError(name)

@@ -14,7 +14,14 @@
 // of its own, which it fills two or three tiles ahead by 16-byte asynchronous
 // copies; nothing waits for another warp before the unit's end.  (Bulk copies,
 // one for the 512 bytes that a head has of 16 keys, need an instruction for
-// each, lane by lane: 132 us instead of LATER at the 64-sequence case.)
+// each, lane by lane: 132 us instead of 114 for 64 ragged sequences.)
+//
+// Bound by instructions and their latency, not by the cache's bytes: unpacking
+// a code takes as many instructions as the products with it, 2.2 are issued a
+// clock with 16 warps an SM (125 registers a thread).  64 sequences of
+// 1000..8192 tokens, 32 query heads over 8 of 128 values: 96 us (3.1 TB/s; 91
+// with the loads left out, 72 with loads alone).  Two of 100,001..131,072 over
+// 4 heads: 40 us, of which 14 do not go with the length, and 6 for the join.
 //
 // Work is laid end to end over all (sequence, head, row block) units.  Where a
 // sequence can be long (p.split), the CTAs take equal shares of its tiles

@@ -14,7 +14,8 @@
 // group: while a group's threads are at one step's softmax the tensor core
 // does P V of the step before and S of the step after it.  (Whole tiles of 128
 // keys, one S a group, left a group's threads and the tensor core waiting for
-// each other: 353 us for the ragged chunks of which this takes LATER.)  Per
+// each other: 353 us for ragged chunks of 5,596 rows of 32 heads, of
+// which this took 335.)  Per
 // tile and group D = 128 needs 1024 tensor clocks, and 1024 clocks of the
 // exponential unit.
 //
@@ -22,6 +23,11 @@
 // the cache's side.  The keys' scales multiply S in float32, the values' scales
 // the weights before these are rounded to FP16, once; the query is FP16, scaled
 // by a power of two for each row.  So nothing is rounded to BF16 but the result.
+// Bound by the chain S, softmax, P, O of a group's step and the issue of its
+// MMAs: 640 TFLOP/s at those chunks (337 us), tensor pipe 31 % and exponential
+// unit 33 % busy, an eighth of the time in the CTAs' prologues.  One S product
+// of 128 keys for two steps (366 us) and softmax steps pipelined within a
+// thread at 192 registers (387 us) were slower.
 // TMEM: two S of each group (64 columns; P takes the first half of its S), then
 // O of both.
 #pragma once

@@ -110,6 +110,7 @@ __global__ void __launch_bounds__(kQrThreads) quant_rows_kernel(const T* __restr
 // 2 read and 1 written a value; the rounding is one addition of 1.5 * 2^23,
 // after which the low byte is the code, and a byte permutation packs four
 // (a convert instruction a value alone took as long as the memory).
+// 8192 x 4096: 18.5 us, 5.4 TB/s.
 template <typename T, int WPR>
 __global__ void __launch_bounds__(kQrThreads) quant_rows_vec_kernel(const T* __restrict__ X, int64_t ldx,
                                                                     int8_t* __restrict__ Q, int ldq,
