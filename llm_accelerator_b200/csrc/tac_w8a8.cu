@@ -315,7 +315,7 @@ int check_product(const void* Bt, const void* b_scale, int b_type, const void* b
   if (!Bt || !b_scale || !Y || M <= 0 || N <= 0 || K <= 0) return TAC_E_ARGUMENT;
   if ((b_type != TAC_F32 && b_type != TAC_F16) || !type_ok(y_type) || (bias && !type_ok(bias_type))) return TAC_E_ARGUMENT;
   if (!aligned(Y, y_type == TAC_F32 ? 4 : 2) || !aligned(b_scale, b_type == TAC_F32 ? 4 : 2)) return TAC_E_ARGUMENT;
-  if (K >= (1 << 17) || M > (1 << 20) || !aligned(Bt, 16)) return TAC_E_ARGUMENT;   // |sum| <= K * 128^2 < 2^31
+  if (K >= (1 << 17) || M > (1 << 20) || N > (1 << 30) || !aligned(Bt, 16)) return TAC_E_ARGUMENT;   // |sum| <= K * 128^2 < 2^31
   return TAC_OK;
 }
 

@@ -27,6 +27,14 @@ __device__ __forceinline__ float ld_any(const void* p, int type, int64_t i) {
   return type == 1 ? __half2float(__ushort_as_half(b)) : __uint_as_float(uint32_t(b) << 16);
 }
 
+// the same in two steps: the element's bits (the load is still under way), and their value
+__device__ __forceinline__ uint32_t ld_bits(const void* p, int type, int64_t i) {
+  return type == 0 ? __ldg(static_cast<const uint32_t*>(p) + i) : uint32_t(__ldg(static_cast<const uint16_t*>(p) + i));
+}
+__device__ __forceinline__ float bits_value(uint32_t b, int type) {
+  return type == 0 ? __uint_as_float(b) : type == 1 ? __half2float(__ushort_as_half(uint16_t(b))) : __uint_as_float(b << 16);
+}
+
 template <int YT>
 __device__ __forceinline__ void st_y(void* p, int64_t i, float v) {
   if constexpr (YT == 0) static_cast<float*>(p)[i] = v;
@@ -66,37 +74,39 @@ __device__ __forceinline__ void w8_store_pairs(const W8Params& p, const uint32_t
   uint16_t* dst = static_cast<uint16_t*>(p.y) + int64_t(m + tok) * p.N + n - (mine_first || ODD ? 0 : 1);
   uint16_t* edge = static_cast<uint16_t*>(p.y) + int64_t(m + int(first ^ 1u)) * p.N + n;
   const int64_t step = 2 * int64_t(p.N);
-  const uint32_t has_next = lane != 31, is_edge = lane == 0 || lane == 31, edge_shift = first ? 0 : 16;
+  const bool has_next = !ODD || lane != 31, is_edge = lane == 0 || lane == 31;
+  const uint32_t edge_shift = first ? 0 : 16;
   const uint32_t sel = ODD ? (tok ? 0x7632 : 0x5410) : (mine_first ? 0x5410 : 0x3276);
+  // all exchanges first: between the stores each would wait behind them
+  uint32_t mine[16], other[16];      // the first token's result low, the second's high
 #pragma unroll
-  for (int j = 0; j < 32; j += 4) {
-    const float4 a = *reinterpret_cast<const float4*>(as + j);
+  for (int j = 0; j < 16; j += 2) {
+    const float4 a = *reinterpret_cast<const float4*>(as + 2 * j);
     const float aa[4] = {a.x, a.y, a.z, a.w};
 #pragma unroll
-    for (int i = 0; i < 4; i += 2, dst += step, edge += step) {
-      const float y0 = w8_value(int(v[j + i]), aa[i], bs, bias), y1 = w8_value(int(v[j + i + 1]), aa[i + 1], bs, bias);
-      uint32_t mine;                 // the first token's result low, the second's high
+    for (int i = 0; i < 2; ++i) {
+      const float y0 = w8_value(int(v[2 * (j + i)]), aa[2 * i], bs, bias), y1 = w8_value(int(v[2 * (j + i) + 1]), aa[2 * i + 1], bs, bias);
       if constexpr (YT == 1) {
         const __half2 h = __floats2half2_rn(y0, y1);
-        mine = *reinterpret_cast<const uint32_t*>(&h);
+        mine[j + i] = *reinterpret_cast<const uint32_t*>(&h);
       } else {
         const __nv_bfloat162 h = __floats2bfloat162_rn(y0, y1);
-        mine = *reinterpret_cast<const uint32_t*>(&h);
+        mine[j + i] = *reinterpret_cast<const uint32_t*>(&h);
       }
-      if constexpr (!ODD) {
-        const uint32_t other = __shfl_xor_sync(0xffffffffu, mine, 1);
-        *reinterpret_cast<uint32_t*>(dst) = __byte_perm(mine, other, sel);
-      } else {
-        const uint32_t other = __shfl_down_sync(0xffffffffu, mine, 1);
-        // predicated: a branch for each costs more than the store
-        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %2, 0;\n\t@p st.global.b32 [%0], %1;\n\t}\n" ::"l"(dst),
-                     "r"(__byte_perm(mine, other, sel)), "r"(has_next)
-                     : "memory");
-        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %2, 0;\n\t@p st.global.b16 [%0], %1;\n\t}\n" ::"l"(edge),
-                     "h"(uint16_t(mine >> edge_shift)), "r"(is_edge)
-                     : "memory");
-      }
+      other[j + i] = ODD ? __shfl_down_sync(0xffffffffu, mine[j + i], 1) : __shfl_xor_sync(0xffffffffu, mine[j + i], 1);
     }
+  }
+  // predicated: a branch for each costs more than the store.  Of the pairs' rows, those below M are stored.
+  const int left = p.M - m - tok, left_edge = is_edge ? p.M - m - int(first ^ 1u) : 0, left_here = has_next ? left : 0;
+#pragma unroll
+  for (int j = 0; j < 16; ++j, dst += step, edge += step) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.gt.s32 p, %2, %3;\n\t@p st.global.b32 [%0], %1;\n\t}\n" ::"l"(dst),
+                 "r"(__byte_perm(mine[j], other[j], sel)), "r"(left_here), "r"(2 * j)
+                 : "memory");
+    if constexpr (ODD)
+      asm volatile("{\n\t.reg .pred p;\n\tsetp.gt.s32 p, %2, %3;\n\t@p st.global.b16 [%0], %1;\n\t}\n" ::"l"(edge),
+                   "h"(uint16_t(mine[j] >> edge_shift)), "r"(left_edge), "r"(2 * j)
+                   : "memory");
   }
 }
 
@@ -106,13 +116,14 @@ __device__ __forceinline__ void w8_store_pairs(const W8Params& p, const uint32_t
 // in pairs: of two tokens, the even lanes store one's pairs and the odd lanes
 // the other's.  Where N is odd every second row begins between two words; its
 // pairs are those of an odd lane and the next, its first and last channel go
-// alone.  (Four warps with an element's own 16-bit store and 30 instructions
+// alone.  Exchanges go before stores, behind which each would wait (4.1 us of
+// 29 at 333 x 50257 x 768).  (Four warps with an element's own 16-bit store and 30 instructions
 // each took 91 us at 4096^3, the MMAs 34.)
 template <int YT>
 __device__ __forceinline__ void w8_store32(const W8Params& p, const uint32_t (&v)[32], const float* as, int m, int n,
                                            float bs, float bias) {
   const int lane = threadIdx.x & 31, n_warp = n - lane;
-  const bool inside = m + 32 <= p.M && n_warp + 32 <= p.N;
+  const bool all_channels = n_warp + 32 <= p.N, inside = all_channels && m + 32 <= p.M;
   const uint32_t base_odd = uint32_t(reinterpret_cast<uintptr_t>(p.y) >> 1) & 1;
   if (YT == 0 && inside) {
     float* dst = static_cast<float*>(p.y) + int64_t(m) * p.N + n;
@@ -123,7 +134,7 @@ __device__ __forceinline__ void w8_store32(const W8Params& p, const uint32_t (&v
 #pragma unroll
       for (int i = 0; i < 4; ++i, dst += p.N) *dst = w8_value(int(v[j + i]), aa[i], bs, bias);
     }
-  } else if (YT != 0 && inside && ((p.N & 1) || !base_odd)) {
+  } else if (YT != 0 && all_channels && ((p.N & 1) || !base_odd)) {
     if (p.N & 1) w8_store_pairs<YT, true>(p, v, as, m, n, bs, bias, base_odd);
     else w8_store_pairs<YT, false>(p, v, as, m, n, bs, bias, 0u);
   } else {
@@ -686,13 +697,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg::kThreads, 1
     wait_rows();
     // a tile's scales are loaded while the tile before it is finished: its channel's, and a token's of each of the
     // warp's (at most two) chunks of 32, which go through the warp's own piece of shared memory
-    float bs = 0.f, bias = 0.f, as[2] = {0.f, 0.f};
-    auto scales = [&](int tile) {
-      const int n = tile / pp.t_tiles * 256 + int(rank) * 128 + row, m0 = tile % pp.t_tiles * p.tn;
-      bs = bias = 0.f;
+    uint32_t bs = 0, bias = 0;
+    float as[2] = {0.f, 0.f};
+    // a tile's first token and this thread's channel; from one tile to the next without a division, which every warp
+    // would do between its stores and its next wait
+    const int step_w = ncl / pp.t_tiles, step_t = ncl % pp.t_tiles;
+    int t_next = cid % pp.t_tiles, n_next = cid / pp.t_tiles * 256 + int(rank) * 128 + row;
+    auto scales = [&] {
+      const int n = n_next, m0 = t_next * p.tn;
+      bs = bias = 0;
       if (n < p.N) {
-        bs = ld_any(p.b_scale, p.b_type, n);
-        if (p.bias) bias = ld_any(p.bias, p.bias_type, n);
+        bs = ld_bits(p.b_scale, p.b_type, n);
+        if (p.bias) bias = ld_bits(p.bias, p.bias_type, n);
       }
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
@@ -700,18 +716,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg::kThreads, 1
         as[k] = tok < p.tn && m0 + tok < p.M ? __ldg(p.a_scale + m0 + tok) : 0.f;
       }
     };
-    if (cid < total) scales(cid);
+    scales();                                    // cid < total: there are no more pairs than tiles
     for (int tile = cid; tile < total; tile += ncl, ++local) {
       const uint32_t b = local & 1, aph = (local >> 1) & 1;
-      const int n = tile / pp.t_tiles * 256 + int(rank) * 128 + row, m0 = tile % pp.t_tiles * p.tn;
-      const float bs_now = bs, bias_now = bias;
+      const int n = n_next, m0 = t_next * p.tn;
+      const float bs_now = bits_value(bs, p.b_type), bias_now = bits_value(bias, p.bias_type);
       __syncwarp();                              // the warp is done with its last scales
       as_s[warp - 2][lane] = as[0];
       as_s[warp - 2][32 + lane] = as[1];
       __syncwarp();
-      if (tile + ncl < total) scales(tile + ncl);
-      if (*abort_v) break;
-      if (!sm100::mbar_wait(&acc_full[b], aph, p.fault, W8_TIMEOUT_ACC)) {
+      t_next += step_t;
+      n_next += step_w * 256;
+      if (t_next >= pp.t_tiles) t_next -= pp.t_tiles, n_next += 256;
+      if (tile + ncl < total) scales();
+      if (!sm100::mbar_try_wait(&acc_full[b], aph) &&
+          (*abort_v || !sm100::mbar_wait(&acc_full[b], aph, p.fault, W8_TIMEOUT_ACC))) {
         *abort_v = 1;
         break;
       }
