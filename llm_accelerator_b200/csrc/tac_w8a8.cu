@@ -198,8 +198,8 @@ bool map_rows(CUtensorMap* m, const int8_t* base, int K, int rows, int box_rows)
 constexpr int kSkMaxSmem = 224 * 1024;
 
 // CTAs that share a tile's K blocks: as many as find an SM each, with eight K blocks or more a CTA (two for 16 tokens,
-// whose partial sums are few).  Measured: 64 x 4096 x 1024 takes 7.2 us whole and 8.3 us in four, 64 x 4096 x 4096 12.1
-// and 10.9, 1 x 4096 x 4096 10.0 and 7.7; more CTAs than SMs cost 1 x 4096 x 1024 1.7 us.
+// whose partial sums are few).  Measured, four CTAs a tile against one: 64 x 4096 x 1024 loses 1.1 us of 7, 64 x 4096 x
+// 4096 gains 1.2 of 12, 1 x 4096 x 4096 2.3 of 10; more CTAs than SMs cost 1 x 4096 x 1024 1.7 us.
 int splits(int64_t tiles, int k_blocks, int tn, int sms) {
   int split = 1;
   while (split < 8 && 2 * split * (tn > 16 ? 8 : 2) <= k_blocks && tiles * split * 2 <= sms) split *= 2;

@@ -116,9 +116,10 @@ __device__ __forceinline__ void w8_store_pairs(const W8Params& p, const uint32_t
 // in pairs: of two tokens, the even lanes store one's pairs and the odd lanes
 // the other's.  Where N is odd every second row begins between two words; its
 // pairs are those of an odd lane and the next, its first and last channel go
-// alone.  Exchanges go before stores, behind which each would wait (4.1 us of
-// 29 at 333 x 50257 x 768).  (Four warps with an element's own 16-bit store and 30 instructions
-// each took 91 us at 4096^3, the MMAs 34.)
+// alone (3 us of 24 at 333 x 50257 x 768; collecting them for one store of all
+// rows took as long).  Exchanges go before the stores, behind which each would
+// wait (29 us).  (Four warps with an element's own 16-bit store and 30
+// instructions each took 91 us at 4096^3, the MMAs 34.)
 template <int YT>
 __device__ __forceinline__ void w8_store32(const W8Params& p, const uint32_t (&v)[32], const float* as, int m, int n,
                                            float bs, float bias) {
@@ -151,7 +152,7 @@ __device__ __forceinline__ void w8_store32(const W8Params& p, const uint32_t (&v
 // (integer sums: the split never changes a result).  For products with too
 // few tiles for 148 SMs, where streaming the weights is the work.
 //   warp 0      TMA loads of both operands, warp 1 MMAs, warps 2..5 epilogue.
-// Bound by latency at these sizes: 64 x 4096 x 1024 takes 7.1 us, 0.7 of them
+// Bound by latency at these sizes: 64 x 4096 x 1024 takes 5.6 us, 0.7 of them
 // for its bytes; launch, TMA, MMA and store each wait for the one before.
 constexpr int kSkThreads = 192;
 constexpr int kSkWBytes = 128 * 128;
@@ -572,7 +573,7 @@ __global__ void __launch_bounds__(kSkThreads) w8_rows_kernel(const __grid_consta
 // loops whole and one elected lane issues, so that descriptors stay in uniform
 // registers (4096^3: 87 us with a single thread's loop, 50 with this).
 // 4096^3: 2750 TOPS, tensor pipe 79 % busy, L2 hit rate 87 %.  Outputs wider
-// than K is deep are bound by the stores (333 x 50257 x 768: 29 us).
+// than K is deep are bound by the stores (333 x 50257 x 768: 24 us).
 struct PairCfg {
   static constexpr int kStages = 6;
   static constexpr int kStageBytes = 2 * 16384;
