@@ -194,7 +194,7 @@ struct Cuts {
   // the share that tile x lies in
   __device__ uint32_t share(uint32_t x) const {
     const uint32_t big = rem * (base + 1);
-    return x < big ? x / (base + 1) : rem + (x - big) / base;
+    return min(x < big ? x / (base + 1) : rem + (x - big) / base, parts - 1);
   }
 };
 
@@ -211,8 +211,10 @@ __device__ inline Start find_start(const Kv4RowsParams& p, int rows, uint32_t gr
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const bool one = p.s.batch <= kRowsThreads;    // a thread for each sequence: one pass does
   Start st;
-  st.first = 0;
+  st.x0 = st.x1 = st.first = 0;
   st.b = p.s.batch;
+  // sequences that share rows (offsets that go back) can have more tiles than 32 bits count: then nothing may be found
+  if (threadIdx.x == 0) *found = st;
   uint32_t base = 0;
   for (int pass = one ? 1 : 0; pass < 2; ++pass) {
     base = 0;

@@ -362,6 +362,11 @@ def test_malformed_offsets_stay_inside():
         kv4.attention(q, b.cache, b.d_table, _i32(lens), _i32(ptr))
         kv4.append(b.cache, x, x, b.d_table, _i32(lens), _i32(ptr))
         kv4.read(b.cache, b.d_table, _i32(lens), _i32(ptr), total=10)
+    # many sequences that all claim the same rows, contexts whole and shared out, by both kernels
+    for hist, T, heads in (([40] * 300, 300, 2), ([40] * 299 + [3000], 300, 2), ([700] * 8, 9000, 6)):
+        b = Batch(hist, heads, 64, 16)
+        ptr = _i32([0, T] * (len(hist) // 2) + [0])
+        assert kv4.attention(queries(T, heads, 64, torch.float16), b.cache, b.d_table, b.d_lens, ptr).shape == (T, heads, 64)
     torch.cuda.synchronize()
 
 
