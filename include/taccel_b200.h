@@ -350,8 +350,9 @@ int tac_quantize_rows_i8(const void* X, int x_type, int64_t ldx, int8_t* Q, floa
 /* Y[M,N] (y_type) = (A[M,K] @ Bt[N,K]^T) * a_scale[m] * b_scale[n] (+ bias[n]):
  * INT8 x INT8 with exact int32 sums, ((float(sum) * a_scale) * b_scale) + bias
  * in float32 and one rounding.  A, Bt row-major and 16-byte aligned, K a
- * multiple of 16 below 2^17; any M up to 2^20 and any N.  b_scale is TAC_F32
- * or TAC_F16 (the type tac_quantize_weight_i8 writes); bias may be null.
+ * multiple of 16 below 2^17; any M up to 2^20 and N up to 2^30.  b_scale is
+ * TAC_F32 or TAC_F16 (the type tac_quantize_weight_i8 writes); bias may be null.
+ * Floating-point arrays are aligned to their elements.
  * Asynchronous on `stream`; tac_gemm_status reports device faults. */
 int tac_gemm_i8_scaled(const int8_t* A, const int8_t* Bt, const float* a_scale, const void* b_scale,
                        int b_scale_type, const void* bias, int bias_type, void* Y, int y_type, int M, int N,

@@ -398,7 +398,7 @@ extern "C" int tac_kv4_append(const tac_kv4_cache* cache, const int32_t* page_ta
   if (int s = take_cache(cache, a.c)) return s;
   if (int s = take_seqs(page_table, lens, indptr, batch, width, total, a.c, a.s)) return s;
   if (!K || !V || (type != TAC_F32 && type != TAC_F16 && type != TAC_BF16) || k_tok < 0 || k_head < 0 || v_tok < 0 ||
-      v_head < 0)
+      v_head < 0 || !aligned(K, type == TAC_F32 ? 4 : 2) || !aligned(V, type == TAC_F32 ? 4 : 2))
     return TAC_E_ARGUMENT;
   a.x[0] = K, a.x[1] = V;
   a.tok[0] = k_tok, a.tok[1] = v_tok;

@@ -314,7 +314,8 @@ int check_product(const void* Bt, const void* b_scale, int b_type, const void* b
                   int y_type, int M, int N, int K) {
   if (!Bt || !b_scale || !Y || M <= 0 || N <= 0 || K <= 0) return TAC_E_ARGUMENT;
   if ((b_type != TAC_F32 && b_type != TAC_F16) || !type_ok(y_type) || (bias && !type_ok(bias_type))) return TAC_E_ARGUMENT;
-  if (!aligned(Y, y_type == TAC_F32 ? 4 : 2) || !aligned(b_scale, b_type == TAC_F32 ? 4 : 2)) return TAC_E_ARGUMENT;
+  auto elem = [](int type) { return type == TAC_F32 ? 4 : 2; };
+  if (!aligned(Y, elem(y_type)) || !aligned(b_scale, elem(b_type)) || (bias && !aligned(bias, elem(bias_type)))) return TAC_E_ARGUMENT;
   if (K >= (1 << 17) || M > (1 << 20) || N > (1 << 30) || !aligned(Bt, 16)) return TAC_E_ARGUMENT;   // |sum| <= K * 128^2 < 2^31
   return TAC_OK;
 }
@@ -393,7 +394,8 @@ uint64_t align256(uint64_t v) { return (v + 255) & ~uint64_t(255); }
 
 extern "C" int tac_quantize_rows_i8(const void* X, int x_type, int64_t ldx, int8_t* Q, float* scale, int M, int K,
                                     void* stream) {
-  if (!X || !Q || !scale || !type_ok(x_type) || M <= 0 || K <= 0 || (M > 1 && ldx < K) || !aligned(Q, 16))
+  if (!X || !Q || !scale || !type_ok(x_type) || M <= 0 || K <= 0 || (M > 1 && ldx < K) || !aligned(Q, 16) ||
+      !aligned(X, x_type == TAC_F32 ? 4 : 2) || !aligned(scale, 4))
     return TAC_E_ARGUMENT;
   return launch_quant_rows(X, x_type, ldx, Q, scale, M, K, static_cast<cudaStream_t>(stream));
 }
@@ -401,7 +403,7 @@ extern "C" int tac_quantize_rows_i8(const void* X, int x_type, int64_t ldx, int8
 extern "C" int tac_gemm_i8_scaled(const int8_t* A, const int8_t* Bt, const float* a_scale, const void* b_scale,
                                   int b_scale_type, const void* bias, int bias_type, void* Y, int y_type, int M, int N,
                                   int K, void* stream) {
-  if (!A || !a_scale || K % 16 || !aligned(A, 16)) return TAC_E_ARGUMENT;
+  if (!A || !a_scale || K % 16 || !aligned(A, 16) || !aligned(a_scale, 4)) return TAC_E_ARGUMENT;
   if (int s = check_product(Bt, b_scale, b_scale_type, bias, bias_type, Y, y_type, M, N, K)) return s;
   return run_product(A, Bt, a_scale, b_scale, b_scale_type, bias, bias_type, Y, y_type, M, N, K, false,
                      static_cast<cudaStream_t>(stream));
@@ -415,7 +417,7 @@ extern "C" uint64_t tac_linear_w8a8_workspace_bytes(int M, int K) {
 extern "C" int tac_linear_w8a8(const void* X, int x_type, int64_t ldx, const int8_t* Bt, const void* b_scale,
                                int b_scale_type, const void* bias, int bias_type, void* Y, int y_type, void* workspace,
                                uint64_t workspace_bytes, int M, int N, int K, void* stream) {
-  if (!X || !type_ok(x_type) || (M > 1 && ldx < K)) return TAC_E_ARGUMENT;
+  if (!X || !type_ok(x_type) || (M > 1 && ldx < K) || !aligned(X, x_type == TAC_F32 ? 4 : 2)) return TAC_E_ARGUMENT;
   if (int s = check_product(Bt, b_scale, b_scale_type, bias, bias_type, Y, y_type, M, N, K)) return s;
   const int Kp = (K + 15) / 16 * 16;
   cudaStream_t st = static_cast<cudaStream_t>(stream);

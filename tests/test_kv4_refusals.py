@@ -50,7 +50,8 @@ def test_cache_and_batch(call):
         assert call(seqs=_seqs(**bad)) == L.E_ARGUMENT, bad
 
 
-@pytest.mark.parametrize("bad", [dict(K=None), dict(V=None), dict(t=3), dict(ks=(-1, 64)), dict(vs=(128, -64))])
+@pytest.mark.parametrize("bad", [dict(K=None), dict(V=None), dict(t=3), dict(ks=(-1, 64)), dict(vs=(128, -64)),
+                                 dict(K=C.c_void_p(4097)), dict(V=C.c_void_p(4098), t=L.TYPE_F32)])
 def test_append(bad):
     assert _append(**bad) == L.E_ARGUMENT
 

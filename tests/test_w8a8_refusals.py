@@ -28,20 +28,23 @@ def _rows(X=P, xt=L.TYPE_F16, ldx=32, Q=P, s=P, M=4, K=32):
 
 @pytest.mark.parametrize("bad", [dict(A=None), dict(Bt=None), dict(sa=None), dict(sb=None), dict(Y=None), dict(M=0),
                                  dict(N=-1), dict(K=0), dict(K=40), dict(A=ODD), dict(Bt=ODD), dict(sbt=L.TYPE_BF16),
-                                 dict(yt=3), dict(bias=P, bt=7), dict(K=1 << 17), dict(M=(1 << 20) + 1)])
+                                 dict(yt=3), dict(bias=P, bt=7), dict(K=1 << 17), dict(M=(1 << 20) + 1),
+                                 dict(N=(1 << 30) + 1), dict(Y=C.c_void_p(4097)), dict(Y=C.c_void_p(4098), yt=L.TYPE_F32),
+                                 dict(sb=C.c_void_p(4098)), dict(sb=C.c_void_p(4097), sbt=L.TYPE_F16), dict(sa=C.c_void_p(4098)),
+                                 dict(bias=C.c_void_p(4097), bt=L.TYPE_BF16)])
 def test_gemm_refusals(bad):
     assert _gemm(**bad) == L.E_ARGUMENT
 
 
 @pytest.mark.parametrize("bad", [dict(X=None), dict(Bt=None), dict(sb=None), dict(Y=None), dict(ws=None),
                                  dict(ws=C.c_void_p(4096 + 16)), dict(wn=100), dict(ldx=31), dict(xt=3), dict(yt=-1),
-                                 dict(M=0), dict(N=0), dict(K=-5), dict(Bt=ODD), dict(K=1 << 17)])
+                                 dict(M=0), dict(N=0), dict(K=-5), dict(Bt=ODD), dict(K=1 << 17), dict(X=C.c_void_p(4097))])
 def test_linear_refusals(bad):
     assert _linear(**bad) == L.E_ARGUMENT
 
 
 @pytest.mark.parametrize("bad", [dict(X=None), dict(Q=None), dict(s=None), dict(xt=3), dict(ldx=31), dict(Q=ODD),
-                                 dict(M=0), dict(K=0)])
+                                 dict(M=0), dict(K=0), dict(X=C.c_void_p(4098), xt=L.TYPE_F32), dict(s=C.c_void_p(4098))])
 def test_quantize_rows_refusals(bad):
     assert _rows(**bad) == L.E_ARGUMENT
 
