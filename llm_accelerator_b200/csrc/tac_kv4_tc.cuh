@@ -162,7 +162,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv4_tc_kernel(Kv4TcParams pp) {
   __shared__ float rf_s[kTcRows];
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-  // ---- this CTA's rows: later row blocks, which see more keys, come first ----
+  // ---- this CTA's rows: later row blocks, which see more keys, come first (sequences by length instead of by number
+  // made no difference) ----
   const int h = blockIdx.x % p.c.heads;
   int blk = pp.blocks - 1 - int(blockIdx.x / p.c.heads), b = 0;
   const int64_t cap = int64_t(p.s.width) * p.c.page_size;
