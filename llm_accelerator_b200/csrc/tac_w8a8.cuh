@@ -571,8 +571,8 @@ __global__ void __launch_bounds__(kSkThreads) w8_rows_kernel(const __grid_consta
 // loads, warp 1 issues the MMAs, 16 warps are the epilogue; waits as in
 // tac_gemm_tc2.cuh, and no load uses multicast.  Both issuing warps run their
 // loops whole and one elected lane issues, so that descriptors stay in uniform
-// registers (4096^3: 87 us with a single thread's loop, 50 with this).
-// 4096^3: 2750 TOPS, tensor pipe 79 % busy, L2 hit rate 87 %.  Outputs wider
+// registers (4096^3: 87 us with a single thread's loop, 49 with this).
+// 4096^3: 2800 TOPS, tensor pipe 80 % busy, L2 hit rate 84 %.  Outputs wider
 // than K is deep are bound by the stores (333 x 50257 x 768: 24 us).
 struct PairCfg {
   static constexpr int kStages = 6;
