@@ -245,9 +245,14 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv4_tc_kernel(Kv4TcParams pp) {
       // MN-major: a key's 64 values a row of 128 bytes, 8 keys 1024 bytes, blocks of 64 values 16 KB apart
       const uint64_t vd = sm100::smem_desc_sw128(sm100::smem_u32(v_sm), kTcKeys * 128, 1024);
       const int steps = 2 * tiles;
+      // the warp's own waits have one verdict: elect.sync needs every lane
+      bool go = true;
+      auto wait_all = [&](uint64_t* bar, uint32_t parity, int code) {
+        go = go && sm100::mbar_wait_warp(bar, parity, abort_v, pp.fault, code);
+      };
       auto qk = [&](int j, int g) {              // S of step j: 64 keys are 8 KB of each block
         const uint64_t qg = qd + g * (kTile >> 4), ki = kd + ((j >> 1) & 1) * (kTile >> 4) + (j & 1) * (8192 >> 4);
-        if (!*abort_v && sm100::elect_one()) {
+        if (go && sm100::elect_one()) {
 #pragma unroll
           for (int k = 0; k < D / 16; ++k) {
             const uint32_t o = ((k >> 2) * (kTcKeys * 128) + (k & 3) * 32) >> 4;
@@ -258,22 +263,22 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv4_tc_kernel(Kv4TcParams pp) {
         }
         __syncwarp();
       };
-      wait(&q_full, 0, KV4_TIMEOUT_TILE);
-      wait(&k_full[0], 0, KV4_TIMEOUT_TILE);
+      wait_all(&q_full, 0, KV4_TIMEOUT_TILE);
+      wait_all(&k_full[0], 0, KV4_TIMEOUT_TILE);
       sm100::tc_fence_after();
       for (int j = 0; j < 2; ++j)
         for (int g = 0; g < groups; ++g) qk(j, g);
       for (int j = 0; j < steps; ++j) {
         if (!(j & 1)) {
           const int i = j >> 1;
-          wait(&v_full[i & 1], (i >> 1) & 1, KV4_TIMEOUT_TILE);
-          if (i + 1 < tiles) wait(&k_full[(i + 1) & 1], ((i + 1) >> 1) & 1, KV4_TIMEOUT_TILE);
+          wait_all(&v_full[i & 1], (i >> 1) & 1, KV4_TIMEOUT_TILE);
+          if (i + 1 < tiles) wait_all(&k_full[(i + 1) & 1], ((i + 1) >> 1) & 1, KV4_TIMEOUT_TILE);
         }
         const uint64_t vi = vd + ((j >> 1) & 1) * (kTile >> 4) + (j & 1) * (4 * 2048 >> 4);
         for (int g = 0; g < groups; ++g) {
-          wait(&p_full[g][j & 1], (j >> 1) & 1, KV4_TIMEOUT_P);
+          wait_all(&p_full[g][j & 1], (j >> 1) & 1, KV4_TIMEOUT_P);
           sm100::tc_fence_after();
-          if (!*abort_v && sm100::elect_one()) {
+          if (go && sm100::elect_one()) {
 #pragma unroll
             for (int k = 0; k < 4; ++k)
               mma_f16_ts(tmem + 256 + g * 128, tmem + g * 128 + (j & 1) * 64 + k * 8, vi + k * (2048 >> 4), kIdO, j || k);

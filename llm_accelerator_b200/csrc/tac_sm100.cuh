@@ -67,6 +67,24 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, int* e
   return false;
 }
 
+// The same for a whole warp, which gets one verdict: its lanes poll, run out
+// and see the CTA's abort flag at different times, and a loop that some of
+// them leave would wait for good at its next elect.sync, __syncwarp or tcgen05
+// access.  False where the phase is not complete and the flag is set, which a
+// wait that runs out does.
+__device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* err,
+                                               int code) {
+  if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+  for (uint32_t i = 0; i < kSpinLimit; ++i) {
+    if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+    if (__any_sync(0xffffffffu, *abort_flag != 0)) return false;
+    if (i > 1024) __nanosleep(32);
+  }
+  *abort_flag = 1;
+  if (err) atomicCAS(err, 0, code);
+  return false;
+}
+
 // 2-D TMA tile load into shared memory, completing on `bar` (tx bytes).
 __device__ __forceinline__ void tma_load_2d(void* smem_dst, const CUtensorMap* map, int32_t c0, int32_t c1,
                                            uint64_t* bar) {

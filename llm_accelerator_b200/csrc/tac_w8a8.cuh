@@ -274,10 +274,7 @@ __global__ void __launch_bounds__(kSkThreads)
     __syncwarp();
     wait_rows();
     for (int kb = kb0; kb < kb1; ++kb) {
-      if (!sm100::mbar_wait(&empty_bar[s], ph, p.fault, W8_TIMEOUT_EMPTY) || *abort_v) {
-        *abort_v = 1;
-        break;
-      }
+      if (!sm100::mbar_wait_warp(&empty_bar[s], ph, abort_v, p.fault, W8_TIMEOUT_EMPTY)) break;
       if (sm100::elect_one()) {
         uint8_t* st = smem + s * stage_bytes;
         if (kb - kb0 >= early) {
@@ -298,10 +295,7 @@ __global__ void __launch_bounds__(kSkThreads)
     const uint64_t w0 = sm100::smem_desc_sw128(sm100::smem_u32(smem), 16, 1024);
     uint32_t s = 0, ph = 0;
     for (int kb = kb0; kb < kb1; ++kb) {
-      if (!sm100::mbar_wait(&full_bar[s], ph, p.fault, W8_TIMEOUT_FULL) || *abort_v) {
-        *abort_v = 1;
-        break;
-      }
+      if (!sm100::mbar_wait_warp(&full_bar[s], ph, abort_v, p.fault, W8_TIMEOUT_FULL)) break;
       sm100::tc_fence_after();
       const uint64_t dw = w0 + s * (stage_bytes >> 4);
       if (sm100::elect_one()) {
@@ -330,7 +324,7 @@ __global__ void __launch_bounds__(kSkThreads)
     wait_rows();
     for (int i = threadIdx.x - 64; i < p.tn; i += 128) as_s[i] = m0 + i < p.M ? __ldg(p.a_scale + m0 + i) : 0.f;
     asm volatile("bar.sync 1, 128;\n" ::: "memory");   // as_s, among the epilogue's warps
-    acc_ok = sm100::mbar_wait(&acc_bar, 0, p.fault, W8_TIMEOUT_ACC);
+    acc_ok = sm100::mbar_wait_warp(&acc_bar, 0, abort_v, p.fault, W8_TIMEOUT_ACC);
     __syncwarp();
     sm100::tc_fence_after();
   }
@@ -466,10 +460,7 @@ __global__ void __launch_bounds__(kSkThreads) w8_rows_kernel(const __grid_consta
   if (warp == 0) {
     uint32_t s = 0, ph = 1, issued = 0;
     for (int kb = kb0; kb < kb1; ++kb) {
-      if (!sm100::mbar_wait(&empty_bar[s], ph, p.fault, W8_TIMEOUT_EMPTY) || *abort_v) {
-        *abort_v = 1;
-        break;
-      }
+      if (!sm100::mbar_wait_warp(&empty_bar[s], ph, abort_v, p.fault, W8_TIMEOUT_EMPTY)) break;
       if (kb - kb0 >= early && sm100::elect_one()) {
         sm100::mbar_arrive_expect_tx(&full_bar[s], kSkWBytes);
         sm100::tma_load_2d(smem + s * kSkWBytes, &tm_w, kb * 128, n0, &full_bar[s]);
@@ -485,13 +476,10 @@ __global__ void __launch_bounds__(kSkThreads) w8_rows_kernel(const __grid_consta
     const uint32_t idesc = sm100::idesc_i8(128, kTn, 0);
     const uint64_t w0 = sm100::smem_desc_sw128(sm100::smem_u32(smem), 16, 1024);
     const uint64_t r0 = sm100::smem_desc_sw128(sm100::smem_u32(rows_sm), 16, 1024);
-    if (!sm100::mbar_wait(&rows_bar, 0, p.fault, W8_TIMEOUT_FULL)) *abort_v = 1;
+    const bool rows = sm100::mbar_wait_warp(&rows_bar, 0, abort_v, p.fault, W8_TIMEOUT_FULL);
     uint32_t s = 0, ph = 0;
-    for (int kb = kb0; kb < kb1; ++kb) {
-      if (*abort_v || !sm100::mbar_wait(&full_bar[s], ph, p.fault, W8_TIMEOUT_FULL)) {
-        *abort_v = 1;
-        break;
-      }
+    for (int kb = kb0; rows && kb < kb1; ++kb) {
+      if (!sm100::mbar_wait_warp(&full_bar[s], ph, abort_v, p.fault, W8_TIMEOUT_FULL)) break;
       sm100::tc_fence_after();
       const uint64_t dw = w0 + s * (kSkWBytes >> 4), dr = r0 + (kb - kb0) * (kTn * 128 >> 4);
       if (sm100::elect_one()) {
@@ -549,7 +537,7 @@ __global__ void __launch_bounds__(kSkThreads) w8_rows_kernel(const __grid_consta
       bs = ld_any(p.b_scale, p.b_type, n);
       if (p.bias) bias = ld_any(p.bias, p.bias_type, n);
     }
-    acc_ok = sm100::mbar_wait(&acc_bar, 0, p.fault, W8_TIMEOUT_ACC);
+    acc_ok = sm100::mbar_wait_warp(&acc_bar, 0, abort_v, p.fault, W8_TIMEOUT_ACC);
     __syncwarp();
     sm100::tc_fence_after();
   }
@@ -627,13 +615,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg::kThreads, 1
   if (warp == 0) {
     uint32_t s = 0, ph = 1, issued = 0;
     wait_rows();
-    for (int tile = cid; tile < total && !*abort_v; tile += ncl) {
+    bool go = true;
+    for (int tile = cid; go && tile < total; tile += ncl) {
       const int n0 = tile / pp.t_tiles * 256 + int(rank) * 128, m0 = tile % pp.t_tiles * p.tn + int(rank) * half;
       for (int kb = 0; kb < p.k_blocks; ++kb) {
-        if (!sm100::mbar_wait(&empty_bar[s], ph, p.fault, W8_TIMEOUT_EMPTY) || *abort_v) {
-          *abort_v = 1;
-          break;
-        }
+        go = sm100::mbar_wait_warp(&empty_bar[s], ph, abort_v, p.fault, W8_TIMEOUT_EMPTY);
+        if (!go) break;
         if (sm100::elect_one()) {
           if (rank == 0) sm100::mbar_arrive_expect_tx(&full_bar[s], 2 * (16384 + half * 128));
           const uint32_t bar0 = sm100::mapa_shared(&full_bar[s], 0);
@@ -656,20 +643,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg::kThreads, 1
       const uint32_t idesc = sm100::idesc_i8(256, p.tn, 0);
       const uint64_t w0 = sm100::smem_desc_sw128(sm100::smem_u32(smem), 16, 1024);
       uint32_t s = 0, ph = 0, local = 0;
-      for (int tile = cid; tile < total && !*abort_v; tile += ncl, ++local) {
+      for (int tile = cid; tile < total; tile += ncl, ++local) {
         const uint32_t b = local & 1, aph = (local >> 1) & 1;
-        if (!sm100::mbar_wait(&acc_empty[b], aph ^ 1, p.fault, W8_TIMEOUT_ACC)) {
-          *abort_v = 1;
-          break;
-        }
+        if (!sm100::mbar_wait_warp(&acc_empty[b], aph ^ 1, abort_v, p.fault, W8_TIMEOUT_ACC)) break;
         sm100::tc_fence_after();
         bool ok = true;
         for (int kb = 0; kb < p.k_blocks; ++kb) {
-          if (!sm100::mbar_wait(&full_bar[s], ph, p.fault, W8_TIMEOUT_FULL) || *abort_v) {
-            *abort_v = 1;
-            ok = false;
-            break;
-          }
+          ok = sm100::mbar_wait_warp(&full_bar[s], ph, abort_v, p.fault, W8_TIMEOUT_FULL);
+          if (!ok) break;
           sm100::tc_fence_after();
           const uint64_t dw = w0 + s * (PairCfg::kStageBytes >> 4);
           if (sm100::elect_one()) {
@@ -730,12 +711,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg::kThreads, 1
       n_next += step_w * 256;
       if (t_next >= pp.t_tiles) t_next -= pp.t_tiles, n_next += 256;
       if (tile + ncl < total) scales();
-      if (!sm100::mbar_try_wait(&acc_full[b], aph) &&
-          (*abort_v || !sm100::mbar_wait(&acc_full[b], aph, p.fault, W8_TIMEOUT_ACC))) {
-        *abort_v = 1;
-        break;
-      }
-      __syncwarp();
+      if (!sm100::mbar_wait_warp(&acc_full[b], aph, abort_v, p.fault, W8_TIMEOUT_ACC)) break;
       sm100::tc_fence_after();
       // The accumulator is free once its values are in registers.  The arrival is relaxed: as a release it would wait
       // for the warp's stores of this tile and the last.

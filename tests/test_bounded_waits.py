@@ -1,0 +1,29 @@
+"""The kernels whose warps issue whole, with one elected lane (tac_w8a8.cuh, tac_kv4_tc.cuh), read as text: a wait that
+runs out cannot be caused without breaking a kernel, so what is checked is that no lane acts on a verdict of its own."""
+from __future__ import annotations
+
+import re
+from pathlib import Path
+
+import pytest
+
+CSRC = Path(__file__).resolve().parent.parent / "llm_accelerator_b200" / "csrc"
+FILES = sorted(p.name for p in CSRC.glob("*.cuh") if "elect_one()" in p.read_text() and p.name != "tac_sm100.cuh")
+
+
+def test_the_files_are_found():
+    assert {"tac_w8a8.cuh", "tac_kv4_tc.cuh"} <= set(FILES)
+
+
+@pytest.mark.parametrize("name", FILES)
+def test_no_lane_leaves_a_loop_by_itself(name):
+    """elect.sync, __syncwarp and tcgen05 accesses wait for every lane.  Per-lane waits are those whose verdict nothing
+    but the abort flag takes; what an elected lane does depends on no lane's own read of that flag."""
+    for line in (CSRC / name).read_text().splitlines():
+        if "mbar_wait(" in line or "mbar_try_wait(" in line:
+            verdict_unused = re.match(r"\s*sm100::mbar_wait\(.*_DRAIN\);$", line)
+            flag_only = re.match(r"\s*if \(!\*abort_v && !sm100::mbar_wait\(.*\)\) \*abort_v = 1;$", line) or \
+                re.match(r"\s*if \(sm100::mbar_try_wait\(bar, parity\)\) return;$", line)
+            assert verdict_unused or flag_only, line
+        if "elect_one()" in line or "for (" in line or "while (" in line:
+            assert "abort_v" not in line, line
