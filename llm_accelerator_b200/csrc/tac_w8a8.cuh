@@ -417,12 +417,12 @@ __global__ void __launch_bounds__(kSkThreads) w8_rows_kernel(const __grid_consta
     load8(pp, m, kb0 * 128 + (i - m * per) * 8, v);
     return m;
   };
-  auto largest = [&](int m, const float (&v)[8]) {
+  auto largest = [&](int i, int m, const float (&v)[8]) {
     uint32_t mb = 0;
 #pragma unroll
     for (int j = 0; j < 8; ++j) mb = max(mb, __float_as_uint(v[j]) & 0x7fffffffu);
-    // 16 lanes of one row first: a row has a multiple of 16 chunks
-    const uint32_t lanes = __activemask();
+    // 16 lanes of one row first: a row has a multiple of 16 chunks, so of a warp's 32 all or the lower half are items
+    const uint32_t lanes = (i | 31) < items ? 0xffffffffu : 0x0000ffffu;
 #pragma unroll
     for (int o = 1; o < 16; o <<= 1) mb = max(mb, __shfl_xor_sync(lanes, mb, o));
     if ((lane & 15) == 0) atomicMax(&row_max[m], mb);
@@ -441,11 +441,11 @@ __global__ void __launch_bounds__(kSkThreads) w8_rows_kernel(const __grid_consta
     for (int i = t; i < per * 8; i += 128) reinterpret_cast<uint4*>(rows_sm)[i] = make_uint4(0, 0, 0, 0);
 #pragma unroll
     for (int k = 0; k < kHeld; ++k)
-      if (t + k * 128 < items) largest((t + k * 128) / per, held[k]);
+      if (t + k * 128 < items) largest(t + k * 128, (t + k * 128) / per, held[k]);
     for (int i = t + kHeld * 128; i < items; i += 128) {
       float v[8];
       const int m = item(i, v);
-      largest(m, v);
+      largest(i, m, v);
     }
     asm volatile("bar.sync 1, 128;\n" ::: "memory");
     // this CTA's maxima to every CTA of the cluster

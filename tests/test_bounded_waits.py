@@ -27,3 +27,10 @@ def test_no_lane_leaves_a_loop_by_itself(name):
             assert verdict_unused or flag_only, line
         if "elect_one()" in line or "for (" in line or "while (" in line:
             assert "abort_v" not in line, line
+
+
+def test_no_mask_is_read_off_the_converged_lanes():
+    """__activemask says which lanes happen to be converged, not which take part: a collective that goes by it can lose
+    lanes."""
+    for p in sorted(CSRC.iterdir()):
+        assert "__activemask" not in p.read_text(), p.name

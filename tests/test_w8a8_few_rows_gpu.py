@@ -1,0 +1,39 @@
+"""linear_w8a8 of up to 16 rows (one launch, rows quantised inside) against the same layer in two calls.
+
+Both quantise by the same float32 formula, sum integers and share their epilogue, so results are equal bit for bit;
+tests/test_w8a8_gpu.py holds the two calls against the definition in 64 bits."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+from llm_accelerator_b200 import _lib as L
+
+pytestmark = pytest.mark.gpu
+
+
+def _two_calls(x, Bt, sb, bias=None):
+    from llm_accelerator_b200 import gemm, ptq
+    q, s = ptq.quantize_rows(x)
+    return gemm.gemm_i8_scaled(q, Bt, s, sb, bias=bias, out_dtype=x.dtype)
+
+
+def _weights(N, K, seed=0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    Bt = torch.randint(-127, 128, (N, -(-K // 16) * 16), generator=g, dtype=torch.int8, device="cuda")
+    return Bt, torch.rand(N, generator=g, device="cuda") * 1e-3 + 1e-4
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("M,K", [(1, 100), (3, 100), (3, 250), (16, 17), (15, 255), (16, 128)])
+def test_the_largest_value_at_every_column(M, K, dtype):
+    """The row's maximum in each lane's chunk in turn: rows whose last chunks are ragged, warps with half their lanes."""
+    from llm_accelerator_b200 import gemm
+    Bt, sb = _weights(130, K)
+    base = torch.randn((M, K + 1), device="cuda").to(dtype)
+    for off in (0, 1):                                # rows with and without whole 16-byte chunks
+        for c in range(K):
+            x = base.clone()[:, off:off + K]
+            x[torch.arange(M), (c + 37 * torch.arange(M)) % K] = -50.0
+            assert torch.equal(gemm.linear_w8a8(x, Bt, sb), _two_calls(x, Bt, sb))
+    assert L.lib.tac_gemm_status(None) == L.OK
