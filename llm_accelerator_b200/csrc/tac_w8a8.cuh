@@ -407,6 +407,9 @@ __global__ void __launch_bounds__(kSkThreads) w8_rows_kernel(const __grid_consta
   sm100::tc_fence_after();
   const uint32_t tmem = tmem_base;
   volatile int* abort_v = &abort_flag;
+  // The maxima go into the other CTAs' shared memory, which may be written once every CTA of the cluster runs: it says so
+  // here, and the wait below lies behind the rows' loads.
+  if (nsplit > 1) sm100::cluster_arrive();
 
   const int early = min(S, kb1 - kb0);
   const int t = threadIdx.x - 64, per = (kb1 - kb0) * 16, items = p.M * per;   // 8-value chunks of this CTA's columns
@@ -448,14 +451,20 @@ __global__ void __launch_bounds__(kSkThreads) w8_rows_kernel(const __grid_consta
       largest(i, m, v);
     }
     asm volatile("bar.sync 1, 128;\n" ::: "memory");
+    __syncwarp();
+    if (nsplit > 1) sm100::cluster_wait();
     // this CTA's maxima to every CTA of the cluster
     for (int i = t; i < kTn * nsplit; i += 128)
       asm volatile("st.shared::cluster.u32 [%0], %1;\n" ::"r"(sm100::mapa_shared(&all_max[rank][i % kTn], i / kTn)), "r"(row_max[i % kTn])
                    : "memory");
   }
   __syncwarp();
-  if (nsplit > 1) sm100::cluster_sync();
-  else __syncthreads();
+  if (nsplit > 1) {
+    if (warp < 2) sm100::cluster_wait();         // of the first arrival, which the other warps have waited for
+    sm100::cluster_sync();
+  } else {
+    __syncthreads();
+  }
 
   if (warp == 0) {
     uint32_t s = 0, ph = 1, issued = 0;

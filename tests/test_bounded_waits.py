@@ -34,3 +34,14 @@ def test_no_mask_is_read_off_the_converged_lanes():
     lanes."""
     for p in sorted(CSRC.iterdir()):
         assert "__activemask" not in p.read_text(), p.name
+
+
+def test_other_ctas_are_written_to_only_once_they_run():
+    """A store into another CTA's shared memory lies behind a cluster barrier of the same kernel: before one, that CTA may
+    not have started."""
+    kernels = re.split(r"__global__", (CSRC / "tac_w8a8.cuh").read_text())[1:]
+    writers = [k for k in kernels if "st.shared::cluster" in k]
+    assert writers
+    for k in writers:
+        before = k[:k.index("st.shared::cluster")]
+        assert before.count("cluster_arrive()") == 1 and before.count("cluster_wait()") == 1 or "cluster_sync()" in before

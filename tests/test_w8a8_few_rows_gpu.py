@@ -37,3 +37,32 @@ def test_the_largest_value_at_every_column(M, K, dtype):
             x[torch.arange(M), (c + 37 * torch.arange(M)) % K] = -50.0
             assert torch.equal(gemm.linear_w8a8(x, Bt, sb), _two_calls(x, Bt, sb))
     assert L.lib.tac_gemm_status(None) == L.OK
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("M,N,K", [(1, 130, 600), (1, 4096, 1024), (3, 300, 2000), (5, 129, 1025), (16, 1000, 4096),
+                                   (16, 4700, 1500), (7, 256, 8192), (2, 9472, 1024)])
+def test_rows_shared_by_a_cluster(M, N, K, dtype):
+    """K split over 2, 4 and 8 CTAs, the largest value in each CTA's share in turn, call after call, beside a kernel that
+    keeps other SMs busy (CTAs of a cluster then start at different times)."""
+    from llm_accelerator_b200 import gemm
+    Bt, sb = _weights(N, K, N + K)
+    bias = torch.randn(N, device="cuda").to(dtype)
+    x = torch.randn((M, K), device="cuda").to(dtype)
+    side, load = torch.cuda.Stream(), torch.randn((2048, 2048), device="cuda")
+    rows = torch.arange(M)
+    want, got = [], []
+    for i in range(24):
+        y = x.clone()
+        y[rows, (i * K // 24 + 131 * rows) % K] = 40.0 + i
+        want.append((y, _two_calls(y, Bt, sb, bias)))
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        for _ in range(8):
+            load = (load @ load).clamp_(-1, 1)
+    for y, _ in want:
+        got.append(gemm.linear_w8a8(y, Bt, sb, bias=bias))
+    torch.cuda.synchronize()
+    for g, (_, w) in zip(got, want):
+        assert torch.equal(g, w)
+    assert L.lib.tac_gemm_status(None) == L.OK
