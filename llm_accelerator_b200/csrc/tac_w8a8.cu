@@ -350,6 +350,8 @@ int run_product(const int8_t* A, const int8_t* Bt, const float* a_scale, const v
   return y_type == TAC_F32 ? pick_product<0>(A, Bt, p, st) : y_type == TAC_F16 ? pick_product<1>(A, Bt, p, st) : pick_product<2>(A, Bt, p, st);
 }
 
+static_assert(kRowsMostK / 128 * kRowsMost * 128 + 2 * kSkWBytes + 1024 <= kSkMaxSmem, "whole rows and a ring fit");
+
 // Few rows: one launch, no workspace.
 bool few_rows(int M, int K) { return M <= kRowsMost && K <= kRowsMostK; }
 
@@ -370,13 +372,15 @@ int launch_rows(W8RowsParams pp, const int8_t* Bt, cudaStream_t st) {
   const int64_t tiles = (p.N + 127) / 128;
   const int split = splits(tiles, p.k_blocks, p.tn, sms);
   const int per = (p.k_blocks + split - 1) / split;
-  p.stages = std::min(per, tiles * split > sms ? 4 : 8);
+  // weights in flight: four stages where two CTAs share an SM, else eight, of what the rows' codes leave (five of 64 blocks)
+  const int rows_bytes = per * kRowsMost * 128;
+  p.stages = std::min({per, tiles * split > sms ? 4 : 8, (kSkMaxSmem - 1024 - rows_bytes) / kSkWBytes});
   CUtensorMap tw;
   if (!map_rows(&tw, Bt, p.K, p.N, 128)) return TAC_E_CUDA;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(uint32_t(tiles), 1, split);
   cfg.blockDim = dim3(kSkThreads);
-  cfg.dynamicSmemBytes = p.stages * kSkWBytes + per * kRowsMost * 128 + 1024;   // the partial sums (10 KB) fit the first stage
+  cfg.dynamicSmemBytes = p.stages * kSkWBytes + rows_bytes + 1024;   // the partial sums (10 KB) fit the first stage
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;

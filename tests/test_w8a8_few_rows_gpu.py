@@ -66,3 +66,16 @@ def test_rows_shared_by_a_cluster(M, N, K, dtype):
     for g, (_, w) in zip(got, want):
         assert torch.equal(g, w)
     assert L.lib.tac_gemm_status(None) == L.OK
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("N", [9472, 9473, 10240, 18944, 18945])
+@pytest.mark.parametrize("K", [6016, 6017, 6032, 7168, 8192])
+def test_long_rows_over_every_number_of_channel_tiles(N, K, dtype):
+    """74 to 149 channel tiles: CTAs that hold rows of up to 64 K blocks beside their ring of weights."""
+    from llm_accelerator_b200 import gemm
+    Bt, sb = _weights(N, K)
+    for M in (1, 16):
+        x = torch.randn((M, K), device="cuda").to(dtype)
+        assert torch.equal(gemm.linear_w8a8(x, Bt, sb), _two_calls(x, Bt, sb))
+    assert L.lib.tac_gemm_status(None) == L.OK
