@@ -9,6 +9,7 @@
 #include "tac_kv4.cuh"
 #include "tac_kv4_rows.cuh"
 #include "tac_kv4_tc.cuh"
+#include "tac_launch.cuh"
 
 namespace tac {
 int* gemm_fault_word();
@@ -19,7 +20,6 @@ namespace {
 using namespace tac;
 
 bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
-int status() { return cudaGetLastError() == cudaSuccess ? TAC_OK : TAC_E_CUDA; }
 
 int sm_count() {
   static int sms[64] = {};
@@ -299,12 +299,12 @@ void set_run(RowArgs& a, int* grid) {
 }
 
 template <int D>
-void launch_append(const RowArgs& a, int grid, cudaStream_t st) {
+int launch_append(const RowArgs& a, int grid, cudaStream_t st) {
   // no more threads than a token's rows keep busy
   const int threads = std::min(kRowThreads, (2 * a.c.heads * (D / 16) + 31) / 32 * 32);
-  if (a.vec && a.type == TAC_F16) kv4_append_kernel<D, TAC_F16><<<grid, threads, 0, st>>>(a);
-  else if (a.vec && a.type == TAC_BF16) kv4_append_kernel<D, TAC_BF16><<<grid, threads, 0, st>>>(a);
-  else kv4_append_kernel<D, -1><<<grid, threads, 0, st>>>(a);
+  if (a.vec && a.type == TAC_F16) return launch(kv4_append_kernel<D, TAC_F16>, grid, threads, 0, st, a);
+  if (a.vec && a.type == TAC_BF16) return launch(kv4_append_kernel<D, TAC_BF16>, grid, threads, 0, st, a);
+  return launch(kv4_append_kernel<D, -1>, grid, threads, 0, st, a);
 }
 
 // ---- attention ------------------------------------------------------------------------------------------------------
@@ -338,13 +338,10 @@ int launch_rows(Kv4RowsParams p, void* workspace, cudaStream_t st) {
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return TAC_E_CUDA;
   if (!smem_set[dev]) {
-    if (cudaFuncSetAttribute(kv4_rows_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, rows_smem(D, NT)) !=
-        cudaSuccess)
-      return TAC_E_CUDA;
+    if (int e = status(cudaFuncSetAttribute(kv4_rows_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, rows_smem(D, NT)))) return e;
     smem_set[dev] = true;
   }
-  kv4_rows_kernel<D, NT><<<grid, kRowsThreads, rows_smem(D, NT), st>>>(p);
-  if (int s = status()) return s;
+  if (int s = launch(kv4_rows_kernel<D, NT>, grid, kRowsThreads, rows_smem(D, NT), st, p)) return s;
   if (!p.split) return TAC_OK;
   // launched while the first kernel still runs; it waits for that kernel's end before it reads
   cudaLaunchConfig_t cfg = {};
@@ -356,7 +353,7 @@ int launch_rows(Kv4RowsParams p, void* workspace, cudaStream_t st) {
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kv4_join_kernel<D, NT>, p) == cudaSuccess ? TAC_OK : TAC_E_CUDA;
+  return status(cudaLaunchKernelEx(&cfg, kv4_join_kernel<D, NT>, p));
 }
 
 // The prompt kernel (256 rows a CTA, one CTA an SM) where it is faster than the row kernel, whose time goes with all
@@ -375,8 +372,7 @@ int launch_tc(const Kv4RowsParams& r, cudaStream_t st) {
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return TAC_E_CUDA;
   if (!smem_set[dev]) {
-    if (cudaFuncSetAttribute(kv4_tc_kernel<D, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, tc_smem(D)) != cudaSuccess)
-      return TAC_E_CUDA;
+    if (int e = status(cudaFuncSetAttribute(kv4_tc_kernel<D, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, tc_smem(D)))) return e;
     smem_set[dev] = true;
   }
   Kv4TcParams p{};
@@ -385,8 +381,7 @@ int launch_tc(const Kv4RowsParams& r, cudaStream_t st) {
   if (!p.fault) return TAC_E_CUDA;
   p.blocks = int((int64_t(r.s.total) * r.group + kTcRows - 1) / kTcRows) + r.s.batch;
   if (int64_t(p.blocks) * r.c.heads > (int64_t(1) << 31) - 1) return TAC_E_ARGUMENT;
-  kv4_tc_kernel<D, BF16><<<p.blocks * r.c.heads, kTcThreads, tc_smem(D), st>>>(p);
-  return status();
+  return launch(kv4_tc_kernel<D, BF16>, p.blocks * r.c.heads, kTcThreads, tc_smem(D), st, p);
 }
 
 }  // namespace
@@ -409,9 +404,7 @@ extern "C" int tac_kv4_append(const tac_kv4_cache* cache, const int32_t* page_ta
   set_run(a, &grid);
   if (grid <= 0) return TAC_E_CUDA;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (cache->head_dim == 64) launch_append<64>(a, grid, st);
-  else launch_append<128>(a, grid, st);
-  return status();
+  return cache->head_dim == 64 ? launch_append<64>(a, grid, st) : launch_append<128>(a, grid, st);
 }
 
 extern "C" int tac_kv4_read(const tac_kv4_cache* cache, const int32_t* page_table, const int32_t* lens,
@@ -425,9 +418,7 @@ extern "C" int tac_kv4_read(const tac_kv4_cache* cache, const int32_t* page_tabl
   set_run(a, &grid);
   if (grid <= 0) return TAC_E_CUDA;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (cache->head_dim == 64) kv4_read_kernel<64><<<grid, kRowThreads, 0, st>>>(a);
-  else kv4_read_kernel<128><<<grid, kRowThreads, 0, st>>>(a);
-  return status();
+  return launch(cache->head_dim == 64 ? kv4_read_kernel<64> : kv4_read_kernel<128>, grid, kRowThreads, 0, st, a);
 }
 
 extern "C" uint64_t tac_kv4_attention_workspace_bytes(int batch, int width, int page_size, int total, int q_heads,

@@ -8,6 +8,7 @@
 #include <type_traits>
 
 #include "../../include/taccel_b200.h"
+#include "tac_launch.cuh"
 #include "tac_tmap.h"
 #include "tac_w8a8.cuh"
 
@@ -21,7 +22,6 @@ using namespace tac;
 
 bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 bool type_ok(int t) { return t == TAC_F32 || t == TAC_F16 || t == TAC_BF16; }
-int status() { return cudaGetLastError() == cudaSuccess ? TAC_OK : TAC_E_CUDA; }
 
 int sm_count() {
   static int sms[64] = {};
@@ -167,25 +167,18 @@ __global__ void __launch_bounds__(kQrThreads) quant_rows_vec_kernel(const T* __r
 }
 
 template <typename T>
-void quant_rows_16(const T* X, int64_t ldx, int8_t* Q, int ldq, float* scale, int M, int K, cudaStream_t st) {
+int quant_rows_16(const T* X, int64_t ldx, int8_t* Q, int ldq, float* scale, int M, int K, cudaStream_t st) {
   const bool vec = K % 8 == 0 && K <= 8192 && aligned(X, 16) && (M == 1 || ldx % 8 == 0);
-  if (vec && K <= 2048)
-    quant_rows_vec_kernel<T, 1><<<(M + 3) / 4, kQrThreads, 0, st>>>(X, ldx, Q, ldq, scale, M, K);
-  else if (vec)
-    quant_rows_vec_kernel<T, 4><<<M, kQrThreads, 0, st>>>(X, ldx, Q, ldq, scale, M, K);
-  else
-    quant_rows_kernel<<<M, kQrThreads, 0, st>>>(X, ldx, Q, ldq, scale, K);
+  if (vec && K <= 2048) return launch(quant_rows_vec_kernel<T, 1>, (M + 3) / 4, kQrThreads, 0, st, X, ldx, Q, ldq, scale, M, K);
+  if (vec) return launch(quant_rows_vec_kernel<T, 4>, M, kQrThreads, 0, st, X, ldx, Q, ldq, scale, M, K);
+  return launch(quant_rows_kernel<T>, M, kQrThreads, 0, st, X, ldx, Q, ldq, scale, K);
 }
 
 int launch_quant_rows(const void* X, int type, int64_t ldx, int8_t* Q, float* scale, int M, int K, cudaStream_t st) {
   const int ldq = (K + 15) / 16 * 16;
-  if (type == TAC_F32)
-    quant_rows_kernel<<<M, kQrThreads, 0, st>>>(static_cast<const float*>(X), ldx, Q, ldq, scale, K);
-  else if (type == TAC_F16)
-    quant_rows_16(static_cast<const __half*>(X), ldx, Q, ldq, scale, M, K, st);
-  else
-    quant_rows_16(static_cast<const __nv_bfloat16*>(X), ldx, Q, ldq, scale, M, K, st);
-  return status();
+  if (type == TAC_F32) return launch(quant_rows_kernel<float>, M, kQrThreads, 0, st, static_cast<const float*>(X), ldx, Q, ldq, scale, K);
+  if (type == TAC_F16) return quant_rows_16(static_cast<const __half*>(X), ldx, Q, ldq, scale, M, K, st);
+  return quant_rows_16(static_cast<const __nv_bfloat16*>(X), ldx, Q, ldq, scale, M, K, st);
 }
 
 // ---- scaled product -------------------------------------------------------------------------------------------------
@@ -213,8 +206,7 @@ int launch_splitk(const int8_t* A, const int8_t* Bt, W8Params p, cudaStream_t st
   const int sms = sm_count();
   if (!sms || cudaGetDevice(&dev) != cudaSuccess) return TAC_E_CUDA;
   if (!smem_set[dev]) {
-    if (cudaFuncSetAttribute(w8_splitk_kernel<YT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSkMaxSmem) != cudaSuccess)
-      return TAC_E_CUDA;
+    if (int e = status(cudaFuncSetAttribute(w8_splitk_kernel<YT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSkMaxSmem))) return e;
     smem_set[dev] = true;
   }
   p.k_blocks = (p.K + 127) / 128;
@@ -244,7 +236,7 @@ int launch_splitk(const int8_t* A, const int8_t* Bt, W8Params p, cudaStream_t st
     attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
   }
-  return cudaLaunchKernelEx(&cfg, w8_splitk_kernel<YT>, tw, ta, p) == cudaSuccess ? TAC_OK : TAC_E_CUDA;
+  return status(cudaLaunchKernelEx(&cfg, w8_splitk_kernel<YT>, tw, ta, p));
 }
 
 // Tokens of a pair tile: the multiple of 32 that leaves the least work on the
@@ -306,7 +298,7 @@ int launch_pair(const int8_t* A, const int8_t* Bt, W8Params p, int clusters, int
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = p.after_rows ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, w8_pair_kernel<YT>, tw, ta, pp) == cudaSuccess ? TAC_OK : TAC_E_CUDA;
+  return status(cudaLaunchKernelEx(&cfg, w8_pair_kernel<YT>, tw, ta, pp));
 }
 
 // Checks that both products share; also the limits of 32-bit sums and of the grid.
@@ -362,8 +354,7 @@ int launch_rows(W8RowsParams pp, const int8_t* Bt, cudaStream_t st) {
   const int sms = sm_count();
   if (!sms || cudaGetDevice(&dev) != cudaSuccess) return TAC_E_CUDA;
   if (!smem_set[dev]) {
-    if (cudaFuncSetAttribute(w8_rows_kernel<YT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSkMaxSmem) != cudaSuccess)
-      return TAC_E_CUDA;
+    if (int e = status(cudaFuncSetAttribute(w8_rows_kernel<YT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSkMaxSmem))) return e;
     smem_set[dev] = true;
   }
   W8Params& p = pp.g;
@@ -389,7 +380,7 @@ int launch_rows(W8RowsParams pp, const int8_t* Bt, cudaStream_t st) {
   attr[0].val.clusterDim.z = split;
   cfg.attrs = attr;
   cfg.numAttrs = split > 1;
-  return cudaLaunchKernelEx(&cfg, w8_rows_kernel<YT>, tw, pp) == cudaSuccess ? TAC_OK : TAC_E_CUDA;
+  return status(cudaLaunchKernelEx(&cfg, w8_rows_kernel<YT>, tw, pp));
 }
 
 uint64_t align256(uint64_t v) { return (v + 255) & ~uint64_t(255); }
