@@ -549,7 +549,8 @@ __global__ void __launch_bounds__(kRowsThreads, rows_ctas(D, NT)) kv4_rows_kerne
             vx = max(ve[n][i], min(vx, 253u));
             corr[i] *= __uint_as_float((127u - min(vx - ve[n][i], 126u)) << 23);   // 2^(ve - vx)
             ve[n][i] = vx;
-            vlim = min(vlim, (vx + kSlackV) << 23);
+            // a row that has seen no key has no mu yet: the next tile comes here whatever its values' scales are
+            vlim = min(vlim, begun >> (2 * n + i) & 1 ? (vx + kSlackV) << 23 : 0u);
           }
           zo[n][0] *= corr[0];
           zo[n][1] *= corr[1];

@@ -1,0 +1,43 @@
+"""Attention over the 4-bit cache where a softmax state begins late or sits at the ends of the types, on the GPU against
+the definition in 64 bits (tests/kv4_helpers.py derives the tolerances)."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+from kv4_helpers import Batch, check, check_lse, queries, reference
+
+pytestmark = pytest.mark.gpu
+
+
+def _i32(x):
+    return torch.tensor(x, dtype=torch.int32, device="cuda")
+
+
+def _reload(b):
+    """The cache after changes to b.host and b.table."""
+    for t, h in zip((b.cache.k_codes, b.cache.k_params, b.cache.v_codes, b.cache.v_params), b.host):
+        t.copy_(h)
+    b.d_table = b.table.cuda()
+
+
+@pytest.mark.parametrize("scores", [-173.0, -20.0, 100.0])
+@pytest.mark.parametrize("zeros", [256, 512])
+@pytest.mark.parametrize("D,group,new", [(64, 1, 1), (64, 1, 12), (128, 4, 1), (128, 4, 5), (64, 16, 600), (64, 16, 1000)])
+def test_a_context_that_begins_with_missing_pages_and_zero_values(D, group, new, zeros, scores):
+    """The first 256 positions have no page, the next `zeros` hold values of zero, and all scores are alike (in powers of
+    two, far below 2^-126 in the first case): the keys of the zeros weigh as much as the others."""
+    from llm_accelerator_b200 import kv4
+    b = Batch([1024], 1, D, 16)
+    b.table[0, :16] = -1
+    b.host[0][:] = 0xFF                                   # keys: 15 in every channel
+    b.host[1][:] = 0x3F800000
+    for j in range(16, 16 + zeros // 16):
+        b.host[2][int(b.table[0, j])] = 0
+        b.host[3][int(b.table[0, j])] = 0
+    _reload(b)
+    q = torch.full((new, group, D), scores * 0.6931471805599453 / (15 * D ** 0.5), dtype=torch.float16, device="cuda")
+    out, lse = kv4.attention(q, b.cache, b.d_table, b.d_lens, _i32([0, new]), return_lse=True, causal=new < 20)
+    want, wlse, tol = reference(b, q, [0, new], causal=new < 20)
+    check(out, want, tol)
+    check_lse(lse, wlse)
