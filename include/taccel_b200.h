@@ -424,7 +424,8 @@ int tac_kv4_read(const tac_kv4_cache* cache, const int32_t* page_table, const in
  * [total][q_heads][head_dim] contiguous, of the same type; lse (or null)
  * float32 [total][q_heads] gets log sum_j exp(scale * Q . k_j).  A row that
  * sees no token gets zeros and an lse of -inf; rows of no sequence are left as
- * they are.  The workspace (256-byte aligned, at least the bytes of the query
+ * they are.  Weights times the values' scales are rounded to FP16; with scales
+ * above 2^107 (values of 10^33) they can overflow in calls of many rows.  The workspace (256-byte aligned, at least the bytes of the query
  * below; null where that gives 0) must not be shared by calls that overlap. */
 uint64_t tac_kv4_attention_workspace_bytes(int batch, int width, int page_size, int total, int q_heads, int kv_heads,
                                            int head_dim);

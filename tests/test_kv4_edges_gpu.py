@@ -41,3 +41,26 @@ def test_a_context_that_begins_with_missing_pages_and_zero_values(D, group, new,
     want, wlse, tol = reference(b, q, [0, new], causal=new < 20)
     check(out, want, tol)
     check_lse(lse, wlse)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("loud", [None, 3, 700, 1290])
+@pytest.mark.parametrize("D,group,new,vmul", [(64, 1, 1, 2.0 ** 103), (64, 4, 9, 2.0 ** 103), (64, 16, 1100, 2.0 ** 103),
+                                              (128, 16, 1300, 2.0 ** 103), (128, 16, 700, 2.0 ** 91)])
+def test_the_largest_values(D, group, new, vmul, loud, dtype):
+    """Scales of up to 2^105 (what is promised ends at 2^107), one token louder than the others by 2^3 or 2^12; both
+    kernels, and a row's unit that starts low and ends high.  FP16 results beyond its range are infinities."""
+    from llm_accelerator_b200 import kv4
+    b = Batch([1300], 1, D, 32, vscale=vmul)
+    if loud is not None:
+        b.host[3][int(b.table[0, loud // 32]), 0, loud % 32] += (12 if vmul < 2.0 ** 100 else 3) << 23
+        _reload(b)
+    q = queries(new, group, D, dtype)
+    out, lse = kv4.attention(q, b.cache, b.d_table, b.d_lens, _i32([0, new]), return_lse=True)
+    want, wlse, tol = reference(b, q, [0, new])
+    if dtype == torch.float16:
+        sure = want.abs() > tol + 65536
+        assert (out.cpu()[sure].double() == torch.copysign(torch.tensor(float("inf")).double(), want[sure])).all()
+    else:
+        check(out, want, tol)
+    check_lse(lse, wlse)
