@@ -53,12 +53,15 @@ class Kv4Cache:
 
     @classmethod
     def from_tensors(cls, k_codes, k_params, v_codes, v_params) -> "Kv4Cache":
-        """A cache over tensors that the caller holds (a layer's slice of a larger allocation, a loaded prefix)."""
+        """A cache over tensors that the caller holds (a layer's slice of a larger allocation, a loaded prefix), each of
+        which begins on a 16-byte boundary."""
         self = cls.__new__(cls)
         self._set(k_codes, k_params, v_codes, v_params)
         return self
 
     def _set(self, k_codes, k_params, v_codes, v_params):
+        if any(t.data_ptr() & 15 for t in (k_codes, k_params, v_codes, v_params)):
+            raise ValueError("the cache's tensors must begin on 16-byte boundaries")
         for c, p in ((k_codes, k_params), (v_codes, v_params)):
             if c.dtype != torch.uint8 or p.dtype != torch.int32:
                 raise TypeError("codes must be uint8 and parameter words int32")
