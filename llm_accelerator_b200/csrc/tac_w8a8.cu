@@ -334,7 +334,6 @@ int run_product(const int8_t* A, const int8_t* Bt, const float* a_scale, const v
   p.y = Y;
   p.b_type = b_type;
   p.bias_type = bias_type;
-  p.y_type = y_type;
   p.M = M;
   p.N = N;
   p.K = K;
@@ -420,7 +419,7 @@ extern "C" int tac_linear_w8a8(const void* X, int x_type, int64_t ldx, const int
     W8RowsParams pp{};
     pp.g.b_scale = b_scale, pp.g.b_type = b_scale_type;
     pp.g.bias = bias, pp.g.bias_type = bias_type;
-    pp.g.y = Y, pp.g.y_type = y_type;
+    pp.g.y = Y;
     pp.g.M = M, pp.g.N = N, pp.g.K = Kp;
     if (!(pp.g.fault = fault_word())) return TAC_E_CUDA;
     pp.x = X, pp.x_type = x_type, pp.ldx = ldx, pp.k_real = K;

@@ -47,7 +47,7 @@ struct W8Params {
   const void* b_scale;
   const void* bias;          // or null
   void* y;
-  int b_type, bias_type, y_type;
+  int b_type, bias_type;
   int M, N, K;
   int k_blocks;              // 128-byte blocks of K
   int tn;                    // tokens of a tile
