@@ -15,6 +15,8 @@ positions of a sequence; numbers outside [0, pages) stand for pages without toke
 int32 [batch]: tokens of each sequence, the new ones included.  indptr int32 [batch + 1]: new tokens of sequence b are
 rows indptr[b] .. indptr[b + 1) of k, v and q, the last of its positions; None: one new token a sequence, row b.  All
 are device tensors that are read when the call runs, so a captured call follows them.
+
+The calls are for inference: no gradient flows through them, also from tensors that require one.
 """
 from __future__ import annotations
 

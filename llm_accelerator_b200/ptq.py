@@ -60,7 +60,7 @@ def quantize_tensor(W, per_channel: bool = True):
 def quantize_rows(X):
     """(q int8 [M, K_pad], scale float32 [M]) of X [M, K] (float32, float16 or bfloat16, contiguous rows at any row
     stride): t = max(max |x|, 1e-8), scale = t / 127, q = rint(x * (127 / t)); K_pad = K rounded up to 16, padding
-    columns zero.  A row that holds an infinity or a NaN gets the scale NaN."""
+    columns zero.  A row that holds an infinity or a NaN gets the scale NaN.  No gradient flows through the call."""
     import torch
     from ._tensors import call, type_code
     xt = type_code(X.dtype, "X")

@@ -4,6 +4,8 @@
 ``linear_w8a8``       the same product of floating-point rows, each quantised to INT8 in the call
 ``linear_workspace``  workspace of linear_w8a8 calls
 ``pad_k16``           INT8 weights padded to whole groups of 16 columns
+
+The products are for inference: no gradient flows through them, also from rows, scales or a bias that require one.
 """
 from __future__ import annotations
 
