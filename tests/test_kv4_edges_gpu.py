@@ -64,3 +64,50 @@ def test_the_largest_values(D, group, new, vmul, loud, dtype):
     else:
         check(out, want, tol)
     check_lse(lse, wlse)
+
+
+def _sharp(b, q):
+    """(out, tol) float64 of one sequence's last rows, causal, with the tolerance of tests/kv4_helpers.py but for the unit
+    of the weights: FP16 weights below 2^-14 of it are off by 2^-25 of it, it is at most the largest scale among the keys
+    that the ROW sees, and the sum that they are divided by is at least z = sum exp(score - top)."""
+    q = q.cpu().double()
+    c, group, D = q.shape
+    n = b.lens[0]
+    K, ok = b.rows(0, 0, 0, n)
+    V, _ = b.rows(0, 1, 0, n)
+    scales = torch.stack([(b.host[3][int(b.table[0, j // b.page]), 0, j % b.page] & -65536).view(torch.float32).double()
+                          for j in range(n)])
+    seen = torch.arange(n)[None, :] <= (n - c + torch.arange(c))[:, None]
+    s = torch.einsum("cgd,nd->cgn", q, K) * D ** -0.5
+    ds = (torch.einsum("cgd,nd->cgn", q.abs(), K.abs()) * (2 * D + 4) * 2.0 ** -24
+          + q.abs().amax(-1, keepdim=True) * K.abs().sum(-1) * 2.0 ** -25) * D ** -0.5
+    s = s.masked_fill(~seen[:, None], float("-inf"))
+    p = torch.exp(s - s.amax(-1, keepdim=True))
+    z = p.sum(-1, keepdim=True)
+    p = p / z
+    rel = 2.0 ** -11 + 2.0 ** -19 + 2 * ds.masked_fill(~seen[:, None], 0).amax(-1, keepdim=True) + n * 2.0 ** -24
+    big = torch.where(seen, scales[None, :], 0.0).amax(-1)[:, None, None]
+    out = p @ V
+    tol = rel * (p @ V.abs()) + seen.sum(-1)[:, None, None] * 2.0 ** -25 * 15 * big / z
+    return out, tol + 2.0 ** -8 * out.abs() * (1 + 2.0 ** -8) + 2.0 ** -134
+
+
+@pytest.mark.parametrize("n,group,new", [(700, 1, 1), (700, 1, 130), (700, 4, 9), (1500, 16, 700), (1500, 16, 1400)])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("back", [5, 90, 400])
+def test_a_loud_token_coarsens_only_the_rows_that_see_it(back, D, n, group, new):
+    """One token, `back` before the end, with values 2^20 times the others'.  Rows before it are held to the ordinary
+    tolerance, of which a row of zeros would be far outside."""
+    from llm_accelerator_b200 import kv4
+    b = Batch([n], 1, D, 16)
+    pos = n - back
+    b.host[3][int(b.table[0, pos // 16]), 0, pos % 16] += 20 << 23
+    _reload(b)
+    q = queries(new, group, D, torch.bfloat16)
+    got = kv4.attention(q, b.cache, b.d_table, b.d_lens, _i32([0, new])).cpu().double()
+    want, tol = _sharp(b, q)
+    over = (got - want).abs() / tol
+    assert over.max() <= 1, f"worst {over.max():.3f} of the tolerance"
+    quiet = torch.arange(n - new, n) < pos
+    if quiet.any():
+        assert (tol[quiet].mean() < 0.05 * want[quiet].abs().mean()) and want[quiet].abs().max() < 50
