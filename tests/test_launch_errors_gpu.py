@@ -4,6 +4,10 @@ The failure is the host's: a stream whose capture has been invalidated refuses e
 from __future__ import annotations
 
 import ctypes as C
+import subprocess
+import sys
+import textwrap
+from pathlib import Path
 
 import pytest
 import torch
@@ -11,6 +15,7 @@ import torch
 from llm_accelerator_b200 import _lib as L
 
 pytestmark = pytest.mark.gpu
+ROOT = Path(__file__).resolve().parent.parent
 
 
 class _Refusing:
@@ -73,11 +78,21 @@ def test_failed_launches_fail_alone():
 
 
 def test_calls_do_not_report_what_an_earlier_call_left():
-    """An entry point that leaves the runtime's last error behind does not fail the calls after it."""
-    calls, keep = _calls()
-    for name, call in calls.items():
-        engine = C.c_void_p()
-        assert L.lib.tac_engine_create(999, 1, 1 << 16, 0, C.byref(engine)) == L.E_CUDA     # there is no such device
-        assert call(None) == L.OK, name
-    torch.cuda.synchronize()
-    del keep
+    """An entry point that leaves the runtime's last error behind does not fail the calls after it.  In a process of its
+    own, which the error ends with."""
+    code = textwrap.dedent(f"""
+        import ctypes as C, sys
+        sys.path[:0] = [{str(ROOT)!r}, {str(ROOT / 'tests')!r}]
+        import torch
+        from llm_accelerator_b200 import _lib as L
+        from test_launch_errors_gpu import _calls
+        calls, keep = _calls()
+        for name, call in calls.items():
+            engine = C.c_void_p()
+            assert L.lib.tac_engine_create(999, 1, 1 << 16, 0, C.byref(engine)) == L.E_CUDA     # there is no such device
+            assert call(None) == L.OK, name
+        torch.cuda.synchronize()
+        print("ok")
+    """)
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and r.stdout.strip().endswith("ok"), r.stdout + r.stderr
