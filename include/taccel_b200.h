@@ -361,10 +361,15 @@ int tac_gemm_i8_scaled(const int8_t* A, const int8_t* Bt, const float* a_scale, 
 /* The same product of floating-point rows, quantised in the call as
  * tac_quantize_rows_i8 does: Y = linear(X[M,K]) with Bt [N, K_pad] int8, K_pad
  * = K rounded up to 16.  A multiplier in columns K .. K_pad of Bt meets a zero.
- * Up to 16 rows of up to 8192 columns take one launch and no workspace (the
- * query gives 0, workspace may be null).  Calls that share a workspace
- * (256-byte aligned, at least the queried bytes) must not overlap. */
+ * Up to 16 rows of up to 8192 columns can go in one launch and need no
+ * workspace (the query gives 0, workspace may be null).  That is the faster way
+ * for a few thousand values only: the second query gives, for the current
+ * device, the workspace with which a call of these sizes is fastest, 0 where
+ * none is used; a call that gets it takes two launches.  Results are the same
+ * either way.  Calls that share a workspace (256-byte aligned, at least the
+ * queried bytes) must not overlap. */
 uint64_t tac_linear_w8a8_workspace_bytes(int M, int K);
+uint64_t tac_linear_w8a8_best_workspace_bytes(int M, int N, int K);
 int tac_linear_w8a8(const void* X, int x_type, int64_t ldx, const int8_t* Bt, const void* b_scale,
                     int b_scale_type, const void* bias, int bias_type, void* Y, int y_type, void* workspace,
                     uint64_t workspace_bytes, int M, int N, int K, void* stream);

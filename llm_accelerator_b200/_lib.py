@@ -120,6 +120,7 @@ SIGNATURES = {
     "tac_quantize_rows_i8": (_I, [_P, _I, _I64, _P, _P, _I, _I, _P]),
     "tac_gemm_i8_scaled": (_I, [_P, _P, _P, _P, _I, _P, _I, _P, _I, _I, _I, _I, _P]),
     "tac_linear_w8a8_workspace_bytes": (_U64, [_I, _I]),
+    "tac_linear_w8a8_best_workspace_bytes": (_U64, [_I, _I, _I]),
     "tac_linear_w8a8": (_I, [_P, _I, _I64, _P, _P, _I, _P, _I, _P, _I, _P, _U64, _I, _I, _I, _P]),
     "tac_kv4_append": (_I, [_P, _P, _P, _P, _I, _I, _I, _P, _I64, _I64, _P, _I64, _I64, _I, _P]),
     "tac_kv4_read": (_I, [_P, _P, _P, _P, _I, _I, _I, _P, _P, _P]),

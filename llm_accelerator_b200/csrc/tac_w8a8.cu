@@ -343,8 +343,26 @@ int run_product(const int8_t* A, const int8_t* Bt, const float* a_scale, const v
 
 static_assert(kRowsMostK / 128 * kRowsMost * 128 + 2 * kSkWBytes + 1024 <= kSkMaxSmem, "whole rows and a ring fit");
 
-// Few rows: one launch, no workspace.
+// Few rows: one launch is possible, with no workspace.
 bool few_rows(int M, int K) { return M <= kRowsMost && K <= kRowsMostK; }
+
+// Where one launch is faster than the quantiser and the product, for a call that the host waits for: it spares the second
+// launch and the workspace (5.5 us a call, 3 us of latency), but its 128 threads quantise every row in each of the N / 128
+// CTAs before the first MMA, and whole rows of long K leave an SM one CTA.  On the device alone it is behind everywhere, by
+// 0.8 us where a CTA has few values and by 250 where it has 131,072.  Microseconds, one launch against two, on the device
+// and for a call alone:
+//    1 x 4096 x 1024    7.0 / 5.8   22.6 / 25.7      1 x 28672 x 1024    9.1 /  9.1   24.5 / 28.8
+//   16 x 4096 x 1024    9.7 / 6.4   25.2 / 26.4      8 x 28672 x 1024   14.8 /  9.1   30.1 / 28.4
+//    4 x 4096 x 4096   12.0 / 8.8   27.6 / 28.6      1 x 28672 x 4096   34.0 / 22.0
+//    8 x 4096 x 4096   15.1 / 8.8   31.2 / 28.9      1 x 10240 x 8192   27.0 / 19.4
+//    1 x 4096 x 8192   13.7 / 11.0  29.0 / 31.0     16 x 28672 x 8192  292.3 / 41.7
+// (N x K behind the rows.)
+bool one_launch(int M, int N, int K, int sms) {
+  if (!few_rows(M, K)) return false;
+  const int64_t tiles = (int64_t(N) + 127) / 128;
+  const int k_blocks = (K + 127) / 128, split = splits(tiles, k_blocks, kRowsMost, sms);
+  return M * 128 * ((k_blocks + split - 1) / split) <= (tiles > sms ? 2048 : 4096);
+}
 
 template <int YT>
 int launch_rows(W8RowsParams pp, const int8_t* Bt, cudaStream_t st) {
@@ -403,9 +421,17 @@ extern "C" int tac_gemm_i8_scaled(const int8_t* A, const int8_t* Bt, const float
                      static_cast<cudaStream_t>(stream));
 }
 
+namespace {
+// Codes and scales of M rows.
+uint64_t rows_bytes(int M, int K) { return align256(uint64_t(M) * ((uint64_t(K) + 15) / 16 * 16)) + align256(uint64_t(M) * 4); }
+}  // namespace
+
 extern "C" uint64_t tac_linear_w8a8_workspace_bytes(int M, int K) {
-  if (M <= 0 || K <= 0 || few_rows(M, K)) return 0;
-  return align256(uint64_t(M) * ((uint64_t(K) + 15) / 16 * 16)) + align256(uint64_t(M) * 4);
+  return M <= 0 || K <= 0 || few_rows(M, K) ? 0 : rows_bytes(M, K);
+}
+
+extern "C" uint64_t tac_linear_w8a8_best_workspace_bytes(int M, int N, int K) {
+  return M <= 0 || N <= 0 || K <= 0 || one_launch(M, N, K, sm_count()) ? 0 : rows_bytes(M, K);
 }
 
 extern "C" int tac_linear_w8a8(const void* X, int x_type, int64_t ldx, const int8_t* Bt, const void* b_scale,
@@ -415,7 +441,8 @@ extern "C" int tac_linear_w8a8(const void* X, int x_type, int64_t ldx, const int
   if (int s = check_product(Bt, b_scale, b_scale_type, bias, bias_type, Y, y_type, M, N, K)) return s;
   const int Kp = (K + 15) / 16 * 16;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (few_rows(M, K)) {
+  const bool room = workspace && aligned(workspace, 256) && workspace_bytes >= rows_bytes(M, K);
+  if (few_rows(M, K) && !(room && !one_launch(M, N, K, sm_count()))) {
     W8RowsParams pp{};
     pp.g.b_scale = b_scale, pp.g.b_type = b_scale_type;
     pp.g.bias = bias, pp.g.bias_type = bias_type;
@@ -426,7 +453,7 @@ extern "C" int tac_linear_w8a8(const void* X, int x_type, int64_t ldx, const int
     pp.x_vec = x_type != TAC_F32 && aligned(X, 16) && (M == 1 || ldx % 8 == 0);
     return y_type == TAC_F32 ? launch_rows<0>(pp, Bt, st) : y_type == TAC_F16 ? launch_rows<1>(pp, Bt, st) : launch_rows<2>(pp, Bt, st);
   }
-  if (!workspace || !aligned(workspace, 256) || workspace_bytes < tac_linear_w8a8_workspace_bytes(M, K)) return TAC_E_ARGUMENT;
+  if (!room) return TAC_E_ARGUMENT;
   int8_t* q = static_cast<int8_t*>(workspace);
   float* s = reinterpret_cast<float*>(q + align256(uint64_t(M) * Kp));
   if (int e = launch_quant_rows(X, x_type, ldx, q, s, M, K, st)) return e;

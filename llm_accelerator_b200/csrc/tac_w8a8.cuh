@@ -343,8 +343,10 @@ __global__ void __launch_bounds__(kSkThreads)
 // way, the epilogue's warps take the largest magnitude of each row over this
 // CTA's K blocks, the cluster's CTAs tell each other theirs, and the rows'
 // codes go straight into the swizzled operand, which stays in shared memory.
-// A launch of its own for the quantiser costs more than reading the few rows
-// once for each 128 channels (1 x 4096 x 1024: 6.7 us).
+// For a call that the host waits for, a launch of its own for the quantiser
+// costs more than reading the rows once for each 128 channels, as long as they
+// are few thousand values (one_launch has both sides; 1 x 4096 x 1024: 7.0 us
+// on the device with weights out of HBM, 6.6 with weights in L2).
 constexpr int kRowsMost = 16, kRowsMostK = 8192;
 
 struct W8RowsParams {

@@ -9,13 +9,16 @@ The products are for inference: no gradient flows through them, also from rows, 
 """
 from __future__ import annotations
 
+from functools import lru_cache
+
 import torch
 
 from . import _lib as L
 from ._tensors import TYPES, call, type_code
 
 _I8, _F32, _F16 = torch.int8, torch.float32, torch.float16
-_gemm, _linear, _ws_bytes = L.lib.tac_gemm_i8_scaled, L.lib.tac_linear_w8a8, L.lib.tac_linear_w8a8_workspace_bytes
+_gemm, _linear = L.lib.tac_gemm_i8_scaled, L.lib.tac_linear_w8a8
+_ws_bytes = lru_cache(maxsize=1024)(L.lib.tac_linear_w8a8_best_workspace_bytes)   # sizes alone decide
 
 
 def _check(rows, Bt, b_scale, bias, out, out_dtype, M, K):
@@ -105,8 +108,9 @@ def linear_w8a8(X, Bt, b_scale, bias=None, out=None, ws=None):
         if ws is not None:
             if ws.get_device() != X.get_device() or ws.dtype is not torch.uint8 or not ws.is_contiguous():
                 raise ValueError("ws must be a linear_workspace on X's device")
-        elif M > 16 or _ws_bytes(M, K):
-            ws = linear_workspace(M, K, X.device)
+        else:
+            need = _ws_bytes(M, N, K)
+            ws = torch.empty(need + 256, dtype=torch.uint8, device=X.device) if need else None
         if ws is not None:
             p = ws.data_ptr()
             wp = (p + 255) & ~255
@@ -118,4 +122,5 @@ def linear_w8a8(X, Bt, b_scale, bias=None, out=None, ws=None):
 
 def linear_workspace(M: int, K: int, device="cuda"):
     """A workspace for linear_w8a8 calls of at most M rows of K columns (calls that share one must not overlap)."""
-    return torch.empty(int(_ws_bytes(M, K)) + 256, dtype=torch.uint8, device=device)
+    codes, scales = M * ((K + 15) // 16 * 16), 4 * M
+    return torch.empty((codes + 255) // 256 * 256 + (scales + 255) // 256 * 256 + 256, dtype=torch.uint8, device=device)
