@@ -359,7 +359,8 @@ int launch_rows(Kv4RowsParams p, void* workspace, cudaStream_t st) {
 // The prompt kernel (256 rows a CTA, one CTA an SM) where it is faster than the row kernel, whose time goes with all
 // rows: measured per key, 3.6e-6 us a row and key-value head against 0.025 us a round of CTAs over the SMs at D = 128,
 // 2.3e-6 against 0.021 at D = 64 (64 rows for each of 64 heads: 63 us by rows, 136 by the prompt kernel; 512 rows for
-// each of 16: 113 and 103).  The rows of a sequence are taken at their mean.
+// each of 16: 113 and 103).  The rows of a sequence are taken at their mean, and only batches of like sequences have been
+// measured: one with a long chunk beside decode rows goes whole to one kernel, which is not the best for either part.
 bool use_tc(int batch, int total, int group, int kv_heads, int head_dim) {
   const double rows = double(total) * group / batch, units = double(batch) * kv_heads;
   const double rounds = std::max(1.0, units * std::ceil(rows / kTcRows) / 148);

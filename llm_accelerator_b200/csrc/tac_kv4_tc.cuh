@@ -24,7 +24,7 @@
 // the weights before these are rounded to FP16, once; the query is FP16, scaled
 // by a power of two for each row.  So nothing is rounded to BF16 but the result.
 // Bound by the chain S, softmax, P, O of a group's step and the issue of its
-// MMAs: 640 TFLOP/s at those chunks (337 us), tensor pipe 31 % and exponential
+// MMAs: 630 TFLOP/s at those chunks (342 us), tensor pipe 31 % and exponential
 // unit 33 % busy, an eighth of the time in the CTAs' prologues.  One S product
 // of 128 keys for two steps (366 us) and softmax steps pipelined within a
 // thread at 192 registers (387 us) were slower.
