@@ -347,6 +347,24 @@ enum tac_type { TAC_F32 = 0, TAC_F16 = 1, TAC_BF16 = 2 };
 int tac_quantize_rows_i8(const void* X, int x_type, int64_t ldx, int8_t* Q, float* scale, int M, int K,
                          void* stream);
 
+/* What such codes stand for: Y[M,K] (y_type, contiguous) = Q[m][k] * scale[m], Q
+ * [M, K_pad] 16-byte aligned. */
+int tac_dequantize_rows_i8(const int8_t* Q, const float* scale, void* Y, int y_type, int M, int K, void* stream);
+
+/* Root-mean-square norm of rows: Y[M,K] = h / sqrt(mean_k h^2 + eps) * W[k] with
+ * h = X, or X + R where R is not null; then H gets h.  X, R, H and Y are of
+ * `type` (row strides ldx, ldr, ldh in elements, Y contiguous), W [K] of w_type,
+ * each aligned to its elements.  Sums are float32, of the unrounded h.  H may be
+ * R or X itself and may not overlap them otherwise.  No counterpart in the
+ * reference, whose programs have LayerNorm (simulator.py:893-934). */
+int tac_rms_norm(const void* X, int type, int64_t ldx, const void* R, int64_t ldr, void* H, int64_t ldh,
+                 const void* W, int w_type, float eps, void* Y, int M, int K, void* stream);
+
+/* The same with the result quantised as tac_quantize_rows_i8 does, from float32:
+ * Q [M, K_pad] (16-byte aligned) and scale [M]. */
+int tac_rms_norm_i8(const void* X, int type, int64_t ldx, const void* R, int64_t ldr, void* H, int64_t ldh,
+                    const void* W, int w_type, float eps, int8_t* Q, float* scale, int M, int K, void* stream);
+
 /* Y[M,N] (y_type) = (A[M,K] @ Bt[N,K]^T) * a_scale[m] * b_scale[n] (+ bias[n]):
  * INT8 x INT8 with exact int32 sums, ((float(sum) * a_scale) * b_scale) + bias
  * in float32 and one rounding.  A, Bt row-major and 16-byte aligned, K a
@@ -438,6 +456,18 @@ int tac_kv4_attention(const tac_kv4_cache* cache, const int32_t* page_table, con
                       const int32_t* indptr, int batch, int width, int total, const void* Q, int64_t q_tok,
                       int64_t q_head, int q_heads, int type, float scale, int causal, void* O, float* lse,
                       void* workspace, uint64_t workspace_bytes, void* stream);
+
+/* ---- Probabilities of tokens -------------------------------------------------
+ * Of the softmax of each row of X[M,V] (`type`, row stride ldx elements):
+ * logprob[m] = log p(tokens[m]) (tokens int32, or int64 with tokens_64 != 0; NaN
+ * for one outside [0, V)), entropy[m] = -sum p log p, and with top > 0 (at most
+ * 32 and V) the likeliest tokens, equal logits by the lowest index first:
+ * top_ids[M][top] and their log-probabilities.  Logits of -inf have no part in
+ * the sums; a row of them alone, or with a NaN or +inf, gives NaN.  Arrays are
+ * aligned to their elements.  The reference answers with logits and the greedy
+ * token only (host_runner.py:75-95). */
+int tac_token_logprobs(const void* X, int type, int64_t ldx, const void* tokens, int tokens_64, int M, int V, int top,
+                       float* logprob, float* entropy, float* top_logprobs, int32_t* top_ids, void* stream);
 
 /* ---- Offline weight quantisation ------------------------------------------
  * Per-channel (per_channel = 1) or per-tensor symmetric INT8 quantisation of

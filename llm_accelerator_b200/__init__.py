@@ -12,6 +12,8 @@ classes keep the reference interfaces:
 * ``gemm``           - stand-alone INT8 GEMM kernels with requant epilogues, INT8 linear layers with a scale for
   each token and channel
 * ``kv4``            - 4-bit paged key / value cache and attention over it
+* ``norm``           - root-mean-square norm with the residual's addition, to rows or INT8 rows
+* ``logprobs``       - log-probabilities of given tokens, entropy and the likeliest tokens of rows of logits
 """
 from .bundle import ProgramBundle, RelocationSite, RuntimeConfigAttnSite, RuntimePatchSite  # noqa: F401
 from .errors import (ConfigError, DRAMAccessError, EngineError, IllegalBufferError,  # noqa: F401
@@ -27,6 +29,6 @@ def __getattr__(name):
     import importlib
     if name in _LAZY:
         return getattr(importlib.import_module(f".{_LAZY[name]}", __name__), name)
-    if name in ("gemm", "kv4"):
+    if name in ("gemm", "kv4", "logprobs", "norm"):
         return importlib.import_module(f".{name}", __name__)
     raise AttributeError(name)

@@ -127,6 +127,10 @@ SIGNATURES = {
     "tac_kv4_attention_workspace_bytes": (_U64, [_I, _I, _I, _I, _I, _I, _I]),
     "tac_kv4_attention": (_I, [_P, _P, _P, _P, _I, _I, _I, _P, _I64, _I64, _I, _I, C.c_float, _I, _P, _P, _P, _U64,
                                _P]),
+    "tac_rms_norm": (_I, [_P, _I, _I64, _P, _I64, _P, _I64, _P, _I, C.c_float, _P, _I, _I, _P]),
+    "tac_rms_norm_i8": (_I, [_P, _I, _I64, _P, _I64, _P, _I64, _P, _I, C.c_float, _P, _P, _I, _I, _P]),
+    "tac_dequantize_rows_i8": (_I, [_P, _P, _P, _I, _I, _I, _P]),
+    "tac_token_logprobs": (_I, [_P, _I, _I64, _P, _I, _I, _I, _I, _P, _P, _P, _P, _P]),
     "tac_quantize_weight_i8": (_I, [_P, _I, _I, _I, _P, _P, _P, _P]),
     "tac_bundle_open": (_I, [C.c_char_p, C.POINTER(BundleView), C.POINTER(_P)]),
     "tac_bundle_close": (_I, [_P]),

@@ -1,0 +1,356 @@
+// Root-mean-square norm of rows with the residual's addition, its form with
+// INT8 codes and a scale for each row, and what such codes stand for.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cstdint>
+
+#include "../../include/taccel_b200.h"
+#include "tac_launch.cuh"
+
+namespace {
+
+using namespace tac;
+
+bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+bool type_ok(int t) { return t == TAC_F32 || t == TAC_F16 || t == TAC_BF16; }
+int elem(int type) { return type == TAC_F32 ? 4 : 2; }
+
+__device__ __forceinline__ float to_f(float v) { return v; }
+__device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ void from_f(float& d, float v) { d = v; }
+__device__ __forceinline__ void from_f(__half& d, float v) { d = __float2half_rn(v); }
+__device__ __forceinline__ void from_f(__nv_bfloat16& d, float v) { d = __float2bfloat16_rn(v); }
+
+// N consecutive values in 16-byte accesses (4-byte and 2-byte ones for a single value).
+template <typename T, int N>
+__device__ __forceinline__ void load_n(const T* p, float (&v)[N]) {
+  if constexpr (N == 1) {
+    v[0] = to_f(*p);
+  } else {
+    constexpr int kPer = 16 / sizeof(T);
+#pragma unroll
+    for (int i = 0; i < N; i += kPer) {
+      union {
+        uint4 u;
+        T t[kPer];
+      } a;
+      a.u = *reinterpret_cast<const uint4*>(p + i);
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) v[i + j] = to_f(a.t[j]);
+    }
+  }
+}
+template <typename T, int N>
+__device__ __forceinline__ void store_n(T* p, const float (&v)[N]) {
+  if constexpr (N == 1) {
+    from_f(*p, v[0]);
+  } else {
+    constexpr int kPer = 16 / sizeof(T);
+#pragma unroll
+    for (int i = 0; i < N; i += kPer) {
+      union {
+        uint4 u;
+        T t[kPer];
+      } a;
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) from_f(a.t[j], v[i + j]);
+      *reinterpret_cast<uint4*>(p + i) = a.u;
+    }
+  }
+}
+
+struct NormParams {
+  const void* x;
+  const void* r;             // or null
+  void* h;                   // where there is an r
+  const void* w;
+  void* y;                   // rows of the input's type, or codes
+  float* scale;              // of codes
+  int64_t ldx, ldr, ldh;
+  int w_type, w_vec;         // w_vec: the weight is of the rows' type and aligned to 16 bytes
+  int M, K;
+  int ldq;                   // columns of the codes, K rounded up to 16
+  float eps;
+};
+
+__device__ __forceinline__ float weight(const NormParams& p, int k) {
+  if (p.w_type == TAC_F32) return __ldg(static_cast<const float*>(p.w) + k);
+  const uint16_t b = __ldg(static_cast<const uint16_t*>(p.w) + k);
+  return p.w_type == TAC_F16 ? __half2float(__ushort_as_half(b)) : __uint_as_float(uint32_t(b) << 16);
+}
+
+// What a row's sums give: the factor of h * w, and for codes the factor of y
+// and the scale.  max_bits: the largest magnitude of h * w as bits, in which
+// infinities and NaN order above every finite value.
+struct RowNorm {
+  float rstd, inv, scale;
+};
+template <bool I8>
+__device__ __forceinline__ RowNorm row_norm(const NormParams& p, float ss, uint32_t max_bits) {
+  RowNorm n;
+  n.rstd = __frsqrt_rn(ss / float(p.K) + p.eps);
+  n.inv = n.scale = 0.f;
+  if (I8) {
+    const float top = __uint_as_float(max_bits) * n.rstd;
+    const bool finite = top < __uint_as_float(0x7f800000u);      // false for NaN too
+    const float t = fmaxf(top, 1e-8f);
+    n.inv = finite ? __fdiv_rn(127.0f, t) : 0.f;
+    n.scale = finite ? __fdiv_rn(t, 127.0f) : __uint_as_float(0x7fc00000u);
+  }
+  return n;
+}
+
+// The low byte is the code of y = hw * rstd; 0 in a row without a scale.
+__device__ __forceinline__ uint32_t code_bits(float hw, const RowNorm& n) {
+  const float q = __fmul_rn(__fmul_rn(hw, n.rstd), n.inv);
+  return n.inv == 0.f ? 0u : __float_as_uint(__fadd_rn(q, 12582912.f));   // 1.5 * 2^23: rounds to whole numbers
+}
+
+template <int WPR>
+__device__ __forceinline__ void reduce_row(float& ss, uint32_t& mb) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+  mb = __reduce_max_sync(0xffffffffu, mb);
+  if constexpr (WPR > 1) {
+    __shared__ float red_s[WPR];
+    __shared__ uint32_t red_m[WPR];
+    const int warp = threadIdx.x >> 5;
+    if ((threadIdx.x & 31) == 0) red_s[warp] = ss, red_m[warp] = mb;
+    __syncthreads();
+    ss = 0.f;
+    mb = 0;
+#pragma unroll
+    for (int w = 0; w < WPR; ++w) ss += red_s[w], mb = max(mb, red_m[w]);
+  }
+}
+
+// WPR warps a row (one: four rows a CTA), CH loads of VEC consecutive values a
+// thread.  A row is read once and stays in registers as h * w: the sum of h^2
+// and the largest |h * w| are reduced together, because the norm's factor is
+// the same for the whole row, so that one exchange among the warps gives both
+// the norm and the codes' scale.  h goes out, rounded, as soon as it is there;
+// the norm is of the unrounded sum.
+template <typename T, int VEC, bool I8, int WPR, int CH>
+__global__ void __launch_bounds__(WPR == 1 ? 128 : 32 * WPR) norm_kernel(NormParams p) {
+  constexpr int kLanes = 32 * WPR;
+  const int64_t row = WPR == 1 ? int64_t(blockIdx.x) * 4 + (threadIdx.x >> 5) : blockIdx.x;
+  if (row >= p.M) return;                        // a whole warp (WPR 1); otherwise none
+  const int t = threadIdx.x % kLanes;
+  const T* x = static_cast<const T*>(p.x) + row * p.ldx;
+  const T* r = p.r ? static_cast<const T*>(p.r) + row * p.ldr : nullptr;
+  T* h = p.r ? static_cast<T*>(p.h) + row * p.ldh : nullptr;
+  float v[CH][VEC];
+  float ss = 0.f;
+  uint32_t mb = 0;
+#pragma unroll
+  for (int c = 0; c < CH; ++c) {
+    const int k = (t + c * kLanes) * VEC;
+    if (k < p.K) load_n<T, VEC>(x + k, v[c]);
+  }
+  if (r) {
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      const int k = (t + c * kLanes) * VEC;
+      if (k < p.K) {
+        float a[VEC];
+        load_n<T, VEC>(r + k, a);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) v[c][j] += a[j];
+      }
+    }
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      const int k = (t + c * kLanes) * VEC;
+      if (k < p.K) store_n<T, VEC>(h + k, v[c]);
+    }
+  }
+#pragma unroll
+  for (int c = 0; c < CH; ++c) {
+    const int k = (t + c * kLanes) * VEC;
+    if (k < p.K) {
+      float w[VEC];
+      if (VEC > 1 && p.w_vec) {
+        load_n<T, VEC>(static_cast<const T*>(p.w) + k, w);
+      } else {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) w[j] = weight(p, k + j);
+      }
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        ss = fmaf(v[c][j], v[c][j], ss);
+        v[c][j] *= w[j];
+        if (I8) mb = max(mb, __float_as_uint(v[c][j]) & 0x7fffffffu);
+      }
+    }
+  }
+  reduce_row<WPR>(ss, mb);
+  const RowNorm n = row_norm<I8>(p, ss, mb);
+  if constexpr (!I8) {
+    T* y = static_cast<T*>(p.y) + row * p.K;
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      const int k = (t + c * kLanes) * VEC;
+      if (k < p.K) {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) v[c][j] *= n.rstd;
+        store_n<T, VEC>(y + k, v[c]);
+      }
+    }
+  } else {
+    uint8_t* q = static_cast<uint8_t*>(p.y) + row * p.ldq;
+    if (t == 0) p.scale[row] = n.scale;
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      const int k = (t + c * kLanes) * VEC;
+      if (k >= p.K) break;
+      if constexpr (VEC == 1) {
+        q[k] = uint8_t(code_bits(v[c][0], n));
+      } else {
+#pragma unroll
+        for (int j = 0; j < VEC; j += 4) {
+          const uint32_t lo = __byte_perm(code_bits(v[c][j], n), code_bits(v[c][j + 1], n), 0x0040);
+          const uint32_t hi = __byte_perm(code_bits(v[c][j + 2], n), code_bits(v[c][j + 3], n), 0x0040);
+          reinterpret_cast<uint32_t*>(q + k)[j / 4] = __byte_perm(lo, hi, 0x5410);
+        }
+      }
+    }
+    for (int k = p.K + t; k < p.ldq; k += kLanes) q[k] = 0;      // the padding columns
+  }
+}
+
+// Rows too long for registers: they are read again for the results.  h is
+// written then, so that it may lie over the residual.
+constexpr int kLongThreads = 1024;
+template <typename T, bool I8>
+__global__ void __launch_bounds__(kLongThreads) norm_long_kernel(NormParams p) {
+  const int64_t row = blockIdx.x;
+  const T* x = static_cast<const T*>(p.x) + row * p.ldx;
+  const T* r = p.r ? static_cast<const T*>(p.r) + row * p.ldr : nullptr;
+  float ss = 0.f;
+  uint32_t mb = 0;
+  for (int k = threadIdx.x; k < p.K; k += kLongThreads) {
+    const float v = to_f(x[k]) + (r ? to_f(r[k]) : 0.f);
+    ss = fmaf(v, v, ss);
+    if (I8) mb = max(mb, __float_as_uint(v * weight(p, k)) & 0x7fffffffu);
+  }
+  reduce_row<kLongThreads / 32>(ss, mb);
+  const RowNorm n = row_norm<I8>(p, ss, mb);
+  if (I8 && threadIdx.x == 0) p.scale[row] = n.scale;
+  for (int k = threadIdx.x; k < p.K; k += kLongThreads) {
+    const float v = to_f(x[k]) + (r ? to_f(r[k]) : 0.f);
+    if (r) from_f(static_cast<T*>(p.h)[row * p.ldh + k], v);
+    const float hw = v * weight(p, k);
+    if constexpr (I8) static_cast<uint8_t*>(p.y)[row * p.ldq + k] = uint8_t(code_bits(hw, n));
+    else from_f(static_cast<T*>(p.y)[row * p.K + k], hw * n.rstd);
+  }
+  if constexpr (I8)
+    for (int k = p.K + threadIdx.x; k < p.ldq; k += kLongThreads) static_cast<uint8_t*>(p.y)[row * p.ldq + k] = 0;
+}
+
+template <typename T, bool I8>
+int launch_norm(const NormParams& p, cudaStream_t st) {
+  constexpr int kVec = 16 / sizeof(T);
+  const int e = sizeof(T);
+  auto rows_vec = [&](const void* a, int64_t ld) { return aligned(a, 16) && (p.M == 1 || (ld * e) % 16 == 0); };
+  const bool vec = p.K % kVec == 0 && rows_vec(p.x, p.ldx) && (!p.r || (rows_vec(p.r, p.ldr) && rows_vec(p.h, p.ldh))) &&
+                   (I8 || rows_vec(p.y, p.K));
+  if (vec && p.K <= 32 * 4 * kVec) return launch(norm_kernel<T, kVec, I8, 1, 4>, (p.M + 3) / 4, 128, 0, st, p);
+  if (vec && p.K <= 128 * 4 * kVec) return launch(norm_kernel<T, kVec, I8, 4, 4>, p.M, 128, 0, st, p);
+  if (vec && p.K <= 512 * 4 * kVec) return launch(norm_kernel<T, kVec, I8, 16, 4>, p.M, 512, 0, st, p);
+  if (p.K <= 128 * 32) return launch(norm_kernel<T, 1, I8, 4, 32>, p.M, 128, 0, st, p);
+  if (p.K <= 512 * 32) return launch(norm_kernel<T, 1, I8, 16, 32>, p.M, 512, 0, st, p);
+  return launch(norm_long_kernel<T, I8>, p.M, kLongThreads, 0, st, p);
+}
+
+template <bool I8>
+int pick_norm(NormParams p, int type, cudaStream_t st) {
+  if (type == TAC_F32) return launch_norm<float, I8>(p, st);
+  if (type == TAC_F16) return launch_norm<__half, I8>(p, st);
+  return launch_norm<__nv_bfloat16, I8>(p, st);
+}
+
+// Checks that both forms share.
+int check_norm(const void* X, int type, int64_t ldx, const void* R, int64_t ldr, const void* H, int64_t ldh, const void* W,
+               int w_type, const void* Y, float eps, int M, int K) {
+  if (!X || !W || !Y || !type_ok(type) || !type_ok(w_type) || M <= 0 || K <= 0 || !R != !H) return TAC_E_ARGUMENT;
+  if (M > 1 && (ldx < K || (R && (ldr < K || ldh < K)))) return TAC_E_ARGUMENT;
+  const int e = elem(type);
+  if (!aligned(X, e) || (R && (!aligned(R, e) || !aligned(H, e))) || !aligned(W, elem(w_type))) return TAC_E_ARGUMENT;
+  return eps >= 0.f && eps <= 1e30f ? TAC_OK : TAC_E_ARGUMENT;   // NaN is neither
+}
+
+NormParams norm_params(const void* X, int type, int64_t ldx, const void* R, int64_t ldr, void* H, int64_t ldh, const void* W,
+                       int w_type, void* Y, float* scale, float eps, int M, int K) {
+  NormParams p{};
+  p.x = X, p.r = R, p.h = H, p.w = W, p.y = Y, p.scale = scale;
+  p.ldx = ldx, p.ldr = ldr, p.ldh = ldh;
+  p.w_type = w_type, p.w_vec = w_type == type && aligned(W, 16);
+  p.M = M, p.K = K, p.ldq = int((int64_t(K) + 15) / 16 * 16);
+  p.eps = eps;
+  return p;
+}
+
+// ---- the values of codes ---------------------------------------------------------------------------------------------
+constexpr int kDqThreads = 256;
+
+// VEC codes a thread; a row is cut into `cuts` CTAs.
+template <typename T, int VEC>
+__global__ void __launch_bounds__(kDqThreads) dequant_rows_kernel(const int8_t* __restrict__ Q, int ldq,
+                                                                  const float* __restrict__ scale, T* __restrict__ Y, int K,
+                                                                  int cuts) {
+  const int64_t row = blockIdx.x / cuts;
+  const int k = ((blockIdx.x % cuts) * kDqThreads + threadIdx.x) * VEC;
+  if (k >= K) return;
+  const float s = __ldg(scale + row);
+  float v[VEC];
+  if constexpr (VEC == 1) {
+    v[0] = float(Q[row * ldq + k]) * s;
+  } else {
+    const uint2 u = __ldg(reinterpret_cast<const uint2*>(Q + row * ldq + k));
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) v[j] = float(int8_t((j < 4 ? u.x : u.y) >> (8 * (j & 3)))) * s;
+  }
+  store_n<T, VEC>(Y + row * K + k, v);
+}
+
+template <typename T>
+int launch_dequant(const int8_t* Q, int ldq, const float* scale, T* Y, int M, int K, cudaStream_t st) {
+  const bool vec = K % 8 == 0 && aligned(Y, 16);
+  const int64_t per = int64_t(kDqThreads) * (vec ? 8 : 1), cuts = (K + per - 1) / per;
+  if (M * cuts > 0x7fffffff) return TAC_E_ARGUMENT;
+  if (vec) return launch(dequant_rows_kernel<T, 8>, unsigned(M * cuts), kDqThreads, 0, st, Q, ldq, scale, Y, K, int(cuts));
+  return launch(dequant_rows_kernel<T, 1>, unsigned(M * cuts), kDqThreads, 0, st, Q, ldq, scale, Y, K, int(cuts));
+}
+
+}  // namespace
+
+extern "C" int tac_rms_norm(const void* X, int type, int64_t ldx, const void* R, int64_t ldr, void* H, int64_t ldh,
+                            const void* W, int w_type, float eps, void* Y, int M, int K, void* stream) {
+  if (int s = check_norm(X, type, ldx, R, ldr, H, ldh, W, w_type, Y, eps, M, K)) return s;
+  if (!aligned(Y, elem(type))) return TAC_E_ARGUMENT;
+  return pick_norm<false>(norm_params(X, type, ldx, R, ldr, H, ldh, W, w_type, Y, nullptr, eps, M, K), type,
+                          static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int tac_rms_norm_i8(const void* X, int type, int64_t ldx, const void* R, int64_t ldr, void* H, int64_t ldh,
+                               const void* W, int w_type, float eps, int8_t* Q, float* scale, int M, int K, void* stream) {
+  if (int s = check_norm(X, type, ldx, R, ldr, H, ldh, W, w_type, Q, eps, M, K)) return s;
+  if (!scale || !aligned(Q, 16) || !aligned(scale, 4) || K > (1 << 30)) return TAC_E_ARGUMENT;
+  return pick_norm<true>(norm_params(X, type, ldx, R, ldr, H, ldh, W, w_type, Q, scale, eps, M, K), type,
+                         static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int tac_dequantize_rows_i8(const int8_t* Q, const float* scale, void* Y, int y_type, int M, int K, void* stream) {
+  if (!Q || !scale || !Y || !type_ok(y_type) || M <= 0 || K <= 0 || K > (1 << 30) || !aligned(Q, 16) || !aligned(scale, 4) ||
+      !aligned(Y, elem(y_type)))
+    return TAC_E_ARGUMENT;
+  const int ldq = (K + 15) / 16 * 16;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (y_type == TAC_F32) return launch_dequant(Q, ldq, scale, static_cast<float*>(Y), M, K, st);
+  if (y_type == TAC_F16) return launch_dequant(Q, ldq, scale, static_cast<__half*>(Y), M, K, st);
+  return launch_dequant(Q, ldq, scale, static_cast<__nv_bfloat16*>(Y), M, K, st);
+}

@@ -11,6 +11,7 @@ from . import _lib as L
 from .errors import EngineError
 
 _lib = L.lib
+SRAM_BYTES = 448 * 1024   # ABUF, WBUF and ACCUM, with which a sequence's block begins
 
 # numpy views of the plan records (layout of tac::DevOp / Segment / Task)
 DEVOP_DTYPE = np.dtype([
@@ -281,3 +282,11 @@ class Engine:
         sb, ss, sh = C.c_void_p(), C.c_uint64(), C.c_void_p()
         L.check(_lib.tac_engine_layout(self.handle, C.byref(sb), C.byref(ss), C.byref(sh)), "tac_engine_layout")
         return sb.value, ss.value, sh.value
+
+    def dram_address(self, addr: int):
+        """(device address of byte `addr` of sequence 0's writable DRAM, bytes from one sequence's to the next), until a
+        program with a larger arena runs."""
+        if not self.shared_bytes <= addr < self.dram_bytes:
+            raise ValueError(f"address {addr:#x} is not in the writable DRAM [{self.shared_bytes:#x}, {self.dram_bytes:#x})")
+        base, stride, _ = self.layout()
+        return base + SRAM_BYTES + addr - self.shared_bytes, stride

@@ -11,6 +11,8 @@ device-memory plumbing).
 ``quantize_rows(X)``           tac_quantize_rows_i8: activations to int8, a
                                scale for each row (the A operand and a_scale
                                of ``gemm.gemm_i8_scaled``)
+``dequantize_rows(q, scale)``  tac_dequantize_rows_i8: the values such rows
+                               stand for
 ``rotate_residual_stream_state_dict(sd, model_args, R)``
                                QuaRot's offline weight rotation
                                (software/taccel/quantizer/rotation.py:158-321):
@@ -78,6 +80,34 @@ def quantize_rows(X):
         call("tac_quantize_rows_i8", L.lib.tac_quantize_rows_i8, X.get_device(), X.data_ptr(), xt, ldx, q.data_ptr(),
              scale.data_ptr(), M, K)
     return q, scale
+
+
+def dequantize_rows(q, scale, K=None, dtype=None):
+    """[M, K] q[m, k] * scale[m] (float32 unless `dtype` is float16 or bfloat16): the values that the rows of
+    ``quantize_rows`` or ``norm.rms_norm_i8`` stand for.  q int8 [M, K_pad], scale float32 [M]; K, by default all
+    columns, leaves out the padding ones.  No gradient flows through the call."""
+    import torch
+    from ._tensors import call, type_code
+    dtype = torch.float32 if dtype is None else dtype
+    yt = type_code(dtype, "dtype")
+    if q.dtype is not torch.int8 or scale.dtype is not torch.float32:
+        raise TypeError("q must be int8 and scale float32")
+    shape = q.shape
+    if len(shape) != 2 or shape[1] == 0 or shape[1] % 16 or scale.shape != shape[:1]:
+        raise ValueError(f"q must be [M, a multiple of 16] with scale [M], got {tuple(shape)} and {tuple(scale.shape)}")
+    if not (q.is_contiguous() and scale.is_contiguous()):
+        raise ValueError("q and scale must be contiguous")
+    dev = q.get_device()
+    if dev < 0 or scale.get_device() != dev:
+        raise ValueError("q and scale must be on one CUDA device")
+    K = shape[1] if K is None else K
+    if not shape[1] - 16 < K <= shape[1]:
+        raise ValueError(f"K must be {shape[1] - 15} to {shape[1]}, got {K}")
+    y = torch.empty((shape[0], K), dtype=dtype, device=q.device)
+    if shape[0]:
+        call("tac_dequantize_rows_i8", L.lib.tac_dequantize_rows_i8, dev, q.data_ptr(), scale.data_ptr(), y.data_ptr(),
+             yt, shape[0], K)
+    return y
 
 
 def rotate_residual_stream_state_dict(state_dict: dict, model_args: dict, R) -> list:

@@ -272,6 +272,20 @@ class BatchedRunner:
         """Greedy token of every sequence (device int32[batch]) from this step's logits."""
         self.engine.argmax_f16(self.logits_offset(name), vocab, out_dev_ptr, stream)
 
+    def token_logprobs(self, name: str, tokens, vocab: int, top: int = 0):
+        """Log-probabilities of one token a sequence, the entropy and the `top` likeliest tokens from this step's
+        logits, as device tensors (``logprobs.token_logprobs``); tokens: int32 or int64, a tensor on the runner's
+        device or a sequence.  Runs on torch's current stream, on which the step has to have run too."""
+        import torch
+        from . import logprobs
+        if not 0 < vocab <= self.logits_count:
+            raise ValueError(f"vocab must be 1 to {self.logits_count}, got {vocab}")
+        if not torch.is_tensor(tokens):
+            tokens = torch.as_tensor(np.asarray(tokens, dtype=np.int64).reshape(self.batch))
+        tokens = tokens.to(torch.device("cuda", self.device))
+        address, stride = self.engine.dram_address(self.logits_offset(name))
+        return logprobs.of_rows(address, L.TYPE_F16, stride // 2, self.batch, vocab, tokens, top)
+
     def step_async(self, name: str, tokens, positions, stream=None) -> None:
         """One step, its runtime parameters computed from tokens and positions
         on the host without building the instruction words (the same values
