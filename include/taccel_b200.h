@@ -457,6 +457,43 @@ int tac_kv4_attention(const tac_kv4_cache* cache, const int32_t* page_table, con
                       int64_t q_head, int q_heads, int type, float scale, int causal, void* O, float* lse,
                       void* workspace, uint64_t workspace_bytes, void* stream);
 
+/* ---- 4-bit microscaled rows (MXFP4) ------------------------------------------
+ * Rows of K values in blocks of 32 along K (the last may have fewer): codes
+ * [rows][16 * blocks], E2M1, value 2j in the low and 2j + 1 in the high half of
+ * byte j, and a scale byte a block, which stands for 2^(byte - 127), 255 for
+ * NaN.  Scale bytes are laid out as the tensor cores take them: with `pieces` =
+ * K / 256 rounded up, times 2, the byte of row m and block b is at
+ *   ((m / 128) * pieces + b / 4) * 512 + (m % 32) * 16 + (m % 128 / 32) * 4 + b % 4,
+ * bytes of no row or block below 255.  Both arrays are 16-byte aligned and of
+ * the sizes the two queries give.  K at most 2^24.  No counterpart in the
+ * reference, whose weights are INT8. */
+uint64_t tac_mxfp4_code_bytes(int rows, int K);
+uint64_t tac_mxfp4_scale_bytes(int rows, int K);
+
+/* Rows of X[M,K] (x_type, row stride ldx elements) to that form: scale byte =
+ * max(floor(log2 max |x|) + 125, 0) of the block, codes the nearest E2M1 values
+ * of x / 2^(byte - 127), ties to the even code, magnitudes at most 6.  A block
+ * that holds an infinity or a NaN gets the byte 255 and codes 0. */
+int tac_mxfp4_quantize(const void* X, int x_type, int64_t ldx, uint8_t* codes, uint8_t* scales, int M, int K,
+                       void* stream);
+
+/* What such rows stand for: Y[M,K] (y_type, contiguous), rounded once. */
+int tac_mxfp4_values(const uint8_t* codes, const uint8_t* scales, void* Y, int y_type, int M, int K, void* stream);
+
+/* Y[M,N] (y_type) = A[M,K] @ B[N,K]^T (+ bias[n]) of two operands in that form;
+ * float32 sums, one rounding.  M up to 2^20 and N up to 2^30; bias may be null.
+ * Asynchronous on `stream`; tac_gemm_status reports device faults. */
+int tac_mxfp4_gemm(const uint8_t* a_codes, const uint8_t* a_scales, const uint8_t* b_codes, const uint8_t* b_scales,
+                   const void* bias, int bias_type, void* Y, int y_type, int M, int N, int K, void* stream);
+
+/* The same product of floating-point rows X[M,K], quantised in the call as
+ * tac_mxfp4_quantize does.  Calls that share a workspace (256-byte aligned, at
+ * least the bytes of the query; null where that gives 0) must not overlap. */
+uint64_t tac_linear_mxfp4_workspace_bytes(int M, int N, int K);
+int tac_linear_mxfp4(const void* X, int x_type, int64_t ldx, const uint8_t* b_codes, const uint8_t* b_scales,
+                     const void* bias, int bias_type, void* Y, int y_type, void* workspace, uint64_t workspace_bytes,
+                     int M, int N, int K, void* stream);
+
 /* ---- Probabilities of tokens -------------------------------------------------
  * Of the softmax of each row of X[M,V] (`type`, row stride ldx elements):
  * logprob[m] = log p(tokens[m]) (tokens int32, or int64 with tokens_64 != 0; NaN

@@ -12,6 +12,7 @@ classes keep the reference interfaces:
 * ``gemm``           - stand-alone INT8 GEMM kernels with requant epilogues, INT8 linear layers with a scale for
   each token and channel
 * ``kv4``            - 4-bit paged key / value cache and attention over it
+* ``mxfp4``          - 4-bit microscaled rows (MXFP4): quantiser, products, linear layers
 * ``norm``           - root-mean-square norm with the residual's addition, to rows or INT8 rows
 * ``logprobs``       - log-probabilities of given tokens, entropy and the likeliest tokens of rows of logits
 """
@@ -29,6 +30,6 @@ def __getattr__(name):
     import importlib
     if name in _LAZY:
         return getattr(importlib.import_module(f".{_LAZY[name]}", __name__), name)
-    if name in ("gemm", "kv4", "logprobs", "norm"):
+    if name in ("gemm", "kv4", "logprobs", "mxfp4", "norm"):
         return importlib.import_module(f".{name}", __name__)
     raise AttributeError(name)

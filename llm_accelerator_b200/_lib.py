@@ -131,6 +131,13 @@ SIGNATURES = {
     "tac_rms_norm_i8": (_I, [_P, _I, _I64, _P, _I64, _P, _I64, _P, _I, C.c_float, _P, _P, _I, _I, _P]),
     "tac_dequantize_rows_i8": (_I, [_P, _P, _P, _I, _I, _I, _P]),
     "tac_token_logprobs": (_I, [_P, _I, _I64, _P, _I, _I, _I, _I, _P, _P, _P, _P, _P]),
+    "tac_mxfp4_code_bytes": (_U64, [_I, _I]),
+    "tac_mxfp4_scale_bytes": (_U64, [_I, _I]),
+    "tac_mxfp4_quantize": (_I, [_P, _I, _I64, _P, _P, _I, _I, _P]),
+    "tac_mxfp4_values": (_I, [_P, _P, _P, _I, _I, _I, _P]),
+    "tac_mxfp4_gemm": (_I, [_P, _P, _P, _P, _P, _I, _P, _I, _I, _I, _I, _P]),
+    "tac_linear_mxfp4_workspace_bytes": (_U64, [_I, _I, _I]),
+    "tac_linear_mxfp4": (_I, [_P, _I, _I64, _P, _P, _P, _I, _P, _I, _P, _U64, _I, _I, _I, _P]),
     "tac_quantize_weight_i8": (_I, [_P, _I, _I, _I, _P, _P, _P, _P]),
     "tac_bundle_open": (_I, [C.c_char_p, C.POINTER(BundleView), C.POINTER(_P)]),
     "tac_bundle_close": (_I, [_P]),

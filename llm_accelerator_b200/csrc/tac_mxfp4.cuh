@@ -1,0 +1,359 @@
+// Products of 4-bit microscaled rows:
+//   y[m, n] = sum_k A[m, k] B[n, k] (+ bias[n])
+// A [M, K] and B [N, K] E2M1 codes, two a byte and K-major, each 32 values
+// along K with one power of two (E8M0).  tcgen05 kind::mxf4 multiplies codes
+// and scales and sums in float32; one rounding to the output's type.
+//
+// Orientation: the 128 rows of the MMA are channels (B) and its columns tokens
+// (A), as in the INT8 products: few padded tokens in a ragged batch, a thread
+// of the epilogue holds one channel, and a warp stores 32 consecutive channels
+// of one token whatever the alignment of N.
+//
+// Scales lie in memory as TMEM wants them: for each 128 rows and 128 columns
+// (four blocks) one piece of 512 bytes, 16 bytes for each of 32 lanes, in it
+// the four blocks' bytes of rows lane, lane + 32, lane + 64, lane + 96.  Pieces
+// of 128 rows follow each other along K, an even number of them, so that a
+// stage of 256 columns is 1024 bytes that one bulk copy brings to shared
+// memory and two tcgen05.cp to four columns each of TMEM.
+#pragma once
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cstdint>
+
+#include "tac_sm100.cuh"
+
+namespace tac {
+
+enum MxFault : int { MX_TIMEOUT_EMPTY = 21, MX_TIMEOUT_FULL = 22, MX_TIMEOUT_ACC = 23, MX_TIMEOUT_DRAIN = 24 };
+
+constexpr int kMxStageK = 256;       // columns of a stage: 128 bytes of codes, 1024 of scales for 128 rows
+constexpr int kMxSfBytes = 1024;
+
+// 512-byte pieces of scales along K for each 128 rows
+__host__ __device__ constexpr int64_t mx_pieces(int64_t K) { return (K + kMxStageK - 1) / kMxStageK * 2; }
+
+struct MxParams {
+  const uint8_t* a_scale;    // tokens'
+  const uint8_t* b_scale;    // channels'
+  const void* bias;          // or null
+  void* y;
+  int bias_type;
+  int M, N;
+  int k_stages;              // stages of 256 columns
+  int tn;                    // tokens of a tile
+  int stages;                // of the ring
+  int* fault;
+  int after_rows;            // launched while the row quantiser may still run: A and its scales wait for its end
+};
+
+// ---- PTX ------------------------------------------------------------------------------------------------------------
+namespace sm100 {
+
+// Instruction descriptor of kind::mxf4 with block scales: E2M1 operands (code 1), E8M0 scales (bit 23), both K-major.
+// sf: which half of a scale word the MMA's 64 columns take (0 or 2).
+__host__ __device__ constexpr uint32_t idesc_mxf4(uint32_t M, uint32_t N, uint32_t sf) {
+  return (sf << 4) | (1u << 7) | (1u << 10) | ((N >> 3) << 17) | (1u << 23) | ((M >> 4) << 24) | (sf << 29);
+}
+
+// D(tmem) [+]= A x B with scales in TMEM, 64 columns; issued by one thread.
+__device__ __forceinline__ void mma_mxf4(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t sf_a,
+                                         uint32_t sf_b, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%5], [%6], p;\n\t}\n" ::"r"(tmem_d),
+      "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate), "r"(sf_a), "r"(sf_b));
+}
+
+// One 512-byte piece of scales from shared memory to four columns, for all four quarters of TMEM's lanes.
+__device__ __forceinline__ void cp_scales(uint32_t taddr, uint64_t desc) {
+  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;\n" ::"r"(taddr), "l"(desc));
+}
+
+// Shared-memory descriptor of such a piece: rows of 16 bytes one after the other, no swizzle.
+__device__ __forceinline__ uint64_t smem_desc_scales(uint32_t saddr) {
+  return uint64_t((saddr >> 4) & 0x3FFF) | (uint64_t(1) << 16) | (uint64_t(128 >> 4) << 32) | (uint64_t(1) << 46);
+}
+
+}  // namespace sm100
+
+// ---- epilogue -------------------------------------------------------------------------------------------------------
+__device__ __forceinline__ float mx_ld(const void* p, int type, int64_t i) {
+  if (type == 0) return __ldg(static_cast<const float*>(p) + i);
+  const uint16_t b = __ldg(static_cast<const uint16_t*>(p) + i);
+  return type == 1 ? __half2float(__ushort_as_half(b)) : __uint_as_float(uint32_t(b) << 16);
+}
+
+template <int YT>
+__device__ __forceinline__ void mx_st(void* p, int64_t i, float v) {
+  if constexpr (YT == 0) static_cast<float*>(p)[i] = v;
+  else if constexpr (YT == 1) static_cast<__half*>(p)[i] = __float2half_rn(v);
+  else static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
+}
+
+template <int YT>
+__device__ __forceinline__ uint32_t mx_pair(float lo, float hi) {
+  if constexpr (YT == 1) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  } else {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+}
+
+// 16-bit results of 32 tokens (m ..) and a warp's 32 channels, in pairs of
+// channels: lanes exchange with their neighbours, and of two tokens the even
+// lanes store one's pairs and the odd lanes the other's.  With an odd N every
+// second row begins between two words: its pairs are those of an odd lane and
+// the next, its first and last channel go alone.  Exchanges go before the
+// stores, behind which each would wait.
+template <int YT, bool ODD>
+__device__ __forceinline__ void mx_store_pairs(const MxParams& p, const uint32_t (&v)[32], int m, int n, float bias,
+                                               uint32_t base_odd) {
+  const int lane = threadIdx.x & 31;
+  const uint32_t first = ODD ? (base_odd ^ uint32_t(m & 1)) : 0u;   // the token of a pair whose row is word-aligned here
+  const bool mine_first = (lane & 1) == 0;
+  const int tok = mine_first ? int(first) : int(first ^ 1u);
+  uint16_t* dst = static_cast<uint16_t*>(p.y) + int64_t(m + tok) * p.N + n - (mine_first || ODD ? 0 : 1);
+  uint16_t* edge = static_cast<uint16_t*>(p.y) + int64_t(m + int(first ^ 1u)) * p.N + n;
+  const int64_t step = 2 * int64_t(p.N);
+  const bool has_next = !ODD || lane != 31, is_edge = lane == 0 || lane == 31;
+  const uint32_t edge_shift = first ? 0 : 16;
+  const uint32_t sel = ODD ? (tok ? 0x7632 : 0x5410) : (mine_first ? 0x5410 : 0x3276);
+  uint32_t mine[16], other[16];      // the first token's result low, the second's high
+#pragma unroll
+  for (int j = 0; j < 16; ++j) {
+    mine[j] = mx_pair<YT>(__uint_as_float(v[2 * j]) + bias, __uint_as_float(v[2 * j + 1]) + bias);
+    other[j] = ODD ? __shfl_down_sync(0xffffffffu, mine[j], 1) : __shfl_xor_sync(0xffffffffu, mine[j], 1);
+  }
+  const int left = p.M - m - tok, left_edge = is_edge ? p.M - m - int(first ^ 1u) : 0, left_here = has_next ? left : 0;
+#pragma unroll
+  for (int j = 0; j < 16; ++j, dst += step, edge += step) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.gt.s32 p, %2, %3;\n\t@p st.global.b32 [%0], %1;\n\t}\n" ::"l"(dst),
+                 "r"(__byte_perm(mine[j], other[j], sel)), "r"(left_here), "r"(2 * j)
+                 : "memory");
+    if constexpr (ODD)
+      asm volatile("{\n\t.reg .pred p;\n\tsetp.gt.s32 p, %2, %3;\n\t@p st.global.b16 [%0], %1;\n\t}\n" ::"l"(edge),
+                   "h"(uint16_t(mine[j] >> edge_shift)), "r"(left_edge), "r"(2 * j)
+                   : "memory");
+  }
+}
+
+// 32 tokens (m .. m + 31) of a warp's 32 consecutive channels (n its own); v the sums.
+template <int YT>
+__device__ __forceinline__ void mx_store32(const MxParams& p, const uint32_t (&v)[32], int m, int n, float bias) {
+  const int lane = threadIdx.x & 31;
+  const bool all_channels = n - lane + 32 <= p.N, inside = all_channels && m + 32 <= p.M;
+  const uint32_t base_odd = uint32_t(reinterpret_cast<uintptr_t>(p.y) >> 1) & 1;
+  if (YT == 0 && inside) {
+    float* dst = static_cast<float*>(p.y) + int64_t(m) * p.N + n;
+#pragma unroll
+    for (int j = 0; j < 32; ++j, dst += p.N) *dst = __uint_as_float(v[j]) + bias;
+  } else if (YT != 0 && all_channels && ((p.N & 1) || !base_odd)) {
+    if (p.N & 1) mx_store_pairs<YT, true>(p, v, m, n, bias, base_odd);
+    else mx_store_pairs<YT, false>(p, v, m, n, bias, 0u);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 32; ++j)
+      if (m + j < p.M && n < p.N) mx_st<YT>(p.y, int64_t(m + j) * p.N + n, __uint_as_float(v[j]) + bias);
+  }
+}
+
+// ---- split-K over a cluster -----------------------------------------------------------------------------------------
+// A 128-channel x tn-token tile for each cluster of S CTAs; CTA r sums its
+// share of the stages, leaves the float32 partial sums in its shared memory,
+// and after a cluster barrier finishes every S-th token from all S partials,
+// in the order of the ranks.  For products with too few tiles for 148 SMs,
+// where streaming the weights is the work.
+//   warp 0      loads, warp 1 MMAs, warps 2..5 epilogue.
+// A stage's scales have columns of TMEM of their own, so a copy never meets
+// an MMA that still reads the last ones.
+constexpr int kMxSkThreads = 192;
+constexpr int kMxWBytes = 128 * 128;
+constexpr int kMxSkStages = 8, kMxSkCols = 256, kMxSkSfCol = 128;     // TMEM: sums, then 16 columns of scales a stage
+
+__host__ __device__ constexpr int mx_sk_stage_bytes(int tn) { return kMxWBytes + tn * 128 + 2 * kMxSfBytes; }
+
+// Partial sums of a split tile in shared memory: [128 channels][tn + 4], the padding against bank conflicts.
+__host__ __device__ constexpr int mx_sk_part_bytes(int tn) { return 128 * (tn + 4) * 4; }
+
+// The tile's results, or the CTA's partial sums to shared memory (over its stages: every copy and MMA has ended) and,
+// after the cluster's barrier, CTA r's share of the tokens from all partials.  All threads of the CTA.
+template <int YT>
+__device__ __forceinline__ void mx_splitk_finish(const MxParams& p, uint8_t* smem, uint32_t tmem, int warp, int row, int n, int m0,
+                                                 int rank, int nsplit, float bias, bool acc_ok) {
+  const uint32_t t_addr = tmem + (uint32_t((warp & 3) * 32) << 16);
+  if (nsplit == 1) {
+    if (warp >= 2 && acc_ok)
+      for (int c = 0; c < p.tn; c += 32) {
+        uint32_t v[32];
+        __syncwarp();
+        sm100::tmem_ld32(t_addr + c, v);
+        mx_store32<YT>(p, v, m0 + c, n, bias);   // a tile of 16 tokens has no more than 16 rows before M
+      }
+    return;
+  }
+  float* const mine = reinterpret_cast<float*>(smem) + row * (p.tn + 4);
+  if (warp >= 2) {
+    for (int c = 0; c < p.tn; c += 32) {
+      uint32_t v[32];
+      __syncwarp();
+      sm100::tmem_ld32(t_addr + c, v);
+#pragma unroll
+      for (int j = 0; j < 32; j += 4)
+        if (c + j < p.tn) *reinterpret_cast<uint4*>(mine + c + j) = make_uint4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+    }
+  }
+  __syncwarp();
+  sm100::cluster_sync();
+  const int per = max(4, p.tn / nsplit), first = rank * per;    // tokens of this CTA
+  if (warp >= 2 && first < p.tn) {
+    uint32_t base[8];
+#pragma unroll
+    for (int r = 0; r < 8; ++r) base[r] = sm100::mapa_shared(mine + first, r < nsplit ? r : 0);
+    for (int k = 0; k < per; k += 4) {
+      if (m0 + first + k >= p.M) break;
+      float4 v[8];
+#pragma unroll
+      for (int r = 0; r < 8; ++r) {
+        v[r] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (r < nsplit)
+          asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];\n"
+                       : "=f"(v[r].x), "=f"(v[r].y), "=f"(v[r].z), "=f"(v[r].w)
+                       : "r"(base[r] + k * 4)
+                       : "memory");
+      }
+      float acc[4] = {};
+#pragma unroll
+      for (int r = 0; r < 8; ++r) acc[0] += v[r].x, acc[1] += v[r].y, acc[2] += v[r].z, acc[3] += v[r].w;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int m = m0 + first + k + j;
+        if (m < p.M && n < p.N) mx_st<YT>(p.y, int64_t(m) * p.N + n, acc[j] + bias);
+      }
+    }
+  }
+  __syncwarp();
+  sm100::cluster_sync();                         // no CTA leaves while another reads its partial sums
+}
+
+// The four MMAs of a stage, and before them its scales' copies.  w_sf, a_sf: shared memory; sf: TMEM columns of the stage.
+__device__ __forceinline__ void mx_stage_mma(uint32_t tmem, uint32_t sf, uint64_t dw, uint64_t da, uint64_t w_sf, uint64_t a_sf,
+                                             uint32_t idesc0, uint32_t idesc2, bool first) {
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    sm100::cp_scales(sf + 4 * j, w_sf + j * (512 >> 4));
+    sm100::cp_scales(sf + 8 + 4 * j, a_sf + j * (512 >> 4));
+  }
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    sm100::mma_mxf4(tmem, dw + 2 * k, da + 2 * k, k & 1 ? idesc2 : idesc0, sf + 4 * (k >> 1), sf + 8 + 4 * (k >> 1), !first || k);
+}
+
+template <int YT>
+__global__ void __launch_bounds__(kMxSkThreads)
+    mx_splitk_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_a, MxParams p) {
+  extern __shared__ uint8_t dyn_smem[];
+  __shared__ __align__(8) uint64_t full_bar[kMxSkStages], empty_bar[kMxSkStages], acc_bar;
+  __shared__ uint32_t tmem_base;
+  __shared__ int abort_flag;
+
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(dyn_smem) + 1023) & ~uintptr_t(1023));
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  const int n0 = blockIdx.x * 128, m0 = blockIdx.y * p.tn;
+  const int nsplit = gridDim.z, rank = blockIdx.z;
+  const int kb0 = int(int64_t(p.k_stages) * rank / nsplit), kb1 = int(int64_t(p.k_stages) * (rank + 1) / nsplit);
+  const int S = p.stages, stage_bytes = mx_sk_stage_bytes(p.tn);
+  const int sf_off = kMxWBytes + p.tn * 128;     // of a stage: channels' scales, then tokens'
+  const uint8_t* w_scale = p.b_scale + int64_t(n0 / 128) * p.k_stages * kMxSfBytes;
+  const uint8_t* a_scale = p.a_scale + int64_t(m0 / 128) * p.k_stages * kMxSfBytes;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S; ++s) {
+      sm100::mbar_init(&full_bar[s], 1);
+      sm100::mbar_init(&empty_bar[s], 1);
+    }
+    sm100::mbar_init(&acc_bar, 1);
+    abort_flag = 0;
+    sm100::mbar_fence_init();
+  }
+  if (warp == 1) sm100::tmem_alloc(&tmem_base, kMxSkCols);
+  sm100::tc_fence_before();
+  __syncthreads();
+  sm100::tc_fence_after();
+  const uint32_t tmem = tmem_base;
+  volatile int* abort_v = &abort_flag;
+
+  if (warp == 0) {
+    uint32_t s = 0, ph = 1, issued = 0;
+    auto weights = [&](int i, int kb) {
+      uint8_t* st = smem + i * stage_bytes;
+      sm100::mbar_arrive_expect_tx(&full_bar[i], stage_bytes);
+      sm100::tma_load_2d(st, &tm_w, kb * 128, n0, &full_bar[i]);
+      sm100::bulk_g2s(st + sf_off, w_scale + int64_t(kb) * kMxSfBytes, kMxSfBytes, &full_bar[i]);
+    };
+    // the first stages' weights need not wait for the rows
+    const int early = min(S, kb1 - kb0);
+    if (sm100::elect_one())
+      for (int i = 0; i < early; ++i) weights(i, kb0 + i);
+    __syncwarp();
+    asm volatile("griddepcontrol.wait;\n" ::: "memory");
+    for (int kb = kb0; kb < kb1; ++kb) {
+      if (!sm100::mbar_wait_warp(&empty_bar[s], ph, abort_v, p.fault, MX_TIMEOUT_EMPTY)) break;
+      if (sm100::elect_one()) {
+        uint8_t* st = smem + s * stage_bytes;
+        if (kb - kb0 >= early) weights(s, kb);
+        sm100::tma_load_2d(st + kMxWBytes, &tm_a, kb * 128, m0, &full_bar[s]);
+        sm100::bulk_g2s(st + sf_off + kMxSfBytes, a_scale + int64_t(kb) * kMxSfBytes, kMxSfBytes, &full_bar[s]);
+      }
+      __syncwarp();
+      ++issued;
+      if (++s == uint32_t(S)) s = 0, ph ^= 1;
+    }
+    // the copies still in flight land before the CTA goes on
+    for (uint32_t j = issued > uint32_t(S) ? issued - S : 0; j < issued; ++j)
+      sm100::mbar_wait(&full_bar[j % S], (j / S) & 1, p.fault, MX_TIMEOUT_DRAIN);
+  } else if (warp == 1) {
+    const uint32_t idesc0 = sm100::idesc_mxf4(128, p.tn, 0), idesc2 = sm100::idesc_mxf4(128, p.tn, 2);
+    const uint64_t w0 = sm100::smem_desc_sw128(sm100::smem_u32(smem), 16, 1024);
+    const uint64_t sf0 = sm100::smem_desc_scales(sm100::smem_u32(smem) + sf_off);
+    uint32_t s = 0, ph = 0;
+    for (int kb = kb0; kb < kb1; ++kb) {
+      if (!sm100::mbar_wait_warp(&full_bar[s], ph, abort_v, p.fault, MX_TIMEOUT_FULL)) break;
+      sm100::tc_fence_after();
+      const uint64_t dw = w0 + s * (stage_bytes >> 4), sf = sf0 + s * (stage_bytes >> 4);
+      if (sm100::elect_one()) {
+        mx_stage_mma(tmem, tmem + kMxSkSfCol + 16 * s, dw, dw + (kMxWBytes >> 4), sf, sf + (kMxSfBytes >> 4), idesc0, idesc2, kb == kb0);
+        sm100::mma_commit(&empty_bar[s]);
+      }
+      __syncwarp();
+      if (++s == uint32_t(S)) s = 0, ph ^= 1;
+    }
+    // arrives once every MMA has completed, also after a failed wait
+    if (sm100::elect_one()) sm100::mma_commit(&acc_bar);
+    __syncwarp();
+    sm100::mbar_wait(&acc_bar, 0, p.fault, MX_TIMEOUT_DRAIN);
+  }
+  const int row = (warp & 3) * 32 + lane;     // TMEM lane = channel of the tile (warps 2..5)
+  const int n = n0 + row;
+  float bias = 0.f;
+  bool acc_ok = false;
+  if (warp >= 2) {
+    if (n < p.N && p.bias) bias = mx_ld(p.bias, p.bias_type, n);
+    acc_ok = sm100::mbar_wait_warp(&acc_bar, 0, abort_v, p.fault, MX_TIMEOUT_ACC);
+    __syncwarp();
+    sm100::tc_fence_after();
+  }
+  mx_splitk_finish<YT>(p, smem, tmem, warp, row, n, m0, rank, nsplit, bias, acc_ok);
+  sm100::tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    __syncwarp();
+    sm100::tc_fence_after();
+    sm100::tmem_dealloc(tmem, kMxSkCols);
+  }
+}
+
+}  // namespace tac

@@ -1,0 +1,177 @@
+"""4-bit microscaled rows (MXFP4) and linear layers of them.
+
+``Mxfp4``                    rows held as E2M1 codes with a power of two for each 32 columns
+``quantize(X)``              floating-point rows to that form
+``gemm(a, b)``               Y = A @ B^T (+ bias) of two operands in that form
+``linear(X, w)``             the same product of floating-point rows, quantised in the call
+``linear_workspace(M, K)``   workspace of linear calls
+
+A block of 32 values along K (the last one may have fewer) has e = max(floor(log2 max |x|) - 2, -127) and stands for 2^e
+times the nearest of 0, 0.5, 1, 1.5, 2, 3, 4, 6 with a sign: ties go to the even code, magnitudes above 6 to 6.  A block
+that holds an infinity or a NaN stands for NaN.  Products are summed in float32 and rounded once.  A few channels much
+larger than the rest take the steps of their whole block: rotate rows and weights by ``quarot.fwht_f16`` first where there
+are such.
+
+The calls are for inference: no gradient flows through them, also from tensors that require one.
+"""
+from __future__ import annotations
+
+import torch
+
+from . import _lib as L
+from ._tensors import call, type_code
+
+_U8, _F16, _F32 = torch.uint8, torch.float16, torch.float32
+_quantize, _values, _gemm, _linear = (L.lib.tac_mxfp4_quantize, L.lib.tac_mxfp4_values, L.lib.tac_mxfp4_gemm,
+                                      L.lib.tac_linear_mxfp4)
+
+
+def _scale_shape(rows: int, cols: int):
+    """[128 rows][128 columns][row % 32][row / 32 % 4][block]; an even number of column groups."""
+    return -(-rows // 128), -(-cols // 256) * 2, 32, 4, 4
+
+
+class Mxfp4:
+    """`rows` rows of `cols` values: codes uint8 [rows, 16 blocks] (value 2j in the low, 2j + 1 in the high half of byte j),
+    scales uint8 (the bytes e + 127, 255 for NaN) as the tensor cores take them.  ``from_tensors`` takes scale bytes
+    [rows, blocks] and ``scale_bytes`` gives them back; blocks = cols / 32 rounded up."""
+
+    def __init__(self, codes, scales, cols: int):
+        if codes.dtype is not _U8 or scales.dtype is not _U8:
+            raise TypeError("codes and scales must be uint8")
+        shape = codes.shape
+        if len(shape) != 2 or cols <= 0 or shape[1] != (cols + 31) // 32 * 16:
+            raise ValueError(f"codes of {cols} columns must be [rows, {(cols + 31) // 32 * 16}], got {tuple(shape)}")
+        if scales.shape != _scale_shape(shape[0], cols):
+            raise ValueError(f"scales must be {_scale_shape(shape[0], cols)}, got {tuple(scales.shape)}")
+        if not (codes.is_contiguous() and scales.is_contiguous()):
+            raise ValueError("codes and scales must be contiguous")
+        dev = codes.get_device()
+        if dev < 0 or scales.get_device() != dev:
+            raise ValueError("codes and scales must be on one CUDA device")
+        if (codes.data_ptr() | scales.data_ptr()) & 15:
+            raise ValueError("codes and scales must begin on 16-byte boundaries")
+        self._set(codes, scales, shape[0], cols, dev)
+
+    def _set(self, codes, scales, rows, cols, index):
+        self.codes, self.scales, self.rows, self.cols = codes, scales, rows, cols
+        self.device, self._index = codes.device, index
+        self._pointers = codes.data_ptr(), scales.data_ptr()
+
+    @classmethod
+    def _empty(cls, rows, cols, device, index):
+        self = cls.__new__(cls)
+        self._set(torch.empty((rows, (cols + 31) // 32 * 16), dtype=_U8, device=device),
+                  torch.empty(_scale_shape(rows, cols), dtype=_U8, device=device), rows, cols, index)
+        return self
+
+    @classmethod
+    def from_tensors(cls, codes, scale_bytes, cols: int) -> "Mxfp4":
+        """Of codes [rows, 16 blocks] and scale bytes [rows, blocks]; the scales are laid out once, here.  Columns from
+        `cols` on of the last block must have the code 0."""
+        if scale_bytes.dtype is not _U8:
+            raise TypeError("scale_bytes must be uint8")
+        rows, blocks = codes.shape[0] if codes.dim() == 2 else -1, (cols + 31) // 32
+        if rows < 0 or scale_bytes.shape != (rows, blocks):
+            raise ValueError(f"codes and scale_bytes must be [rows, {16 * blocks}] and [rows, {blocks}], got "
+                             f"{tuple(codes.shape)} and {tuple(scale_bytes.shape)}")
+        r, c = _scale_shape(rows, cols)[:2]
+        laid = torch.zeros((r * 128, c * 4), dtype=_U8, device=scale_bytes.device)
+        laid[:rows, :blocks] = scale_bytes
+        return cls(codes, laid.view(r, 4, 32, c, 4).permute(0, 3, 2, 1, 4).contiguous(), cols)
+
+    def scale_bytes(self):
+        """uint8 [rows, blocks]."""
+        r, c = self.scales.shape[:2]
+        return self.scales.permute(0, 3, 2, 1, 4).reshape(r * 128, c * 4)[:self.rows, :(self.cols + 31) // 32]
+
+    def values(self, dtype=_F32):
+        """[rows, cols] that the codes stand for, rounded to `dtype`."""
+        yt = type_code(dtype, "dtype")
+        y = torch.empty((self.rows, self.cols), dtype=dtype, device=self.device)
+        if self.rows:
+            call("tac_mxfp4_values", _values, self._index, *self._pointers, y.data_ptr(), yt, self.rows, self.cols)
+        return y
+
+
+def _rows(X):
+    """(type, row stride, M, K, device) of floating-point rows X."""
+    xt = type_code(X.dtype, "X")
+    shape, stride = X.shape, X.stride()
+    if len(shape) != 2 or shape[1] == 0 or (shape[1] > 1 and stride[1] != 1):
+        raise ValueError(f"X must be [M, K] with contiguous rows, got shape {tuple(shape)}, stride {stride}")
+    M, K = shape
+    ldx = stride[0] if M > 1 else K
+    if ldx < K:
+        raise ValueError(f"rows of X overlap (stride {ldx}, {K} columns)")
+    dev = X.get_device()
+    if dev < 0:
+        raise ValueError("X must be on a CUDA device")
+    return xt, ldx, M, K, dev
+
+
+def quantize(X) -> Mxfp4:
+    """X [M, K] (float32, float16 or bfloat16, contiguous rows at any row stride) in 4-bit form."""
+    xt, ldx, M, K, dev = _rows(X)
+    q = Mxfp4._empty(M, K, X.device, dev)
+    if M:
+        call("tac_mxfp4_quantize", _quantize, dev, X.data_ptr(), xt, ldx, *q._pointers, M, K)
+    return q
+
+
+def _result(w, M, K, dev, bias, out, dtype):
+    """Checks of what both products share; (out, its type, bias pointer, bias type)."""
+    if w.cols != K or w._index != dev:
+        raise ValueError(f"the operands must have one number of columns and one device, got {K} and {w.cols} columns")
+    N = w.rows
+    bp, bt = None, 0
+    if bias is not None:
+        bt = type_code(bias.dtype, "bias")
+        if bias.shape != (N,) or not bias.is_contiguous() or bias.get_device() != dev:
+            raise ValueError(f"bias must be a contiguous [{N}] tensor on the operands' device")
+        bp = bias.data_ptr()
+    yt = type_code(dtype, "out_dtype")
+    if out is None:
+        out = torch.empty((M, N), dtype=dtype, device=w.device)
+    elif out.dtype is not dtype or out.shape != (M, N) or not out.is_contiguous() or out.get_device() != dev:
+        raise ValueError(f"out must be a contiguous {dtype} [{M}, {N}] tensor on the operands' device")
+    return out, yt, bp, bt
+
+
+def gemm(a: Mxfp4, b: Mxfp4, bias=None, out_dtype=None, out=None):
+    """Y [a.rows, b.rows] = A @ B^T (+ bias[n]); bias and output float32, float16 or bfloat16 (default: out's type, else
+    float16)."""
+    if out_dtype is None:
+        out_dtype = _F16 if out is None else out.dtype
+    M, K, dev = a.rows, a.cols, a._index
+    out, yt, bp, bt = _result(b, M, K, dev, bias, out, out_dtype)
+    if M and b.rows:
+        call("tac_mxfp4_gemm", _gemm, dev, *a._pointers, *b._pointers, bp, bt, out.data_ptr(), yt, M, b.rows, K)
+    return out
+
+
+def linear(X, w: Mxfp4, bias=None, out=None, ws=None):
+    """Y [M, N] in X's type = X [M, K] @ w^T (+ bias[n]), X quantised as ``quantize`` does.
+
+    X float32, float16 or bfloat16 with contiguous rows at any row stride.  ws: a ``linear_workspace`` to reuse across
+    calls on one stream; by default a call allocates its own.  A block of X with an infinity or a NaN gives a row of
+    NaN."""
+    xt, ldx, M, K, dev = _rows(X)
+    out, yt, bp, bt = _result(w, M, K, dev, bias, out, X.dtype)
+    N = w.rows
+    if M and N:
+        if ws is None:
+            ws = torch.empty(L.lib.tac_linear_mxfp4_workspace_bytes(M, N, K) + 256, dtype=_U8, device=X.device)
+        elif ws.get_device() != dev or ws.dtype is not _U8 or not ws.is_contiguous():
+            raise ValueError("ws must be a linear_workspace on X's device")
+        p = ws.data_ptr()
+        wp = (p + 255) & ~255
+        call("tac_linear_mxfp4", _linear, dev, X.data_ptr(), xt, ldx, *w._pointers, bp, bt, out.data_ptr(), yt, wp,
+             max(ws.numel() - (wp - p), 0), M, N, K)
+    return out
+
+
+def linear_workspace(M: int, K: int, device="cuda"):
+    """A workspace for linear calls of at most M rows of K columns (calls that share one must not overlap)."""
+    codes, scales = L.lib.tac_mxfp4_code_bytes(M, K), L.lib.tac_mxfp4_scale_bytes(M, K)
+    return torch.empty((codes + 255) // 256 * 256 + (scales + 255) // 256 * 256 + 256, dtype=_U8, device=device)
