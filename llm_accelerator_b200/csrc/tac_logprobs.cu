@@ -1,10 +1,10 @@
 // Log-probabilities of given tokens, the entropy and the likeliest tokens of
 // rows of logits, in one read of the logits.
 //
-// With m the largest logit, d = (x - m) log2 e, S = sum 2^d and T = sum 2^d d:
-//   log p(v) = (x_v - m) - ln S,   entropy = ln S - ln 2 * T / S,
+// With m the largest logit, d = x - m, S = sum e^d and T = sum e^d d:
+//   log p(v) = (x_v - m) - ln S,   entropy = ln S - T / S,
 // in which nothing cancels (all d <= 0).  A thread keeps (m, S, T) of what it
-// has read, rescaled as its m grows; two such triples join into one.
+// has read, rescaled as its m grows; such triples join into one.
 //
 // The k likeliest: k of the threads' largest values give a lower bound on the
 // k-th largest logit, so only threads whose largest value reaches the bound
@@ -25,9 +25,9 @@ namespace {
 
 using namespace tac;
 
-constexpr int kThreads = 256, kWarps = kThreads / 32, kMostTop = 32, kMostCtas = 8;
-constexpr int kRoom = kThreads * 8 + 64;   // collected entries: all of a share that leaves a thread without any
+constexpr int kMostTop = 32, kMostCtas = 8;
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.693147180559945309417f;
+
 
 struct LpParams {
   const void* x;
@@ -41,6 +41,12 @@ struct LpParams {
   int32_t* top_ids;
 };
 
+// 16 bytes that will not be read again, or only a few of them
+__device__ __forceinline__ uint4 load_once(const uint4* p) {
+  uint4 u;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];\n" : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w) : "l"(p));
+  return u;
+}
 __device__ __forceinline__ float ninf() { return __uint_as_float(0xff800000u); }
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -68,16 +74,46 @@ __device__ __forceinline__ uint64_t entry(uint32_t key, int64_t i) { return uint
 struct Sums {
   float m, s, t;             // m -inf: nothing yet, s = t = 0
 };
-__device__ __forceinline__ void add_scaled(Sums& a, float m, float s, float t) {
-  if (m == ninf()) return;
-  const float d = max_nan((m - a.m) * kLog2e, -200.f), f = ex2(d);   // -200: 2^d is 0, and d stays finite
-  a.s = fmaf(s, f, a.s);
-  a.t = fmaf(fmaf(d, s, t), f, a.t);
+// The same sums about another m, at least their own: e^-200 is 0, and d stays finite.
+__device__ __forceinline__ void about(Sums& a, float m) {
+  const float d = a.m == ninf() ? 0.f : max_nan(a.m - m, -200.f), f = ex2(d * kLog2e);
+  a.t = fmaf(d, a.s, a.t) * f;
+  a.s *= f;
+  a.m = m;
 }
-__device__ __forceinline__ Sums join(const Sums& a, const Sums& b) {
-  Sums r{max_nan(a.m, b.m), 0.f, 0.f};
-  add_scaled(r, a.m, a.s, a.t);
-  add_scaled(r, b.m, b.s, b.t);
+// The sums of neighbouring lanes, in all of them, about the largest of their `m`, which is no less than what theirs are about.
+template <int LANES>
+__device__ __forceinline__ Sums join(Sums a, float m) {
+#pragma unroll
+  for (int o = LANES / 2; o; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+  about(a, m);
+#pragma unroll
+  for (int o = LANES / 2; o; o >>= 1) {
+    a.s += __shfl_xor_sync(0xffffffffu, a.s, o);
+    a.t += __shfl_xor_sync(0xffffffffu, a.t, o);
+  }
+  return a;
+}
+
+// Pairs of float32 values in one register pair.
+__device__ __forceinline__ uint64_t pair_of(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};\n" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ float2 of_pair(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;\n" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;\n" : "=l"(r) : "l"(a), "l"(b), "l"(c));
   return r;
 }
 
@@ -91,8 +127,13 @@ struct Vec<float> {
   static __device__ __forceinline__ void values(const uint4& u, float (&v)[4]) {
     v[0] = __uint_as_float(u.x), v[1] = __uint_as_float(u.y), v[2] = __uint_as_float(u.z), v[3] = __uint_as_float(u.w);
   }
-  static __device__ __forceinline__ float largest(const uint4& u) {
-    return max_nan(max_nan(__uint_as_float(u.x), __uint_as_float(u.y)), max_nan(__uint_as_float(u.z), __uint_as_float(u.w)));
+  template <int NV>
+  static __device__ __forceinline__ float largest(const uint4 (&u)[NV]) {
+    float m = __uint_as_float(u[0].x);
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      m = max_nan(max_nan(m, __uint_as_float(u[i].x)), max_nan(max_nan(__uint_as_float(u[i].y), __uint_as_float(u[i].z)), __uint_as_float(u[i].w)));
+    return m;
   }
 };
 template <>
@@ -111,8 +152,12 @@ struct Vec<__half> {
       v[2 * j] = f.x, v[2 * j + 1] = f.y;
     }
   }
-  static __device__ __forceinline__ float largest(const uint4& u) {
-    const float2 f = __half22float2(__hmax2_nan(__hmax2_nan(pair(u.x), pair(u.y)), __hmax2_nan(pair(u.z), pair(u.w))));
+  template <int NV>
+  static __device__ __forceinline__ float largest(const uint4 (&u)[NV]) {
+    __half2 m = pair(u[0].x);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) m = __hmax2_nan(__hmax2_nan(m, pair(u[i].x)), __hmax2_nan(__hmax2_nan(pair(u[i].y), pair(u[i].z)), pair(u[i].w)));
+    const float2 f = __half22float2(m);
     return max_nan(f.x, f.y);
   }
 };
@@ -129,36 +174,68 @@ struct Vec<__nv_bfloat16> {
 #pragma unroll
     for (int j = 0; j < 4; ++j) v[2 * j] = __uint_as_float(w[j] << 16), v[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
   }
-  static __device__ __forceinline__ float largest(const uint4& u) {
-    const __nv_bfloat162 m = __hmax2_nan(__hmax2_nan(pair(u.x), pair(u.y)), __hmax2_nan(pair(u.z), pair(u.w)));
+  template <int NV>
+  static __device__ __forceinline__ float largest(const uint4 (&u)[NV]) {
+    __nv_bfloat162 m = pair(u[0].x);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) m = __hmax2_nan(__hmax2_nan(m, pair(u[i].x)), __hmax2_nan(__hmax2_nan(pair(u[i].y), pair(u[i].z)), pair(u[i].w)));
     const uint32_t b = *reinterpret_cast<const uint32_t*>(&m);
     return max_nan(__uint_as_float(b << 16), __uint_as_float(b & 0xffff0000u));
   }
 };
 
-// Adds NV loads' values to a thread's sums.
-template <typename T, int NV>
-__device__ __forceinline__ void take(Sums& a, const uint4 (&u)[NV]) {
-  float m = Vec<T>::largest(u[0]);
-#pragma unroll
-  for (int i = 1; i < NV; ++i) m = max_nan(m, Vec<T>::largest(u[i]));
-  if (m == ninf()) return;
-  if (!(m <= a.m)) {                             // a NaN too
-    Sums r{max_nan(a.m, m), 0.f, 0.f};
-    add_scaled(r, a.m, a.s, a.t);
-    a = r;
-  }
+// Adds the values of NV loads, `apart` from `from` on, to a thread's sums; the
+// largest of them.  The sums stay
+// about a value that the largest may pass by kSlack (e^16 is no strain on
+// float32): they are rescaled a few times a row, not in every call.  A value of
+// -inf makes e^d d, and with it t, a NaN, and values whose c overflows an
+// infinity: then each difference is taken, and lifted, by itself.
+// Eight values cost about 36 instructions and eight exponentials (16 a clock and
+// SM): 46 us for 4096 x 50257, whose bytes take 63.
+constexpr float kSlack = 16.f;
+template <typename T, int NV, bool HELD>
+__device__ __forceinline__ float take(Sums& a, const uint4 (&u)[NV], const uint4* from, int apart) {
+  constexpr int N = Vec<T>::kN;
+  const float m = Vec<T>::template largest<NV>(u);
+  if (m == ninf()) return m;
+  if (!(m <= a.m + kSlack)) about(a, max_nan(a.m, m));   // a NaN too
+  // y = x log2 e - c with c = m log2 e rounded, which the same correction for all values makes good
+  const float c = a.m * kLog2e, over = fmaf(a.m, kLog2e, -c);
+  const uint64_t minus_c = pair_of(-c, -c), log2e = pair_of(kLog2e, kLog2e);
+  uint64_t s = 0, t = 0;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    float v[Vec<T>::kN];
+    float v[N];
     Vec<T>::values(u[i], v);
 #pragma unroll
-    for (int j = 0; j < Vec<T>::kN; ++j) {
-      const float d = max_nan((v[j] - a.m) * kLog2e, -200.f), e = ex2(d);
-      a.s += e;
-      a.t = fmaf(e, d, a.t);
+    for (int j = 0; j < N; j += 2) {
+      const uint64_t y = fma2(pair_of(v[j], v[j + 1]), log2e, minus_c);
+      const float2 yy = of_pair(y);
+      const uint64_t e = pair_of(ex2(yy.x), ex2(yy.y));
+      s = add2(s, e);
+      t = fma2(e, y, t);
     }
   }
+  const float2 ss = of_pair(s), tt = of_pair(t);
+  const float s1 = ss.x + ss.y, t1 = tt.x + tt.y;
+  if (fabsf(t1) < __uint_as_float(0x7f800000u)) {
+    const float f = ex2(-over);
+    a.s = fmaf(s1, f, a.s);
+    a.t = fmaf(fmaf(-over, s1, t1) * f, kLn2, a.t);
+  } else {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      float v[N];
+      Vec<T>::values(HELD ? u[i] : __ldg(from + i * apart), v);   // held, they cost the loop 16 registers
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        const float d = max_nan(v[j] - a.m, -200.f), e = ex2(d * kLog2e);
+        a.s += e;
+        a.t = fmaf(e, d, a.t);
+      }
+    }
+  }
+  return m;
 }
 
 // One row's share: elements [e0, e1), of which whole aligned 16-byte pieces
@@ -170,90 +247,100 @@ struct Share {
   int c0, c1;
 };
 
-// The thread's elements, each once: f(value, index); false ends it.
-template <typename T, typename F>
-__device__ __forceinline__ void each(const Share& s, F f) {
-  constexpr int N = Vec<T>::kN;
+// The thread's elements of `least` or more (all where it is NaN), each once: f(value, index); false ends it.
+template <typename T, int NT, typename F>
+__device__ __forceinline__ void each(const Share& s, float least, F f) {
+  constexpr int N = Vec<T>::kN, kAtOnce = 4;
   const int64_t v0 = s.first + int64_t(s.c0) * N, v1 = s.first + int64_t(s.c1) * N;
   if (int64_t i = s.e0 + threadIdx.x; i < v0 && !f(Vec<T>::one(s.row, i), i)) return;
   if (int64_t i = v1 + threadIdx.x; i < s.e1 && !f(Vec<T>::one(s.row, i), i)) return;
   const uint4* p = reinterpret_cast<const uint4*>(static_cast<const T*>(s.row) + s.first);
-  for (int c = s.c0 + threadIdx.x; c < s.c1; c += kThreads) {
-    float v[N];
-    Vec<T>::values(__ldg(p + c), v);
-    const int64_t i = s.first + int64_t(c) * N;
+#pragma unroll 1
+  for (int c = s.c0 + threadIdx.x; c < s.c1; c += kAtOnce * NT) {
+    uint4 u[kAtOnce];
 #pragma unroll
-    for (int j = 0; j < N; ++j)
-      if (!f(v[j], i + j)) return;
+    for (int q = 0; q < kAtOnce; ++q) u[q] = c + q * NT < s.c1 ? __ldg(p + c + q * NT) : Vec<T>::none();
+#pragma unroll
+    for (int q = 0; q < kAtOnce; ++q) {
+      if (c + q * NT >= s.c1) return;
+      if (Vec<T>::template largest<1>({u[q]}) < least) continue;
+      float v[N];
+      Vec<T>::values(u[q], v);
+      const int64_t i = s.first + int64_t(c + q * NT) * N;
+#pragma unroll
+      for (int j = 0; j < N; ++j)
+        if (!f(v[j], i + j)) return;
+    }
   }
 }
 
+// Kept small: what shared memory takes of an SM is lost to the loads in flight,
+// which land in L1 (4096 x 50257: 78 us with 92 KB an SM, 83 with 175, 97 with
+// all that shared memory may have).
+template <int NT>                      // threads of a row
 struct LpShared {
+  static constexpr int kWarps = NT / 32, kMostOfWarp = kMostTop / kWarps + 2;
+  static constexpr int kRoom = 320;              // collected entries: all of a share that leaves a thread without any
+  static constexpr int kSlots = NT == 256 ? 4 : NT == 128 ? 8 : 16;    // largest values that a thread keeps, of as many stretches of its pieces
+  static constexpr int kList = 256;              // stretches that are read again
   uint64_t list[kMostTop];             // the share's k first, in order
-  Sums sums;
-  uint32_t bound[kWarps];
+  uint32_t bounds[kMostOfWarp * kWarps], bound;
   Sums warp_sums[kWarps];
-  int count, found[kWarps];
+  int count, stretches, found[kWarps];
   uint64_t best[kWarps];
-  uint64_t room[kRoom];
+  float largest[kSlots * NT];
+  uint16_t stretch[kList];
+  __align__(16) uint64_t room[kRoom];
+};
+struct LpParts {                       // of the CTAs of a cluster, in CTA 0
+  __align__(16) uint64_t lists[kMostCtas * kMostTop];
+  uint64_t joined[kMostTop];
+  Sums sums[kMostCtas];
 };
 
-// Places the n entries of `from` that order among the first k into list[0 .. k).
+// Places the n entries of `from` (16-byte aligned) that order among the first k into list[0 .. k).
+template <int NT>
 __device__ __forceinline__ void place(const uint64_t* from, int n, int k, uint64_t* list) {
-  for (int i = threadIdx.x; i < n; i += kThreads) {
+  for (int i = threadIdx.x; i < n; i += NT) {
     const uint64_t e = from[i];
-    int before = 0;
+    int before = 0, j = 0;
 #pragma unroll 4
-    for (int j = 0; j < n; ++j) before += from[j] > e;
+    for (; j + 1 < n; j += 2) {
+      const ulonglong2 o = *reinterpret_cast<const ulonglong2*>(from + j);
+      before += int(o.x > e) + int(o.y > e);
+    }
+    if (j < n) before += from[j] > e;
     if (e && before < k) list[before] = e;
   }
 }
 
-// The share's k first entries to sm.list; largest: of the thread's elements.
-template <typename T>
-__device__ void first_k(LpShared& sm, const Share& s, int k, float largest, bool any) {
+// An entry of key `least` or more to sm.room, while there is room; false once it is full.
+template <int NT>
+__device__ __forceinline__ bool keep(LpShared<NT>& sm, uint32_t least, float v, int64_t i) {
+  const uint32_t key = key_of(v);
+  if (key < least) return true;
+  const int at = atomicAdd(&sm.count, 1);
+  if (at < LpShared<NT>::kRoom) sm.room[at] = entry(key, i);
+  return at < LpShared<NT>::kRoom;
+}
+
+// More entries or stretches reach the bound than there is room for.  Many equal
+// values (a row with fewer than k unmasked ones): those above the bound, then of
+// those at the bound the first, in the order of their indices.
+template <typename T, int NT>
+__device__ __noinline__ void first_k_rare(LpShared<NT>& sm, const Share& s, int k, uint32_t mine, bool any, uint32_t bound) {
+  constexpr int kWarps = NT / 32, kRoom = LpShared<NT>::kRoom;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t mine = any ? key_of(largest) : 0u;
-  // In each warp ceil(k / warps) threads hold a value of its bound or more: k at least of the least of the bounds.
-  uint32_t q = mine, bound = 0;
-  for (int i = 0; i < (k + kWarps - 1) / kWarps; ++i) {
-    bound = __reduce_max_sync(0xffffffffu, q);
-    const uint32_t who = __ballot_sync(0xffffffffu, q == bound);
-    if (lane == __ffs(who) - 1) q = 0;
-  }
-  if (lane == 0) sm.bound[warp] = bound;
-  if (threadIdx.x < kMostTop) sm.list[threadIdx.x] = 0;
-  if (threadIdx.x == 0) sm.count = 0;
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < kWarps; ++w) bound = min(bound, sm.bound[w]);
-  auto collect = [&](uint32_t least) {           // entries of this key or more, up to the room
-    if (any && mine >= least)
-      each<T>(s, [&](float v, int64_t i) {
-        const uint32_t key = key_of(v);
-        if (key < least) return true;
-        const int at = atomicAdd(&sm.count, 1);
-        if (at < kRoom) sm.room[at] = entry(key, i);
-        return at < kRoom;
-      });
-    __syncthreads();
-    return sm.count;
-  };
-  int n = collect(bound);
-  if (n <= kRoom) {
-    place(sm.room, n, k, sm.list);
-    __syncthreads();
-    return;
-  }
-  // Many equal values (a row with fewer than k unmasked ones): those above the bound, then of those at the bound the
-  // first, in the order of their indices.
   __syncthreads();
   if (threadIdx.x == 0) sm.count = 0;
   __syncthreads();
-  n = bound == 0xffffffffu ? 0 : collect(bound + 1);
+  if (bound != 0xffffffffu && any && mine > bound)
+    each<T, NT>(s, value_of(bound), [&](float v, int64_t i) { return keep<NT>(sm, bound + 1, v, i); });
+  __syncthreads();
+  int n = sm.count;
   if (n <= kRoom) {
-    place(sm.room, n, k, sm.list);
-    for (int64_t base = s.e0; n < k && base < s.e1; base += kThreads) {
+    place<NT>(sm.room, n, k, sm.list);
+    for (int64_t base = s.e0; n < k && base < s.e1; base += NT) {
       const int64_t i = base + threadIdx.x;
       const bool hit = i < s.e1 && key_of(Vec<T>::one(s.row, i)) == bound;
       const uint32_t who = __ballot_sync(0xffffffffu, hit);
@@ -274,7 +361,7 @@ __device__ void first_k(LpShared& sm, const Share& s, int k, float largest, bool
   uint64_t last = ~0ull;
   for (int r = 0; r < k; ++r) {
     uint64_t best = 0;
-    each<T>(s, [&](float v, int64_t i) {
+    each<T, NT>(s, __uint_as_float(0x7fc00000u), [&](float v, int64_t i) {
       const uint64_t e = entry(key_of(v), i);
       if (e < last && e > best) best = e;
       return true;
@@ -293,112 +380,212 @@ __device__ void first_k(LpShared& sm, const Share& s, int k, float largest, bool
   __syncthreads();
 }
 
-// One cluster of CTAs a row (one CTA where there are many rows); CTA 0 joins
-// the parts.
-template <typename T>
-__global__ void __launch_bounds__(kThreads) logprobs_kernel(LpParams p, int ctas) {
-  constexpr int N = Vec<T>::kN, kAtOnce = 4;
-  __shared__ LpShared sm;
-  const int64_t row = blockIdx.x / ctas;
-  const int rank = blockIdx.x % ctas, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+// The share's k first entries to sm.list; largest: of the thread's elements, sm.largest: of its stretches of 2^log_stretch
+// pieces each.
+template <typename T, int NT>
+__device__ __forceinline__ void first_k(LpShared<NT>& sm, const Share& s, int k, float largest, bool any, int slots, int log_stretch) {
+  constexpr int N = Vec<T>::kN, kWarps = NT / 32, kRoom = LpShared<NT>::kRoom, kList = LpShared<NT>::kList;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t mine = any ? key_of(largest) : 0u;
+  // The k-th of some threads' largest values is a bound: those of each warp's first few threads, at least k in all.
+  const int each_warp = min(k, (k + kWarps - 1) / kWarps + 2), some = each_warp * kWarps;
+  uint32_t q = mine, bound = 0;
+  for (int i = 0; i < each_warp; ++i) {
+    bound = __reduce_max_sync(0xffffffffu, q);
+    const uint32_t who = __ballot_sync(0xffffffffu, q == bound);
+    if (lane == __ffs(who) - 1) {
+      q = 0;
+      if (kWarps > 1) sm.bounds[warp * each_warp + i] = bound;
+    }
+  }
+  if (threadIdx.x < kMostTop) sm.list[threadIdx.x] = 0;
+  if (threadIdx.x == 0) sm.count = sm.stretches = 0;
+  __syncthreads();
+  if constexpr (kWarps > 1) {
+    if (int(threadIdx.x) < some) {
+      const uint32_t v = sm.bounds[threadIdx.x];
+      int before = 0;
+#pragma unroll 4
+      for (int i = 0; i < some; i += kWarps) {
+#pragma unroll
+        for (int j = 0; j < kWarps; ++j) before += sm.bounds[i + j] > v || (sm.bounds[i + j] == v && i + j < int(threadIdx.x));
+      }
+      if (before == k - 1) sm.bound = v;
+    }
+    __syncthreads();
+    bound = sm.bound;
+  }
+  // What reaches the bound lies in a few stretches, which all threads read again together.
+  const float low = value_of(bound);             // NaN where nothing is below
+  if (any && mine >= bound) {
+    for (int i = 0; i < slots; ++i)
+      if (!(sm.largest[i * NT + threadIdx.x] < low)) {
+        const int at = atomicAdd(&sm.stretches, 1);
+        if (at < kList) sm.stretch[at] = uint16_t(i * NT + threadIdx.x);
+      }
+    if (threadIdx.x < N) {                       // the ends
+      const int64_t i = s.e0 + threadIdx.x, j = s.first + int64_t(s.c1) * N + threadIdx.x;
+      if (i < s.first + int64_t(s.c0) * N) keep<NT>(sm, bound, Vec<T>::one(s.row, i), i);
+      if (j < s.e1) keep<NT>(sm, bound, Vec<T>::one(s.row, j), j);
+    }
+  }
+  __syncthreads();
+  const int stretches = sm.stretches;
+  const uint4* p = reinterpret_cast<const uint4*>(static_cast<const T*>(s.row) + s.first);
+  for (int t = threadIdx.x; t < min(stretches, kList) << log_stretch; t += NT) {
+    const int of = sm.stretch[t >> log_stretch];
+    const int c = s.c0 + of % NT + ((of / NT << log_stretch) + (t & ((1 << log_stretch) - 1))) * NT;
+    if (c >= s.c1) continue;
+    const uint4 u = __ldg(p + c);
+    if (Vec<T>::template largest<1>({u}) < low) continue;
+    if (*static_cast<volatile int*>(&sm.count) > kRoom) break;
+    float v[N];
+    Vec<T>::values(u, v);
+    uint32_t hits = 0;
+#pragma unroll
+    for (int j = 0; j < N; ++j) hits |= uint32_t(!(v[j] < low)) << j;
+    for (; hits; hits &= hits - 1) {
+      const int j = __ffs(hits) - 1;
+      float x = v[0];
+#pragma unroll
+      for (int q = 1; q < N; ++q) x = j == q ? v[q] : x;
+      keep<NT>(sm, bound, x, s.first + int64_t(c) * N + j);
+    }
+  }
+  __syncthreads();
+  const int n = sm.count;
+  if (n <= kRoom && stretches <= kList) {
+    place<NT>(sm.room, n, k, sm.list);
+    __syncthreads();
+    return;
+  }
+  first_k_rare<T, NT>(sm, s, k, mine, any, bound);
+}
+
+template <typename T, bool CLUSTER>
+__device__ __forceinline__ Share share_of(const LpParams& p, int64_t row, int rank, int log_ctas) {
   Share s;
   s.row = static_cast<const T*>(p.x) + row * p.ld;
   const int64_t off = (16 - (reinterpret_cast<uintptr_t>(s.row) & 15)) & 15;
   s.first = min(int64_t(off / sizeof(T)), int64_t(p.V));
-  const int pieces = int((p.V - s.first) / N);
-  s.c0 = int(int64_t(pieces) * rank / ctas), s.c1 = int(int64_t(pieces) * (rank + 1) / ctas);
-  s.e0 = rank == 0 ? 0 : s.first + int64_t(s.c0) * N;
-  s.e1 = rank == ctas - 1 ? p.V : s.first + int64_t(s.c1) * N;
+  const int pieces = int((p.V - s.first) / Vec<T>::kN);
+  s.c0 = 0, s.c1 = pieces, s.e0 = 0, s.e1 = p.V;
+  if (CLUSTER) {
+    s.c0 = int(int64_t(pieces) * rank >> log_ctas), s.c1 = int(int64_t(pieces) * (rank + 1) >> log_ctas);
+    if (rank) s.e0 = s.first + int64_t(s.c0) * Vec<T>::kN;
+    if (rank + 1 != 1 << log_ctas) s.e1 = s.first + int64_t(s.c1) * Vec<T>::kN;
+  }
+  return s;
+}
 
+// NT threads a row, or a cluster of CTAs of 256 where there are few rows: CTA 0
+// then joins the parts, which the others write into its shared memory.
+constexpr int kAtOnce = 4;             // loads of a thread in flight
+
+template <typename T, int NT, bool CLUSTER>
+__global__ void __launch_bounds__(NT, CLUSTER ? 4 : NT == 32 ? 32 : 1536 / NT) logprobs_kernel(LpParams p, int log_ctas) {
+  constexpr int N = Vec<T>::kN, kWarps = NT / 32;
+  __shared__ LpShared<NT> sm;
+  const int ctas = CLUSTER ? 1 << log_ctas : 1, rank = CLUSTER ? blockIdx.x & (ctas - 1) : 0;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t row = CLUSTER ? blockIdx.x >> log_ctas : blockIdx.x;
+  if (CLUSTER) sm100::cluster_arrive();         // CTA 0's shared memory may be written once it runs
+  const Share s = share_of<T, CLUSTER>(p, row, rank, log_ctas);
   float token_x = __uint_as_float(0x7fc00000u);  // a token outside the vocabulary has no probability
   if (rank == 0 && threadIdx.x == 0) {
     const int64_t tok = p.tok64 ? __ldg(static_cast<const int64_t*>(p.tokens) + row) : __ldg(static_cast<const int32_t*>(p.tokens) + row);
     if (tok >= 0 && tok < p.V) token_x = Vec<T>::one(s.row, tok);
   }
+  // the ends, fewer than N elements each
+  float v0 = ninf(), v1 = ninf();
+  if (const int64_t i = s.e0 + threadIdx.x; i < s.first + int64_t(s.c0) * N) v0 = Vec<T>::one(s.row, i);
+  if (const int64_t i = s.first + int64_t(s.c1) * N + threadIdx.x; i < s.e1) v1 = Vec<T>::one(s.row, i);
 
   Sums a{ninf(), 0.f, 0.f};
-  const uint4* pieces_p = reinterpret_cast<const uint4*>(static_cast<const T*>(s.row) + s.first);
-  int c = s.c0 + threadIdx.x;
-  for (; c + (kAtOnce - 1) * kThreads < s.c1; c += kAtOnce * kThreads) {
+  const uint4* pieces = reinterpret_cast<const uint4*>(static_cast<const T*>(s.row) + s.first);
+  // stretches of 2^log_stretch pieces a thread, at most kSlots of them
+  const int groups = ((s.c1 - s.c0 + NT - 1) / NT + kAtOnce - 1) / kAtOnce;
+  int log_groups = 0;
+  while (groups > LpShared<NT>::kSlots << log_groups) ++log_groups;
+  const int log_stretch = log_groups + 2, slots = (groups + (1 << log_groups) - 1) >> log_groups;
+  static_assert(kAtOnce == 4, "log_stretch");
+  int c = s.c0 + threadIdx.x, group = 0;
+  float most = ninf(), largest = ninf();         // of the stretch, of all
+#pragma unroll 1
+  for (; c + (kAtOnce - 1) * NT < s.c1; c += kAtOnce * NT) {
     uint4 u[kAtOnce];
 #pragma unroll
-    for (int i = 0; i < kAtOnce; ++i) u[i] = __ldg(pieces_p + c + i * kThreads);
-    take<T, kAtOnce>(a, u);
+    for (int i = 0; i < kAtOnce; ++i) u[i] = load_once(pieces + c + i * NT);
+    most = max_nan(most, take<T, kAtOnce, CLUSTER>(a, u, pieces + c, NT));
+    if ((++group & ((1 << log_groups) - 1)) == 0) {
+      sm.largest[((group - 1) >> log_groups) * NT + threadIdx.x] = most;
+      largest = max_nan(largest, most);
+      most = ninf();
+    }
   }
   {
-    uint4 u[kAtOnce - 1];
+    uint4 u[kAtOnce - 1][1];
 #pragma unroll
-    for (int i = 0; i < kAtOnce - 1; ++i) u[i] = c + i * kThreads < s.c1 ? __ldg(pieces_p + c + i * kThreads) : Vec<T>::none();
-    // the ends, fewer than N elements each
-    float v0 = ninf(), v1 = ninf();
-    if (const int64_t i = s.e0 + threadIdx.x; i < s.first + int64_t(s.c0) * N) v0 = Vec<T>::one(s.row, i);
-    if (const int64_t i = s.first + int64_t(s.c1) * N + threadIdx.x; i < s.e1) v1 = Vec<T>::one(s.row, i);
-    take<T, kAtOnce - 1>(a, u);
-    if (threadIdx.x < N) a = join(a, join(Sums{v0, 1.f, 0.f}, Sums{v1, 1.f, 0.f}));
+    for (int i = 0; i < kAtOnce - 1; ++i) u[i][0] = c + i * NT < s.c1 ? load_once(pieces + c + i * NT) : Vec<T>::none();
+#pragma unroll
+    for (int i = 0; i < kAtOnce - 1; ++i)
+      if (c + i * NT < s.c1) most = max_nan(most, take<T, 1, CLUSTER>(a, u[i], pieces + c + i * NT, 0));
+    if (group >> log_groups < slots) sm.largest[(group >> log_groups) * NT + threadIdx.x] = most;
+    largest = max_nan(largest, most);
   }
-  const float largest = a.m;
-
-  auto warp_join = [](Sums v) {
+  if (threadIdx.x < N) {
 #pragma unroll
-    for (int o = 16; o; o >>= 1)
-      v = join(v, Sums{__shfl_xor_sync(0xffffffffu, v.m, o), __shfl_xor_sync(0xffffffffu, v.s, o),
-                       __shfl_xor_sync(0xffffffffu, v.t, o)});
-    return v;
-  };
-  a = warp_join(a);
+    for (int i = 0; i < 2; ++i) {
+      const float x = i ? v1 : v0;
+      if (x == ninf()) continue;
+      about(a, max_nan(a.m, x));
+      largest = max_nan(largest, x);
+      const float d = max_nan(x - a.m, -200.f), e = ex2(d * kLog2e);
+      a.s += e;
+      a.t = fmaf(e, d, a.t);
+    }
+  }
+  a = join<32>(a, largest);
   if (lane == 0) sm.warp_sums[warp] = a;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    Sums r = sm.warp_sums[0];
-    for (int w = 1; w < kWarps; ++w) r = join(r, sm.warp_sums[w]);
-    sm.sums = r;
-  }
   if (p.top) {
     // has this thread any element?
     const bool any = s.c0 + int(threadIdx.x) < s.c1 || s.e0 + threadIdx.x < s.first + int64_t(s.c0) * N ||
                      s.first + int64_t(s.c1) * N + threadIdx.x < s.e1;
-    first_k<T>(sm, s, p.top, largest, any);
+    first_k<T, NT>(sm, s, p.top, largest, any, slots, log_stretch);
   } else {
     __syncthreads();
   }
-
-  Sums all = sm.sums;
-  uint64_t* list = sm.list;
-  if (ctas > 1) {
+  if (!CLUSTER && warp) return;                  // one warp has lanes for all results
+  Sums all = join<kWarps>(sm.warp_sums[lane % kWarps], sm.warp_sums[lane % kWarps].m);
+  const uint64_t* list = sm.list;
+  if constexpr (CLUSTER) {
+    __shared__ LpParts parts;
     __syncwarp();
-    sm100::cluster_sync();
-    if (rank == 0) {
-      auto remote32 = [](const void* q, int r) {
-        uint32_t v;
-        asm volatile("ld.shared::cluster.u32 %0, [%1];\n" : "=r"(v) : "r"(sm100::mapa_shared(q, r)) : "memory");
-        return v;
-      };
-      for (int r = 1; r < ctas; ++r)
-        all = join(all, Sums{__uint_as_float(remote32(&sm.sums.m, r)), __uint_as_float(remote32(&sm.sums.s, r)),
-                             __uint_as_float(remote32(&sm.sums.t, r))});
-      if (p.top) {
-        // every share's list, then the first of all of them behind it
-        const int n = ctas * p.top;
-        for (int i = threadIdx.x; i < n; i += kThreads) {
-          const uint64_t* q = &sm.list[i % p.top];
-          uint64_t v;
-          asm volatile("ld.shared::cluster.u64 %0, [%1];\n" : "=l"(v) : "r"(sm100::mapa_shared(q, i / p.top)) : "memory");
-          sm.room[i] = v;
-        }
-        list = sm.room + kMostCtas * kMostTop;
-        __syncthreads();
-        place(sm.room, n, p.top, list);
-        __syncthreads();
+    sm100::cluster_wait();
+    if (warp == 0) {
+      if (lane < 3) {
+        const float v = lane == 0 ? all.m : lane == 1 ? all.s : all.t;
+        asm volatile("st.shared::cluster.f32 [%0], %1;\n" ::"r"(sm100::mapa_shared(&parts.sums[rank].m + lane, 0)), "f"(v) : "memory");
       }
+    } else if (warp == 1 && lane < p.top) {
+      asm volatile("st.shared::cluster.u64 [%0], %1;\n" ::"r"(sm100::mapa_shared(&parts.lists[rank * p.top + lane], 0)), "l"(sm.list[lane])
+                   : "memory");
     }
     __syncwarp();
-    sm100::cluster_sync();                       // no CTA leaves while CTA 0 reads its shared memory
+    sm100::cluster_sync();
     if (rank != 0) return;
+    all = lane % kMostCtas < ctas ? parts.sums[lane % kMostCtas] : Sums{ninf(), 0.f, 0.f};
+    all = join<kMostCtas>(all, all.m);
+    if (p.top) {
+      place<NT>(parts.lists, ctas * p.top, p.top, parts.joined);
+      list = parts.joined;
+      __syncthreads();
+    }
   }
   const float log_s = logf(all.s);
   if (threadIdx.x == 0) {
     p.lp[row] = (token_x - all.m) - log_s;
-    p.entropy[row] = log_s - kLn2 * (all.t / all.s);
+    p.entropy[row] = log_s - all.t / all.s;
   }
   if (int(threadIdx.x) < p.top) {
     const uint64_t e = list[threadIdx.x];
@@ -407,27 +594,42 @@ __global__ void __launch_bounds__(kThreads) logprobs_kernel(LpParams p, int ctas
   }
 }
 
-template <typename T>
-int launch_logprobs(const LpParams& p, cudaStream_t st) {
-  int dev = 0, sms = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
-    return TAC_E_CUDA;
-  // CTAs a row: up to eight while all find a place at once, with two loads a thread or more
-  int ctas = 1;
-  while (ctas < kMostCtas && int64_t(p.M) * ctas * 2 <= 4 * sms && p.V >= 2 * ctas * 2 * kThreads * Vec<T>::kN) ctas *= 2;
-  if (int64_t(p.M) * ctas > 0x7fffffff) return TAC_E_ARGUMENT;
+template <typename T, int NT, bool CLUSTER>
+int launch_rows(const LpParams& p, int log_ctas, cudaStream_t st) {
+  if ((int64_t(p.M) << log_ctas) > 0x7fffffff) return TAC_E_ARGUMENT;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(unsigned(p.M) * ctas);
-  cfg.blockDim = dim3(kThreads);
+  cfg.gridDim = dim3(unsigned(p.M) << log_ctas);
+  cfg.blockDim = dim3(NT);
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = ctas;
+  attr[0].val.clusterDim.x = 1u << log_ctas;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = ctas > 1;
-  return status(cudaLaunchKernelEx(&cfg, logprobs_kernel<T>, p, ctas));
+  cfg.numAttrs = CLUSTER;
+  return status(cudaLaunchKernelEx(&cfg, logprobs_kernel<T, NT, CLUSTER>, p, log_ctas));
+}
+
+template <typename T>
+int launch_logprobs(const LpParams& p, cudaStream_t st) {
+  static int sms_of[64] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return TAC_E_CUDA;
+  if (!sms_of[dev]) {
+    if (int e = status(cudaDeviceGetAttribute(&sms_of[dev], cudaDevAttrMultiProcessorCount, dev))) return e;
+  }
+  // CTAs a row: up to eight while all find a place at once, with two loads a thread or more
+  const int sms = sms_of[dev], pieces = p.V / Vec<T>::kN;
+  int log_ctas = 0;
+  while (2 << log_ctas <= kMostCtas && (int64_t(p.M) << (log_ctas + 1)) <= 4 * sms && pieces >> (log_ctas + 1) >= 2 * 256) ++log_ctas;
+  if (log_ctas) return launch_rows<T, 256, true>(p, log_ctas, st);
+  // A warp a row, which needs no barrier, for short rows: those of two groups of loads, and where there are rows for many
+  // warps an SM those of twelve.  Against four warps a row, microseconds with five tokens picked, 16-bit logits:
+  //   1000 x 1000  5.4 / 5.6   20000 x 1000  28 / 57   1000 x 8000  10.8 / 8.9   4000 x 12000  23 / 28
+  //   20000 x 12000  106 / 114   4000 x 32000  54 / 56   20000 x 32000  255 / 216   4096 x 50257  91 / 78
+  if (pieces <= 32 * 2 * kAtOnce || (pieces <= 32 * 12 * kAtOnce && p.M >= 8 * sms)) return launch_rows<T, 32, false>(p, 0, st);
+  return launch_rows<T, 128, false>(p, 0, st);
 }
 
 }  // namespace
