@@ -54,64 +54,6 @@ int64_t scale_bytes(int64_t rows, int64_t K) { return (rows + 127) / 128 * mx_pi
 // 127)) to the nearest, ties to the even code, magnitudes at most 6; a block
 // with an infinity or a NaN gets the byte 255 (NaN) and codes 0.  Powers of two
 // divide exactly, so nothing here rounds but the code itself.
-template <typename T>
-__device__ __forceinline__ float to_f(T v);
-template <>
-__device__ __forceinline__ float to_f(float v) { return v; }
-template <>
-__device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
-template <>
-__device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
-
-template <typename T>
-__device__ __forceinline__ void load8(const T* x, int k, int K, bool vec, float (&v)[8]) {
-  if (vec && k + 8 <= K) {
-    constexpr int kPer = 16 / sizeof(T);
-#pragma unroll
-    for (int i = 0; i < 8; i += kPer) {
-      union {
-        uint4 u;
-        T t[kPer];
-      } a;
-      a.u = __ldg(reinterpret_cast<const uint4*>(x + k + i));
-#pragma unroll
-      for (int j = 0; j < kPer; ++j) v[i + j] = to_f(a.t[j]);
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = k + j < K ? to_f(x[k + j]) : 0.f;
-  }
-}
-
-// Largest magnitude of a block whose four lanes hold eight values each, as bits: infinities and NaN order above all others.
-__device__ __forceinline__ uint32_t block_max(const float (&v)[8]) {
-  uint32_t m = 0;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(v[j]) & 0x7fffffffu);
-  m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
-  return max(m, __shfl_xor_sync(0xffffffffu, m, 2));
-}
-__device__ __forceinline__ uint32_t scale_byte(uint32_t max_bits) {
-  const uint32_t e = max_bits >> 23;
-  return e == 255 ? 255u : e > 2 ? e - 2 : 0u;
-}
-// Eight codes, value 0 in the lowest four bits.
-__device__ __forceinline__ uint32_t codes8(const float (&v)[8], uint32_t byte) {
-  if (byte == 255) return 0u;
-  const float inv = __uint_as_float((254u - byte) << 23);
-  uint32_t r;
-  asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
-      "cvt.rn.satfinite.e2m1x2.f32 b0, %2, %1;\n\t"
-      "cvt.rn.satfinite.e2m1x2.f32 b1, %4, %3;\n\t"
-      "cvt.rn.satfinite.e2m1x2.f32 b2, %6, %5;\n\t"
-      "cvt.rn.satfinite.e2m1x2.f32 b3, %8, %7;\n\t"
-      "mov.b32 %0, {b0, b1, b2, b3};\n\t}\n"
-      : "=r"(r)
-      : "f"(v[0] * inv), "f"(v[1] * inv), "f"(v[2] * inv), "f"(v[3] * inv), "f"(v[4] * inv), "f"(v[5] * inv), "f"(v[6] * inv),
-        "f"(v[7] * inv));
-  return r;
-}
-
 // A warp takes 256 columns of the four rows whose scales share 16 bytes (lane +
 // 0, 32, 64, 96 of 128): a lane eight values of each, four lanes a block.
 constexpr int kQmThreads = 256;
@@ -127,20 +69,20 @@ __global__ void __launch_bounds__(kQmThreads) mx_quant_kernel(const T* __restric
   const int64_t tile = task / k_stages / 32;
   const int k = chunk * kMxStageK + lane * 8;
   const int64_t ldc = int64_t((K + 31) / 32) * 16;
-  float v[4][8];
+  MxHeld<T> held[4];
 #pragma unroll
   for (int g = 0; g < 4; ++g) {
     const int64_t m = tile * 128 + g * 32 + r;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[g][j] = 0.f;
-    if (m < M) load8(X + m * ldx, k, K, vec, v[g]);
+    if (m < M) held[g].load(X + m * ldx, k, K, vec);
   }
   uint32_t word[4];
 #pragma unroll
   for (int g = 0; g < 4; ++g) {
     const int64_t m = tile * 128 + g * 32 + r;
-    const uint32_t byte = scale_byte(block_max(v[g]));
-    const uint32_t c = codes8(v[g], byte);
+    float v[8] = {};
+    if (m < M) held[g].values(v);
+    const uint32_t byte = scale_byte(block_max(v));
+    const uint32_t c = codes8(v, byte);
     if (m < M && k / 2 < ldc) *reinterpret_cast<uint32_t*>(codes + m * ldc + k / 2) = c;
     // the bytes of a lane's four blocks, lanes 0 and 16 of each half
     uint32_t b = byte << (8 * ((lane >> 2) & 3));
@@ -251,7 +193,7 @@ int launch_splitk(const MxOperands& o, MxParams p, cudaStream_t st) {
   const int per = (p.k_stages + split - 1) / split, sb = mx_sk_stage_bytes(p.tn);
   // in flight: 96 KB where two CTAs share an SM, else twice that
   p.stages = std::min(std::min(per, kMxSkStages), std::max(2, (tiles * split > sms ? 96 : 190) * 1024 / sb));
-  const int part = split > 1 ? mx_sk_part_bytes(p.tn) : 0;
+  const int part = split > 1 ? std::max(mx_sk_part_bytes(p.tn), mx_sk_least_smem(mx_sk_cols(p.tn, p.stages))) : 0;
   CUtensorMap tw, ta;
   if (!map_rows(&tw, o.b_codes, o.K, p.N, 128) || !map_rows(&ta, o.a_codes, o.K, p.M, p.tn)) return TAC_E_CUDA;
   cudaLaunchConfig_t cfg = {};
@@ -274,6 +216,89 @@ int launch_splitk(const MxOperands& o, MxParams p, cudaStream_t st) {
   return status(cudaLaunchKernelEx(&cfg, mx_splitk_kernel<YT>, tw, ta, p));
 }
 
+// Scales of rows as 32-bit words: a box is a stage of `pieces` times 128 rows; rows past the last read as 0.
+bool map_scales(CUtensorMap* m, const uint8_t* base, int k_stages, int rows, int pieces) {
+  const cuuint64_t dims[2] = {cuuint64_t(k_stages) * (kMxSfBytes / 4), cuuint64_t((rows + 127) / 128)};
+  const cuuint64_t strides[1] = {cuuint64_t(k_stages) * kMxSfBytes};
+  const cuuint32_t box[2] = {kMxSfBytes / 4, cuuint32_t(pieces)};
+  return tmap_encode(m, CU_TENSOR_MAP_DATA_TYPE_UINT32, base, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_NONE);
+}
+
+// Tokens of a pair tile: the number that leaves the least work on the fullest
+// pair.  A stage costs, in nanoseconds: what its operands take from L2, 80 bytes
+// a nanosecond and SM, and a little more.
+int pair_tokens(int M, int N, int clusters) {
+  constexpr int kStageCost[4] = {273, 315, 436, 499};      // 64, 128, 192, 256 tokens (4096^3)
+  const int64_t wt = (N + 255) / 256;
+  int best = 0;
+  int64_t cost = 0;
+  for (int tn = 256; tn >= 64; tn -= 64) {
+    const int64_t tiles = wt * ((M + tn - 1) / tn), c = (tiles + clusters - 1) / clusters * kStageCost[tn / 64 - 1];
+    if (!best || c < cost) best = tn, cost = c;
+  }
+  return best;
+}
+
+// Largest number of CTA pairs that run at once; 0 where none does.
+template <int YT>
+int pair_clusters(int dev) {
+  static int clusters[64];
+  static bool done[64] = {};
+  if (!done[dev]) {
+    int n = 0;
+    const int sms = sm_count();
+    if (cudaFuncSetAttribute(mx_pair_kernel<YT>, cudaFuncAttributeMaxDynamicSharedMemorySize, MxPairCfg::kSmem) == cudaSuccess) {
+      cudaLaunchConfig_t cfg = {};
+      cfg.gridDim = dim3(2 * (sms / 2));
+      cfg.blockDim = dim3(MxPairCfg::kThreads);
+      cfg.dynamicSmemBytes = MxPairCfg::kSmem;
+      if (cudaOccupancyMaxActiveClusters(&n, mx_pair_kernel<YT>, &cfg) != cudaSuccess) n = 0;
+    }
+    cudaGetLastError();
+    clusters[dev] = std::min(n, sms / 2);
+    done[dev] = true;
+  }
+  return clusters[dev];
+}
+
+template <int YT>
+int launch_pair(const MxOperands& o, MxParams p, int clusters, int tn, cudaStream_t st) {
+  MxPairParams pp{};
+  p.tn = tn;
+  pp.g = p;
+  pp.w_tiles = (p.N + 255) / 256;
+  pp.t_tiles = (p.M + tn - 1) / tn;
+  CUtensorMap tw, ta, tws, tas;
+  if (!map_rows(&tw, o.b_codes, o.K, p.N, 128) || !map_rows(&ta, o.a_codes, o.K, p.M, tn / 2) ||
+      !map_scales(&tws, p.b_scale, p.k_stages, p.N, 1) || !map_scales(&tas, p.a_scale, p.k_stages, p.M, tn > 128 ? 2 : 1))
+    return TAC_E_CUDA;
+  const int64_t tiles = int64_t(pp.w_tiles) * pp.t_tiles;
+  if (tiles > (1 << 30)) return TAC_E_ARGUMENT;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(2 * int(std::min<int64_t>(tiles, clusters)));
+  cfg.blockDim = dim3(MxPairCfg::kThreads);
+  cfg.dynamicSmemBytes = MxPairCfg::kSmem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = p.after_rows ? 1 : 0;
+  return status(cudaLaunchKernelEx(&cfg, mx_pair_kernel<YT>, tw, ta, tws, tas, pp));
+}
+
+template <int YT>
+int pick_product(const MxOperands& o, const MxParams& p, cudaStream_t st) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return TAC_E_CUDA;
+  const int clusters = pair_clusters<YT>(dev);
+  if (p.M > 128 && clusters > 0) {
+    const int tn = pair_tokens(p.M, p.N, clusters);
+    if (int64_t((p.N + 255) / 256) * ((p.M + tn - 1) / tn) * 2 >= clusters) return launch_pair<YT>(o, p, clusters, tn, st);
+  }
+  return launch_splitk<YT>(o, p, st);
+}
+
 // Checks that both products share; also the limits of the grids.
 int check_product(const void* b_codes, const void* b_scales, const void* bias, int bias_type, const void* Y, int y_type, int M, int N,
                   int K) {
@@ -294,7 +319,67 @@ int run_product(const uint8_t* a_codes, const uint8_t* a_scales, const uint8_t* 
   p.after_rows = after_rows;
   if (!(p.fault = fault_word())) return TAC_E_CUDA;
   const MxOperands o{a_codes, b_codes, K};
-  return y_type == TAC_F32 ? launch_splitk<0>(o, p, st) : y_type == TAC_F16 ? launch_splitk<1>(o, p, st) : launch_splitk<2>(o, p, st);
+  return y_type == TAC_F32 ? pick_product<0>(o, p, st) : y_type == TAC_F16 ? pick_product<1>(o, p, st) : pick_product<2>(o, p, st);
+}
+
+// ---- few rows -------------------------------------------------------------------------------------------------------
+struct MxRowsShape {
+  int tn, split, per;        // tokens of the tile, CTAs that share a tile's stages, stages of a CTA at most
+  int64_t tiles;
+};
+MxRowsShape rows_shape(int M, int N, int K, int sms) {
+  MxRowsShape r;
+  r.tn = M <= 16 ? 16 : M <= 32 ? 32 : 64;
+  r.tiles = (int64_t(N) + 127) / 128;
+  const int k_stages = int(mx_pieces(K) / 2);
+  r.split = splits(r.tiles, k_stages, r.tn, sms);
+  r.per = (k_stages + r.split - 1) / r.split;
+  return r;
+}
+
+// One launch where a CTA's values are all in flight at once and there is a CTA for each SM at most.
+bool one_launch(int M, int N, int K, int sms) {
+  if (M > kMxRowsMost || !sms) return false;
+  const MxRowsShape r = rows_shape(M, N, K, sms);
+  return r.tiles <= sms && int64_t(r.per) * M * 32 <= 256 * kMxRowsHeld;
+}
+
+template <typename T, int YT>
+int launch_rows_as(MxRowsParams pp, const MxOperands& o, cudaStream_t st) {
+  static bool smem_set[64] = {};
+  int dev = 0;
+  const int sms = sm_count();
+  if (!sms || cudaGetDevice(&dev) != cudaSuccess) return TAC_E_CUDA;
+  if (!smem_set[dev]) {
+    if (int e = status(cudaFuncSetAttribute(mx_rows_kernel<T, YT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMxMaxSmem))) return e;
+    smem_set[dev] = true;
+  }
+  MxParams& p = pp.g;
+  const MxRowsShape r = rows_shape(p.M, p.N, o.K, sms);
+  p.tn = r.tn;
+  const int rows = r.per * mx_rows_bytes(r.tn), sb = kMxWBytes + kMxSfBytes;
+  p.stages = std::min({r.per, kMxSkStages, (kMxMaxSmem - 1024 - rows) / sb});     // the rows are 192 KB at most, of one token
+  const int part = r.split > 1 ? std::max(mx_sk_part_bytes(r.tn), mx_sk_least_smem(mx_sk_cols(r.tn, p.stages))) : 0;
+  CUtensorMap tw;
+  if (!map_rows(&tw, o.b_codes, o.K, p.N, 128)) return TAC_E_CUDA;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(unsigned(r.tiles), 1, r.split);
+  cfg.blockDim = dim3(kMxRowsThreads);
+  cfg.dynamicSmemBytes = std::max(p.stages * sb + rows, part) + 1024;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 1;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = r.split;
+  cfg.attrs = attr;
+  cfg.numAttrs = r.split > 1;
+  return status(cudaLaunchKernelEx(&cfg, mx_rows_kernel<T, YT>, tw, pp));
+}
+
+template <typename T>
+int launch_rows(const MxRowsParams& pp, const MxOperands& o, int y_type, cudaStream_t st) {
+  return y_type == TAC_F32 ? launch_rows_as<T, 0>(pp, o, st) : y_type == TAC_F16 ? launch_rows_as<T, 1>(pp, o, st) : launch_rows_as<T, 2>(pp, o, st);
 }
 
 uint64_t align256(uint64_t v) { return (v + 255) & ~uint64_t(255); }
@@ -336,7 +421,7 @@ extern "C" int tac_mxfp4_gemm(const uint8_t* a_codes, const uint8_t* a_scales, c
 }
 
 extern "C" uint64_t tac_linear_mxfp4_workspace_bytes(int M, int N, int K) {
-  if (M <= 0 || N <= 0 || K <= 0) return 0;
+  if (M <= 0 || N <= 0 || K <= 0 || one_launch(M, N, K, sm_count())) return 0;
   return align256(code_bytes(M, K)) + align256(scale_bytes(M, K));
 }
 
@@ -346,6 +431,21 @@ extern "C" int tac_linear_mxfp4(const void* X, int x_type, int64_t ldx, const ui
   if (!X || !type_ok(x_type) || (M > 1 && ldx < K) || !aligned(X, elem(x_type))) return TAC_E_ARGUMENT;
   if (int s = check_product(b_codes, b_scales, bias, bias_type, Y, y_type, M, N, K)) return s;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (one_launch(M, N, K, sm_count())) {
+    MxRowsParams pp{};
+    pp.g.b_scale = b_scales;
+    pp.g.bias = bias, pp.g.bias_type = bias_type;
+    pp.g.y = Y;
+    pp.g.M = M, pp.g.N = N;
+    pp.g.k_stages = int(mx_pieces(K) / 2);
+    if (!(pp.g.fault = fault_word())) return TAC_E_CUDA;
+    pp.x = X, pp.x_type = x_type, pp.ldx = ldx, pp.K = K;
+    pp.x_vec = aligned(X, 16) && (M == 1 || (ldx * elem(x_type)) % 16 == 0);
+    const MxOperands o{nullptr, b_codes, K};
+    return x_type == TAC_F32   ? launch_rows<float>(pp, o, y_type, st)
+           : x_type == TAC_F16 ? launch_rows<__half>(pp, o, y_type, st)
+                               : launch_rows<__nv_bfloat16>(pp, o, y_type, st);
+  }
   if (!workspace || !aligned(workspace, 256) || workspace_bytes < tac_linear_mxfp4_workspace_bytes(M, N, K)) return TAC_E_ARGUMENT;
   uint8_t* codes = static_cast<uint8_t*>(workspace);
   uint8_t* scales = codes + align256(code_bytes(M, K));

@@ -22,16 +22,20 @@ inline PFN_cuTensorMapEncodeTiled_v12000 tmap_encode_fn() {
   return fn;
 }
 
-// Tiled int8 map of `rank` dimensions (innermost first); strides in bytes for
+// Tiled map of `rank` dimensions (innermost first); strides in bytes for
 // dimensions 1..rank-1.
-inline bool tmap_encode_u8(CUtensorMap* m, const void* base, int rank, const cuuint64_t* dims,
-                           const cuuint64_t* strides, const cuuint32_t* box, CUtensorMapSwizzle swizzle) {
+inline bool tmap_encode(CUtensorMap* m, CUtensorMapDataType type, const void* base, int rank, const cuuint64_t* dims,
+                        const cuuint64_t* strides, const cuuint32_t* box, CUtensorMapSwizzle swizzle) {
   auto fn = tmap_encode_fn();
   if (!fn) return false;
   cuuint32_t estr[5] = {1, 1, 1, 1, 1};
-  return fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, rank, const_cast<void*>(base), dims, strides, box, estr,
-            CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  return fn(m, type, rank, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+inline bool tmap_encode_u8(CUtensorMap* m, const void* base, int rank, const cuuint64_t* dims,
+                           const cuuint64_t* strides, const cuuint32_t* box, CUtensorMapSwizzle swizzle) {
+  return tmap_encode(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, base, rank, dims, strides, box, swizzle);
 }
 
 }  // namespace tac

@@ -10,7 +10,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib as L
-from ._tensors import call, type_code
+from ._tensors import call, empty, type_code
 
 _logprobs = L.lib.tac_token_logprobs
 _F32, _I32, _I64 = torch.float32, torch.int32, torch.int64
@@ -51,17 +51,15 @@ def of_rows(address: int, xt: int, ld: int, M: int, V: int, tokens, top: int):
         raise ValueError(f"tokens must be a contiguous [{M}] tensor, got {tuple(tokens.shape)}")
     if not 0 <= top <= min(MOST_TOP, V):
         raise ValueError(f"top must be 0 to {min(MOST_TOP, V)}, got {top}")
-    dev = tokens.device
-    lp = torch.empty(M, dtype=_F32, device=dev)
-    entropy = torch.empty(M, dtype=_F32, device=dev)
+    dev = tokens.get_device()
+    lp, entropy = empty((M,), _F32, dev), empty((M,), _F32, dev)
     if not top:
         if M:
-            call("tac_token_logprobs", _logprobs, dev.index, address, xt, ld, tokens.data_ptr(), tokens.dtype is _I64, M, V, 0,
+            call("tac_token_logprobs", _logprobs, dev, address, xt, ld, tokens.data_ptr(), tokens.dtype is _I64, M, V, 0,
                  lp.data_ptr(), entropy.data_ptr(), None, None)
         return lp, entropy
-    top_lp = torch.empty((M, top), dtype=_F32, device=dev)
-    ids = torch.empty((M, top), dtype=_I32, device=dev)
+    top_lp, ids = empty((M, top), _F32, dev), empty((M, top), _I32, dev)
     if M:
-        call("tac_token_logprobs", _logprobs, dev.index, address, xt, ld, tokens.data_ptr(), tokens.dtype is _I64, M, V, top,
+        call("tac_token_logprobs", _logprobs, dev, address, xt, ld, tokens.data_ptr(), tokens.dtype is _I64, M, V, top,
              lp.data_ptr(), entropy.data_ptr(), top_lp.data_ptr(), ids.data_ptr())
     return lp, entropy, top_lp, ids

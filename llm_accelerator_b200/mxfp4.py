@@ -16,14 +16,17 @@ The calls are for inference: no gradient flows through them, also from tensors t
 """
 from __future__ import annotations
 
+from functools import lru_cache
+
 import torch
 
 from . import _lib as L
-from ._tensors import call, type_code
+from ._tensors import TYPES, call, empty, type_code
 
 _U8, _F16, _F32 = torch.uint8, torch.float16, torch.float32
 _quantize, _values, _gemm, _linear = (L.lib.tac_mxfp4_quantize, L.lib.tac_mxfp4_values, L.lib.tac_mxfp4_gemm,
                                       L.lib.tac_linear_mxfp4)
+_ws_bytes = lru_cache(maxsize=1024)(L.lib.tac_linear_mxfp4_workspace_bytes)   # sizes alone decide
 
 
 def _scale_shape(rows: int, cols: int):
@@ -51,19 +54,12 @@ class Mxfp4:
             raise ValueError("codes and scales must be on one CUDA device")
         if (codes.data_ptr() | scales.data_ptr()) & 15:
             raise ValueError("codes and scales must begin on 16-byte boundaries")
-        self._set(codes, scales, shape[0], cols, dev)
-
-    def _set(self, codes, scales, rows, cols, index):
-        self.codes, self.scales, self.rows, self.cols = codes, scales, rows, cols
-        self.device, self._index = codes.device, index
+        self.codes, self.scales, self.rows, self.cols, self._index = codes, scales, shape[0], cols, dev
         self._pointers = codes.data_ptr(), scales.data_ptr()
 
-    @classmethod
-    def _empty(cls, rows, cols, device, index):
-        self = cls.__new__(cls)
-        self._set(torch.empty((rows, (cols + 31) // 32 * 16), dtype=_U8, device=device),
-                  torch.empty(_scale_shape(rows, cols), dtype=_U8, device=device), rows, cols, index)
-        return self
+    @property
+    def device(self):
+        return self.codes.device
 
     @classmethod
     def from_tensors(cls, codes, scale_bytes, cols: int) -> "Mxfp4":
@@ -87,10 +83,13 @@ class Mxfp4:
 
     def values(self, dtype=_F32):
         """[rows, cols] that the codes stand for, rounded to `dtype`."""
-        yt = type_code(dtype, "dtype")
-        y = torch.empty((self.rows, self.cols), dtype=dtype, device=self.device)
-        if self.rows:
-            call("tac_mxfp4_values", _values, self._index, *self._pointers, y.data_ptr(), yt, self.rows, self.cols)
+        yt = TYPES.get(dtype)
+        if yt is None:
+            type_code(dtype, "dtype")
+        M, K, dev = self.rows, self.cols, self._index
+        y = empty((M, K), dtype, dev)
+        if M:
+            call("tac_mxfp4_values", _values, dev, *self._pointers, y.data_ptr(), yt, M, K)
         return y
 
 
@@ -113,14 +112,19 @@ def _rows(X):
 def quantize(X) -> Mxfp4:
     """X [M, K] (float32, float16 or bfloat16, contiguous rows at any row stride) in 4-bit form."""
     xt, ldx, M, K, dev = _rows(X)
-    q = Mxfp4._empty(M, K, X.device, dev)
+    q = Mxfp4.__new__(Mxfp4)
+    q.rows, q.cols, q._index = M, K, dev
+    tiles, groups = (M + 127) // 128, (K + 255) // 256 * 2
+    q.codes = empty((M, (K + 31) // 32 * 16), _U8, dev)
+    q.scales = empty((tiles, groups, 32, 4, 4), _U8, dev, (groups * 512, 512, 16, 4, 1))
+    q._pointers = codes, scales = q.codes.data_ptr(), q.scales.data_ptr()
     if M:
-        call("tac_mxfp4_quantize", _quantize, dev, X.data_ptr(), xt, ldx, *q._pointers, M, K)
+        call("tac_mxfp4_quantize", _quantize, dev, X.data_ptr(), xt, ldx, codes, scales, M, K)
     return q
 
 
 def _result(w, M, K, dev, bias, out, dtype):
-    """Checks of what both products share; (out, its type, bias pointer, bias type)."""
+    """Checks of what both products share; (out, its type, N, bias pointer, bias type)."""
     if w.cols != K or w._index != dev:
         raise ValueError(f"the operands must have one number of columns and one device, got {K} and {w.cols} columns")
     N = w.rows
@@ -132,10 +136,10 @@ def _result(w, M, K, dev, bias, out, dtype):
         bp = bias.data_ptr()
     yt = type_code(dtype, "out_dtype")
     if out is None:
-        out = torch.empty((M, N), dtype=dtype, device=w.device)
+        out = empty((M, N), dtype, dev)
     elif out.dtype is not dtype or out.shape != (M, N) or not out.is_contiguous() or out.get_device() != dev:
         raise ValueError(f"out must be a contiguous {dtype} [{M}, {N}] tensor on the operands' device")
-    return out, yt, bp, bt
+    return out, yt, N, bp, bt
 
 
 def gemm(a: Mxfp4, b: Mxfp4, bias=None, out_dtype=None, out=None):
@@ -144,9 +148,9 @@ def gemm(a: Mxfp4, b: Mxfp4, bias=None, out_dtype=None, out=None):
     if out_dtype is None:
         out_dtype = _F16 if out is None else out.dtype
     M, K, dev = a.rows, a.cols, a._index
-    out, yt, bp, bt = _result(b, M, K, dev, bias, out, out_dtype)
-    if M and b.rows:
-        call("tac_mxfp4_gemm", _gemm, dev, *a._pointers, *b._pointers, bp, bt, out.data_ptr(), yt, M, b.rows, K)
+    out, yt, N, bp, bt = _result(b, M, K, dev, bias, out, out_dtype)
+    if M and N:
+        call("tac_mxfp4_gemm", _gemm, dev, *a._pointers, *b._pointers, bp, bt, out.data_ptr(), yt, M, N, K)
     return out
 
 
@@ -154,20 +158,23 @@ def linear(X, w: Mxfp4, bias=None, out=None, ws=None):
     """Y [M, N] in X's type = X [M, K] @ w^T (+ bias[n]), X quantised as ``quantize`` does.
 
     X float32, float16 or bfloat16 with contiguous rows at any row stride.  ws: a ``linear_workspace`` to reuse across
-    calls on one stream; by default a call allocates its own.  A block of X with an infinity or a NaN gives a row of
-    NaN."""
+    calls on one stream; by default a call allocates its own where it needs one.  A block of X with an infinity or a NaN
+    gives a row of NaN."""
     xt, ldx, M, K, dev = _rows(X)
-    out, yt, bp, bt = _result(w, M, K, dev, bias, out, X.dtype)
-    N = w.rows
+    out, yt, N, bp, bt = _result(w, M, K, dev, bias, out, X.dtype)
     if M and N:
-        if ws is None:
-            ws = torch.empty(L.lib.tac_linear_mxfp4_workspace_bytes(M, N, K) + 256, dtype=_U8, device=X.device)
-        elif ws.get_device() != dev or ws.dtype is not _U8 or not ws.is_contiguous():
-            raise ValueError("ws must be a linear_workspace on X's device")
-        p = ws.data_ptr()
-        wp = (p + 255) & ~255
-        call("tac_linear_mxfp4", _linear, dev, X.data_ptr(), xt, ldx, *w._pointers, bp, bt, out.data_ptr(), yt, wp,
-             max(ws.numel() - (wp - p), 0), M, N, K)
+        wp, wn = None, 0
+        if ws is not None:
+            if ws.get_device() != dev or ws.dtype is not _U8 or not ws.is_contiguous():
+                raise ValueError("ws must be a linear_workspace on X's device")
+        else:
+            need = _ws_bytes(M, N, K)
+            ws = empty((need,), _U8, dev) if need else None
+        if ws is not None:
+            p = ws.data_ptr()
+            wp = (p + 255) & ~255
+            wn = max(ws.numel() - (wp - p), 0)
+        call("tac_linear_mxfp4", _linear, dev, X.data_ptr(), xt, ldx, *w._pointers, bp, bt, out.data_ptr(), yt, wp, wn, M, N, K)
     return out
 
 

@@ -14,52 +14,57 @@ from __future__ import annotations
 import torch
 
 from . import _lib as L
-from ._tensors import call, type_code
+from ._tensors import TYPES, call, empty, type_code
 
 _norm, _norm_i8 = L.lib.tac_rms_norm, L.lib.tac_rms_norm_i8
+_I8, _F32 = torch.int8, torch.float32
 
 
-def _rows(x, shape, dtype, dev, what):
+def _row_stride(x, dtype, shape, dev, what):
     """Row stride of x, which is to be a [M, K] tensor of this type with contiguous rows on device `dev`."""
     if x.dtype is not dtype:
         raise TypeError(f"{what} must be {dtype} as x, got {x.dtype}")
     if x.shape != shape or x.get_device() != dev:
         raise ValueError(f"{what} must be {tuple(shape)} on x's device, got {tuple(x.shape)} on {x.device}")
     M, K = shape
-    stride = x.stride()
-    if K > 1 and stride[1] != 1:
-        raise ValueError(f"the rows of {what} must be contiguous, got strides {stride}")
-    if M > 1 and stride[0] < K:
-        raise ValueError(f"rows of {what} overlap (stride {stride[0]}, {K} columns)")
-    return stride[0] if M > 1 else K
+    row, step = x.stride()
+    if step != 1 and K > 1:
+        raise ValueError(f"the rows of {what} must be contiguous, got strides {(row, step)}")
+    if M < 2:
+        return K
+    if row < K:
+        raise ValueError(f"rows of {what} overlap (stride {row}, {K} columns)")
+    return row
 
 
 def _args(x, weight, eps, residual, residual_out):
-    """Checks of what both norms share; (arguments of the C call up to eps, the new residual)."""
+    """Checks of what both norms share; (device, M, K, arguments of the C call up to eps, the new residual)."""
     dtype, shape, dev = x.dtype, x.shape, x.get_device()
     xt = type_code(dtype, "x")
     if len(shape) != 2 or shape[1] == 0:
         raise ValueError(f"x must be [M, K], got {tuple(shape)}")
     if dev < 0:
         raise ValueError("x must be on a CUDA device")
-    ldx = _rows(x, shape, dtype, dev, "x")
-    wt = type_code(weight.dtype, "weight")
-    if weight.shape != shape[1:] or not weight.is_contiguous() or weight.get_device() != dev:
-        raise ValueError(f"weight must be a contiguous [{shape[1]}] tensor on x's device")
+    M, K = shape
+    ldx = _row_stride(x, dtype, shape, dev, "x")
+    wt = TYPES.get(weight.dtype)
+    if wt is None:
+        type_code(weight.dtype, "weight")
+    if weight.shape != (K,) or not weight.is_contiguous() or weight.get_device() != dev:
+        raise ValueError(f"weight must be a contiguous [{K}] tensor on x's device")
     if not 0 <= eps <= 1e30:
         raise ValueError(f"eps must not be negative, got {eps}")
     if residual is None:
         if residual_out is not None:
             raise ValueError("residual_out without a residual")
-        return (x.data_ptr(), xt, ldx, None, 0, None, 0, weight.data_ptr(), wt, eps), None
-    ldr = _rows(residual, shape, dtype, dev, "residual")
+        return dev, M, K, (x.data_ptr(), xt, ldx, None, 0, None, 0, weight.data_ptr(), wt, eps), None
+    ldr, ldh = _row_stride(residual, dtype, shape, dev, "residual"), K
     if residual_out is None:
-        residual_out = torch.empty(shape, dtype=dtype, device=x.device)
-        ldh = shape[1]
+        residual_out = empty((M, K), dtype, dev)
     else:
-        ldh = _rows(residual_out, shape, dtype, dev, "residual_out")
-    return (x.data_ptr(), xt, ldx, residual.data_ptr(), ldr, residual_out.data_ptr(), ldh, weight.data_ptr(), wt,
-            eps), residual_out
+        ldh = _row_stride(residual_out, dtype, shape, dev, "residual_out")
+    return dev, M, K, (x.data_ptr(), xt, ldx, residual.data_ptr(), ldr, residual_out.data_ptr(), ldh, weight.data_ptr(), wt,
+                       eps), residual_out
 
 
 def rms_norm(x, weight, eps: float = 1e-6, residual=None, residual_out=None, out=None):
@@ -69,14 +74,13 @@ def rms_norm(x, weight, eps: float = 1e-6, residual=None, residual_out=None, out
     of any of these types.  residual_out: where h goes, by default a new tensor; it may be `residual` or x itself, but
     may not overlap them otherwise.  A row whose h^2 add up to more than float32 holds (values of 10^18) is zero; an
     infinity or a NaN makes NaN of its own place, a NaN of its whole row."""
-    args, h = _args(x, weight, eps, residual, residual_out)
-    M, K = x.shape
+    dev, M, K, args, h = _args(x, weight, eps, residual, residual_out)
     if out is None:
-        out = torch.empty((M, K), dtype=x.dtype, device=x.device)
-    elif out.dtype is not x.dtype or out.shape != x.shape or not out.is_contiguous() or out.get_device() != x.get_device():
+        out = empty((M, K), x.dtype, dev)
+    elif out.dtype is not x.dtype or out.shape != x.shape or not out.is_contiguous() or out.get_device() != dev:
         raise ValueError(f"out must be a contiguous {x.dtype} [{M}, {K}] tensor on x's device")
     if M:
-        call("tac_rms_norm", _norm, x.get_device(), *args, out.data_ptr(), M, K)
+        call("tac_rms_norm", _norm, dev, *args, out.data_ptr(), M, K)
     return out if h is None else (out, h)
 
 
@@ -85,10 +89,8 @@ def rms_norm_i8(x, weight, eps: float = 1e-6, residual=None, residual_out=None):
     scale, h).  t = max(max |y|, 1e-8), scale = t / 127, code = rint(y * (127 / t)) as in ``ptq.quantize_rows``; K_pad = K
     rounded up to 16, padding columns zero.  A row of y that holds an infinity or a NaN gets the scale NaN.
     ``ptq.dequantize_rows`` gives the values back."""
-    args, h = _args(x, weight, eps, residual, residual_out)
-    M, K = x.shape
-    q = torch.empty((M, (K + 15) // 16 * 16), dtype=torch.int8, device=x.device)
-    scale = torch.empty(M, dtype=torch.float32, device=x.device)
+    dev, M, K, args, h = _args(x, weight, eps, residual, residual_out)
+    q, scale = empty((M, (K + 15) // 16 * 16), _I8, dev), empty((M,), _F32, dev)
     if M:
-        call("tac_rms_norm_i8", _norm_i8, x.get_device(), *args, q.data_ptr(), scale.data_ptr(), M, K)
+        call("tac_rms_norm_i8", _norm_i8, dev, *args, q.data_ptr(), scale.data_ptr(), M, K)
     return (q, scale) if h is None else (q, scale, h)

@@ -22,7 +22,12 @@ device-memory plumbing).
 """
 from __future__ import annotations
 
+import torch
+
 from . import _lib as L
+from ._tensors import TYPES, call, empty, type_code
+
+_dequantize = L.lib.tac_dequantize_rows_i8
 
 
 def _stream():
@@ -82,14 +87,13 @@ def quantize_rows(X):
     return q, scale
 
 
-def dequantize_rows(q, scale, K=None, dtype=None):
-    """[M, K] q[m, k] * scale[m] (float32 unless `dtype` is float16 or bfloat16): the values that the rows of
+def dequantize_rows(q, scale, K=None, dtype=torch.float32):
+    """[M, K] q[m, k] * scale[m], rounded to `dtype` (float32, float16 or bfloat16): the values that the rows of
     ``quantize_rows`` or ``norm.rms_norm_i8`` stand for.  q int8 [M, K_pad], scale float32 [M]; K, by default all
     columns, leaves out the padding ones.  No gradient flows through the call."""
-    import torch
-    from ._tensors import call, type_code
-    dtype = torch.float32 if dtype is None else dtype
-    yt = type_code(dtype, "dtype")
+    yt = TYPES.get(dtype)
+    if yt is None:
+        type_code(dtype, "dtype")
     if q.dtype is not torch.int8 or scale.dtype is not torch.float32:
         raise TypeError("q must be int8 and scale float32")
     shape = q.shape
@@ -100,13 +104,14 @@ def dequantize_rows(q, scale, K=None, dtype=None):
     dev = q.get_device()
     if dev < 0 or scale.get_device() != dev:
         raise ValueError("q and scale must be on one CUDA device")
-    K = shape[1] if K is None else K
-    if not shape[1] - 16 < K <= shape[1]:
-        raise ValueError(f"K must be {shape[1] - 15} to {shape[1]}, got {K}")
-    y = torch.empty((shape[0], K), dtype=dtype, device=q.device)
-    if shape[0]:
-        call("tac_dequantize_rows_i8", L.lib.tac_dequantize_rows_i8, dev, q.data_ptr(), scale.data_ptr(), y.data_ptr(),
-             yt, shape[0], K)
+    M, most = shape
+    if K is None:
+        K = most
+    elif not most - 16 < K <= most:
+        raise ValueError(f"K must be {most - 15} to {most}, got {K}")
+    y = empty((M, K), dtype, dev)
+    if M:
+        call("tac_dequantize_rows_i8", _dequantize, dev, q.data_ptr(), scale.data_ptr(), y.data_ptr(), yt, M, K)
     return y
 
 
