@@ -20,6 +20,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cstdint>
+#include <type_traits>
 
 #include "tac_sm100.cuh"
 
@@ -383,22 +384,53 @@ __global__ void __launch_bounds__(kMxSkThreads)
 }
 
 // ---- rows to codes --------------------------------------------------------------------------------------------------
-// Largest magnitude of a block whose four lanes hold eight values each, as bits: infinities and NaN order above all others.
-__device__ __forceinline__ uint32_t block_max(const float (&v)[8]) {
-  uint32_t m = 0;
+// Eight values of a row held as they were loaded: 16-bit ones in one register quadruple, float32 ones in two.
+template <typename T>
+struct MxHeld {
+  uint4 u[sizeof(T) / 2];
+  __device__ __forceinline__ void load(const T* x, int left, bool vec) {     // `left` values of the row from x on
+    if (vec && left >= 8) {
 #pragma unroll
-  for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(v[j]) & 0x7fffffffu);
-  m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
-  return max(m, __shfl_xor_sync(0xffffffffu, m, 2));
-}
-__device__ __forceinline__ uint32_t scale_byte(uint32_t max_bits) {
-  const uint32_t e = max_bits >> 23;
-  return e == 255 ? 255u : e > 2 ? e - 2 : 0u;
-}
+      for (int i = 0; i < int(sizeof(T) / 2); ++i) u[i] = __ldg(reinterpret_cast<const uint4*>(x) + i);
+    } else {
+      T* t = reinterpret_cast<T*>(u);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) t[j] = j < left ? x[j] : T(0.f);
+    }
+  }
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int i = 0; i < int(sizeof(T) / 2); ++i) u[i] = make_uint4(0, 0, 0, 0);
+  }
+  __device__ __forceinline__ void values(float (&v)[8]) const {
+    const T* t = reinterpret_cast<const T*>(u);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = float(t[j]);
+  }
+  // Exponent bits of the largest magnitude, as float32, of the block that four neighbouring lanes hold.  Magnitudes are
+  // compared as whole numbers, in which infinities and NaN order above all others.
+  __device__ __forceinline__ uint32_t block_exponent() const {
+    uint32_t m;
+    if constexpr (sizeof(T) == 2) {
+      const uint32_t m2 = __vmaxu2(__vmaxu2(u[0].x & 0x7fff7fffu, u[0].y & 0x7fff7fffu), __vmaxu2(u[0].z & 0x7fff7fffu, u[0].w & 0x7fff7fffu));
+      m = max(m2 & 0xffffu, m2 >> 16);
+    } else {
+      m = 0;
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        m = max(m, max(max(u[i].x & 0x7fffffffu, u[i].y & 0x7fffffffu), max(u[i].z & 0x7fffffffu, u[i].w & 0x7fffffffu)));
+    }
+    m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+    m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+    if constexpr (std::is_same<T, __half>::value) return __float_as_uint(__half2float(__ushort_as_half(uint16_t(m)))) >> 23;
+    return sizeof(T) == 2 ? m >> 7 : m >> 23;
+  }
+};
+
+__device__ __forceinline__ uint32_t scale_byte(uint32_t exponent) { return exponent == 255 ? 255u : max(exponent, 2u) - 2; }
 // Eight codes, value 0 in the lowest four bits.
 __device__ __forceinline__ uint32_t codes8(const float (&v)[8], uint32_t byte) {
-  if (byte == 255) return 0u;
-  const float inv = __uint_as_float((254u - byte) << 23);
+  const float inv = __uint_as_float((254u - byte) << 23);        // of 255 a NaN
   uint32_t r;
   asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
       "cvt.rn.satfinite.e2m1x2.f32 b0, %2, %1;\n\t"
@@ -409,7 +441,7 @@ __device__ __forceinline__ uint32_t codes8(const float (&v)[8], uint32_t byte) {
       : "=r"(r)
       : "f"(v[0] * inv), "f"(v[1] * inv), "f"(v[2] * inv), "f"(v[3] * inv), "f"(v[4] * inv), "f"(v[5] * inv), "f"(v[6] * inv),
         "f"(v[7] * inv));
-  return r;
+  return byte == 255 ? 0u : r;
 }
 
 // ---- the split-K product of few floating-point rows, quantised in the kernel -----------------------------------------
@@ -432,27 +464,6 @@ struct MxRowsParams {
 
 // Bytes of a stage's rows: codes of tn tokens and their scales.
 __host__ __device__ constexpr int mx_rows_bytes(int tn) { return tn * 128 + kMxSfBytes; }
-
-// Eight values of a row held as they were loaded: 16-bit ones in one register quadruple, float32 ones in two.
-template <typename T>
-struct MxHeld {
-  uint4 u[sizeof(T) / 2];
-  __device__ __forceinline__ void load(const T* x, int k, int K, bool vec) {
-    if (vec && k + 8 <= K) {
-#pragma unroll
-      for (int i = 0; i < int(sizeof(T) / 2); ++i) u[i] = __ldg(reinterpret_cast<const uint4*>(x + k) + i);
-    } else {
-      T* t = reinterpret_cast<T*>(u);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) t[j] = k + j < K ? x[k + j] : T(0.f);
-    }
-  }
-  __device__ __forceinline__ void values(float (&v)[8]) const {
-    const T* t = reinterpret_cast<const T*>(u);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = float(t[j]);
-  }
-};
 
 template <typename T, int YT>
 __global__ void __launch_bounds__(kMxRowsThreads) mx_rows_kernel(const __grid_constant__ CUtensorMap tm_w, MxRowsParams pp) {
@@ -540,14 +551,15 @@ __global__ void __launch_bounds__(kMxRowsThreads) mx_rows_kernel(const __grid_co
       const int i = t + j * 256;
       if (i - lane >= items) break;              // whole warps
       stage[j] = i / of_stage, m[j] = (i - stage[j] * of_stage) >> 5;
-      held[j].load(x + m[j] * pp.ldx, (kb0 + stage[j]) * kMxStageK + lane * 8, pp.K, pp.x_vec);
+      const int k = (kb0 + stage[j]) * kMxStageK + lane * 8;
+      held[j].load(x + m[j] * pp.ldx + k, pp.K - k, pp.x_vec);
     }
 #pragma unroll
     for (int j = 0; j < kMxRowsHeld; ++j) {
       if (t + j * 256 - lane >= items) break;
       float v[8];
       held[j].values(v);
-      const uint32_t byte = scale_byte(block_max(v));
+      const uint32_t byte = scale_byte(held[j].block_exponent());
       uint8_t* codes = rows_sm + stage[j] * row_bytes;
       *reinterpret_cast<uint32_t*>(codes + m[j] * 128 + ((((lane >> 2) ^ m[j]) & 7) << 4) + (lane & 3) * 4) = codes8(v, byte);
       if ((lane & 3) == 0)

@@ -9,6 +9,7 @@
 
 #include "../../include/taccel_b200.h"
 #include "tac_launch.cuh"
+#include "tac_rows.cuh"
 
 namespace {
 
@@ -61,6 +62,22 @@ __device__ __forceinline__ void store_n(T* p, const float (&v)[N]) {
       *reinterpret_cast<uint4*>(p + i) = a.u;
     }
   }
+}
+
+// Eight 16-bit values as float32 and back.
+template <typename T>
+__device__ __forceinline__ void unpack8(const uint4& u, float (&v)[8]) {
+  const T* t = reinterpret_cast<const T*>(&u);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = to_f(t[j]);
+}
+template <typename T>
+__device__ __forceinline__ uint4 pack8(const float (&v)[8]) {
+  uint4 u;
+  T* t = reinterpret_cast<T*>(&u);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) from_f(t[j], v[j]);
+  return u;
 }
 
 struct NormParams {
@@ -133,31 +150,42 @@ __device__ __forceinline__ void reduce_row(float& ss, uint32_t& mb) {
 // and the largest |h * w| are reduced together, because the norm's factor is
 // the same for the whole row, so that one exchange among the warps gives both
 // the norm and the codes' scale.  h goes out, rounded, as soon as it is there;
-// the norm is of the unrounded sum.
-template <typename T, int VEC, bool I8, int WPR, int CH>
+// the norm is of the unrounded sum.  ANY: 16-bit rows of any alignment and
+// length, by whole warps (tac_rows.cuh).
+template <typename T, int VEC, bool ANY, bool I8, int WPR, int CH>
 __global__ void __launch_bounds__(WPR == 1 ? 128 : 32 * WPR) norm_kernel(NormParams p) {
   constexpr int kLanes = 32 * WPR;
   const int64_t row = WPR == 1 ? int64_t(blockIdx.x) * 4 + (threadIdx.x >> 5) : blockIdx.x;
   if (row >= p.M) return;                        // a whole warp (WPR 1); otherwise none
-  const int t = threadIdx.x % kLanes;
+  const int t = threadIdx.x % kLanes, lane = threadIdx.x & 31;
   const T* x = static_cast<const T*>(p.x) + row * p.ldx;
   const T* r = p.r ? static_cast<const T*>(p.r) + row * p.ldr : nullptr;
   T* h = p.r ? static_cast<T*>(p.h) + row * p.ldh : nullptr;
+  // whether chunk c has values for this thread, or with ANY for its warp
+  auto live = [&](int k) { return ANY ? k - lane * VEC < p.K : k < p.K; };
+  auto load = [&](const T* a, int k, float (&v)[VEC]) {
+    if constexpr (ANY) unpack8<T>(load8_any(reinterpret_cast<const uint16_t*>(a + k), p.K - k), v);
+    else load_n<T, VEC>(a + k, v);
+  };
+  auto store = [&](T* a, int k, const float (&v)[VEC]) {
+    if constexpr (ANY) store8_any(reinterpret_cast<uint16_t*>(a + k), pack8<T>(v), p.K - k);
+    else store_n<T, VEC>(a + k, v);
+  };
   float v[CH][VEC];
   float ss = 0.f;
   uint32_t mb = 0;
 #pragma unroll
   for (int c = 0; c < CH; ++c) {
     const int k = (t + c * kLanes) * VEC;
-    if (k < p.K) load_n<T, VEC>(x + k, v[c]);
+    if (live(k)) load(x, k, v[c]);
   }
   if (r) {
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
       const int k = (t + c * kLanes) * VEC;
-      if (k < p.K) {
+      if (live(k)) {
         float a[VEC];
-        load_n<T, VEC>(r + k, a);
+        load(r, k, a);
 #pragma unroll
         for (int j = 0; j < VEC; ++j) v[c][j] += a[j];
       }
@@ -165,19 +193,19 @@ __global__ void __launch_bounds__(WPR == 1 ? 128 : 32 * WPR) norm_kernel(NormPar
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
       const int k = (t + c * kLanes) * VEC;
-      if (k < p.K) store_n<T, VEC>(h + k, v[c]);
+      if (live(k)) store(h, k, v[c]);
     }
   }
 #pragma unroll
   for (int c = 0; c < CH; ++c) {
     const int k = (t + c * kLanes) * VEC;
-    if (k < p.K) {
+    if (live(k)) {
       float w[VEC];
-      if (VEC > 1 && p.w_vec) {
+      if (VEC > 1 && p.w_vec && (!ANY || k + VEC <= p.K)) {
         load_n<T, VEC>(static_cast<const T*>(p.w) + k, w);
       } else {
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) w[j] = weight(p, k + j);
+        for (int j = 0; j < VEC; ++j) w[j] = !ANY || k + j < p.K ? weight(p, k + j) : 0.f;
       }
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
@@ -194,10 +222,10 @@ __global__ void __launch_bounds__(WPR == 1 ? 128 : 32 * WPR) norm_kernel(NormPar
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
       const int k = (t + c * kLanes) * VEC;
-      if (k < p.K) {
+      if (live(k)) {
 #pragma unroll
         for (int j = 0; j < VEC; ++j) v[c][j] *= n.rstd;
-        store_n<T, VEC>(y + k, v[c]);
+        store(y, k, v[c]);
       }
     }
   } else {
@@ -209,7 +237,7 @@ __global__ void __launch_bounds__(WPR == 1 ? 128 : 32 * WPR) norm_kernel(NormPar
       if (k >= p.K) break;
       if constexpr (VEC == 1) {
         q[k] = uint8_t(code_bits(v[c][0], n));
-      } else {
+      } else {                                   // zeros for values past K, whose v is 0
 #pragma unroll
         for (int j = 0; j < VEC; j += 4) {
           const uint32_t lo = __byte_perm(code_bits(v[c][j], n), code_bits(v[c][j + 1], n), 0x0040);
@@ -218,7 +246,7 @@ __global__ void __launch_bounds__(WPR == 1 ? 128 : 32 * WPR) norm_kernel(NormPar
         }
       }
     }
-    for (int k = p.K + t; k < p.ldq; k += kLanes) q[k] = 0;      // the padding columns
+    for (int k = (p.K + VEC - 1) / VEC * VEC + t; k < p.ldq; k += kLanes) q[k] = 0;      // the padding columns
   }
 }
 
@@ -258,11 +286,17 @@ int launch_norm(const NormParams& p, cudaStream_t st) {
   auto rows_vec = [&](const void* a, int64_t ld) { return aligned(a, 16) && (p.M == 1 || (ld * e) % 16 == 0); };
   const bool vec = p.K % kVec == 0 && rows_vec(p.x, p.ldx) && (!p.r || (rows_vec(p.r, p.ldr) && rows_vec(p.h, p.ldh))) &&
                    (I8 || rows_vec(p.y, p.K));
-  if (vec && p.K <= 32 * 4 * kVec) return launch(norm_kernel<T, kVec, I8, 1, 4>, (p.M + 3) / 4, 128, 0, st, p);
-  if (vec && p.K <= 128 * 4 * kVec) return launch(norm_kernel<T, kVec, I8, 4, 4>, p.M, 128, 0, st, p);
-  if (vec && p.K <= 512 * 4 * kVec) return launch(norm_kernel<T, kVec, I8, 16, 4>, p.M, 512, 0, st, p);
-  if (p.K <= 128 * 32) return launch(norm_kernel<T, 1, I8, 4, 32>, p.M, 128, 0, st, p);
-  if (p.K <= 512 * 32) return launch(norm_kernel<T, 1, I8, 16, 32>, p.M, 512, 0, st, p);
+  if (vec && p.K <= 32 * 4 * kVec) return launch(norm_kernel<T, kVec, false, I8, 1, 4>, (p.M + 3) / 4, 128, 0, st, p);
+  if (vec && p.K <= 128 * 4 * kVec) return launch(norm_kernel<T, kVec, false, I8, 4, 4>, p.M, 128, 0, st, p);
+  if (vec && p.K <= 512 * 4 * kVec) return launch(norm_kernel<T, kVec, false, I8, 16, 4>, p.M, 512, 0, st, p);
+  if constexpr (sizeof(T) == 2) {
+    if (p.K <= 32 * 32) return launch(norm_kernel<T, 8, true, I8, 1, 4>, (p.M + 3) / 4, 128, 0, st, p);
+    if (p.K <= 128 * 32) return launch(norm_kernel<T, 8, true, I8, 4, 4>, p.M, 128, 0, st, p);
+    if (p.K <= 512 * 32) return launch(norm_kernel<T, 8, true, I8, 16, 4>, p.M, 512, 0, st, p);
+  } else {
+    if (p.K <= 128 * 32) return launch(norm_kernel<T, 1, false, I8, 4, 32>, p.M, 128, 0, st, p);
+    if (p.K <= 512 * 32) return launch(norm_kernel<T, 1, false, I8, 16, 32>, p.M, 512, 0, st, p);
+  }
   return launch(norm_long_kernel<T, I8>, p.M, kLongThreads, 0, st, p);
 }
 
@@ -295,35 +329,56 @@ NormParams norm_params(const void* X, int type, int64_t ldx, const void* R, int6
 }
 
 // ---- the values of codes ---------------------------------------------------------------------------------------------
-constexpr int kDqThreads = 256;
+constexpr int kDqThreads = 256, kDqRows = 4;
 
-// VEC codes a thread; a row is cut into `cuts` CTAs.
-template <typename T, int VEC>
+// Eight codes of each of four rows a thread, all loads first (8192 x 4096 to
+// BF16: 14.6 us; one row a thread takes 20); a row is cut into `cuts` CTAs.  VEC:
+// aligned rows; otherwise 16-bit ones are written by whole warps (tac_rows.cuh).
+template <typename T, bool VEC>
 __global__ void __launch_bounds__(kDqThreads) dequant_rows_kernel(const int8_t* __restrict__ Q, int ldq,
-                                                                  const float* __restrict__ scale, T* __restrict__ Y, int K,
-                                                                  int cuts) {
-  const int64_t row = blockIdx.x / cuts;
-  const int k = ((blockIdx.x % cuts) * kDqThreads + threadIdx.x) * VEC;
-  if (k >= K) return;
-  const float s = __ldg(scale + row);
-  float v[VEC];
-  if constexpr (VEC == 1) {
-    v[0] = float(Q[row * ldq + k]) * s;
-  } else {
-    const uint2 u = __ldg(reinterpret_cast<const uint2*>(Q + row * ldq + k));
+                                                                  const float* __restrict__ scale, T* __restrict__ Y, int M, int K,
+                                                                  uint32_t cuts) {
+  const uint32_t group = blockIdx.x / cuts;
+  const int64_t row = int64_t(group) * kDqRows;
+  const int k = int((blockIdx.x - group * cuts) * kDqThreads + threadIdx.x) * 8;
+  constexpr bool kAny = !VEC && sizeof(T) == 2;
+  if (kAny ? k - int(threadIdx.x & 31) * 8 >= K : k >= K) return;        // whole warps, where they write together
+  const int rows = int(min(int64_t(kDqRows), M - row));
+  uint2 u[kDqRows];
+  float s[kDqRows];
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) v[j] = float(int8_t((j < 4 ? u.x : u.y) >> (8 * (j & 3)))) * s;
+  for (int r = 0; r < kDqRows; ++r) {
+    if (r >= rows) break;
+    s[r] = __ldg(scale + row + r);
+    u[r] = make_uint2(0, 0);
+    if (k < K) u[r] = __ldg(reinterpret_cast<const uint2*>(Q + (row + r) * ldq + k));
   }
-  store_n<T, VEC>(Y + row * K + k, v);
+#pragma unroll
+  for (int r = 0; r < kDqRows; ++r) {
+    if (r >= rows) break;
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = float(int8_t((j < 4 ? u[r].x : u[r].y) >> (8 * (j & 3)))) * s[r];
+    T* y = Y + (row + r) * K + k;
+    if constexpr (VEC) {
+      store_n<T, 8>(y, v);
+    } else if constexpr (kAny) {
+      store8_any(reinterpret_cast<uint16_t*>(y), pack8<T>(v), K - k);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (k + j < K) y[j] = v[j];
+    }
+  }
 }
 
 template <typename T>
 int launch_dequant(const int8_t* Q, int ldq, const float* scale, T* Y, int M, int K, cudaStream_t st) {
-  const bool vec = K % 8 == 0 && aligned(Y, 16);
-  const int64_t per = int64_t(kDqThreads) * (vec ? 8 : 1), cuts = (K + per - 1) / per;
-  if (M * cuts > 0x7fffffff) return TAC_E_ARGUMENT;
-  if (vec) return launch(dequant_rows_kernel<T, 8>, unsigned(M * cuts), kDqThreads, 0, st, Q, ldq, scale, Y, K, int(cuts));
-  return launch(dequant_rows_kernel<T, 1>, unsigned(M * cuts), kDqThreads, 0, st, Q, ldq, scale, Y, K, int(cuts));
+  const int64_t per = kDqThreads * 8, cuts = (K + per - 1) / per, ctas = (int64_t(M) + kDqRows - 1) / kDqRows * cuts;
+  if (ctas > 0x7fffffff) return TAC_E_ARGUMENT;
+  if (K % 8 == 0 && aligned(Y, 16))
+    return launch(dequant_rows_kernel<T, true>, unsigned(ctas), kDqThreads, 0, st, Q, ldq, scale, Y, M, K, uint32_t(cuts));
+  return launch(dequant_rows_kernel<T, false>, unsigned(ctas), kDqThreads, 0, st, Q, ldq, scale, Y, M, K, uint32_t(cuts));
 }
 
 }  // namespace
