@@ -320,14 +320,20 @@ int launch_pair(const MxOperands& o, MxParams p, int clusters, int tn, cudaStrea
   return status(cudaLaunchKernelEx(&cfg, mx_pair_kernel<YT>, tw, ta, tws, tas, pp));
 }
 
+// Pairs from 65 tokens and an eighth of the pairs on; fewer tiles leave SMs
+// idle that share a tile's K.  Microseconds, pairs / split K:
+//   64 x 4096 x 4096    7.9 /  7.9   100 x 4096 x 4096    8.2 / 10.6   128 x 16384 x 4096  11.8 / 12.4
+//   20 x 50257 x 768    8.1 /  6.8   100 x 50257 x 768   10.6 / 13.6   200 x 1000 x 1000    6.5 /  9.2
+//   64 x 28672 x 1024   7.0 /  6.0   600 x 640 x 1000     5.5 /  5.4   130 x 700 x 8192    12.6 / 11.2
+// (M x N x K.)
 template <int YT>
 int pick_product(const MxOperands& o, const MxParams& p, cudaStream_t st) {
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return TAC_E_CUDA;
-  const int clusters = pair_clusters<YT>(dev);
-  if (p.M > 128 && clusters > 0) {
+  const int clusters = p.M > 64 ? pair_clusters<YT>(dev) : 0;
+  if (clusters > 0) {
     const int tn = pair_tokens(p.M, p.N, clusters);
-    if (int64_t((p.N + 255) / 256) * ((p.M + tn - 1) / tn) * 2 >= clusters) return launch_pair<YT>(o, p, clusters, tn, st);
+    if (int64_t((p.N + 255) / 256) * ((p.M + tn - 1) / tn) * 8 >= clusters) return launch_pair<YT>(o, p, clusters, tn, st);
   }
   return launch_splitk<YT>(o, p, st);
 }

@@ -118,6 +118,28 @@ def test_products_that_are_exact(M, N, K):
     assert torch.equal(got.double(), want)
 
 
+# Tiles of 64, 128, 192 and 256 tokens on pairs of CTAs, in one round and (the last three) in more than two, with token tiles
+# that begin inside a piece of scales, ragged last tiles, and 16-bit rows that begin between two words
+PAIRS = [(200, 4000, 320), (100, 4096, 512), (128, 3001, 96), (195, 19035, 96), (513, 15225, 288), (386, 19018, 544), (700, 13001, 1030),
+         (1537, 6000, 200), (4100, 2050, 64)]
+
+
+@pytest.mark.parametrize("M,N,K", PAIRS)
+def test_products_on_pairs(M, N, K):
+    from llm_accelerator_b200 import mxfp4
+    a, sa = random_rows(M, K, 11, 126, 128)
+    b, sb = random_rows(N, K, 12, 126, 128)
+    want = values(a, sa, K).cuda() @ values(b, sb, K).t().cuda()
+    qa, qb = on_device(a, sa, K), on_device(b, sb, K)
+    assert torch.equal(mxfp4.gemm(qa, qb, out_dtype=F32).double(), want)
+    bias = torch.arange(N, device="cuda").remainder(64).float()
+    # exact before the one rounding
+    assert torch.equal(mxfp4.gemm(qa, qb, bias=bias, out_dtype=BF16), (want + bias.double()).to(BF16))
+    out = torch.full((M + 1, N), -3.0, dtype=F16, device="cuda")
+    mxfp4.gemm(qa, qb, out=out[:M])
+    assert torch.equal(out[:M], want.to(F16)) and (out[M] == -3).all()
+
+
 @pytest.mark.parametrize("M,N,K", SIZES)
 def test_products(M, N, K):
     from llm_accelerator_b200 import mxfp4
