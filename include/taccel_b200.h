@@ -354,8 +354,9 @@ int tac_dequantize_rows_i8(const int8_t* Q, const float* scale, void* Y, int y_t
 /* Root-mean-square norm of rows: Y[M,K] = h / sqrt(mean_k h^2 + eps) * W[k] with
  * h = X, or X + R where R is not null; then H gets h.  X, R, H and Y are of
  * `type` (row strides ldx, ldr, ldh in elements, Y contiguous), W [K] of w_type,
- * each aligned to its elements.  Sums are float32, of the unrounded h.  H may be
- * R or X itself and may not overlap them otherwise.  No counterpart in the
+ * each aligned to its elements, K at most 2^30.  Sums are float32, of the
+ * unrounded h.  H may be R or X itself, Y likewise where their row stride is K;
+ * otherwise they may not overlap, and H and Y not at all.  No counterpart in the
  * reference, whose programs have LayerNorm (simulator.py:893-934). */
 int tac_rms_norm(const void* X, int type, int64_t ldx, const void* R, int64_t ldr, void* H, int64_t ldh,
                  const void* W, int w_type, float eps, void* Y, int M, int K, void* stream);

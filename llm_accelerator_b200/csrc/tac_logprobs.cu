@@ -478,7 +478,7 @@ __device__ __forceinline__ Share share_of(const LpParams& p, int64_t row, int ra
   return s;
 }
 
-// NT threads a row, or a cluster of CTAs of 256 where there are few rows: CTA 0
+// NT threads a row, or a cluster of CTAs of 256 where there are few: CTA 0
 // then joins the parts, which the others write into its shared memory.
 constexpr int kAtOnce = 4;             // loads of a thread in flight
 
@@ -619,16 +619,21 @@ int launch_logprobs(const LpParams& p, cudaStream_t st) {
   if (!sms_of[dev]) {
     if (int e = status(cudaDeviceGetAttribute(&sms_of[dev], cudaDevAttrMultiProcessorCount, dev))) return e;
   }
-  // CTAs a row: up to eight while all find a place at once, with two loads a thread or more
+  // CTAs a row: up to eight of 256 threads while there are three an SM at most and each thread has four loads.  Picking
+  // tokens is slower in more CTAs: 64 x 50257 with twenty takes 8.3 us in four CTAs a row, 11.1 in eight; 148 rows take 9.4
+  // in two, 14.7 in four.
   const int sms = sms_of[dev], pieces = p.V / Vec<T>::kN;
   int log_ctas = 0;
-  while (2 << log_ctas <= kMostCtas && (int64_t(p.M) << (log_ctas + 1)) <= 4 * sms && pieces >> (log_ctas + 1) >= 2 * 256) ++log_ctas;
+  while (2 << log_ctas <= kMostCtas && (int64_t(p.M) << (log_ctas + 1)) <= 3 * sms && pieces >> (log_ctas + 1) >= 4 * 256) ++log_ctas;
   if (log_ctas) return launch_rows<T, 256, true>(p, log_ctas, st);
   // A warp a row, which needs no barrier, for short rows: those of two groups of loads, and where there are rows for many
   // warps an SM those of twelve.  Against four warps a row, microseconds with five tokens picked, 16-bit logits:
   //   1000 x 1000  5.4 / 5.6   20000 x 1000  28 / 57   1000 x 8000  10.8 / 8.9   4000 x 12000  23 / 28
   //   20000 x 12000  106 / 114   4000 x 32000  54 / 56   20000 x 32000  255 / 216   4096 x 50257  91 / 78
   if (pieces <= 32 * 2 * kAtOnce || (pieces <= 32 * 12 * kAtOnce && p.M >= 8 * sms)) return launch_rows<T, 32, false>(p, 0, st);
+  // Eight warps a row while those of four would not fill the SMs: 400 x 50257 in 14.3 against 18.8 us, 888 x 50257 in 22.1
+  // against 23.4 (4096 rows 81 against 78).
+  if (p.M <= 6 * sms && pieces >= 4 * 256) return launch_rows<T, 256, false>(p, 0, st);
   return launch_rows<T, 128, false>(p, 0, st);
 }
 

@@ -195,9 +195,10 @@ __host__ __device__ constexpr int mx_sk_cols(int tn, int stages) {
   const int need = mx_sk_sf_col(tn) + 16 * stages;
   return need <= 64 ? 64 : need <= 128 ? 128 : 256;
 }
-// Shared memory that keeps the CTAs of an SM to as many as TMEM has room for.  A CTA that waits for TMEM would hold up its
-// cluster, whose other CTAs hold theirs meanwhile, and clusters, of two calls say, could wait for one another.
-__host__ __device__ constexpr int mx_sk_least_smem(int cols) { return 227 * 1024 / (512 / cols + 1) + 1024; }
+// Shared memory that keeps the CTAs of an SM to half of its TMEM.  A CTA that waits for TMEM would hold up its cluster,
+// whose other CTAs hold theirs meanwhile, and clusters, of two calls or of this product and the INT8 one, could wait for one
+// another.
+__host__ __device__ constexpr int mx_sk_least_smem(int cols) { return 227 * 1024 / (256 / cols + 1) + 1024; }
 
 __host__ __device__ constexpr int mx_sk_stage_bytes(int tn) { return kMxWBytes + tn * 128 + 2 * kMxSfBytes; }
 

@@ -310,7 +310,9 @@ int pick_norm(NormParams p, int type, cudaStream_t st) {
 // Checks that both forms share.
 int check_norm(const void* X, int type, int64_t ldx, const void* R, int64_t ldr, const void* H, int64_t ldh, const void* W,
                int w_type, const void* Y, float eps, int M, int K) {
-  if (!X || !W || !Y || !type_ok(type) || !type_ok(w_type) || M <= 0 || K <= 0 || !R != !H) return TAC_E_ARGUMENT;
+  if (!X || !W || !Y || !type_ok(type) || !type_ok(w_type) || M <= 0 || K <= 0 || K > (1 << 30) || !R != !H ||
+      (H && H == Y))
+    return TAC_E_ARGUMENT;
   if (M > 1 && (ldx < K || (R && (ldr < K || ldh < K)))) return TAC_E_ARGUMENT;
   const int e = elem(type);
   if (!aligned(X, e) || (R && (!aligned(R, e) || !aligned(H, e))) || !aligned(W, elem(w_type))) return TAC_E_ARGUMENT;
@@ -394,7 +396,7 @@ extern "C" int tac_rms_norm(const void* X, int type, int64_t ldx, const void* R,
 extern "C" int tac_rms_norm_i8(const void* X, int type, int64_t ldx, const void* R, int64_t ldr, void* H, int64_t ldh,
                                const void* W, int w_type, float eps, int8_t* Q, float* scale, int M, int K, void* stream) {
   if (int s = check_norm(X, type, ldx, R, ldr, H, ldh, W, w_type, Q, eps, M, K)) return s;
-  if (!scale || !aligned(Q, 16) || !aligned(scale, 4) || K > (1 << 30)) return TAC_E_ARGUMENT;
+  if (!scale || !aligned(Q, 16) || !aligned(scale, 4)) return TAC_E_ARGUMENT;
   return pick_norm<true>(norm_params(X, type, ldx, R, ldr, H, ldh, W, w_type, Q, scale, eps, M, K), type,
                          static_cast<cudaStream_t>(stream));
 }

@@ -10,7 +10,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib as L
-from ._tensors import call, empty, type_code
+from ._tensors import TYPES, call, empty, type_code
 
 _logprobs = L.lib.tac_token_logprobs
 _F32, _I32, _I64 = torch.float32, torch.int32, torch.int64
@@ -28,14 +28,19 @@ def token_logprobs(logits, tokens, top: int = 0):
     part in the entropy; where fewer than `top` are unmasked, masked ones follow with -inf.  A token outside [0, V) (the
     padding of a batch) has the log-probability NaN.  A row that is masked whole, or holds a NaN or +inf, gives NaN; its
     top tokens are still ordered, NaN before all numbers."""
-    xt = type_code(logits.dtype, "logits")
-    shape, stride = logits.shape, logits.stride()
-    if len(shape) != 2 or shape[1] == 0 or (shape[1] > 1 and stride[1] != 1):
-        raise ValueError(f"logits must be [M, V] with contiguous rows, got shape {tuple(shape)}, stride {stride}")
+    xt, shape = TYPES.get(logits.dtype), logits.shape
+    if xt is None:
+        type_code(logits.dtype, "logits")
+    if len(shape) != 2 or shape[1] == 0:
+        raise ValueError(f"logits must be [M, V], got {tuple(shape)}")
     M, V = shape
-    ld = stride[0] if M > 1 else V
-    if ld < V:
-        raise ValueError(f"rows of logits overlap (stride {ld}, {V} columns)")
+    ld, step = logits.stride()
+    if step != 1 or ld < V:
+        if step != 1 and V > 1:
+            raise ValueError(f"the rows of logits must be contiguous, got strides {(ld, step)}")
+        if M > 1 and ld < V:
+            raise ValueError(f"rows of logits overlap (stride {ld}, {V} columns)")
+        ld = max(ld, V)
     dev = logits.get_device()
     if dev < 0 or tokens.get_device() != dev:
         raise ValueError("logits and tokens must be on one CUDA device")
@@ -45,7 +50,8 @@ def token_logprobs(logits, tokens, top: int = 0):
 def of_rows(address: int, xt: int, ld: int, M: int, V: int, tokens, top: int):
     """``token_logprobs`` of rows that no tensor holds: M rows of V logits of type xt from `address` on, ld elements from
     one to the next, on the device of `tokens`."""
-    if tokens.dtype is not _I32 and tokens.dtype is not _I64:
+    wide = tokens.dtype is _I64
+    if not wide and tokens.dtype is not _I32:
         raise TypeError(f"tokens must be int32 or int64, got {tokens.dtype}")
     if tokens.shape != (M,) or not tokens.is_contiguous():
         raise ValueError(f"tokens must be a contiguous [{M}] tensor, got {tuple(tokens.shape)}")
@@ -55,11 +61,11 @@ def of_rows(address: int, xt: int, ld: int, M: int, V: int, tokens, top: int):
     lp, entropy = empty((M,), _F32, dev), empty((M,), _F32, dev)
     if not top:
         if M:
-            call("tac_token_logprobs", _logprobs, dev, address, xt, ld, tokens.data_ptr(), tokens.dtype is _I64, M, V, 0,
+            call("tac_token_logprobs", _logprobs, dev, address, xt, ld, tokens.data_ptr(), wide, M, V, 0,
                  lp.data_ptr(), entropy.data_ptr(), None, None)
         return lp, entropy
     top_lp, ids = empty((M, top), _F32, dev), empty((M, top), _I32, dev)
     if M:
-        call("tac_token_logprobs", _logprobs, dev, address, xt, ld, tokens.data_ptr(), tokens.dtype is _I64, M, V, top,
+        call("tac_token_logprobs", _logprobs, dev, address, xt, ld, tokens.data_ptr(), wide, M, V, top,
              lp.data_ptr(), entropy.data_ptr(), top_lp.data_ptr(), ids.data_ptr())
     return lp, entropy, top_lp, ids

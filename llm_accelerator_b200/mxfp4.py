@@ -95,15 +95,19 @@ class Mxfp4:
 
 def _rows(X):
     """(type, row stride, M, K, device) of floating-point rows X."""
-    xt = type_code(X.dtype, "X")
-    shape, stride = X.shape, X.stride()
-    if len(shape) != 2 or shape[1] == 0 or (shape[1] > 1 and stride[1] != 1):
-        raise ValueError(f"X must be [M, K] with contiguous rows, got shape {tuple(shape)}, stride {stride}")
+    xt, shape, dev = TYPES.get(X.dtype), X.shape, X.get_device()
+    if xt is None:
+        type_code(X.dtype, "X")
+    if len(shape) != 2 or shape[1] == 0:
+        raise ValueError(f"X must be [M, K], got {tuple(shape)}")
     M, K = shape
-    ldx = stride[0] if M > 1 else K
-    if ldx < K:
-        raise ValueError(f"rows of X overlap (stride {ldx}, {K} columns)")
-    dev = X.get_device()
+    ldx, step = X.stride()
+    if step != 1 or ldx < K:
+        if step != 1 and K > 1:
+            raise ValueError(f"the rows of X must be contiguous, got strides {(ldx, step)}")
+        if M > 1 and ldx < K:
+            raise ValueError(f"rows of X overlap (stride {ldx}, {K} columns)")
+        ldx = max(ldx, K)
     if dev < 0:
         raise ValueError("X must be on a CUDA device")
     return xt, ldx, M, K, dev

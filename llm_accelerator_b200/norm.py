@@ -28,32 +28,31 @@ def _row_stride(x, dtype, shape, dev, what):
         raise ValueError(f"{what} must be {tuple(shape)} on x's device, got {tuple(x.shape)} on {x.device}")
     M, K = shape
     row, step = x.stride()
+    if step == 1 and row >= K:
+        return row
     if step != 1 and K > 1:
         raise ValueError(f"the rows of {what} must be contiguous, got strides {(row, step)}")
-    if M < 2:
-        return K
-    if row < K:
+    if M > 1 and row < K:
         raise ValueError(f"rows of {what} overlap (stride {row}, {K} columns)")
-    return row
+    return max(row, K)
 
 
 def _args(x, weight, eps, residual, residual_out):
     """Checks of what both norms share; (device, M, K, arguments of the C call up to eps, the new residual)."""
-    dtype, shape, dev = x.dtype, x.shape, x.get_device()
-    xt = type_code(dtype, "x")
+    dtype, shape, dev, wt = x.dtype, x.shape, x.get_device(), TYPES.get(weight.dtype)
+    xt = TYPES.get(dtype)
+    if xt is None or wt is None:
+        type_code(dtype, "x"), type_code(weight.dtype, "weight")
     if len(shape) != 2 or shape[1] == 0:
         raise ValueError(f"x must be [M, K], got {tuple(shape)}")
     if dev < 0:
         raise ValueError("x must be on a CUDA device")
     M, K = shape
-    ldx = _row_stride(x, dtype, shape, dev, "x")
-    wt = TYPES.get(weight.dtype)
-    if wt is None:
-        type_code(weight.dtype, "weight")
-    if weight.shape != (K,) or not weight.is_contiguous() or weight.get_device() != dev:
+    if weight.shape != shape[1:] or weight.get_device() != dev or not weight.is_contiguous():
         raise ValueError(f"weight must be a contiguous [{K}] tensor on x's device")
     if not 0 <= eps <= 1e30:
         raise ValueError(f"eps must not be negative, got {eps}")
+    ldx = _row_stride(x, dtype, shape, dev, "x")
     if residual is None:
         if residual_out is not None:
             raise ValueError("residual_out without a residual")
@@ -72,13 +71,15 @@ def rms_norm(x, weight, eps: float = 1e-6, residual=None, residual_out=None, out
 
     x, residual and residual_out [M, K] float32, float16 or bfloat16 with contiguous rows at any row stride; weight [K]
     of any of these types.  residual_out: where h goes, by default a new tensor; it may be `residual` or x itself, but
-    may not overlap them otherwise.  A row whose h^2 add up to more than float32 holds (values of 10^18) is zero; an
+    may not overlap them otherwise.  out: y's tensor, which may be x or the residual (of one row stride, K).  A row whose h^2 add up to more than float32 holds (values of 10^18) is zero; an
     infinity or a NaN makes NaN of its own place, a NaN of its whole row."""
     dev, M, K, args, h = _args(x, weight, eps, residual, residual_out)
     if out is None:
         out = empty((M, K), x.dtype, dev)
     elif out.dtype is not x.dtype or out.shape != x.shape or not out.is_contiguous() or out.get_device() != dev:
         raise ValueError(f"out must be a contiguous {x.dtype} [{M}, {K}] tensor on x's device")
+    elif h is not None and out.data_ptr() == h.data_ptr() and M:
+        raise ValueError("out and residual_out must not be one tensor")
     if M:
         call("tac_rms_norm", _norm, dev, *args, out.data_ptr(), M, K)
     return out if h is None else (out, h)

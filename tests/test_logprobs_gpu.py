@@ -64,7 +64,8 @@ def _logits(M, V, dtype, seed, pad=0, spread=3.0):
 @pytest.mark.parametrize("dtype", [F16, BF16, F32])
 @pytest.mark.parametrize("M,V,pad,top", [(1, 1, 0, 1), (2, 2, 1, 2), (3, 7, 0, 5), (1, 31, 0, 31), (5, 100, 3, 20), (2, 257, 0, 32),
                                          (3, 2054, 1, 32), (4, 4099, 0, 8), (1, 8192, 0, 20), (2, 16391, 6, 20), (1, 50257, 0, 5),
-                                         (7, 50257, 0, 20), (64, 50257, 47, 32), (160, 33000, 0, 3), (700, 1500, 0, 5),
+                                         (7, 50257, 0, 20), (64, 50257, 47, 32), (160, 33000, 0, 3), (700, 1500, 0, 5), (250, 50257, 1, 20), (460, 9001, 3, 7),
+                                         (1200, 9001, 0, 32), (1250, 3001, 5, 32),
                                          (1, 262144, 0, 32), (2, 131073, 0, 0)])
 def test_against_64_bits(M, V, pad, top, dtype):
     x, tokens = _logits(M, V, dtype, M * 7 + V, pad)

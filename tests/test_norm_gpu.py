@@ -106,6 +106,17 @@ def test_the_new_residual_may_lie_over_an_input(K, over):
             _check_i8(*got, y, K)
 
 
+@pytest.mark.parametrize("K", [1024, 1001, 20001])
+def test_the_result_may_lie_over_an_input(K):
+    from llm_accelerator_b200 import norm
+    x, r, w = _inputs(30, K, F16, F16, 12)
+    want, _ = norm.rms_norm(x, w, residual=r)
+    for over in range(2):
+        a, b = x.clone(), r.clone()
+        y, _ = norm.rms_norm(a, w, residual=b, out=(a, b)[over])
+        assert torch.equal(y, want)
+
+
 def test_rows_without_finite_values_stay_among_themselves():
     from llm_accelerator_b200 import norm
     for K in (64, 777, 4096, 17000):

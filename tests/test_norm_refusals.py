@@ -10,14 +10,15 @@ from llm_accelerator_b200 import _lib as L
 from llm_accelerator_b200 import norm, ptq
 
 P = C.c_void_p(4096)     # never dereferenced: the checks come first
+Q = C.c_void_p(8192)
 ODD, HALF = C.c_void_p(4097), C.c_void_p(4098)
 
 
-def _norm(X=P, t=L.TYPE_F16, ldx=32, R=P, ldr=32, H=P, ldh=32, W=P, wt=L.TYPE_F16, eps=1e-6, Y=P, M=4, K=32):
+def _norm(X=P, t=L.TYPE_F16, ldx=32, R=P, ldr=32, H=P, ldh=32, W=P, wt=L.TYPE_F16, eps=1e-6, Y=Q, M=4, K=32):
     return L.lib.tac_rms_norm(X, t, ldx, R, ldr, H, ldh, W, wt, eps, Y, M, K, None)
 
 
-def _i8(X=P, t=L.TYPE_F16, ldx=32, R=P, ldr=32, H=P, ldh=32, W=P, wt=L.TYPE_F16, eps=1e-6, Q=P, s=P, M=4, K=32):
+def _i8(X=P, t=L.TYPE_F16, ldx=32, R=P, ldr=32, H=P, ldh=32, W=P, wt=L.TYPE_F16, eps=1e-6, Q=Q, s=P, M=4, K=32):
     return L.lib.tac_rms_norm_i8(X, t, ldx, R, ldr, H, ldh, W, wt, eps, Q, s, M, K, None)
 
 
@@ -26,7 +27,7 @@ BAD = [dict(X=None), dict(W=None), dict(R=None), dict(H=None), dict(t=3), dict(w
        dict(X=ODD), dict(R=ODD), dict(H=ODD), dict(W=ODD), dict(W=HALF, wt=L.TYPE_F32), dict(X=HALF, t=L.TYPE_F32)]
 
 
-@pytest.mark.parametrize("bad", BAD + [dict(Y=None), dict(Y=ODD)])
+@pytest.mark.parametrize("bad", BAD + [dict(Y=None), dict(Y=ODD), dict(Y=P), dict(K=(1 << 30) + 1, ldx=1 << 31, ldr=1 << 31, ldh=1 << 31)])
 def test_norm_refusals(bad):
     assert _norm(**bad) == L.E_ARGUMENT
 
@@ -88,6 +89,8 @@ def test_python_checks_on_a_device():
         norm.rms_norm(x, w.int())
     with pytest.raises(ValueError):
         norm.rms_norm(x.t(), torch.ones(4, device="cuda"))
+    with pytest.raises(ValueError):
+        norm.rms_norm(x, w, residual=x, residual_out=(y := torch.empty_like(x)), out=y)
     with pytest.raises(ValueError):
         norm.rms_norm(x, w, out=x.half())
     with pytest.raises(ValueError):
