@@ -258,8 +258,7 @@ bool map_scales(CUtensorMap* m, const uint8_t* base, int k_stages, int rows, int
 }
 
 // Tokens of a pair tile: the number that leaves the least work on the fullest
-// pair.  A stage costs, in nanoseconds: what its operands take from L2, 80 bytes
-// a nanosecond and SM, and a little more.
+// pair.  A stage costs, in nanoseconds: mostly its operands' loads.
 int pair_tokens(int M, int N, int clusters) {
   constexpr int kStageCost[4] = {273, 315, 436, 499};      // 64, 128, 192, 256 tokens (4096^3)
   const int64_t wt = (N + 255) / 256;

@@ -600,9 +600,13 @@ __global__ void __launch_bounds__(kMxRowsThreads) mx_rows_kernel(const __grid_co
 // columns would fill it: they overlap by 64, which the epilogue reads first, so
 // that the next tile's MMAs wait for a quarter of it only.  A stage's scales
 // take the columns of an earlier stage once that one's MMAs have completed.
-//   Bound by the operands' way out of L2, about 80 bytes a nanosecond and SM
-// (11 TB/s in all): 16384 x 8192 x 8192 in 404 us, 5.45 PFLOP/s; 4096^3 in 31.
-// Outputs wider than K is deep are bound by the epilogue (333 x 50257 x 768: 21
+//   Bound by the operands' way into the SM, 91 bytes a nanosecond at most
+// (measured with loads alone, on one SM as on all), and by the copies of scales
+// between the MMAs: 16384 x 8192 x 8192 takes 405 us (5.4 PFLOP/s), 356 without
+// these copies, 322 without the operands' loads, 284 without both; 4096^3 takes
+// 31.5.  Copying a stage ahead of the MMAs made nothing faster, the last round's
+// tiles in halves 4096^3 by 1.5 %.
+//   Outputs wider than K is deep are bound by the epilogue (333 x 50257 x 768: 21
 // us, 12 without stores); 16-byte stores out of shared memory, for runs of 256
 // bytes, took as long for odd rows and 3.5 us longer for even ones.
 struct MxPairCfg {
