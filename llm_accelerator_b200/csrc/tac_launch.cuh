@@ -25,4 +25,27 @@ int launch(void (*kernel)(P...), unsigned grid, int threads, size_t smem, cudaSt
   return status(cudaLaunchKernelEx(&cfg, kernel, P(args)...));
 }
 
+// The same for a kernel whose threads all begin with after_previous(): its CTAs
+// may take their places while the last ones of the kernel before it run, if
+// that one lets them (let_next), which spares the gap between two launches.
+template <typename... P, typename... A>
+int launch_behind(void (*kernel)(P...), unsigned grid, int threads, size_t smem, cudaStream_t st, A... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return status(cudaLaunchKernelEx(&cfg, kernel, P(args)...));
+}
+
+// All kernels before this one have completed, and their results are visible.
+__device__ __forceinline__ void after_previous() { asm volatile("griddepcontrol.wait;\n" ::: "memory"); }
+// The next kernel's CTAs may start where there is room; called by every CTA.
+__device__ __forceinline__ void let_next() { asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory"); }
+
 }  // namespace tac

@@ -489,6 +489,8 @@ __global__ void __launch_bounds__(NT, CLUSTER ? 4 : NT == 32 ? 32 : 1536 / NT) l
   const int ctas = CLUSTER ? 1 << log_ctas : 1, rank = CLUSTER ? blockIdx.x & (ctas - 1) : 0;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t row = CLUSTER ? blockIdx.x >> log_ctas : blockIdx.x;
+  after_previous();
+  let_next();
   if (CLUSTER) sm100::cluster_arrive();         // CTA 0's shared memory may be written once it runs
   const Share s = share_of<T, CLUSTER>(p, row, rank, log_ctas);
   float token_x = __uint_as_float(0x7fc00000u);  // a token outside the vocabulary has no probability
@@ -601,13 +603,15 @@ int launch_rows(const LpParams& p, int log_ctas, cudaStream_t st) {
   cfg.gridDim = dim3(unsigned(p.M) << log_ctas);
   cfg.blockDim = dim3(NT);
   cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = 1u << log_ctas;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = 1u << log_ctas;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = CLUSTER;
+  cfg.numAttrs = CLUSTER ? 2 : 1;
   return status(cudaLaunchKernelEx(&cfg, logprobs_kernel<T, NT, CLUSTER>, p, log_ctas));
 }
 

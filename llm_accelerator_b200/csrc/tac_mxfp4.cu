@@ -65,7 +65,8 @@ template <typename T>
 __global__ void __launch_bounds__(kQmThreads) mx_quant_kernel(const T* __restrict__ X, int64_t ldx, uint8_t* __restrict__ codes,
                                                               uint8_t* __restrict__ scales, int M, int K, int vec, uint32_t tasks,
                                                               uint32_t k_stages) {
-  asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
+  after_previous();
+  let_next();
   const uint32_t task = blockIdx.x * (kQmThreads / 32) + (threadIdx.x >> 5);
   if (task >= tasks) return;                     // a whole warp
   const int lane = threadIdx.x & 31;
@@ -108,7 +109,7 @@ int launch_quant(const void* X, int type, int64_t ldx, uint8_t* codes, uint8_t* 
   const int vec = aligned(X, 16) && (M == 1 || (ldx * elem(type)) % 16 == 0);
   const auto go = [&](auto* x) {
     using T = std::remove_const_t<std::remove_pointer_t<decltype(x)>>;
-    return launch(mx_quant_kernel<T>, unsigned(ctas), kQmThreads, 0, st, x, ldx, codes, scales, M, K, vec, uint32_t(tasks),
+    return launch_behind(mx_quant_kernel<T>, unsigned(ctas), kQmThreads, 0, st, x, ldx, codes, scales, M, K, vec, uint32_t(tasks),
                   uint32_t(k_stages));
   };
   if (type == TAC_F32) return go(static_cast<const float*>(X));
@@ -138,6 +139,8 @@ __device__ __forceinline__ int64_t quant_row(int64_t tile, int pair, int g) { re
 template <typename T>
 __global__ void __launch_bounds__(kQmThreads) mx_values_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
                                                                T* __restrict__ Y, int M, int K, int vec, uint32_t tasks, uint32_t k_stages) {
+  after_previous();
+  let_next();
   const uint32_t task = blockIdx.x * (kQmThreads / 32) + (threadIdx.x >> 5);
   if (task >= tasks) return;
   const int lane = threadIdx.x & 31;
@@ -242,10 +245,8 @@ int launch_splitk(const MxOperands& o, MxParams p, cudaStream_t st) {
     attr[cfg.numAttrs].val.clusterDim.y = 1;
     attr[cfg.numAttrs++].val.clusterDim.z = split;
   }
-  if (p.after_rows) {
-    attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
-  }
+  attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
   return status(cudaLaunchKernelEx(&cfg, mx_splitk_kernel<YT>, tw, ta, p));
 }
 
@@ -315,7 +316,7 @@ int launch_pair(const MxOperands& o, MxParams p, int clusters, int tn, cudaStrea
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = p.after_rows ? 1 : 0;
+  cfg.numAttrs = 1;
   return status(cudaLaunchKernelEx(&cfg, mx_pair_kernel<YT>, tw, ta, tws, tas, pp));
 }
 
@@ -405,13 +406,15 @@ int launch_rows_as(MxRowsParams pp, const MxOperands& o, cudaStream_t st) {
   cfg.blockDim = dim3(kMxRowsThreads);
   cfg.dynamicSmemBytes = std::max(p.stages * sb + rows, part) + 1024;
   cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = 1;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = r.split;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = 1;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = r.split;
   cfg.attrs = attr;
-  cfg.numAttrs = r.split > 1;
+  cfg.numAttrs = r.split > 1 ? 2 : 1;
   return status(cudaLaunchKernelEx(&cfg, mx_rows_kernel<T, YT>, tw, pp));
 }
 
@@ -444,7 +447,7 @@ extern "C" int tac_mxfp4_values(const uint8_t* codes, const uint8_t* scales, voi
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const auto go = [&](auto* y) {
     using T = std::remove_pointer_t<decltype(y)>;
-    return launch(mx_values_kernel<T>, unsigned(ctas), kQmThreads, 0, st, codes, scales, y, M, K, vec, uint32_t(tasks),
+    return launch_behind(mx_values_kernel<T>, unsigned(ctas), kQmThreads, 0, st, codes, scales, y, M, K, vec, uint32_t(tasks),
                   uint32_t(k_stages));
   };
   if (y_type == TAC_F32) return go(static_cast<float*>(Y));

@@ -22,6 +22,7 @@
 #include <cstdint>
 #include <type_traits>
 
+#include "tac_launch.cuh"
 #include "tac_sm100.cuh"
 
 namespace tac {
@@ -45,7 +46,7 @@ struct MxParams {
   int tn;                    // tokens of a tile
   int stages;                // of the ring
   int* fault;
-  int after_rows;            // launched while the row quantiser may still run: A and its scales wait for its end
+  int after_rows;            // launched behind the row quantiser, which may still run: A and its scales wait for its end
 };
 
 // ---- PTX ------------------------------------------------------------------------------------------------------------
@@ -313,6 +314,9 @@ __global__ void __launch_bounds__(kMxSkThreads)
   sm100::tc_fence_after();
   const uint32_t tmem = tmem_base;
   volatile int* abort_v = &abort_flag;
+  // Behind the row quantiser, which has seen the kernels before it complete, the weights are there already.
+  if (!p.after_rows) after_previous();
+  let_next();
 
   if (warp == 0) {
     uint32_t s = 0, ph = 1, issued = 0;
@@ -327,7 +331,7 @@ __global__ void __launch_bounds__(kMxSkThreads)
     if (sm100::elect_one())
       for (int i = 0; i < early; ++i) weights(i, kb0 + i);
     __syncwarp();
-    asm volatile("griddepcontrol.wait;\n" ::: "memory");
+    after_previous();
     for (int kb = kb0; kb < kb1; ++kb) {
       if (!sm100::mbar_wait_warp(&empty_bar[s], ph, abort_v, p.fault, MX_TIMEOUT_EMPTY)) break;
       if (sm100::elect_one()) {
@@ -500,6 +504,8 @@ __global__ void __launch_bounds__(kMxRowsThreads) mx_rows_kernel(const __grid_co
   sm100::tc_fence_after();
   const uint32_t tmem = tmem_base;
   volatile int* abort_v = &abort_flag;
+  after_previous();
+  let_next();
 
   if (warp == 0) {
     uint32_t s = 0, ph = 1, issued = 0;
@@ -662,10 +668,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MxPairCfg::kThreads,
   sm100::tc_fence_after();
   const uint32_t tmem = tmem_base;
   volatile int* abort_v = &abort_flag;
+  after_previous();
+  let_next();
 
   if (warp == 0) {
     uint32_t s = 0, ph = 1, issued = 0;
-    asm volatile("griddepcontrol.wait;\n" ::: "memory");
     bool go = true;
     for (int tile = cid; go && tile < total; tile += ncl) {
       const int n0 = tile / pp.t_tiles * 256 + int(rank) * 128, mt = tile % pp.t_tiles * p.tn, m0 = mt + int(rank) * half;
@@ -754,7 +761,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MxPairCfg::kThreads,
     // would do between its stores and its next wait
     const int step_w = ncl / pp.t_tiles, step_t = ncl % pp.t_tiles;
     int t_next = cid % pp.t_tiles, n_next = cid / pp.t_tiles * 256 + int(rank) * 128 + row;
-    asm volatile("griddepcontrol.wait;\n" ::: "memory");
     // the bias of a tile is loaded while the tile before it is finished
     float bias = p.bias && n_next < p.N ? mx_ld(p.bias, p.bias_type, n_next) : 0.f;
     for (int tile = cid; tile < total; tile += ncl, ++local) {

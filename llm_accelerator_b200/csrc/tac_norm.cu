@@ -155,6 +155,8 @@ __device__ __forceinline__ void reduce_row(float& ss, uint32_t& mb) {
 template <typename T, int VEC, bool ANY, bool I8, int WPR, int CH>
 __global__ void __launch_bounds__(WPR == 1 ? 128 : 32 * WPR) norm_kernel(NormParams p) {
   constexpr int kLanes = 32 * WPR;
+  after_previous();
+  let_next();
   const int64_t row = WPR == 1 ? int64_t(blockIdx.x) * 4 + (threadIdx.x >> 5) : blockIdx.x;
   if (row >= p.M) return;                        // a whole warp (WPR 1); otherwise none
   const int t = threadIdx.x % kLanes, lane = threadIdx.x & 31;
@@ -255,6 +257,8 @@ __global__ void __launch_bounds__(WPR == 1 ? 128 : 32 * WPR) norm_kernel(NormPar
 constexpr int kLongThreads = 1024;
 template <typename T, bool I8>
 __global__ void __launch_bounds__(kLongThreads) norm_long_kernel(NormParams p) {
+  after_previous();
+  let_next();
   const int64_t row = blockIdx.x;
   const T* x = static_cast<const T*>(p.x) + row * p.ldx;
   const T* r = p.r ? static_cast<const T*>(p.r) + row * p.ldr : nullptr;
@@ -286,18 +290,18 @@ int launch_norm(const NormParams& p, cudaStream_t st) {
   auto rows_vec = [&](const void* a, int64_t ld) { return aligned(a, 16) && (p.M == 1 || (ld * e) % 16 == 0); };
   const bool vec = p.K % kVec == 0 && rows_vec(p.x, p.ldx) && (!p.r || (rows_vec(p.r, p.ldr) && rows_vec(p.h, p.ldh))) &&
                    (I8 || rows_vec(p.y, p.K));
-  if (vec && p.K <= 32 * 4 * kVec) return launch(norm_kernel<T, kVec, false, I8, 1, 4>, (p.M + 3) / 4, 128, 0, st, p);
-  if (vec && p.K <= 128 * 4 * kVec) return launch(norm_kernel<T, kVec, false, I8, 4, 4>, p.M, 128, 0, st, p);
-  if (vec && p.K <= 512 * 4 * kVec) return launch(norm_kernel<T, kVec, false, I8, 16, 4>, p.M, 512, 0, st, p);
+  if (vec && p.K <= 32 * 4 * kVec) return launch_behind(norm_kernel<T, kVec, false, I8, 1, 4>, (p.M + 3) / 4, 128, 0, st, p);
+  if (vec && p.K <= 128 * 4 * kVec) return launch_behind(norm_kernel<T, kVec, false, I8, 4, 4>, p.M, 128, 0, st, p);
+  if (vec && p.K <= 512 * 4 * kVec) return launch_behind(norm_kernel<T, kVec, false, I8, 16, 4>, p.M, 512, 0, st, p);
   if constexpr (sizeof(T) == 2) {
-    if (p.K <= 32 * 32) return launch(norm_kernel<T, 8, true, I8, 1, 4>, (p.M + 3) / 4, 128, 0, st, p);
-    if (p.K <= 128 * 32) return launch(norm_kernel<T, 8, true, I8, 4, 4>, p.M, 128, 0, st, p);
-    if (p.K <= 512 * 32) return launch(norm_kernel<T, 8, true, I8, 16, 4>, p.M, 512, 0, st, p);
+    if (p.K <= 32 * 32) return launch_behind(norm_kernel<T, 8, true, I8, 1, 4>, (p.M + 3) / 4, 128, 0, st, p);
+    if (p.K <= 128 * 32) return launch_behind(norm_kernel<T, 8, true, I8, 4, 4>, p.M, 128, 0, st, p);
+    if (p.K <= 512 * 32) return launch_behind(norm_kernel<T, 8, true, I8, 16, 4>, p.M, 512, 0, st, p);
   } else {
-    if (p.K <= 128 * 32) return launch(norm_kernel<T, 1, false, I8, 4, 32>, p.M, 128, 0, st, p);
-    if (p.K <= 512 * 32) return launch(norm_kernel<T, 1, false, I8, 16, 32>, p.M, 512, 0, st, p);
+    if (p.K <= 128 * 32) return launch_behind(norm_kernel<T, 1, false, I8, 4, 32>, p.M, 128, 0, st, p);
+    if (p.K <= 512 * 32) return launch_behind(norm_kernel<T, 1, false, I8, 16, 32>, p.M, 512, 0, st, p);
   }
-  return launch(norm_long_kernel<T, I8>, p.M, kLongThreads, 0, st, p);
+  return launch_behind(norm_long_kernel<T, I8>, p.M, kLongThreads, 0, st, p);
 }
 
 template <bool I8>
@@ -340,6 +344,8 @@ template <typename T, bool VEC>
 __global__ void __launch_bounds__(kDqThreads) dequant_rows_kernel(const int8_t* __restrict__ Q, int ldq,
                                                                   const float* __restrict__ scale, T* __restrict__ Y, int M, int K,
                                                                   uint32_t cuts) {
+  after_previous();
+  let_next();
   const uint32_t group = blockIdx.x / cuts;
   const int64_t row = int64_t(group) * kDqRows;
   const int k = int((blockIdx.x - group * cuts) * kDqThreads + threadIdx.x) * 8;
@@ -379,8 +385,8 @@ int launch_dequant(const int8_t* Q, int ldq, const float* scale, T* Y, int M, in
   const int64_t per = kDqThreads * 8, cuts = (K + per - 1) / per, ctas = (int64_t(M) + kDqRows - 1) / kDqRows * cuts;
   if (ctas > 0x7fffffff) return TAC_E_ARGUMENT;
   if (K % 8 == 0 && aligned(Y, 16))
-    return launch(dequant_rows_kernel<T, true>, unsigned(ctas), kDqThreads, 0, st, Q, ldq, scale, Y, M, K, uint32_t(cuts));
-  return launch(dequant_rows_kernel<T, false>, unsigned(ctas), kDqThreads, 0, st, Q, ldq, scale, Y, M, K, uint32_t(cuts));
+    return launch_behind(dequant_rows_kernel<T, true>, unsigned(ctas), kDqThreads, 0, st, Q, ldq, scale, Y, M, K, uint32_t(cuts));
+  return launch_behind(dequant_rows_kernel<T, false>, unsigned(ctas), kDqThreads, 0, st, Q, ldq, scale, Y, M, K, uint32_t(cuts));
 }
 
 }  // namespace
