@@ -266,3 +266,19 @@ def test_grid_of_values():
     got = on_device(codes, scales, 32).values().cpu().double()
     want = (GRID * torch.exp2(scales.double() - 127)).float().double()    # 2^128 and more is infinite in float32
     assert torch.equal(got[:, :8], want) and torch.equal(got[:, 8:16], -want)
+
+
+@pytest.mark.parametrize("M", [1, 100, 300])
+@pytest.mark.parametrize("one,other", [(0, 254), (254, 0), (1, 253), (20, 234), (127, 0), (0, 127), (200, 30)])
+def test_products_at_the_ends_of_the_scales(M, one, other):
+    """2^-127 is half of float32's smallest normal number as a scale, and no less a scale for it."""
+    from llm_accelerator_b200 import mxfp4
+    K, N = 96, 300
+    a, _ = random_rows(M, K, 21)
+    b, _ = random_rows(N, K, 22)
+    sa, sb = torch.full((M, 3), one), torch.full((N, 3), other)
+    want = (values(a, sa, K) @ values(b, sb, K).t()).float()
+    got = mxfp4.gemm(on_device(a, sa, K), on_device(b, sb, K), out_dtype=F32).cpu()
+    # sums of a few multiples of one step are exact; below float32's normal numbers they may be taken for zero
+    tiny = want.abs() < 2.0 ** -126
+    assert torch.equal(got[~tiny], want[~tiny]) and bool((got[tiny].abs() < 2.0 ** -126).all())
