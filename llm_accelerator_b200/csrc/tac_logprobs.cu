@@ -7,9 +7,12 @@
 // has read, rescaled as its m grows; such triples join into one.
 //
 // The k likeliest: k of the threads' largest values give a lower bound on the
-// k-th largest logit, so only threads whose largest value reaches the bound
-// read their share again (from L1 or L2) and collect what does.  The few
-// collected entries are placed by counting how many order before each.
+// k-th largest logit (where a warp has the row and k is most of its lanes, k of
+// the largest values of their stretches: 2000 x 5000 with k = 32 takes 19 us so,
+// 116 with a bound that hundreds of values reach).  Only stretches whose largest
+// value reaches the bound are read again, from L1 or L2, and what does is
+// collected.  The few collected entries are placed by counting how many order
+// before each.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -27,7 +30,6 @@ using namespace tac;
 
 constexpr int kMostTop = 32, kMostCtas = 8;
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.693147180559945309417f;
-
 
 struct LpParams {
   const void* x;
@@ -65,6 +67,7 @@ __device__ __forceinline__ uint32_t key_of(float x) {
   const uint32_t b = __float_as_uint(x + 0.0f);
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
+constexpr uint32_t kLeastKey = ~0xff800000u;     // of -inf
 __device__ __forceinline__ float value_of(uint32_t key) {
   return __uint_as_float(key & 0x80000000u ? (key == 0xffffffffu ? 0x7fc00000u : key ^ 0x80000000u) : ~key);
 }
@@ -121,7 +124,7 @@ template <typename T>
 struct Vec;
 template <>
 struct Vec<float> {
-  static constexpr int kN = 4;
+  static constexpr int kN = 4, kLow = 0;   // values of 16 bytes, lowest bits of a key that say nothing
   static __device__ __forceinline__ float one(const void* p, int64_t i) { return __ldg(static_cast<const float*>(p) + i); }
   static __device__ __forceinline__ uint4 none() { return make_uint4(0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u); }
   static __device__ __forceinline__ void values(const uint4& u, float (&v)[4]) {
@@ -138,7 +141,7 @@ struct Vec<float> {
 };
 template <>
 struct Vec<__half> {
-  static constexpr int kN = 8;
+  static constexpr int kN = 8, kLow = 13;
   static __device__ __forceinline__ float one(const void* p, int64_t i) {
     return __half2float(__ushort_as_half(__ldg(static_cast<const uint16_t*>(p) + i)));
   }
@@ -163,7 +166,7 @@ struct Vec<__half> {
 };
 template <>
 struct Vec<__nv_bfloat16> {
-  static constexpr int kN = 8;
+  static constexpr int kN = 8, kLow = 16;
   static __device__ __forceinline__ float one(const void* p, int64_t i) {
     return __uint_as_float(uint32_t(__ldg(static_cast<const uint16_t*>(p) + i)) << 16);
   }
@@ -247,7 +250,7 @@ struct Share {
   int c0, c1;
 };
 
-// The thread's elements of `least` or more (all where it is NaN), each once: f(value, index); false ends it.
+// The thread's elements above `least` (all where it is NaN) and some others, each once: f(value, index); false ends it.
 template <typename T, int NT, typename F>
 __device__ __forceinline__ void each(const Share& s, float least, F f) {
   constexpr int N = Vec<T>::kN, kAtOnce = 4;
@@ -263,7 +266,7 @@ __device__ __forceinline__ void each(const Share& s, float least, F f) {
 #pragma unroll
     for (int q = 0; q < kAtOnce; ++q) {
       if (c + q * NT >= s.c1) return;
-      if (Vec<T>::template largest<1>({u[q]}) < least) continue;
+      if (Vec<T>::template largest<1>({u[q]}) <= least) continue;
       float v[N];
       Vec<T>::values(u[q], v);
       const int64_t i = s.first + int64_t(c + q * NT) * N;
@@ -298,6 +301,25 @@ struct LpParts {                       // of the CTAs of a cluster, in CTA 0
   Sums sums[kMostCtas];
 };
 
+// A key that at least k of a warp's, and few more, reach: the largest there is unless exactly k reach a smaller one, found
+// bit by bit.  key(i): the lane's of n times 32, at most kMost of them; kLow: how many of the lowest bits say nothing.
+template <int kLow, int kMost, typename F>
+__device__ __forceinline__ uint32_t reached_by(int k, int n, F key) {
+  uint32_t q[kMost], least = 0;
+#pragma unroll
+  for (int i = 0; i < kMost; ++i) q[i] = i < n ? key(i) : 0u;
+  for (int bit = 31; bit >= kLow; --bit) {
+    const uint32_t t = least | 1u << bit;
+    int count = 0;
+#pragma unroll
+    for (int i = 0; i < kMost; ++i)
+      if (i < n) count += __popc(__ballot_sync(0xffffffffu, q[i] >= t));
+    if (count >= k) least = t;
+    if (count == k) break;
+  }
+  return least;
+}
+
 // Places the n entries of `from` (16-byte aligned) that order among the first k into list[0 .. k).
 template <int NT>
 __device__ __forceinline__ void place(const uint64_t* from, int n, int k, uint64_t* list) {
@@ -314,6 +336,31 @@ __device__ __forceinline__ void place(const uint64_t* from, int n, int k, uint64
   }
 }
 
+// The same for the n collected ones.  A warp that has many first leaves out those that cannot be among the k.
+template <typename T, int NT>
+__device__ __forceinline__ void place_room(LpShared<NT>& sm, int n, int k) {
+  if constexpr (NT == 32) {
+    const int lane = threadIdx.x;
+    if (n > 64) {
+      const uint32_t least = reached_by<Vec<T>::kLow, LpShared<NT>::kRoom / 32>(k, (n + 31) / 32, [&](int i) {
+        return i * 32 + lane < n ? uint32_t(sm.room[i * 32 + lane] >> 32) : 0u;
+      });
+      int left = 0;
+      for (int i = 0; i < n; i += 32) {
+        const uint64_t e = i + lane < n ? sm.room[i + lane] : 0;
+        const bool stays = uint32_t(e >> 32) >= least && i + lane < n;
+        const uint32_t who = __ballot_sync(0xffffffffu, stays);
+        __syncwarp();                            // read before one of them is written over
+        if (stays) sm.room[left + __popc(who & ((1u << lane) - 1))] = e;
+        left += __popc(who);
+      }
+      n = left;
+      __syncwarp();
+    }
+  }
+  place<NT>(sm.room, n, k, sm.list);
+}
+
 // An entry of key `least` or more to sm.room, while there is room; false once it is full.
 template <int NT>
 __device__ __forceinline__ bool keep(LpShared<NT>& sm, uint32_t least, float v, int64_t i) {
@@ -324,9 +371,10 @@ __device__ __forceinline__ bool keep(LpShared<NT>& sm, uint32_t least, float v, 
   return at < LpShared<NT>::kRoom;
 }
 
-// More entries or stretches reach the bound than there is room for.  Many equal
-// values (a row with fewer than k unmasked ones): those above the bound, then of
-// those at the bound the first, in the order of their indices.
+// The bound is -inf, as in a row with fewer than k unmasked values, or more
+// entries or stretches reach it than there is room for, as where many are equal:
+// those above the bound, then of those at the bound the first, in the order of
+// their indices.
 template <typename T, int NT>
 __device__ __noinline__ void first_k_rare(LpShared<NT>& sm, const Share& s, int k, uint32_t mine, bool any, uint32_t bound) {
   constexpr int kWarps = NT / 32, kRoom = LpShared<NT>::kRoom;
@@ -339,7 +387,7 @@ __device__ __noinline__ void first_k_rare(LpShared<NT>& sm, const Share& s, int 
   __syncthreads();
   int n = sm.count;
   if (n <= kRoom) {
-    place<NT>(sm.room, n, k, sm.list);
+    place_room<T, NT>(sm, n, k);
     for (int64_t base = s.e0; n < k && base < s.e1; base += NT) {
       const int64_t i = base + threadIdx.x;
       const bool hit = i < s.e1 && key_of(Vec<T>::one(s.row, i)) == bound;
@@ -390,12 +438,16 @@ __device__ __forceinline__ void first_k(LpShared<NT>& sm, const Share& s, int k,
   // The k-th of some threads' largest values is a bound: those of each warp's first few threads, at least k in all.
   const int each_warp = min(k, (k + kWarps - 1) / kWarps + 2), some = each_warp * kWarps;
   uint32_t q = mine, bound = 0;
-  for (int i = 0; i < each_warp; ++i) {
-    bound = __reduce_max_sync(0xffffffffu, q);
-    const uint32_t who = __ballot_sync(0xffffffffu, q == bound);
-    if (lane == __ffs(who) - 1) {
-      q = 0;
-      if (kWarps > 1) sm.bounds[warp * each_warp + i] = bound;
+  if (kWarps == 1 && k > 20) {                   // of 32 threads too low a bound: the largest values of their stretches
+    bound = reached_by<Vec<T>::kLow, LpShared<NT>::kSlots>(k, slots, [&](int i) { return key_of(sm.largest[i * NT + lane]); });
+  } else {
+    for (int i = 0; i < each_warp; ++i) {
+      bound = __reduce_max_sync(0xffffffffu, q);
+      const uint32_t who = __ballot_sync(0xffffffffu, q == bound);
+      if (lane == __ffs(who) - 1) {
+        q = 0;
+        if (kWarps > 1) sm.bounds[warp * each_warp + i] = bound;
+      }
     }
   }
   if (threadIdx.x < kMostTop) sm.list[threadIdx.x] = 0;
@@ -415,8 +467,10 @@ __device__ __forceinline__ void first_k(LpShared<NT>& sm, const Share& s, int k,
     __syncthreads();
     bound = sm.bound;
   }
+  // Fewer than k threads have more than -inf: what is above it, and of those at -inf the first.
+  if (bound <= kLeastKey) return first_k_rare<T, NT>(sm, s, k, mine, any, kLeastKey);
   // What reaches the bound lies in a few stretches, which all threads read again together.
-  const float low = value_of(bound);             // NaN where nothing is below
+  const float low = value_of(bound);             // NaN where only NaN are first
   if (any && mine >= bound) {
     for (int i = 0; i < slots; ++i)
       if (!(sm.largest[i * NT + threadIdx.x] < low)) {
@@ -432,9 +486,32 @@ __device__ __forceinline__ void first_k(LpShared<NT>& sm, const Share& s, int k,
   __syncthreads();
   const int stretches = sm.stretches;
   const uint4* p = reinterpret_cast<const uint4*>(static_cast<const T*>(s.row) + s.first);
-  for (int t = threadIdx.x; t < min(stretches, kList) << log_stretch; t += NT) {
+  const int reread = min(stretches, kList) << log_stretch;
+  auto piece = [&](int t) {
     const int of = sm.stretch[t >> log_stretch];
-    const int c = s.c0 + of % NT + ((of / NT << log_stretch) + (t & ((1 << log_stretch) - 1))) * NT;
+    return s.c0 + of % NT + ((of / NT << log_stretch) + (t & ((1 << log_stretch) - 1))) * NT;
+  };
+  if constexpr (kWarps == 1) {
+    int count = sm.count;
+    for (int t = lane; t - lane < reread && count <= kRoom; t += NT) {
+      const int c = t < reread ? piece(t) : s.c1;
+      const uint4 u = c < s.c1 ? __ldg(p + c) : Vec<T>::none();
+      if (__all_sync(0xffffffffu, Vec<T>::template largest<1>({u}) < low)) continue;
+      float v[N];
+      Vec<T>::values(u, v);
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        const uint32_t key = key_of(v[j]), who = __ballot_sync(0xffffffffu, key >= bound);
+        const int at = count + __popc(who & ((1u << lane) - 1));
+        if (key >= bound && at < kRoom) sm.room[at] = entry(key, s.first + int64_t(c) * N + j);
+        count += __popc(who);
+      }
+    }
+    __syncwarp();
+    if (lane == 0) sm.count = count;
+  } else
+  for (int t = threadIdx.x; t < reread; t += NT) {
+    const int c = piece(t);
     if (c >= s.c1) continue;
     const uint4 u = __ldg(p + c);
     if (Vec<T>::template largest<1>({u}) < low) continue;
@@ -455,7 +532,7 @@ __device__ __forceinline__ void first_k(LpShared<NT>& sm, const Share& s, int k,
   __syncthreads();
   const int n = sm.count;
   if (n <= kRoom && stretches <= kList) {
-    place<NT>(sm.room, n, k, sm.list);
+    place_room<T, NT>(sm, n, k);
     __syncthreads();
     return;
   }
@@ -509,7 +586,10 @@ __global__ void __launch_bounds__(NT, CLUSTER ? 4 : NT == 32 ? 32 : 1536 / NT) l
   const int groups = ((s.c1 - s.c0 + NT - 1) / NT + kAtOnce - 1) / kAtOnce;
   int log_groups = 0;
   while (groups > LpShared<NT>::kSlots << log_groups) ++log_groups;
-  const int log_stretch = log_groups + 2, slots = (groups + (1 << log_groups) - 1) >> log_groups;
+  // a warp's short row: each piece
+  const bool single = NT == 32 && s.c1 - s.c0 <= kAtOnce * NT;
+  const int log_stretch = single ? 0 : log_groups + 2;
+  const int slots = single ? (s.c1 - s.c0 + NT - 1) / NT : (groups + (1 << log_groups) - 1) >> log_groups;
   static_assert(kAtOnce == 4, "log_stretch");
   int c = s.c0 + threadIdx.x, group = 0;
   float most = ninf(), largest = ninf();         // of the stretch, of all
@@ -519,7 +599,12 @@ __global__ void __launch_bounds__(NT, CLUSTER ? 4 : NT == 32 ? 32 : 1536 / NT) l
 #pragma unroll
     for (int i = 0; i < kAtOnce; ++i) u[i] = load_once(pieces + c + i * NT);
     most = max_nan(most, take<T, kAtOnce, CLUSTER>(a, u, pieces + c, NT));
-    if ((++group & ((1 << log_groups) - 1)) == 0) {
+    if (single) {
+#pragma unroll
+      for (int i = 0; i < kAtOnce; ++i) sm.largest[i * NT + threadIdx.x] = Vec<T>::template largest<1>({u[i]});
+      ++group;
+      largest = most;
+    } else if ((++group & ((1 << log_groups) - 1)) == 0) {
       sm.largest[((group - 1) >> log_groups) * NT + threadIdx.x] = most;
       largest = max_nan(largest, most);
       most = ninf();
@@ -530,9 +615,13 @@ __global__ void __launch_bounds__(NT, CLUSTER ? 4 : NT == 32 ? 32 : 1536 / NT) l
 #pragma unroll
     for (int i = 0; i < kAtOnce - 1; ++i) u[i][0] = c + i * NT < s.c1 ? load_once(pieces + c + i * NT) : Vec<T>::none();
 #pragma unroll
-    for (int i = 0; i < kAtOnce - 1; ++i)
-      if (c + i * NT < s.c1) most = max_nan(most, take<T, 1, CLUSTER>(a, u[i], pieces + c + i * NT, 0));
-    if (group >> log_groups < slots) sm.largest[(group >> log_groups) * NT + threadIdx.x] = most;
+    for (int i = 0; i < kAtOnce - 1; ++i) {
+      const float of = c + i * NT < s.c1 ? take<T, 1, CLUSTER>(a, u[i], pieces + c + i * NT, 0) : ninf();
+      if (single && group == 0 && i < slots) sm.largest[i * NT + threadIdx.x] = of;
+      most = max_nan(most, of);
+    }
+    if (single && group == 0 && slots == kAtOnce) sm.largest[(kAtOnce - 1) * NT + threadIdx.x] = ninf();
+    if (!single && group >> log_groups < slots) sm.largest[(group >> log_groups) * NT + threadIdx.x] = most;
     largest = max_nan(largest, most);
   }
   if (threadIdx.x < N) {

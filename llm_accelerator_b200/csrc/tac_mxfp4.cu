@@ -61,7 +61,8 @@ int64_t scale_bytes(int64_t rows, int64_t K) { return (rows + 127) / 128 * mx_pi
 // rows' scale bytes changed places in two exchanges and places were 32 bits
 // (8192 x 4096: 15.5 us, 5.5 TB/s; 21 with 123 instructions for eight values).
 constexpr int kQmThreads = 256;
-template <typename T>
+// ANY: 16-bit rows that begin anywhere.
+template <typename T, bool ANY>
 __global__ void __launch_bounds__(kQmThreads) mx_quant_kernel(const T* __restrict__ X, int64_t ldx, uint8_t* __restrict__ codes,
                                                               uint8_t* __restrict__ scales, int M, int K, int vec, uint32_t tasks,
                                                               uint32_t k_stages) {
@@ -75,12 +76,23 @@ __global__ void __launch_bounds__(kQmThreads) mx_quant_kernel(const T* __restric
   const int ldc = (K + 31) / 32 * 16;
   const T* x = X + m0 * ldx + k;
   MxHeld<T> held[4];
+  if constexpr (ANY) {
+    AnySpan<1> rows[4];
+    const int left = K - int(chunk) * kMxStageK;
 #pragma unroll
-  for (int g = 0; g < 4; ++g) {
-    held[g].clear();
-    if (m0 + g * 32 >= M) continue;              // whole warps
-    if (vec || sizeof(T) == 4) held[g].load(x + g * 32 * ldx, K - k, vec);
-    else held[g].u[0] = load8_any(reinterpret_cast<const uint16_t*>(x + g * 32 * ldx), K - k);
+    for (int g = 0; g < 4; ++g)                  // a row behind the last has nothing left
+      rows[g].load(reinterpret_cast<const uint16_t*>(x - lane * 8 + g * 32 * ldx), 1, m0 + g * 32 < M ? left : -8);
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      rows[g].values(1, left);
+      held[g].u[0] = rows[g].v[0];
+    }
+  } else {
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      held[g].clear();
+      if (m0 + g * 32 < M) held[g].load(x + g * 32 * ldx, K - k, vec);
+    }
   }
   uint8_t* c = codes + int64_t(m0) * ldc + k / 2;
   uint32_t bytes = 0;
@@ -109,8 +121,13 @@ int launch_quant(const void* X, int type, int64_t ldx, uint8_t* codes, uint8_t* 
   const int vec = aligned(X, 16) && (M == 1 || (ldx * elem(type)) % 16 == 0);
   const auto go = [&](auto* x) {
     using T = std::remove_const_t<std::remove_pointer_t<decltype(x)>>;
-    return launch_behind(mx_quant_kernel<T>, unsigned(ctas), kQmThreads, 0, st, x, ldx, codes, scales, M, K, vec, uint32_t(tasks),
-                  uint32_t(k_stages));
+    if constexpr (sizeof(T) == 2) {
+      if (!vec)
+        return launch_behind(mx_quant_kernel<T, true>, unsigned(ctas), kQmThreads, 0, st, x, ldx, codes, scales, M, K, vec,
+                             uint32_t(tasks), uint32_t(k_stages));
+    }
+    return launch_behind(mx_quant_kernel<T, false>, unsigned(ctas), kQmThreads, 0, st, x, ldx, codes, scales, M, K, vec,
+                         uint32_t(tasks), uint32_t(k_stages));
   };
   if (type == TAC_F32) return go(static_cast<const float*>(X));
   if (type == TAC_F16) return go(static_cast<const __half*>(X));
@@ -132,7 +149,9 @@ __device__ __forceinline__ __half2 e2m1x2(uint32_t byte) {
 // A warp has 256 columns of the eight rows whose scales share 32 bytes (two
 // neighbours, and those 32, 64 and 96 behind them): a lane eight values of each.
 // 8192 x 4096 to BF16: 16.5 us, 5.1 TB/s, bound by the writes; with one row a
-// thread 21.
+// thread 21.  Float32 values are not a lane's eight but one of each block, 6111
+// x 7579 in 36 us (eight a lane one by one took 184, in 16 bytes where rows
+// allow it 49).
 constexpr int kQmRows = 8;
 __device__ __forceinline__ int64_t quant_row(int64_t tile, int pair, int g) { return tile * 128 + (g >> 1) * 32 + pair * 2 + (g & 1); }
 
@@ -164,28 +183,34 @@ __global__ void __launch_bounds__(kQmThreads) mx_values_kernel(const uint8_t* __
     const uint32_t byte = (word[g] >> (8 * ((lane >> 2) & 3))) & 0xffu;
     // 2^(byte - 127); the byte 0 is half the smallest normal number, 255 NaN
     const float s = byte == 255 ? __uint_as_float(0x7fc00000u) : byte ? __uint_as_float(byte << 23) : __uint_as_float(0x00400000u);
-    T* y = Y + m * K + k;
-    union {
-      uint4 u[8 * sizeof(T) / 16];
-      T t[8];
-    } a;
+    if constexpr (sizeof(T) == 4) {              // a block of 32 columns at a time, for runs of 128 bytes wherever rows begin
+      const int k0 = int(chunk) * kMxStageK + lane;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float2 f = __half22float2(e2m1x2((c[g] >> (8 * j)) & 0xffu));
-      from_f(a.t[2 * j], f.x * s);
-      from_f(a.t[2 * j + 1], f.y * s);
-    }
-    if (vec) {
-      if (k < K) {
-#pragma unroll
-        for (int i = 0; i < int(8 * sizeof(T) / 16); ++i) reinterpret_cast<uint4*>(y)[i] = a.u[i];
+      for (int j = 0; j < 8; ++j) {
+        const uint32_t of = __shfl_sync(0xffffffffu, c[g], j * 4 + (lane >> 3));
+        const float2 f = __half22float2(e2m1x2((of >> (4 * (lane & 6))) & 0xffu));
+        const float v = (lane & 1 ? f.y : f.x) * __shfl_sync(0xffffffffu, s, j * 4);
+        if (k0 + j * 32 < K) Y[m * K + k0 + j * 32] = v;
       }
-    } else if constexpr (sizeof(T) == 2) {
-      store8_any(reinterpret_cast<uint16_t*>(y), a.u[0], K - k);
     } else {
+      T* y = Y + m * K + k;
+      union {
+        uint4 u;
+        T t[8];
+      } a;
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (k + j < K) y[j] = a.t[j];
+      for (int j = 0; j < 4; ++j) {
+        const float2 f = __half22float2(e2m1x2((c[g] >> (8 * j)) & 0xffu));
+        from_f(a.t[2 * j], f.x * s);
+        from_f(a.t[2 * j + 1], f.y * s);
+      }
+      if (vec) {
+        if (k < K) *reinterpret_cast<uint4*>(y) = a.u;
+      } else {
+        AnySpan<1> row;
+        row.v[0] = a.u;
+        row.store(reinterpret_cast<uint16_t*>(y - lane * 8), 1, K - int(chunk) * kMxStageK);
+      }
     }
   }
 }

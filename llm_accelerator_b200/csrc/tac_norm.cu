@@ -26,57 +26,51 @@ __device__ __forceinline__ void from_f(float& d, float v) { d = v; }
 __device__ __forceinline__ void from_f(__half& d, float v) { d = __float2half_rn(v); }
 __device__ __forceinline__ void from_f(__nv_bfloat16& d, float v) { d = __float2bfloat16_rn(v); }
 
-// N consecutive values in 16-byte accesses (4-byte and 2-byte ones for a single value).
+// N consecutive values in 16-byte accesses.
 template <typename T, int N>
 __device__ __forceinline__ void load_n(const T* p, float (&v)[N]) {
-  if constexpr (N == 1) {
-    v[0] = to_f(*p);
-  } else {
-    constexpr int kPer = 16 / sizeof(T);
+  constexpr int kPer = 16 / sizeof(T);
+  static_assert(N % kPer == 0, "whole accesses");
 #pragma unroll
-    for (int i = 0; i < N; i += kPer) {
-      union {
-        uint4 u;
-        T t[kPer];
-      } a;
-      a.u = *reinterpret_cast<const uint4*>(p + i);
+  for (int i = 0; i < N; i += kPer) {
+    union {
+      uint4 u;
+      T t[kPer];
+    } a;
+    a.u = *reinterpret_cast<const uint4*>(p + i);
 #pragma unroll
-      for (int j = 0; j < kPer; ++j) v[i + j] = to_f(a.t[j]);
-    }
+    for (int j = 0; j < kPer; ++j) v[i + j] = to_f(a.t[j]);
   }
 }
 template <typename T, int N>
 __device__ __forceinline__ void store_n(T* p, const float (&v)[N]) {
-  if constexpr (N == 1) {
-    from_f(*p, v[0]);
-  } else {
-    constexpr int kPer = 16 / sizeof(T);
+  constexpr int kPer = 16 / sizeof(T);
+  static_assert(N % kPer == 0, "whole accesses");
 #pragma unroll
-    for (int i = 0; i < N; i += kPer) {
-      union {
-        uint4 u;
-        T t[kPer];
-      } a;
+  for (int i = 0; i < N; i += kPer) {
+    union {
+      uint4 u;
+      T t[kPer];
+    } a;
 #pragma unroll
-      for (int j = 0; j < kPer; ++j) from_f(a.t[j], v[i + j]);
-      *reinterpret_cast<uint4*>(p + i) = a.u;
-    }
+    for (int j = 0; j < kPer; ++j) from_f(a.t[j], v[i + j]);
+    *reinterpret_cast<uint4*>(p + i) = a.u;
   }
 }
 
-// Eight 16-bit values as float32 and back.
+// The values of 16 bytes as float32 and back.
 template <typename T>
-__device__ __forceinline__ void unpack8(const uint4& u, float (&v)[8]) {
+__device__ __forceinline__ void unpack(const uint4& u, float (&v)[16 / sizeof(T)]) {
   const T* t = reinterpret_cast<const T*>(&u);
 #pragma unroll
-  for (int j = 0; j < 8; ++j) v[j] = to_f(t[j]);
+  for (int j = 0; j < int(16 / sizeof(T)); ++j) v[j] = to_f(t[j]);
 }
 template <typename T>
-__device__ __forceinline__ uint4 pack8(const float (&v)[8]) {
+__device__ __forceinline__ uint4 pack(const float (&v)[16 / sizeof(T)]) {
   uint4 u;
   T* t = reinterpret_cast<T*>(&u);
 #pragma unroll
-  for (int j = 0; j < 8; ++j) from_f(t[j], v[j]);
+  for (int j = 0; j < int(16 / sizeof(T)); ++j) from_f(t[j], v[j]);
   return u;
 }
 
@@ -88,16 +82,42 @@ struct NormParams {
   void* y;                   // rows of the input's type, or codes
   float* scale;              // of codes
   int64_t ldx, ldr, ldh;
-  int w_type, w_vec;         // w_vec: the weight is of the rows' type and aligned to 16 bytes
+  int w_type, w_vec;         // w_vec: the weight is aligned to 16 bytes
   int M, K;
   int ldq;                   // columns of the codes, K rounded up to 16
   float eps;
 };
 
-__device__ __forceinline__ float weight(const NormParams& p, int k) {
-  if (p.w_type == TAC_F32) return __ldg(static_cast<const float*>(p.w) + k);
-  const uint16_t b = __ldg(static_cast<const uint16_t*>(p.w) + k);
+__device__ __forceinline__ float half_of(const NormParams& p, uint16_t b) {
   return p.w_type == TAC_F16 ? __half2float(__ushort_as_half(b)) : __uint_as_float(uint32_t(b) << 16);
+}
+// The weights of columns k to k + VEC, 0 past K.  The type is asked for once and
+// not at each load, which would wait for the one before it.
+template <int VEC>
+__device__ __forceinline__ void weights(const NormParams& p, int k, float (&w)[VEC]) {
+  const bool whole = p.w_vec && k + VEC <= p.K;
+  if (p.w_type == TAC_F32) {
+    const float* a = static_cast<const float*>(p.w) + k;
+    if (whole) {
+      load_n<float, VEC>(a, w);
+    } else {
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) w[j] = k + j < p.K ? __ldg(a + j) : 0.f;
+    }
+  } else {
+    const uint16_t* a = static_cast<const uint16_t*>(p.w) + k;
+    uint16_t b[VEC];
+    if (VEC == 8 && whole) {
+      *reinterpret_cast<uint4*>(b) = __ldg(reinterpret_cast<const uint4*>(a));
+    } else if (VEC == 4 && whole) {
+      *reinterpret_cast<uint2*>(b) = __ldg(reinterpret_cast<const uint2*>(a));
+    } else {
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) b[j] = k + j < p.K ? __ldg(a + j) : uint16_t(0);
+    }
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) w[j] = half_of(p, b[j]);
+  }
 }
 
 // What a row's sums give: the factor of h * w, and for codes the factor of y
@@ -145,163 +165,225 @@ __device__ __forceinline__ void reduce_row(float& ss, uint32_t& mb) {
   }
 }
 
-// WPR warps a row (one: four rows a CTA), CH loads of VEC consecutive values a
-// thread.  A row is read once and stays in registers as h * w: the sum of h^2
-// and the largest |h * w| are reduced together, because the norm's factor is
-// the same for the whole row, so that one exchange among the warps gives both
-// the norm and the codes' scale.  h goes out, rounded, as soon as it is there;
-// the norm is of the unrounded sum.  ANY: 16-bit rows of any alignment and
-// length, by whole warps (tac_rows.cuh).
-template <typename T, int VEC, bool ANY, bool I8, int WPR, int CH>
-__global__ void __launch_bounds__(WPR == 1 ? 128 : 32 * WPR) norm_kernel(NormParams p) {
-  constexpr int kLanes = 32 * WPR;
+// The weighed values h * w of one load, and what they add to the row's sums.
+template <bool I8, int VEC>
+__device__ __forceinline__ void weigh(const NormParams& p, int k, float (&v)[VEC], float& ss, uint32_t& mb) {
+  float w[VEC];
+  weights<VEC>(p, k, w);
+#pragma unroll
+  for (int j = 0; j < VEC; ++j) {
+    ss = fmaf(v[j], v[j], ss);
+    v[j] *= w[j];
+    if (I8) mb = max(mb, __float_as_uint(v[j]) & 0x7fffffffu);
+  }
+}
+
+// Their codes; 0 for values past the row, which are 0.
+template <int VEC>
+__device__ __forceinline__ void store_codes(uint8_t* q, const float (&v)[VEC], const RowNorm& n) {
+#pragma unroll
+  for (int j = 0; j < VEC; j += 4) {
+    const uint32_t lo = __byte_perm(code_bits(v[j], n), code_bits(v[j + 1], n), 0x0040);
+    const uint32_t hi = __byte_perm(code_bits(v[j + 2], n), code_bits(v[j + 3], n), 0x0040);
+    reinterpret_cast<uint32_t*>(q)[j / 4] = __byte_perm(lo, hi, 0x5410);
+  }
+}
+
+// A thread's share of a row: CH loads of 16 bytes, VEC values each, the c-th
+// from at(c) on.  ANY: the row begins and ends anywhere, and a warp's loads
+// follow one another, which AnySpan needs; otherwise the row is a whole number
+// of aligned loads, which the warps take in turn.
+template <typename T, bool ANY, int CH>
+struct RowShare {
+  static constexpr int VEC = 16 / sizeof(T);
+  int K, first, step, chunks;          // of chunks that hold any of the row, the first `chunks` at most
+
+  // `warps` warps share columns [k, K)
+  __device__ __forceinline__ RowShare(int K, int k, int warp, int warps) : K(K) {
+    const int lane = threadIdx.x & 31;
+    if (ANY) {
+      chunks = min(CH, ((K - k + VEC - 1) / VEC + 32 * warps - 1) / (32 * warps));
+      first = k + (warp * chunks * 32 + lane) * VEC;
+      step = 32 * VEC;
+    } else {
+      chunks = CH;
+      first = k + (warp * 32 + lane) * VEC;
+      step = 32 * warps * VEC;
+    }
+  }
+  __device__ __forceinline__ int at(int c) const { return first + c * step; }
+  __device__ __forceinline__ bool live(int c) const { return (!ANY || c < chunks) && at(c) < K; }
+
+  // what the row has from `begin` on, or more than the share holds, in 16-bit values
+  __device__ __forceinline__ int units(int begin) const { return min(K - begin, (CH + 1) * 32 * VEC) * int(sizeof(T) / 2); }
+
+  // x (+ r) to v; h = x + r out where there is one
+  __device__ __forceinline__ void sum(const T* x, const T* r, T* h, float (&v)[CH][VEC]) const {
+    if constexpr (ANY) {
+      const int begin = first - int(threadIdx.x & 31) * VEC, left = units(begin);
+      AnySpan<CH> a, b;
+      a.load(reinterpret_cast<const uint16_t*>(x + begin), chunks, left);
+      if (r) b.load(reinterpret_cast<const uint16_t*>(r + begin), chunks, left);
+      a.values(chunks, left);
+#pragma unroll
+      for (int c = 0; c < CH; ++c) unpack<T>(a.v[c], v[c]);
+      if (r) {
+        b.values(chunks, left);
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+          float t[VEC];
+          unpack<T>(b.v[c], t);
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) v[c][j] += t[j];
+        }
+      }
+    } else {
+#pragma unroll
+      for (int c = 0; c < CH; ++c)
+        if (live(c)) load_n<T, VEC>(x + at(c), v[c]);
+      if (r) {
+#pragma unroll
+        for (int c = 0; c < CH; ++c)
+          if (live(c)) {
+            float t[VEC];
+            load_n<T, VEC>(r + at(c), t);
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) v[c][j] += t[j];
+          }
+      }
+    }
+    if (h) store(h, v);
+  }
+  __device__ __forceinline__ void store(T* y, const float (&v)[CH][VEC]) const {
+    if constexpr (ANY) {
+      const int begin = first - int(threadIdx.x & 31) * VEC;
+      AnySpan<CH> a;
+#pragma unroll
+      for (int c = 0; c < CH; ++c) a.v[c] = pack<T>(v[c]);
+      a.store(reinterpret_cast<uint16_t*>(y + begin), chunks, units(begin));
+    } else {
+#pragma unroll
+      for (int c = 0; c < CH; ++c)
+        if (live(c)) store_n<T, VEC>(y + at(c), v[c]);
+    }
+  }
+};
+
+// WPR warps a row (one: four rows a CTA), CH loads of 16 bytes a thread.  A row
+// is read once and stays in registers as h * w: the sum of h^2 and the largest
+// |h * w| are reduced together, because the norm's factor is the same for the
+// whole row, so that one exchange among the warps gives both the norm and the
+// codes' scale.  h goes out, rounded, as soon as it is there; the norm is of the
+// unrounded sum.
+template <typename T, bool ANY, bool I8, int WPR, int CH>
+__global__ void __launch_bounds__(WPR == 1 ? 128 : 32 * WPR, WPR == 16 ? 2 : 1) norm_kernel(NormParams p) {
+  using Row = RowShare<T, ANY, CH>;
+  constexpr int VEC = Row::VEC, kLanes = 32 * WPR;
   after_previous();
   let_next();
   const int64_t row = WPR == 1 ? int64_t(blockIdx.x) * 4 + (threadIdx.x >> 5) : blockIdx.x;
   if (row >= p.M) return;                        // a whole warp (WPR 1); otherwise none
-  const int t = threadIdx.x % kLanes, lane = threadIdx.x & 31;
-  const T* x = static_cast<const T*>(p.x) + row * p.ldx;
-  const T* r = p.r ? static_cast<const T*>(p.r) + row * p.ldr : nullptr;
-  T* h = p.r ? static_cast<T*>(p.h) + row * p.ldh : nullptr;
-  // whether chunk c has values for this thread, or with ANY for its warp
-  auto live = [&](int k) { return ANY ? k - lane * VEC < p.K : k < p.K; };
-  auto load = [&](const T* a, int k, float (&v)[VEC]) {
-    if constexpr (ANY) unpack8<T>(load8_any(reinterpret_cast<const uint16_t*>(a + k), p.K - k), v);
-    else load_n<T, VEC>(a + k, v);
-  };
-  auto store = [&](T* a, int k, const float (&v)[VEC]) {
-    if constexpr (ANY) store8_any(reinterpret_cast<uint16_t*>(a + k), pack8<T>(v), p.K - k);
-    else store_n<T, VEC>(a + k, v);
-  };
+  const Row s(p.K, 0, WPR == 1 ? 0 : threadIdx.x >> 5, WPR);
   float v[CH][VEC];
   float ss = 0.f;
   uint32_t mb = 0;
+  s.sum(static_cast<const T*>(p.x) + row * p.ldx, p.r ? static_cast<const T*>(p.r) + row * p.ldr : nullptr,
+        p.r ? static_cast<T*>(p.h) + row * p.ldh : nullptr, v);
 #pragma unroll
-  for (int c = 0; c < CH; ++c) {
-    const int k = (t + c * kLanes) * VEC;
-    if (live(k)) load(x, k, v[c]);
-  }
-  if (r) {
-#pragma unroll
-    for (int c = 0; c < CH; ++c) {
-      const int k = (t + c * kLanes) * VEC;
-      if (live(k)) {
-        float a[VEC];
-        load(r, k, a);
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) v[c][j] += a[j];
-      }
-    }
-#pragma unroll
-    for (int c = 0; c < CH; ++c) {
-      const int k = (t + c * kLanes) * VEC;
-      if (live(k)) store(h, k, v[c]);
-    }
-  }
-#pragma unroll
-  for (int c = 0; c < CH; ++c) {
-    const int k = (t + c * kLanes) * VEC;
-    if (live(k)) {
-      float w[VEC];
-      if (VEC > 1 && p.w_vec && (!ANY || k + VEC <= p.K)) {
-        load_n<T, VEC>(static_cast<const T*>(p.w) + k, w);
-      } else {
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) w[j] = !ANY || k + j < p.K ? weight(p, k + j) : 0.f;
-      }
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        ss = fmaf(v[c][j], v[c][j], ss);
-        v[c][j] *= w[j];
-        if (I8) mb = max(mb, __float_as_uint(v[c][j]) & 0x7fffffffu);
-      }
-    }
-  }
+  for (int c = 0; c < CH; ++c)
+    if (s.live(c)) weigh<I8, VEC>(p, s.at(c), v[c], ss, mb);
   reduce_row<WPR>(ss, mb);
   const RowNorm n = row_norm<I8>(p, ss, mb);
   if constexpr (!I8) {
-    T* y = static_cast<T*>(p.y) + row * p.K;
 #pragma unroll
-    for (int c = 0; c < CH; ++c) {
-      const int k = (t + c * kLanes) * VEC;
-      if (live(k)) {
+    for (int c = 0; c < CH; ++c)
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) v[c][j] *= n.rstd;
-        store(y, k, v[c]);
-      }
-    }
+      for (int j = 0; j < VEC; ++j) v[c][j] *= n.rstd;
+    s.store(static_cast<T*>(p.y) + row * p.K, v);
   } else {
     uint8_t* q = static_cast<uint8_t*>(p.y) + row * p.ldq;
+    const int t = threadIdx.x % kLanes;
     if (t == 0) p.scale[row] = n.scale;
 #pragma unroll
-    for (int c = 0; c < CH; ++c) {
-      const int k = (t + c * kLanes) * VEC;
-      if (k >= p.K) break;
-      if constexpr (VEC == 1) {
-        q[k] = uint8_t(code_bits(v[c][0], n));
-      } else {                                   // zeros for values past K, whose v is 0
-#pragma unroll
-        for (int j = 0; j < VEC; j += 4) {
-          const uint32_t lo = __byte_perm(code_bits(v[c][j], n), code_bits(v[c][j + 1], n), 0x0040);
-          const uint32_t hi = __byte_perm(code_bits(v[c][j + 2], n), code_bits(v[c][j + 3], n), 0x0040);
-          reinterpret_cast<uint32_t*>(q + k)[j / 4] = __byte_perm(lo, hi, 0x5410);
-        }
-      }
-    }
+    for (int c = 0; c < CH; ++c)
+      if (s.live(c)) store_codes<VEC>(q + s.at(c), v[c], n);
     for (int k = (p.K + VEC - 1) / VEC * VEC + t; k < p.ldq; k += kLanes) q[k] = 0;      // the padding columns
   }
 }
 
 // Rows too long for registers: they are read again for the results.  h is
 // written then, so that it may lie over the residual.
-constexpr int kLongThreads = 1024;
+constexpr int kLongWarps = 16, kLongLoads = 2;
 template <typename T, bool I8>
-__global__ void __launch_bounds__(kLongThreads) norm_long_kernel(NormParams p) {
+__global__ void __launch_bounds__(32 * kLongWarps, 2) norm_long_kernel(NormParams p) {
+  using Row = RowShare<T, true, kLongLoads>;
+  constexpr int VEC = Row::VEC, kStep = 32 * kLongWarps * kLongLoads * VEC;
   after_previous();
   let_next();
   const int64_t row = blockIdx.x;
+  const int warp = threadIdx.x >> 5;
   const T* x = static_cast<const T*>(p.x) + row * p.ldx;
   const T* r = p.r ? static_cast<const T*>(p.r) + row * p.ldr : nullptr;
   float ss = 0.f;
   uint32_t mb = 0;
-  for (int k = threadIdx.x; k < p.K; k += kLongThreads) {
-    const float v = to_f(x[k]) + (r ? to_f(r[k]) : 0.f);
-    ss = fmaf(v, v, ss);
-    if (I8) mb = max(mb, __float_as_uint(v * weight(p, k)) & 0x7fffffffu);
+  for (int k = 0; k < p.K; k += kStep) {
+    const Row s(p.K, k, warp, kLongWarps);
+    float v[kLongLoads][VEC];
+    s.sum(x, r, nullptr, v);
+#pragma unroll
+    for (int c = 0; c < kLongLoads; ++c)
+      if (s.live(c)) weigh<I8, VEC>(p, s.at(c), v[c], ss, mb);
   }
-  reduce_row<kLongThreads / 32>(ss, mb);
+  reduce_row<kLongWarps>(ss, mb);
   const RowNorm n = row_norm<I8>(p, ss, mb);
+  uint8_t* q = I8 ? static_cast<uint8_t*>(p.y) + row * p.ldq : nullptr;
   if (I8 && threadIdx.x == 0) p.scale[row] = n.scale;
-  for (int k = threadIdx.x; k < p.K; k += kLongThreads) {
-    const float v = to_f(x[k]) + (r ? to_f(r[k]) : 0.f);
-    if (r) from_f(static_cast<T*>(p.h)[row * p.ldh + k], v);
-    const float hw = v * weight(p, k);
-    if constexpr (I8) static_cast<uint8_t*>(p.y)[row * p.ldq + k] = uint8_t(code_bits(hw, n));
-    else from_f(static_cast<T*>(p.y)[row * p.K + k], hw * n.rstd);
+  for (int k = 0; k < p.K; k += kStep) {
+    const Row s(p.K, k, warp, kLongWarps);
+    float v[kLongLoads][VEC];
+    s.sum(x, r, r ? static_cast<T*>(p.h) + row * p.ldh : nullptr, v);
+#pragma unroll
+    for (int c = 0; c < kLongLoads; ++c) {
+      if (!s.live(c)) continue;
+      weigh<I8, VEC>(p, s.at(c), v[c], ss, mb);
+      if constexpr (I8) store_codes<VEC>(q + s.at(c), v[c], n);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) v[c][j] *= n.rstd;
+    }
+    if constexpr (!I8) s.store(static_cast<T*>(p.y) + row * p.K, v);
   }
   if constexpr (I8)
-    for (int k = p.K + threadIdx.x; k < p.ldq; k += kLongThreads) static_cast<uint8_t*>(p.y)[row * p.ldq + k] = 0;
+    for (int k = (p.K + VEC - 1) / VEC * VEC + threadIdx.x; k < p.ldq; k += 32 * kLongWarps) q[k] = 0;
+}
+
+// As few warps a row as hold it in four loads a thread; float32 rows of any
+// alignment in eight, with which more rows are under way on an SM (3184 x 4095
+// with a residual: 43 us, 51 with four; aligned 35), unless they take more than
+// 16 warps would have registers for.
+template <typename T, bool ANY, bool I8>
+int launch_rows(const NormParams& p, cudaStream_t st) {
+  constexpr bool kWide = ANY && sizeof(T) == 4;
+  constexpr int kLoads = kWide ? 8 : 4, kOf = kLoads * 16 / sizeof(T);
+  if (p.K <= 32 * kOf) return launch_behind(norm_kernel<T, ANY, I8, 1, kLoads>, (p.M + 3) / 4, 128, 0, st, p);
+  if (p.K <= 128 * kOf) return launch_behind(norm_kernel<T, ANY, I8, 4, kLoads>, p.M, 128, 0, st, p);
+  if constexpr (kWide) {
+    if (p.K <= 1024 * 16) return launch_behind(norm_kernel<T, ANY, I8, 32, 4>, p.M, 1024, 0, st, p);
+  } else {
+    if (p.K <= 512 * kOf) return launch_behind(norm_kernel<T, ANY, I8, 16, 4>, p.M, 512, 0, st, p);
+    if constexpr (sizeof(T) == 4) {
+      if (p.K <= 1024 * kOf) return launch_behind(norm_kernel<T, ANY, I8, 16, 8>, p.M, 512, 0, st, p);
+    }
+  }
+  return launch_behind(norm_long_kernel<T, I8>, p.M, 32 * kLongWarps, 0, st, p);
 }
 
 template <typename T, bool I8>
 int launch_norm(const NormParams& p, cudaStream_t st) {
-  constexpr int kVec = 16 / sizeof(T);
-  const int e = sizeof(T);
-  auto rows_vec = [&](const void* a, int64_t ld) { return aligned(a, 16) && (p.M == 1 || (ld * e) % 16 == 0); };
-  const bool vec = p.K % kVec == 0 && rows_vec(p.x, p.ldx) && (!p.r || (rows_vec(p.r, p.ldr) && rows_vec(p.h, p.ldh))) &&
-                   (I8 || rows_vec(p.y, p.K));
-  if (vec && p.K <= 32 * 4 * kVec) return launch_behind(norm_kernel<T, kVec, false, I8, 1, 4>, (p.M + 3) / 4, 128, 0, st, p);
-  if (vec && p.K <= 128 * 4 * kVec) return launch_behind(norm_kernel<T, kVec, false, I8, 4, 4>, p.M, 128, 0, st, p);
-  if (vec && p.K <= 512 * 4 * kVec) return launch_behind(norm_kernel<T, kVec, false, I8, 16, 4>, p.M, 512, 0, st, p);
-  if constexpr (sizeof(T) == 2) {
-    if (p.K <= 32 * 32) return launch_behind(norm_kernel<T, 8, true, I8, 1, 4>, (p.M + 3) / 4, 128, 0, st, p);
-    if (p.K <= 128 * 32) return launch_behind(norm_kernel<T, 8, true, I8, 4, 4>, p.M, 128, 0, st, p);
-    if (p.K <= 512 * 32) return launch_behind(norm_kernel<T, 8, true, I8, 16, 4>, p.M, 512, 0, st, p);
-  } else {
-    if (p.K <= 128 * 32) return launch_behind(norm_kernel<T, 1, false, I8, 4, 32>, p.M, 128, 0, st, p);
-    if (p.K <= 512 * 32) return launch_behind(norm_kernel<T, 1, false, I8, 16, 32>, p.M, 512, 0, st, p);
-  }
-  return launch_behind(norm_long_kernel<T, I8>, p.M, kLongThreads, 0, st, p);
+  auto whole = [&](const void* a, int64_t ld) { return aligned(a, 16) && (p.M == 1 || ld * int64_t(sizeof(T)) % 16 == 0); };
+  const bool loads = p.K % (16 / int(sizeof(T))) == 0 && whole(p.x, p.ldx) && (!p.r || (whole(p.r, p.ldr) && whole(p.h, p.ldh))) &&
+                     (I8 || whole(p.y, p.K));
+  if (loads) return launch_rows<T, false, I8>(p, st);
+  return launch_rows<T, true, I8>(p, st);
 }
 
 template <bool I8>
@@ -328,7 +410,7 @@ NormParams norm_params(const void* X, int type, int64_t ldx, const void* R, int6
   NormParams p{};
   p.x = X, p.r = R, p.h = H, p.w = W, p.y = Y, p.scale = scale;
   p.ldx = ldx, p.ldr = ldr, p.ldh = ldh;
-  p.w_type = w_type, p.w_vec = w_type == type && aligned(W, 16);
+  p.w_type = w_type, p.w_vec = aligned(W, 16);
   p.M = M, p.K = K, p.ldq = int((int64_t(K) + 15) / 16 * 16);
   p.eps = eps;
   return p;
@@ -371,7 +453,10 @@ __global__ void __launch_bounds__(kDqThreads) dequant_rows_kernel(const int8_t* 
     if constexpr (VEC) {
       store_n<T, 8>(y, v);
     } else if constexpr (kAny) {
-      store8_any(reinterpret_cast<uint16_t*>(y), pack8<T>(v), K - k);
+      AnySpan<1> a;
+      a.v[0] = pack<T>(v);
+      const int before = int(threadIdx.x & 31) * 8;
+      a.store(reinterpret_cast<uint16_t*>(y - before), 1, K - k + before);
     } else {
 #pragma unroll
       for (int j = 0; j < 8; ++j)

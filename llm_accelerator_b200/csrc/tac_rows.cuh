@@ -1,31 +1,13 @@
-// 16-bit rows that begin anywhere: a warp whose lanes hold eight consecutive
-// values each reads and writes them in aligned 16-byte accesses, in which a
-// lane's eight are its own piece's end and its neighbour's beginning.  (Values
-// one by one, 2 bytes a lane, took three times as long as aligned rows.)
+// Rows that begin anywhere, counted in 16-bit values: a warp whose lanes hold
+// eight consecutive ones each reads and writes them in aligned 16-byte accesses,
+// in which a lane's eight are its own piece's end and its neighbour's beginning.
+// Rows of float32 are such rows of two values each.  (One value a lane and load
+// took three times as long as aligned rows.)
 #pragma once
 #include <cstdint>
+#include <type_traits>
 
 namespace tac {
-
-// The eight values from place `by` (0..7, one for the whole warp) on of sixteen.
-__device__ __forceinline__ uint4 eight_from(const uint4& a, const uint4& b, int by) {
-  uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-  if (by & 4) {
-#pragma unroll
-    for (int i = 0; i < 6; ++i) w[i] = w[i + 2];
-  }
-  if (by & 2) {
-#pragma unroll
-    for (int i = 0; i < 5; ++i) w[i] = w[i + 1];
-  }
-  const uint32_t sel = by & 1 ? 0x5432 : 0x3210;
-  return make_uint4(__byte_perm(w[0], w[1], sel), __byte_perm(w[1], w[2], sel), __byte_perm(w[2], w[3], sel), __byte_perm(w[3], w[4], sel));
-}
-
-__device__ __forceinline__ uint4 of_next_lane(const uint4& a) {
-  return make_uint4(__shfl_down_sync(0xffffffffu, a.x, 1), __shfl_down_sync(0xffffffffu, a.y, 1), __shfl_down_sync(0xffffffffu, a.z, 1),
-                    __shfl_down_sync(0xffffffffu, a.w, 1));
-}
 
 // Values [0, n) of the eight, zeros behind them.
 __device__ __forceinline__ uint4 first_of(uint4 a, int n) {
@@ -34,34 +16,87 @@ __device__ __forceinline__ uint4 first_of(uint4 a, int n) {
   return make_uint4(word(a.x, 0), word(a.y, 2), word(a.z, 4), word(a.w, 6));
 }
 
-// Whole warps: lane i has the eight values from p = (lane 0's) + 8 i on, of which the row still has `left` (also none or
-// fewer); zeros for the rest.  Bytes beside the row are read only in 16-byte pieces that hold some of it.
-__device__ __forceinline__ uint4 load8_any(const uint16_t* p, int left) {
-  const int off = int(reinterpret_cast<uintptr_t>(p) >> 1) & 7;          // values from the aligned place to p
-  const uint4* q = reinterpret_cast<const uint4*>(p - off);
-  uint4 own = make_uint4(0, 0, 0, 0), last = own;
-  if (left + off > 0) own = *q;                  // no read-only load: the row may be written by this kernel later
-  if (off == 0) return first_of(own, left);
-  if ((threadIdx.x & 31) == 31 && left > 8 - off) last = q[1];
-  uint4 next = of_next_lane(own);
-  if ((threadIdx.x & 31) == 31) next = last;
-  return first_of(eight_from(own, next, off), left);
-}
+// Whole warps: `chunks` (at most CH) times 32 lanes of eight values from p on, lane i of chunk c at p + 256 c + 8 i, of which
+// the row still has `left` (also none).  Reading is split, so that many loads are under way before the first is waited for:
+// load() takes the aligned pieces that the chunks begin in, and the one in which the last of them ends; values() gives the
+// eight of each lane, zeros behind the row.  Bytes beside the row are read only in pieces that hold some of it, and of a
+// piece that two warps share each uses its own values, so that other warps may write theirs meanwhile.
+template <int CH>
+struct AnySpan {
+  uint4 v[CH], tail;
+  int off;                             // values from the aligned place to p
 
-// The same places written; values from `left` on are not.
-__device__ __forceinline__ void store8_any(uint16_t* p, const uint4& v, int left) {
-  const int off = int(reinterpret_cast<uintptr_t>(p) >> 1) & 7, head = (8 - off) & 7, lane = threadIdx.x & 31;
-  auto some = [](uint16_t* d, const uint4& a, int n) {                   // n < 8 of them
-    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+  // Places 2 S + odd to 2 S + odd + 7 of a lane's eight and those behind them, which are the next lane's, or the next chunk's.
+  template <int S>
+  __device__ __forceinline__ uint4 behind(int c, int chunks, uint32_t odd) const {
+    const uint4 over = c + 1 < CH && c + 1 < chunks ? v[c + 1 < CH ? c + 1 : c] : tail;
+    const bool first = (threadIdx.x & 31) == 0;
+    const int from = (threadIdx.x + 1) & 31;
+    uint32_t w[8] = {v[c].x, v[c].y, v[c].z, v[c].w};
+    w[4] = __shfl_sync(0xffffffffu, first ? over.x : v[c].x, from);
+    if (S >= 1) w[5] = __shfl_sync(0xffffffffu, first ? over.y : v[c].y, from);
+    if (S >= 2) w[6] = __shfl_sync(0xffffffffu, first ? over.z : v[c].z, from);
+    if (S >= 3) w[7] = __shfl_sync(0xffffffffu, first ? over.w : v[c].w, from);
+    const uint32_t sel = odd ? 0x5432 : 0x3210;
+    return make_uint4(__byte_perm(w[S], w[S + 1], sel), __byte_perm(w[S + 1], w[S + 2], sel), __byte_perm(w[S + 2], w[S + 3], sel),
+                      __byte_perm(w[S + 3], w[S + 4], sel));
+  }
+  // f(integral constant S) for places from `by` (0..7, the warp's) on
+  template <typename F>
+  __device__ __forceinline__ static void shifted(int by, F f) {
+    switch (by >> 1) {
+      case 0: return f(std::integral_constant<int, 0>());
+      case 1: return f(std::integral_constant<int, 1>());
+      case 2: return f(std::integral_constant<int, 2>());
+      default: return f(std::integral_constant<int, 3>());
+    }
+  }
+  __device__ __forceinline__ void load(const uint16_t* p, int chunks, int left) {
+    const int lane = threadIdx.x & 31;
+    off = int(reinterpret_cast<uintptr_t>(p) >> 1) & 7;
+    const uint4* q = reinterpret_cast<const uint4*>(p - off) + lane;     // no read-only loads: the row may be written later
 #pragma unroll
-    for (int i = 0; i < 7; ++i)
-      if (i < n) d[i] = uint16_t(w[i >> 1] >> (16 * (i & 1)));
-  };
-  const uint4 moved = off ? eight_from(v, of_next_lane(v), head) : v;
-  const int n = lane == 31 && off ? min(8 - head, left - head) : left - head;    // the last lane's neighbour is another warp's
-  if (n >= 8) *reinterpret_cast<uint4*>(p + head) = moved;
-  else some(p + head, moved, n);
-  if (lane == 0) some(p, v, min(head, left));
-}
+    for (int c = 0; c < CH; ++c) v[c] = c < chunks && left + off > 256 * c + 8 * lane ? q[32 * c] : make_uint4(0, 0, 0, 0);
+    tail = lane == 0 && off && left + off > 256 * chunks ? q[32 * chunks] : make_uint4(0, 0, 0, 0);
+  }
+  __device__ __forceinline__ void values(int chunks, int left) {
+    if (off) {
+      shifted(off, [&](auto by) {
+#pragma unroll
+        for (int c = 0; c < CH; ++c)
+          if (c < chunks) v[c] = behind<by.value>(c, chunks, off & 1);   // v[c + 1] is still as it was read
+      });
+    }
+#pragma unroll
+    for (int c = 0; c < CH; ++c)
+      if (left < 256 * (c + 1)) v[c] = first_of(v[c], left - 256 * c - 8 * int(threadIdx.x & 31));
+  }
+  // The lanes' values to such places; those from `left` on are not written.
+  __device__ __forceinline__ void store(uint16_t* p, int chunks, int left) {
+    const int lane = threadIdx.x & 31;
+    off = int(reinterpret_cast<uintptr_t>(p) >> 1) & 7;
+    const int head = (8 - off) & 7;
+    auto some = [](uint16_t* d, const uint4& a, int n) {                 // n < 8 of them
+      const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+      for (int i = 0; i < 7; ++i)
+        if (i < n) d[i] = uint16_t(w[i >> 1] >> (16 * (i & 1)));
+    };
+    tail = make_uint4(0, 0, 0, 0);               // another warp's
+    shifted(head, [&](auto by) {
+#pragma unroll
+      for (int c = 0; c < CH; ++c) {
+        if (c >= chunks) break;
+        uint16_t* d = p + 256 * c + 8 * lane + head;
+        const uint4 moved = off ? behind<by.value>(c, chunks, head & 1) : v[c];
+        int n = left - 256 * c - 8 * lane - head;
+        if (off && lane == 31 && c + 1 == chunks) n = min(n, 8 - head);
+        if (n >= 8) *reinterpret_cast<uint4*>(d) = moved;
+        else some(d, moved, n);
+      }
+    });
+    if (lane == 0) some(p, v[0], min(head, left));
+  }
+};
 
 }  // namespace tac

@@ -248,3 +248,18 @@ def test_the_batched_runner_gives_them_for_its_step():
         r.token_logprobs("decode", [0] * 5, r.logits_count + 1)
     with pytest.raises(ValueError):
         r.token_logprobs("decode", [0] * 4, 10)
+
+
+@pytest.mark.parametrize("top", [8, 20, 21, 32])
+@pytest.mark.parametrize("V", [33, 100, 255, 500, 776, 900, 1024, 1027, 2048, 3001])
+def test_many_of_short_rows(V, top):
+    """Rows of a warp each: with fewer of its threads' values than are picked, equal ones, masked ones, all or none."""
+    for dtype in (F16, F32):
+        x, tokens = _logits(50, V, dtype, V + top, V % 3)
+        x = x.clone()
+        x[::3] = torch.where(torch.rand((17, V), generator=torch.Generator().manual_seed(V)).cuda() < 1 / 64, x[::3], -INF)
+        x[1::6] = x[1::6].round()                  # a few dozen values, many times each
+        x[4] = 0.0
+        x[7] = torch.arange(V, device="cuda").to(dtype) / 8
+        x[10] = -x[7]
+        _check(x, tokens, top)

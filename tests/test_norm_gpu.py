@@ -193,3 +193,21 @@ def test_another_stream_and_a_captured_call():
         y2, _ = norm.rms_norm(x, w, residual=r)
     stream.synchronize()
     assert torch.equal(y2, want)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("M,K,pad", [(3, 8544, 128), (2, 8543, 0), (5, 13548, 5), (160, 4095, 1), (4, 2047, 0), (2, 16381, 7), (3, 40004, 4)])
+def test_wide_rows_at_any_alignment(M, K, pad, dtype):
+    """Shares of a row that end inside, at and behind its last 16 bytes, for weights of either size and alignment."""
+    from llm_accelerator_b200 import norm
+    for wtype, shift in ((dtype, 0), (F32, 1), (BF16, 1)):
+        x, r, w = _inputs(M, K, dtype, wtype, M + K, pad, True)
+        if shift:
+            w = torch.cat([w[:1], w])[1:]
+        h, y = _exact(x, r, w, 1e-5)
+        got, new = norm.rms_norm(x, w, 1e-5, residual=r)
+        _near(new, h, ULP, dtype)
+        _near(got, y, NORM, dtype)
+        q, scale, same = norm.rms_norm_i8(x, w, 1e-5, residual=r)
+        assert torch.equal(same, new)
+        _check_i8(q, scale, y, K)
