@@ -720,10 +720,13 @@ int launch_logprobs(const LpParams& p, cudaStream_t st) {
   while (2 << log_ctas <= kMostCtas && (int64_t(p.M) << (log_ctas + 1)) <= 3 * sms && pieces >> (log_ctas + 1) >= 4 * 256) ++log_ctas;
   if (log_ctas) return launch_rows<T, 256, true>(p, log_ctas, st);
   // A warp a row, which needs no barrier, for short rows: those of two groups of loads, and where there are rows for many
-  // warps an SM those of twelve.  Against four warps a row, microseconds with five tokens picked, 16-bit logits:
-  //   1000 x 1000  5.4 / 5.6   20000 x 1000  28 / 57   1000 x 8000  10.8 / 8.9   4000 x 12000  23 / 28
-  //   20000 x 12000  106 / 114   4000 x 32000  54 / 56   20000 x 32000  255 / 216   4096 x 50257  91 / 78
-  if (pieces <= 32 * 2 * kAtOnce || (pieces <= 32 * 12 * kAtOnce && p.M >= 8 * sms)) return launch_rows<T, 32, false>(p, 0, st);
+  // warps an SM those of twelve (five, where no tokens are picked) unless many are picked, for which four warps have the
+  // better bound.  Against four warps a row, microseconds with five tokens picked (with 20; with none), 16-bit logits:
+  //   1000 x 1000  5.4 / 5.6   20000 x 1000  28 / 57   2000 x 2600  7.7 / 10.4 (10.9 / 11.8; 5.4 / 6.4), masked rows
+  //   among them 9.2 / 11.3 (17.6 / 12.8)   1300 x 5000  9.6 / 9.0   4000 x 5000  16.8 / 20.4 (23.8 / 23.3; 14.3 / 14.1)
+  //   4000 x 9000  24.1 / 25.5 (33.9 / 29.3; 21.9 / 18.7)   20000 x 12000  106 / 114   4096 x 50257  91 / 78
+  const int most = p.M < 12 * sms || p.top > 8 ? 2 : p.top ? 12 : 5;
+  if (pieces <= 32 * most * kAtOnce) return launch_rows<T, 32, false>(p, 0, st);
   // Eight warps a row while those of four would not fill the SMs: 400 x 50257 in 14.3 against 18.8 us, 888 x 50257 in 22.1
   // against 23.4 (4096 rows 81 against 78).
   if (p.M <= 6 * sms && pieces >= 4 * 256) return launch_rows<T, 256, false>(p, 0, st);

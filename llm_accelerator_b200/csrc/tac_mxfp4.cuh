@@ -119,42 +119,47 @@ __device__ __forceinline__ uint32_t mx_pair(float lo, float hi) {
   }
 }
 
-// 16-bit results of 32 tokens (m ..) and a warp's 32 channels, in pairs of
-// channels: lanes exchange with their neighbours, and of two tokens the even
-// lanes store one's pairs and the odd lanes the other's.  With an odd N every
-// second row begins between two words: its pairs are those of an odd lane and
-// the next, its first and last channel go alone.  Exchanges go before the
-// stores, behind which each would wait.
-template <int YT, bool ODD>
-__device__ __forceinline__ void mx_store_pairs(const MxParams& p, const uint32_t (&v)[32], int m, int n, float bias,
-                                               uint32_t base_odd) {
-  const int lane = threadIdx.x & 31;
-  const uint32_t first = ODD ? (base_odd ^ uint32_t(m & 1)) : 0u;   // the token of a pair whose row is word-aligned here
-  const bool mine_first = (lane & 1) == 0;
-  const int tok = mine_first ? int(first) : int(first ^ 1u);
-  uint16_t* dst = static_cast<uint16_t*>(p.y) + int64_t(m + tok) * p.N + n - (mine_first || ODD ? 0 : 1);
-  uint16_t* edge = static_cast<uint16_t*>(p.y) + int64_t(m + int(first ^ 1u)) * p.N + n;
+// 16-bit results of 32 tokens (m ..) and a warp's 32 channels.  What bounds
+// these stores is the way out of the SM, in requests and in 32-byte sectors (1.4
+// cycles each): with an odd N a row's channels go one by one, 64 bytes in one
+// request, because pairs would leave the ends of every second row to requests
+// of their own (836 x 49977 x 160: 37 us, 45 in pairs).
+template <int YT>
+__device__ __forceinline__ void mx_store_singles(const MxParams& p, const uint32_t (&v)[32], int m, int n, float bias) {
+  uint16_t* dst = static_cast<uint16_t*>(p.y) + int64_t(m) * p.N + n;
+  const int left = p.M - m;
+  uint32_t two[16];
+#pragma unroll
+  for (int j = 0; j < 16; ++j) two[j] = mx_pair<YT>(__uint_as_float(v[2 * j]) + bias, __uint_as_float(v[2 * j + 1]) + bias);
+#pragma unroll
+  for (int j = 0; j < 32; ++j, dst += p.N)
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.gt.s32 p, %2, %3;\n\t@p st.global.b16 [%0], %1;\n\t}\n" ::"l"(dst),
+                 "h"(uint16_t(two[j >> 1] >> (16 * (j & 1)))), "r"(left), "r"(j)
+                 : "memory");
+}
+
+// With an even N in pairs of channels, half the stores (836 x 49978 x 160: 33 us):
+// lanes exchange with their neighbours, and of two tokens the even lanes store
+// one's pairs and the odd lanes the other's.  Exchanges go before the stores,
+// behind which each would wait.
+template <int YT>
+__device__ __forceinline__ void mx_store_pairs(const MxParams& p, const uint32_t (&v)[32], int m, int n, float bias) {
+  const int odd = threadIdx.x & 1;
+  uint16_t* dst = static_cast<uint16_t*>(p.y) + int64_t(m + odd) * p.N + n - odd;
   const int64_t step = 2 * int64_t(p.N);
-  const bool has_next = !ODD || lane != 31, is_edge = lane == 0 || lane == 31;
-  const uint32_t edge_shift = first ? 0 : 16;
-  const uint32_t sel = ODD ? (tok ? 0x7632 : 0x5410) : (mine_first ? 0x5410 : 0x3276);
+  const uint32_t sel = odd ? 0x3276 : 0x5410;
   uint32_t mine[16], other[16];      // the first token's result low, the second's high
 #pragma unroll
   for (int j = 0; j < 16; ++j) {
     mine[j] = mx_pair<YT>(__uint_as_float(v[2 * j]) + bias, __uint_as_float(v[2 * j + 1]) + bias);
-    other[j] = ODD ? __shfl_down_sync(0xffffffffu, mine[j], 1) : __shfl_xor_sync(0xffffffffu, mine[j], 1);
+    other[j] = __shfl_xor_sync(0xffffffffu, mine[j], 1);
   }
-  const int left = p.M - m - tok, left_edge = is_edge ? p.M - m - int(first ^ 1u) : 0, left_here = has_next ? left : 0;
+  const int left = p.M - m - odd;
 #pragma unroll
-  for (int j = 0; j < 16; ++j, dst += step, edge += step) {
+  for (int j = 0; j < 16; ++j, dst += step)
     asm volatile("{\n\t.reg .pred p;\n\tsetp.gt.s32 p, %2, %3;\n\t@p st.global.b32 [%0], %1;\n\t}\n" ::"l"(dst),
-                 "r"(__byte_perm(mine[j], other[j], sel)), "r"(left_here), "r"(2 * j)
+                 "r"(__byte_perm(mine[j], other[j], sel)), "r"(left), "r"(2 * j)
                  : "memory");
-    if constexpr (ODD)
-      asm volatile("{\n\t.reg .pred p;\n\tsetp.gt.s32 p, %2, %3;\n\t@p st.global.b16 [%0], %1;\n\t}\n" ::"l"(edge),
-                   "h"(uint16_t(mine[j] >> edge_shift)), "r"(left_edge), "r"(2 * j)
-                   : "memory");
-  }
 }
 
 // 32 tokens (m .. m + 31) of a warp's 32 consecutive channels (n its own); v the sums.
@@ -162,14 +167,14 @@ template <int YT>
 __device__ __forceinline__ void mx_store32(const MxParams& p, const uint32_t (&v)[32], int m, int n, float bias) {
   const int lane = threadIdx.x & 31;
   const bool all_channels = n - lane + 32 <= p.N, inside = all_channels && m + 32 <= p.M;
-  const uint32_t base_odd = uint32_t(reinterpret_cast<uintptr_t>(p.y) >> 1) & 1;
+  const bool odd = (p.N | int(reinterpret_cast<uintptr_t>(p.y) >> 1)) & 1;
   if (YT == 0 && inside) {
     float* dst = static_cast<float*>(p.y) + int64_t(m) * p.N + n;
 #pragma unroll
     for (int j = 0; j < 32; ++j, dst += p.N) *dst = __uint_as_float(v[j]) + bias;
-  } else if (YT != 0 && all_channels && ((p.N & 1) || !base_odd)) {
-    if (p.N & 1) mx_store_pairs<YT, true>(p, v, m, n, bias, base_odd);
-    else mx_store_pairs<YT, false>(p, v, m, n, bias, 0u);
+  } else if (YT != 0 && all_channels) {
+    if (odd) mx_store_singles<YT>(p, v, m, n, bias);
+    else mx_store_pairs<YT>(p, v, m, n, bias);
   } else {
 #pragma unroll
     for (int j = 0; j < 32; ++j)
