@@ -192,16 +192,45 @@ struct Vec<__nv_bfloat16> {
 // about a value that the largest may pass by kSlack (e^16 is no strain on
 // float32): they are rescaled a few times a row, not in every call.  A value of
 // -inf makes e^d d, and with it t, a NaN, and values whose c overflows an
-// infinity: then each difference is taken, and lifted, by itself.
+// infinity: then, and in the rest of the row, each difference is taken, and
+// lifted, by itself (2000 x 50257, one token in 64 unmasked in every third row:
+// 43 us, 56 while each group of a row was tried first).
 // Eight values cost about 36 instructions and eight exponentials (16 a clock and
 // SM): 46 us for 4096 x 50257, whose bytes take 63.
 constexpr float kSlack = 16.f;
+template <typename T>
+__device__ __forceinline__ void take_each(Sums& a, const uint4& u) {
+  constexpr int N = Vec<T>::kN;
+  float v[N];
+  Vec<T>::values(u, v);
+  const uint64_t minus_m = pair_of(-a.m, -a.m);
+  uint64_t s = 0, t = 0;
+#pragma unroll
+  for (int j = 0; j < N; j += 2) {
+    const float2 dd = of_pair(add2(pair_of(v[j], v[j + 1]), minus_m));
+    const float d0 = max_nan(dd.x, -200.f), d1 = max_nan(dd.y, -200.f);
+    const uint64_t e = pair_of(ex2(d0 * kLog2e), ex2(d1 * kLog2e));
+    s = add2(s, e);
+    t = fma2(e, pair_of(d0, d1), t);
+  }
+  const float2 ss = of_pair(s), tt = of_pair(t);
+  a.s += ss.x + ss.y;
+  a.t += tt.x + tt.y;
+}
 template <typename T, int NV, bool HELD>
-__device__ __forceinline__ float take(Sums& a, const uint4 (&u)[NV], const uint4* from, int apart) {
+__device__ __forceinline__ float take(Sums& a, const uint4 (&u)[NV], const uint4* from, int apart, bool& by_each) {
   constexpr int N = Vec<T>::kN;
   const float m = Vec<T>::template largest<NV>(u);
-  if (m == ninf()) return m;
+  if (m == ninf()) {
+    by_each = true;                              // a masked row: sooner than at its first value, which other lanes have elsewhere
+    return m;
+  }
   if (!(m <= a.m + kSlack)) about(a, max_nan(a.m, m));   // a NaN too
+  if (by_each) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) take_each<T>(a, u[i]);
+    return m;
+  }
   // y = x log2 e - c with c = m log2 e rounded, which the same correction for all values makes good
   const float c = a.m * kLog2e, over = fmaf(a.m, kLog2e, -c);
   const uint64_t minus_c = pair_of(-c, -c), log2e = pair_of(kLog2e, kLog2e);
@@ -226,17 +255,9 @@ __device__ __forceinline__ float take(Sums& a, const uint4 (&u)[NV], const uint4
     a.s = fmaf(s1, f, a.s);
     a.t = fmaf(fmaf(-over, s1, t1) * f, kLn2, a.t);
   } else {
+    by_each = true;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      float v[N];
-      Vec<T>::values(HELD ? u[i] : __ldg(from + i * apart), v);   // held, they cost the loop 16 registers
-#pragma unroll
-      for (int j = 0; j < N; ++j) {
-        const float d = max_nan(v[j] - a.m, -200.f), e = ex2(d * kLog2e);
-        a.s += e;
-        a.t = fmaf(e, d, a.t);
-      }
-    }
+    for (int i = 0; i < NV; ++i) take_each<T>(a, HELD ? u[i] : __ldg(from + i * apart));   // held, they cost the loop 16 registers
   }
   return m;
 }
@@ -581,6 +602,7 @@ __global__ void __launch_bounds__(NT, CLUSTER ? 4 : NT == 32 ? 32 : 1536 / NT) l
   if (const int64_t i = s.first + int64_t(s.c1) * N + threadIdx.x; i < s.e1) v1 = Vec<T>::one(s.row, i);
 
   Sums a{ninf(), 0.f, 0.f};
+  bool by_each = false;
   const uint4* pieces = reinterpret_cast<const uint4*>(static_cast<const T*>(s.row) + s.first);
   // stretches of 2^log_stretch pieces a thread, at most kSlots of them
   const int groups = ((s.c1 - s.c0 + NT - 1) / NT + kAtOnce - 1) / kAtOnce;
@@ -598,7 +620,7 @@ __global__ void __launch_bounds__(NT, CLUSTER ? 4 : NT == 32 ? 32 : 1536 / NT) l
     uint4 u[kAtOnce];
 #pragma unroll
     for (int i = 0; i < kAtOnce; ++i) u[i] = load_once(pieces + c + i * NT);
-    most = max_nan(most, take<T, kAtOnce, CLUSTER>(a, u, pieces + c, NT));
+    most = max_nan(most, take<T, kAtOnce, CLUSTER>(a, u, pieces + c, NT, by_each));
     if (single) {
 #pragma unroll
       for (int i = 0; i < kAtOnce; ++i) sm.largest[i * NT + threadIdx.x] = Vec<T>::template largest<1>({u[i]});
@@ -616,7 +638,7 @@ __global__ void __launch_bounds__(NT, CLUSTER ? 4 : NT == 32 ? 32 : 1536 / NT) l
     for (int i = 0; i < kAtOnce - 1; ++i) u[i][0] = c + i * NT < s.c1 ? load_once(pieces + c + i * NT) : Vec<T>::none();
 #pragma unroll
     for (int i = 0; i < kAtOnce - 1; ++i) {
-      const float of = c + i * NT < s.c1 ? take<T, 1, CLUSTER>(a, u[i], pieces + c + i * NT, 0) : ninf();
+      const float of = c + i * NT < s.c1 ? take<T, 1, CLUSTER>(a, u[i], pieces + c + i * NT, 0, by_each) : ninf();
       if (single && group == 0 && i < slots) sm.largest[i * NT + threadIdx.x] = of;
       most = max_nan(most, of);
     }
@@ -712,12 +734,21 @@ int launch_logprobs(const LpParams& p, cudaStream_t st) {
   if (!sms_of[dev]) {
     if (int e = status(cudaDeviceGetAttribute(&sms_of[dev], cudaDevAttrMultiProcessorCount, dev))) return e;
   }
-  // CTAs a row: up to eight of 256 threads while there are three an SM at most and each thread has four loads.  Picking
-  // tokens is slower in more CTAs: 64 x 50257 with twenty takes 8.3 us in four CTAs a row, 11.1 in eight; 148 rows take 9.4
-  // in two, 14.7 in four.
+  // CTAs a row, two, four or eight of 256 threads: while all run at once, four an SM, if each thread has 12 loads; with
+  // fewer, for which picking tokens in more CTAs costs more than it gives, two while there are three an SM, four while there
+  // are two and eight while there is one, of which not many pick.  Microseconds in one, two, four, eight of them, 16-bit logits, none / 32 picked:
+  //    20 x 50257     5.9 /  9.5    4.8 /  8.3    4.0 /  8.1    4.3 / 10.6
+  //    20 x 121000   11.3 / 15.1    7.4 / 11.3    5.3 /  9.3    4.7 / 11.1
+  //   105 x 50257     6.8 / 10.3    6.0 /  9.7    6.1 / 11.1    9.2 / 21.7
+  //   224 x 121000   20.6 / 25.1   15.9 / 21.0   17.4 / 26.9   24.0 / 43.7
+  //    41 x 243278   31.3 / 37.1   17.6 / 22.4   11.2 / 16.0    9.6 / 17.4
   const int sms = sms_of[dev], pieces = p.V / Vec<T>::kN;
+  const auto pays = [&](int log) {
+    const int64_t ctas = int64_t(p.M) << log, loads = (pieces >> log) / 256;
+    return loads >= 12 ? ctas <= 4 * sms : loads >= 4 && ctas <= (4 - log) * sms && (log < 3 || p.top <= 20);
+  };
   int log_ctas = 0;
-  while (2 << log_ctas <= kMostCtas && (int64_t(p.M) << (log_ctas + 1)) <= 3 * sms && pieces >> (log_ctas + 1) >= 4 * 256) ++log_ctas;
+  while (2 << log_ctas <= kMostCtas && pays(log_ctas + 1)) ++log_ctas;
   if (log_ctas) return launch_rows<T, 256, true>(p, log_ctas, st);
   // A warp a row, which needs no barrier, for short rows: those of two groups of loads, and where there are rows for many
   // warps an SM those of twelve (five, where no tokens are picked) unless many are picked, for which four warps have the
