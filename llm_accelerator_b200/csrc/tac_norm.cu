@@ -359,24 +359,17 @@ __global__ void __launch_bounds__(32 * kLongWarps, 2) norm_long_kernel(NormParam
 // As few warps a row as hold it in four loads a thread, of one, two, four,
 // eight and sixteen (with one, four and sixteen alone, rows whose threads have
 // two loads or fewer leave too little under way: 2784 x 6560 BF16 to INT8 takes
-// 26 us in eight warps, 39 in sixteen); float32 rows of any alignment in eight, with which more rows are under way on an SM (3184 x 4095
-// with a residual: 43 us, 51 with four; aligned 35), unless they take more than
-// 16 warps would have registers for.
+// 26 us in eight warps, 39 in sixteen).
 template <typename T, bool ANY, bool I8>
 int launch_rows(const NormParams& p, cudaStream_t st) {
-  constexpr bool kWide = ANY && sizeof(T) == 4;
-  constexpr int kLoads = kWide ? 8 : 4, kOf = kLoads * 16 / sizeof(T);
-  if (p.K <= 32 * kOf) return launch_behind(norm_kernel<T, ANY, I8, 1, kLoads>, (p.M + 3) / 4, 128, 0, st, p);
-  if (p.K <= 64 * kOf) return launch_behind(norm_kernel<T, ANY, I8, 2, kLoads>, p.M, 64, 0, st, p);
-  if (p.K <= 128 * kOf) return launch_behind(norm_kernel<T, ANY, I8, 4, kLoads>, p.M, 128, 0, st, p);
-  if (p.K <= 256 * kOf) return launch_behind(norm_kernel<T, ANY, I8, 8, kLoads>, p.M, 256, 0, st, p);
-  if constexpr (kWide) {
-    if (p.K <= 1024 * 16) return launch_behind(norm_kernel<T, ANY, I8, 32, 4>, p.M, 1024, 0, st, p);
-  } else {
-    if (p.K <= 512 * kOf) return launch_behind(norm_kernel<T, ANY, I8, 16, 4>, p.M, 512, 0, st, p);
-    if constexpr (sizeof(T) == 4) {
-      if (p.K <= 1024 * kOf) return launch_behind(norm_kernel<T, ANY, I8, 16, 8>, p.M, 512, 0, st, p);
-    }
+  constexpr int kOf = 64 / sizeof(T);            // values of four loads
+  if (p.K <= 32 * kOf) return launch_behind(norm_kernel<T, ANY, I8, 1, 4>, (p.M + 3) / 4, 128, 0, st, p);
+  if (p.K <= 64 * kOf) return launch_behind(norm_kernel<T, ANY, I8, 2, 4>, p.M, 64, 0, st, p);
+  if (p.K <= 128 * kOf) return launch_behind(norm_kernel<T, ANY, I8, 4, 4>, p.M, 128, 0, st, p);
+  if (p.K <= 256 * kOf) return launch_behind(norm_kernel<T, ANY, I8, 8, 4>, p.M, 256, 0, st, p);
+  if (p.K <= 512 * kOf) return launch_behind(norm_kernel<T, ANY, I8, 16, 4>, p.M, 512, 0, st, p);
+  if constexpr (sizeof(T) == 4) {                // as 16-bit rows, to 16384; eight loads and their shifts need too many registers
+    if (p.K <= 1024 * kOf) return launch_behind(norm_kernel<T, ANY, I8, ANY ? 32 : 16, ANY ? 4 : 8>, p.M, ANY ? 1024 : 512, 0, st, p);
   }
   return launch_behind(norm_long_kernel<T, I8>, p.M, 32 * kLongWarps, 0, st, p);
 }
