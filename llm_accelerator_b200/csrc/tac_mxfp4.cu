@@ -114,9 +114,12 @@ __global__ void __launch_bounds__(kQmThreads) mx_quant_kernel(const T* __restric
     *reinterpret_cast<uint32_t*>(scales + ((int64_t(tile) * k_stages + chunk) * 2 + (lane >> 4)) * 512 + r * 16 + (lane & 12)) = bytes;
 }
 
+int64_t quant_tasks(int M, int k_stages) { return (int64_t(M) + 127) / 128 * 32 * k_stages; }
+int64_t quant_ctas(int M, int k_stages) { return (quant_tasks(M, k_stages) + kQmThreads / 32 - 1) / (kQmThreads / 32); }
+
 int launch_quant(const void* X, int type, int64_t ldx, uint8_t* codes, uint8_t* scales, int M, int K, cudaStream_t st) {
   const int k_stages = int(mx_pieces(K) / 2);
-  const int64_t tasks = (int64_t(M) + 127) / 128 * 32 * k_stages, ctas = (tasks + kQmThreads / 32 - 1) / (kQmThreads / 32);
+  const int64_t tasks = quant_tasks(M, k_stages), ctas = quant_ctas(M, k_stages);
   if (tasks > 0x7fffffff) return TAC_E_ARGUMENT;             // rows of 4 TB
   const int vec = aligned(X, 16) && (M == 1 || (ldx * elem(type)) % 16 == 0);
   const auto go = [&](auto* x) {
@@ -332,8 +335,12 @@ int launch_pair(const MxOperands& o, MxParams p, int clusters, int tn, cudaStrea
     return TAC_E_CUDA;
   const int64_t tiles = int64_t(pp.w_tiles) * pp.t_tiles;
   if (tiles > (1 << 30)) return TAC_E_ARGUMENT;
+  // Behind the quantiser this kernel starts while that one runs, but not on an SM that holds two of its CTAs.  Where it has one
+  // for each SM at most, pairs without a tile keep the last call's SMs from being free, on which the quantiser's CTAs would
+  // gather: 300 x 9000 x 768 in 7.4 us, 9.4 without them.
+  const bool fill = p.after_rows && quant_ctas(p.M, p.k_stages) <= 2 * clusters && tiles * 2 > clusters;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(2 * int(std::min<int64_t>(tiles, clusters)));
+  cfg.gridDim = dim3(2 * int(fill ? clusters : std::min<int64_t>(tiles, clusters)));
   cfg.blockDim = dim3(MxPairCfg::kThreads);
   cfg.dynamicSmemBytes = MxPairCfg::kSmem;
   cfg.stream = st;
@@ -345,12 +352,14 @@ int launch_pair(const MxOperands& o, MxParams p, int clusters, int tn, cudaStrea
   return status(cudaLaunchKernelEx(&cfg, mx_pair_kernel<YT>, tw, ta, tws, tas, pp));
 }
 
-// Pairs from 65 tokens and an eighth of the pairs on; fewer tiles leave SMs
-// idle that share a tile's K.  Microseconds, pairs / split K:
-//   64 x 4096 x 4096    7.9 /  7.9   100 x 4096 x 4096    8.2 / 10.6   128 x 16384 x 4096  11.8 / 12.4
-//   20 x 50257 x 768    8.1 /  6.8   100 x 50257 x 768   10.6 / 13.6   200 x 1000 x 1000    6.5 /  9.2
-//   64 x 28672 x 1024   7.0 /  6.0   600 x 640 x 1000     5.5 /  5.4   130 x 700 x 8192    12.6 / 11.2
+// Pairs from 65 tokens on, unless K is long and there are tiles for fewer than
+// an eighth of the pairs: a stage costs a pair 0.23 us, sharing K 3 us.
+// Microseconds, pairs / split K:
+//   64 x 4096 x 4096    7.9 /  7.7   100 x 4096 x 4096    8.2 / 10.6   128 x 16384 x 4096  11.8 / 12.4
+//   20 x 50257 x 768    8.1 /  6.8   100 x 50257 x 768   10.6 / 13.6    85 x 250 x 2048     5.0 /  6.9
+//   85 x 250 x 4096     6.9 /  7.9   200 x 60 x 4096      6.7 /  8.7    85 x 640 x 8192    10.4 /  8.7
 // (M x N x K.)
+constexpr int kPairStages = 24;
 template <int YT>
 int pick_product(const MxOperands& o, const MxParams& p, cudaStream_t st) {
   int dev = 0;
@@ -358,7 +367,7 @@ int pick_product(const MxOperands& o, const MxParams& p, cudaStream_t st) {
   const int clusters = p.M > 64 ? pair_clusters<YT>(dev) : 0;
   if (clusters > 0) {
     const int tn = pair_tokens(p.M, p.N, clusters);
-    if (int64_t((p.N + 255) / 256) * ((p.M + tn - 1) / tn) * 8 >= clusters) return launch_pair<YT>(o, p, clusters, tn, st);
+    if (p.k_stages <= kPairStages || int64_t((p.N + 255) / 256) * ((p.M + tn - 1) / tn) * 8 >= clusters) return launch_pair<YT>(o, p, clusters, tn, st);
   }
   return launch_splitk<YT>(o, p, st);
 }
@@ -388,25 +397,31 @@ int run_product(const uint8_t* a_codes, const uint8_t* a_scales, const uint8_t* 
 
 // ---- few rows -------------------------------------------------------------------------------------------------------
 struct MxRowsShape {
-  int tn, split, per;        // tokens of the tile, CTAs that share a tile's stages, stages of a CTA at most
-  int64_t tiles;
+  int tn, split, per;        // tokens of a tile, CTAs that share a tile's stages, stages of a CTA at most
+  int64_t w_tiles, t_tiles;
 };
+// The largest tile of at most 64 rows of which each CTA quantises its part at once, if there is a CTA for each SM at most;
+// else tn is 0.  (More rows are faster in two launches: 300 x 768 x 768 in 5.5 us, 6.8 in one.)
 MxRowsShape rows_shape(int M, int N, int K, int sms) {
-  MxRowsShape r;
-  r.tn = M <= 16 ? 16 : M <= 32 ? 32 : 64;
-  r.tiles = (int64_t(N) + 127) / 128;
+  MxRowsShape r{};
+  if (M > 64) return r;
+  r.w_tiles = (int64_t(N) + 127) / 128;
   const int k_stages = int(mx_pieces(K) / 2);
-  r.split = splits(r.tiles, k_stages, r.tn, sms);
-  r.per = (k_stages + r.split - 1) / r.split;
+  for (int tn = M <= 16 ? 16 : M <= 32 ? 32 : 64; tn >= 16; tn /= 2) {
+    r.t_tiles = (M + tn - 1) / tn;
+    const int64_t tiles = r.w_tiles * r.t_tiles;
+    if (tiles > sms) break;
+    r.split = splits(tiles, k_stages, tn, sms);
+    r.per = (k_stages + r.split - 1) / r.split;
+    if (r.per * std::min(M, tn) * 32 <= 256 * kMxRowsHeld) {
+      r.tn = tn;
+      break;
+    }
+  }
   return r;
 }
 
-// One launch where a CTA's values are all in flight at once and there is a CTA for each SM at most.
-bool one_launch(int M, int N, int K, int sms) {
-  if (M > kMxRowsMost || !sms) return false;
-  const MxRowsShape r = rows_shape(M, N, K, sms);
-  return r.tiles <= sms && int64_t(r.per) * M * 32 <= 256 * kMxRowsHeld;
-}
+bool one_launch(int M, int N, int K, int sms) { return sms && rows_shape(M, N, K, sms).tn; }
 
 template <typename T, int YT>
 int launch_rows_as(MxRowsParams pp, const MxOperands& o, cudaStream_t st) {
@@ -427,7 +442,7 @@ int launch_rows_as(MxRowsParams pp, const MxOperands& o, cudaStream_t st) {
   CUtensorMap tw;
   if (!map_rows(&tw, o.b_codes, o.K, p.N, 128)) return TAC_E_CUDA;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(unsigned(r.tiles), 1, r.split);
+  cfg.gridDim = dim3(unsigned(r.w_tiles), unsigned(r.t_tiles), r.split);
   cfg.blockDim = dim3(kMxRowsThreads);
   cfg.dynamicSmemBytes = std::max(p.stages * sb + rows, part) + 1024;
   cfg.stream = st;

@@ -119,67 +119,64 @@ __device__ __forceinline__ uint32_t mx_pair(float lo, float hi) {
   }
 }
 
-// 16-bit results of 32 tokens (m ..) and a warp's 32 channels.  What bounds
-// these stores is the way out of the SM, in requests and in 32-byte sectors (1.4
-// cycles each): with an odd N a row's channels go one by one, 64 bytes in one
-// request, because pairs would leave the ends of every second row to requests
-// of their own (836 x 49977 x 160: 37 us, 45 in pairs).
+// Results of 32 tokens (m ..) and a warp's 32 channels, of which this lane has
+// one, where p.N has it.  What bounds these stores is the way out of the SM, in
+// requests and in 32-byte sectors (1.4 cycles each): with an odd N a row's
+// 16-bit channels go one by one, 64 bytes in one request, because pairs would
+// leave the ends of every second row to requests of their own (836 x 49977 x
+// 160: 37 us, 45 in pairs).
 template <int YT>
 __device__ __forceinline__ void mx_store_singles(const MxParams& p, const uint32_t (&v)[32], int m, int n, float bias) {
-  uint16_t* dst = static_cast<uint16_t*>(p.y) + int64_t(m) * p.N + n;
-  const int left = p.M - m;
-  uint32_t two[16];
+  const int left = n < p.N ? p.M - m : 0;
+  if constexpr (YT == 0) {
+    float* dst = static_cast<float*>(p.y) + int64_t(m) * p.N + n;
 #pragma unroll
-  for (int j = 0; j < 16; ++j) two[j] = mx_pair<YT>(__uint_as_float(v[2 * j]) + bias, __uint_as_float(v[2 * j + 1]) + bias);
+    for (int j = 0; j < 32; ++j, dst += p.N)
+      asm volatile("{\n\t.reg .pred p;\n\tsetp.gt.s32 p, %2, %3;\n\t@p st.global.f32 [%0], %1;\n\t}\n" ::"l"(dst),
+                   "f"(__uint_as_float(v[j]) + bias), "r"(left), "r"(j)
+                   : "memory");
+  } else {
+    uint16_t* dst = static_cast<uint16_t*>(p.y) + int64_t(m) * p.N + n;
+    uint32_t two = 0;
 #pragma unroll
-  for (int j = 0; j < 32; ++j, dst += p.N)
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.gt.s32 p, %2, %3;\n\t@p st.global.b16 [%0], %1;\n\t}\n" ::"l"(dst),
-                 "h"(uint16_t(two[j >> 1] >> (16 * (j & 1)))), "r"(left), "r"(j)
-                 : "memory");
+    for (int j = 0; j < 32; ++j, dst += p.N) {
+      two = j & 1 ? two >> 16 : mx_pair<YT>(__uint_as_float(v[j]) + bias, __uint_as_float(v[j + 1 < 32 ? j + 1 : j]) + bias);
+      asm volatile("{\n\t.reg .pred p;\n\tsetp.gt.s32 p, %2, %3;\n\t@p st.global.b16 [%0], %1;\n\t}\n" ::"l"(dst),
+                   "h"(uint16_t(two)), "r"(left), "r"(j)
+                   : "memory");
+    }
+  }
 }
 
 // With an even N in pairs of channels, half the stores (836 x 49978 x 160: 33 us):
-// lanes exchange with their neighbours, and of two tokens the even lanes store
-// one's pairs and the odd lanes the other's.  Exchanges go before the stores,
-// behind which each would wait.
+// of two tokens the even lanes store one's pairs and the odd lanes the other's,
+// and lanes exchange what their neighbours store, of four tokens at a time.
+// Exchanges go before the stores, behind which each would wait.
 template <int YT>
 __device__ __forceinline__ void mx_store_pairs(const MxParams& p, const uint32_t (&v)[32], int m, int n, float bias) {
   const int odd = threadIdx.x & 1;
   uint16_t* dst = static_cast<uint16_t*>(p.y) + int64_t(m + odd) * p.N + n - odd;
   const int64_t step = 2 * int64_t(p.N);
-  const uint32_t sel = odd ? 0x3276 : 0x5410;
-  uint32_t mine[16], other[16];      // the first token's result low, the second's high
+  const uint32_t give = odd ? 0x5410 : 0x7632, sel0 = odd ? 0x3254 : 0x5410, sel1 = odd ? 0x3276 : 0x7610;
+  uint32_t mine[16], other[8];       // the first token's result low, the second's high; the neighbour's of two pairs of tokens
 #pragma unroll
-  for (int j = 0; j < 16; ++j) {
-    mine[j] = mx_pair<YT>(__uint_as_float(v[2 * j]) + bias, __uint_as_float(v[2 * j + 1]) + bias);
-    other[j] = __shfl_xor_sync(0xffffffffu, mine[j], 1);
-  }
+  for (int j = 0; j < 16; ++j) mine[j] = mx_pair<YT>(__uint_as_float(v[2 * j]) + bias, __uint_as_float(v[2 * j + 1]) + bias);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) other[j] = __shfl_xor_sync(0xffffffffu, __byte_perm(mine[2 * j], mine[2 * j + 1], give), 1);
   const int left = p.M - m - odd;
 #pragma unroll
   for (int j = 0; j < 16; ++j, dst += step)
     asm volatile("{\n\t.reg .pred p;\n\tsetp.gt.s32 p, %2, %3;\n\t@p st.global.b32 [%0], %1;\n\t}\n" ::"l"(dst),
-                 "r"(__byte_perm(mine[j], other[j], sel)), "r"(left), "r"(2 * j)
+                 "r"(__byte_perm(mine[j], other[j >> 1], j & 1 ? sel1 : sel0)), "r"(left), "r"(2 * j)
                  : "memory");
 }
 
 // 32 tokens (m .. m + 31) of a warp's 32 consecutive channels (n its own); v the sums.
 template <int YT>
 __device__ __forceinline__ void mx_store32(const MxParams& p, const uint32_t (&v)[32], int m, int n, float bias) {
-  const int lane = threadIdx.x & 31;
-  const bool all_channels = n - lane + 32 <= p.N, inside = all_channels && m + 32 <= p.M;
-  const bool odd = (p.N | int(reinterpret_cast<uintptr_t>(p.y) >> 1)) & 1;
-  if (YT == 0 && inside) {
-    float* dst = static_cast<float*>(p.y) + int64_t(m) * p.N + n;
-#pragma unroll
-    for (int j = 0; j < 32; ++j, dst += p.N) *dst = __uint_as_float(v[j]) + bias;
-  } else if (YT != 0 && all_channels) {
-    if (odd) mx_store_singles<YT>(p, v, m, n, bias);
-    else mx_store_pairs<YT>(p, v, m, n, bias);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 32; ++j)
-      if (m + j < p.M && n < p.N) mx_st<YT>(p.y, int64_t(m + j) * p.N + n, __uint_as_float(v[j]) + bias);
-  }
+  const bool all_channels = n - int(threadIdx.x & 31) + 32 <= p.N;
+  if (YT != 0 && all_channels && ((p.N | int(reinterpret_cast<uintptr_t>(p.y) >> 1)) & 1) == 0) mx_store_pairs<YT>(p, v, m, n, bias);
+  else mx_store_singles<YT>(p, v, m, n, bias);
 }
 
 // ---- split-K over a cluster -----------------------------------------------------------------------------------------
@@ -211,6 +208,42 @@ __host__ __device__ constexpr int mx_sk_stage_bytes(int tn) { return kMxWBytes +
 // Partial sums of a split tile in shared memory: [128 channels][tn + 4], the padding against bank conflicts.
 __host__ __device__ constexpr int mx_sk_part_bytes(int tn) { return 128 * (tn + 4) * 4; }
 
+// CTA `rank`'s share of the tokens from the partial sums of NS CTAs, in the order of the ranks.  Eight reads of four tokens
+// are under way at once: one after the other, 16 waits for other CTAs' memory made a split of 128 tokens 4 us slower.
+template <int YT, int NS>
+__device__ __forceinline__ void mx_sum_parts(const MxParams& p, const float* mine, int n, int m0, int rank, float bias) {
+  constexpr int kAtOnce = 8 / NS;
+  const int per = max(4, p.tn / NS), first = rank * per, last = min(min(first + per, p.tn), p.M - m0);
+  uint32_t base[NS];
+#pragma unroll
+  for (int r = 0; r < NS; ++r) base[r] = sm100::mapa_shared(mine + first, r);
+  for (int c = first; c < last; c += 4 * kAtOnce) {
+    float4 v[kAtOnce][NS];
+#pragma unroll
+    for (int q = 0; q < kAtOnce; ++q)
+#pragma unroll
+      for (int r = 0; r < NS; ++r) {
+        v[q][r] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (c + 4 * q < last)
+          asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];\n"
+                       : "=f"(v[q][r].x), "=f"(v[q][r].y), "=f"(v[q][r].z), "=f"(v[q][r].w)
+                       : "r"(base[r] + (c - first + 4 * q) * 4)
+                       : "memory");
+      }
+#pragma unroll
+    for (int q = 0; q < kAtOnce; ++q) {
+      float acc[4] = {};
+#pragma unroll
+      for (int r = 0; r < NS; ++r) acc[0] += v[q][r].x, acc[1] += v[q][r].y, acc[2] += v[q][r].z, acc[3] += v[q][r].w;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int t = c + 4 * q + j;
+        if (t < last && n < p.N) mx_st<YT>(p.y, int64_t(m0 + t) * p.N + n, acc[j] + bias);
+      }
+    }
+  }
+}
+
 // The tile's results, or the CTA's partial sums to shared memory (over its stages: every copy and MMA has ended) and,
 // after the cluster's barrier, CTA r's share of the tokens from all partials.  All threads of the CTA.
 template <int YT>
@@ -241,35 +274,16 @@ __device__ __forceinline__ void mx_splitk_finish(const MxParams& p, uint8_t* sme
   }
   __syncwarp();
   sm100::cluster_sync();
-  const int per = max(4, p.tn / nsplit), first = rank * per;    // tokens of this CTA
-  if (epi && first < p.tn) {
-    uint32_t base[8];
-#pragma unroll
-    for (int r = 0; r < 8; ++r) base[r] = sm100::mapa_shared(mine + first, r < nsplit ? r : 0);
-    for (int k = 0; k < per; k += 4) {
-      if (m0 + first + k >= p.M) break;
-      float4 v[8];
-#pragma unroll
-      for (int r = 0; r < 8; ++r) {
-        v[r] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (r < nsplit)
-          asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];\n"
-                       : "=f"(v[r].x), "=f"(v[r].y), "=f"(v[r].z), "=f"(v[r].w)
-                       : "r"(base[r] + k * 4)
-                       : "memory");
-      }
-      float acc[4] = {};
-#pragma unroll
-      for (int r = 0; r < 8; ++r) acc[0] += v[r].x, acc[1] += v[r].y, acc[2] += v[r].z, acc[3] += v[r].w;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int m = m0 + first + k + j;
-        if (m < p.M && n < p.N) mx_st<YT>(p.y, int64_t(m) * p.N + n, acc[j] + bias);
-      }
-    }
+  if (epi) {
+    if (nsplit == 2) mx_sum_parts<YT, 2>(p, mine, n, m0, rank, bias);
+    else if (nsplit == 4) mx_sum_parts<YT, 4>(p, mine, n, m0, rank, bias);
+    else mx_sum_parts<YT, 8>(p, mine, n, m0, rank, bias);
   }
   __syncwarp();
-  sm100::cluster_sync();                         // no CTA leaves while another reads its partial sums
+  // No CTA leaves while another reads its partial sums.  Relaxed: what was read has been summed, and a release would wait for
+  // the stores of the results.
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;\n" ::: "memory");
+  sm100::cluster_wait();
 }
 
 // The four MMAs of a stage, and before them its scales' copies.  w_sf, a_sf: shared memory; sf: TMEM columns of the stage.
@@ -462,7 +476,7 @@ __device__ __forceinline__ uint32_t codes8(const float (&v)[8], uint32_t byte) {
 // four by four, each wait for memory cost 1.4 us.  Rows past M keep what was
 // there: a token's column of the result depends on no other.
 //   warp 0      weights, warp 1 MMAs, warps 2..9 rows, warps 2..5 epilogue.
-constexpr int kMxRowsThreads = 64 + 256, kMxRowsMost = 64, kMxRowsHeld = 8;
+constexpr int kMxRowsThreads = 64 + 256, kMxRowsHeld = 8;
 
 struct MxRowsParams {
   MxParams g;
@@ -477,7 +491,9 @@ __host__ __device__ constexpr int mx_rows_bytes(int tn) { return tn * 128 + kMxS
 
 template <typename T, int YT>
 __global__ void __launch_bounds__(kMxRowsThreads) mx_rows_kernel(const __grid_constant__ CUtensorMap tm_w, MxRowsParams pp) {
-  const MxParams& p = pp.g;
+  MxParams p = pp.g;
+  const int m0 = blockIdx.y * p.tn;
+  p.M = min(p.M, m0 + p.tn);                     // of this tile: a TMEM load may bring columns behind its own
   extern __shared__ uint8_t dyn_smem[];
   __shared__ __align__(8) uint64_t full_bar[kMxSkStages], empty_bar[kMxSkStages], rows_bar, acc_bar;
   __shared__ uint32_t tmem_base;
@@ -554,14 +570,15 @@ __global__ void __launch_bounds__(kMxRowsThreads) mx_rows_kernel(const __grid_co
     sm100::mbar_wait(&acc_bar, 0, p.fault, MX_TIMEOUT_DRAIN);
   } else {
     // items of eight values, 32 a row and stage: a warp's 32 are one row's of one stage, four lanes a block
-    const int t = threadIdx.x - 64, of_stage = p.M * 32, items = (kb1 - kb0) * of_stage;
-    const T* x = static_cast<const T*>(pp.x);
+    const int of_stage = (p.M - m0) * 32, items = (kb1 - kb0) * of_stage;
+    const T* x = static_cast<const T*>(pp.x) + m0 * pp.ldx;
+    const int t = threadIdx.x - 64;
     MxHeld<T> held[kMxRowsHeld];
     int stage[kMxRowsHeld], m[kMxRowsHeld];
 #pragma unroll
     for (int j = 0; j < kMxRowsHeld; ++j) {
       const int i = t + j * 256;
-      if (i - lane >= items) break;              // whole warps
+      if (i - lane >= items) break;            // whole warps
       stage[j] = i / of_stage, m[j] = (i - stage[j] * of_stage) >> 5;
       const int k = (kb0 + stage[j]) * kMxStageK + lane * 8;
       held[j].load(x + m[j] * pp.ldx + k, pp.K - k, pp.x_vec);
@@ -591,7 +608,7 @@ __global__ void __launch_bounds__(kMxRowsThreads) mx_rows_kernel(const __grid_co
     __syncwarp();
     sm100::tc_fence_after();
   }
-  mx_splitk_finish<YT>(p, smem, tmem, warp, row, n, 0, rank, nsplit, bias, acc_ok);
+  mx_splitk_finish<YT>(p, smem, tmem, warp, row, n, m0, rank, nsplit, bias, acc_ok);
   sm100::tc_fence_before();
   __syncthreads();
   if (warp == 1) {
@@ -617,9 +634,13 @@ __global__ void __launch_bounds__(kMxRowsThreads) mx_rows_kernel(const __grid_co
 // these copies, 322 without the operands' loads, 284 without both; 4096^3 takes
 // 31.5.  Copying a stage ahead of the MMAs made nothing faster, the last round's
 // tiles in halves 4096^3 by 1.5 %.
-//   Outputs wider than K is deep are bound by the epilogue (333 x 50257 x 768: 21
+//   Outputs wider than K is deep are bound by the epilogue (333 x 50257 x 768: 17
 // us, 12 without stores); 16-byte stores out of shared memory, for runs of 256
-// bytes, took as long for odd rows and 3.5 us longer for even ones.
+// bytes, took 20 and for even rows 3.5 us longer than pairs.
+//   88 registers, so that a CTA of the row quantiser fits beside it in each
+// quarter of the SM's (five warps' of the 18, two of its): this kernel is then in
+// place when the rows are quantised.  (333 x 50257 x 768 from BF16 rows: 18.1 us,
+// 20.7 with the 96 that the compiler would take.)
 struct MxPairCfg {
   static constexpr int kStages = 6;
   static constexpr int kStageBytes = 2 * 16384 + 3 * kMxSfBytes;
@@ -634,7 +655,7 @@ struct MxPairParams {
 };
 
 template <int YT>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MxPairCfg::kThreads, 1)
+__global__ void __cluster_dims__(2, 1, 1) __maxnreg__(88)
     mx_pair_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_a,
                    const __grid_constant__ CUtensorMap tm_ws, const __grid_constant__ CUtensorMap tm_as, MxPairParams pp) {
   constexpr int S = MxPairCfg::kStages;
