@@ -282,3 +282,25 @@ def test_products_at_the_ends_of_the_scales(M, one, other):
     # sums of a few multiples of one step are exact; below float32's normal numbers they may be taken for zero
     tiny = want.abs() < 2.0 ** -126
     assert torch.equal(got[~tiny], want[~tiny]) and bool((got[tiny].abs() < 2.0 ** -126).all())
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("M,N,K", [(133, 22, 512), (4700, 60, 100), (300, 9000, 768), (66, 31, 6144), (67, 33, 6400), (200, 60, 8192),
+                                   (85, 301, 7000), (40, 260, 2048), (64, 100, 4096), (50, 129, 1500), (33, 600, 3000)])
+def test_linear_calls_behind_each_other(M, N, K, dtype):
+    """Few channels, K shared by CTAs or by none, tiles of 16 to 256 tokens, pairs with and without a tile; each call starts
+    while the one before it ends."""
+    from llm_accelerator_b200 import mxfp4
+    g = torch.Generator().manual_seed(M + N)
+    x = torch.randn((M, K), generator=g).to(dtype)
+    b, sb = random_rows(N, K, 3, 115, 120)
+    bias = torch.randn(N, generator=g)
+    A, B = values(*quantise(x), K), values(b, sb, K)
+    room, want = _sum_room(A, B, K), A @ B.t() + bias.double()
+    room = room + 2.0 ** -23 * (want.abs() + bias.double().abs())
+    w, x, bias = on_device(b, sb, K), x.cuda(), bias.cuda()
+    flipped = x.flip(0).contiguous()
+    got = [mxfp4.linear(x if i % 2 == 0 else flipped, w, bias=bias) for i in range(6)]
+    _near(got[0], want, room, dtype)
+    for i, y in enumerate(got):
+        assert torch.equal(y if i % 2 == 0 else y.flip(0), got[0])
