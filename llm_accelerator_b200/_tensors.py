@@ -1,9 +1,21 @@
-"""What the torch front ends of the stand-alone kernels share: type codes and calls on a tensor's device."""
+"""What the torch front ends of the stand-alone kernels share: type codes, calls on a tensor's device, and ``front``, the
+C++ side of their usual calls, each of which gives None where Python has to look at the arguments."""
 from __future__ import annotations
+
+import ctypes as C
 
 import torch
 
 from . import _lib as L
+
+try:
+    from . import _front as front
+except ImportError as e:
+    raise ImportError("_front.so is not built for this torch; run `python -m llm_accelerator_b200.build` first") from e
+
+front.bind(*(C.cast(getattr(L.lib, "tac_" + name), C.c_void_p).value for name in (
+    "rms_norm", "rms_norm_i8", "dequantize_rows_i8", "mxfp4_quantize", "mxfp4_values", "mxfp4_gemm", "linear_mxfp4",
+    "linear_mxfp4_workspace_bytes", "token_logprobs")))
 
 TYPES = {torch.float32: L.TYPE_F32, torch.float16: L.TYPE_F16, torch.bfloat16: L.TYPE_BF16}
 _current = torch._C._cuda_getDevice

@@ -1,4 +1,4 @@
-"""Builds libtaccel_b200.so (sm_100a) in-tree with nvcc.
+"""Builds libtaccel_b200.so (sm_100a) in-tree with nvcc, and _front.so, the torch front ends' usual calls in C++.
 
 The library holds the host compiler (instruction stream -> device plan), the
 executor kernels and the stand-alone GEMM kernels.  It is built in the package
@@ -19,6 +19,8 @@ LIB = PKG / "libtaccel_b200.so"
 OBJDIR = PKG.parent / "_build"
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
+CXX = os.environ.get("CXX", "g++")
+FRONT, FRONT_SRC = PKG / "_front.so", CSRC / "tac_front.cc"
 FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", f"-I{INCLUDE}", f"-I{CSRC}"]
 
 
@@ -37,6 +39,33 @@ def up_to_date() -> bool:
     return all(p.stat().st_mtime <= t for p in _deps())
 
 
+def front_up_to_date() -> bool:
+    # of this torch: the module speaks to its C++ side
+    t = FRONT.stat().st_mtime if FRONT.exists() else 0
+    return all(p.stat().st_mtime <= t for p in (FRONT_SRC, INCLUDE / "taccel_b200.h", _torch_dir() / "version.py"))
+
+
+def _torch_dir() -> Path:
+    import torch
+    return Path(torch.__file__).resolve().parent
+
+
+def build_front() -> Path:
+    """Compile the extension module of the torch front ends, which calls the library by addresses."""
+    import sysconfig
+    t = _torch_dir()
+    tmp = FRONT.with_suffix(".so.tmp")
+    cmd = [CXX, "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-D_GLIBCXX_USE_CXX11_ABI=1", f"-I{INCLUDE}",
+           *(f"-isystem{p}" for p in (t / "include", t / "include/torch/csrc/api/include", "/usr/local/cuda/include",
+                                      sysconfig.get_path("include"))),
+           str(FRONT_SRC), "-o", str(tmp), f"-L{t / 'lib'}", "-ltorch_python", "-ltorch_cuda", "-ltorch_cpu", "-lc10_cuda", "-lc10"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"{CXX} failed for {FRONT_SRC.name}:\n{r.stdout}\n{r.stderr}")
+    os.replace(tmp, FRONT)
+    return FRONT
+
+
 def _compile(src: Path, verbose: bool) -> Path:
     obj = OBJDIR / (src.name + ".o")
     cmd = [NVCC, *ARCH, *FLAGS, "-c", str(src), "-o", str(obj)]
@@ -51,7 +80,9 @@ def _compile(src: Path, verbose: bool) -> Path:
 
 
 def build(force: bool = False, verbose: bool = False) -> Path:
-    """Compile every CUDA / C++ source for sm_100a and link the shared library."""
+    """Compile every CUDA / C++ source for sm_100a and link the shared library; and the front ends' module."""
+    if force or not front_up_to_date():
+        build_front()
     if not force and up_to_date():
         return LIB
     OBJDIR.mkdir(exist_ok=True)

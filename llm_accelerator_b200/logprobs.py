@@ -10,7 +10,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib as L
-from ._tensors import TYPES, call, empty, type_code
+from ._tensors import TYPES, call, empty, front, type_code
 
 _logprobs = L.lib.tac_token_logprobs
 _F32, _I32, _I64 = torch.float32, torch.int32, torch.int64
@@ -28,6 +28,9 @@ def token_logprobs(logits, tokens, top: int = 0):
     part in the entropy; where fewer than `top` are unmasked, masked ones follow with -inf.  A token outside [0, V) (the
     padding of a batch) has the log-probability NaN.  A row that is masked whole, or holds a NaN or +inf, gives NaN; its
     top tokens are still ordered, NaN before all numbers."""
+    result = front.token_logprobs(logits, tokens, top)
+    if result is not None:
+        return result
     xt, shape = TYPES.get(logits.dtype), logits.shape
     if xt is None:
         type_code(logits.dtype, "logits")

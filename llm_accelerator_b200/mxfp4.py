@@ -21,7 +21,7 @@ from functools import lru_cache
 import torch
 
 from . import _lib as L
-from ._tensors import TYPES, call, empty, type_code
+from ._tensors import TYPES, call, empty, front, type_code
 
 _U8, _F16, _F32 = torch.uint8, torch.float16, torch.float32
 _quantize, _values, _gemm, _linear = (L.lib.tac_mxfp4_quantize, L.lib.tac_mxfp4_values, L.lib.tac_mxfp4_gemm,
@@ -83,10 +83,13 @@ class Mxfp4:
 
     def values(self, dtype=_F32):
         """[rows, cols] that the codes stand for, rounded to `dtype`."""
+        M, K, dev = self.rows, self.cols, self._index
+        y = front.values(self._pointers, M, K, dev, dtype)
+        if y is not None:
+            return y
         yt = TYPES.get(dtype)
         if yt is None:
             type_code(dtype, "dtype")
-        M, K, dev = self.rows, self.cols, self._index
         y = empty((M, K), dtype, dev)
         if M:
             call("tac_mxfp4_values", _values, dev, *self._pointers, y.data_ptr(), yt, M, K)
@@ -115,8 +118,12 @@ def _rows(X):
 
 def quantize(X) -> Mxfp4:
     """X [M, K] (float32, float16 or bfloat16, contiguous rows at any row stride) in 4-bit form."""
-    xt, ldx, M, K, dev = _rows(X)
     q = Mxfp4.__new__(Mxfp4)
+    done = front.quantize(X)
+    if done is not None:
+        q.codes, q.scales, q.rows, q.cols, q._index, q._pointers = done
+        return q
+    xt, ldx, M, K, dev = _rows(X)
     q.rows, q.cols, q._index = M, K, dev
     tiles, groups = (M + 127) // 128, (K + 255) // 256 * 2
     q.codes = empty((M, (K + 31) // 32 * 16), _U8, dev)
@@ -152,6 +159,10 @@ def gemm(a: Mxfp4, b: Mxfp4, bias=None, out_dtype=None, out=None):
     if out_dtype is None:
         out_dtype = _F16 if out is None else out.dtype
     M, K, dev = a.rows, a.cols, a._index
+    if out is None and type(b) is Mxfp4:
+        y = front.gemm(a._pointers, M, K, dev, b._pointers, b.rows, b.cols, b._index, bias, out_dtype)
+        if y is not None:
+            return y
     out, yt, N, bp, bt = _result(b, M, K, dev, bias, out, out_dtype)
     if M and N:
         call("tac_mxfp4_gemm", _gemm, dev, *a._pointers, *b._pointers, bp, bt, out.data_ptr(), yt, M, N, K)
@@ -164,6 +175,10 @@ def linear(X, w: Mxfp4, bias=None, out=None, ws=None):
     X float32, float16 or bfloat16 with contiguous rows at any row stride.  ws: a ``linear_workspace`` to reuse across
     calls on one stream; by default a call allocates its own where it needs one.  A block of X with an infinity or a NaN
     gives a row of NaN."""
+    if out is None and ws is None and type(w) is Mxfp4:
+        y = front.linear(X, w._pointers, w.rows, w.cols, w._index, bias)
+        if y is not None:
+            return y
     xt, ldx, M, K, dev = _rows(X)
     out, yt, N, bp, bt = _result(w, M, K, dev, bias, out, X.dtype)
     if M and N:

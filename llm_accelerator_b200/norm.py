@@ -14,7 +14,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib as L
-from ._tensors import TYPES, call, empty, type_code
+from ._tensors import TYPES, call, empty, front, type_code
 
 _norm, _norm_i8 = L.lib.tac_rms_norm, L.lib.tac_rms_norm_i8
 _I8, _F32 = torch.int8, torch.float32
@@ -73,6 +73,10 @@ def rms_norm(x, weight, eps: float = 1e-6, residual=None, residual_out=None, out
     of any of these types.  residual_out: where h goes, by default a new tensor; it may be `residual` or x itself, but
     may not overlap them otherwise.  out: y's tensor, which may be x or the residual (of one row stride, K).  A row whose h^2 add up to more than float32 holds (values of 10^18) is zero; an
     infinity or a NaN makes NaN of its own place, a NaN of its whole row."""
+    if residual_out is None and out is None:
+        result = front.rms_norm(x, weight, eps, residual)
+        if result is not None:
+            return result
     dev, M, K, args, h = _args(x, weight, eps, residual, residual_out)
     if out is None:
         out = empty((M, K), x.dtype, dev)
@@ -90,6 +94,10 @@ def rms_norm_i8(x, weight, eps: float = 1e-6, residual=None, residual_out=None):
     scale, h).  t = max(max |y|, 1e-8), scale = t / 127, code = rint(y * (127 / t)) as in ``ptq.quantize_rows``; K_pad = K
     rounded up to 16, padding columns zero.  A row of y that holds an infinity or a NaN gets the scale NaN.
     ``ptq.dequantize_rows`` gives the values back."""
+    if residual_out is None:
+        result = front.rms_norm_i8(x, weight, eps, residual)
+        if result is not None:
+            return result
     dev, M, K, args, h = _args(x, weight, eps, residual, residual_out)
     q, scale = empty((M, (K + 15) // 16 * 16), _I8, dev), empty((M,), _F32, dev)
     if M:

@@ -25,7 +25,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib as L
-from ._tensors import TYPES, call, empty, type_code
+from ._tensors import TYPES, call, empty, front, type_code
 
 _dequantize = L.lib.tac_dequantize_rows_i8
 
@@ -91,6 +91,9 @@ def dequantize_rows(q, scale, K=None, dtype=torch.float32):
     """[M, K] q[m, k] * scale[m], rounded to `dtype` (float32, float16 or bfloat16): the values that the rows of
     ``quantize_rows`` or ``norm.rms_norm_i8`` stand for.  q int8 [M, K_pad], scale float32 [M]; K, by default all
     columns, leaves out the padding ones.  No gradient flows through the call."""
+    y = front.dequantize_rows(q, scale, K, dtype)
+    if y is not None:
+        return y
     yt = TYPES.get(dtype)
     if yt is None:
         type_code(dtype, "dtype")
