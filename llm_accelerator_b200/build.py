@@ -53,9 +53,11 @@ def _torch_dir() -> Path:
 def build_front() -> Path:
     """Compile the extension module of the torch front ends, which calls the library by addresses."""
     import sysconfig
-    t = _torch_dir()
+
+    import torch
+    t, abi = _torch_dir(), int(torch.compiled_with_cxx11_abi())
     tmp = FRONT.with_suffix(".so.tmp")
-    cmd = [CXX, "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-D_GLIBCXX_USE_CXX11_ABI=1", f"-I{INCLUDE}",
+    cmd = [CXX, "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", f"-D_GLIBCXX_USE_CXX11_ABI={abi}", f"-I{INCLUDE}",
            *(f"-isystem{p}" for p in (t / "include", t / "include/torch/csrc/api/include", "/usr/local/cuda/include",
                                       sysconfig.get_path("include"))),
            str(FRONT_SRC), "-o", str(tmp), f"-L{t / 'lib'}", "-ltorch_python", "-ltorch_cuda", "-ltorch_cpu", "-lc10_cuda", "-lc10"]

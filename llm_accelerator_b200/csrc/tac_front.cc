@@ -86,14 +86,15 @@ at::Tensor empty(at::IntArrayRef sizes, at::ScalarType type, int64_t dev) {
 }
 void* stream(int64_t dev) { return c10::cuda::getCurrentCUDAStream(c10::DeviceIndex(dev)).stream(); }
 
-// The launch without the interpreter's lock.
+// The launch without the interpreter's lock, which an exception (a tensor without memory) takes back too.
+struct Unlocked {
+  PyThreadState* const state = PyEval_SaveThread();
+  ~Unlocked() { PyEval_RestoreThread(state); }
+};
 template <typename F>
 bool launched(F f) {
-  int status;
-  Py_BEGIN_ALLOW_THREADS
-  status = f();
-  Py_END_ALLOW_THREADS
-  return status == 0;
+  Unlocked u;
+  return f() == 0;
 }
 
 template <typename... T>

@@ -338,7 +338,7 @@ __device__ __forceinline__ uint32_t reached_by(int k, int n, F key) {
     if (count >= k) least = t;
     if (count == k) break;
   }
-  return least;
+  return least & 0x80000000u ? least : least | ((1u << kLow) - 1);      // of values below 0 those bits are set
 }
 
 // Places the n entries of `from` (16-byte aligned) that order among the first k into list[0 .. k).
@@ -736,7 +736,8 @@ int launch_logprobs(const LpParams& p, cudaStream_t st) {
   }
   // CTAs a row, two, four or eight of 256 threads: while all run at once, four an SM, if each thread has 12 loads; with
   // fewer, for which picking tokens in more CTAs costs more than it gives, two while there are three an SM, four while there
-  // are two and eight while there is one, of which not many pick.  Microseconds in one, two, four, eight of them, 16-bit logits, none / 32 picked:
+  // are two and eight while there is one and no more than 20 are picked.  Microseconds in one, two, four, eight of them, 16-bit
+  // logits, none / 32 picked:
   //    20 x 50257     5.9 /  9.5    4.8 /  8.3    4.0 /  8.1    4.3 / 10.6
   //    20 x 121000   11.3 / 15.1    7.4 / 11.3    5.3 /  9.3    4.7 / 11.1
   //   105 x 50257     6.8 / 10.3    6.0 /  9.7    6.1 / 11.1    9.2 / 21.7

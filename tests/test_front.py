@@ -70,6 +70,22 @@ def test_usual_calls_are_answered_alike(M, K, pad, dtype, monkeypatch):
 
 
 @pytest.mark.gpu
+def test_tensors_without_memory_and_threads():
+    from concurrent.futures import ThreadPoolExecutor
+
+    from llm_accelerator_b200 import norm
+    from llm_accelerator_b200.errors import EngineError
+    w, freed = torch.ones(64, device="cuda"), torch.ones((4, 64), device="cuda")
+    freed.untyped_storage().resize_(0)                 # a null address, which the library refuses
+    with pytest.raises(EngineError):
+        norm.rms_norm(freed, w)
+    x = torch.randn((4, 64), generator=torch.Generator().manual_seed(1)).cuda()
+    want = norm.rms_norm(x, w)
+    with ThreadPoolExecutor(4) as pool:                # the interpreter's lock has been taken back
+        assert all(torch.equal(y, want) for y in pool.map(lambda _: norm.rms_norm(x, w), range(200)))
+
+
+@pytest.mark.gpu
 def test_refusals_are_those_of_python():
     from llm_accelerator_b200 import logprobs, mxfp4, norm, ptq
     x, w = torch.ones((4, 64), dtype=F16, device="cuda"), torch.ones(64, device="cuda")

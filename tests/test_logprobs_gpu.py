@@ -263,3 +263,13 @@ def test_many_of_short_rows(V, top):
         x[7] = torch.arange(V, device="cuda").to(dtype) / 8
         x[10] = -x[7]
         _check(x, tokens, top)
+
+
+@pytest.mark.parametrize("V", [200, 1000, 5000])
+def test_equal_logits_below_zero(V):
+    """More of them than a share's list has places for; some rows with a few above and below."""
+    for dtype in (F16, BF16, F32):
+        x = torch.full((1800, V), -1.5, dtype=dtype, device="cuda")
+        x[1::2, 3:V:7] = -2.5
+        x[::5, 11:V:97] = -0.5
+        _check(x, torch.arange(1800, device="cuda") % V, 32)
