@@ -273,3 +273,10 @@ def test_equal_logits_below_zero(V):
         x[1::2, 3:V:7] = -2.5
         x[::5, 11:V:97] = -0.5
         _check(x, torch.arange(1800, device="cuda") % V, 32)
+
+
+def test_rows_of_two_ctas_each():
+    """More rows than SMs, long ones."""
+    x, tokens = _logits(500, 100003, F16, 5, 1)
+    x[::3, ::2] = -INF
+    _check(x, tokens, 20)

@@ -36,7 +36,7 @@ def _near(got, want, rel, dtype):
     assert bool((d <= room).all()), float((d / room).max())
 
 
-# one warp, four and sixteen a row; single values for odd widths, unaligned rows; too long for registers
+# one warp to sixteen a row; rows that begin and end anywhere; too long for registers
 SHAPES = [(1, 1, 0), (3, 7, 0), (5, 32, 0), (4, 512, 0), (7, 1024, 8), (9, 1032, 0), (33, 4096, 0), (6, 4096, 5),
           (3, 8192, 0), (2, 16384, 16), (5, 1000, 3), (4, 4097, 0), (2, 16383, 0), (2, 20001, 0), (300, 768, 0)]
 
