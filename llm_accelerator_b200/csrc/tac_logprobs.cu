@@ -191,13 +191,15 @@ struct Vec<__nv_bfloat16> {
 // largest of them.  The sums stay
 // about a value that the largest may pass by kSlack (e^16 is no strain on
 // float32): they are rescaled a few times a row, not in every call.  A value of
-// -inf makes e^d d, and with it t, a NaN, and values whose c overflows an
-// infinity: then, and in the rest of the row, each difference is taken, and
-// lifted, by itself (2000 x 50257, one token in 64 unmasked in every third row:
-// 43 us, 56 while each group of a row was tried first).
+// -inf makes e^d d, and with it t, a NaN; and c is rounded by half its last
+// place, which all terms' exponents share and e^-over makes good while that is
+// small (below 2^24 one half at most; from 2^31 on it can pass all exponents
+// that float32 has).  Otherwise, and in the rest of the row, each difference is
+// taken, and lifted, by itself (2000 x 50257, one token in 64 unmasked in every
+// third row: 43 us, 56 while each group of a row was tried first).
 // Eight values cost about 36 instructions and eight exponentials (16 a clock and
 // SM): 46 us for 4096 x 50257, whose bytes take 63.
-constexpr float kSlack = 16.f;
+constexpr float kSlack = 16.f, kLargest = 16777216.f;
 template <typename T>
 __device__ __forceinline__ void take_each(Sums& a, const uint4& u) {
   constexpr int N = Vec<T>::kN;
@@ -250,7 +252,7 @@ __device__ __forceinline__ float take(Sums& a, const uint4 (&u)[NV], const uint4
   }
   const float2 ss = of_pair(s), tt = of_pair(t);
   const float s1 = ss.x + ss.y, t1 = tt.x + tt.y;
-  if (fabsf(t1) < __uint_as_float(0x7f800000u)) {
+  if (fabsf(t1) < __uint_as_float(0x7f800000u) && fabsf(c) < kLargest) {
     const float f = ex2(-over);
     a.s = fmaf(s1, f, a.s);
     a.t = fmaf(fmaf(-over, s1, t1) * f, kLn2, a.t);
