@@ -111,13 +111,37 @@ bool number(PyObject* o, int64_t* v) {
   *v = PyLong_AsLongLongAndOverflow(o, &overflow);
   return !overflow;
 }
-// The two addresses of 4-bit rows.
-bool pointers(PyObject* o, const uint8_t** codes, const uint8_t** scales) {
-  if (!PyTuple_CheckExact(o) || PyTuple_GET_SIZE(o) != 2) return false;
-  *codes = static_cast<const uint8_t*>(PyLong_AsVoidPtr(PyTuple_GET_ITEM(o, 0)));
-  *scales = static_cast<const uint8_t*>(PyLong_AsVoidPtr(PyTuple_GET_ITEM(o, 1)));
-  return *codes && *scales;
-}
+// 4-bit rows on device `dev`, of four arguments: their codes and scales, rows, columns, device.  Codes and scales are two
+// tensors, which have rows and device themselves (then None), or their addresses.
+struct Rows4 {
+  const uint8_t *codes = nullptr, *scales = nullptr;
+  int64_t rows = 0, cols = 0;
+  bool of(PyObject* const* a, int64_t dev) {
+    if (dev < 0 || !PyTuple_CheckExact(a[0]) || PyTuple_GET_SIZE(a[0]) != 2 || !number(a[2], &cols) || cols <= 0 || cols > INT_MAX)
+      return false;
+    PyObject *c = PyTuple_GET_ITEM(a[0], 0), *s = PyTuple_GET_ITEM(a[0], 1);
+    if (a[1] == Py_None && a[3] == Py_None) {
+      const at::Tensor *ct = tensor(c, dev), *st = tensor(s, dev);
+      if (!ct || !st || ct->scalar_type() != at::kByte || st->scalar_type() != at::kByte || ct->dim() != 2 ||
+          !ct->is_contiguous() || !st->is_contiguous() || ct->size(1) != (cols + 31) / 32 * 16)
+        return false;
+      rows = ct->size(0);
+      const int64_t shape[] = {(rows + 127) / 128, (cols + 255) / 256 * 2, 32, 4, 4};
+      if (st->sizes() != at::IntArrayRef(shape)) return false;
+      codes = static_cast<const uint8_t*>(ct->const_data_ptr());
+      scales = static_cast<const uint8_t*>(st->const_data_ptr());
+      if ((reinterpret_cast<uintptr_t>(codes) | reinterpret_cast<uintptr_t>(scales)) & 15) return false;
+    } else {
+      int64_t at = -1;
+      if (!PyLong_CheckExact(c) || !PyLong_CheckExact(s) || !number(a[1], &rows) || !number(a[3], &at) || at != dev) return false;
+      codes = static_cast<const uint8_t*>(PyLong_AsVoidPtr(c));
+      scales = static_cast<const uint8_t*>(PyLong_AsVoidPtr(s));
+    }
+    return codes && scales && rows > 0 && rows <= INT_MAX;
+  }
+  // device_of their tensors
+  static int64_t device(PyObject* o) { return PyTuple_CheckExact(o) && PyTuple_GET_SIZE(o) == 2 ? device_of(PyTuple_GET_ITEM(o, 0)) : -1; }
+};
 
 struct NormCall {
   Rows x, r;
@@ -192,7 +216,7 @@ PyObject* dequantize_rows(PyObject*, PyObject* const* a, Py_ssize_t n) {      //
   END_HANDLE_TH_ERRORS
 }
 
-PyObject* quantize(PyObject*, PyObject* const* a, Py_ssize_t n) {             // X; (codes, scales, M, K, device, addresses)
+PyObject* quantize(PyObject*, PyObject* const* a, Py_ssize_t n) {             // X; (codes, scales, K)
   HANDLE_TH_ERRORS
   Rows x;
   if (n != 1) Py_RETURN_NONE;
@@ -203,69 +227,61 @@ PyObject* quantize(PyObject*, PyObject* const* a, Py_ssize_t n) {             //
   uint8_t *c = static_cast<uint8_t*>(codes.data_ptr()), *s = static_cast<uint8_t*>(scales.data_ptr());
   const auto run = [&] { return lib.quantize(x.t->const_data_ptr(), x.type, x.ld, c, s, x.M, x.K, stream(dev)); };
   if (!launched(run)) Py_RETURN_NONE;
-  return Py_BuildValue("(NNiiL(KK))", THPVariable_Wrap(codes), THPVariable_Wrap(scales), x.M, x.K, static_cast<long long>(dev),
-                       static_cast<unsigned long long>(reinterpret_cast<uintptr_t>(c)),
-                       static_cast<unsigned long long>(reinterpret_cast<uintptr_t>(s)));
+  return Py_BuildValue("(NNi)", THPVariable_Wrap(codes), THPVariable_Wrap(scales), x.K);
   END_HANDLE_TH_ERRORS
 }
 
-// rows, columns and device of 4-bit rows
-bool sizes(PyObject* const* a, int64_t* rows, int64_t* cols, int64_t* dev) {
-  return number(a[0], rows) && number(a[1], cols) && number(a[2], dev) && *rows > 0 && *rows <= INT_MAX && *cols > 0 &&
-         *cols <= INT_MAX && *dev >= 0;
-}
-
-PyObject* values(PyObject*, PyObject* const* a, Py_ssize_t n) {               // addresses, rows, columns, device, dtype
+PyObject* values(PyObject*, PyObject* const* a, Py_ssize_t n) {               // 4-bit rows, dtype
   HANDLE_TH_ERRORS
-  const uint8_t *c, *s;
-  int64_t M, K, dev;
-  if (n != 5 || !pointers(a[0], &c, &s) || !sizes(a + 1, &M, &K, &dev) || dev != c10::cuda::current_device() || !THPDtype_Check(a[4]))
-    Py_RETURN_NONE;
+  Rows4 x;
+  if (n != 5) Py_RETURN_NONE;
+  const int64_t dev = Rows4::device(a[0]);
+  if (!x.of(a, dev) || !THPDtype_Check(a[4])) Py_RETURN_NONE;
   const at::ScalarType out = reinterpret_cast<THPDtype*>(a[4])->scalar_type;
   if (type_of(out) < 0) Py_RETURN_NONE;
-  const at::Tensor y = empty({M, K}, out, dev);
-  const auto run = [&] { return lib.values(c, s, y.data_ptr(), type_of(out), int(M), int(K), stream(dev)); };
+  const at::Tensor y = empty({x.rows, x.cols}, out, dev);
+  const auto run = [&] { return lib.values(x.codes, x.scales, y.data_ptr(), type_of(out), int(x.rows), int(x.cols), stream(dev)); };
   if (!launched(run)) Py_RETURN_NONE;
   return THPVariable_Wrap(y);
   END_HANDLE_TH_ERRORS
 }
 
-PyObject* gemm(PyObject*, PyObject* const* a, Py_ssize_t n) {    // addresses, rows, columns, device of both; bias, dtype
+PyObject* gemm(PyObject*, PyObject* const* args, Py_ssize_t n) {              // 4-bit rows twice, bias, dtype
   HANDLE_TH_ERRORS
-  const uint8_t *ac, *as, *bc, *bs;
-  int64_t M, K, N, Kb, dev, other;
+  Rows4 a, b;
   Vector bias;
-  if (n != 10 || !pointers(a[0], &ac, &as) || !sizes(a + 1, &M, &K, &dev) || !pointers(a[4], &bc, &bs) ||
-      !sizes(a + 5, &N, &Kb, &other) || K != Kb || dev != other || dev != c10::cuda::current_device() || !bias.of(a[8], N, dev) || !THPDtype_Check(a[9]))
+  if (n != 10) Py_RETURN_NONE;
+  const int64_t dev = Rows4::device(args[0]);
+  if (!a.of(args, dev) || !b.of(args + 4, dev) || a.cols != b.cols || !bias.of(args[8], b.rows, dev) || !THPDtype_Check(args[9]))
     Py_RETURN_NONE;
-  const at::ScalarType out = reinterpret_cast<THPDtype*>(a[9])->scalar_type;
+  const at::ScalarType out = reinterpret_cast<THPDtype*>(args[9])->scalar_type;
   if (type_of(out) < 0) Py_RETURN_NONE;
-  const at::Tensor y = empty({M, N}, out, dev);
+  const at::Tensor y = empty({a.rows, b.rows}, out, dev);
   const auto run = [&] {
-    return lib.gemm(ac, as, bc, bs, bias.p, bias.type, y.data_ptr(), type_of(out), int(M), int(N), int(K), stream(dev));
+    return lib.gemm(a.codes, a.scales, b.codes, b.scales, bias.p, bias.type, y.data_ptr(), type_of(out), int(a.rows), int(b.rows),
+                    int(a.cols), stream(dev));
   };
   if (!launched(run)) Py_RETURN_NONE;
   return THPVariable_Wrap(y);
   END_HANDLE_TH_ERRORS
 }
 
-PyObject* linear(PyObject*, PyObject* const* a, Py_ssize_t n) {               // X; addresses, rows, columns, device; bias
+PyObject* linear(PyObject*, PyObject* const* a, Py_ssize_t n) {               // X; 4-bit rows; bias
   HANDLE_TH_ERRORS
-  const uint8_t *c, *s;
-  int64_t N, K, other;
+  Rows4 w;
   Rows x;
   Vector bias;
   if (n != 6) Py_RETURN_NONE;
   const int64_t dev = device_of(a[0]);
-  if (!x.of(a[0], dev) || !pointers(a[1], &c, &s) || !sizes(a + 2, &N, &K, &other) || K != x.K || other != dev || !bias.of(a[5], N, dev))
-    Py_RETURN_NONE;
+  if (!x.of(a[0], dev) || !w.of(a + 1, dev) || w.cols != x.K || !bias.of(a[5], w.rows, dev)) Py_RETURN_NONE;
+  const int N = int(w.rows);
   const at::Tensor y = empty({x.M, N}, x.t->scalar_type(), dev);
-  const int64_t bytes = int64_t(lib.linear_bytes(x.M, int(N), x.K));
+  const int64_t bytes = int64_t(lib.linear_bytes(x.M, N, x.K));
   at::Tensor ws;
   if (bytes) ws = empty({bytes}, at::kByte, dev);
   const auto run = [&] {
-    return lib.linear(x.t->const_data_ptr(), x.type, x.ld, c, s, bias.p, bias.type, y.data_ptr(), x.type,
-                      bytes ? ws.data_ptr() : nullptr, uint64_t(bytes), x.M, int(N), x.K, stream(dev));
+    return lib.linear(x.t->const_data_ptr(), x.type, x.ld, w.codes, w.scales, bias.p, bias.type, y.data_ptr(), x.type,
+                      bytes ? ws.data_ptr() : nullptr, uint64_t(bytes), x.M, N, x.K, stream(dev));
   };
   if (!launched(run)) Py_RETURN_NONE;
   return THPVariable_Wrap(y);

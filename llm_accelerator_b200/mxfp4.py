@@ -34,32 +34,48 @@ def _scale_shape(rows: int, cols: int):
     return -(-rows // 128), -(-cols // 256) * 2, 32, 4, 4
 
 
+def _check_tensors(codes, scales, cols: int):
+    if codes.dtype is not _U8 or scales.dtype is not _U8:
+        raise TypeError("codes and scales must be uint8")
+    shape = codes.shape
+    if len(shape) != 2 or cols <= 0 or shape[1] != (cols + 31) // 32 * 16:
+        raise ValueError(f"codes of {cols} columns must be [rows, {(cols + 31) // 32 * 16}], got {tuple(shape)}")
+    if scales.shape != _scale_shape(shape[0], cols):
+        raise ValueError(f"scales must be {_scale_shape(shape[0], cols)}, got {tuple(scales.shape)}")
+    if not (codes.is_contiguous() and scales.is_contiguous()):
+        raise ValueError("codes and scales must be contiguous")
+    dev = codes.get_device()
+    if dev < 0 or scales.get_device() != dev:
+        raise ValueError("codes and scales must be on one CUDA device")
+    if (codes.data_ptr() | scales.data_ptr()) & 15:
+        raise ValueError("codes and scales must begin on 16-byte boundaries")
+
+
 class Mxfp4:
     """`rows` rows of `cols` values: codes uint8 [rows, 16 blocks] (value 2j in the low, 2j + 1 in the high half of byte j),
     scales uint8 (the bytes e + 127, 255 for NaN) as the tensor cores take them.  ``from_tensors`` takes scale bytes
-    [rows, blocks] and ``scale_bytes`` gives them back; blocks = cols / 32 rounded up."""
+    [rows, blocks] and ``scale_bytes`` gives them back; blocks = cols / 32 rounded up.  Every call takes the tensors that
+    codes and scales are then, so that a copy, a loaded one or one that was given other tensors works on its own."""
 
     def __init__(self, codes, scales, cols: int):
-        if codes.dtype is not _U8 or scales.dtype is not _U8:
-            raise TypeError("codes and scales must be uint8")
-        shape = codes.shape
-        if len(shape) != 2 or cols <= 0 or shape[1] != (cols + 31) // 32 * 16:
-            raise ValueError(f"codes of {cols} columns must be [rows, {(cols + 31) // 32 * 16}], got {tuple(shape)}")
-        if scales.shape != _scale_shape(shape[0], cols):
-            raise ValueError(f"scales must be {_scale_shape(shape[0], cols)}, got {tuple(scales.shape)}")
-        if not (codes.is_contiguous() and scales.is_contiguous()):
-            raise ValueError("codes and scales must be contiguous")
-        dev = codes.get_device()
-        if dev < 0 or scales.get_device() != dev:
-            raise ValueError("codes and scales must be on one CUDA device")
-        if (codes.data_ptr() | scales.data_ptr()) & 15:
-            raise ValueError("codes and scales must begin on 16-byte boundaries")
-        self.codes, self.scales, self.rows, self.cols, self._index = codes, scales, shape[0], cols, dev
-        self._pointers = codes.data_ptr(), scales.data_ptr()
+        _check_tensors(codes, scales, cols)
+        self.codes, self.scales, self.cols = codes, scales, cols
+
+    @property
+    def rows(self) -> int:
+        return self.codes.shape[0]
 
     @property
     def device(self):
         return self.codes.device
+
+    @property
+    def _index(self) -> int:
+        return self.codes.get_device()
+
+    @property
+    def _pointers(self):
+        return self.codes.data_ptr(), self.scales.data_ptr()
 
     @classmethod
     def from_tensors(cls, codes, scale_bytes, cols: int) -> "Mxfp4":
@@ -83,10 +99,11 @@ class Mxfp4:
 
     def values(self, dtype=_F32):
         """[rows, cols] that the codes stand for, rounded to `dtype`."""
-        M, K, dev = self.rows, self.cols, self._index
-        y = front.values(self._pointers, M, K, dev, dtype)
+        y = front.values((self.codes, self.scales), None, self.cols, None, dtype)
         if y is not None:
             return y
+        _check_tensors(self.codes, self.scales, self.cols)
+        M, K, dev = self.rows, self.cols, self._index
         yt = TYPES.get(dtype)
         if yt is None:
             type_code(dtype, "dtype")
@@ -121,21 +138,21 @@ def quantize(X) -> Mxfp4:
     q = Mxfp4.__new__(Mxfp4)
     done = front.quantize(X)
     if done is not None:
-        q.codes, q.scales, q.rows, q.cols, q._index, q._pointers = done
+        q.codes, q.scales, q.cols = done
         return q
     xt, ldx, M, K, dev = _rows(X)
-    q.rows, q.cols, q._index = M, K, dev
     tiles, groups = (M + 127) // 128, (K + 255) // 256 * 2
     q.codes = empty((M, (K + 31) // 32 * 16), _U8, dev)
     q.scales = empty((tiles, groups, 32, 4, 4), _U8, dev, (groups * 512, 512, 16, 4, 1))
-    q._pointers = codes, scales = q.codes.data_ptr(), q.scales.data_ptr()
+    q.cols = K
     if M:
-        call("tac_mxfp4_quantize", _quantize, dev, X.data_ptr(), xt, ldx, codes, scales, M, K)
+        call("tac_mxfp4_quantize", _quantize, dev, X.data_ptr(), xt, ldx, *q._pointers, M, K)
     return q
 
 
 def _result(w, M, K, dev, bias, out, dtype):
     """Checks of what both products share; (out, its type, N, bias pointer, bias type)."""
+    _check_tensors(w.codes, w.scales, w.cols)
     if w.cols != K or w._index != dev:
         raise ValueError(f"the operands must have one number of columns and one device, got {K} and {w.cols} columns")
     N = w.rows
@@ -158,11 +175,12 @@ def gemm(a: Mxfp4, b: Mxfp4, bias=None, out_dtype=None, out=None):
     float16)."""
     if out_dtype is None:
         out_dtype = _F16 if out is None else out.dtype
-    M, K, dev = a.rows, a.cols, a._index
     if out is None and type(b) is Mxfp4:
-        y = front.gemm(a._pointers, M, K, dev, b._pointers, b.rows, b.cols, b._index, bias, out_dtype)
+        y = front.gemm((a.codes, a.scales), None, a.cols, None, (b.codes, b.scales), None, b.cols, None, bias, out_dtype)
         if y is not None:
             return y
+    _check_tensors(a.codes, a.scales, a.cols)
+    M, K, dev = a.rows, a.cols, a._index
     out, yt, N, bp, bt = _result(b, M, K, dev, bias, out, out_dtype)
     if M and N:
         call("tac_mxfp4_gemm", _gemm, dev, *a._pointers, *b._pointers, bp, bt, out.data_ptr(), yt, M, N, K)
@@ -176,7 +194,7 @@ def linear(X, w: Mxfp4, bias=None, out=None, ws=None):
     calls on one stream; by default a call allocates its own where it needs one.  A block of X with an infinity or a NaN
     gives a row of NaN."""
     if out is None and ws is None and type(w) is Mxfp4:
-        y = front.linear(X, w._pointers, w.rows, w.cols, w._index, bias)
+        y = front.linear(X, (w.codes, w.scales), None, w.cols, None, bias)
         if y is not None:
             return y
     xt, ldx, M, K, dev = _rows(X)
