@@ -13,9 +13,9 @@ try:
 except ImportError as e:
     raise ImportError("_front.so is not built for this torch; run `python -m llm_accelerator_b200.build` first") from e
 
-front.bind(*(C.cast(getattr(L.lib, "tac_" + name), C.c_void_p).value for name in (
-    "rms_norm", "rms_norm_i8", "dequantize_rows_i8", "mxfp4_quantize", "mxfp4_values", "mxfp4_gemm", "linear_mxfp4",
-    "linear_mxfp4_workspace_bytes", "token_logprobs")))
+ENTRIES = ("rms_norm", "rms_norm_i8", "dequantize_rows_i8", "mxfp4_quantize", "mxfp4_values", "mxfp4_gemm", "linear_mxfp4",
+           "linear_mxfp4_workspace_bytes", "token_logprobs")
+front.bind(*(C.cast(getattr(L.lib, "tac_" + name), C.c_void_p).value for name in ENTRIES), L.check)
 
 TYPES = {torch.float32: L.TYPE_F32, torch.float16: L.TYPE_F16, torch.bfloat16: L.TYPE_BF16}
 _current = torch._C._cuda_getDevice

@@ -3,7 +3,8 @@
 // (rms_norm_i8 of one row: 5 us of the host's time, 10 in Python, of which the
 // launch takes 2.6).  A function here answers only calls that need no word of
 // explanation; for every other one, and for those that the library refuses, it
-// gives None, and the Python front end says what is wrong or does the rest.
+// gives None, and the Python front end says what is wrong or does the rest.  A
+// launch that fails raises as it would there, and is not tried again.
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
@@ -92,9 +93,18 @@ struct Unlocked {
   ~Unlocked() { PyEval_RestoreThread(state); }
 };
 template <typename F>
-bool launched(F f) {
+int launched(F f) {
   Unlocked u;
-  return f() == 0;
+  return f();
+}
+
+PyObject* check = nullptr;             // raises the error of (status, name)
+
+// What a call gives whose launch did not go well: None where the library refused its arguments, before any launch.
+PyObject* failed(int status, const char* name) {
+  if (status == TAC_E_ARGUMENT) Py_RETURN_NONE;
+  Py_XDECREF(PyObject_CallFunction(check, "is", status, name));
+  return PyErr_Occurred() ? nullptr : PyErr_Format(PyExc_RuntimeError, "%s failed (status %d)", name, status);
 }
 
 template <typename... T>
@@ -173,7 +183,7 @@ PyObject* rms_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return lib.rms_norm(c.x.t->const_data_ptr(), c.x.type, c.x.ld, c.residual(), c.r.ld, c.sum(), c.x.K, c.w.p, c.w.type, c.eps,
                         y.data_ptr(), c.x.M, c.x.K, stream(c.dev));
   };
-  if (!launched(run)) Py_RETURN_NONE;
+  if (const int status = launched(run)) return failed(status, "tac_rms_norm");
   return c.r.t ? tuple(y, c.h) : THPVariable_Wrap(y);
   END_HANDLE_TH_ERRORS
 }
@@ -187,7 +197,7 @@ PyObject* rms_norm_i8(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return lib.rms_norm_i8(c.x.t->const_data_ptr(), c.x.type, c.x.ld, c.residual(), c.r.ld, c.sum(), c.x.K, c.w.p, c.w.type, c.eps,
                            static_cast<int8_t*>(q.data_ptr()), static_cast<float*>(scale.data_ptr()), c.x.M, c.x.K, stream(c.dev));
   };
-  if (!launched(run)) Py_RETURN_NONE;
+  if (const int status = launched(run)) return failed(status, "tac_rms_norm_i8");
   return c.r.t ? tuple(q, scale, c.h) : tuple(q, scale);
   END_HANDLE_TH_ERRORS
 }
@@ -211,7 +221,7 @@ PyObject* dequantize_rows(PyObject*, PyObject* const* a, Py_ssize_t n) {      //
     return lib.dequantize(static_cast<const int8_t*>(q->const_data_ptr()), static_cast<const float*>(scale->const_data_ptr()),
                           y.data_ptr(), type_of(out), int(M), int(K), stream(dev));
   };
-  if (!launched(run)) Py_RETURN_NONE;
+  if (const int status = launched(run)) return failed(status, "tac_dequantize_rows_i8");
   return THPVariable_Wrap(y);
   END_HANDLE_TH_ERRORS
 }
@@ -226,7 +236,7 @@ PyObject* quantize(PyObject*, PyObject* const* a, Py_ssize_t n) {             //
   const at::Tensor scales = empty({(int64_t(x.M) + 127) / 128, (int64_t(x.K) + 255) / 256 * 2, 32, 4, 4}, at::kByte, dev);
   uint8_t *c = static_cast<uint8_t*>(codes.data_ptr()), *s = static_cast<uint8_t*>(scales.data_ptr());
   const auto run = [&] { return lib.quantize(x.t->const_data_ptr(), x.type, x.ld, c, s, x.M, x.K, stream(dev)); };
-  if (!launched(run)) Py_RETURN_NONE;
+  if (const int status = launched(run)) return failed(status, "tac_mxfp4_quantize");
   return Py_BuildValue("(NNi)", THPVariable_Wrap(codes), THPVariable_Wrap(scales), x.K);
   END_HANDLE_TH_ERRORS
 }
@@ -241,7 +251,7 @@ PyObject* values(PyObject*, PyObject* const* a, Py_ssize_t n) {               //
   if (type_of(out) < 0) Py_RETURN_NONE;
   const at::Tensor y = empty({x.rows, x.cols}, out, dev);
   const auto run = [&] { return lib.values(x.codes, x.scales, y.data_ptr(), type_of(out), int(x.rows), int(x.cols), stream(dev)); };
-  if (!launched(run)) Py_RETURN_NONE;
+  if (const int status = launched(run)) return failed(status, "tac_mxfp4_values");
   return THPVariable_Wrap(y);
   END_HANDLE_TH_ERRORS
 }
@@ -261,7 +271,7 @@ PyObject* gemm(PyObject*, PyObject* const* args, Py_ssize_t n) {              //
     return lib.gemm(a.codes, a.scales, b.codes, b.scales, bias.p, bias.type, y.data_ptr(), type_of(out), int(a.rows), int(b.rows),
                     int(a.cols), stream(dev));
   };
-  if (!launched(run)) Py_RETURN_NONE;
+  if (const int status = launched(run)) return failed(status, "tac_mxfp4_gemm");
   return THPVariable_Wrap(y);
   END_HANDLE_TH_ERRORS
 }
@@ -283,7 +293,7 @@ PyObject* linear(PyObject*, PyObject* const* a, Py_ssize_t n) {               //
     return lib.linear(x.t->const_data_ptr(), x.type, x.ld, w.codes, w.scales, bias.p, bias.type, y.data_ptr(), x.type,
                       bytes ? ws.data_ptr() : nullptr, uint64_t(bytes), x.M, N, x.K, stream(dev));
   };
-  if (!launched(run)) Py_RETURN_NONE;
+  if (const int status = launched(run)) return failed(status, "tac_linear_mxfp4");
   return THPVariable_Wrap(y);
   END_HANDLE_TH_ERRORS
 }
@@ -308,14 +318,14 @@ PyObject* token_logprobs(PyObject*, PyObject* const* a, Py_ssize_t n) {       //
                         top ? static_cast<float*>(top_lp.data_ptr()) : nullptr, top ? static_cast<int32_t*>(ids.data_ptr()) : nullptr,
                         stream(dev));
   };
-  if (!launched(run)) Py_RETURN_NONE;
+  if (const int status = launched(run)) return failed(status, "tac_token_logprobs");
   return top ? tuple(lp, entropy, top_lp, ids) : tuple(lp, entropy);
   END_HANDLE_TH_ERRORS
 }
 
-PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {                 // addresses, in the order of Entries
+PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {                 // addresses, in the order of Entries; check
   void* p[9];
-  if (n != 9) return PyErr_Format(PyExc_TypeError, "bind() takes 9 addresses");
+  if (n != 10 || !PyCallable_Check(a[9])) return PyErr_Format(PyExc_TypeError, "bind() takes 9 addresses and a function");
   for (int i = 0; i < 9; ++i)
     if (!(p[i] = PyLong_AsVoidPtr(a[i]))) return PyErr_Occurred() ? nullptr : PyErr_Format(PyExc_ValueError, "a null address");
   lib = {reinterpret_cast<decltype(lib.rms_norm)>(p[0]),     reinterpret_cast<decltype(lib.rms_norm_i8)>(p[1]),
@@ -323,6 +333,9 @@ PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {                 //
          reinterpret_cast<decltype(lib.values)>(p[4]),       reinterpret_cast<decltype(lib.gemm)>(p[5]),
          reinterpret_cast<decltype(lib.linear)>(p[6]),       reinterpret_cast<decltype(lib.linear_bytes)>(p[7]),
          reinterpret_cast<decltype(lib.logprobs)>(p[8])};
+  Py_INCREF(a[9]);
+  Py_XDECREF(check);
+  check = a[9];
   Py_RETURN_NONE;
 }
 
