@@ -1,5 +1,5 @@
 """What the torch front ends of the stand-alone kernels share: type codes, calls on a tensor's device, and ``front``, the
-C++ side of their usual calls, each of which gives None where Python has to look at the arguments."""
+C++ side of the usual calls of some, each of which gives None where Python has to look at the arguments."""
 from __future__ import annotations
 
 import ctypes as C
@@ -8,14 +8,40 @@ import torch
 
 from . import _lib as L
 
-try:
-    from . import _front as front
-except ImportError as e:
-    raise ImportError("_front.so is not built for this torch; run `python -m llm_accelerator_b200.build` first") from e
-
 ENTRIES = ("rms_norm", "rms_norm_i8", "dequantize_rows_i8", "mxfp4_quantize", "mxfp4_values", "mxfp4_gemm", "linear_mxfp4",
            "linear_mxfp4_workspace_bytes", "token_logprobs")
-front.bind(*(C.cast(getattr(L.lib, "tac_" + name), C.c_void_p).value for name in ENTRIES), L.check)
+
+
+class _PythonOnly:
+    """In place of a ``front`` that is not built: leaves every call to Python."""
+
+    def __getattr__(self, name):
+        return lambda *args: None
+
+
+def _load_front():
+    import importlib.util
+    import warnings
+
+    from .build import front_path
+    spec = importlib.util.spec_from_file_location(f"{__package__}._front", front_path())
+    try:
+        module = importlib.util.module_from_spec(spec)
+    except ImportError as e:
+        warnings.warn(f"the torch front ends' C++ side is not built for this torch and Python, and their calls take longer: "
+                      f"run `python -m llm_accelerator_b200.build` ({e})", RuntimeWarning, stacklevel=3)
+        return _PythonOnly()
+    spec.loader.exec_module(module)
+    module.bind(*(C.cast(getattr(L.lib, "tac_" + name), C.c_void_p).value for name in ENTRIES), L.check)
+    return module
+
+
+def __getattr__(name):
+    if name != "front":                # loaded for the modules that have calls in it
+        raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
+    globals()["front"] = found = _load_front()
+    return found
+
 
 TYPES = {torch.float32: L.TYPE_F32, torch.float16: L.TYPE_F16, torch.bfloat16: L.TYPE_BF16}
 _current = torch._C._cuda_getDevice

@@ -1,14 +1,18 @@
-"""Builds libtaccel_b200.so (sm_100a) in-tree with nvcc, and _front.so, the torch front ends' usual calls in C++.
+"""Builds libtaccel_b200.so (sm_100a) in-tree with nvcc, and behind it `_front`, the torch front ends' usual calls in C++.
 
 The library holds the host compiler (instruction stream -> device plan), the
 executor kernels and the stand-alone GEMM kernels.  It is built in the package
 directory so it travels with the source tree; nothing is cached outside it.
+`_front` speaks to torch's C++ side: its file is named by the torch and the
+Python that it is built for, and without either's headers it is left out (the
+front ends then make their calls in Python).
 """
 from __future__ import annotations
 
 import os
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
@@ -20,7 +24,7 @@ OBJDIR = PKG.parent / "_build"
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 CXX = os.environ.get("CXX", "g++")
-FRONT, FRONT_SRC = PKG / "_front.so", CSRC / "tac_front.cc"
+FRONT_SRC = CSRC / "tac_front.cc"
 FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", f"-I{INCLUDE}", f"-I{CSRC}"]
 
 
@@ -39,9 +43,29 @@ def up_to_date() -> bool:
     return all(p.stat().st_mtime <= t for p in _deps())
 
 
+def front_path() -> Path:
+    """The file of the extension module for this torch and this Python."""
+    import torch
+    abi = int(torch.compiled_with_cxx11_abi())
+    return PKG / f"_front.torch-{torch.__version__}-abi{abi}{sysconfig.get_config_var('EXT_SUFFIX')}"
+
+
+def front_missing() -> str | None:
+    """Why the extension module cannot be built here, or None."""
+    try:
+        import torch
+    except ImportError:
+        return "torch is not installed"
+    if torch.version.cuda is None:
+        return "torch is built without CUDA"
+    if not Path(sysconfig.get_path("include"), "Python.h").exists():
+        return "Python's headers are not installed"
+    return None
+
+
 def front_up_to_date() -> bool:
-    # of this torch: the module speaks to its C++ side
-    t = FRONT.stat().st_mtime if FRONT.exists() else 0
+    f = front_path()
+    t = f.stat().st_mtime if f.exists() else 0
     return all(p.stat().st_mtime <= t for p in (FRONT_SRC, INCLUDE / "taccel_b200.h", _torch_dir() / "version.py"))
 
 
@@ -52,11 +76,9 @@ def _torch_dir() -> Path:
 
 def build_front() -> Path:
     """Compile the extension module of the torch front ends, which calls the library by addresses."""
-    import sysconfig
-
     import torch
-    t, abi = _torch_dir(), int(torch.compiled_with_cxx11_abi())
-    tmp = FRONT.with_suffix(".so.tmp")
+    t, abi, front = _torch_dir(), int(torch.compiled_with_cxx11_abi()), front_path()
+    tmp = front.with_name(front.name + ".tmp")
     cmd = [CXX, "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", f"-D_GLIBCXX_USE_CXX11_ABI={abi}", f"-I{INCLUDE}",
            *(f"-isystem{p}" for p in (t / "include", t / "include/torch/csrc/api/include", "/usr/local/cuda/include",
                                       sysconfig.get_path("include"))),
@@ -64,8 +86,8 @@ def build_front() -> Path:
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"{CXX} failed for {FRONT_SRC.name}:\n{r.stdout}\n{r.stderr}")
-    os.replace(tmp, FRONT)
-    return FRONT
+    os.replace(tmp, front)
+    return front
 
 
 def _compile(src: Path, verbose: bool) -> Path:
@@ -81,10 +103,8 @@ def _compile(src: Path, verbose: bool) -> Path:
     return obj
 
 
-def build(force: bool = False, verbose: bool = False) -> Path:
-    """Compile every CUDA / C++ source for sm_100a and link the shared library; and the front ends' module."""
-    if force or not front_up_to_date():
-        build_front()
+def build_library(force: bool = False, verbose: bool = False) -> Path:
+    """Compile every CUDA / C++ source for sm_100a and link the shared library."""
     if not force and up_to_date():
         return LIB
     OBJDIR.mkdir(exist_ok=True)
@@ -97,6 +117,16 @@ def build(force: bool = False, verbose: bool = False) -> Path:
         raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
     os.replace(tmp, LIB)
     return LIB
+
+
+def build(force: bool = False, verbose: bool = False) -> Path:
+    """The shared library, and then the front ends' module, where torch is there for it."""
+    lib = build_library(force, verbose)
+    if why := front_missing():
+        sys.stderr.write(f"the torch front ends' module is left out: {why}\n")
+    elif force or not front_up_to_date():
+        build_front()
+    return lib
 
 
 if __name__ == "__main__":

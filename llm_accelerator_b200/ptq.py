@@ -22,10 +22,14 @@ device-memory plumbing).
 """
 from __future__ import annotations
 
-import torch
-
 from . import _lib as L
-from ._tensors import TYPES, call, empty, front, type_code
+
+try:
+    import torch
+    from ._tensors import TYPES, call, empty, front, type_code
+except ModuleNotFoundError as e:       # the functions need it, once they are called
+    if e.name != "torch":
+        raise
 
 _dequantize = L.lib.tac_dequantize_rows_i8
 
@@ -87,10 +91,12 @@ def quantize_rows(X):
     return q, scale
 
 
-def dequantize_rows(q, scale, K=None, dtype=torch.float32):
-    """[M, K] q[m, k] * scale[m], rounded to `dtype` (float32, float16 or bfloat16): the values that the rows of
-    ``quantize_rows`` or ``norm.rms_norm_i8`` stand for.  q int8 [M, K_pad], scale float32 [M]; K, by default all
+def dequantize_rows(q, scale, K=None, dtype=None):
+    """[M, K] q[m, k] * scale[m], rounded to `dtype` (float32, the default, float16 or bfloat16): the values that the rows
+    of ``quantize_rows`` or ``norm.rms_norm_i8`` stand for.  q int8 [M, K_pad], scale float32 [M]; K, by default all
     columns, leaves out the padding ones.  No gradient flows through the call."""
+    if dtype is None:
+        dtype = torch.float32
     y = front.dequantize_rows(q, scale, K, dtype)
     if y is not None:
         return y
