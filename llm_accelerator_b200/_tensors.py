@@ -3,6 +3,7 @@ C++ side of the usual calls of some, each of which gives None where Python has t
 from __future__ import annotations
 
 import ctypes as C
+from functools import lru_cache
 
 import torch
 
@@ -75,3 +76,14 @@ def call(name: str, fn, index: int, *args) -> None:
             status = fn(*args, _stream(index))
     if status:
         L.check(status, name)
+
+
+def of_device(query):
+    """The workspace query f(index, *sizes) of CUDA device `index`, by whose SMs `query` goes; asked once."""
+    @lru_cache(maxsize=1024)
+    def f(index: int, *sizes) -> int:
+        if _current() == index:
+            return query(*sizes)
+        with torch.cuda.device(index):
+            return query(*sizes)
+    return f

@@ -16,17 +16,15 @@ The calls are for inference: no gradient flows through them, also from tensors t
 """
 from __future__ import annotations
 
-from functools import lru_cache
-
 import torch
 
 from . import _lib as L
-from ._tensors import TYPES, call, empty, front, type_code
+from ._tensors import TYPES, call, empty, front, of_device, type_code
 
 _U8, _F16, _F32 = torch.uint8, torch.float16, torch.float32
 _quantize, _values, _gemm, _linear = (L.lib.tac_mxfp4_quantize, L.lib.tac_mxfp4_values, L.lib.tac_mxfp4_gemm,
                                       L.lib.tac_linear_mxfp4)
-_ws_bytes = lru_cache(maxsize=1024)(L.lib.tac_linear_mxfp4_workspace_bytes)   # sizes alone decide
+_ws_bytes = of_device(L.lib.tac_linear_mxfp4_workspace_bytes)
 
 
 def _scale_shape(rows: int, cols: int):
@@ -205,7 +203,7 @@ def linear(X, w: Mxfp4, bias=None, out=None, ws=None):
             if ws.get_device() != dev or ws.dtype is not _U8 or not ws.is_contiguous():
                 raise ValueError("ws must be a linear_workspace on X's device")
         else:
-            need = _ws_bytes(M, N, K)
+            need = _ws_bytes(dev, M, N, K)
             ws = empty((need,), _U8, dev) if need else None
         if ws is not None:
             p = ws.data_ptr()

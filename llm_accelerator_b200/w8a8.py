@@ -9,16 +9,14 @@ The products are for inference: no gradient flows through them, also from rows, 
 """
 from __future__ import annotations
 
-from functools import lru_cache
-
 import torch
 
 from . import _lib as L
-from ._tensors import TYPES, call, type_code
+from ._tensors import TYPES, call, of_device, type_code
 
 _I8, _F32, _F16 = torch.int8, torch.float32, torch.float16
 _gemm, _linear = L.lib.tac_gemm_i8_scaled, L.lib.tac_linear_w8a8
-_ws_bytes = lru_cache(maxsize=1024)(L.lib.tac_linear_w8a8_best_workspace_bytes)   # sizes alone decide
+_ws_bytes = of_device(L.lib.tac_linear_w8a8_best_workspace_bytes)
 
 
 def _check(rows, Bt, b_scale, bias, out, out_dtype, M, K):
@@ -109,7 +107,7 @@ def linear_w8a8(X, Bt, b_scale, bias=None, out=None, ws=None):
             if ws.get_device() != X.get_device() or ws.dtype is not torch.uint8 or not ws.is_contiguous():
                 raise ValueError("ws must be a linear_workspace on X's device")
         else:
-            need = _ws_bytes(M, N, K)
+            need = _ws_bytes(X.get_device(), M, N, K)
             ws = torch.empty(need + 256, dtype=torch.uint8, device=X.device) if need else None
         if ws is not None:
             p = ws.data_ptr()
