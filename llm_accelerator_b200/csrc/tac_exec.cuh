@@ -2966,6 +2966,7 @@ static_assert(kSegTableOff + kMaxSegRuns * 13 <= kMaxQStage && kMaxQStage + 1638
               "MAX_ABS staging overlaps the segment table or exceeds the op shared memory");
 static_assert(kExecOpSmem % 1024 == 0 || kTcSmem <= kExecOpSmem, "half regions must keep the stage alignment slack");
 static_assert(kExecSmem <= 227 * 1024, "executor shared memory exceeds one CTA's limit");
+static_assert(kHalves * kTcCols <= 256 && kExecSmem >= sm100::tmem_least_smem(256), "CTAs behind a grid barrier could wait for TMEM");
 
 // A is a __grid_constant__ parameter: the op functions take its address
 // without a per-thread copy in local memory.

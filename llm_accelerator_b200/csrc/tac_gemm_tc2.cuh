@@ -42,6 +42,7 @@ struct Tc2Cfg {
   static constexpr uint32_t kIdesc = sm100::idesc_i8(2 * kBM, kBN, 1);
   static constexpr uint32_t kIdescK = sm100::idesc_i8(2 * kBM, kBN, 0);
 };
+static_assert(sm100::tmem_alone(Tc2Cfg::kSmem), "two clusters could wait for each other's TMEM");
 
 // p.m_tiles counts 256-row pair tiles, p.n_tiles 256-column tiles;
 // p.total_units = m_tiles * n_tiles.  Launched with clusters of two CTAs.

@@ -257,7 +257,7 @@ int launch_splitk(const MxOperands& o, MxParams p, cudaStream_t st) {
   const int per = (p.k_stages + split - 1) / split, sb = mx_sk_stage_bytes(p.tn);
   // in flight: 96 KB where two CTAs share an SM, else twice that
   p.stages = std::min(std::min(per, kMxSkStages), std::max(2, (tiles * split > sms ? 96 : 190) * 1024 / sb));
-  const int part = split > 1 ? std::max(mx_sk_part_bytes(p.tn), mx_sk_least_smem(mx_sk_cols(p.tn, p.stages))) : 0;
+  const int part = split > 1 ? std::max(mx_sk_part_bytes(p.tn), sm100::tmem_least_smem(mx_sk_cols(p.tn, p.stages))) : 0;
   CUtensorMap tw, ta;
   if (!map_rows(&tw, o.b_codes, o.K, p.N, 128) || !map_rows(&ta, o.a_codes, o.K, p.M, p.tn)) return TAC_E_CUDA;
   cudaLaunchConfig_t cfg = {};
@@ -438,7 +438,7 @@ int launch_rows_as(MxRowsParams pp, const MxOperands& o, cudaStream_t st) {
   p.tn = r.tn;
   const int rows = r.per * mx_rows_bytes(r.tn), sb = kMxWBytes + kMxSfBytes;
   p.stages = std::min({r.per, kMxSkStages, (kMxMaxSmem - 1024 - rows) / sb});     // the rows are 192 KB at most, of one token
-  const int part = r.split > 1 ? std::max(mx_sk_part_bytes(r.tn), mx_sk_least_smem(mx_sk_cols(r.tn, p.stages))) : 0;
+  const int part = r.split > 1 ? std::max(mx_sk_part_bytes(r.tn), sm100::tmem_least_smem(mx_sk_cols(r.tn, p.stages))) : 0;
   CUtensorMap tw;
   if (!map_rows(&tw, o.b_codes, o.K, p.N, 128)) return TAC_E_CUDA;
   cudaLaunchConfig_t cfg = {};

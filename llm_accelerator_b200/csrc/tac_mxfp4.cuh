@@ -198,11 +198,6 @@ __host__ __device__ constexpr int mx_sk_cols(int tn, int stages) {
   const int need = mx_sk_sf_col(tn) + 16 * stages;
   return need <= 64 ? 64 : need <= 128 ? 128 : 256;
 }
-// Shared memory that keeps the CTAs of an SM to half of its TMEM.  A CTA that waits for TMEM would hold up its cluster,
-// whose other CTAs hold theirs meanwhile, and clusters, of two calls or of this product and the INT8 one, could wait for one
-// another.
-__host__ __device__ constexpr int mx_sk_least_smem(int cols) { return 227 * 1024 / (256 / cols + 1) + 1024; }
-
 __host__ __device__ constexpr int mx_sk_stage_bytes(int tn) { return kMxWBytes + tn * 128 + 2 * kMxSfBytes; }
 
 // Partial sums of a split tile in shared memory: [128 channels][tn + 4], the padding against bank conflicts.
@@ -648,6 +643,7 @@ struct MxPairCfg {
   static constexpr int kEpi = 512;     // epilogue threads: four warps a quadrant of TMEM, a fourth of the tokens each
   static constexpr int kThreads = 64 + kEpi;
 };
+static_assert(sm100::tmem_alone(MxPairCfg::kSmem), "two clusters could wait for each other's TMEM");
 
 struct MxPairParams {
   MxParams g;

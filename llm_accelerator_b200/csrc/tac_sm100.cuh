@@ -132,6 +132,20 @@ __device__ __forceinline__ void bulk_g2s(void* smem_dst, const void* gsrc, uint3
 __device__ __forceinline__ void fence_proxy_async() { asm volatile("fence.proxy.async;\n" ::: "memory"); }
 
 // ---- TMEM -----------------------------------------------------------------------
+// A CTA that waits for TMEM while others of its cluster (or grid, where that has
+// a barrier) hold theirs could wait for one that waits for it, of another call or
+// kernel.  Shared memory keeps that from happening: with what each such CTA takes
+// of an SM's 228 KB (1 KB of them for the system), all that fit one find their
+// columns there: 384 at most for any mix of up to 256 columns each, and nothing
+// beside one of 512.
+constexpr int kSmSmem = 228 * 1024, kCtaSmem = 1024;
+__host__ __device__ constexpr int tmem_least_smem(int cols) {
+  const int half = 227 * 1024 / (256 / cols + 1) + 1024;
+  return half > 34 * 1024 ? half : 34 * 1024;
+}
+// Of one of 512 columns: no other fits beside it.
+__host__ __device__ constexpr bool tmem_alone(int smem) { return smem + kCtaSmem + tmem_least_smem(32) + kCtaSmem > kSmSmem; }
+
 __device__ __forceinline__ void tmem_alloc(uint32_t* smem_result, uint32_t ncols) {
   asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(smem_result)),
                "r"(ncols));

@@ -216,7 +216,7 @@ int launch_splitk(const int8_t* A, const int8_t* Bt, W8Params p, cudaStream_t st
   const int per = (p.k_blocks + split - 1) / split, sb = sk_stage_bytes(p.tn);
   // in flight: 96 KB where two CTAs share an SM, else twice that
   p.stages = std::min(std::min(per, 8), std::max(2, (tiles * split > sms ? 96 : 190) * 1024 / sb));
-  const int part = split > 1 ? sk_part_bytes(p.tn) : 0;
+  const int part = split > 1 ? std::max(sk_part_bytes(p.tn), sm100::tmem_least_smem(sk_cols(p.tn))) : 0;
   CUtensorMap tw, ta;
   if (!map_rows(&tw, Bt, p.K, p.N, 128) || !map_rows(&ta, A, p.K, p.M, p.tn)) return TAC_E_CUDA;
   cudaLaunchConfig_t cfg = {};
@@ -388,7 +388,8 @@ int launch_rows(W8RowsParams pp, const int8_t* Bt, cudaStream_t st) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(uint32_t(tiles), 1, split);
   cfg.blockDim = dim3(kSkThreads);
-  cfg.dynamicSmemBytes = p.stages * kSkWBytes + rows_bytes + 1024;   // the partial sums (10 KB) fit the first stage
+  // the partial sums (10 KB) fit the first stage
+  cfg.dynamicSmemBytes = std::max(p.stages * kSkWBytes + rows_bytes, split > 1 ? sm100::tmem_least_smem(sk_cols(p.tn)) : 0) + 1024;
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;

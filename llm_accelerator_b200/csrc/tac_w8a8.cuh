@@ -158,6 +158,7 @@ constexpr int kSkThreads = 192;
 constexpr int kSkWBytes = 128 * 128;
 
 __host__ __device__ constexpr int sk_stage_bytes(int tn) { return kSkWBytes + tn * 128; }
+__host__ __device__ constexpr int sk_cols(int tn) { return tn <= 32 ? 32 : tn <= 64 ? 64 : 128; }   // of TMEM
 
 // Partial sums of a split tile in shared memory: [128 channels][tn + 4], so that a channel's tokens are read 16 bytes at
 // a time from the other CTAs and the padding spreads the channels over the banks.
@@ -244,7 +245,7 @@ __global__ void __launch_bounds__(kSkThreads)
   const int nsplit = gridDim.z, rank = blockIdx.z;
   const int kb0 = int(int64_t(p.k_blocks) * rank / nsplit), kb1 = int(int64_t(p.k_blocks) * (rank + 1) / nsplit);
   const int S = p.stages, stage_bytes = sk_stage_bytes(p.tn);
-  const uint32_t cols = p.tn <= 32 ? 32 : p.tn <= 64 ? 64 : p.tn <= 128 ? 128 : 256;
+  const uint32_t cols = sk_cols(p.tn);
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < S; ++s) {
@@ -580,6 +581,7 @@ struct PairCfg {
   static constexpr int kEpi = 512;     // epilogue threads: four warps a quadrant of TMEM, a fourth of the tokens each
   static constexpr int kThreads = 64 + kEpi;
 };
+static_assert(sm100::tmem_alone(PairCfg::kSmem), "two clusters could wait for each other's TMEM");
 
 struct W8PairParams {
   W8Params g;
