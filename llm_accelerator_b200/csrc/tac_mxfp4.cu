@@ -117,11 +117,13 @@ __global__ void __launch_bounds__(kQmThreads) mx_quant_kernel(const T* __restric
 int64_t quant_tasks(int M, int k_stages) { return (int64_t(M) + 127) / 128 * 32 * k_stages; }
 int64_t quant_ctas(int M, int k_stages) { return (quant_tasks(M, k_stages) + kQmThreads / 32 - 1) / (kQmThreads / 32); }
 
+bool vec_rows(const void* X, int type, int64_t ldx, int M) { return aligned(X, 16) && (M == 1 || (ldx * elem(type)) % 16 == 0); }
+
 int launch_quant(const void* X, int type, int64_t ldx, uint8_t* codes, uint8_t* scales, int M, int K, cudaStream_t st) {
   const int k_stages = int(mx_pieces(K) / 2);
   const int64_t tasks = quant_tasks(M, k_stages), ctas = quant_ctas(M, k_stages);
   if (tasks > 0x7fffffff) return TAC_E_ARGUMENT;             // rows of 4 TB
-  const int vec = aligned(X, 16) && (M == 1 || (ldx * elem(type)) % 16 == 0);
+  const int vec = vec_rows(X, type, ldx, M);
   const auto go = [&](auto* x) {
     using T = std::remove_const_t<std::remove_pointer_t<decltype(x)>>;
     if constexpr (sizeof(T) == 2) {
@@ -239,6 +241,7 @@ struct MxOperands {
   const uint8_t* a_codes;
   const uint8_t* b_codes;
   int K;
+  bool spread;               // pairs without a tile keep the quantiser's CTAs apart
 };
 
 template <int YT>
@@ -337,8 +340,10 @@ int launch_pair(const MxOperands& o, MxParams p, int clusters, int tn, cudaStrea
   if (tiles > (1 << 30)) return TAC_E_ARGUMENT;
   // Behind the quantiser this kernel starts while that one runs, but not on an SM that holds two of its CTAs.  Where it has one
   // for each SM at most, pairs without a tile keep the last call's SMs from being free, on which the quantiser's CTAs would
-  // gather: 300 x 9000 x 768 in 7.4 us, 9.4 without them.
-  const bool fill = p.after_rows && quant_ctas(p.M, p.k_stages) <= 2 * clusters && tiles * 2 > clusters;
+  // gather: 300 x 9000 x 768 in 7.2 us, 9.3 without them (float32 rows 7.7 and 8.9).  The quantiser of 16-bit rows that begin
+  // anywhere has 58 registers a thread, with which not even one CTA fits beside a pair's, and gains nothing (500 x 8192 x 512
+  // in 8.3 us with them, 7.6 without).
+  const bool fill = o.spread && quant_ctas(p.M, p.k_stages) <= 2 * clusters && tiles * 2 > clusters;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(2 * int(fill ? clusters : std::min<int64_t>(tiles, clusters)));
   cfg.blockDim = dim3(MxPairCfg::kThreads);
@@ -382,7 +387,7 @@ int check_product(const void* b_codes, const void* b_scales, const void* bias, i
 }
 
 int run_product(const uint8_t* a_codes, const uint8_t* a_scales, const uint8_t* b_codes, const uint8_t* b_scales, const void* bias,
-                int bias_type, void* Y, int y_type, int M, int N, int K, bool after_rows, cudaStream_t st) {
+                int bias_type, void* Y, int y_type, int M, int N, int K, bool after_rows, bool spread, cudaStream_t st) {
   MxParams p{};
   p.a_scale = a_scales, p.b_scale = b_scales;
   p.bias = bias, p.bias_type = bias_type;
@@ -391,7 +396,7 @@ int run_product(const uint8_t* a_codes, const uint8_t* a_scales, const uint8_t* 
   p.k_stages = int(mx_pieces(K) / 2);
   p.after_rows = after_rows;
   if (!(p.fault = fault_word())) return TAC_E_CUDA;
-  const MxOperands o{a_codes, b_codes, K};
+  const MxOperands o{a_codes, b_codes, K, spread};
   return y_type == TAC_F32 ? pick_product<0>(o, p, st) : y_type == TAC_F16 ? pick_product<1>(o, p, st) : pick_product<2>(o, p, st);
 }
 
@@ -499,7 +504,7 @@ extern "C" int tac_mxfp4_gemm(const uint8_t* a_codes, const uint8_t* a_scales, c
                               const void* bias, int bias_type, void* Y, int y_type, int M, int N, int K, void* stream) {
   if (!a_codes || !a_scales || !aligned(a_codes, 16) || !aligned(a_scales, 16)) return TAC_E_ARGUMENT;
   if (int s = check_product(b_codes, b_scales, bias, bias_type, Y, y_type, M, N, K)) return s;
-  return run_product(a_codes, a_scales, b_codes, b_scales, bias, bias_type, Y, y_type, M, N, K, false, static_cast<cudaStream_t>(stream));
+  return run_product(a_codes, a_scales, b_codes, b_scales, bias, bias_type, Y, y_type, M, N, K, false, false, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" uint64_t tac_linear_mxfp4_workspace_bytes(int M, int N, int K) {
@@ -521,9 +526,9 @@ extern "C" int tac_linear_mxfp4(const void* X, int x_type, int64_t ldx, const ui
     pp.g.M = M, pp.g.N = N;
     pp.g.k_stages = int(mx_pieces(K) / 2);
     if (!(pp.g.fault = fault_word())) return TAC_E_CUDA;
-    pp.x = X, pp.x_type = x_type, pp.ldx = ldx, pp.K = K;
-    pp.x_vec = aligned(X, 16) && (M == 1 || (ldx * elem(x_type)) % 16 == 0);
-    const MxOperands o{nullptr, b_codes, K};
+    pp.x = X, pp.ldx = ldx, pp.K = K;
+    pp.x_vec = vec_rows(X, x_type, ldx, M);
+    const MxOperands o{nullptr, b_codes, K, false};
     return x_type == TAC_F32   ? launch_rows<float>(pp, o, y_type, st)
            : x_type == TAC_F16 ? launch_rows<__half>(pp, o, y_type, st)
                                : launch_rows<__nv_bfloat16>(pp, o, y_type, st);
@@ -532,5 +537,6 @@ extern "C" int tac_linear_mxfp4(const void* X, int x_type, int64_t ldx, const ui
   uint8_t* codes = static_cast<uint8_t*>(workspace);
   uint8_t* scales = codes + align256(code_bytes(M, K));
   if (int e = launch_quant(X, x_type, ldx, codes, scales, M, K, st)) return e;
-  return run_product(codes, scales, b_codes, b_scales, bias, bias_type, Y, y_type, M, N, K, true, st);
+  return run_product(codes, scales, b_codes, b_scales, bias, bias_type, Y, y_type, M, N, K, true,
+                     x_type == TAC_F32 || vec_rows(X, x_type, ldx, M), st);
 }

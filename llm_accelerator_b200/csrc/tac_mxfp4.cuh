@@ -476,7 +476,7 @@ constexpr int kMxRowsThreads = 64 + 256, kMxRowsHeld = 8;
 struct MxRowsParams {
   MxParams g;
   const void* x;
-  int x_type, x_vec;         // x_vec: rows of whole, aligned 16-byte pieces
+  int x_vec;                 // rows of whole, aligned 16-byte pieces
   int64_t ldx;
   int K;                     // columns of x
 };
@@ -632,10 +632,12 @@ __global__ void __launch_bounds__(kMxRowsThreads) mx_rows_kernel(const __grid_co
 //   Outputs wider than K is deep are bound by the epilogue (333 x 50257 x 768: 17
 // us, 12 without stores); 16-byte stores out of shared memory, for runs of 256
 // bytes, took 20 and for even rows 3.5 us longer than pairs.
-//   88 registers, so that a CTA of the row quantiser fits beside it in each
-// quarter of the SM's (five warps' of the 18, two of its): this kernel is then in
-// place when the rows are quantised.  (333 x 50257 x 768 from BF16 rows: 18.1 us,
-// 20.7 with the 96 that the compiler would take.)
+//   88 registers, so that a CTA of the quantiser of aligned 16-bit rows (32 a
+// thread) fits beside it in each quarter of the SM's (five warps' of the 18, two
+// of its): this kernel is then in place when the rows are quantised.  (333 x
+// 50257 x 768 from BF16 rows: 18.1 us, 20.7 with the 96 that the compiler would
+// take.)  The quantisers of float32 rows (48) and of 16-bit rows that begin
+// anywhere (58) do not fit.
 struct MxPairCfg {
   static constexpr int kStages = 6;
   static constexpr int kStageBytes = 2 * 16384 + 3 * kMxSfBytes;
