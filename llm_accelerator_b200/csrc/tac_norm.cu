@@ -363,7 +363,7 @@ __global__ void __launch_bounds__(32 * kLongWarps, 2) norm_long_kernel(NormParam
 template <typename T, bool ANY, bool I8>
 int launch_rows(const NormParams& p, cudaStream_t st) {
   constexpr int kOf = 64 / sizeof(T);            // values of four loads
-  if (p.K <= 32 * kOf) return launch_behind(norm_kernel<T, ANY, I8, 1, 4>, (p.M + 3) / 4, 128, 0, st, p);
+  if (p.K <= 32 * kOf) return launch_behind(norm_kernel<T, ANY, I8, 1, 4>, unsigned(p.M + 3u) / 4, 128, 0, st, p);
   if (p.K <= 64 * kOf) return launch_behind(norm_kernel<T, ANY, I8, 2, 4>, p.M, 64, 0, st, p);
   if (p.K <= 128 * kOf) return launch_behind(norm_kernel<T, ANY, I8, 4, 4>, p.M, 128, 0, st, p);
   if (p.K <= 256 * kOf) return launch_behind(norm_kernel<T, ANY, I8, 8, 4>, p.M, 256, 0, st, p);
