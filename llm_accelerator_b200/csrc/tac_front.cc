@@ -16,6 +16,7 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
 #include <climits>
 #include <cstdint>
 
@@ -84,6 +85,17 @@ struct Vector {
 
 at::Tensor empty(at::IntArrayRef sizes, at::ScalarType type, int64_t dev) {
   return at::detail::empty_cuda(sizes, type, at::Device(at::kCUDA, c10::DeviceIndex(dev)), std::nullopt);
+}
+// A product's result: a new tensor where o is None, o itself where it is as that one would be.
+bool result(PyObject* o, int64_t M, int64_t N, at::ScalarType type, int64_t dev, at::Tensor* y) {
+  if (o == Py_None) {
+    *y = empty({M, N}, type, dev);
+    return true;
+  }
+  const at::Tensor* t = tensor(o, dev);
+  if (!t || t->scalar_type() != type || t->dim() != 2 || t->size(0) != M || t->size(1) != N || !t->is_contiguous()) return false;
+  *y = *t;
+  return true;
 }
 void* stream(int64_t dev) { return c10::cuda::getCurrentCUDAStream(c10::DeviceIndex(dev)).stream(); }
 
@@ -256,17 +268,17 @@ PyObject* values(PyObject*, PyObject* const* a, Py_ssize_t n) {               //
   END_HANDLE_TH_ERRORS
 }
 
-PyObject* gemm(PyObject*, PyObject* const* args, Py_ssize_t n) {              // 4-bit rows twice, bias, dtype
+PyObject* gemm(PyObject*, PyObject* const* args, Py_ssize_t n) {              // 4-bit rows twice, bias, dtype, out
   HANDLE_TH_ERRORS
   Rows4 a, b;
   Vector bias;
-  if (n != 10) Py_RETURN_NONE;
+  if (n != 11) Py_RETURN_NONE;
   const int64_t dev = Rows4::device(args[0]);
   if (!a.of(args, dev) || !b.of(args + 4, dev) || a.cols != b.cols || !bias.of(args[8], b.rows, dev) || !THPDtype_Check(args[9]))
     Py_RETURN_NONE;
   const at::ScalarType out = reinterpret_cast<THPDtype*>(args[9])->scalar_type;
-  if (type_of(out) < 0) Py_RETURN_NONE;
-  const at::Tensor y = empty({a.rows, b.rows}, out, dev);
+  at::Tensor y;
+  if (type_of(out) < 0 || !result(args[10], a.rows, b.rows, out, dev, &y)) Py_RETURN_NONE;
   const auto run = [&] {
     return lib.gemm(a.codes, a.scales, b.codes, b.scales, bias.p, bias.type, y.data_ptr(), type_of(out), int(a.rows), int(b.rows),
                     int(a.cols), stream(dev));
@@ -276,22 +288,32 @@ PyObject* gemm(PyObject*, PyObject* const* args, Py_ssize_t n) {              //
   END_HANDLE_TH_ERRORS
 }
 
-PyObject* linear(PyObject*, PyObject* const* a, Py_ssize_t n) {               // X; 4-bit rows; bias
+PyObject* linear(PyObject*, PyObject* const* a, Py_ssize_t n) {               // X; 4-bit rows; bias, and, or not, out and workspace
   HANDLE_TH_ERRORS
   Rows4 w;
   Rows x;
   Vector bias;
-  if (n != 6) Py_RETURN_NONE;
+  if (n != 6 && n != 8) Py_RETURN_NONE;
   const int64_t dev = device_of(a[0]);
   if (!x.of(a[0], dev) || !w.of(a + 1, dev) || w.cols != x.K || !bias.of(a[5], w.rows, dev)) Py_RETURN_NONE;
   const int N = int(w.rows);
-  const at::Tensor y = empty({x.M, N}, x.t->scalar_type(), dev);
-  const int64_t bytes = int64_t(lib.linear_bytes(x.M, N, x.K));
-  at::Tensor ws;
-  if (bytes) ws = empty({bytes}, at::kByte, dev);
+  at::Tensor y, ws;
+  if (!result(n == 8 ? a[6] : Py_None, x.M, N, x.t->scalar_type(), dev, &y)) Py_RETURN_NONE;
+  void* p = nullptr;
+  int64_t bytes = int64_t(lib.linear_bytes(x.M, N, x.K));
+  if (n == 8 && a[7] != Py_None) {
+    const at::Tensor* t = tensor(a[7], dev);
+    if (!t || t->scalar_type() != at::kByte || !t->is_contiguous()) Py_RETURN_NONE;
+    const uintptr_t from = reinterpret_cast<uintptr_t>(t->data_ptr()), at = (from + 255) & ~uintptr_t(255);
+    p = reinterpret_cast<void*>(at);
+    bytes = std::max<int64_t>(t->numel() - int64_t(at - from), 0);
+  } else if (bytes) {
+    ws = empty({bytes}, at::kByte, dev);
+    p = ws.data_ptr();
+  }
   const auto run = [&] {
-    return lib.linear(x.t->const_data_ptr(), x.type, x.ld, w.codes, w.scales, bias.p, bias.type, y.data_ptr(), x.type,
-                      bytes ? ws.data_ptr() : nullptr, uint64_t(bytes), x.M, N, x.K, stream(dev));
+    return lib.linear(x.t->const_data_ptr(), x.type, x.ld, w.codes, w.scales, bias.p, bias.type, y.data_ptr(), x.type, p, uint64_t(bytes),
+                      x.M, N, x.K, stream(dev));
   };
   if (const int status = launched(run)) return failed(status, "tac_linear_mxfp4");
   return THPVariable_Wrap(y);

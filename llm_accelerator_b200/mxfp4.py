@@ -75,6 +75,11 @@ class Mxfp4:
     def _pointers(self):
         return self.codes.data_ptr(), self.scales.data_ptr()
 
+    def _now(self):
+        """(rows, columns, device, addresses), checked."""
+        _check_tensors(self.codes, self.scales, self.cols)
+        return self.rows, self.cols, self._index, self._pointers
+
     @classmethod
     def from_tensors(cls, codes, scale_bytes, cols: int) -> "Mxfp4":
         """Of codes [rows, 16 blocks] and scale bytes [rows, blocks]; the scales are laid out once, here.  Columns from
@@ -100,14 +105,13 @@ class Mxfp4:
         y = front.values((self.codes, self.scales), None, self.cols, None, dtype)
         if y is not None:
             return y
-        _check_tensors(self.codes, self.scales, self.cols)
-        M, K, dev = self.rows, self.cols, self._index
+        M, K, dev, pointers = self._now()
         yt = TYPES.get(dtype)
         if yt is None:
             type_code(dtype, "dtype")
         y = empty((M, K), dtype, dev)
         if M:
-            call("tac_mxfp4_values", _values, dev, *self._pointers, y.data_ptr(), yt, M, K)
+            call("tac_mxfp4_values", _values, dev, *pointers, y.data_ptr(), yt, M, K)
         return y
 
 
@@ -149,11 +153,10 @@ def quantize(X) -> Mxfp4:
 
 
 def _result(w, M, K, dev, bias, out, dtype):
-    """Checks of what both products share; (out, its type, N, bias pointer, bias type)."""
-    _check_tensors(w.codes, w.scales, w.cols)
-    if w.cols != K or w._index != dev:
-        raise ValueError(f"the operands must have one number of columns and one device, got {K} and {w.cols} columns")
-    N = w.rows
+    """Checks of what both products share; (out, its type, N, w's addresses, bias pointer, bias type)."""
+    N, cols, index, pointers = w._now()
+    if cols != K or index != dev:
+        raise ValueError(f"the operands must have one number of columns and one device, got {K} and {cols} columns")
     bp, bt = None, 0
     if bias is not None:
         bt = type_code(bias.dtype, "bias")
@@ -165,7 +168,7 @@ def _result(w, M, K, dev, bias, out, dtype):
         out = empty((M, N), dtype, dev)
     elif out.dtype is not dtype or out.shape != (M, N) or not out.is_contiguous() or out.get_device() != dev:
         raise ValueError(f"out must be a contiguous {dtype} [{M}, {N}] tensor on the operands' device")
-    return out, yt, N, bp, bt
+    return out, yt, N, pointers, bp, bt
 
 
 def gemm(a: Mxfp4, b: Mxfp4, bias=None, out_dtype=None, out=None):
@@ -173,15 +176,14 @@ def gemm(a: Mxfp4, b: Mxfp4, bias=None, out_dtype=None, out=None):
     float16)."""
     if out_dtype is None:
         out_dtype = _F16 if out is None else out.dtype
-    if out is None and type(b) is Mxfp4:
-        y = front.gemm((a.codes, a.scales), None, a.cols, None, (b.codes, b.scales), None, b.cols, None, bias, out_dtype)
+    if type(b) is Mxfp4:
+        y = front.gemm((a.codes, a.scales), None, a.cols, None, (b.codes, b.scales), None, b.cols, None, bias, out_dtype, out)
         if y is not None:
             return y
-    _check_tensors(a.codes, a.scales, a.cols)
-    M, K, dev = a.rows, a.cols, a._index
-    out, yt, N, bp, bt = _result(b, M, K, dev, bias, out, out_dtype)
+    M, K, dev, rows = a._now()
+    out, yt, N, channels, bp, bt = _result(b, M, K, dev, bias, out, out_dtype)
     if M and N:
-        call("tac_mxfp4_gemm", _gemm, dev, *a._pointers, *b._pointers, bp, bt, out.data_ptr(), yt, M, N, K)
+        call("tac_mxfp4_gemm", _gemm, dev, *rows, *channels, bp, bt, out.data_ptr(), yt, M, N, K)
     return out
 
 
@@ -191,12 +193,12 @@ def linear(X, w: Mxfp4, bias=None, out=None, ws=None):
     X float32, float16 or bfloat16 with contiguous rows at any row stride.  ws: a ``linear_workspace`` to reuse across
     calls on one stream; by default a call allocates its own where it needs one.  A block of X with an infinity or a NaN
     gives a row of NaN."""
-    if out is None and ws is None and type(w) is Mxfp4:
-        y = front.linear(X, (w.codes, w.scales), None, w.cols, None, bias)
+    if type(w) is Mxfp4:
+        y = front.linear(X, (w.codes, w.scales), None, w.cols, None, bias, out, ws)
         if y is not None:
             return y
     xt, ldx, M, K, dev = _rows(X)
-    out, yt, N, bp, bt = _result(w, M, K, dev, bias, out, X.dtype)
+    out, yt, N, channels, bp, bt = _result(w, M, K, dev, bias, out, X.dtype)
     if M and N:
         wp, wn = None, 0
         if ws is not None:
@@ -209,7 +211,7 @@ def linear(X, w: Mxfp4, bias=None, out=None, ws=None):
             p = ws.data_ptr()
             wp = (p + 255) & ~255
             wn = max(ws.numel() - (wp - p), 0)
-        call("tac_linear_mxfp4", _linear, dev, X.data_ptr(), xt, ldx, *w._pointers, bp, bt, out.data_ptr(), yt, wp, wn, M, N, K)
+        call("tac_linear_mxfp4", _linear, dev, X.data_ptr(), xt, ldx, *channels, bp, bt, out.data_ptr(), yt, wp, wn, M, N, K)
     return out
 
 

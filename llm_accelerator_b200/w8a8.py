@@ -102,18 +102,18 @@ def linear_w8a8(X, Bt, b_scale, bias=None, out=None, ws=None):
         raise ValueError(f"rows of X overlap (stride {ldx}, {K} columns)")
     N, out, bp, bt = _check(X, Bt, b_scale, bias, out, X.dtype, M, (K + 15) // 16 * 16)
     if M and N:
-        wp, wn = None, 0
+        wp, wn, dev = None, 0, X.get_device()
         if ws is not None:
-            if ws.get_device() != X.get_device() or ws.dtype is not torch.uint8 or not ws.is_contiguous():
+            if ws.get_device() != dev or ws.dtype is not torch.uint8 or not ws.is_contiguous():
                 raise ValueError("ws must be a linear_workspace on X's device")
         else:
-            need = _ws_bytes(X.get_device(), M, N, K)
+            need = _ws_bytes(dev, M, N, K)
             ws = torch.empty(need + 256, dtype=torch.uint8, device=X.device) if need else None
         if ws is not None:
             p = ws.data_ptr()
             wp = (p + 255) & ~255
             wn = max(ws.numel() - (wp - p), 0)
-        call("tac_linear_w8a8", _linear, X.get_device(), X.data_ptr(), xt, ldx, Bt.data_ptr(), b_scale.data_ptr(),
+        call("tac_linear_w8a8", _linear, dev, X.data_ptr(), xt, ldx, Bt.data_ptr(), b_scale.data_ptr(),
              TYPES[b_scale.dtype], bp, bt, out.data_ptr(), xt, wp, wn, M, N, K)
     return out
 

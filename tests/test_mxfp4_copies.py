@@ -10,6 +10,7 @@ import pytest
 import torch
 
 from llm_accelerator_b200 import mxfp4
+from llm_accelerator_b200.errors import EngineError
 
 
 def _on_host(rows, cols):
@@ -102,3 +103,32 @@ def test_products_after_an_assignment():
         for call in (one.values, lambda: mxfp4.linear(x, one), lambda: mxfp4.gemm(one, two), lambda: mxfp4.gemm(two, one)):
             with pytest.raises((TypeError, ValueError)):
                 call()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M", [1, 200])
+def test_out_and_workspace(M):
+    """The same tensor comes back, with what a call without it gives; those that do not fit are refused."""
+    g = torch.Generator().manual_seed(M)
+    x, w = torch.randn((M, 96), generator=g).cuda(), mxfp4.quantize(torch.randn((50, 96), generator=g).cuda())
+    a, want = mxfp4.quantize(x), mxfp4.linear(x, w)
+    y, ws = torch.full((M, 50), 7.0, device="cuda"), mxfp4.linear_workspace(M, 96)
+    assert mxfp4.linear(x, w, out=y) is y and torch.equal(y, want)
+    for space in (ws, ws[1:], None):
+        y.fill_(7.0)
+        assert mxfp4.linear(x, w, out=y, ws=space) is y and torch.equal(y, want)
+        assert torch.equal(mxfp4.linear(x, w, ws=space), want)
+    half = torch.empty((M, 50), dtype=torch.float16, device="cuda")
+    assert mxfp4.gemm(a, w, out=half) is half and torch.equal(half, mxfp4.gemm(a, w))
+    assert mxfp4.gemm(a, w, out=y, out_dtype=torch.float32) is y and torch.equal(y, want)
+    for bad in (half, y[:, :40], torch.empty((M + 1, 50), device="cuda"), y.cpu(), torch.empty((50, M + 1), device="cuda").t()):
+        with pytest.raises(ValueError):
+            mxfp4.linear(x, w, out=bad)
+    with pytest.raises(ValueError):
+        mxfp4.gemm(a, w, out=half, out_dtype=torch.float32)
+    for bad in (ws.cpu(), ws.int(), ws[::2]):
+        with pytest.raises(ValueError):
+            mxfp4.linear(x, w, ws=bad)
+    if M > 64:
+        with pytest.raises(EngineError):
+            mxfp4.linear(x, w, ws=ws[:300])
