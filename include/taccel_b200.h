@@ -489,8 +489,9 @@ int tac_mxfp4_gemm(const uint8_t* a_codes, const uint8_t* a_scales, const uint8_
 
 /* The same product of floating-point rows X[M,K], quantised in the call as
  * tac_mxfp4_quantize does.  Calls that share a workspace (256-byte aligned, at
- * least the bytes of the query; null where that gives 0) must not overlap.  The
- * query goes by the SMs of the current device too: ask with the call's own. */
+ * least the bytes of the query; null where that gives 0) must not overlap, nor
+ * may X and Y.  The query goes by the SMs of the current device too: ask with
+ * the call's own. */
 uint64_t tac_linear_mxfp4_workspace_bytes(int M, int N, int K);
 int tac_linear_mxfp4(const void* X, int x_type, int64_t ldx, const uint8_t* b_codes, const uint8_t* b_scales,
                      const void* bias, int bias_type, void* Y, int y_type, void* workspace, uint64_t workspace_bytes,

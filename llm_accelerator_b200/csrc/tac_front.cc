@@ -299,6 +299,8 @@ PyObject* linear(PyObject*, PyObject* const* a, Py_ssize_t n) {               //
   const int N = int(w.rows);
   at::Tensor y, ws;
   if (!result(n == 8 ? a[6] : Py_None, x.M, N, x.t->scalar_type(), dev, &y)) Py_RETURN_NONE;
+  const char *xp = static_cast<const char*>(x.t->const_data_ptr()), *yp = static_cast<const char*>(y.const_data_ptr());
+  if (xp < yp + y.nbytes() && yp < xp + ((x.M - 1) * x.ld + x.K) * int64_t(x.t->element_size())) Py_RETURN_NONE;
   void* p = nullptr;
   int64_t bytes = int64_t(lib.linear_bytes(x.M, N, x.K));
   if (n == 8 && a[7] != Py_None) {

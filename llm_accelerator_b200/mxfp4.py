@@ -190,7 +190,7 @@ def gemm(a: Mxfp4, b: Mxfp4, bias=None, out_dtype=None, out=None):
 def linear(X, w: Mxfp4, bias=None, out=None, ws=None):
     """Y [M, N] in X's type = X [M, K] @ w^T (+ bias[n]), X quantised as ``quantize`` does.
 
-    X float32, float16 or bfloat16 with contiguous rows at any row stride.  ws: a ``linear_workspace`` to reuse across
+    X float32, float16 or bfloat16 with contiguous rows at any row stride; out may be X's memory.  ws: a ``linear_workspace`` to reuse across
     calls on one stream; by default a call allocates its own where it needs one.  A block of X with an infinity or a NaN
     gives a row of NaN."""
     if type(w) is Mxfp4:
@@ -198,8 +198,13 @@ def linear(X, w: Mxfp4, bias=None, out=None, ws=None):
         if y is not None:
             return y
     xt, ldx, M, K, dev = _rows(X)
+    given = out
     out, yt, N, channels, bp, bt = _result(w, M, K, dev, bias, out, X.dtype)
     if M and N:
+        if given is not None:
+            x, y, e = X.data_ptr(), out.data_ptr(), X.element_size()
+            if x < y + M * N * e and y < x + ((M - 1) * ldx + K) * e:   # one launch would read rows beside their results
+                return gemm(quantize(X), w, bias, out.dtype, out)
         wp, wn = None, 0
         if ws is not None:
             if ws.get_device() != dev or ws.dtype is not _U8 or not ws.is_contiguous():

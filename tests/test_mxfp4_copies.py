@@ -132,3 +132,16 @@ def test_out_and_workspace(M):
     if M > 64:
         with pytest.raises(EngineError):
             mxfp4.linear(x, w, ws=ws[:300])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,K", [(1, 1024), (40, 512), (64, 4096), (300, 768)])
+def test_results_over_the_rows(M, K):
+    g = torch.Generator().manual_seed(K)
+    w = mxfp4.quantize(torch.randn((K, K), generator=g).cuda())
+    for dtype in (torch.bfloat16, torch.float32):
+        for at in (0, 8):
+            space = torch.randn(M * K + 64, generator=g).to(dtype).cuda()
+            x, y = space[:M * K].view(M, K), space[at:at + M * K].view(M, K)
+            want = mxfp4.gemm(mxfp4.quantize(x), w, out_dtype=dtype)
+            assert mxfp4.linear(x, w, out=y) is y and torch.equal(y, want)
