@@ -760,7 +760,8 @@ int launch_logprobs(const LpParams& p, cudaStream_t st) {
   int log_ctas = 0;
   while (2 << log_ctas <= kMostCtas && pays(log_ctas + 1)) ++log_ctas;
   // Four rows for some SMs and three for others: halves even that out where 16-bit logits are bound by their exponentials (500
-  // x 121000 in 29 against 37 us with none picked, 39 against 46 with 32; float32 gains nothing).
+  // x 121000 in 29 against 38 us with none picked, 35 against 43 with 20; 590 rows in 32 against 38).  Elsewhere rows in one
+  // CTA each are faster: 400 x 121000 in 24.2 against 25.6 us, 660 in 38.2 against 39.0, float32 500 x 121000 in 45 against 46.
   if (sizeof(T) == 2 && !log_ctas && p.M > 3 * sms && p.M <= 4 * sms && pieces >= 2 * 24 * 256) log_ctas = 1;
   if (log_ctas) return launch_rows<T, 256, true>(p, log_ctas, st);
   // A warp a row, which needs no barrier, for short rows: those of two groups of loads, and where there are rows for many

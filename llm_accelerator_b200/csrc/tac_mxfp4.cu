@@ -290,7 +290,8 @@ bool map_scales(CUtensorMap* m, const uint8_t* base, int k_stages, int rows, int
 }
 
 // Tokens of a pair tile: the number that leaves the least work on the fullest
-// pair.  A stage costs, in nanoseconds: mostly its operands' loads.
+// pair.  A stage costs, in nanoseconds: mostly its operands' loads.  The costs are
+// those of long K; the epilogue is not in them.
 int pair_tokens(int M, int N, int clusters) {
   constexpr int kStageCost[4] = {273, 315, 436, 499};      // 64, 128, 192, 256 tokens (4096^3)
   const int64_t wt = (N + 255) / 256;

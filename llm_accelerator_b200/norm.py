@@ -71,8 +71,10 @@ def rms_norm(x, weight, eps: float = 1e-6, residual=None, residual_out=None, out
 
     x, residual and residual_out [M, K] float32, float16 or bfloat16 with contiguous rows at any row stride; weight [K]
     of any of these types.  residual_out: where h goes, by default a new tensor; it may be `residual` or x itself, but
-    may not overlap them otherwise.  out: y's tensor, which may be x or the residual (of one row stride, K).  A row whose h^2 add up to more than float32 holds (values of 10^18) is zero; an
-    infinity or a NaN makes NaN of its own place, a NaN of its whole row."""
+    may not overlap them otherwise.  out: y's tensor, which may be x or the residual (of one row stride, K).  A row whose h^2
+    add up to more than float32 holds (values of 10^18) is zero; with an eps of 0 one whose h^2 are too small for it (values
+    below 10^-19) loses places, and below 10^-23 is infinite.  An infinity makes NaN of its own place, a NaN of its whole
+    row."""
     if residual_out is None and out is None:
         result = front.rms_norm(x, weight, eps, residual)
         if result is not None:
