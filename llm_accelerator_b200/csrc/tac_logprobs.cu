@@ -199,14 +199,16 @@ struct Vec<__nv_bfloat16> {
 // (2.5e-6) with 8 and 9.8e-7 (6.7e-6) with 16; 77 us with each of them, and 888
 // rows take 22.6 with none, 22.3 with 4, 22.1 with 16.  A value of
 // -inf makes e^d d, and with it t, a NaN; and c is rounded by half its last
-// place, which all terms' exponents share and e^-over makes good while that is
-// small (below 2^24 one half at most; from 2^31 on it can pass all exponents
-// that float32 has).  Otherwise, and in the rest of the row, each difference is
-// taken, and lifted, by itself (2000 x 50257, one token in 64 unmasked in every
-// third row: 43 us, 56 while each group of a row was tried first).
+// place, which all terms' exponents share and e^-over makes good while it is 64
+// at most, below kLargest (further on it can pass all exponents that float32
+// has).  Otherwise, and in the rest of the row, each difference is taken, and
+// lifted, by itself (2000 x 50257, one token in 64 unmasked in every third row:
+// 43 us, 56 while each group of a row was tried first; 4096 x 50257 with -10^9
+// for all but one token in 64 77 us, with -10^10, which some lanes of a warp
+// meet first and others do not, 122).
 // Eight values cost about 36 instructions and eight exponentials (16 a clock and
 // SM): 46 us for 4096 x 50257, whose bytes take 63.
-constexpr float kSlack = 4.f, kLargest = 16777216.f;
+constexpr float kSlack = 4.f, kLargest = 2147483648.f;
 template <typename T>
 __device__ __forceinline__ void take_each(Sums& a, const uint4& u) {
   constexpr int N = Vec<T>::kN;
